@@ -31,6 +31,7 @@
 #include "bsearch.h"
 #include "bs_internal.h"
 #include "bs_io.hpp"
+#include "bs_memory.h"
 
 using bsb::DevCounters;
 using bsb::LaunchShape;
@@ -673,6 +674,19 @@ bs_status ensure_entry(bs_index* ix) {
 }
 
 }  // namespace
+
+namespace bsb {
+
+bs_status report_error(bs_status status, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    std::vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    return fail(status, "%s", buf);
+}
+
+}  // namespace bsb
 
 extern "C" {
 

@@ -250,6 +250,165 @@ BS_API bs_status bs_merge_shards(const float* dists, const uint32_t* ids, uint32
                                  uint32_t K, const uint32_t* id_offsets, uint32_t K_out, uint32_t* out_ids,
                                  float* out_dists, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Token memory: the attention of a language model whose context is searched.
+ * No counterpart in the reference.  Keys and values of the tokens a model has
+ * read live in an 8-bit cache; tokens that the cache gives up are rows for an
+ * index (bs_index_create), found again by bs_search.
+ *
+ * All pointers are device pointers on the current device; every call is
+ * asynchronous on `stream` and allocates nothing: scratch is the caller's, of
+ * the size the matching *_workspace call gives (0 bytes: NULL is fine).
+ * Lengths, tables and positions are read on the device, so none of the calls
+ * waits for them and all can be captured in a CUDA graph.  What only the
+ * device can see to be wrong (a block id outside the cache, lengths outside
+ * their buffers) is not read or written; it sets an error bit that
+ * bs_memory_take_errors returns.
+ *
+ * dim is a multiple of 16 up to 128.  q, k and v have strides in elements
+ * between tokens and between heads; they and the base address are multiples
+ * of 16 bytes, the last dimension is contiguous.  Outputs are contiguous. */
+typedef enum bs_dtype { BS_F32 = 0, BS_F16 = 1, BS_BF16 = 2 } bs_dtype;
+
+/* The 8-bit cache: blocks of `block` tokens (16, 32, 64 or 128).  A value is
+ * code * scale, one scale per block and head. */
+typedef struct bs_token_cache {
+    int8_t* k;                /* [num_blocks][kv_heads][block][dim], 16-byte aligned */
+    int8_t* v;
+    float* k_scale;           /* [num_blocks][kv_heads]                       */
+    float* v_scale;
+    uint32_t num_blocks;
+    int32_t kv_heads;
+    int32_t block;
+    int32_t dim;
+} bs_token_cache;
+
+/* Attention of packed prompts.  Sequence b's queries are rows cu_q[b] ..
+ * cu_q[b+1] of q and its keys rows cu_k[b] .. cu_k[b+1] of k and v; both lists
+ * start at 0, ascend and end at total_q and total_k.  With `causal`, query i
+ * of Lq sees the keys j <= i + Lk - Lq (the last query sees all), else all.
+ * Query head h goes with key head h / (q_heads / kv_heads).
+ *   s_j = scale * <q, k_j>,  lse = log sum_j exp(s_j),  out = sum_j exp(s_j - lse) v_j
+ * A query that sees no key gives out = 0, lse = -infinity. */
+typedef struct bs_prompt_attention_desc {
+    const void* q;            /* [total_q][q_heads][dim]                      */
+    const void* k;            /* [total_k][kv_heads][dim]                     */
+    const void* v;
+    void* out;                /* [total_q][q_heads][dim], type dtype          */
+    float* lse;               /* [total_q][q_heads], or NULL                  */
+    int64_t q_stride[2];      /* elements from token to token, head to head   */
+    int64_t k_stride[2];
+    int64_t v_stride[2];
+    const int32_t* cu_q;      /* [num_seqs + 1]                               */
+    const int32_t* cu_k;
+    uint32_t total_q, total_k, num_seqs;
+    int32_t q_heads, kv_heads, dim;
+    int32_t dtype;            /* BS_F16 or BS_BF16                            */
+    int32_t causal;
+    float scale;
+} bs_prompt_attention_desc;
+
+BS_API bs_status bs_prompt_attention(const bs_prompt_attention_desc* desc, void* stream);
+
+/* Appends tokens: rows cu[b] .. cu[b+1] of k and v become positions start[b],
+ * start[b] + 1, ... of sequence b, whose position p lies in block
+ * table[b][p / block].  A block's scale is max|x| * (1 / 127) over its new tokens
+ * (0 when that maximum is below 1e-30), and where it holds earlier tokens
+ * (positions below start[b]) at least the scale it has; those tokens' codes
+ * are rounded anew when the scale grows.  code = rint(x * (1 / scale)),
+ * clamped to +-127.  Values must be finite.  A block is written by one
+ * sequence of a call only. */
+typedef struct bs_cache_write_desc {
+    const void* k;            /* [total][kv_heads][dim]                       */
+    const void* v;
+    int64_t k_stride[2];
+    int64_t v_stride[2];
+    const int32_t* cu;        /* [num_seqs + 1]                               */
+    const int32_t* table;     /* [num_seqs][table_width]                      */
+    const int32_t* start;     /* [num_seqs]                                   */
+    uint32_t total, num_seqs, table_width;
+    int32_t dtype;
+} bs_cache_write_desc;
+
+BS_API bs_status bs_cache_write(const bs_token_cache* cache, const bs_cache_write_desc* desc, void* stream);
+
+/* Reads values back (as rows for an index, for instance): out[b][h][i] is the
+ * value at position positions[b][h][i] of sequence b (position_head_stride 0:
+ * the same positions for every head).  Zeros where the position is negative
+ * or not below lens[b]. */
+typedef struct bs_cache_read_desc {
+    const int32_t* table;     /* [num_seqs][table_width]                      */
+    const int32_t* lens;      /* [num_seqs]                                   */
+    const int32_t* positions; /* [num_seqs][heads or 1][count]                */
+    int64_t position_seq_stride, position_head_stride;
+    void* k;                  /* [num_seqs][kv_heads][count][dim], or NULL    */
+    void* v;                  /* or NULL                                      */
+    uint32_t num_seqs, table_width, count;
+    int32_t dtype;            /* BS_F32, BS_F16 or BS_BF16                    */
+} bs_cache_read_desc;
+
+BS_API bs_status bs_cache_read(const bs_token_cache* cache, const bs_cache_read_desc* desc, void* stream);
+
+/* Attention over the cache.  Sequence b holds lens[b] tokens, the last
+ * `queries` of which are the query tokens: query i sees the positions below
+ * lens[b] - queries + 1 + i (one query: all).  out, lse as in
+ * bs_prompt_attention.  With out_mass, the weight that each cached token got,
+ *   out_mass[b][h][j] = mass[b][h][j] + sum over the queries and the heads of
+ *                       key head h of exp(s_j - lse)        (j < lens[b])
+ * and 0 for lens[b] <= j < mass_width; mass may be NULL (zeros) or out_mass. */
+typedef struct bs_cache_attention_desc {
+    const void* q;            /* [num_seqs][queries][q_heads][dim]            */
+    int64_t q_stride[3];      /* elements from sequence to sequence, token to token, head to head */
+    const int32_t* table;     /* [num_seqs][table_width]                      */
+    const int32_t* lens;      /* [num_seqs], at most table_width * block      */
+    void* out;                /* [num_seqs][queries][q_heads][dim], type dtype */
+    float* lse;               /* [num_seqs][queries][q_heads], or NULL        */
+    const float* mass;        /* [num_seqs][kv_heads][mass_width], or NULL    */
+    float* out_mass;          /* the same shape, or NULL                      */
+    void* workspace;
+    size_t workspace_bytes;
+    uint32_t num_seqs, table_width, mass_width;
+    int32_t queries, q_heads;
+    int32_t dtype;            /* BS_F16 or BS_BF16                            */
+    float scale;
+} bs_cache_attention_desc;
+
+BS_API bs_status bs_cache_attention(const bs_token_cache* cache, const bs_cache_attention_desc* desc, void* stream);
+BS_API bs_status bs_cache_attention_workspace(const bs_token_cache* cache, const bs_cache_attention_desc* desc,
+                                              size_t* bytes);
+
+/* Eviction by accumulated attention weight.  Of a sequence of n = lens[b] >
+ * budget tokens stay, for each head apart: the first `sinks`, the last
+ * `recent`, and of the others the budget - sinks - recent with the largest
+ * mass (ties: the lower position; NaN counts as largest); of a shorter one
+ * all.  The tokens that stay move, in order, into the blocks of new_table,
+ * which must not be blocks of any sequence of `table`.  kept[b][h][i] is the
+ * old position of new position i (-1 past the end), new_mass its mass (0 past
+ * the end), new_lens[b] = min(lens[b], budget).  A new block's scale is the
+ * largest of its tokens' old scales; codes become rint(code * (old / new)). */
+typedef struct bs_cache_evict_desc {
+    const float* mass;        /* [num_seqs][kv_heads][mass_width]             */
+    const int32_t* table;     /* [num_seqs][table_width]                      */
+    const int32_t* lens;      /* [num_seqs], at most mass_width               */
+    const int32_t* new_table; /* [num_seqs][new_table_width]                  */
+    int32_t* kept;            /* [num_seqs][kv_heads][budget]                 */
+    int32_t* new_lens;        /* [num_seqs]                                   */
+    float* new_mass;          /* [num_seqs][kv_heads][budget]                 */
+    void* workspace;
+    size_t workspace_bytes;
+    uint32_t num_seqs, table_width, new_table_width, mass_width;
+    int32_t budget, sinks, recent;
+} bs_cache_evict_desc;
+
+BS_API bs_status bs_cache_evict(const bs_token_cache* cache, const bs_cache_evict_desc* desc, void* stream);
+BS_API bs_status bs_cache_evict_workspace(const bs_token_cache* cache, const bs_cache_evict_desc* desc, size_t* bytes);
+
+/* Error bits that token-memory kernels have set on the current device since
+ * the last call, ordered after the work queued on `stream`, then cleared;
+ * synchronises `stream`.  Bits: 1 a wait inside a kernel gave up, 2 a block id
+ * outside the cache, 4 lengths outside their buffers. */
+BS_API bs_status bs_memory_take_errors(void* stream, uint32_t* flags);
+
 /* Device buffers on the index's device (for callers that stage queries once
  * and search many times, like the reference CLI's timed loop,
  * src/gpu_cli.cu:400-421). */

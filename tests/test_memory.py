@@ -1,0 +1,123 @@
+"""CPU: the token-memory entries' checks that need no GPU, and the 64-bit
+definitions that the GPU tests go by against an independent formulation."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import beam_search_collab_b200 as B
+import memory_ref as R
+from beam_search_collab_b200 import memory as M
+
+
+def cache(**kw):
+    c = M._Cache(64, 64, 64, 64, 4, 2, 32, 64)
+    for k, v in kw.items():
+        setattr(c, k, v)
+    return c
+
+
+def status(name, *args):
+    rc = getattr(M._lib(), name)(*args)
+    return rc, B.lib().bs_last_error().decode()
+
+
+def test_null_descriptors():
+    c = cache()
+    for name in ("bs_cache_write", "bs_cache_read", "bs_cache_attention", "bs_cache_evict"):
+        assert status(name, c, None, None) == (1, "desc is NULL")
+    assert status("bs_prompt_attention", None, None) == (1, "desc is NULL")
+    assert status("bs_cache_read", None, M._Read(), None) == (1, "cache is NULL")
+    assert status("bs_memory_take_errors", None, None)[0] == 1
+    assert status("bs_cache_evict_workspace", c, M._Evict(), None)[0] == 1
+
+
+@pytest.mark.parametrize("field,value,code,text", [
+    ("dtype", 0, 1, "BS_F16 or BS_BF16"), ("dim", 0, 1, "positive"), ("dim", 24, 2, "multiple of 16"), ("dim", 144, 2, "up to 128"),
+    ("q_heads", 3, 1, "multiple of kv_heads"), ("kv_heads", 0, 1, "multiple of kv_heads"), ("q_heads", 258, 2, "128 query heads"),
+    ("scale", math.nan, 1, "NaN"), ("total_k", 1 << 30, 2, "2^30"), ("num_seqs", 65536, 2, "65535"), ("cu_q", None, 1, "NULL"),
+    ("out", None, 1, "NULL"), ("k", 72, 1, "16-byte aligned"), ("q_stride", (4, 64), 1, "multiples of 8"),
+    ("v_stride", (-8, 64), 1, "non-negative")])
+def test_prompt_checks(field, value, code, text):
+    d = M._Prompt(64, 64, 64, 64, 64, (128, 64), (128, 64), (128, 64), 64, 64, 10, 10, 1, 2, 2, 64, 1, 1, 0.1)
+    setattr(d, field, (ctypes.c_int64 * 2)(*value) if isinstance(value, tuple) else value)
+    rc, why = status("bs_prompt_attention", d, None)
+    assert rc == code and text in why, (rc, why)
+
+
+@pytest.mark.parametrize("field,value,code,text", [("block", 24, 1, "16, 32, 64 or 128"), ("dim", 40, 2, "multiple of 16"),
+                                                   ("kv_heads", 0, 1, "kv_heads"), ("kv_heads", 70000, 1, "kv_heads")])
+def test_cache_checks(field, value, code, text):
+    d = M._Read(64, 64, 64, 0, 0, 64, 64, 1, 1, 1, 0)
+    rc, why = status("bs_cache_read", cache(**{field: value}), d, None)
+    assert rc == code and text in why, (rc, why)
+
+
+@pytest.mark.parametrize("field,value,code,text", [
+    ("queries", 0, 1, "queries"), ("queries", 1025, 1, "queries"), ("q_heads", 5, 1, "multiple"), ("dtype", 0, 1, "BS_F16"),
+    ("table_width", 1 << 26, 2, "2^30"), ("lens", None, 1, "NULL"), ("out_mass", None, 1, "mass without out_mass"),
+    ("mass_width", 0, 1, "mass_width is 0"), ("scale", math.nan, 1, "NaN"), ("q", 65, 1, "aligned")])
+def test_attention_checks(field, value, code, text):
+    d = M._Attention(64, (256, 256, 64), 64, 64, 64, 64, 64, 64, None, 0, 1, 2, 64, 1, 4, 1, 0.1)
+    setattr(d, field, value)
+    rc, why = status("bs_cache_attention", cache(), d, None)
+    assert rc == code and text in why, (rc, why)
+
+
+@pytest.mark.parametrize("field,value,code,text", [
+    ("budget", 0, 1, "budget"), ("sinks", -1, 1, "sinks"), ("recent", 30, 1, "sinks + recent"), ("new_table_width", 0, 1, "room"),
+    ("mass_width", 1 << 30, 2, "mass_width"), ("kept", None, 1, "NULL")])
+def test_evict_checks(field, value, code, text):
+    d = M._Evict(64, 64, 64, 64, 64, 64, 64, None, 0, 1, 4, 1, 128, 32, 4, 8)
+    setattr(d, field, value)
+    rc, why = status("bs_cache_evict", cache(), d, None)
+    assert rc == code and text in why, (rc, why)
+
+
+def test_nothing_to_do_is_done_without_a_gpu():
+    d = M._Prompt(None, None, None, None, None, (0, 0), (0, 0), (0, 0), None, None, 0, 0, 0, 2, 2, 64, 1, 1, 0.1)
+    assert status("bs_prompt_attention", d, None)[0] == 0
+    assert status("bs_cache_write", cache(), M._Write(dtype=1), None)[0] == 0
+    assert status("bs_cache_read", cache(), M._Read(dtype=1), None)[0] == 0
+    assert status("bs_cache_attention", cache(), M._Attention(queries=1, q_heads=2, dtype=1), None)[0] == 0
+
+
+def test_host_tensors_are_refused():
+    q = torch.zeros((4, 2, 64), dtype=torch.float16)
+    with pytest.raises(ValueError, match="CUDA"):
+        M.prompt_attention(q, q, q, torch.tensor([0, 4], dtype=torch.int32))
+    with pytest.raises(ValueError, match="CUDA"):
+        M.TokenCache(torch.zeros((2, 2, 16, 64), dtype=torch.int8), None, None, None)
+
+
+def test_merge_is_the_attention_over_both_sets():
+    g = torch.Generator().manual_seed(0)
+    s, v = torch.randn((5, 9), generator=g, dtype=torch.float64), torch.randn((9, 4), generator=g, dtype=torch.float64)
+    part = lambda a, b: (torch.softmax(s[:, a:b], 1) @ v[a:b], torch.logsumexp(s[:, a:b], 1))  # noqa: E731
+    nothing = (torch.zeros((5, 4), dtype=torch.float64), torch.full((5,), -math.inf, dtype=torch.float64))
+    out, lse = M.merge(*zip(part(0, 3), part(3, 9), nothing))
+    assert torch.allclose(out, torch.softmax(s, 1) @ v, atol=1e-6) and torch.allclose(lse, torch.logsumexp(s, 1))
+    out, lse = M.merge(*zip(nothing, nothing))
+    assert (out == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_definition(causal):
+    g = torch.Generator().manual_seed(1)
+    lens_q, lens_k = [3, 0, 5], [4, 2, 2]
+    q = torch.randn((8, 4, 16), generator=g, dtype=torch.float64)
+    k, v = (torch.randn((8, 2, 16), generator=g, dtype=torch.float64) for _ in range(2))
+    out, lse, weighted, _ = R.prompt(q, k, v, lens_q, lens_k, causal, 0.25)
+    a = b = 0
+    for nq, nk in zip(lens_q, lens_k):
+        for i in range(nq):
+            for h in range(4):
+                n = max(0, nk - nq + 1 + i) if causal else nk
+                s = (k[b:b + n, h // 2] * q[a + i, h]).sum(1) * 0.25
+                w = torch.softmax(s, 0)
+                want = (w[:, None] * v[b:b + n, h // 2]).sum(0) if n else torch.zeros(16, dtype=torch.float64)
+                assert torch.allclose(out[a + i, h], want)
+                assert torch.allclose(lse[a + i, h], torch.logsumexp(s, 0)) if n else lse[a + i, h] == -math.inf
+        a, b = a + nq, b + nk
+    assert (weighted >= out.abs() - 1e-12).all()
