@@ -1,5 +1,28 @@
 // bs_cache_attention.cu -- attention over the 8-bit token cache
 // (include/bsearch.h, bs_cache_attention).
+//
+// A few query rows (the heads that share a key head, times the query tokens)
+// meet a long cache once, so the time is the cache's bytes.  Every (sequence,
+// key head) is a segment of tiles of 16 tokens -- a tile never spans two
+// blocks, so it has one scale -- and all segments' tiles, end to end, are cut
+// into equal shares, one per thread block, whatever the lengths are.  A share
+// can end inside a segment; the pieces are joined by a second kernel.
+//
+// The matrix instructions are m16n8k16 with the TOKENS as the 16 rows of the
+// scores and the DIMENSIONS as the 16 rows of the outputs; the query rows are
+// the 8 columns.  So a code is converted once for 8 * NT query rows and few
+// rows waste little:
+//   S^T[token][row] = K[token][dim] Q^T[dim][row]
+//   O^T[dim][row]  += V^T[dim][token] P^T[token][row]
+// A sum over dimensions or tokens may take them in any order, so each lane's
+// share of a fragment is what lies side by side in memory.
+//
+// Codes become f16 exactly (|code| <= 128); bf16 queries become f16 exactly
+// too, each row scaled by a power of two (elements 2^-31 below the row's
+// largest and less lose bits, far under a 32-bit sum's rounding).  Scores,
+// weights' sums and outputs are 32-bit.  A weight is rounded to f16 (relative
+// 2^-11, a quarter of the output's own rounding or less) where it meets the
+// values; the sum of weights takes it unrounded.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -12,125 +35,694 @@ using namespace dev;
 
 namespace {
 
+constexpr int kWarps = 4;              // per block; they take a segment's tiles in turn
+constexpr int kThreads = kWarps * 32;
+constexpr int kStages = 3;             // tiles a warp has in flight or in use
+// Resident blocks: 3 x 165 registers for 8 query rows, 2 x 232 for 16 (at 3 they spill).
+constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+constexpr int kTile = 16;              // tokens
+constexpr float kNoScore = -1e30f;     // running maximum before the first score
+constexpr float kSlack = 8.f;          // weights may grow to 2^kSlack before the maximum is moved
+
 struct CacheArgs {
     bs_token_cache c;
     bs_cache_attention_desc d;
     unsigned int* errors;
-    float* lse;        // [num_seqs][queries][q_heads]
+    float* lse;          // [num_seqs][queries][q_heads]
+    float* part_o;       // [row tiles][blocks][2][8 * NT][dim]: unfinished outputs
+    float* part_ml;      // [row tiles][blocks][2][8 * NT][2]: their maximum (log2) and sum
+    float* scores;       // [num_seqs][kv_heads][rows][score_width], log2 units, or null
+    uint32_t group;      // query heads per key head
+    uint32_t rows;       // group * queries
+    uint32_t score_width;
+    uint32_t shares;     // thread blocks per row tile
 };
-
-template <typename T>
-__device__ __forceinline__ const T* query_row(const CacheArgs& a, uint32_t b, uint32_t i, uint32_t h) {
-    return static_cast<const T*>(a.d.q) + b * a.d.q_stride[0] + i * a.d.q_stride[1] + h * a.d.q_stride[2];
-}
 
 __device__ __forceinline__ uint32_t held_tokens(const CacheArgs& a, uint32_t b) {
     const int32_t len = a.d.lens[b];
     const int64_t most = static_cast<int64_t>(a.d.table_width) * a.c.block;
     if (len >= 0 && len <= most) return len;
-    if (threadIdx.x == 0) atomicOr(a.errors, kMemErrLength);
+    atomicOr(a.errors, kMemErrLength);
     return len < 0 ? 0 : static_cast<uint32_t>(most);
 }
 
-// The block of a position, or one past the cache's last where there is none.
-__device__ __forceinline__ uint32_t block_of(const CacheArgs& a, uint32_t b, uint32_t pos) {
-    const uint32_t id = a.d.table[static_cast<uint64_t>(b) * a.d.table_width + pos / a.c.block];
-    if (id < a.c.num_blocks) return id;
-    atomicOr(a.errors, kMemErrBlock);
-    return a.c.num_blocks;
+__device__ __forceinline__ uint32_t tiles_of(uint32_t len) { return (len + kTile - 1) / kTile; }
+
+// Shares: W tiles over n blocks, block i has [first(i), first(i + 1)).  A
+// block gets at least one tile for each of its warps.
+__device__ __forceinline__ uint32_t used_shares(uint64_t w, uint32_t n) {
+    const uint64_t most = (w + kWarps - 1) / kWarps;
+    return most < n ? static_cast<uint32_t>(most) : n;
+}
+__device__ __forceinline__ uint64_t share_first(uint64_t w, uint32_t n, uint32_t i) {
+    return w / n * i + min(static_cast<uint64_t>(i), w % n);
+}
+// The block whose share holds tile x.
+__device__ __forceinline__ uint32_t share_of(uint64_t w, uint32_t n, uint64_t x) {
+    const uint64_t q = w / n, r = w % n, wide = r * (q + 1);
+    return static_cast<uint32_t>(x < wide ? x / (q + 1) : r + (x - wide) / q);
 }
 
-template <typename T>
-__device__ __forceinline__ float score(const CacheArgs& a, const T* q, uint32_t b, uint32_t g, uint32_t pos) {
-    const uint32_t id = block_of(a, b, pos);
-    if (id == a.c.num_blocks) return -INFINITY;
-    const uint64_t slab = static_cast<uint64_t>(id) * a.c.kv_heads + g;
-    const int8_t* k = a.c.k + (slab * a.c.block + pos % a.c.block) * a.c.dim;
-    float dot = 0.f;
-    for (int32_t x = 0; x < a.c.dim; ++x) dot += static_cast<float>(q[x]) * k[x];
-    return dot * (a.c.k_scale[slab] * a.d.scale);
-}
-
-// One warp per query and head.
-template <typename T>
-__global__ void __launch_bounds__(32) k_cache_rows(const CacheArgs a) {
-    const uint32_t lane = threadIdx.x, h = blockIdx.x, i = blockIdx.y, b = blockIdx.z;
-    const uint32_t g = h / (a.d.q_heads / a.c.kv_heads), dim = a.c.dim, block = a.c.block;
-    const int64_t n = static_cast<int64_t>(held_tokens(a, b)) - a.d.queries + 1 + i;
-    const T* q = query_row<T>(a, b, i, h);
-    float top = -INFINITY, sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t j0 = 0; j0 < n; j0 += 32) {
-        const float s = j0 + lane < n ? score<T>(a, q, b, g, static_cast<uint32_t>(j0 + lane)) : -INFINITY;
-        float m = s;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
-        const float next = fmaxf(top, m);
-        const float safe = next == -INFINITY ? 0.f : next;
-        const float shrink = expf(top - safe), p = expf(s - safe);
-        sum = sum * shrink + p;
-        top = next;
-        for (int x = 0; x < 4; ++x) acc[x] *= shrink;
-        for (int64_t j = j0; j < j0 + 32 && j < n; ++j) {
-            const float w = __shfl_sync(kFull, p, static_cast<int>(j - j0));
-            const uint32_t id = block_of(a, b, static_cast<uint32_t>(j));
-            if (id == a.c.num_blocks) continue;
-            const uint64_t slab = static_cast<uint64_t>(id) * a.c.kv_heads + g;
-            const int8_t* v = a.c.v + (slab * block + j % block) * dim;
-            const float ws = w * a.c.v_scale[slab];
-            for (int x = 0; x < 4; ++x)
-                if (lane + 32 * x < dim) acc[x] += ws * v[lane + 32 * x];
-        }
+// Tiles of one key head's segments before sequence b, and of all sequences;
+// every thread of the block (a multiple of 32 threads) gets both.
+__device__ __forceinline__ void count_tiles(const CacheArgs& a, uint32_t b, uint64_t& before, uint64_t& all, uint64_t* warp_sums) {
+    uint64_t mine = 0, total = 0;
+    for (uint32_t i = threadIdx.x; i < a.d.num_seqs; i += blockDim.x) {
+        const uint32_t t = tiles_of(held_tokens(a, i));
+        total += t;
+        mine += i < b ? t : 0;
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-    const uint64_t row = (static_cast<uint64_t>(b) * a.d.queries + i) * a.d.q_heads + h;
-    T* out = static_cast<T*>(a.d.out) + row * dim;
-    for (int x = 0; x < 4; ++x)
-        if (lane + 32 * x < dim) out[lane + 32 * x] = static_cast<T>(acc[x] * inv);
-    if (lane == 0) a.lse[row] = sum == 0.f ? -INFINITY : top + logf(sum);
+    for (int o = 16; o > 0; o >>= 1) {
+        mine += __shfl_xor_sync(kFull, mine, o);
+        total += __shfl_xor_sync(kFull, total, o);
+    }
+    const uint32_t warps = blockDim.x / 32, warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) {
+        warp_sums[warp] = mine;
+        warp_sums[warps + warp] = total;
+    }
+    __syncthreads();
+    before = all = 0;
+    for (uint32_t i = 0; i < warps; ++i) {
+        before += warp_sums[i];
+        all += warp_sums[warps + i];
+    }
+    __syncthreads();
 }
 
-// One thread per token and key head: its weight over all queries and heads.
-template <typename T>
-__global__ void __launch_bounds__(256) k_cache_mass(const CacheArgs a) {
-    const uint32_t j = blockIdx.x * 256 + threadIdx.x, g = blockIdx.y, b = blockIdx.z;
-    const uint32_t len = held_tokens(a, b);
+// Where a block is in its share: a piece is a run of tiles of one segment.
+struct Piece {
+    uint32_t b, h, len;
+    uint32_t t, end;        // tiles of the segment
+    uint64_t left;          // tiles of the share after this piece
+};
+
+__device__ __forceinline__ void next_piece(const CacheArgs& a, Piece& p) {
+    if (p.left == 0) {
+        p.t = p.end = 0;
+        p.b = a.d.num_seqs;
+        return;
+    }
+    if (++p.h == static_cast<uint32_t>(a.c.kv_heads)) {
+        p.h = 0;
+        do {
+            ++p.b;
+            p.len = held_tokens(a, p.b);
+        } while (p.len == 0);
+    }
+    const uint32_t tiles = tiles_of(p.len);
+    p.t = 0;
+    p.end = p.left < tiles ? static_cast<uint32_t>(p.left) : tiles;
+    p.left -= p.end;
+}
+
+__device__ __forceinline__ unsigned smem_addr(const void* p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(void* dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transposed8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Bytes [x, y] (in bits 0-7 and 8-15, or 16-23 and 24-31) biased by 128 ->
+// two f16 of the codes: 0x6400 | u is 1024 + u, minus 1152.
+__device__ __forceinline__ uint32_t codes_to_half2(uint32_t biased, uint32_t selector) {
+    const uint32_t u = __byte_perm(biased, 0x64646464u, selector);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&u), __float2half2_rn(1152.f));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+constexpr uint32_t kLow = 0x4140u, kHigh = 0x4342u;
+
+// NW words (of 4 codes) per lane of a key row: the lane's quarter of it.
+template <int NW>
+__device__ __forceinline__ void load_key_words(uint32_t (&w)[NW], const unsigned char* row, uint32_t c) {
+    const unsigned char* p = row + c * (NW * 4);
+    if constexpr (NW % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < NW / 4; ++i) *reinterpret_cast<uint4*>(&w[4 * i]) = reinterpret_cast<const uint4*>(p)[i];
+    } else if constexpr (NW % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < NW / 2; ++i) *reinterpret_cast<uint2*>(&w[2 * i]) = reinterpret_cast<const uint2*>(p)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < NW; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    }
+}
+
+// The lane's codes of one value row: output row tile t (16 dimensions) takes
+// the bytes 2t (tile row g) and 2t + 1 (row g + 8) of these words.  In memory
+// they are 16 g + 2t, 8 g + 2t, or, by pairs of tiles, 32 (t / 2) + 4 g + 2 (t % 2)
+// (a last single tile: 16 t + 2 g); value_dim gives the dimension.
+template <int NW>
+__device__ __forceinline__ void load_value_words(uint32_t (&w)[(NW + 1) / 2], const unsigned char* row, uint32_t g) {
+    if constexpr (NW == 8) {
+        *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(row + 16 * g);
+    } else if constexpr (NW == 4) {
+        *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(row + 8 * g);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NW / 2; ++i) w[i] = *reinterpret_cast<const uint32_t*>(row + 32 * i + 4 * g);
+        if constexpr (NW % 2) w[NW / 2] = *reinterpret_cast<const uint16_t*>(row + 16 * (NW - 1) + 2 * g);
+    }
+}
+template <int NW>
+__device__ __forceinline__ constexpr uint32_t value_dim(int t, uint32_t g) {
+    if (NW == 8) return 16 * g + 2 * t;
+    if (NW == 4) return 8 * g + 2 * t;
+    if (NW % 2 && t == NW - 1) return 16 * t + 2 * g;
+    return 32 * (t / 2) + 4 * g + 2 * (t % 2);
+}
+
+// Rows of a stage are an odd number of 16-byte units apart: the lanes of a
+// shared-memory access then fall on different banks.
+template <int NW>
+constexpr int kPitch = 16 * (NW | 1);
+template <int NW>
+constexpr int kStageBytes = 2 * kTile * kPitch<NW> + 16;      // keys, values, the two scales
+template <int NW, int NT>
+constexpr int kJoinBytes = 2 * 8 * NT * NW * 16 * 4;           // two warps' outputs
+template <int NW, int NT>
+constexpr size_t kSplitSmem = kWarps * kStages * kStageBytes<NW> + kJoinBytes<NW, NT> + kWarps * (8 * NT * 2 + 4) * 4 + 128;
+
+// One share of the tiles for one row tile of 8 * NT query rows.
+// Registers: outputs NW * NT * 4, queries NW * NT * 2, and about 60.
+template <int NW, int NT>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(const __grid_constant__ CacheArgs a) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    constexpr int kDim = NW * 16, kRows = 8 * NT;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    unsigned char* ring = smem + warp * kStages * kStageBytes<NW>;
+    float* join_o = reinterpret_cast<float*>(smem + kWarps * kStages * kStageBytes<NW>);
+    float* join_ml = join_o + 2 * kRows * kDim;                 // [warps][kRows][2]
+    uint64_t* sums = reinterpret_cast<uint64_t*>(smem);         // before the ring is used
+
+    // this block's share, and the piece it begins with
+    const uint32_t hkv = a.c.kv_heads, row0 = blockIdx.y * kRows;
+    uint64_t before, all;
+    count_tiles(a, 0, before, all, sums);
+    const uint64_t w_all = all * hkv;
+    const uint32_t n = used_shares(w_all, a.shares);
+    if (blockIdx.x >= n) return;
+    const uint64_t first = share_first(w_all, n, blockIdx.x);
+    Piece at;
+    {
+        uint64_t seen = 0;
+        uint32_t b = 0, tiles = 0;
+        for (uint32_t b0 = 0;; b0 += 32) {                       // 32 sequences at a time
+            const uint32_t len = b0 + lane < a.d.num_seqs ? held_tokens(a, b0 + lane) : 0;
+            uint64_t sum = static_cast<uint64_t>(tiles_of(len)) * hkv;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint64_t up = __shfl_up_sync(kFull, sum, o);
+                if (lane >= static_cast<uint32_t>(o)) sum += up;
+            }
+            const unsigned past = __ballot_sync(kFull, seen + sum > first);
+            if (past) {
+                const int l = __ffs(past) - 1;
+                b = b0 + l;
+                at.len = __shfl_sync(kFull, len, l);
+                tiles = tiles_of(at.len);
+                seen += __shfl_sync(kFull, sum, l) - static_cast<uint64_t>(tiles) * hkv;
+                break;
+            }
+            seen += __shfl_sync(kFull, sum, 31);
+        }
+        const uint64_t count = share_first(w_all, n, blockIdx.x + 1) - first;
+        at.b = b;
+        at.h = static_cast<uint32_t>((first - seen) / tiles);
+        at.t = static_cast<uint32_t>((first - seen) % tiles);
+        at.end = min(static_cast<uint64_t>(tiles), at.t + count);
+        at.left = count - (at.end - at.t);
+    }
+
+    // the copies run ahead of the arithmetic: `ahead` is the piece whose
+    // tiles are being requested, ahead_t the next tile of this warp in it
+    Piece ahead = at;
+    uint32_t ahead_t = at.t + warp;
+    uint32_t next_id = kNoNode;
+    bool have_next;
+    auto find_next = [&]() {            // to this warp's next tile, and its block's id
+        while (ahead_t >= ahead.end && ahead.b < a.d.num_seqs) {
+            next_piece(a, ahead);
+            ahead_t = ahead.t + warp;
+        }
+        have_next = ahead.b < a.d.num_seqs;
+        if (have_next)
+            next_id = a.d.table[static_cast<uint64_t>(ahead.b) * a.d.table_width + ahead_t * kTile / a.c.block];
+    };
+    auto request = [&](uint32_t stage) {
+        if (have_next) {
+            unsigned char* s = ring + stage * kStageBytes<NW>;
+            float* scales = reinterpret_cast<float*>(s + 2 * kTile * kPitch<NW>);
+            if (next_id < a.c.num_blocks) {
+                const uint64_t slab = static_cast<uint64_t>(next_id) * hkv + ahead.h;
+                const uint64_t row = (slab * a.c.block + (ahead_t * kTile) % a.c.block) * kDim;
+                for (uint32_t i = lane; i < kTile * NW; i += 32) {
+                    const uint32_t r = i / NW, x = i % NW;
+                    copy16(s + r * kPitch<NW> + x * 16, a.c.k + row + i * 16);
+                    copy16(s + (kTile + r) * kPitch<NW> + x * 16, a.c.v + row + i * 16);
+                }
+                if (lane == 0) copy4(scales, a.c.k_scale + slab);
+                if (lane == 1) copy4(scales + 1, a.c.v_scale + slab);
+            } else if (lane == 0) {
+                scales[0] = 0.f;
+                scales[1] = -1.f;          // no such block: its tokens are not seen
+                atomicOr(a.errors, kMemErrBlock);
+            }
+            ahead_t += kWarps;
+            find_next();
+        }
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+    };
+    find_next();
+    __syncthreads();                         // `sums` is done with
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) request(i);
+    uint32_t stage = 0, fill = kStages - 1;
+
+    for (bool first_piece = true; at.b < a.d.num_seqs; next_piece(a, at), first_piece = false) {
+        // this piece's query rows as the columns of K Q^T: column j is row row0 + j
+        uint32_t q[NT][NW][2];
+        float row_scale[NT][2];          // of columns 2c and 2c + 1
+        int32_t limit[NT][2];            // tokens that row sees
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t r = row0 + 8 * nt + g;
+            float2 x[NW][2];
+            float top = 0.f;
+            const bool real = r < a.rows;
+            const int64_t off = at.b * a.d.q_stride[0] + (r / a.group) * a.d.q_stride[1] +
+                                (at.h * a.group + r % a.group) * a.d.q_stride[2] + c * (NW * 4);
+#pragma unroll
+            for (int j = 0; j < NW; ++j) {
+                const uint2 u = real ? *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.d.q) + off + 4 * j) : make_uint2(0, 0);
+                if (a.d.dtype == BS_F16) {
+                    q[nt][j][0] = u.x;
+                    q[nt][j][1] = u.y;
+                } else {
+                    x[j][0] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
+                    x[j][1] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+                    top = fmaxf(fmaxf(top, fmaxf(fabsf(x[j][0].x), fabsf(x[j][0].y))), fmaxf(fabsf(x[j][1].x), fabsf(x[j][1].y)));
+                }
+            }
+            float scale = a.d.scale * 1.4426950408889634f;
+            if (a.d.dtype != BS_F16) {
+                top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
+                // 2^e with top * 2^e in [2^12, 2^13); rows of zeros, infinities and NaN as they are
+                const int e = top > 0.f && top < INFINITY ? 12 - ilogbf(top) : 0;
+#pragma unroll
+                for (int j = 0; j < NW; ++j) {
+                    const __half2 lo = __floats2half2_rn(scalbnf(x[j][0].x, e), scalbnf(x[j][0].y, e));
+                    const __half2 hi = __floats2half2_rn(scalbnf(x[j][1].x, e), scalbnf(x[j][1].y, e));
+                    q[nt][j][0] = *reinterpret_cast<const uint32_t*>(&lo);
+                    q[nt][j][1] = *reinterpret_cast<const uint32_t*>(&hi);
+                }
+                scale = scalbnf(scale, -e);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                row_scale[nt][i] = __shfl_sync(kFull, scale, (2 * c + i) * 4);
+                const uint32_t col = row0 + 8 * nt + 2 * c + i;
+                limit[nt][i] = static_cast<int32_t>(at.len) - a.d.queries + 1 + static_cast<int32_t>(col / a.group);
+            }
+        }
+        float o[NT][NW][4];
+        float top[NT][2], sum[NT][2], unit = 1e-30f;     // outputs count in 2^top * unit
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            top[nt][0] = top[nt][1] = kNoScore;
+            sum[nt][0] = sum[nt][1] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NW; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+        }
+        float* score_at = a.scores ? a.scores + (static_cast<uint64_t>(at.b) * hkv + at.h) * a.rows * a.score_width : nullptr;
+
+        for (uint32_t t = at.t + warp; t < at.end; t += kWarps) {
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
+            __syncwarp();
+            request(fill);               // the stage that the last tile used
+            fill = fill + 1 == kStages ? 0 : fill + 1;
+            const unsigned char* s = ring + stage * kStageBytes<NW>;
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+            const float2 scales = *reinterpret_cast<const float2*>(s + 2 * kTile * kPitch<NW>);
+
+            float z[NT][4];
+            {
+                uint32_t k0[NW], k1[NW];
+                load_key_words<NW>(k0, s + g * kPitch<NW>, c);
+                load_key_words<NW>(k1, s + (g + 8) * kPitch<NW>, c);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) z[nt][0] = z[nt][1] = z[nt][2] = z[nt][3] = 0.f;
+#pragma unroll
+                for (int j = 0; j < NW; ++j) {
+                    const uint32_t u0 = k0[j] ^ 0x80808080u, u1 = k1[j] ^ 0x80808080u;
+                    const uint32_t a0 = codes_to_half2(u0, kLow), a1 = codes_to_half2(u1, kLow);
+                    const uint32_t a2 = codes_to_half2(u0, kHigh), a3 = codes_to_half2(u1, kHigh);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma16(z[nt], a0, a1, a2, a3, q[nt][j][0], q[nt][j][1]);
+                }
+            }
+            const int32_t pos = static_cast<int32_t>(t * kTile + g);
+            const bool edge = static_cast<int32_t>((t + 1) * kTile) > static_cast<int32_t>(at.len) - a.d.queries + 1;
+            bool move = scales.y > 4.f * unit;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    z[nt][i] *= row_scale[nt][i & 1] * scales.x;
+                    if ((edge && pos + (i & 2) * 4 >= limit[nt][i & 1]) || scales.y < 0.f) z[nt][i] = -INFINITY;
+                    move |= z[nt][i] > top[nt][i & 1] + kSlack;
+                }
+            if (score_at) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t col = row0 + 8 * nt + 2 * c + i;
+                        if (col < a.rows) {
+                            float* p = score_at + static_cast<uint64_t>(col) * a.score_width + pos;
+                            p[0] = z[nt][i];
+                            p[8] = z[nt][2 + i];
+                        }
+                    }
+            }
+            if (__any_sync(kFull, move)) {       // rare: the maxima move, what was summed is rescaled
+                const float new_unit = fmaxf(unit, scales.y);
+                const float by_unit = unit / new_unit;
+                unit = new_unit;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float m = fmaxf(z[nt][i], z[nt][2 + i]);
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, x));
+                        m = fmaxf(m, top[nt][i]);
+                        const float shrink = exp2_fast(top[nt][i] - m);
+                        top[nt][i] = m;
+                        sum[nt][i] *= shrink;
+#pragma unroll
+                        for (int j = 0; j < NW; ++j) {
+                            o[nt][j][i] *= shrink * by_unit;
+                            o[nt][j][2 + i] *= shrink * by_unit;
+                        }
+                    }
+            }
+            const float v_scale = scales.y / unit;
+            uint32_t p[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[i] = exp2_fast(z[nt][i] - top[nt][i & 1]);
+                    sum[nt][i & 1] += w[i];
+                    w[i] *= v_scale;
+                }
+                const __half2 lo = __floats2half2_rn(w[0], w[1]), hi = __floats2half2_rn(w[2], w[3]);
+                p[nt][0] = transposed8x8(*reinterpret_cast<const uint32_t*>(&lo));
+                p[nt][1] = transposed8x8(*reinterpret_cast<const uint32_t*>(&hi));
+            }
+            {
+                const unsigned char* v = s + kTile * kPitch<NW>;
+                constexpr int kWords = (NW + 1) / 2;
+                uint32_t v0[kWords], v1[kWords], v2[kWords], v3[kWords];
+                load_value_words<NW>(v0, v + (2 * c) * kPitch<NW>, g);
+                load_value_words<NW>(v1, v + (2 * c + 1) * kPitch<NW>, g);
+                load_value_words<NW>(v2, v + (2 * c + 8) * kPitch<NW>, g);
+                load_value_words<NW>(v3, v + (2 * c + 9) * kPitch<NW>, g);
+#pragma unroll
+                for (int j = 0; j < NW; ++j) {
+                    const uint32_t pick = j % 2 ? 0x7362u : 0x5140u;      // the two tokens' bytes side by side
+                    const uint32_t x = __byte_perm(v0[j / 2], v1[j / 2], pick) ^ 0x80808080u;
+                    const uint32_t y = __byte_perm(v2[j / 2], v3[j / 2], pick) ^ 0x80808080u;
+                    const uint32_t a0 = codes_to_half2(x, kLow), a1 = codes_to_half2(x, kHigh);
+                    const uint32_t a2 = codes_to_half2(y, kLow), a3 = codes_to_half2(y, kHigh);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma16(o[nt][j], a0, a1, a2, a3, p[nt][0], p[nt][1]);
+                }
+            }
+            __syncwarp();
+        }
+
+        // the warps' maxima, then their sums and outputs as one
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) sum[nt][i] += __shfl_xor_sync(kFull, sum[nt][i], x);
+                if (g == 0) {
+                    float* ml = join_ml + (warp * kRows + 8 * nt + 2 * c + i) * 2;
+                    ml[0] = top[nt][i];
+                    ml[1] = sum[nt][i];
+                }
+            }
+        __syncthreads();
+        float all_top[NT][2], all_sum[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float* ml = join_ml + (8 * nt + 2 * c + i) * 2;
+                float m = kNoScore, l = 0.f;
+#pragma unroll
+                for (int x = 0; x < kWarps; ++x) m = fmaxf(m, ml[x * kRows * 2]);
+#pragma unroll
+                for (int x = 0; x < kWarps; ++x) l += ml[x * kRows * 2 + 1] * exp2_fast(ml[x * kRows * 2] - m);
+                const float f = exp2_fast(top[nt][i] - m) * unit;
+                all_top[nt][i] = m;
+                all_sum[nt][i] = l;
+#pragma unroll
+                for (int j = 0; j < NW; ++j) {
+                    o[nt][j][i] *= f;
+                    o[nt][j][2 + i] *= f;
+                }
+            }
+        auto put = [&](float* to) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < NW; ++j) *reinterpret_cast<float4*>(to + ((nt * NW + j) * 32 + lane) * 4) = *reinterpret_cast<float4*>(o[nt][j]);
+        };
+        auto add = [&](const float* from) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < NW; ++j) {
+                    const float4 x = *reinterpret_cast<const float4*>(from + ((nt * NW + j) * 32 + lane) * 4);
+                    o[nt][j][0] += x.x, o[nt][j][1] += x.y, o[nt][j][2] += x.z, o[nt][j][3] += x.w;
+                }
+        };
+        if (warp >= 2) put(join_o + (warp - 2) * kRows * kDim);
+        __syncthreads();
+        if (warp < 2) add(join_o + warp * kRows * kDim);
+        __syncthreads();
+        if (warp == 1) put(join_o);
+        __syncthreads();
+        if (warp == 0) {
+            add(join_o);
+            const bool whole = at.t == 0 && at.end == tiles_of(at.len);
+            const uint64_t slot = (static_cast<uint64_t>(blockIdx.y) * a.shares + blockIdx.x) * 2 + (first_piece ? 0 : 1);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t r = 8 * nt + 2 * c + i, col = row0 + r;
+                    if (col >= a.rows) continue;
+                    const float l = all_sum[nt][i];
+                    if (whole) {
+                        const uint64_t row = (static_cast<uint64_t>(at.b) * a.d.queries + col / a.group) * a.d.q_heads +
+                                             at.h * a.group + col % a.group;
+                        const float inv = l == 0.f ? 0.f : 1.f / l;
+                        if (g == 0) a.lse[row] = l == 0.f ? -INFINITY : (all_top[nt][i] + log2f(l)) * 0.6931471805599453f;
+#pragma unroll
+                        for (int j = 0; j < NW; ++j) {
+                            const float x = o[nt][j][i] * inv, y = o[nt][j][2 + i] * inv;
+                            const uint64_t e = row * kDim + value_dim<NW>(j, g);
+                            if (a.d.dtype == BS_F16) *reinterpret_cast<__half2*>(static_cast<__half*>(a.d.out) + e) = __floats2half2_rn(x, y);
+                            else *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.d.out) + e) = __floats2bfloat162_rn(x, y);
+                        }
+                    } else {
+                        if (g == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * kRows + r) * 2) = make_float2(all_top[nt][i], l);
+#pragma unroll
+                        for (int j = 0; j < NW; ++j)
+                            *reinterpret_cast<float2*>(a.part_o + (slot * kRows + r) * kDim + value_dim<NW>(j, g)) =
+                                make_float2(o[nt][j][i], o[nt][j][2 + i]);
+                    }
+                }
+        }
+    }
+}
+
+// One block per (sequence, key head, row tile): joins the pieces of a segment
+// that lies in several shares, writes zeros for an empty one.  Deterministic:
+// the pieces are added in order.
+constexpr int kJoinThreads = 128;
+__global__ void __launch_bounds__(kJoinThreads) k_cache_join(const __grid_constant__ CacheArgs a, uint32_t tile_rows) {
+    __shared__ uint64_t sums[2 * kJoinThreads / 32];
+    const uint32_t h = blockIdx.x, rt = blockIdx.y, b = blockIdx.z, hkv = a.c.kv_heads, dim = a.c.dim;
+    uint64_t before, all;
+    count_tiles(a, b, before, all, sums);
+    const uint32_t tiles = tiles_of(held_tokens(a, b));
+    const uint64_t w_all = all * hkv, s0 = before * hkv + static_cast<uint64_t>(h) * tiles;
+    const uint32_t rows = min(tile_rows, a.rows - rt * tile_rows);
+    uint32_t n = 0, i0 = 0, i1 = 0, slot0 = 0;
+    if (tiles) {
+        n = used_shares(w_all, a.shares);
+        i0 = share_of(w_all, n, s0);
+        i1 = share_of(w_all, n, s0 + tiles - 1);
+        if (i0 == i1) return;                                   // done by that share
+        slot0 = share_first(w_all, n, i0) >= s0 ? 0 : 1;        // later shares begin inside the segment: slot 0
+    }
+    for (uint32_t e = threadIdx.x; e < rows * (dim / 4); e += kJoinThreads) {
+        const uint32_t r = e / (dim / 4), x = e % (dim / 4) * 4, col = rt * tile_rows + r;
+        float m = kNoScore, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (tiles) {
+            auto slot = [&](uint32_t i) { return ((static_cast<uint64_t>(rt) * a.shares + i) * 2 + (i == i0 ? slot0 : 0)) * tile_rows + r; };
+            for (uint32_t i = i0; i <= i1; ++i) m = fmaxf(m, a.part_ml[slot(i) * 2]);
+            for (uint32_t i = i0; i <= i1; ++i) {
+                const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot(i) * 2);
+                const float4 o = *reinterpret_cast<const float4*>(a.part_o + slot(i) * dim + x);
+                const float f = exp2_fast(ml.x - m);
+                l += ml.y * f;
+                acc.x += o.x * f, acc.y += o.y * f, acc.z += o.z * f, acc.w += o.w * f;
+            }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const uint64_t row = (static_cast<uint64_t>(b) * a.d.queries + col / a.group) * a.d.q_heads + h * a.group + col % a.group;
+        if (x == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        if (a.d.dtype == BS_F16) {
+            __half2* p = reinterpret_cast<__half2*>(static_cast<__half*>(a.d.out) + row * dim + x);
+            p[0] = __floats2half2_rn(acc.x * inv, acc.y * inv);
+            p[1] = __floats2half2_rn(acc.z * inv, acc.w * inv);
+        } else {
+            __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.d.out) + row * dim + x);
+            p[0] = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
+            p[1] = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+        }
+    }
+}
+
+// One thread per token and key head: its weight over all query rows, from the
+// scores that the first kernel left and the rows' lse.
+__global__ void __launch_bounds__(256) k_cache_mass(const __grid_constant__ CacheArgs a) {
+    const uint32_t j = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y, b = blockIdx.z;
     if (j >= a.d.mass_width) return;
-    const uint32_t group = a.d.q_heads / a.c.kv_heads;
-    const uint64_t at = (static_cast<uint64_t>(b) * a.c.kv_heads + g) * a.d.mass_width + j;
+    const uint32_t len = held_tokens(a, b);
+    const uint64_t seg = static_cast<uint64_t>(b) * a.c.kv_heads + h, at = seg * a.d.mass_width + j;
     float w = 0.f;
     if (j < len) {
         w = a.d.mass ? a.d.mass[at] : 0.f;
-        for (int32_t i = 0; i < a.d.queries; ++i) {
-            if (static_cast<int64_t>(j) >= static_cast<int64_t>(len) - a.d.queries + 1 + i) continue;
-            for (uint32_t h = g * group; h < (g + 1) * group; ++h) {
-                const float lse = a.lse[(static_cast<uint64_t>(b) * a.d.queries + i) * a.d.q_heads + h];
-                w += expf(score<T>(a, query_row<T>(a, b, i, h), b, g, j) - lse);
-            }
+        const float* s = a.scores + seg * a.rows * a.score_width + j;
+        for (uint32_t r = 0; r < a.rows; ++r) {
+            const float lse = a.lse[(static_cast<uint64_t>(b) * a.d.queries + r / a.group) * a.d.q_heads + h * a.group + r % a.group];
+            const float z = s[static_cast<uint64_t>(r) * a.score_width];
+            if (z != -INFINITY) w += exp2_fast(z - lse * 1.4426950408889634f);
         }
     }
     a.d.out_mass[at] = w;
 }
 
-template <typename T>
-cudaError_t attention_typed(const CacheArgs& a, cudaStream_t stream) {
-    k_cache_rows<T><<<dim3(a.d.q_heads, a.d.queries, a.d.num_seqs), 32, 0, stream>>>(a);
-    if (a.d.out_mass)
-        k_cache_mass<T><<<dim3((a.d.mass_width + 255) / 256, a.c.kv_heads, a.d.num_seqs), 256, 0, stream>>>(a);
+struct Layout {
+    uint32_t nt, row_tiles, shares, score_width;
+    size_t lse, part_o, part_ml, scores, total;
+};
+
+Layout plan(const bs_token_cache& c, const bs_cache_attention_desc& d, const MemoryDevice& dev) {
+    Layout l{};
+    const uint32_t rows = static_cast<uint32_t>(d.q_heads / c.kv_heads) * d.queries;
+    l.nt = rows <= 8 ? 1 : 2;
+    l.row_tiles = (rows + 8 * l.nt - 1) / (8 * l.nt);
+    const uint64_t tokens = static_cast<uint64_t>(d.table_width) * c.block;      // a multiple of the tile
+    const uint64_t most = (static_cast<uint64_t>(d.num_seqs) * c.kv_heads * (tokens / kTile) + kWarps - 1) / kWarps;
+    const uint64_t cap = static_cast<uint64_t>(dev.num_sms) * blocks_per_sm(l.nt);
+    l.shares = static_cast<uint32_t>(most < cap ? most : cap);
+    l.score_width = static_cast<uint32_t>(tokens);
+    auto take = [&l](size_t bytes) {
+        const size_t at = l.total;
+        l.total += (bytes + 255) & ~static_cast<size_t>(255);
+        return at;
+    };
+    const size_t slots = static_cast<size_t>(l.row_tiles) * l.shares * 2 * 8 * l.nt;
+    l.lse = take(d.lse ? 0 : static_cast<size_t>(d.num_seqs) * d.queries * d.q_heads * 4);
+    l.part_ml = take(slots * 8);
+    l.part_o = take(slots * c.dim * 4);
+    l.scores = take(d.out_mass ? static_cast<size_t>(d.num_seqs) * c.kv_heads * rows * tokens * 4 : 0);
+    return l;
+}
+
+template <int NW, int NT>
+cudaError_t launch_split(const CacheArgs& a, uint32_t row_tiles, cudaStream_t stream) {
+    const cudaError_t e = cudaFuncSetAttribute(k_cache_split<NW, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitSmem<NW, NT>);
+    if (e != cudaSuccess) return e;
+    k_cache_split<NW, NT><<<dim3(a.shares, row_tiles), kThreads, kSplitSmem<NW, NT>, stream>>>(a);
     return cudaGetLastError();
+}
+
+template <int NT>
+cudaError_t launch_split(const CacheArgs& a, uint32_t row_tiles, cudaStream_t stream) {
+    switch (a.c.dim / 16) {
+        case 1: return launch_split<1, NT>(a, row_tiles, stream);
+        case 2: return launch_split<2, NT>(a, row_tiles, stream);
+        case 3: return launch_split<3, NT>(a, row_tiles, stream);
+        case 4: return launch_split<4, NT>(a, row_tiles, stream);
+        case 5: return launch_split<5, NT>(a, row_tiles, stream);
+        case 6: return launch_split<6, NT>(a, row_tiles, stream);
+        case 7: return launch_split<7, NT>(a, row_tiles, stream);
+        default: return launch_split<8, NT>(a, row_tiles, stream);
+    }
 }
 
 }  // namespace
 
-size_t cache_attention_scratch(const bs_token_cache&, const bs_cache_attention_desc& d, const MemoryDevice&) {
-    return d.lse ? 0 : static_cast<size_t>(d.num_seqs) * d.queries * d.q_heads * 4;
+size_t cache_attention_scratch(const bs_token_cache& c, const bs_cache_attention_desc& d, const MemoryDevice& dev) {
+    return plan(c, d, dev).total;
 }
 
 cudaError_t launch_cache_attention(const bs_token_cache& c, const bs_cache_attention_desc& d, const MemoryDevice& dev,
                                    cudaStream_t stream) {
-    const CacheArgs a{c, d, dev.errors, d.lse ? d.lse : static_cast<float*>(d.workspace)};
-    return d.dtype == BS_F16 ? attention_typed<__half>(a, stream) : attention_typed<__nv_bfloat16>(a, stream);
+    const Layout l = plan(c, d, dev);
+    unsigned char* work = static_cast<unsigned char*>(d.workspace);
+    CacheArgs a{c, d, dev.errors};
+    a.lse = d.lse ? d.lse : reinterpret_cast<float*>(work + l.lse);
+    a.part_o = reinterpret_cast<float*>(work + l.part_o);
+    a.part_ml = reinterpret_cast<float*>(work + l.part_ml);
+    a.scores = d.out_mass ? reinterpret_cast<float*>(work + l.scores) : nullptr;
+    a.group = d.q_heads / c.kv_heads;
+    a.rows = a.group * d.queries;
+    a.score_width = l.score_width;
+    a.shares = l.shares;
+    cudaError_t e = cudaSuccess;
+    if (l.shares) e = l.nt == 1 ? launch_split<1>(a, l.row_tiles, stream) : launch_split<2>(a, l.row_tiles, stream);
+    if (e != cudaSuccess) return e;
+    k_cache_join<<<dim3(c.kv_heads, l.row_tiles, d.num_seqs), kJoinThreads, 0, stream>>>(a, 8 * l.nt);
+    if (d.out_mass)
+        k_cache_mass<<<dim3((d.mass_width + 255) / 256, c.kv_heads, d.num_seqs), 256, 0, stream>>>(a);
+    return cudaGetLastError();
 }
 
 }  // namespace bsb
