@@ -3,10 +3,11 @@
 //
 // A few query rows (the heads that share a key head, times the query tokens)
 // meet a long cache once, so the time is the cache's bytes.  Every (sequence,
-// key head) is a segment of tiles of 16 tokens -- a tile never spans two
-// blocks, so it has one scale -- and all segments' tiles, end to end, are cut
-// into equal shares, one per thread block, whatever the lengths are.  A share
-// can end inside a segment; the pieces are joined by a second kernel.
+// key head) is a segment of tiles of 32 tokens, and all segments, end to end,
+// are cut into shares of equal cost, one per thread block, whatever the
+// lengths are.  A share can end inside a segment; the pieces are joined by a
+// second kernel.  A half of a tile (16 tokens) never spans two blocks, so it
+// has one scale.
 //
 // The matrix instructions are m16n8k16 with the TOKENS as the 16 rows of the
 // scores and the DIMENSIONS as the 16 rows of the outputs; the query rows are
@@ -38,9 +39,8 @@ namespace {
 constexpr int kWarps = 4;              // per block; they take a segment's tiles in turn
 constexpr int kThreads = kWarps * 32;
 constexpr int kStages = 3;             // tiles a warp has in flight or in use
-// Resident blocks: 3 x 165 registers for 8 query rows, 2 x 232 for 16 (at 3 they spill).
-constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
-constexpr int kTile = 16;              // tokens
+constexpr int kBlocksPerSm = 2;
+constexpr int kTile = 32;              // tokens: two halves of 16, independent chains of instructions
 constexpr float kNoScore = -1e30f;     // running maximum before the first score
 constexpr float kSlack = 8.f;          // weights may grow to 2^kSlack before the maximum is moved
 
@@ -56,6 +56,7 @@ struct CacheArgs {
     uint32_t rows;       // group * queries
     uint32_t score_width;
     uint32_t shares;     // thread blocks per row tile
+    uint32_t block_log2;
 };
 
 __device__ __forceinline__ uint32_t held_tokens(const CacheArgs& a, uint32_t b) {
@@ -68,27 +69,31 @@ __device__ __forceinline__ uint32_t held_tokens(const CacheArgs& a, uint32_t b) 
 
 __device__ __forceinline__ uint32_t tiles_of(uint32_t len) { return (len + kTile - 1) / kTile; }
 
-// Shares: W tiles over n blocks, block i has [first(i), first(i + 1)).  A
-// block gets at least one tile for each of its warps.
+// Shares.  A segment costs its tiles and kStart more for its queries and its
+// last reduction (measured: about 3 us against 0.45 us a tile of one block);
+// of W such units over n blocks, block i has first(i) .. first(i + 1).  A
+// segment's first kStart units stand for no tiles.
+constexpr uint32_t kStart = 6;
+__device__ __forceinline__ uint32_t cost_of(uint32_t len) { return len ? tiles_of(len) + kStart : 0; }
 __device__ __forceinline__ uint32_t used_shares(uint64_t w, uint32_t n) {
-    const uint64_t most = (w + kWarps - 1) / kWarps;
+    const uint64_t most = (w + kStart + kWarps - 1) / (kStart + kWarps);      // a tile for each warp at least
     return most < n ? static_cast<uint32_t>(most) : n;
 }
 __device__ __forceinline__ uint64_t share_first(uint64_t w, uint32_t n, uint32_t i) {
     return w / n * i + min(static_cast<uint64_t>(i), w % n);
 }
-// The block whose share holds tile x.
+// The block whose share holds unit x.
 __device__ __forceinline__ uint32_t share_of(uint64_t w, uint32_t n, uint64_t x) {
     const uint64_t q = w / n, r = w % n, wide = r * (q + 1);
     return static_cast<uint32_t>(x < wide ? x / (q + 1) : r + (x - wide) / q);
 }
 
-// Tiles of one key head's segments before sequence b, and of all sequences;
+// Cost of one key head's segments before sequence b, and of all sequences;
 // every thread of the block (a multiple of 32 threads) gets both.
-__device__ __forceinline__ void count_tiles(const CacheArgs& a, uint32_t b, uint64_t& before, uint64_t& all, uint64_t* warp_sums) {
+__device__ __forceinline__ void count_cost(const CacheArgs& a, uint32_t b, uint64_t& before, uint64_t& all, uint64_t* warp_sums) {
     uint64_t mine = 0, total = 0;
     for (uint32_t i = threadIdx.x; i < a.d.num_seqs; i += blockDim.x) {
-        const uint32_t t = tiles_of(held_tokens(a, i));
+        const uint32_t t = cost_of(held_tokens(a, i));
         total += t;
         mine += i < b ? t : 0;
     }
@@ -115,8 +120,16 @@ __device__ __forceinline__ void count_tiles(const CacheArgs& a, uint32_t b, uint
 struct Piece {
     uint32_t b, h, len;
     uint32_t t, end;        // tiles of the segment
-    uint64_t left;          // tiles of the share after this piece
+    uint64_t left;          // units of the share after this piece
 };
+
+// The piece of segment (b, h) from its unit `from` on.
+__device__ __forceinline__ void cut_piece(Piece& p, uint32_t from) {
+    const uint32_t cost = cost_of(p.len), take = p.left < cost - from ? static_cast<uint32_t>(p.left) : cost - from;
+    p.t = from > kStart ? from - kStart : 0;
+    p.end = from + take > kStart ? from + take - kStart : 0;
+    p.left -= take;
+}
 
 __device__ __forceinline__ void next_piece(const CacheArgs& a, Piece& p) {
     if (p.left == 0) {
@@ -131,10 +144,7 @@ __device__ __forceinline__ void next_piece(const CacheArgs& a, Piece& p) {
             p.len = held_tokens(a, p.b);
         } while (p.len == 0);
     }
-    const uint32_t tiles = tiles_of(p.len);
-    p.t = 0;
-    p.end = p.left < tiles ? static_cast<uint32_t>(p.left) : tiles;
-    p.left -= p.end;
+    cut_piece(p, 0);
 }
 
 __device__ __forceinline__ unsigned smem_addr(const void* p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
@@ -174,13 +184,25 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t biased, uint32_t sel
 }
 constexpr uint32_t kLow = 0x4140u, kHigh = 0x4342u;
 
+// Rows of a stage are an odd number of 16-byte units apart, so that the lanes
+// of a shared-memory access fall on different banks; rows of 128 bytes have no
+// gap (two blocks would not fit an SM) but their units permuted: unit x of row
+// r lies at x ^ (r & 7).
+template <int NW>
+constexpr int kPitch = NW == 8 ? 128 : 16 * (NW | 1);
+template <int NW>
+__device__ __forceinline__ uint32_t unit_at(uint32_t x, uint32_t row) {
+    return 16 * (NW == 8 ? x ^ (row & 7) : x);
+}
 // NW words (of 4 codes) per lane of a key row: the lane's quarter of it.
 template <int NW>
-__device__ __forceinline__ void load_key_words(uint32_t (&w)[NW], const unsigned char* row, uint32_t c) {
-    const unsigned char* p = row + c * (NW * 4);
+__device__ __forceinline__ void load_key_words(uint32_t (&w)[NW], const unsigned char* tile, uint32_t r, uint32_t c) {
+    const unsigned char* p = tile + r * kPitch<NW> + c * (NW * 4);
     if constexpr (NW % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < NW / 4; ++i) *reinterpret_cast<uint4*>(&w[4 * i]) = reinterpret_cast<const uint4*>(p)[i];
+        for (int i = 0; i < NW / 4; ++i)
+            *reinterpret_cast<uint4*>(&w[4 * i]) =
+                *reinterpret_cast<const uint4*>(tile + r * kPitch<NW> + unit_at<NW>(c * (NW / 4) + i, r));
     } else if constexpr (NW % 2 == 0) {
 #pragma unroll
         for (int i = 0; i < NW / 2; ++i) *reinterpret_cast<uint2*>(&w[2 * i]) = reinterpret_cast<const uint2*>(p)[i];
@@ -195,9 +217,10 @@ __device__ __forceinline__ void load_key_words(uint32_t (&w)[NW], const unsigned
 // they are 16 g + 2t, 8 g + 2t, or, by pairs of tiles, 32 (t / 2) + 4 g + 2 (t % 2)
 // (a last single tile: 16 t + 2 g); value_dim gives the dimension.
 template <int NW>
-__device__ __forceinline__ void load_value_words(uint32_t (&w)[(NW + 1) / 2], const unsigned char* row, uint32_t g) {
+__device__ __forceinline__ void load_value_words(uint32_t (&w)[(NW + 1) / 2], const unsigned char* tile, uint32_t r, uint32_t g) {
+    const unsigned char* row = tile + r * kPitch<NW>;
     if constexpr (NW == 8) {
-        *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(row + 16 * g);
+        *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(row + unit_at<NW>(g, r));
     } else if constexpr (NW == 4) {
         *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(row + 8 * g);
     } else {
@@ -214,12 +237,8 @@ __device__ __forceinline__ constexpr uint32_t value_dim(int t, uint32_t g) {
     return 32 * (t / 2) + 4 * g + 2 * (t % 2);
 }
 
-// Rows of a stage are an odd number of 16-byte units apart: the lanes of a
-// shared-memory access then fall on different banks.
 template <int NW>
-constexpr int kPitch = 16 * (NW | 1);
-template <int NW>
-constexpr int kStageBytes = 2 * kTile * kPitch<NW> + 16;      // keys, values, the two scales
+constexpr int kStageBytes = 2 * kTile * kPitch<NW> + 16;      // keys, values, (key, value) scales of the halves
 template <int NW, int NT>
 constexpr int kJoinBytes = 2 * 8 * NT * NW * 16 * 4;           // two warps' outputs
 template <int NW, int NT>
@@ -228,7 +247,7 @@ constexpr size_t kSplitSmem = kWarps * kStages * kStageBytes<NW> + kJoinBytes<NW
 // One share of the tiles for one row tile of 8 * NT query rows.
 // Registers: outputs NW * NT * 4, queries NW * NT * 2, and about 60.
 template <int NW, int NT>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(const __grid_constant__ CacheArgs a) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_cache_split(const __grid_constant__ CacheArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr int kDim = NW * 16, kRows = 8 * NT;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -240,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(con
     // this block's share, and the piece it begins with
     const uint32_t hkv = a.c.kv_heads, row0 = blockIdx.y * kRows;
     uint64_t before, all;
-    count_tiles(a, 0, before, all, sums);
+    count_cost(a, 0, before, all, sums);
     const uint64_t w_all = all * hkv;
     const uint32_t n = used_shares(w_all, a.shares);
     if (blockIdx.x >= n) return;
@@ -248,10 +267,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(con
     Piece at;
     {
         uint64_t seen = 0;
-        uint32_t b = 0, tiles = 0;
+        uint32_t b = 0;
         for (uint32_t b0 = 0;; b0 += 32) {                       // 32 sequences at a time
             const uint32_t len = b0 + lane < a.d.num_seqs ? held_tokens(a, b0 + lane) : 0;
-            uint64_t sum = static_cast<uint64_t>(tiles_of(len)) * hkv;
+            const uint64_t mine = static_cast<uint64_t>(cost_of(len)) * hkv;
+            uint64_t sum = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const uint64_t up = __shfl_up_sync(kFull, sum, o);
@@ -262,53 +282,62 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(con
                 const int l = __ffs(past) - 1;
                 b = b0 + l;
                 at.len = __shfl_sync(kFull, len, l);
-                tiles = tiles_of(at.len);
-                seen += __shfl_sync(kFull, sum, l) - static_cast<uint64_t>(tiles) * hkv;
+                seen += __shfl_sync(kFull, sum - mine, l);
                 break;
             }
             seen += __shfl_sync(kFull, sum, 31);
         }
-        const uint64_t count = share_first(w_all, n, blockIdx.x + 1) - first;
+        const uint32_t cost = cost_of(at.len);
         at.b = b;
-        at.h = static_cast<uint32_t>((first - seen) / tiles);
-        at.t = static_cast<uint32_t>((first - seen) % tiles);
-        at.end = min(static_cast<uint64_t>(tiles), at.t + count);
-        at.left = count - (at.end - at.t);
+        at.h = static_cast<uint32_t>((first - seen) / cost);
+        at.left = share_first(w_all, n, blockIdx.x + 1) - first;
+        cut_piece(at, static_cast<uint32_t>((first - seen) % cost));
     }
 
     // the copies run ahead of the arithmetic: `ahead` is the piece whose
     // tiles are being requested, ahead_t the next tile of this warp in it
     Piece ahead = at;
     uint32_t ahead_t = at.t + warp;
-    uint32_t next_id = kNoNode;
+    uint32_t next_id[2];
     bool have_next;
-    auto find_next = [&]() {            // to this warp's next tile, and its block's id
+    auto find_next = [&]() {            // to this warp's next tile, and its halves' block ids
         while (ahead_t >= ahead.end && ahead.b < a.d.num_seqs) {
             next_piece(a, ahead);
             ahead_t = ahead.t + warp;
         }
         have_next = ahead.b < a.d.num_seqs;
-        if (have_next)
-            next_id = a.d.table[static_cast<uint64_t>(ahead.b) * a.d.table_width + ahead_t * kTile / a.c.block];
+        if (have_next) {
+            const int32_t* row = a.d.table + static_cast<uint64_t>(ahead.b) * a.d.table_width;
+            next_id[0] = row[ahead_t * kTile >> a.block_log2];
+            next_id[1] = next_id[0];
+            if (a.block_log2 == 4 && ahead_t * kTile + 16 < ahead.len) next_id[1] = row[ahead_t * 2 + 1];
+        }
     };
     auto request = [&](uint32_t stage) {
         if (have_next) {
             unsigned char* s = ring + stage * kStageBytes<NW>;
             float* scales = reinterpret_cast<float*>(s + 2 * kTile * kPitch<NW>);
-            if (next_id < a.c.num_blocks) {
-                const uint64_t slab = static_cast<uint64_t>(next_id) * hkv + ahead.h;
-                const uint64_t row = (slab * a.c.block + (ahead_t * kTile) % a.c.block) * kDim;
-                for (uint32_t i = lane; i < kTile * NW; i += 32) {
-                    const uint32_t r = i / NW, x = i % NW;
-                    copy16(s + r * kPitch<NW> + x * 16, a.c.k + row + i * 16);
-                    copy16(s + (kTile + r) * kPitch<NW> + x * 16, a.c.v + row + i * 16);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t id = next_id[half], pos = ahead_t * kTile + 16 * half;
+                if (id < a.c.num_blocks && pos < ahead.len) {
+                    const uint64_t slab = static_cast<uint64_t>(id) * hkv + ahead.h;
+                    const uint64_t row = ((slab << a.block_log2) + (pos & (a.c.block - 1))) * kDim + lane * 16;
+                    const int8_t* k = a.c.k + row;
+                    const int8_t* v = a.c.v + row;
+#pragma unroll
+                    for (int j = 0; j < (NW + 1) / 2; ++j) {
+                        const uint32_t i = lane + 32 * j, r = i / NW + 16 * half, x = i % NW;
+                        if (NW % 2 && i >= 16 * NW) break;
+                        copy16(s + r * kPitch<NW> + unit_at<NW>(x, r), k + j * 512);
+                        copy16(s + (kTile + r) * kPitch<NW> + unit_at<NW>(x, r), v + j * 512);
+                    }
+                    if (lane < 2) copy4(scales + 2 * half + lane, (lane ? a.c.v_scale : a.c.k_scale) + slab);
+                } else if (lane == 0) {       // no tokens to see: a value scale below zero says so
+                    scales[2 * half] = 0.f;
+                    scales[2 * half + 1] = -1.f;
+                    if (pos < ahead.len) atomicOr(a.errors, kMemErrBlock);
                 }
-                if (lane == 0) copy4(scales, a.c.k_scale + slab);
-                if (lane == 1) copy4(scales + 1, a.c.v_scale + slab);
-            } else if (lane == 0) {
-                scales[0] = 0.f;
-                scales[1] = -1.f;          // no such block: its tokens are not seen
-                atomicOr(a.errors, kMemErrBlock);
             }
             ahead_t += kWarps;
             find_next();
@@ -321,55 +350,65 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(con
     for (int i = 0; i < kStages - 1; ++i) request(i);
     uint32_t stage = 0, fill = kStages - 1;
 
+    // where this lane's query rows (columns of the products) lie within a
+    // sequence and key head, and which query its columns 2c and 2c + 1 are
+    int64_t row_off[NT];
+    int32_t col_query[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const uint32_t r = row0 + 8 * nt + g, col = row0 + 8 * nt + 2 * c;
+        row_off[nt] = (r / a.group) * a.d.q_stride[1] + (r % a.group) * a.d.q_stride[2] + c * (NW * 4);
+        col_query[nt][0] = static_cast<int32_t>(col / a.group);
+        col_query[nt][1] = static_cast<int32_t>((col + 1) / a.group);
+    }
+
     for (bool first_piece = true; at.b < a.d.num_seqs; next_piece(a, at), first_piece = false) {
+        if (at.t == at.end) continue;      // a share that ends before a segment's first tile
         // this piece's query rows as the columns of K Q^T: column j is row row0 + j
         uint32_t q[NT][NW][2];
         float row_scale[NT][2];          // of columns 2c and 2c + 1
         int32_t limit[NT][2];            // tokens that row sees
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const uint32_t r = row0 + 8 * nt + g;
-            float2 x[NW][2];
-            float top = 0.f;
-            const bool real = r < a.rows;
-            const int64_t off = at.b * a.d.q_stride[0] + (r / a.group) * a.d.q_stride[1] +
-                                (at.h * a.group + r % a.group) * a.d.q_stride[2] + c * (NW * 4);
+            const uint16_t* row = static_cast<const uint16_t*>(a.d.q) + at.b * a.d.q_stride[0] +
+                                  static_cast<int64_t>(at.h) * a.group * a.d.q_stride[2] + row_off[nt];
 #pragma unroll
             for (int j = 0; j < NW; ++j) {
-                const uint2 u = real ? *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.d.q) + off + 4 * j) : make_uint2(0, 0);
-                if (a.d.dtype == BS_F16) {
-                    q[nt][j][0] = u.x;
-                    q[nt][j][1] = u.y;
-                } else {
-                    x[j][0] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
-                    x[j][1] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
-                    top = fmaxf(fmaxf(top, fmaxf(fabsf(x[j][0].x), fabsf(x[j][0].y))), fmaxf(fabsf(x[j][1].x), fabsf(x[j][1].y)));
-                }
+                const uint2 u = row0 + 8 * nt + g < a.rows ? *reinterpret_cast<const uint2*>(row + 4 * j) : make_uint2(0, 0);
+                q[nt][j][0] = u.x;
+                q[nt][j][1] = u.y;
             }
             float scale = a.d.scale * 1.4426950408889634f;
             if (a.d.dtype != BS_F16) {
-                top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
-                // 2^e with top * 2^e in [2^12, 2^13); rows of zeros, infinities and NaN as they are
-                const int e = top > 0.f && top < INFINITY ? 12 - ilogbf(top) : 0;
+                // times 2^e with the row's largest in [2^12, 2^13); rows of zeros, infinities and NaN as they are
+                uint32_t top = 0;        // magnitudes of bf16 order as integers
 #pragma unroll
-                for (int j = 0; j < NW; ++j) {
-                    const __half2 lo = __floats2half2_rn(scalbnf(x[j][0].x, e), scalbnf(x[j][0].y, e));
-                    const __half2 hi = __floats2half2_rn(scalbnf(x[j][1].x, e), scalbnf(x[j][1].y, e));
-                    q[nt][j][0] = *reinterpret_cast<const uint32_t*>(&lo);
-                    q[nt][j][1] = *reinterpret_cast<const uint32_t*>(&hi);
-                }
-                scale = scalbnf(scale, -e);
+                for (int j = 0; j < NW; ++j)
+                    top = __vmaxu2(top, __vmaxu2(q[nt][j][0] & 0x7fff7fffu, q[nt][j][1] & 0x7fff7fffu));
+                top = max(top >> 16, top & 0xffffu);
+                top = max(top, __shfl_xor_sync(kFull, top, 1));
+                top = max(top, __shfl_xor_sync(kFull, top, 2));
+                uint32_t e = top >> 7;   // biased exponent
+                e = top == 0 || e == 255 ? 139 : e < 13 ? 13 : e;
+                const float up = __uint_as_float((266 - e) << 23), down = __uint_as_float((e - 12) << 23);
+#pragma unroll
+                for (int j = 0; j < NW; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const __half2 h = __floats2half2_rn(__uint_as_float(q[nt][j][i] << 16) * up,
+                                                            __uint_as_float(q[nt][j][i] & 0xffff0000u) * up);
+                        q[nt][j][i] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                scale *= down;
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 row_scale[nt][i] = __shfl_sync(kFull, scale, (2 * c + i) * 4);
-                const uint32_t col = row0 + 8 * nt + 2 * c + i;
-                limit[nt][i] = static_cast<int32_t>(at.len) - a.d.queries + 1 + static_cast<int32_t>(col / a.group);
+                limit[nt][i] = static_cast<int32_t>(at.len) - a.d.queries + 1 + col_query[nt][i];
             }
         }
         float o[NT][NW][4];
-        float top[NT][2], sum[NT][2], unit = 1e-30f;     // outputs count in 2^top * unit
+        float top[NT][2], sum[NT][2], unit = 1e-30f, inv_unit = 1e30f;     // outputs count in 2^top * unit
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             top[nt][0] = top[nt][1] = kNoScore;
@@ -377,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(con
 #pragma unroll
             for (int j = 0; j < NW; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
         }
-        float* score_at = a.scores ? a.scores + (static_cast<uint64_t>(at.b) * hkv + at.h) * a.rows * a.score_width : nullptr;
+        float* score_at = a.scores ? a.scores + ((static_cast<uint64_t>(at.b) * hkv + at.h) * a.rows + row0 + 2 * c) * a.score_width + g : nullptr;
 
         for (uint32_t t = at.t + warp; t < at.end; t += kWarps) {
             asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
@@ -386,57 +425,73 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(con
             fill = fill + 1 == kStages ? 0 : fill + 1;
             const unsigned char* s = ring + stage * kStageBytes<NW>;
             stage = stage + 1 == kStages ? 0 : stage + 1;
-            const float2 scales = *reinterpret_cast<const float2*>(s + 2 * kTile * kPitch<NW>);
+            const float4 sc = *reinterpret_cast<const float4*>(s + 2 * kTile * kPitch<NW>);
+            const float k_scale[2] = {sc.x, sc.z}, v_scale[2] = {sc.y, sc.w};
 
-            float z[NT][4];
+            float z[2][NT][4];           // [half]: tokens g and g + 8 (+ 16 half), columns 2c and 2c + 1
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) z[half][nt][0] = z[half][nt][1] = z[half][nt][2] = z[half][nt][3] = 0.f;
             {
-                uint32_t k0[NW], k1[NW];
-                load_key_words<NW>(k0, s + g * kPitch<NW>, c);
-                load_key_words<NW>(k1, s + (g + 8) * kPitch<NW>, c);
+                uint32_t k[2][2][NW];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) z[nt][0] = z[nt][1] = z[nt][2] = z[nt][3] = 0.f;
-#pragma unroll
-                for (int j = 0; j < NW; ++j) {
-                    const uint32_t u0 = k0[j] ^ 0x80808080u, u1 = k1[j] ^ 0x80808080u;
-                    const uint32_t a0 = codes_to_half2(u0, kLow), a1 = codes_to_half2(u1, kLow);
-                    const uint32_t a2 = codes_to_half2(u0, kHigh), a3 = codes_to_half2(u1, kHigh);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma16(z[nt], a0, a1, a2, a3, q[nt][j][0], q[nt][j][1]);
+                for (int half = 0; half < 2; ++half) {
+                    load_key_words<NW>(k[half][0], s, 16 * half + g, c);
+                    load_key_words<NW>(k[half][1], s, 16 * half + g + 8, c);
                 }
+#pragma unroll
+                for (int j = 0; j < NW; ++j)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t u0 = k[half][0][j] ^ 0x80808080u, u1 = k[half][1][j] ^ 0x80808080u;
+                        const uint32_t a0 = codes_to_half2(u0, kLow), a1 = codes_to_half2(u1, kLow);
+                        const uint32_t a2 = codes_to_half2(u0, kHigh), a3 = codes_to_half2(u1, kHigh);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma16(z[half][nt], a0, a1, a2, a3, q[nt][j][0], q[nt][j][1]);
+                    }
             }
-            const int32_t pos = static_cast<int32_t>(t * kTile + g);
-            const bool edge = static_cast<int32_t>((t + 1) * kTile) > static_cast<int32_t>(at.len) - a.d.queries + 1;
-            bool move = scales.y > 4.f * unit;
+            const bool edge = static_cast<int32_t>((t + 1) * kTile) > static_cast<int32_t>(at.len) - a.d.queries + 1 ||
+                              fminf(v_scale[0], v_scale[1]) < 0.f;
+            bool move = fmaxf(v_scale[0], v_scale[1]) > 4.f * unit;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    z[nt][i] *= row_scale[nt][i & 1] * scales.x;
-                    if ((edge && pos + (i & 2) * 4 >= limit[nt][i & 1]) || scales.y < 0.f) z[nt][i] = -INFINITY;
-                    move |= z[nt][i] > top[nt][i & 1] + kSlack;
-                }
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        z[half][nt][i] *= row_scale[nt][i & 1] * k_scale[half];
+                        if (edge) {
+                            const int32_t pos = static_cast<int32_t>(t * kTile + 16 * half + g) + (i & 2) * 4;
+                            if (pos >= limit[nt][i & 1] || v_scale[half] < 0.f) z[half][nt][i] = -INFINITY;
+                        }
+                        move |= z[half][nt][i] > top[nt][i & 1] + kSlack;
+                    }
             if (score_at) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t col = row0 + 8 * nt + 2 * c + i;
-                        if (col < a.rows) {
-                            float* p = score_at + static_cast<uint64_t>(col) * a.score_width + pos;
-                            p[0] = z[nt][i];
-                            p[8] = z[nt][2 + i];
+                    for (int i = 0; i < 2; ++i)
+                        if (row0 + 8 * nt + 2 * c + i < a.rows) {
+                            float* p = score_at + static_cast<uint64_t>(8 * nt + i) * a.score_width + t * kTile;
+                            p[0] = z[0][nt][i];
+                            p[8] = z[0][nt][2 + i];
+                            if (t * kTile + 16 < at.len) {
+                                p[16] = z[1][nt][i];
+                                p[24] = z[1][nt][2 + i];
+                            }
                         }
-                    }
             }
             if (__any_sync(kFull, move)) {       // rare: the maxima move, what was summed is rescaled
-                const float new_unit = fmaxf(unit, scales.y);
+                const float new_unit = fmaxf(unit, fmaxf(v_scale[0], v_scale[1]));
                 const float by_unit = unit / new_unit;
                 unit = new_unit;
+                inv_unit = 1.f / unit;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float m = fmaxf(z[nt][i], z[nt][2 + i]);
+                        float m = fmaxf(fmaxf(z[0][nt][i], z[0][nt][2 + i]), fmaxf(z[1][nt][i], z[1][nt][2 + i]));
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, x));
                         m = fmaxf(m, top[nt][i]);
@@ -450,29 +505,30 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(con
                         }
                     }
             }
-            const float v_scale = scales.y / unit;
-            uint32_t p[NT][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float w[4];
+            for (int half = 0; half < 2; ++half) {
+                const float by = v_scale[half] * inv_unit;
+                uint32_t p[NT][2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    w[i] = exp2_fast(z[nt][i] - top[nt][i & 1]);
-                    sum[nt][i & 1] += w[i];
-                    w[i] *= v_scale;
+                for (int nt = 0; nt < NT; ++nt) {
+                    float w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        w[i] = exp2_fast(z[half][nt][i] - top[nt][i & 1]);
+                        sum[nt][i & 1] += w[i];
+                        w[i] *= by;
+                    }
+                    const __half2 lo = __floats2half2_rn(w[0], w[1]), hi = __floats2half2_rn(w[2], w[3]);
+                    p[nt][0] = transposed8x8(*reinterpret_cast<const uint32_t*>(&lo));
+                    p[nt][1] = transposed8x8(*reinterpret_cast<const uint32_t*>(&hi));
                 }
-                const __half2 lo = __floats2half2_rn(w[0], w[1]), hi = __floats2half2_rn(w[2], w[3]);
-                p[nt][0] = transposed8x8(*reinterpret_cast<const uint32_t*>(&lo));
-                p[nt][1] = transposed8x8(*reinterpret_cast<const uint32_t*>(&hi));
-            }
-            {
                 const unsigned char* v = s + kTile * kPitch<NW>;
                 constexpr int kWords = (NW + 1) / 2;
                 uint32_t v0[kWords], v1[kWords], v2[kWords], v3[kWords];
-                load_value_words<NW>(v0, v + (2 * c) * kPitch<NW>, g);
-                load_value_words<NW>(v1, v + (2 * c + 1) * kPitch<NW>, g);
-                load_value_words<NW>(v2, v + (2 * c + 8) * kPitch<NW>, g);
-                load_value_words<NW>(v3, v + (2 * c + 9) * kPitch<NW>, g);
+                load_value_words<NW>(v0, v, 16 * half + 2 * c, g);
+                load_value_words<NW>(v1, v, 16 * half + 2 * c + 1, g);
+                load_value_words<NW>(v2, v, 16 * half + 2 * c + 8, g);
+                load_value_words<NW>(v3, v, 16 * half + 2 * c + 9, g);
 #pragma unroll
                 for (int j = 0; j < NW; ++j) {
                     const uint32_t pick = j % 2 ? 0x7362u : 0x5140u;      // the two tokens' bytes side by side
@@ -554,8 +610,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(con
                     if (col >= a.rows) continue;
                     const float l = all_sum[nt][i];
                     if (whole) {
-                        const uint64_t row = (static_cast<uint64_t>(at.b) * a.d.queries + col / a.group) * a.d.q_heads +
-                                             at.h * a.group + col % a.group;
+                        const uint32_t query = col_query[nt][i];
+                        const uint64_t row = (static_cast<uint64_t>(at.b) * a.d.queries + query) * a.d.q_heads + at.h * a.group +
+                                             (col - query * a.group);
                         const float inv = l == 0.f ? 0.f : 1.f / l;
                         if (g == 0) a.lse[row] = l == 0.f ? -INFINITY : (all_top[nt][i] + log2f(l)) * 0.6931471805599453f;
 #pragma unroll
@@ -577,33 +634,36 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(con
     }
 }
 
-// One block per (sequence, key head, row tile): joins the pieces of a segment
-// that lies in several shares, writes zeros for an empty one.  Deterministic:
-// the pieces are added in order.
+// Joins the pieces of a segment that lies in several shares, writes zeros for
+// an empty one; a thread has four dimensions of one row, `parts` blocks share
+// a (sequence, key head, row tile).  Deterministic: pieces are added in order.
 constexpr int kJoinThreads = 128;
-__global__ void __launch_bounds__(kJoinThreads) k_cache_join(const __grid_constant__ CacheArgs a, uint32_t tile_rows) {
+__global__ void __launch_bounds__(kJoinThreads) k_cache_join(const __grid_constant__ CacheArgs a, uint32_t tile_rows, uint32_t parts) {
     __shared__ uint64_t sums[2 * kJoinThreads / 32];
-    const uint32_t h = blockIdx.x, rt = blockIdx.y, b = blockIdx.z, hkv = a.c.kv_heads, dim = a.c.dim;
+    const uint32_t h = blockIdx.x / parts, rt = blockIdx.y, b = blockIdx.z, hkv = a.c.kv_heads, dim = a.c.dim;
     uint64_t before, all;
-    count_tiles(a, b, before, all, sums);
+    count_cost(a, b, before, all, sums);
     const uint32_t tiles = tiles_of(held_tokens(a, b));
-    const uint64_t w_all = all * hkv, s0 = before * hkv + static_cast<uint64_t>(h) * tiles;
+    const uint64_t w_all = all * hkv, s0 = before * hkv + static_cast<uint64_t>(h) * (tiles + kStart);
     const uint32_t rows = min(tile_rows, a.rows - rt * tile_rows);
     uint32_t n = 0, i0 = 0, i1 = 0, slot0 = 0;
     if (tiles) {
         n = used_shares(w_all, a.shares);
-        i0 = share_of(w_all, n, s0);
-        i1 = share_of(w_all, n, s0 + tiles - 1);
+        i0 = share_of(w_all, n, s0 + kStart);                   // the segment's first and last tile
+        i1 = share_of(w_all, n, s0 + kStart + tiles - 1);
         if (i0 == i1) return;                                   // done by that share
         slot0 = share_first(w_all, n, i0) >= s0 ? 0 : 1;        // later shares begin inside the segment: slot 0
     }
-    for (uint32_t e = threadIdx.x; e < rows * (dim / 4); e += kJoinThreads) {
+    const uint32_t e = blockIdx.x % parts * kJoinThreads + threadIdx.x;
+    if (e < rows * (dim / 4)) {
         const uint32_t r = e / (dim / 4), x = e % (dim / 4) * 4, col = rt * tile_rows + r;
         float m = kNoScore, l = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         if (tiles) {
             auto slot = [&](uint32_t i) { return ((static_cast<uint64_t>(rt) * a.shares + i) * 2 + (i == i0 ? slot0 : 0)) * tile_rows + r; };
+#pragma unroll 8
             for (uint32_t i = i0; i <= i1; ++i) m = fmaxf(m, a.part_ml[slot(i) * 2]);
+#pragma unroll 8
             for (uint32_t i = i0; i <= i1; ++i) {
                 const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot(i) * 2);
                 const float4 o = *reinterpret_cast<const float4*>(a.part_o + slot(i) * dim + x);
@@ -627,24 +687,41 @@ __global__ void __launch_bounds__(kJoinThreads) k_cache_join(const __grid_consta
     }
 }
 
-// One thread per token and key head: its weight over all query rows, from the
-// scores that the first kernel left and the rows' lse.
-__global__ void __launch_bounds__(256) k_cache_mass(const __grid_constant__ CacheArgs a) {
-    const uint32_t j = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y, b = blockIdx.z;
-    if (j >= a.d.mass_width) return;
+// One thread per four tokens of a key head: their weights over all query
+// rows, from the scores that the first kernel left and the rows' lse.
+constexpr int kMassThreads = 128;
+__global__ void __launch_bounds__(kMassThreads) k_cache_mass(const __grid_constant__ CacheArgs a) {
+    const uint32_t j = (blockIdx.x * kMassThreads + threadIdx.x) * 4, h = blockIdx.y, b = blockIdx.z;
+    const uint32_t width = a.d.mass_width;
+    if (j >= width) return;
     const uint32_t len = held_tokens(a, b);
-    const uint64_t seg = static_cast<uint64_t>(b) * a.c.kv_heads + h, at = seg * a.d.mass_width + j;
-    float w = 0.f;
-    if (j < len) {
-        w = a.d.mass ? a.d.mass[at] : 0.f;
+    const uint64_t seg = static_cast<uint64_t>(b) * a.c.kv_heads + h, at = seg * width + j;
+    const uint32_t n = j < len ? min(len - j, 4u) : 0;
+    // four at once where their place is a multiple of 16 bytes
+    const bool whole = j + 4 <= width && width % 4 == 0 &&
+                       ((reinterpret_cast<uintptr_t>(a.d.mass) | reinterpret_cast<uintptr_t>(a.d.out_mass)) & 15) == 0;
+    float w[4] = {0.f, 0.f, 0.f, 0.f};
+    if (n && a.d.mass) {
+        if (whole) *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(a.d.mass + at);
+        else
+            for (uint32_t i = 0; i < n && j + i < width; ++i) w[i] = a.d.mass[at + i];
+    }
+    if (n) {
         const float* s = a.scores + seg * a.rows * a.score_width + j;
         for (uint32_t r = 0; r < a.rows; ++r) {
-            const float lse = a.lse[(static_cast<uint64_t>(b) * a.d.queries + r / a.group) * a.d.q_heads + h * a.group + r % a.group];
-            const float z = s[static_cast<uint64_t>(r) * a.score_width];
-            if (z != -INFINITY) w += exp2_fast(z - lse * 1.4426950408889634f);
+            const float lse = a.lse[(static_cast<uint64_t>(b) * a.d.queries + r / a.group) * a.d.q_heads + h * a.group + r % a.group] *
+                              1.4426950408889634f;
+            const float4 z = *reinterpret_cast<const float4*>(s + static_cast<uint64_t>(r) * a.score_width);
+            if (z.x != -INFINITY) w[0] += exp2_fast(z.x - lse);
+            if (z.y != -INFINITY) w[1] += exp2_fast(z.y - lse);
+            if (z.z != -INFINITY) w[2] += exp2_fast(z.z - lse);
+            if (z.w != -INFINITY) w[3] += exp2_fast(z.w - lse);
         }
     }
-    a.d.out_mass[at] = w;
+    for (uint32_t i = n; i < 4; ++i) w[i] = 0.f;
+    if (whole) *reinterpret_cast<float4*>(a.d.out_mass + at) = *reinterpret_cast<const float4*>(w);
+    else
+        for (uint32_t i = 0; i < 4 && j + i < width; ++i) a.d.out_mass[at + i] = w[i];
 }
 
 struct Layout {
@@ -657,9 +734,10 @@ Layout plan(const bs_token_cache& c, const bs_cache_attention_desc& d, const Mem
     const uint32_t rows = static_cast<uint32_t>(d.q_heads / c.kv_heads) * d.queries;
     l.nt = rows <= 8 ? 1 : 2;
     l.row_tiles = (rows + 8 * l.nt - 1) / (8 * l.nt);
-    const uint64_t tokens = static_cast<uint64_t>(d.table_width) * c.block;      // a multiple of the tile
-    const uint64_t most = (static_cast<uint64_t>(d.num_seqs) * c.kv_heads * (tokens / kTile) + kWarps - 1) / kWarps;
-    const uint64_t cap = static_cast<uint64_t>(dev.num_sms) * blocks_per_sm(l.nt);
+    const uint64_t tokens = static_cast<uint64_t>(d.table_width) * c.block;
+    const uint64_t most = (static_cast<uint64_t>(d.num_seqs) * c.kv_heads * ((tokens + kTile - 1) / kTile + kStart) + kStart + kWarps - 1) /
+                          (kStart + kWarps);
+    const uint64_t cap = static_cast<uint64_t>(dev.num_sms) * kBlocksPerSm;
     l.shares = static_cast<uint32_t>(most < cap ? most : cap);
     l.score_width = static_cast<uint32_t>(tokens);
     auto take = [&l](size_t bytes) {
@@ -716,12 +794,15 @@ cudaError_t launch_cache_attention(const bs_token_cache& c, const bs_cache_atten
     a.rows = a.group * d.queries;
     a.score_width = l.score_width;
     a.shares = l.shares;
+    a.block_log2 = c.block == 16 ? 4 : c.block == 32 ? 5 : c.block == 64 ? 6 : 7;
     cudaError_t e = cudaSuccess;
     if (l.shares) e = l.nt == 1 ? launch_split<1>(a, l.row_tiles, stream) : launch_split<2>(a, l.row_tiles, stream);
     if (e != cudaSuccess) return e;
-    k_cache_join<<<dim3(c.kv_heads, l.row_tiles, d.num_seqs), kJoinThreads, 0, stream>>>(a, 8 * l.nt);
+    const uint32_t tile_rows = a.rows < 8 * l.nt ? a.rows : 8 * l.nt;
+    const uint32_t parts = (tile_rows * (c.dim / 4) + kJoinThreads - 1) / kJoinThreads;
+    k_cache_join<<<dim3(c.kv_heads * parts, l.row_tiles, d.num_seqs), kJoinThreads, 0, stream>>>(a, 8 * l.nt, parts);
     if (d.out_mass)
-        k_cache_mass<<<dim3((d.mass_width + 255) / 256, c.kv_heads, d.num_seqs), 256, 0, stream>>>(a);
+        k_cache_mass<<<dim3((d.mass_width + 4 * kMassThreads - 1) / (4 * kMassThreads), c.kv_heads, d.num_seqs), kMassThreads, 0, stream>>>(a);
     return cudaGetLastError();
 }
 
