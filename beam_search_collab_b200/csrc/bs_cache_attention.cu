@@ -634,56 +634,82 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_cache_split(const __
     }
 }
 
-// Joins the pieces of a segment that lies in several shares, writes zeros for
-// an empty one; a thread has four dimensions of one row, `parts` blocks share
-// a (sequence, key head, row tile).  Deterministic: pieces are added in order.
+// One block per row: joins the pieces of a segment that lies in several
+// shares, writes zeros for an empty one.  A lane has four dimensions, the
+// warps take the pieces in turn.  Always the same order of additions.
+// Launched while the first kernel still runs; waits for it before it reads.
 constexpr int kJoinThreads = 128;
-__global__ void __launch_bounds__(kJoinThreads) k_cache_join(const __grid_constant__ CacheArgs a, uint32_t tile_rows, uint32_t parts) {
-    __shared__ uint64_t sums[2 * kJoinThreads / 32];
-    const uint32_t h = blockIdx.x / parts, rt = blockIdx.y, b = blockIdx.z, hkv = a.c.kv_heads, dim = a.c.dim;
+__global__ void __launch_bounds__(kJoinThreads) k_cache_join(const __grid_constant__ CacheArgs a, uint32_t tile_rows, uint32_t used_rows) {
+    constexpr uint32_t kJoinWarps = kJoinThreads / 32;
+    __shared__ uint64_t sums[2 * kJoinWarps];
+    __shared__ float4 parts[kJoinWarps][32];
+    const uint32_t h = blockIdx.x / used_rows, r = blockIdx.x % used_rows, rt = blockIdx.y, b = blockIdx.z;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hkv = a.c.kv_heads, dim = a.c.dim, col = rt * tile_rows + r;
     uint64_t before, all;
     count_cost(a, b, before, all, sums);
     const uint32_t tiles = tiles_of(held_tokens(a, b));
+    cudaGridDependencySynchronize();       // in every block: what follows this kernel may count on both being done
+    if (col >= a.rows) return;
     const uint64_t w_all = all * hkv, s0 = before * hkv + static_cast<uint64_t>(h) * (tiles + kStart);
-    const uint32_t rows = min(tile_rows, a.rows - rt * tile_rows);
-    uint32_t n = 0, i0 = 0, i1 = 0, slot0 = 0;
+    uint32_t i0 = 0, pieces = 0, slot0 = 0;
     if (tiles) {
-        n = used_shares(w_all, a.shares);
+        const uint32_t n = used_shares(w_all, a.shares);
         i0 = share_of(w_all, n, s0 + kStart);                   // the segment's first and last tile
-        i1 = share_of(w_all, n, s0 + kStart + tiles - 1);
-        if (i0 == i1) return;                                   // done by that share
+        pieces = share_of(w_all, n, s0 + kStart + tiles - 1) - i0 + 1;
+        if (pieces == 1) return;                                // done by that share
         slot0 = share_first(w_all, n, i0) >= s0 ? 0 : 1;        // later shares begin inside the segment: slot 0
     }
-    const uint32_t e = blockIdx.x % parts * kJoinThreads + threadIdx.x;
-    if (e < rows * (dim / 4)) {
-        const uint32_t r = e / (dim / 4), x = e % (dim / 4) * 4, col = rt * tile_rows + r;
-        float m = kNoScore, l = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (tiles) {
-            auto slot = [&](uint32_t i) { return ((static_cast<uint64_t>(rt) * a.shares + i) * 2 + (i == i0 ? slot0 : 0)) * tile_rows + r; };
-#pragma unroll 8
-            for (uint32_t i = i0; i <= i1; ++i) m = fmaxf(m, a.part_ml[slot(i) * 2]);
-#pragma unroll 8
-            for (uint32_t i = i0; i <= i1; ++i) {
-                const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot(i) * 2);
-                const float4 o = *reinterpret_cast<const float4*>(a.part_o + slot(i) * dim + x);
-                const float f = exp2_fast(ml.x - m);
-                l += ml.y * f;
-                acc.x += o.x * f, acc.y += o.y * f, acc.z += o.z * f, acc.w += o.w * f;
+    auto slot = [&](uint32_t i) { return ((static_cast<uint64_t>(rt) * a.shares + i0 + i) * 2 + (i == 0 ? slot0 : 0)) * tile_rows + r; };
+    float m = kNoScore, l = 0.f;
+    for (uint32_t i = lane; i < pieces; i += 32) m = fmaxf(m, a.part_ml[slot(i) * 2]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+    for (uint32_t i = lane; i < pieces; i += 32) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot(i) * 2);
+        l += ml.y * exp2_fast(ml.x - m);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(kFull, l, o);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (lane * 4 < dim) {
+        constexpr uint32_t kBatch = 4;                          // loads in flight
+        for (uint32_t i = warp; i < pieces; i += kJoinWarps * kBatch) {
+            float4 o[kBatch];
+            float f[kBatch];
+#pragma unroll
+            for (uint32_t u = 0; u < kBatch; ++u) {
+                const uint32_t x = i + u * kJoinWarps, at = x < pieces ? x : i;
+                f[u] = a.part_ml[slot(at) * 2];
+                o[u] = *reinterpret_cast<const float4*>(a.part_o + slot(at) * dim + lane * 4);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < kBatch; ++u) {
+                if (i + u * kJoinWarps >= pieces) break;
+                const float w = exp2_fast(f[u] - m);
+                acc.x += o[u].x * w, acc.y += o[u].y * w, acc.z += o[u].z * w, acc.w += o[u].w * w;
             }
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const uint64_t row = (static_cast<uint64_t>(b) * a.d.queries + col / a.group) * a.d.q_heads + h * a.group + col % a.group;
-        if (x == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-        if (a.d.dtype == BS_F16) {
-            __half2* p = reinterpret_cast<__half2*>(static_cast<__half*>(a.d.out) + row * dim + x);
-            p[0] = __floats2half2_rn(acc.x * inv, acc.y * inv);
-            p[1] = __floats2half2_rn(acc.z * inv, acc.w * inv);
-        } else {
-            __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.d.out) + row * dim + x);
-            p[0] = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
-            p[1] = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-        }
+    }
+    parts[warp][lane] = acc;
+    __syncthreads();
+    if (warp != 0 || lane * 4 >= dim) return;
+#pragma unroll
+    for (uint32_t x = 1; x < kJoinWarps; ++x) {
+        const float4 o = parts[x][lane];
+        acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const uint64_t row = (static_cast<uint64_t>(b) * a.d.queries + col / a.group) * a.d.q_heads + h * a.group + col % a.group;
+    if (lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    const uint64_t at = row * dim + lane * 4;
+    if (a.d.dtype == BS_F16) {
+        __half2* p = reinterpret_cast<__half2*>(static_cast<__half*>(a.d.out) + at);
+        p[0] = __floats2half2_rn(acc.x * inv, acc.y * inv);
+        p[1] = __floats2half2_rn(acc.z * inv, acc.w * inv);
+    } else {
+        __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.d.out) + at);
+        p[0] = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
+        p[1] = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
     }
 }
 
@@ -693,8 +719,9 @@ constexpr int kMassThreads = 128;
 __global__ void __launch_bounds__(kMassThreads) k_cache_mass(const __grid_constant__ CacheArgs a) {
     const uint32_t j = (blockIdx.x * kMassThreads + threadIdx.x) * 4, h = blockIdx.y, b = blockIdx.z;
     const uint32_t width = a.d.mass_width;
-    if (j >= width) return;
     const uint32_t len = held_tokens(a, b);
+    cudaGridDependencySynchronize();       // in every block, as above
+    if (j >= width) return;
     const uint64_t seg = static_cast<uint64_t>(b) * a.c.kv_heads + h, at = seg * width + j;
     const uint32_t n = j < len ? min(len - j, 4u) : 0;
     // four at once where their place is a multiple of 16 bytes
@@ -753,6 +780,22 @@ Layout plan(const bs_token_cache& c, const bs_cache_attention_desc& d, const Mem
     return l;
 }
 
+// A kernel that may start while the one before it on the stream still runs
+// (and waits for it by itself).
+template <typename... Params, typename... Given>
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, Given... given) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.stream = stream;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, Params(given)...);
+}
+
 template <int NW, int NT>
 cudaError_t launch_split(const CacheArgs& a, uint32_t row_tiles, cudaStream_t stream) {
     const cudaError_t e = cudaFuncSetAttribute(k_cache_split<NW, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitSmem<NW, NT>);
@@ -798,12 +841,12 @@ cudaError_t launch_cache_attention(const bs_token_cache& c, const bs_cache_atten
     cudaError_t e = cudaSuccess;
     if (l.shares) e = l.nt == 1 ? launch_split<1>(a, l.row_tiles, stream) : launch_split<2>(a, l.row_tiles, stream);
     if (e != cudaSuccess) return e;
-    const uint32_t tile_rows = a.rows < 8 * l.nt ? a.rows : 8 * l.nt;
-    const uint32_t parts = (tile_rows * (c.dim / 4) + kJoinThreads - 1) / kJoinThreads;
-    k_cache_join<<<dim3(c.kv_heads * parts, l.row_tiles, d.num_seqs), kJoinThreads, 0, stream>>>(a, 8 * l.nt, parts);
-    if (d.out_mass)
-        k_cache_mass<<<dim3((d.mass_width + 4 * kMassThreads - 1) / (4 * kMassThreads), c.kv_heads, d.num_seqs), kMassThreads, 0, stream>>>(a);
-    return cudaGetLastError();
+    const uint32_t tile_rows = 8 * l.nt, used_rows = a.rows < tile_rows ? a.rows : tile_rows;
+    e = launch_after(k_cache_join, dim3(c.kv_heads * used_rows, l.row_tiles, d.num_seqs), kJoinThreads, stream, a, tile_rows, used_rows);
+    if (e == cudaSuccess && d.out_mass)
+        e = launch_after(k_cache_mass, dim3((d.mass_width + 4 * kMassThreads - 1) / (4 * kMassThreads), c.kv_heads, d.num_seqs),
+                         kMassThreads, stream, a);
+    return e;
 }
 
 }  // namespace bsb
