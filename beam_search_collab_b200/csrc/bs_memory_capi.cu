@@ -139,7 +139,8 @@ BS_API bs_status bs_prompt_attention(const bs_prompt_attention_desc* d, void* st
     if (bs_status s = check_dtype16(d->dtype)) return s;
     if (bs_status s = check_dim(d->dim)) return s;
     if (bs_status s = check_heads(d->q_heads, d->kv_heads)) return s;
-    if (std::isnan(d->scale)) return report_error(BS_ERR_INVALID_ARGUMENT, "scale is NaN");
+    if (!(d->scale > 0.f) || std::isinf(d->scale))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "scale must be positive and finite (not 0, negative, infinite or NaN)");
     if (d->total_q >= (1u << 30) || d->total_k >= (1u << 30) || d->num_seqs > 65535)
         return report_error(BS_ERR_UNSUPPORTED, "at most 65535 sequences of fewer than 2^30 tokens in all are supported");
     if (d->total_q == 0 || d->num_seqs == 0) return BS_OK;
@@ -148,6 +149,10 @@ BS_API bs_status bs_prompt_attention(const bs_prompt_attention_desc* d, void* st
     if (!aligned16({d->q, d->k, d->v, d->out}) || !strides_ok(d->q_stride, 2) || !strides_ok(d->k_stride, 2) ||
         !strides_ok(d->v_stride, 2))
         return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign);
+    // one head or token for many (a stride of 0) has no tensor map
+    if ((d->total_q > 1 && d->q_stride[0] == 0) || (d->q_heads > 1 && d->q_stride[1] == 0) ||
+        (d->total_k > 1 && (d->k_stride[0] == 0 || d->v_stride[0] == 0)) || (d->kv_heads > 1 && (d->k_stride[1] == 0 || d->v_stride[1] == 0)))
+        return report_error(BS_ERR_UNSUPPORTED, "a stride of 0 (a broadcast tensor) is not supported: make it contiguous");
     MemoryDevice dev;
     if (bs_status s = memory_device(dev)) return s;
     if (!on_device(dev.device, {d->q, d->k, d->v, d->out, d->lse, d->cu_q, d->cu_k}))
@@ -203,7 +208,8 @@ static bs_status check_attention(const bs_token_cache* c, const bs_cache_attenti
     if (bs_status s = check_heads(d->q_heads, c->kv_heads)) return s;
     if (bs_status s = check_table(c, d->num_seqs, d->table_width)) return s;
     if (d->queries <= 0 || d->queries > 1024) return report_error(BS_ERR_INVALID_ARGUMENT, "queries must be in 1..1024");
-    if (std::isnan(d->scale)) return report_error(BS_ERR_INVALID_ARGUMENT, "scale is NaN");
+    if (!(d->scale > 0.f) || std::isinf(d->scale))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "scale must be positive and finite (not 0, negative, infinite or NaN)");
     if (d->out_mass && d->mass_width >= (1u << 30)) return report_error(BS_ERR_UNSUPPORTED, "mass_width must be below 2^30");
     return BS_OK;
 }
