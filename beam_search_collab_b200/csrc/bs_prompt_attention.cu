@@ -100,6 +100,11 @@ __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uin
                  "r"(a), "l"(b), "r"(what), "r"(static_cast<unsigned>(add))
                  : "memory");
 }
+__device__ __forceinline__ bool elected() {
+    unsigned yes;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(yes));
+    return yes != 0;
+}
 // The barrier completes when every matrix instruction issued so far has.
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_addr(bar)) : "memory");
@@ -107,19 +112,36 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
-__device__ __forceinline__ void wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+// (The registers are named so that nothing computed from them moves ahead.)
+__device__ __forceinline__ void wait_loads32(float* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]),
+                   "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]),
+                   "+f"(r[14]), "+f"(r[15]), "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]),
+                   "+f"(r[21]), "+f"(r[22]), "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]),
+                   "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void wait_loads16(float* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]),
+                   "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]),
+                   "+f"(r[14]), "+f"(r[15])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 
 // 32, 16 or 1 columns of the warp's 32 TMEM lanes: a register each.
 __device__ __forceinline__ void tmem_load32(uint32_t at, float* r) {
-    uint32_t* u = reinterpret_cast<uint32_t*>(r);
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
-        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
-          "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]),
-          "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]),
-          "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]),
+          "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]),
+          "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]),
+          "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
         : "r"(at)
         : "memory");
 }
@@ -133,25 +155,23 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* u) {
         : "memory");
 }
 __device__ __forceinline__ void tmem_load16(uint32_t at, float* r) {
-    uint32_t* u = reinterpret_cast<uint32_t*>(r);
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
-        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
-          "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]),
+          "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
         : "r"(at)
         : "memory");
 }
 __device__ __forceinline__ void tmem_store16(uint32_t at, const float* r) {
-    const uint32_t* u = reinterpret_cast<const uint32_t*>(r);
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};\n" ::"r"(u[0]),
-        "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]),
-        "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(at)
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};\n" ::"f"(r[0]),
+        "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]), "f"(r[10]), "f"(r[11]),
+        "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15]), "r"(at)
         : "memory");
 }
 __device__ __forceinline__ uint32_t tmem_load1(uint32_t at) {
     uint32_t u;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n" : "=r"(u) : "r"(at) : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\ntcgen05.wait::ld.sync.aligned;\n" : "=r"(u) : "r"(at) : "memory");
     return u;
 }
 
@@ -162,16 +182,24 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     float2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;\n"
-        : "=l"(reinterpret_cast<uint64_t&>(r))
-        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)), "l"(reinterpret_cast<const uint64_t&>(c)));
+    asm("{\n .reg .b64 a, b, c, r;\n mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7}; fma.rn.f32x2 r, a, b, c; mov.b64 {%0, %1}, r;\n}\n"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return r;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 r;
-    asm("add.rn.f32x2 %0, %1, %2;\n"
-        : "=l"(reinterpret_cast<uint64_t&>(r))
-        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+    asm("{\n .reg .b64 a, b, r;\n mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; add.rn.f32x2 r, a, b; mov.b64 {%0, %1}, r;\n}\n"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n .reg .b64 a, b, r;\n mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mul.rn.f32x2 r, a, b; mov.b64 {%0, %1}, r;\n}\n"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
 }
 
@@ -199,6 +227,69 @@ struct Type16<__nv_bfloat16> {
 // Stages of keys or values that fit beside the query tiles.
 template <int BOXES>
 constexpr int kStagesOf = BOXES == 2 ? 5 : 8;
+
+// 2^x for two x on the FMA pipe (the special-function pipe gives 16 results a
+// clock and SM, half of what the matrix pipe can take): n = round(x),
+// 2^(x - n) by the polynomial of degree 4 with the least largest relative
+// error on [-1/2, 1/2] (Remez exchange: 2.6e-6, mean 4e-8), times 2^n.
+// Below -126 it stays at 2^-126, so hidden keys do not come here; NaN stays.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    const float2 magic = make_float2(12582912.f, 12582912.f);      // 1.5 * 2^23: the sum's low bits are n
+    asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(x.x) : "f"(-126.f));
+    asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(x.y) : "f"(-126.f));
+    const float2 t = add2(x, magic);
+    const float2 n = add2(t, make_float2(-12582912.f, -12582912.f));
+    const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+    float2 r = make_float2(0.009570102207362652f, 0.009570102207362652f);
+    r = fma2(r, f, make_float2(0.05591785907745361f, 0.05591785907745361f));
+    r = fma2(r, f, make_float2(0.240247443318367f, 0.240247443318367f));
+    r = fma2(r, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+    r = fma2(r, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+    const float2 scale = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
+                                     __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000));
+    return mul2(r, scale);
+}
+
+// One row of a tile: weights 2^(scale * s + base), packed in p, their sum in
+// `part`; returns the row's largest score.  Scores come from TMEM 32 at a
+// time, the next 32 on their way meanwhile.
+constexpr int kPolyEvery = 4;       // of so many pairs, one by the polynomial
+template <typename T, bool HIDES>
+__device__ __forceinline__ float weights(uint32_t s_at, int32_t left, float scale, float base, uint32_t (&p)[kRows / 2], float& part) {
+    const float2 scale2 = make_float2(scale, scale), base2 = make_float2(base, base);
+    float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    float s[2][32];
+    tmem_load32(s_at, s[0]);
+#pragma unroll
+    for (int c = 0; c < kRows / 32; ++c) {
+        float* now = s[c & 1];
+        wait_loads32(now);
+        if (c + 1 < kRows / 32) tmem_load32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float2 x = make_float2(now[2 * i], now[2 * i + 1]);
+            if (HIDES) {
+                x.x = 32 * c + 2 * i < left ? x.x : -INFINITY;
+                x.y = 32 * c + 2 * i + 1 < left ? x.y : -INFINITY;
+            }
+            m[2 * (i & 1)] = fmaxf(m[2 * (i & 1)], x.x);
+            m[2 * (i & 1) + 1] = fmaxf(m[2 * (i & 1) + 1], x.y);
+            x = fma2(x, scale2, base2);
+            if (!HIDES && i % kPolyEvery == kPolyEvery - 1) {
+                x = exp2_poly(x);
+            } else {
+                x.x = exp2_fast(x.x);
+                x.y = exp2_fast(x.y);
+            }
+            add[i & 1] = add2(add[i & 1], x);
+            p[16 * c + i] = Type16<T>::pack(x.x, x.y);
+        }
+    }
+    add[0] = add2(add[0], add[1]);
+    part = add[0].x + add[0].y;
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
 
 struct Control {
     uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done, raw;
@@ -378,24 +469,41 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
         __syncwarp();
     } else if (warp == 8) {
         // ---------------------------------------------------- matrix products
-        if (lane == 0 && n > 0) {
+        // (the whole warp runs the loop, one elected lane issues)
+        if (n > 0) {
             constexpr uint32_t kCommon = 1u << 4 | Type16<T>::kFormat << 7 | Type16<T>::kFormat << 10 | (kRows >> 4) << 24;
             const uint32_t what_s = kCommon | (kRows >> 3) << 17;
             const uint32_t what_o = kCommon | 1u << 16 | static_cast<uint32_t>(d.dim >> 3) << 17;
+            // what the lane does per instruction counts: operands are a base
+            // and constants (16-byte units)
             const int steps = d.dim / 16;
+            const uint64_t q_base = operand(smem_addr(smem), 16, 1024), k_base = operand(smem_addr(ring), 16, 1024);
+            const uint64_t v_base = operand(smem_addr(ring), kBoxBytes, 1024);
+            constexpr uint32_t kTileUnits = kTileBytes / 16, kBoxUnits = kBoxBytes / 16;
             auto scores = [&](int t, uint32_t stage) {
-                const unsigned q = smem_addr(smem + t * kTileBytes), k = smem_addr(ring + stage * kTileBytes);
-                for (int i = 0; i < steps; ++i) {
-                    const unsigned off = (i >> 2) * kBoxBytes + (i & 3) * 32;
-                    mma_shared(tmem + t * 128, operand(q + off, 16, 1024), operand(k + off, 16, 1024), what_s, i > 0);
+                const uint64_t q = q_base + t * kTileUnits, k = k_base + stage * kTileUnits;
+                if (elected()) {
+#pragma unroll
+                    for (int i = 0; i < 4 * BOXES; ++i) {
+                        const uint32_t off = (i >> 2) * kBoxUnits + (i & 3) * 2;
+                        if (i < steps) mma_shared(tmem + t * 128, q + off, k + off, what_s, i > 0);
+                    }
+                    mma_commit(&ctl.s_full[t]);
                 }
-                mma_commit(&ctl.s_full[t]);
+                __syncwarp();
             };
             auto values = [&](int t, uint32_t stage, bool add) {
-                const unsigned v = smem_addr(ring + stage * kTileBytes);
+                const uint64_t v = v_base + stage * kTileUnits;
+                if (elected()) {
 #pragma unroll
-                for (int i = 0; i < kRows / 16; ++i)
-                    mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + i * 8, operand(v + i * 2048, kBoxBytes, 1024), what_o, add || i > 0);
+                    for (int i = 0; i < kRows / 16; ++i)
+                        mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + i * 8, v + i * 128, what_o, add || i > 0);
+                }
+                __syncwarp();
+            };
+            auto commit = [&](uint64_t* bar) {
+                if (elected()) mma_commit(bar);
+                __syncwarp();
             };
             auto full = [&](int32_t i) { wait(&ctl.full[i % kStages], (i / kStages) & 1); };
             full(0);
@@ -405,8 +513,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                 fence_after();
                 scores(t, 0);
             }
-            mma_commit(&ctl.empty[0]);
-            for (int32_t j = 0; j < n && !*gave_up; ++j) {
+            commit(&ctl.empty[0]);
+            for (int32_t j = 0; j < n; ++j) {
+                if (__any_sync(kFull, *gave_up != 0)) break;
                 const int32_t v_load = 2 * j + 1, k_load = 2 * j + 2;
                 full(v_load);
                 if (j + 1 < n) full(k_load);
@@ -416,14 +525,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                     wait(&ctl.p_full[t], j & 1);
                     fence_after();
                     values(t, v_load % kStages, j > 0 || ctl.keep[t]);
-                    if (j + 1 == tiles[t]) mma_commit(&ctl.o_full[t]);
+                    if (j + 1 == tiles[t]) commit(&ctl.o_full[t]);
                     else scores(t, k_load % kStages);
                 }
-                mma_commit(&ctl.empty[v_load % kStages]);
-                if (j + 1 < n) mma_commit(&ctl.empty[k_load % kStages]);
+                commit(&ctl.empty[v_load % kStages]);
+                if (j + 1 < n) commit(&ctl.empty[k_load % kStages]);
             }
             // TMEM and the stages are in use until this
-            mma_commit(&ctl.done);
+            commit(&ctl.done);
             for (unsigned i = 0; i < kPolls && !barrier_test(&ctl.done, 0); ++i) {}
         }
         __syncwarp();
@@ -439,57 +548,46 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
         const float scale = d.scale * 1.4426950408889634f;
         float top = -INFINITY, sum = 0.f;       // top: of the unscaled scores
         for (int32_t j = 0; j < mine && !*gave_up; ++j) {
-            float s[kRows];
             wait(&ctl.s_full[t], j & 1);        // and the value product before it is done
             fence_after();
-#pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_load32(s_at + 32 * i, s + 32 * i);
-            wait_loads();
             const bool hides = (j + 1) * kRows > all_see;
-            if (hides) {
-                const int32_t left = limit - j * kRows;
+            const int32_t left = limit - j * kRows;         // keys of this tile that the row sees
+            if (j == 0) {
+                float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < kRows; ++i) s[i] = i < left ? s[i] : -INFINITY;
+                for (int c = 0; c < kRows / 32; ++c) {
+                    float s[32];
+                    tmem_load32(s_at + 32 * c, s);
+                    wait_loads32(s);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) m[i & 3] = fmaxf(m[i & 3], 32 * c + i < left ? s[i] : -INFINITY);
+                }
+                top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
             }
-            float m[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-            for (int i = 4; i < kRows; i += 4)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) m[x] = fmaxf(m[x], s[i + x]);
-            const float high = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-            // (-infinity - -infinity is no number, and no reason to move)
-            if (__any_sync(kFull, (high - top) * scale > kSlack)) {
+            uint32_t p[kRows / 2];
+            float part;
+            for (bool again = false;; again = true) {
+                const float base = top == -INFINITY ? 0.f : -top * scale;
+                const float high = hides ? weights<T, true>(s_at, left, scale, base, p, part) : weights<T, false>(s_at, left, scale, base, p, part);
+                // (-infinity - -infinity is no number, and no reason to move)
+                if (again || !__any_sync(kFull, (high - top) * scale > kSlack)) break;
+                // rare: the maximum moves, what was summed is rescaled
                 const float next = fmaxf(top, high);
-                if (j > 0) {
-                    const float shrink = next == -INFINITY ? 1.f : exp2_fast((top - next) * scale);
-                    sum *= shrink;
-                    for (int x = 0; x < d.dim; x += 16) {
-                        float o[16];
-                        tmem_load16(o_at + x, o);
-                        wait_loads();
+                const float shrink = next == -INFINITY ? 1.f : exp2_fast((top - next) * scale);
+                sum *= shrink;
+                for (int x = 0; x < d.dim; x += 16) {
+                    float o[16];
+                    tmem_load16(o_at + x, o);
+                    wait_loads16(o);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] *= shrink;
-                        tmem_store16(o_at + x, o);
-                    }
+                    for (int i = 0; i < 16; ++i) o[i] *= shrink;
+                    tmem_store16(o_at + x, o);
                 }
                 top = next;
             }
-            const float base = top == -INFINITY ? 0.f : -top * scale;
-            const float2 scale2 = make_float2(scale, scale), base2 = make_float2(base, base);
-            float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-            uint32_t p[kRows / 2];
-#pragma unroll
-            for (int i = 0; i < kRows / 2; ++i) {
-                float2 x = fma2(make_float2(s[2 * i], s[2 * i + 1]), scale2, base2);
-                x.x = exp2_fast(x.x);
-                x.y = exp2_fast(x.y);
-                add[i & 1] = add2(add[i & 1], x);
-                p[i] = Type16<T>::pack(x.x, x.y);
-            }
+            sum += part;
             tmem_store32(s_at, p);
             tmem_store32(s_at + 32, p + 32);
-            add[0] = add2(add[0], add[1]);
-            sum += add[0].x + add[0].y;
             wait_stores();
             if (hides) {
                 // value rows that were cleared because they are not finite,
@@ -507,14 +605,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                     for (uint32_t left = odd[w]; left; left &= left - 1) {
                         const int r = 32 * w + __ffs(left) - 1;
                         const uint32_t two = tmem_load1(s_at + r / 2);
-                        wait_loads();
                         const float2 f = Type16<T>::unpack(two);
                         const float weight = r & 1 ? f.y : f.x;
                         const T* v = static_cast<const T*>(d.v) + (k0 + j * kRows + r) * d.v_stride[0] + kv_head * d.v_stride[1];
                         for (int x = 0; x < d.dim; x += 16) {
                             float o[16];
                             tmem_load16(o_at + x, o);
-                            wait_loads();
+                            wait_loads16(o);
                             if (j * kRows + r < limit)
                                 for (int i = 0; i < 16; ++i) o[i] += weight * static_cast<float>(v[x + i]);
                             __syncwarp();
@@ -539,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
             float o[16];
             if (mine > 0) {
                 tmem_load16(o_at + x, o);
-                wait_loads();
+                wait_loads16(o);
             }
             uint32_t u[8];
 #pragma unroll
