@@ -43,7 +43,7 @@ constexpr int kRows = 128;             // query rows of a tile, keys of a tile
 constexpr int kThreads = 320;
 constexpr int kBoxBytes = kRows * 128; // 128 rows of 64 elements
 constexpr unsigned kPolls = 1u << 22;
-constexpr float kSlack = 8.f;
+constexpr float kMost = 256.f;         // weights may grow to this before the maximum is moved
 
 struct PromptArgs {
     bs_prompt_attention_desc d;
@@ -195,14 +195,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return r;
 }
 
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("{\n .reg .b64 a, b, r;\n mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mul.rn.f32x2 r, a, b; mov.b64 {%0, %1}, r;\n}\n"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-
 template <typename T>
 struct Type16;
 template <>
@@ -213,6 +205,10 @@ struct Type16<__half> {
         return *reinterpret_cast<const uint32_t*>(&h);
     }
     static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+    static __device__ __forceinline__ uint32_t larger(uint32_t x, uint32_t y) {
+        const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
 };
 template <>
 struct Type16<__nv_bfloat16> {
@@ -222,43 +218,38 @@ struct Type16<__nv_bfloat16> {
         return *reinterpret_cast<const uint32_t*>(&h);
     }
     static __device__ __forceinline__ float2 unpack(uint32_t u) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u)); }
+    static __device__ __forceinline__ uint32_t larger(uint32_t x, uint32_t y) {
+        const __nv_bfloat162 h = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
 };
 
 // Stages of keys or values that fit beside the query tiles.
 template <int BOXES>
 constexpr int kStagesOf = BOXES == 2 ? 5 : 8;
 
-// 2^x for two x on the FMA pipe (the special-function pipe gives 16 results a
-// clock and SM, half of what the matrix pipe can take): n = round(x),
-// 2^(x - n) by the polynomial of degree 4 with the least largest relative
-// error on [-1/2, 1/2] (Remez exchange: 2.6e-6, mean 4e-8), times 2^n.
-// Below -126 it stays at 2^-126, so hidden keys do not come here; NaN stays.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-    const float2 magic = make_float2(12582912.f, 12582912.f);      // 1.5 * 2^23: the sum's low bits are n
-    asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(x.x) : "f"(-126.f));
-    asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(x.y) : "f"(-126.f));
-    const float2 t = add2(x, magic);
-    const float2 n = add2(t, make_float2(-12582912.f, -12582912.f));
-    const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
-    float2 r = make_float2(0.009570102207362652f, 0.009570102207362652f);
-    r = fma2(r, f, make_float2(0.05591785907745361f, 0.05591785907745361f));
-    r = fma2(r, f, make_float2(0.240247443318367f, 0.240247443318367f));
-    r = fma2(r, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
-    r = fma2(r, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-    const float2 scale = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
-                                     __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000));
-    return mul2(r, scale);
+// The row's largest score among the `left` first of a tile.
+__device__ __forceinline__ float largest(uint32_t s_at, int32_t left) {
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int c = 0; c < kRows / 32; ++c) {
+        float s[32];
+        tmem_load32(s_at + 32 * c, s);
+        wait_loads32(s);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) m[i & 3] = fmaxf(m[i & 3], 32 * c + i < left ? s[i] : -INFINITY);
+    }
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
 // One row of a tile: weights 2^(scale * s + base), packed in p, their sum in
-// `part`; returns the row's largest score.  Scores come from TMEM 32 at a
-// time, the next 32 on their way meanwhile.
-constexpr int kPolyEvery = 4;       // of so many pairs, one by the polynomial
+// `part`; returns the largest weight.  Scores come from TMEM 32 at a time, the
+// next 32 on their way meanwhile.
 template <typename T, bool HIDES>
 __device__ __forceinline__ float weights(uint32_t s_at, int32_t left, float scale, float base, uint32_t (&p)[kRows / 2], float& part) {
     const float2 scale2 = make_float2(scale, scale), base2 = make_float2(base, base);
     float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    uint32_t high[2] = {0, 0};
     float s[2][32];
     tmem_load32(s_at, s[0]);
 #pragma unroll
@@ -273,22 +264,18 @@ __device__ __forceinline__ float weights(uint32_t s_at, int32_t left, float scal
                 x.x = 32 * c + 2 * i < left ? x.x : -INFINITY;
                 x.y = 32 * c + 2 * i + 1 < left ? x.y : -INFINITY;
             }
-            m[2 * (i & 1)] = fmaxf(m[2 * (i & 1)], x.x);
-            m[2 * (i & 1) + 1] = fmaxf(m[2 * (i & 1) + 1], x.y);
             x = fma2(x, scale2, base2);
-            if (!HIDES && i % kPolyEvery == kPolyEvery - 1) {
-                x = exp2_poly(x);
-            } else {
-                x.x = exp2_fast(x.x);
-                x.y = exp2_fast(x.y);
-            }
+            x.x = exp2_fast(x.x);
+            x.y = exp2_fast(x.y);
             add[i & 1] = add2(add[i & 1], x);
             p[16 * c + i] = Type16<T>::pack(x.x, x.y);
+            high[i & 1] = Type16<T>::larger(high[i & 1], p[16 * c + i]);
         }
     }
     add[0] = add2(add[0], add[1]);
     part = add[0].x + add[0].y;
-    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    const float2 h = Type16<T>::unpack(Type16<T>::larger(high[0], high[1]));
+    return fmaxf(h.x, h.y);
 }
 
 struct Control {
@@ -552,27 +539,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
             fence_after();
             const bool hides = (j + 1) * kRows > all_see;
             const int32_t left = limit - j * kRows;         // keys of this tile that the row sees
-            if (j == 0) {
-                float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < kRows / 32; ++c) {
-                    float s[32];
-                    tmem_load32(s_at + 32 * c, s);
-                    wait_loads32(s);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) m[i & 3] = fmaxf(m[i & 3], 32 * c + i < left ? s[i] : -INFINITY);
-                }
-                top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-            }
+            if (j == 0) top = largest(s_at, left);
             uint32_t p[kRows / 2];
             float part;
             for (bool again = false;; again = true) {
                 const float base = top == -INFINITY ? 0.f : -top * scale;
                 const float high = hides ? weights<T, true>(s_at, left, scale, base, p, part) : weights<T, false>(s_at, left, scale, base, p, part);
-                // (-infinity - -infinity is no number, and no reason to move)
-                if (again || !__any_sync(kFull, (high - top) * scale > kSlack)) break;
+                if (again || !__any_sync(kFull, real && high > kMost)) break;     // (other rows hold anything)
                 // rare: the maximum moves, what was summed is rescaled
-                const float next = fmaxf(top, high);
+                const float next = fmaxf(top, largest(s_at, left));
                 const float shrink = next == -INFINITY ? 1.f : exp2_fast((top - next) * scale);
                 sum *= shrink;
                 for (int x = 0; x < d.dim; x += 16) {
