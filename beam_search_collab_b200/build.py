@@ -1,6 +1,7 @@
 """Builds the native parts in-tree (no JIT cache): the sm_100a shared library
 ``lib/libbsearch_b200.so`` (C ABI of include/bsearch.h) and the drop-in CLIs
-``bin/gpu_cli``, ``bin/build_rabitq`` and ``bin/build_graph``.
+``bin/gpu_cli``, ``bin/build_rabitq`` and ``bin/build_graph``, and the PyTorch
+binding of the token-memory operators ``_memory.so``.
 
     python -m beam_search_collab_b200.build [--force]
 
@@ -28,6 +29,7 @@ LIB = os.path.join(LIB_DIR, "libbsearch_b200.so")
 CLI = os.path.join(BIN_DIR, "gpu_cli")
 RQ_CLI = os.path.join(BIN_DIR, "build_rabitq")
 BG_CLI = os.path.join(BIN_DIR, "build_graph")
+MEMORY_PY = os.path.join(PKG, "_memory.so")
 
 CU_SOURCES = ["bs_search.cu", "bs_search_nb.cu", "bs_search_bq.cu", "bs_rabitq.cu", "bs_rabitq_nb.cu", "bs_graph_build.cu", "bs_ground_truth.cu", "bs_load.cu", "bs_entry.cu", "bs_merge.cu", "bs_codebook.cu",
               "bs_prompt_attention.cu", "bs_cache_attention.cu", "bs_token_cache.cu", "bs_memory_capi.cu",
@@ -108,7 +110,27 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if force or _stale(RQ_CLI, [rq_src, LIB, os.path.join(INCLUDE, "bsearch.h")]):
         _run([_cxx(), "-std=c++20", "-O2", "-Wall", "-I", INCLUDE, rq_src, "-o", RQ_CLI,
               "-L", LIB_DIR, "-lbsearch_b200", "-Wl,-rpath,$ORIGIN/../lib"])
+    mem_src = os.path.join(CSRC, "memory_py.cpp")
+    if force or _stale(MEMORY_PY, [mem_src, LIB, os.path.join(INCLUDE, "bsearch.h")]):
+        _run(_memory_py_command(mem_src))
     return LIB
+
+
+def _memory_py_command(src: str) -> list[str]:
+    """The token-memory operators' binding for PyTorch tensors (beam_search_collab_b200/_memory.so)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension as ext
+    cmd = [_cxx(), "-std=c++17", "-O2", "-shared", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_memory",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE,
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]
+    for p in ext.include_paths():
+        cmd += ["-isystem", p]
+    cmd += [src, "-o", MEMORY_PY, "-L", LIB_DIR, "-lbsearch_b200", "-Wl,-rpath,$ORIGIN/lib"]
+    for p in ext.library_paths():
+        cmd += ["-L", p]
+    return cmd + ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
 
 
 def main() -> None:

@@ -7,19 +7,20 @@ import pytest
 import torch
 
 import beam_search_collab_b200 as B
+import memory_abi as A
 import memory_ref as R
 from beam_search_collab_b200 import memory as M
 
 
 def cache(**kw):
-    c = M._Cache(64, 64, 64, 64, 4, 2, 32, 64)
+    c = A._Cache(64, 64, 64, 64, 4, 2, 32, 64)
     for k, v in kw.items():
         setattr(c, k, v)
     return c
 
 
 def status(name, *args):
-    rc = getattr(M._lib(), name)(*args)
+    rc = getattr(A._lib(), name)(*args)
     return rc, B.lib().bs_last_error().decode()
 
 
@@ -28,9 +29,9 @@ def test_null_descriptors():
     for name in ("bs_cache_write", "bs_cache_read", "bs_cache_attention", "bs_cache_evict"):
         assert status(name, c, None, None) == (1, "desc is NULL")
     assert status("bs_prompt_attention", None, None) == (1, "desc is NULL")
-    assert status("bs_cache_read", None, M._Read(), None) == (1, "cache is NULL")
+    assert status("bs_cache_read", None, A._Read(), None) == (1, "cache is NULL")
     assert status("bs_memory_take_errors", None, None)[0] == 1
-    assert status("bs_cache_evict_workspace", c, M._Evict(), None)[0] == 1
+    assert status("bs_cache_evict_workspace", c, A._Evict(), None)[0] == 1
 
 
 @pytest.mark.parametrize("field,value,code,text", [
@@ -40,7 +41,7 @@ def test_null_descriptors():
     ("out", None, 1, "NULL"), ("k", 72, 1, "16-byte aligned"), ("q_stride", (4, 64), 1, "multiples of 8"),
     ("v_stride", (-8, 64), 1, "non-negative")])
 def test_prompt_checks(field, value, code, text):
-    d = M._Prompt(64, 64, 64, 64, 64, (128, 64), (128, 64), (128, 64), 64, 64, 10, 10, 1, 2, 2, 64, 1, 1, 0.1)
+    d = A._Prompt(64, 64, 64, 64, 64, (128, 64), (128, 64), (128, 64), 64, 64, 10, 10, 1, 2, 2, 64, 1, 1, 0.1)
     setattr(d, field, (ctypes.c_int64 * 2)(*value) if isinstance(value, tuple) else value)
     rc, why = status("bs_prompt_attention", d, None)
     assert rc == code and text in why, (rc, why)
@@ -49,7 +50,7 @@ def test_prompt_checks(field, value, code, text):
 @pytest.mark.parametrize("field,value,code,text", [("block", 24, 1, "16, 32, 64 or 128"), ("dim", 40, 2, "multiple of 16"),
                                                    ("kv_heads", 0, 1, "kv_heads"), ("kv_heads", 70000, 1, "kv_heads")])
 def test_cache_checks(field, value, code, text):
-    d = M._Read(64, 64, 64, 0, 0, 64, 64, 1, 1, 1, 0)
+    d = A._Read(64, 64, 64, 0, 0, 64, 64, 1, 1, 1, 0)
     rc, why = status("bs_cache_read", cache(**{field: value}), d, None)
     assert rc == code and text in why, (rc, why)
 
@@ -59,7 +60,7 @@ def test_cache_checks(field, value, code, text):
     ("table_width", 1 << 26, 2, "2^30"), ("lens", None, 1, "NULL"), ("out_mass", None, 1, "mass without out_mass"),
     ("mass_width", 0, 1, "mass_width is 0"), ("scale", math.nan, 1, "NaN"), ("q", 65, 1, "aligned")])
 def test_attention_checks(field, value, code, text):
-    d = M._Attention(64, (256, 256, 64), 64, 64, 64, 64, 64, 64, None, 0, 1, 2, 64, 1, 4, 1, 0.1)
+    d = A._Attention(64, (256, 256, 64), 64, 64, 64, 64, 64, 64, None, 0, 1, 2, 64, 1, 4, 1, 0.1)
     setattr(d, field, value)
     rc, why = status("bs_cache_attention", cache(), d, None)
     assert rc == code and text in why, (rc, why)
@@ -69,26 +70,27 @@ def test_attention_checks(field, value, code, text):
     ("budget", 0, 1, "budget"), ("sinks", -1, 1, "sinks"), ("recent", 30, 1, "sinks + recent"), ("new_table_width", 0, 1, "room"),
     ("mass_width", 1 << 30, 2, "mass_width"), ("kept", None, 1, "NULL")])
 def test_evict_checks(field, value, code, text):
-    d = M._Evict(64, 64, 64, 64, 64, 64, 64, None, 0, 1, 4, 1, 128, 32, 4, 8)
+    d = A._Evict(64, 64, 64, 64, 64, 64, 64, None, 0, 1, 4, 1, 128, 32, 4, 8)
     setattr(d, field, value)
     rc, why = status("bs_cache_evict", cache(), d, None)
     assert rc == code and text in why, (rc, why)
 
 
 def test_nothing_to_do_is_done_without_a_gpu():
-    d = M._Prompt(None, None, None, None, None, (0, 0), (0, 0), (0, 0), None, None, 0, 0, 0, 2, 2, 64, 1, 1, 0.1)
+    d = A._Prompt(None, None, None, None, None, (0, 0), (0, 0), (0, 0), None, None, 0, 0, 0, 2, 2, 64, 1, 1, 0.1)
     assert status("bs_prompt_attention", d, None)[0] == 0
-    assert status("bs_cache_write", cache(), M._Write(dtype=1), None)[0] == 0
-    assert status("bs_cache_read", cache(), M._Read(dtype=1), None)[0] == 0
-    assert status("bs_cache_attention", cache(), M._Attention(queries=1, q_heads=2, dtype=1), None)[0] == 0
+    assert status("bs_cache_write", cache(), A._Write(dtype=1), None)[0] == 0
+    assert status("bs_cache_read", cache(), A._Read(dtype=1), None)[0] == 0
+    assert status("bs_cache_attention", cache(), A._Attention(queries=1, q_heads=2, dtype=1, scale=1.0), None)[0] == 0
 
 
 def test_host_tensors_are_refused():
     q = torch.zeros((4, 2, 64), dtype=torch.float16)
     with pytest.raises(ValueError, match="CUDA"):
         M.prompt_attention(q, q, q, torch.tensor([0, 4], dtype=torch.int32))
+    codes, scales = torch.zeros((2, 2, 16, 64), dtype=torch.int8), torch.zeros((2, 2))
     with pytest.raises(ValueError, match="CUDA"):
-        M.TokenCache(torch.zeros((2, 2, 16, 64), dtype=torch.int8), None, None, None)
+        M.TokenCache(codes, codes, scales, scales)
 
 
 def test_merge_is_the_attention_over_both_sets():
