@@ -1,5 +1,11 @@
 // bs_token_cache.cu -- writing to, reading from and evicting from the 8-bit
 // token cache (include/bsearch.h, bs_token_cache).
+//
+// All of them are bound by memory, provided the conversions stay off the
+// special-function pipe (16 int <-> float conversions a clock and SM: the
+// eviction's move took 60 us through it, as long as all its traffic), so
+// integers are made and read through a float's low bits.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -24,6 +30,33 @@ __device__ __forceinline__ float2 pair_to_float<__nv_bfloat16>(uint32_t u) {
 }
 
 __device__ __forceinline__ uint4 ldg_stream(const void* p) { return __ldcs(static_cast<const uint4*>(p)); }
+
+// Four codes of a word as floats: 0x4b000000 | u is 2^23 + u.
+__device__ __forceinline__ float4 codes_to_floats(uint32_t w) {
+    const uint32_t u = w ^ 0x80808080u;
+    constexpr float kBias = 8388608.f + 128.f;
+    return make_float4(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540)) - kBias,
+                       __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7541)) - kBias,
+                       __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7542)) - kBias,
+                       __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7543)) - kBias);
+}
+
+// rint of four values below 2^22 in magnitude, their low bytes as a word:
+// x + 1.5 * 2^23 rounds to the nearest integer, ties to even.
+__device__ __forceinline__ uint32_t floats_to_codes(float4 x) {
+    constexpr float kMagic = 12582912.f;
+    const uint32_t lo = __byte_perm(__float_as_uint(x.x + kMagic), __float_as_uint(x.y + kMagic), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(x.z + kMagic), __float_as_uint(x.w + kMagic), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
+}
+
+// Codes times a ratio of at most 1, rounded (the product first, to 32 bits).
+__device__ __forceinline__ uint32_t rescaled(uint32_t w, float ratio) {
+    const float4 f = codes_to_floats(w);
+    return floats_to_codes(make_float4(__fmul_rn(f.x, ratio), __fmul_rn(f.y, ratio), __fmul_rn(f.z, ratio), __fmul_rn(f.w, ratio)));
+}
+
+__device__ __forceinline__ float clamp127(float x) { return fmaxf(-127.f, fminf(127.f, x)); }
 
 // ------------------------------------------------------------------- write
 
@@ -116,11 +149,8 @@ __global__ void __launch_bounds__(kWriteThreads) k_cache_write(const WriteArgs a
         const float ratio = __fdiv_rn(old, scale);
         for (uint32_t chunk = threadIdx.x; chunk < held * per_row; chunk += kWriteThreads) {
             uint2* p = reinterpret_cast<uint2*>(codes) + chunk;
-            uint2 u = *p;
-            int8_t* c = reinterpret_cast<int8_t*>(&u);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) c[j] = static_cast<int8_t>(__float2int_rn(c[j] * ratio));
-            *p = u;
+            const uint2 u = *p;
+            *p = make_uint2(rescaled(u.x, ratio), rescaled(u.y, ratio));
         }
     }
 #pragma unroll
@@ -128,15 +158,14 @@ __global__ void __launch_bounds__(kWriteThreads) k_cache_write(const WriteArgs a
         const uint32_t chunk = held * per_row + i * kWriteThreads + threadIdx.x;
         if (chunk >= stop * per_row) continue;
         const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-        uint2 u;
-        int8_t* c = reinterpret_cast<int8_t*>(&u);
+        uint32_t code[2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 f = pair_to_float<T>(w[j]);
-            c[2 * j] = static_cast<int8_t>(max(-127, min(127, __float2int_rn(f.x * inv))));
-            c[2 * j + 1] = static_cast<int8_t>(max(-127, min(127, __float2int_rn(f.y * inv))));
+        for (int j = 0; j < 2; ++j) {
+            const float2 f = pair_to_float<T>(w[2 * j]), h = pair_to_float<T>(w[2 * j + 1]);
+            code[j] = floats_to_codes(make_float4(clamp127(__fmul_rn(f.x, inv)), clamp127(__fmul_rn(f.y, inv)),
+                                                  clamp127(__fmul_rn(h.x, inv)), clamp127(__fmul_rn(h.y, inv))));
         }
-        reinterpret_cast<uint2*>(codes)[chunk] = u;
+        reinterpret_cast<uint2*>(codes)[chunk] = make_uint2(code[0], code[1]);
     }
     if (threadIdx.x == 0) *scale_at = scale;
 }
@@ -163,11 +192,32 @@ struct ReadArgs {
 };
 
 template <typename T>
+__device__ __forceinline__ T rounded(float x);
+template <>
+__device__ __forceinline__ float rounded<float>(float x) {
+    return x;
+}
+template <>
+__device__ __forceinline__ __half rounded<__half>(float x) {
+    return __float2half_rn(x);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float x) {
+    return __float2bfloat16_rn(x);
+}
+
+template <typename T>
 __device__ __forceinline__ void store_values(void* out, uint64_t at, uint4 codes, float scale) {
-    const int8_t* c = reinterpret_cast<const int8_t*>(&codes);
+    const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
     __align__(16) T v[16];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = static_cast<T>(c[j] * scale);
+    for (int j = 0; j < 4; ++j) {
+        const float4 f = codes_to_floats(w[j]);
+        v[4 * j] = rounded<T>(f.x * scale);
+        v[4 * j + 1] = rounded<T>(f.y * scale);
+        v[4 * j + 2] = rounded<T>(f.z * scale);
+        v[4 * j + 3] = rounded<T>(f.w * scale);
+    }
     uint4* p = reinterpret_cast<uint4*>(static_cast<T*>(out) + at);
 #pragma unroll
     for (unsigned j = 0; j < sizeof(v) / 16; ++j) __stcs(p + j, reinterpret_cast<const uint4*>(v)[j]);
@@ -218,17 +268,54 @@ struct EvictArgs {
 // Order of weights as integers: larger weight, larger key; NaN above all.
 __device__ __forceinline__ uint32_t mass_key(float f) { return isnan(f) ? 0xffffffffu : f2ord(f); }
 
-constexpr int kSelectThreads = 1024;
+// Which tokens of one sequence stay for one head: a cluster of blocks holds
+// the row's keys in shared memory, a slice each (what does not fit is read
+// again from L2).  The m-th largest key among the free tokens is found by its
+// digits of 11, 11 and 10 bits, counted by every block and added up through
+// distributed shared memory; then each block numbers the tokens of its slice
+// that stay, in order, from what the blocks before it have.
+//   measured, 32 rows of 8,000 to 65,536 tokens: one block a row, 8-bit digits
+//   from L2 219 us.
+constexpr uint32_t kBins = 2048;
+constexpr uint32_t kMostCached = 46 * 1024;       // keys of a slice in shared memory
+constexpr int kMostCluster = 8;
 
-// One CTA: which tokens of one sequence stay for one head.  The m-th largest
-// key among the free tokens is found digit by digit (8 bits at a time, counted
-// in shared memory); then one ordered pass numbers the tokens that stay.
-__global__ void __launch_bounds__(kSelectThreads) k_evict_select(const EvictArgs a) {
-    __shared__ uint32_t count[256];
+// Exclusive prefix over the block of one number per thread, and the total.
+template <int THREADS>
+__device__ __forceinline__ uint32_t block_prefix(uint32_t x, uint32_t* warp_sums, uint32_t& total) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t sum = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(kFull, sum, o);
+        if (lane >= static_cast<uint32_t>(o)) sum += up;
+    }
+    __syncthreads();                 // the last use of warp_sums is over
+    if (lane == 31) warp_sums[warp] = sum;
+    __syncthreads();
+    const uint32_t mine = lane < THREADS / 32 ? warp_sums[lane] : 0;
+    uint32_t before = lane < warp ? mine : 0, all = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        before += __shfl_xor_sync(kFull, before, o);
+        all += __shfl_xor_sync(kFull, all, o);
+    }
+    total = all;
+    return before + sum - x;
+}
+
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) k_evict_select(const EvictArgs a, uint32_t cached) {
+    namespace cg = cooperative_groups;
+    extern __shared__ uint32_t keys[];             // [cached]
+    __shared__ uint32_t count[3][kBins];
+    __shared__ uint32_t warp_sums[32];
+    __shared__ uint32_t slice_counts[2];           // tokens that stay for certain, tokens equal to the threshold
     __shared__ uint32_t chosen[2];
-    __shared__ uint32_t warp_sum[2][32];
+    const cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t rank = cluster.block_rank(), blocks = cluster.num_blocks();
     const bs_cache_evict_desc& d = a.d;
-    const uint32_t h = blockIdx.x, b = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const uint32_t h = blockIdx.x / blocks, b = blockIdx.y, t = threadIdx.x, lane = t & 31;
     const uint64_t row = static_cast<uint64_t>(b) * a.c.kv_heads + h;
     const float* mass = d.mass + row * d.mass_width;
     int32_t* kept = d.kept + row * d.budget;
@@ -240,74 +327,135 @@ __global__ void __launch_bounds__(kSelectThreads) k_evict_select(const EvictArgs
         len = len < 0 ? 0 : static_cast<int32_t>(most);
     }
     const uint32_t n = len, budget = d.budget, stay = n < budget ? n : budget;
-    if (h == 0 && t == 0) d.new_lens[b] = stay;
-    for (uint32_t i = stay + t; i < budget; i += kSelectThreads) {
+    if (blockIdx.x == 0 && t == 0) d.new_lens[b] = stay;
+    for (uint32_t i = stay + rank * THREADS + t; i < budget; i += blocks * THREADS) {
         kept[i] = -1;
         new_mass[i] = 0.f;
     }
-    if (n <= budget) {
-        for (uint32_t i = t; i < n; i += kSelectThreads) {
+    if (n <= budget) {                             // (the whole cluster)
+        for (uint32_t i = rank * THREADS + t; i < n; i += blocks * THREADS) {
             kept[i] = i;
             new_mass[i] = mass[i];
         }
         return;
     }
-    const uint32_t lo = d.sinks, hi = n - d.recent;
-    uint32_t need = budget - d.sinks - d.recent;      // of the free tokens [lo, hi); fewer than there are
-    uint32_t prefix = 0;
-    for (int shift = 24; shift >= 0 && need; shift -= 8) {
-        for (uint32_t i = t; i < 256; i += kSelectThreads) count[i] = 0;
-        __syncthreads();
-        for (uint32_t i = lo + t; i < hi; i += kSelectThreads) {
-            const uint32_t key = mass_key(mass[i]);
-            if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&count[(key >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (t == 0) {
-            uint32_t left = need, digit = 255;
-            while (count[digit] < left) left -= count[digit--];
-            chosen[0] = prefix | (digit << shift);
-            chosen[1] = left;
-        }
-        __syncthreads();
-        prefix = chosen[0];
-        need = chosen[1];
+    // this block's slice of the row
+    const uint32_t width = ((n + blocks - 1) / blocks + 3) & ~3u;
+    const uint32_t first = min(rank * width, n), size = min(width, n - first);
+    const uint32_t lo = d.sinks, hi = n - d.recent;              // free tokens
+    auto key_of = [&](uint32_t i) { return i < cached ? keys[i] : mass_key(mass[first + i]); };
+    for (uint32_t i = t; i < 3 * kBins; i += THREADS) (&count[0][0])[i] = 0;
+    for (uint32_t i0 = t; i0 < min(size, cached); i0 += 8 * THREADS) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = i0 + u * THREADS < size ? mass[first + i0 + u * THREADS] : 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (i0 + u * THREADS < min(size, cached)) keys[i0 + u * THREADS] = mass_key(x[u]);
     }
-    // stays: forced, above the threshold, or one of the first `need` equal to it
-    const bool any = budget > static_cast<uint32_t>(d.sinks) + d.recent;
-    uint32_t base = 0, base_eq = 0;
-    for (uint32_t i0 = 0; i0 < n; i0 += kSelectThreads) {
-        const uint32_t i = i0 + t;
-        const float w = i < n ? mass[i] : 0.f;
-        const bool is_free = i >= lo && i < hi;
-        const uint32_t key = mass_key(w);
-        const bool eq = is_free && any && key == prefix;
-        const unsigned eq_mask = __ballot_sync(kFull, eq);
-        if (lane == 0) warp_sum[0][warp] = __popc(eq_mask);
-        __syncthreads();
-        uint32_t before = base_eq, total_eq = 0;
-        for (uint32_t k = 0; k < 32; ++k) {
-            before += k < warp ? warp_sum[0][k] : 0;
-            total_eq += warp_sum[0][k];
+    __syncthreads();
+
+    uint32_t need = budget - d.sinks - d.recent;   // of the free tokens; fewer than there are
+    const bool any = need > 0;
+    uint32_t prefix = 0;
+    if (any) {
+#pragma unroll 1
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, above = pass == 0 ? 32 : pass == 1 ? 21 : 10;
+            const uint32_t mask = pass == 2 ? 1023 : 2047;
+            for (uint32_t i0 = 0; i0 < size; i0 += THREADS) {    // (all lanes together)
+                const uint32_t i = i0 + t, at = first + i;
+                const bool in_slice = i < size && at >= lo && at < hi;
+                const uint32_t key = in_slice ? key_of(i) : 0;
+                const bool in = in_slice && (pass == 0 || (key >> above) == (prefix >> above));
+                const unsigned active = __ballot_sync(kFull, in);
+                if (!active) continue;
+                // the lanes that agree with the first one count at once: rows of equal weights do not queue up
+                const uint32_t digit = (key >> shift) & mask;
+                const int lead = __ffs(active) - 1;
+                const uint32_t lead_digit = __shfl_sync(kFull, digit, lead);
+                const unsigned same = __ballot_sync(kFull, in && digit == lead_digit);
+                if (static_cast<int>(lane) == lead) atomicAdd(&count[pass][digit], static_cast<uint32_t>(__popc(same)));
+                else if (in && !(same >> lane & 1)) atomicAdd(&count[pass][digit], 1u);
+            }
+            __syncwarp();
+            cluster.sync();
+            // bins from the largest digit down, kBins / THREADS to a thread
+            constexpr int kEach = kBins / THREADS;
+            uint32_t mine[kEach], sum = 0;
+#pragma unroll
+            for (int u = 0; u < kEach; ++u) {
+                mine[u] = 0;
+                for (uint32_t x = 0; x < blocks; ++x) mine[u] += cluster.map_shared_rank(&count[pass][0], x)[kBins - 1 - (t * kEach + u)];
+                sum += mine[u];
+            }
+            uint32_t total;
+            uint32_t before = block_prefix<THREADS>(sum, warp_sums, total);
+#pragma unroll
+            for (int u = 0; u < kEach; ++u) {
+                if (before < need && need <= before + mine[u]) {
+                    chosen[0] = prefix | (kBins - 1 - (t * kEach + u)) << shift;
+                    chosen[1] = need - before;
+                }
+                before += mine[u];
+            }
+            __syncthreads();
+            prefix = chosen[0];
+            need = chosen[1];
         }
-        before += __popc(eq_mask & ((1u << lane) - 1));
-        const bool in = i < n && (!is_free || (any && key > prefix) || (eq && before < need));
-        const unsigned in_mask = __ballot_sync(kFull, in);
-        if (lane == 0) warp_sum[1][warp] = __popc(in_mask);
-        __syncthreads();
-        uint32_t to = base, total = 0;
-        for (uint32_t k = 0; k < 32; ++k) {
-            to += k < warp ? warp_sum[1][k] : 0;
-            total += warp_sum[1][k];
+    }
+    // a token stays if it is not free, above the threshold, or one of the
+    // first `need` equal to it; both kinds are counted in one number
+    auto kind = [&](uint32_t i) -> uint32_t {      // 1: stays for certain, 65536: equal
+        const uint32_t at = first + i;
+        if (i >= size) return 0;
+        if (at < lo || at >= hi) return 1;
+        if (!any) return 0;
+        const uint32_t key = key_of(i);
+        return key > prefix ? 1 : key == prefix ? 65536u : 0;
+    };
+    uint32_t sure = 0, equal = 0;
+    for (uint32_t i = t; i < size; i += THREADS) {
+        const uint32_t k = kind(i);
+        sure += k & 1;
+        equal += k >> 16;
+    }
+    uint32_t total_sure, total_equal;
+    block_prefix<THREADS>(sure, warp_sums, total_sure);
+    block_prefix<THREADS>(equal, warp_sums, total_equal);
+    if (t == 0) {
+        slice_counts[0] = total_sure;
+        slice_counts[1] = total_equal;
+    }
+    cluster.sync();
+    uint32_t base = 0, base_equal = 0;
+    for (uint32_t x = 0; x < rank; ++x) {
+        base += cluster.map_shared_rank(&slice_counts[0], x)[0];
+        base_equal += cluster.map_shared_rank(&slice_counts[0], x)[1];
+    }
+    cluster.sync();                                // no block ends while another reads it
+    constexpr uint32_t kRun = 4;                   // tokens of a thread, side by side
+    for (uint32_t i0 = 0; i0 < size; i0 += kRun * THREADS) {
+        uint32_t k[kRun], sum = 0, total;
+#pragma unroll
+        for (uint32_t u = 0; u < kRun; ++u) {
+            k[u] = kind(i0 + t * kRun + u);
+            sum += k[u];                           // (at most 4096 of each kind in the block)
         }
-        to += __popc(in_mask & ((1u << lane) - 1));
-        if (in) {
-            kept[to] = i;
-            new_mass[to] = w;
+        const uint32_t before = block_prefix<THREADS>(sum, warp_sums, total);
+        uint32_t to = base + (before & 0xffffu), eq = base_equal + (before >> 16);
+#pragma unroll
+        for (uint32_t u = 0; u < kRun; ++u) {
+            const uint32_t i = first + i0 + t * kRun + u;
+            if (k[u] == 1 || (k[u] && eq < need)) {
+                kept[to + min(eq, need)] = i;
+                new_mass[to + min(eq, need)] = mass[i];
+            }
+            to += k[u] & 1;
+            eq += k[u] >> 16;
         }
-        base += total;
-        base_eq += total_eq;
-        __syncthreads();
+        base += total & 0xffffu;
+        base_equal += total >> 16;
     }
 }
 
@@ -361,23 +509,46 @@ __global__ void __launch_bounds__(kMoveThreads) k_evict_move(const EvictArgs a) 
         }
     }
     __syncthreads();
-    const uint32_t per_row = a.c.dim / 16;
-    for (uint32_t u = t; u < 2 * block * per_row; u += kMoveThreads) {
-        const uint32_t kv = u >= block * per_row, w = u - kv * block * per_row, i = w / per_row, chunk = w % per_row;
-        uint4 codes = make_uint4(0, 0, 0, 0);
-        if (from[i] >= 0) {
-            const int8_t* src = kv ? a.c.v : a.c.k;
-            codes = ldg_stream(src + from[i] * a.c.dim + chunk * 16);
-            const float ratio = top[kv] > 0.f ? __fdiv_rn(scale[kv][i], top[kv]) : 0.f;
-            if (ratio != 1.f) {
-                int8_t* c = reinterpret_cast<int8_t*>(&codes);
+    const uint32_t per_row = a.c.dim / 16, units = 2 * block * per_row;
+    constexpr int kBatch = 4;              // loads of a thread in flight
+    for (uint32_t u0 = t; u0 < units; u0 += kBatch * kMoveThreads) {
+        uint4 codes[kBatch];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) c[j] = static_cast<int8_t>(__float2int_rn(c[j] * ratio));
-            }
+        for (int x = 0; x < kBatch; ++x) {
+            const uint32_t u = u0 + x * kMoveThreads, kv = u >= block * per_row, w = u - kv * block * per_row, i = w / per_row;
+            codes[x] = make_uint4(0, 0, 0, 0);
+            if (u < units && from[i] >= 0) codes[x] = ldg_stream((kv ? a.c.v : a.c.k) + from[i] * a.c.dim + w % per_row * 16);
         }
-        int8_t* dst = (kv ? a.c.v : a.c.k) + (slab * block + i) * a.c.dim + chunk * 16;
-        *reinterpret_cast<uint4*>(dst) = codes;
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x) {
+            const uint32_t u = u0 + x * kMoveThreads, kv = u >= block * per_row, w = u - kv * block * per_row, i = w / per_row;
+            if (u >= units) break;
+            const float ratio = top[kv] > 0.f ? __fdiv_rn(scale[kv][i], top[kv]) : 0.f;
+            if (ratio != 1.f)
+                codes[x] = make_uint4(rescaled(codes[x].x, ratio), rescaled(codes[x].y, ratio), rescaled(codes[x].z, ratio),
+                                      rescaled(codes[x].w, ratio));
+            *reinterpret_cast<uint4*>((kv ? a.c.v : a.c.k) + slab * block * a.c.dim + w * 16) = codes[x];
+        }
     }
+}
+
+template <int THREADS>
+cudaError_t launch_select(const EvictArgs& a, uint32_t cluster, cudaStream_t stream) {
+    const uint32_t slice = ((a.d.mass_width + cluster - 1) / cluster + 3) & ~3u, cached = slice < kMostCached ? slice : kMostCached;
+    cudaError_t e = cudaFuncSetAttribute(k_evict_select<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostCached * 4);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(a.c.kv_heads * cluster, a.d.num_seqs);
+    config.blockDim = dim3(THREADS);
+    config.dynamicSmemBytes = cached * 4;
+    config.stream = stream;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, k_evict_select<THREADS>, a, cached);
 }
 
 }  // namespace
@@ -404,8 +575,13 @@ size_t cache_evict_scratch(const bs_token_cache&, const bs_cache_evict_desc&, co
 cudaError_t launch_cache_evict(const bs_token_cache& c, const bs_cache_evict_desc& d, const MemoryDevice& dev,
                                cudaStream_t stream) {
     const EvictArgs a{c, d, dev.errors};
-    k_evict_select<<<dim3(c.kv_heads, d.num_seqs), kSelectThreads, 0, stream>>>(a);
-    cudaError_t e = cudaGetLastError();
+    // a row goes to more blocks while they would have over 4,096 tokens each
+    // and the rows alone do not fill the GPU
+    uint32_t cluster = 1;
+    while (cluster < kMostCluster && d.mass_width / cluster > 4096 &&
+           static_cast<uint64_t>(c.kv_heads) * d.num_seqs * cluster < static_cast<uint64_t>(dev.num_sms))
+        cluster *= 2;
+    const cudaError_t e = d.mass_width <= 4096 ? launch_select<256>(a, cluster, stream) : launch_select<1024>(a, cluster, stream);
     if (e != cudaSuccess) return e;
     const uint32_t cols = (d.budget + c.block - 1) / c.block;
     const uint32_t used = cols < d.new_table_width ? cols : d.new_table_width;
