@@ -278,7 +278,7 @@ __device__ __forceinline__ uint32_t mass_key(float f) { return isnan(f) ? 0xffff
 //   from L2 219 us.
 constexpr uint32_t kBins = 2048;
 constexpr uint32_t kMostCached = 46 * 1024;       // keys of a slice in shared memory
-constexpr int kMostCluster = 8;
+constexpr uint32_t kMostCluster = 8;
 
 // Exclusive prefix over the block of one number per thread, and the total.
 template <int THREADS>
@@ -305,10 +305,10 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t x, uint32_t* warp_sums
 }
 
 template <int THREADS>
-__global__ void __launch_bounds__(THREADS) k_evict_select(const EvictArgs a, uint32_t cached) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_evict_select(const __grid_constant__ EvictArgs a, uint32_t cached) {
     namespace cg = cooperative_groups;
     extern __shared__ uint32_t keys[];             // [cached]
-    __shared__ uint32_t count[3][kBins];
+    __shared__ __align__(16) uint32_t count[3][kBins];
     __shared__ uint32_t warp_sums[32];
     __shared__ uint32_t slice_counts[2];           // tokens that stay for certain, tokens equal to the threshold
     __shared__ uint32_t chosen[2];
@@ -344,7 +344,12 @@ __global__ void __launch_bounds__(THREADS) k_evict_select(const EvictArgs a, uin
     const uint32_t first = min(rank * width, n), size = min(width, n - first);
     const uint32_t lo = d.sinks, hi = n - d.recent;              // free tokens
     auto key_of = [&](uint32_t i) { return i < cached ? keys[i] : mass_key(mass[first + i]); };
-    for (uint32_t i = t; i < 3 * kBins; i += THREADS) (&count[0][0])[i] = 0;
+    auto sync = [&]() {
+        if (blocks > 1) cluster.sync();
+        else __syncthreads();
+    };
+#pragma unroll
+    for (uint32_t i = t; i < 3 * kBins / 4; i += THREADS) reinterpret_cast<uint4*>(&count[0][0])[i] = make_uint4(0, 0, 0, 0);
     for (uint32_t i0 = t; i0 < min(size, cached); i0 += 8 * THREADS) {
         float x[8];
 #pragma unroll
@@ -363,6 +368,7 @@ __global__ void __launch_bounds__(THREADS) k_evict_select(const EvictArgs a, uin
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, above = pass == 0 ? 32 : pass == 1 ? 21 : 10;
             const uint32_t mask = pass == 2 ? 1023 : 2047;
+#pragma unroll 4
             for (uint32_t i0 = 0; i0 < size; i0 += THREADS) {    // (all lanes together)
                 const uint32_t i = i0 + t, at = first + i;
                 const bool in_slice = i < size && at >= lo && at < hi;
@@ -379,16 +385,26 @@ __global__ void __launch_bounds__(THREADS) k_evict_select(const EvictArgs a, uin
                 else if (in && !(same >> lane & 1)) atomicAdd(&count[pass][digit], 1u);
             }
             __syncwarp();
-            cluster.sync();
+            sync();
             // bins from the largest digit down, kBins / THREADS to a thread
             constexpr int kEach = kBins / THREADS;
-            uint32_t mine[kEach], sum = 0;
+            uint32_t mine[kEach] = {}, sum = 0;
+            const uint32_t top_bin = kBins - (t + 1) * kEach;
 #pragma unroll
-            for (int u = 0; u < kEach; ++u) {
-                mine[u] = 0;
-                for (uint32_t x = 0; x < blocks; ++x) mine[u] += cluster.map_shared_rank(&count[pass][0], x)[kBins - 1 - (t * kEach + u)];
-                sum += mine[u];
+            for (uint32_t x = 0; x < kMostCluster; ++x) {
+                if (x >= blocks) break;
+                const uint4* from = reinterpret_cast<const uint4*>(cluster.map_shared_rank(&count[pass][0], x) + top_bin);
+#pragma unroll
+                for (int u = 0; u < kEach / 4; ++u) {
+                    const uint4 c = from[u];
+                    mine[kEach - 1 - 4 * u] += c.x;
+                    mine[kEach - 2 - 4 * u] += c.y;
+                    mine[kEach - 3 - 4 * u] += c.z;
+                    mine[kEach - 4 - 4 * u] += c.w;
+                }
             }
+#pragma unroll
+            for (int u = 0; u < kEach; ++u) sum += mine[u];
             uint32_t total;
             uint32_t before = block_prefix<THREADS>(sum, warp_sums, total);
 #pragma unroll
@@ -427,13 +443,13 @@ __global__ void __launch_bounds__(THREADS) k_evict_select(const EvictArgs a, uin
         slice_counts[0] = total_sure;
         slice_counts[1] = total_equal;
     }
-    cluster.sync();
+    sync();
     uint32_t base = 0, base_equal = 0;
     for (uint32_t x = 0; x < rank; ++x) {
         base += cluster.map_shared_rank(&slice_counts[0], x)[0];
         base_equal += cluster.map_shared_rank(&slice_counts[0], x)[1];
     }
-    cluster.sync();                                // no block ends while another reads it
+    if (blocks > 1) cluster.sync();                // no block ends while another reads it
     constexpr uint32_t kRun = 4;                   // tokens of a thread, side by side
     for (uint32_t i0 = 0; i0 < size; i0 += kRun * THREADS) {
         uint32_t k[kRun], sum = 0, total;
@@ -579,9 +595,9 @@ cudaError_t launch_cache_evict(const bs_token_cache& c, const bs_cache_evict_des
     // and the rows alone do not fill the GPU
     uint32_t cluster = 1;
     while (cluster < kMostCluster && d.mass_width / cluster > 4096 &&
-           static_cast<uint64_t>(c.kv_heads) * d.num_seqs * cluster < static_cast<uint64_t>(dev.num_sms))
+           static_cast<uint64_t>(c.kv_heads) * d.num_seqs * cluster * 2 <= static_cast<uint64_t>(dev.num_sms))
         cluster *= 2;
-    const cudaError_t e = d.mass_width <= 4096 ? launch_select<256>(a, cluster, stream) : launch_select<1024>(a, cluster, stream);
+    const cudaError_t e = d.mass_width <= 4096 ? launch_select<256>(a, cluster, stream) : launch_select<512>(a, cluster, stream);
     if (e != cudaSuccess) return e;
     const uint32_t cols = (d.budget + c.block - 1) / c.block;
     const uint32_t used = cols < d.new_table_width ? cols : d.new_table_width;
