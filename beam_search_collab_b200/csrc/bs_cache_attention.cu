@@ -38,8 +38,13 @@ namespace {
 
 constexpr int kWarps = 4;              // per block; they take a segment's tiles in turn
 constexpr int kThreads = kWarps * 32;
-constexpr int kStages = 3;             // tiles a warp has in flight or in use
-constexpr int kBlocksPerSm = 2;
+// Tiles a warp has in flight or in use, and resident blocks: 8 query rows fit
+// three blocks with two stages each (35 us for a batch of 76 k tokens and 8
+// key heads, 37 with two blocks of three stages), 16 rows only two (at three
+// they spill: 56 us against 41).
+template <int NT>
+constexpr int kStagesOf = NT == 1 ? 2 : 3;
+constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 constexpr int kTile = 32;              // tokens: two halves of 16, independent chains of instructions
 constexpr float kNoScore = -1e30f;     // running maximum before the first score
 constexpr float kSlack = 8.f;          // weights may grow to 2^kSlack before the maximum is moved
@@ -57,6 +62,7 @@ struct CacheArgs {
     uint32_t score_width;
     uint32_t shares;     // thread blocks per row tile
     uint32_t block_log2;
+    uint32_t direct;     // 1: a thread block per segment, nothing to join
 };
 
 __device__ __forceinline__ uint32_t held_tokens(const CacheArgs& a, uint32_t b) {
@@ -242,14 +248,14 @@ constexpr int kStageBytes = 2 * kTile * kPitch<NW> + 16;      // keys, values, (
 template <int NW, int NT>
 constexpr int kJoinBytes = 2 * 8 * NT * NW * 16 * 4;           // two warps' outputs
 template <int NW, int NT>
-constexpr size_t kSplitSmem = kWarps * kStages * kStageBytes<NW> + kJoinBytes<NW, NT> + kWarps * (8 * NT * 2 + 4) * 4 + 128;
+constexpr size_t kSplitSmem = kWarps * kStagesOf<NT> * kStageBytes<NW> + kJoinBytes<NW, NT> + kWarps * (8 * NT * 2 + 4) * 4 + 128;
 
 // One share of the tiles for one row tile of 8 * NT query rows.
 // Registers: outputs NW * NT * 4, queries NW * NT * 2, and about 60.
 template <int NW, int NT>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_cache_split(const __grid_constant__ CacheArgs a) {
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(const __grid_constant__ CacheArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
-    constexpr int kDim = NW * 16, kRows = 8 * NT;
+    constexpr int kDim = NW * 16, kRows = 8 * NT, kStages = kStagesOf<NT>;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     unsigned char* ring = smem + warp * kStages * kStageBytes<NW>;
     float* join_o = reinterpret_cast<float*>(smem + kWarps * kStages * kStageBytes<NW>);
@@ -258,14 +264,21 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_cache_split(const __
 
     // this block's share, and the piece it begins with
     const uint32_t hkv = a.c.kv_heads, row0 = blockIdx.y * kRows;
-    uint64_t before, all;
-    count_cost(a, 0, before, all, sums);
-    const uint64_t w_all = all * hkv;
-    const uint32_t n = used_shares(w_all, a.shares);
-    if (blockIdx.x >= n) return;
-    const uint64_t first = share_first(w_all, n, blockIdx.x);
     Piece at;
-    {
+    if (a.direct) {
+        at.b = blockIdx.x / hkv;
+        at.h = blockIdx.x % hkv;
+        at.len = held_tokens(a, at.b);
+        at.left = cost_of(at.len);
+        if (at.len) cut_piece(at, 0);
+        else at.t = at.end = 0;
+    } else {
+        uint64_t before, all;
+        count_cost(a, 0, before, all, sums);
+        const uint64_t w_all = all * hkv;
+        const uint32_t n = used_shares(w_all, a.shares);
+        if (blockIdx.x >= n) return;
+        const uint64_t first = share_first(w_all, n, blockIdx.x);
         uint64_t seen = 0;
         uint32_t b = 0;
         for (uint32_t b0 = 0;; b0 += 32) {                       // 32 sequences at a time
@@ -363,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_cache_split(const __
     }
 
     for (bool first_piece = true; at.b < a.d.num_seqs; next_piece(a, at), first_piece = false) {
-        if (at.t == at.end) continue;      // a share that ends before a segment's first tile
+        if (at.t == at.end && !a.direct) continue;      // a share that ends before a segment's first tile
         // this piece's query rows as the columns of K Q^T: column j is row row0 + j
         uint32_t q[NT][NW][2];
         float row_scale[NT][2];          // of columns 2c and 2c + 1
@@ -735,14 +748,25 @@ __global__ void __launch_bounds__(kMassThreads) k_cache_mass(const __grid_consta
     }
     if (n) {
         const float* s = a.scores + seg * a.rows * a.score_width + j;
-        for (uint32_t r = 0; r < a.rows; ++r) {
-            const float lse = a.lse[(static_cast<uint64_t>(b) * a.d.queries + r / a.group) * a.d.q_heads + h * a.group + r % a.group] *
-                              1.4426950408889634f;
-            const float4 z = *reinterpret_cast<const float4*>(s + static_cast<uint64_t>(r) * a.score_width);
-            if (z.x != -INFINITY) w[0] += exp2_fast(z.x - lse);
-            if (z.y != -INFINITY) w[1] += exp2_fast(z.y - lse);
-            if (z.z != -INFINITY) w[2] += exp2_fast(z.z - lse);
-            if (z.w != -INFINITY) w[3] += exp2_fast(z.w - lse);
+        constexpr uint32_t kBatch = 4;             // rows whose scores are on their way together
+        for (uint32_t r0 = 0; r0 < a.rows; r0 += kBatch) {
+            float4 z[kBatch];
+            float lse[kBatch];
+#pragma unroll
+            for (uint32_t u = 0; u < kBatch; ++u) {
+                const uint32_t r = min(r0 + u, a.rows - 1);
+                z[u] = __ldcs(reinterpret_cast<const float4*>(s + static_cast<uint64_t>(r) * a.score_width));
+                lse[u] = a.lse[(static_cast<uint64_t>(b) * a.d.queries + r / a.group) * a.d.q_heads + h * a.group + r % a.group];
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < kBatch; ++u) {
+                if (r0 + u >= a.rows) break;
+                const float l = lse[u] * 1.4426950408889634f;
+                if (z[u].x != -INFINITY) w[0] += exp2_fast(z[u].x - l);
+                if (z[u].y != -INFINITY) w[1] += exp2_fast(z[u].y - l);
+                if (z[u].z != -INFINITY) w[2] += exp2_fast(z[u].z - l);
+                if (z[u].w != -INFINITY) w[3] += exp2_fast(z[u].w - l);
+            }
         }
     }
     for (uint32_t i = n; i < 4; ++i) w[i] = 0.f;
@@ -752,7 +776,7 @@ __global__ void __launch_bounds__(kMassThreads) k_cache_mass(const __grid_consta
 }
 
 struct Layout {
-    uint32_t nt, row_tiles, shares, score_width;
+    uint32_t nt, row_tiles, shares, score_width, direct;
     size_t lse, part_o, part_ml, scores, total;
 };
 
@@ -764,15 +788,19 @@ Layout plan(const bs_token_cache& c, const bs_cache_attention_desc& d, const Mem
     const uint64_t tokens = static_cast<uint64_t>(d.table_width) * c.block;
     const uint64_t most = (static_cast<uint64_t>(d.num_seqs) * c.kv_heads * ((tokens + kTile - 1) / kTile + kStart) + kStart + kWarps - 1) /
                           (kStart + kWarps);
-    const uint64_t cap = static_cast<uint64_t>(dev.num_sms) * kBlocksPerSm;
+    const uint64_t cap = static_cast<uint64_t>(dev.num_sms) * blocks_per_sm(l.nt);
     l.shares = static_cast<uint32_t>(most < cap ? most : cap);
+    // short sequences: a thread block for each segment costs less than a
+    // second kernel (300 tokens: 6 us against 5 + 4)
+    l.direct = tokens <= 1024;
+    if (l.direct) l.shares = d.num_seqs * static_cast<uint32_t>(c.kv_heads);
     l.score_width = static_cast<uint32_t>(tokens);
     auto take = [&l](size_t bytes) {
         const size_t at = l.total;
         l.total += (bytes + 255) & ~static_cast<size_t>(255);
         return at;
     };
-    const size_t slots = static_cast<size_t>(l.row_tiles) * l.shares * 2 * 8 * l.nt;
+    const size_t slots = l.direct ? 0 : static_cast<size_t>(l.row_tiles) * l.shares * 2 * 8 * l.nt;
     l.lse = take(d.lse ? 0 : static_cast<size_t>(d.num_seqs) * d.queries * d.q_heads * 4);
     l.part_ml = take(slots * 8);
     l.part_o = take(slots * c.dim * 4);
@@ -839,10 +867,11 @@ cudaError_t launch_cache_attention(const bs_token_cache& c, const bs_cache_atten
     a.shares = l.shares;
     a.block_log2 = c.block == 16 ? 4 : c.block == 32 ? 5 : c.block == 64 ? 6 : 7;
     cudaError_t e = cudaSuccess;
+    a.direct = l.direct;
     if (l.shares) e = l.nt == 1 ? launch_split<1>(a, l.row_tiles, stream) : launch_split<2>(a, l.row_tiles, stream);
     if (e != cudaSuccess) return e;
     const uint32_t tile_rows = 8 * l.nt, used_rows = a.rows < tile_rows ? a.rows : tile_rows;
-    e = launch_after(k_cache_join, dim3(c.kv_heads * used_rows, l.row_tiles, d.num_seqs), kJoinThreads, stream, a, tile_rows, used_rows);
+    if (!l.direct) e = launch_after(k_cache_join, dim3(c.kv_heads * used_rows, l.row_tiles, d.num_seqs), kJoinThreads, stream, a, tile_rows, used_rows);
     if (e == cudaSuccess && d.out_mass)
         e = launch_after(k_cache_mass, dim3((d.mass_width + 4 * kMassThreads - 1) / (4 * kMassThreads), c.kv_heads, d.num_seqs),
                          kMassThreads, stream, a);
