@@ -808,22 +808,6 @@ Layout plan(const bs_token_cache& c, const bs_cache_attention_desc& d, const Mem
     return l;
 }
 
-// A kernel that may start while the one before it on the stream still runs
-// (and waits for it by itself).
-template <typename... Params, typename... Given>
-cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, Given... given) {
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t config{};
-    config.gridDim = grid;
-    config.blockDim = dim3(threads);
-    config.stream = stream;
-    config.attrs = &attr;
-    config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, kernel, Params(given)...);
-}
-
 template <int NW, int NT>
 cudaError_t launch_split(const CacheArgs& a, uint32_t row_tiles, cudaStream_t stream) {
     const cudaError_t e = cudaFuncSetAttribute(k_cache_split<NW, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitSmem<NW, NT>);

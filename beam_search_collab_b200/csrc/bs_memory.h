@@ -30,6 +30,7 @@ struct MemoryDevice {
 };
 bs_status memory_device(MemoryDevice& out);
 
+size_t prompt_attention_scratch(const bs_prompt_attention_desc& d, const MemoryDevice& dev);
 cudaError_t launch_prompt_attention(const bs_prompt_attention_desc& d, const MemoryDevice& dev, cudaStream_t stream);
 cudaError_t launch_cache_write(const bs_token_cache& c, const bs_cache_write_desc& d, const MemoryDevice& dev,
                                cudaStream_t stream);
@@ -41,5 +42,23 @@ cudaError_t launch_cache_attention(const bs_token_cache& c, const bs_cache_atten
 size_t cache_evict_scratch(const bs_token_cache& c, const bs_cache_evict_desc& d, const MemoryDevice& dev);
 cudaError_t launch_cache_evict(const bs_token_cache& c, const bs_cache_evict_desc& d, const MemoryDevice& dev,
                                cudaStream_t stream);
+
+#ifdef __CUDACC__
+// A kernel that may start while the one before it on the stream still runs
+// (and waits for it by itself, in every block).
+template <typename... Params, typename... Given>
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, Given... given) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.stream = stream;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, Params(given)...);
+}
+#endif
 
 }  // namespace bsb

@@ -134,7 +134,7 @@ using namespace bsb;
 
 extern "C" {
 
-BS_API bs_status bs_prompt_attention(const bs_prompt_attention_desc* d, void* stream) {
+static bs_status check_prompt(const bs_prompt_attention_desc* d) {
     if (!d) return report_error(BS_ERR_INVALID_ARGUMENT, "desc is NULL");
     if (bs_status s = check_dtype16(d->dtype)) return s;
     if (bs_status s = check_dim(d->dim)) return s;
@@ -143,10 +143,24 @@ BS_API bs_status bs_prompt_attention(const bs_prompt_attention_desc* d, void* st
         return report_error(BS_ERR_INVALID_ARGUMENT, "scale must be positive and finite (not 0, negative, infinite or NaN)");
     if (d->total_q >= (1u << 30) || d->total_k >= (1u << 30) || d->num_seqs > 65535)
         return report_error(BS_ERR_UNSUPPORTED, "at most 65535 sequences of fewer than 2^30 tokens in all are supported");
+    return BS_OK;
+}
+
+BS_API bs_status bs_prompt_attention_workspace(const bs_prompt_attention_desc* d, size_t* bytes) {
+    if (!bytes) return report_error(BS_ERR_INVALID_ARGUMENT, "bytes is NULL");
+    if (bs_status s = check_prompt(d)) return s;
+    MemoryDevice dev;
+    if (bs_status s = memory_device(dev)) return s;
+    *bytes = prompt_attention_scratch(*d, dev);
+    return BS_OK;
+}
+
+BS_API bs_status bs_prompt_attention(const bs_prompt_attention_desc* d, void* stream) {
+    if (bs_status s = check_prompt(d)) return s;
     if (d->total_q == 0 || d->num_seqs == 0) return BS_OK;
     if (any_null({d->q, d->out, d->cu_q, d->cu_k}) || (d->total_k && any_null({d->k, d->v})))
         return report_error(BS_ERR_INVALID_ARGUMENT, "a buffer is NULL");
-    if (!aligned16({d->q, d->k, d->v, d->out}) || !strides_ok(d->q_stride, 2) || !strides_ok(d->k_stride, 2) ||
+    if (!aligned16({d->q, d->k, d->v, d->out, d->workspace}) || !strides_ok(d->q_stride, 2) || !strides_ok(d->k_stride, 2) ||
         !strides_ok(d->v_stride, 2))
         return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign);
     // one head or token for many (a stride of 0) has no tensor map
@@ -155,8 +169,12 @@ BS_API bs_status bs_prompt_attention(const bs_prompt_attention_desc* d, void* st
         return report_error(BS_ERR_UNSUPPORTED, "a stride of 0 (a broadcast tensor) is not supported: make it contiguous");
     MemoryDevice dev;
     if (bs_status s = memory_device(dev)) return s;
-    if (!on_device(dev.device, {d->q, d->k, d->v, d->out, d->lse, d->cu_q, d->cu_k}))
+    if (!on_device(dev.device, {d->q, d->k, d->v, d->out, d->lse, d->cu_q, d->cu_k, d->workspace}))
         return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kWhere);
+    const size_t need = prompt_attention_scratch(*d, dev);
+    if (need > (d->workspace ? d->workspace_bytes : 0))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "workspace of %zu bytes, %zu are needed", d->workspace ? d->workspace_bytes : 0,
+                            need);
     const cudaError_t e = launch_prompt_attention(*d, dev, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? BS_OK : cuda_error(e, "prompt attention launch");
 }

@@ -4,7 +4,11 @@
 // One thread block computes two tiles of 128 query rows against the keys they
 // see, 128 at a time, with a running maximum and sum per row.  The rows of a
 // tile are consecutive tokens times the query heads that share a key head, so
-// a tile's keys and values are loaded once for all those heads.
+// a tile's keys and values are loaded once for all those heads.  A block that
+// is done takes over the next one of the grid that has not started (cluster
+// launch control), its copies and first products under the last one's
+// epilogue.  Where there are few tiles of queries and many of keys, the keys
+// are cut into chunks and a second kernel joins them.
 //
 // Warps 0-3 and 4-7 are the softmax of tile 0 and 1 (a thread has one row),
 // warp 8 issues the matrix instructions, warp 9 the copies:
@@ -40,9 +44,13 @@ using namespace dev;
 namespace {
 
 constexpr int kRows = 128;             // query rows of a tile, keys of a tile
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;          // three warpgroups; the last one's warps 10 and 11 have nothing to do
+// Registers: launched with 168 for each of 384 threads (64,512); the softmax
+// warpgroups take 200, the other gives up 64: 2 * 200 + 104 = 504 = 3 * 168.
+constexpr int kSoftmaxRegisters = 200, kOtherRegisters = 104;
 constexpr int kBoxBytes = kRows * 128; // 128 rows of 64 elements
 constexpr unsigned kPolls = 1u << 22;
+constexpr uint32_t kMostChunks = 8;
 constexpr float kMost = 256.f;         // weights may grow to this before the maximum is moved
 
 struct PromptArgs {
@@ -50,6 +58,9 @@ struct PromptArgs {
     unsigned int* errors;
     uint32_t group;            // query heads per key head
     uint32_t tile_tokens;      // tokens of a tile: group * tile_tokens <= 128 rows
+    uint32_t chunks;           // pieces that the keys are cut into
+    float* part_o;             // [chunks][rows][dim], where there are several
+    float2* part_ml;           // [chunks][rows]: maximum (log2), sum
     CUtensorMap q, k, v;
 };
 
@@ -199,7 +210,7 @@ template <typename T>
 struct Type16;
 template <>
 struct Type16<__half> {
-    static constexpr uint32_t kFormat = 0, kExponent = 0x7c007c00u;
+    static constexpr uint32_t kFormat = 0, kExponent = 0x7c007c00u, kExponentOne = 0x04000400u;
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         const __half2 h = __floats2half2_rn(lo, hi);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -212,7 +223,7 @@ struct Type16<__half> {
 };
 template <>
 struct Type16<__nv_bfloat16> {
-    static constexpr uint32_t kFormat = 1, kExponent = 0x7f807f80u;
+    static constexpr uint32_t kFormat = 1, kExponent = 0x7f807f80u, kExponentOne = 0x00800080u;
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -224,15 +235,18 @@ struct Type16<__nv_bfloat16> {
     }
 };
 
-// Stages of keys or values that fit beside the query tiles.
+// Stages of keys or values that fit beside the query tiles and the softmax
+// warps' 4 KB each for outputs.
 template <int BOXES>
-constexpr int kStagesOf = BOXES == 2 ? 5 : 8;
+constexpr int kStagesOf = BOXES == 2 ? 4 : 8;
+constexpr int kStagingBytes = 8 * 4096;
 
 // The row's largest score among the `left` first of a tile.
-__device__ __forceinline__ float largest(uint32_t s_at, int32_t left) {
+__device__ __forceinline__ float largest(uint32_t s_at, int32_t left, int chunks) {
     float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
     for (int c = 0; c < kRows / 32; ++c) {
+        if (c >= chunks) break;
         float s[32];
         tmem_load32(s_at + 32 * c, s);
         wait_loads32(s);
@@ -242,11 +256,13 @@ __device__ __forceinline__ float largest(uint32_t s_at, int32_t left) {
     return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
-// One row of a tile: weights 2^(scale * s + base), packed in p, their sum in
-// `part`; returns the largest weight.  Scores come from TMEM 32 at a time, the
-// next 32 on their way meanwhile.
+// One row of a tile, the first `chunks` times 32 keys: weights
+// 2^(scale * s + base), packed in p, their sum in `part`; returns the largest
+// weight.  Scores come from TMEM 32 at a time, the next 32 on their way
+// meanwhile.
 template <typename T, bool HIDES>
-__device__ __forceinline__ float weights(uint32_t s_at, int32_t left, float scale, float base, uint32_t (&p)[kRows / 2], float& part) {
+__device__ __forceinline__ float weights(uint32_t s_at, int32_t left, float scale, float base, int chunks, uint32_t (&p)[kRows / 2],
+                                         float& part) {
     const float2 scale2 = make_float2(scale, scale), base2 = make_float2(base, base);
     float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     uint32_t high[2] = {0, 0};
@@ -254,9 +270,10 @@ __device__ __forceinline__ float weights(uint32_t s_at, int32_t left, float scal
     tmem_load32(s_at, s[0]);
 #pragma unroll
     for (int c = 0; c < kRows / 32; ++c) {
+        if (HIDES && c >= chunks) break;
         float* now = s[c & 1];
         wait_loads32(now);
-        if (c + 1 < kRows / 32) tmem_load32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
+        if (c + 1 < kRows / 32 && (!HIDES || c + 1 < chunks)) tmem_load32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float2 x = make_float2(now[2 * i], now[2 * i + 1]);
@@ -278,9 +295,44 @@ __device__ __forceinline__ float weights(uint32_t s_at, int32_t left, float scal
     return fmaxf(h.x, h.y);
 }
 
+// A warp's 32 rows, 128 bytes of each (a lane has its own row's), to memory: by
+// way of shared memory, so that 8 lanes write a row's 128 bytes together
+// (16 bytes of 32 rows at a time took 7,700 clocks for two tiles).  `row` is
+// the lane's row in memory, null if it has none; `at` the first byte's place
+// in it, `bytes` the row's length.
+__device__ __forceinline__ void store_rows(const uint32_t (&u)[32], unsigned char* staging, void* row, uint32_t at, uint32_t bytes) {
+    const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+    for (uint32_t k = 0; k < 8; ++k)
+        *reinterpret_cast<uint4*>(staging + lane * 128 + ((k ^ lane) & 7) * 16) = make_uint4(u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]);
+    __syncwarp();
+#pragma unroll
+    for (uint32_t k = 0; k < 8; ++k) {
+        const uint32_t r = 4 * k + lane / 8, unit = lane & 7;
+        const uint4 w = *reinterpret_cast<const uint4*>(staging + r * 128 + ((unit ^ r) & 7) * 16);
+        unsigned char* to = reinterpret_cast<unsigned char*>(__shfl_sync(kFull, reinterpret_cast<uintptr_t>(row), r));
+        if (to && at + unit * 16 < bytes) *reinterpret_cast<uint4*>(to + at + unit * 16) = w;
+    }
+    __syncwarp();
+}
+
+// What a block works on: a pair of tiles and a run of key tiles.
+struct Item {
+    int32_t valid;              // 0: there is no more
+    int32_t q0, k0, lq, lk;     // the sequence's rows
+    int32_t token0;             // first token of the pair
+    int32_t kv_head, chunk;
+    int32_t first, end[2];      // key tiles of each tile of queries: first .. end[t]
+    int32_t all_see;            // keys that every row of the pair sees
+    int32_t most_see[2];        // keys that any row of a tile sees
+};
+
 struct Control {
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done, raw;
+    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], done, raw;
+    uint64_t item_full[2], item_empty[2], next_full;
     uint64_t full[8], empty[8];
+    __align__(16) uint32_t next[4]; // the launch control's answer
+    Item item[2];
     uint32_t not_finite[8][4];      // by stage: value rows cleared because they are not finite
     uint32_t keep[2];               // outputs hold something before the first value product
     uint32_t tmem;
@@ -288,7 +340,28 @@ struct Control {
 };
 
 template <int BOXES>
-constexpr size_t kSmem = 1024 + (2 + kStagesOf<BOXES>) * BOXES * kBoxBytes + sizeof(Control);
+constexpr size_t kSmem = 1024 + (2 + kStagesOf<BOXES>) * BOXES * kBoxBytes + kStagingBytes + sizeof(Control);
+
+// Asks for the next block of the grid that has not started; the answer
+// arrives at `bar`.
+__device__ __forceinline__ void ask_next(void* answer, uint64_t* bar) {
+    barrier_expect(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n" ::"r"(smem_addr(answer)),
+                 "r"(smem_addr(bar))
+                 : "memory");
+}
+__device__ __forceinline__ bool read_next(const void* answer, uint32_t& block) {
+    uint32_t ok, x;
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b128 h;\n ld.shared.b128 h, [%2];\n"
+        " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n selp.u32 %0, 1, 0, p;\n mov.u32 %1, 0;\n"
+        " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n}\n"
+        : "=r"(ok), "=r"(x)
+        : "r"(smem_addr(answer))
+        : "memory");
+    block = x;
+    return ok != 0;
+}
 
 // BOXES: 64-column boxes of a row (1: dim <= 64, 2: dim <= 128).
 template <typename T, int BOXES>
@@ -297,47 +370,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
     unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t{1023});
     constexpr int kStages = kStagesOf<BOXES>, kTileBytes = BOXES * kBoxBytes;
     unsigned char* const ring = smem + 2 * kTileBytes;
-    Control& ctl = *reinterpret_cast<Control*>(smem + (2 + kStages) * kTileBytes);
+    unsigned char* const staging = smem + (2 + kStages) * kTileBytes;
+    Control& ctl = *reinterpret_cast<Control*>(staging + kStagingBytes);
     const bs_prompt_attention_desc& d = a.d;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-    // which sequence, tokens and key head: sequence b has the blocks
-    // base(b) .. base(b + 1), base(b) = cu_q[b] / pair + b, enough for its
-    // ceil(len / pair) pairs of tiles; the last pair, with the most keys, first
-    const uint32_t pair = 2 * a.tile_tokens, kv_head = blockIdx.x % d.kv_heads, place = blockIdx.x / d.kv_heads;
-    uint32_t b = 0;
-    if (d.num_seqs > 1) {
-        uint32_t at_or_below = 0;
-        for (uint32_t b0 = 0; b0 < d.num_seqs; b0 += kThreads) {
-            const uint32_t i = b0 + threadIdx.x;
-            const uint32_t n = __syncthreads_count(i < d.num_seqs && static_cast<uint32_t>(d.cu_q[i]) / pair + i <= place);
-            at_or_below += n;
-            if (n < kThreads) break;
-        }
-        if (at_or_below == 0) return;
-        b = at_or_below - 1;
-    }
-    const int32_t q0 = d.cu_q[b], q1 = d.cu_q[b + 1], k0 = d.cu_k[b], k1 = d.cu_k[b + 1];
-    if (q0 < 0 || q1 < q0 || static_cast<uint32_t>(q1) > d.total_q || k0 < 0 || k1 < k0 || static_cast<uint32_t>(k1) > d.total_k) {
-        if (threadIdx.x == 0) atomicOr(a.errors, kMemErrLength);
-        return;
-    }
-    const int32_t lq = q1 - q0, lk = k1 - k0;
-    const uint32_t pairs = (lq + pair - 1) / pair, local = place - (static_cast<uint32_t>(q0) / pair + b);
-    if (local >= pairs) return;
-    const int32_t token0 = (pairs - 1 - local) * pair;
-    // keys a token sees, and tiles of keys of each tile of queries
-    const int32_t ahead = lk - lq + 1;
-    auto seen = [&](int32_t token) { return d.causal ? max(0, min(lk, token + ahead)) : lk; };
-    int32_t tiles[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int32_t first = token0 + t * static_cast<int32_t>(a.tile_tokens);
-        const int32_t last = min(first + static_cast<int32_t>(a.tile_tokens), lq) - 1;
-        tiles[t] = last < first ? 0 : (seen(last) + kRows - 1) / kRows;
-    }
-    const int32_t n = max(tiles[0], tiles[1]);
-    const int32_t all_see = seen(token0);        // keys that every row of the pair sees
 
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_addr(&ctl.tmem)) : "memory");
@@ -346,12 +382,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
     if (threadIdx.x == 0) {
         for (int t = 0; t < 2; ++t) {
             barrier_init(&ctl.q_full[t], 1);
+            barrier_init(&ctl.q_empty[t], 1);
             barrier_init(&ctl.s_full[t], 1);
             barrier_init(&ctl.p_full[t], 4);
             barrier_init(&ctl.o_full[t], 1);
+            barrier_init(&ctl.item_full[t], 1);
+            barrier_init(&ctl.item_empty[t], 9);
         }
         barrier_init(&ctl.done, 1);
         barrier_init(&ctl.raw, 1);
+        barrier_init(&ctl.next_full, 1);
         for (int s = 0; s < kStages; ++s) {
             barrier_init(&ctl.full[s], 1);
             barrier_init(&ctl.empty[s], 1);
@@ -376,256 +416,446 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
             atomicOr(a.errors, kMemErrWait);
         }
     };
+    auto drain = [&](uint64_t* bar, unsigned phase) {
+        for (unsigned i = 0; i < kPolls && !barrier_test(bar, phase); ++i) {}
+    };
+    // the next item for a warp that does not copy (not valid: the end), and
+    // that it has read it
+    auto next_item = [&](uint32_t i) -> const Item& {
+        wait(&ctl.item_full[i & 1], (i >> 1) & 1);
+        return ctl.item[i & 1];
+    };
+    auto item_read = [&](uint32_t i) {
+        __syncwarp();
+        if (lane == 0) barrier_arrive(&ctl.item_empty[i & 1]);
+    };
+    // keys that a token sees
+    auto seen = [&](int32_t lq, int32_t lk, int32_t token) { return d.causal ? max(0, min(lk, token + lk - lq + 1)) : lk; };
+    // columns of key tile j that a row seeing `most` keys sees, to a multiple of 16
+    auto columns = [&](int32_t most, int32_t j) { return min(kRows, (most - j * kRows + 15) & ~15); };
 
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegisters));
     if (warp == 9) {
         // ------------------------------------------------------------ copies
-        uint32_t stage = 0, phase = 0;
-        if (lane == 0) {
-            for (int t = 0; t < 2; ++t) {
-                if (!tiles[t]) continue;
-                barrier_expect(&ctl.q_full[t], BOXES * 128 * a.group * a.tile_tokens);
-                for (int x = 0; x < BOXES; ++x)
-                    load_box(smem + t * kTileBytes + x * kBoxBytes, &a.q, 64 * x, kv_head * a.group,
-                             q0 + token0 + t * static_cast<int32_t>(a.tile_tokens), &ctl.q_full[t]);
-            }
-        }
-        uint32_t raw_phase = 0;
-        int32_t loads = 0;
+        // Which sequence, tokens and key head a block of the grid stands for:
+        // sequence b has the places base(b) .. base(b + 1), base(b) =
+        // cu_q[b] / pair + b, enough for its ceil(len / pair) pairs of tiles;
+        // the last pair, with the most keys, first.  A place is all key heads,
+        // each all chunks.
+        const uint32_t pair = 2 * a.tile_tokens;
+        uint32_t stage = 0, phase = 0, raw_phase = 0, next_phase = 0, items = 0, q_used[2] = {0, 0}, loads = 0;
+        uint32_t block = blockIdx.x;
         bool stop = false;
-        for (int32_t j = 0; j < n && !stop; ++j) {
+        while (!stop) {
+            // (only this block's own place and those not yet started are asked for)
+            if (lane == 0) ask_next(ctl.next, &ctl.next_full);
+            Item m;
+            m.valid = 1;
+            m.chunk = block % a.chunks;
+            m.kv_head = block / a.chunks % d.kv_heads;
+            const uint32_t place = block / a.chunks / d.kv_heads;
+            uint32_t lo = 0, hi = d.num_seqs;              // base(lo) <= place, the answer is in [lo, hi)
+            while (hi - lo > 1) {                          // 32 probes at a time
+                const uint32_t step = (hi - lo + 31) / 32, at = lo + lane * step;
+                const bool below = at < hi && (at == 0 || static_cast<uint32_t>(d.cu_q[at]) / pair + at <= place);
+                const int last = 31 - __clz(__ballot_sync(kFull, below) | 1u);
+                hi = min(hi, lo + (last + 1) * step);
+                lo = lo + last * step;
+            }
+            const int32_t q1 = d.cu_q[lo + 1], k1 = d.cu_k[lo + 1];
+            m.q0 = d.cu_q[lo];
+            m.k0 = d.cu_k[lo];
+            m.lq = q1 - m.q0;
+            m.lk = k1 - m.k0;
+            bool work = true;
+            if (m.q0 < 0 || m.lq < 0 || static_cast<uint32_t>(q1) > d.total_q || m.k0 < 0 || m.lk < 0 || static_cast<uint32_t>(k1) > d.total_k) {
+                if (lane == 0) atomicOr(a.errors, kMemErrLength);
+                work = false;
+            }
+            const uint32_t pairs = work ? (m.lq + pair - 1) / pair : 0, local = place - (static_cast<uint32_t>(m.q0) / pair + lo);
+            work = local < pairs;
+            if (work) {
+                m.token0 = (pairs - 1 - local) * pair;
+                m.all_see = seen(m.lq, m.lk, m.token0);
+                int32_t tiles[2];
 #pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
-                unsigned char* const dst = ring + stage * kTileBytes;
-                // value rows of this tile that not all rows see, and rows past the sequence
-                const int32_t hidden = max(0, all_see - j * kRows), past = lk - j * kRows;
-                const bool look = kv == 1 && hidden < kRows;
-                if (lane == 0) wait(&ctl.empty[stage], phase ^ 1);
-                stop = __shfl_sync(kFull, *gave_up, 0) != 0;
-                if (stop) break;
-                ++loads;
-                if (lane == 0) {
-                    uint64_t* const bar = look ? &ctl.raw : &ctl.full[stage];
-                    barrier_expect(bar, kTileBytes);
-                    for (int x = 0; x < BOXES; ++x)
-                        load_box(dst + x * kBoxBytes, kv ? &a.v : &a.k, 64 * x, kv_head, k0 + j * kRows, bar);
-                    if (look)
-                        for (unsigned i = 0; i < kPolls && !barrier_test(&ctl.raw, raw_phase); ++i) {}
+                for (int t = 0; t < 2; ++t) {
+                    const int32_t from = m.token0 + t * static_cast<int32_t>(a.tile_tokens);
+                    const int32_t last = min(from + static_cast<int32_t>(a.tile_tokens), m.lq) - 1;
+                    m.most_see[t] = last < from ? 0 : seen(m.lq, m.lk, last);
+                    tiles[t] = (m.most_see[t] + kRows - 1) / kRows;
                 }
-                __syncwarp();
-                if (look) {
-                    raw_phase ^= 1;
-#pragma unroll 1
-                    for (int i = 0; i < kRows / 32; ++i) {
-                        const int32_t r = 32 * i + lane;
-                        bool odd = false;
-                        if (r >= hidden && r < past) {
-#pragma unroll 1
+                const int32_t n = max(tiles[0], tiles[1]), chunks = static_cast<int32_t>(a.chunks);
+                m.first = static_cast<int32_t>(static_cast<int64_t>(n) * m.chunk / chunks);
+                const int32_t end = static_cast<int32_t>(static_cast<int64_t>(n) * (m.chunk + 1) / chunks);
+                m.end[0] = max(m.first, min(end, tiles[0]));
+                m.end[1] = max(m.first, min(end, tiles[1]));
+                const uint32_t slot = items & 1;
+                if (lane == 0) {
+                    wait(&ctl.item_empty[slot], ((items >> 1) & 1) ^ 1);
+                    if (!*gave_up) {
+                        ctl.item[slot] = m;
+                        barrier_arrive(&ctl.item_full[slot]);
+                    }
+                }
+                ++items;
+                if (lane == 0) {
+                    for (int t = 0; t < 2; ++t) {
+                        if (m.end[t] == m.first) continue;
+                        wait(&ctl.q_empty[t], (q_used[t] & 1) ^ 1);
+                        if (*gave_up) break;
+                        ++q_used[t];
+                        barrier_expect(&ctl.q_full[t], BOXES * 128 * a.group * a.tile_tokens);
+                        for (int x = 0; x < BOXES; ++x)
+                            load_box(smem + t * kTileBytes + x * kBoxBytes, &a.q, 64 * x, m.kv_head * a.group,
+                                     m.q0 + m.token0 + t * static_cast<int32_t>(a.tile_tokens), &ctl.q_full[t]);
+                    }
+                }
+                for (int32_t j = m.first; j < max(m.end[0], m.end[1]) && !stop; ++j) {
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv) {
+                        unsigned char* const dst = ring + stage * kTileBytes;
+                        // value rows of this tile that not all rows see, and rows past the sequence
+                        const int32_t hidden = max(0, m.all_see - j * kRows), past = m.lk - j * kRows;
+                        const bool look = kv == 1 && hidden < kRows;
+                        if (lane == 0) wait(&ctl.empty[stage], phase ^ 1);
+                        stop = __shfl_sync(kFull, *gave_up, 0) != 0;
+                        if (stop) break;
+                        ++loads;
+                        if (lane == 0) {
+                            uint64_t* const bar = look ? &ctl.raw : &ctl.full[stage];
+                            barrier_expect(bar, kTileBytes);
                             for (int x = 0; x < BOXES; ++x)
-                                for (int u = 0; u < 8; ++u) {
-                                    const uint4 w = *reinterpret_cast<const uint4*>(dst + x * kBoxBytes + r * 128 + ((u + lane) & 7) * 16);
-                                    constexpr uint32_t e = Type16<T>::kExponent;
-                                    odd |= (__vcmpeq2(w.x & e, e) | __vcmpeq2(w.y & e, e) | __vcmpeq2(w.z & e, e) | __vcmpeq2(w.w & e, e)) != 0;
-                                }
+                                load_box(dst + x * kBoxBytes, kv ? &a.v : &a.k, 64 * x, m.kv_head, m.k0 + j * kRows, bar);
+                            if (look) drain(&ctl.raw, raw_phase);
                         }
-                        const uint32_t rows = __ballot_sync(kFull, odd);
-                        if (lane == 0) ctl.not_finite[stage][i] = rows;
-                        if (odd || r >= past) {
+                        __syncwarp();
+                        if (look) {
+                            raw_phase ^= 1;
 #pragma unroll 1
-                            for (int x = 0; x < BOXES; ++x)
-                                for (int u = 0; u < 8; ++u)
-                                    *reinterpret_cast<uint4*>(dst + x * kBoxBytes + r * 128 + ((u + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            for (int i = 0; i < kRows / 32; ++i) {
+                                const int32_t r = 32 * i + lane;
+                                uint32_t carry = 0;          // an exponent of all ones plus one carries over
+                                if (32 * i + 31 >= hidden && 32 * i < past) {
+#pragma unroll
+                                    for (int x = 0; x < BOXES; ++x)
+#pragma unroll
+                                        for (int u = 0; u < 8; ++u) {
+                                            const uint4 w = *reinterpret_cast<const uint4*>(dst + x * kBoxBytes + r * 128 + ((u + lane) & 7) * 16);
+                                            constexpr uint32_t e = Type16<T>::kExponent, one = Type16<T>::kExponentOne;
+                                            carry |= ((w.x & e) + one) | ((w.y & e) + one) | ((w.z & e) + one) | ((w.w & e) + one);
+                                        }
+                                }
+                                const bool odd = (carry & 0x80008000u) && r >= hidden && r < past;
+                                const uint32_t rows = __ballot_sync(kFull, odd);
+                                if (lane == 0) ctl.not_finite[stage][i] = rows;
+                                if (odd || r >= past) {
+#pragma unroll
+                                    for (int x = 0; x < BOXES; ++x)
+#pragma unroll
+                                        for (int u = 0; u < 8; ++u)
+                                            *reinterpret_cast<uint4*>(dst + x * kBoxBytes + r * 128 + ((u + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
+                                }
+                            }
+                            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) barrier_arrive(&ctl.full[stage]);
+                        }
+                        if (++stage == kStages) {
+                            stage = 0;
+                            phase ^= 1;
                         }
                     }
-                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) barrier_arrive(&ctl.full[stage]);
-                }
-                if (++stage == kStages) {
-                    stage = 0;
-                    phase ^= 1;
                 }
             }
+            // (whatever happened: an answer on its way is waited for)
+            if (lane == 0) drain(&ctl.next_full, next_phase);
+            __syncwarp();
+            next_phase ^= 1;
+            const bool more = read_next(ctl.next, block);
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            stop = __shfl_sync(kFull, stop || *gave_up != 0, 0);
+            if (!more) break;
         }
-        // no copy may be in flight when the block ends
         if (lane == 0) {
+            const uint32_t slot = items & 1;
+            wait(&ctl.item_empty[slot], ((items >> 1) & 1) ^ 1);
+            if (!*gave_up) {
+                ctl.item[slot].valid = 0;
+                barrier_arrive(&ctl.item_full[slot]);
+            }
+            // no copy may be in flight when the block ends
             for (int t = 0; t < 2; ++t)
-                for (unsigned i = 0; tiles[t] && i < kPolls && !barrier_test(&ctl.q_full[t], 0); ++i) {}
-            for (int32_t i = max(0, loads - kStages); i < loads; ++i)
-                for (unsigned x = 0; x < kPolls && !barrier_test(&ctl.full[i % kStages], (i / kStages) & 1); ++x) {}
+                if (q_used[t]) drain(&ctl.q_full[t], (q_used[t] - 1) & 1);
+            for (uint32_t i = loads > kStages ? loads - kStages : 0; i < loads; ++i) drain(&ctl.full[i % kStages], (i / kStages) & 1);
         }
         __syncwarp();
     } else if (warp == 8) {
         // ---------------------------------------------------- matrix products
         // (the whole warp runs the loop, one elected lane issues)
-        if (n > 0) {
-            constexpr uint32_t kCommon = 1u << 4 | Type16<T>::kFormat << 7 | Type16<T>::kFormat << 10 | (kRows >> 4) << 24;
-            const uint32_t what_s = kCommon | (kRows >> 3) << 17;
-            const uint32_t what_o = kCommon | 1u << 16 | static_cast<uint32_t>(d.dim >> 3) << 17;
-            // what the lane does per instruction counts: operands are a base
-            // and constants (16-byte units)
-            const int steps = d.dim / 16;
-            const uint64_t q_base = operand(smem_addr(smem), 16, 1024), k_base = operand(smem_addr(ring), 16, 1024);
-            const uint64_t v_base = operand(smem_addr(ring), kBoxBytes, 1024);
-            constexpr uint32_t kTileUnits = kTileBytes / 16, kBoxUnits = kBoxBytes / 16;
-            auto scores = [&](int t, uint32_t stage) {
-                const uint64_t q = q_base + t * kTileUnits, k = k_base + stage * kTileUnits;
-                if (elected()) {
+        constexpr uint32_t kCommon = 1u << 4 | Type16<T>::kFormat << 7 | Type16<T>::kFormat << 10 | (kRows >> 4) << 24;
+        const uint32_t what_o = kCommon | 1u << 16 | static_cast<uint32_t>(d.dim >> 3) << 17;
+        // what the lane does per instruction counts: operands are a base
+        // and constants (16-byte units)
+        const int steps = d.dim / 16;
+        const uint64_t q_base = operand(smem_addr(smem), 16, 1024), k_base = operand(smem_addr(ring), 16, 1024);
+        const uint64_t v_base = operand(smem_addr(ring), kBoxBytes, 1024);
+        constexpr uint32_t kTileUnits = kTileBytes / 16, kBoxUnits = kBoxBytes / 16;
+        auto scores = [&](int t, uint32_t stage, int32_t cols) {
+            const uint64_t q = q_base + t * kTileUnits, k = k_base + stage * kTileUnits;
+            const uint32_t what_s = kCommon | static_cast<uint32_t>(cols >> 3) << 17;
+            if (elected()) {
 #pragma unroll
-                    for (int i = 0; i < 4 * BOXES; ++i) {
-                        const uint32_t off = (i >> 2) * kBoxUnits + (i & 3) * 2;
-                        if (i < steps) mma_shared(tmem + t * 128, q + off, k + off, what_s, i > 0);
-                    }
-                    mma_commit(&ctl.s_full[t]);
+                for (int i = 0; i < 4 * BOXES; ++i) {
+                    const uint32_t off = (i >> 2) * kBoxUnits + (i & 3) * 2;
+                    if (i < steps) mma_shared(tmem + t * 128, q + off, k + off, what_s, i > 0);
                 }
-                __syncwarp();
-            };
-            auto values = [&](int t, uint32_t stage, bool add) {
-                const uint64_t v = v_base + stage * kTileUnits;
-                if (elected()) {
-#pragma unroll
-                    for (int i = 0; i < kRows / 16; ++i)
-                        mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + i * 8, v + i * 128, what_o, add || i > 0);
-                }
-                __syncwarp();
-            };
-            auto commit = [&](uint64_t* bar) {
-                if (elected()) mma_commit(bar);
-                __syncwarp();
-            };
-            auto full = [&](int32_t i) { wait(&ctl.full[i % kStages], (i / kStages) & 1); };
-            full(0);
-            for (int t = 0; t < 2; ++t) {
-                if (!tiles[t]) continue;
-                wait(&ctl.q_full[t], 0);
-                fence_after();
-                scores(t, 0);
+                mma_commit(&ctl.s_full[t]);
             }
-            commit(&ctl.empty[0]);
-            for (int32_t j = 0; j < n; ++j) {
+            __syncwarp();
+        };
+        auto values = [&](int t, uint32_t stage, bool add, int32_t cols) {
+            const uint64_t v = v_base + stage * kTileUnits;
+            if (elected()) {
+#pragma unroll
+                for (int i = 0; i < kRows / 16; ++i) {
+                    if (16 * i >= cols) break;
+                    mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + i * 8, v + i * 128, what_o, add || i > 0);
+                }
+            }
+            __syncwarp();
+        };
+        auto commit = [&](uint64_t* bar) {
+            if (elected()) mma_commit(bar);
+            __syncwarp();
+        };
+        auto full = [&](uint32_t i) { wait(&ctl.full[i % kStages], (i / kStages) & 1); };
+        uint32_t loads = 0, q_used[2] = {0, 0}, p_used[2] = {0, 0};
+        bool issued = false;
+        for (uint32_t i = 0;; ++i) {
+            const Item m = next_item(i);
+            if (__any_sync(kFull, *gave_up != 0) || !m.valid) break;
+            item_read(i);
+            const int32_t end = max(m.end[0], m.end[1]);
+            if (end == m.first) continue;
+            issued = true;
+            full(loads);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (m.end[t] == m.first) continue;
+                wait(&ctl.q_full[t], q_used[t]++ & 1);
+                fence_after();
+                scores(t, loads % kStages, columns(m.most_see[t], m.first));
+                if (m.end[t] == m.first + 1) commit(&ctl.q_empty[t]);
+            }
+            commit(&ctl.empty[loads % kStages]);
+            for (int32_t j = m.first; j < end; ++j) {
                 if (__any_sync(kFull, *gave_up != 0)) break;
-                const int32_t v_load = 2 * j + 1, k_load = 2 * j + 2;
+                const uint32_t v_load = loads + 1, k_load = loads + 2;
+                loads += 2;
                 full(v_load);
-                if (j + 1 < n) full(k_load);
+                if (j + 1 < end) full(k_load);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    if (j >= tiles[t]) continue;
-                    wait(&ctl.p_full[t], j & 1);
+                    if (j >= m.end[t]) continue;
+                    wait(&ctl.p_full[t], p_used[t]++ & 1);
                     fence_after();
-                    values(t, v_load % kStages, j > 0 || ctl.keep[t]);
-                    if (j + 1 == tiles[t]) commit(&ctl.o_full[t]);
-                    else scores(t, k_load % kStages);
+                    values(t, v_load % kStages, j > m.first || ctl.keep[t], columns(m.most_see[t], j));
+                    if (j + 1 == m.end[t]) {
+                        commit(&ctl.o_full[t]);
+                    } else {
+                        scores(t, k_load % kStages, columns(m.most_see[t], j + 1));
+                        if (j + 2 == m.end[t]) commit(&ctl.q_empty[t]);
+                    }
                 }
                 commit(&ctl.empty[v_load % kStages]);
-                if (j + 1 < n) commit(&ctl.empty[k_load % kStages]);
+                if (j + 1 < end) commit(&ctl.empty[k_load % kStages]);
             }
-            // TMEM and the stages are in use until this
+        }
+        // TMEM and the stages are in use until this
+        if (issued) {
             commit(&ctl.done);
-            for (unsigned i = 0; i < kPolls && !barrier_test(&ctl.done, 0); ++i) {}
+            drain(&ctl.done, 0);
         }
         __syncwarp();
+    }
     } else {
         // ----------------------------------------------------------- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegisters));
         const uint32_t t = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (warp & 3) * 32 << 16;                  // this warp's TMEM lanes
         const uint32_t s_at = tmem + t * 128 + lanes, o_at = tmem + 256 + t * 128 + lanes;
-        const int32_t token = token0 + static_cast<int32_t>(t * a.tile_tokens + row / a.group);
-        const bool real = row < a.group * a.tile_tokens && token < lq;
-        const int32_t limit = real ? seen(token) : 0;
-        const int32_t mine = t ? tiles[1] : tiles[0];
+        const int32_t row_token = static_cast<int32_t>(t * a.tile_tokens + row / a.group);
+        const bool in_tile = row < a.group * a.tile_tokens;
         const float scale = d.scale * 1.4426950408889634f;
-        float top = -INFINITY, sum = 0.f;       // top: of the unscaled scores
-        for (int32_t j = 0; j < mine && !*gave_up; ++j) {
-            wait(&ctl.s_full[t], j & 1);        // and the value product before it is done
-            fence_after();
-            const bool hides = (j + 1) * kRows > all_see;
-            const int32_t left = limit - j * kRows;         // keys of this tile that the row sees
-            if (j == 0) top = largest(s_at, left);
-            uint32_t p[kRows / 2];
-            float part;
-            for (bool again = false;; again = true) {
-                const float base = top == -INFINITY ? 0.f : -top * scale;
-                const float high = hides ? weights<T, true>(s_at, left, scale, base, p, part) : weights<T, false>(s_at, left, scale, base, p, part);
-                if (again || !__any_sync(kFull, real && high > kMost)) break;     // (other rows hold anything)
-                // rare: the maximum moves, what was summed is rescaled
-                const float next = fmaxf(top, largest(s_at, left));
-                const float shrink = next == -INFINITY ? 1.f : exp2_fast((top - next) * scale);
-                sum *= shrink;
-                for (int x = 0; x < d.dim; x += 16) {
-                    float o[16];
-                    tmem_load16(o_at + x, o);
-                    wait_loads16(o);
+        uint32_t s_used = 0, o_used = 0, loads = 0;
+        for (uint32_t i = 0;; ++i) {
+            // (what the loop does not need every time stays in shared memory
+            // till the item is done: registers)
+            const Item& item = next_item(i);
+            if (__any_sync(kFull, *gave_up != 0) || !item.valid) break;
+            const int32_t first = item.first, end = item.end[t], all_see = item.all_see;
+            const bool real = in_tile && item.token0 + row_token < item.lq;
+            const int32_t limit = real ? seen(item.lq, item.lk, item.token0 + row_token) : 0;
+            float top = -INFINITY, sum = 0.f;       // top: of the unscaled scores
+            for (int32_t j = first; j < end && !*gave_up; ++j) {
+                wait(&ctl.s_full[t], s_used++ & 1);        // and the value product before it is done
+                fence_after();
+                const bool hides = (j + 1) * kRows > all_see;
+                const int32_t left = limit - j * kRows;         // keys of this tile that the row sees
+                const int chunks = hides ? (columns(item.most_see[t], j) + 31) / 32 : kRows / 32;
+                if (j == first) top = largest(s_at, left, chunks);
+                uint32_t p[kRows / 2];
+                float part;
+                for (bool again = false;; again = true) {
+                    const float base = top == -INFINITY ? 0.f : -top * scale;
+                    const float high = hides ? weights<T, true>(s_at, left, scale, base, chunks, p, part)
+                                             : weights<T, false>(s_at, left, scale, base, chunks, p, part);
+                    if (again || !__any_sync(kFull, real && high > kMost)) break;     // (other rows hold anything)
+                    // rare: the maximum moves, what was summed is rescaled
+                    const float next = fmaxf(top, largest(s_at, left, chunks));
+                    const float shrink = next == -INFINITY ? 1.f : exp2_fast((top - next) * scale);
+                    sum *= shrink;
+                    for (int x = 0; x < d.dim; x += 16) {
+                        float o[16];
+                        tmem_load16(o_at + x, o);
+                        wait_loads16(o);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] *= shrink;
-                    tmem_store16(o_at + x, o);
-                }
-                top = next;
-            }
-            sum += part;
-            tmem_store32(s_at, p);
-            tmem_store32(s_at + 32, p + 32);
-            wait_stores();
-            if (hides) {
-                // value rows that were cleared because they are not finite,
-                // for the query rows that see them
-                const uint32_t stage = (2 * j + 1) % kStages;
-                wait(&ctl.full[stage], ((2 * j + 1) / kStages) & 1);
-                const uint32_t* odd = ctl.not_finite[stage];
-                if (j == 0 && (odd[0] | odd[1] | odd[2] | odd[3])) {
-                    const float zeros[16] = {};
-                    for (int x = 0; x < d.dim; x += 16) tmem_store16(o_at + x, zeros);
-                    wait_stores();
-                    ctl.keep[t] = 1;
-                }
-                for (int w = 0; w < 4; ++w)
-                    for (uint32_t left = odd[w]; left; left &= left - 1) {
-                        const int r = 32 * w + __ffs(left) - 1;
-                        const uint32_t two = tmem_load1(s_at + r / 2);
-                        const float2 f = Type16<T>::unpack(two);
-                        const float weight = r & 1 ? f.y : f.x;
-                        const T* v = static_cast<const T*>(d.v) + (k0 + j * kRows + r) * d.v_stride[0] + kv_head * d.v_stride[1];
-                        for (int x = 0; x < d.dim; x += 16) {
-                            float o[16];
-                            tmem_load16(o_at + x, o);
-                            wait_loads16(o);
-                            if (j * kRows + r < limit)
-                                for (int i = 0; i < 16; ++i) o[i] += weight * static_cast<float>(v[x + i]);
-                            __syncwarp();
-                            tmem_store16(o_at + x, o);
-                            wait_stores();
-                        }
+                        for (int k = 0; k < 16; ++k) o[k] *= shrink;
+                        tmem_store16(o_at + x, o);
                     }
+                    top = next;
+                }
+                sum += part;
+                tmem_store32(s_at, p);
+                if (chunks > 2) tmem_store32(s_at + 32, p + 32);
+                wait_stores();
+                bool keep = false;
+                if (hides) {
+                    // value rows that were cleared because they are not finite,
+                    // for the query rows that see them
+                    const uint32_t load = loads + 2 * (j - first) + 1, stage = load % kStages;
+                    wait(&ctl.full[stage], (load / kStages) & 1);
+                    const uint32_t* odd = ctl.not_finite[stage];
+                    keep = j == first && (odd[0] | odd[1] | odd[2] | odd[3]);
+                    if (keep) {
+                        const float zeros[16] = {};
+                        for (int x = 0; x < d.dim; x += 16) tmem_store16(o_at + x, zeros);
+                        wait_stores();
+                    }
+                    for (int w = 0; w < 4; ++w)
+                        for (uint32_t rest = odd[w]; rest; rest &= rest - 1) {
+                            const int r = 32 * w + __ffs(rest) - 1;
+                            if (r >= 32 * chunks) break;       // seen by none of this tile
+                            const float2 f = Type16<T>::unpack(tmem_load1(s_at + r / 2));
+                            const float weight = r & 1 ? f.y : f.x;
+                            const T* v = static_cast<const T*>(d.v) + (item.k0 + j * kRows + r) * d.v_stride[0] + item.kv_head * d.v_stride[1];
+                            for (int x = 0; x < d.dim; x += 16) {
+                                float o[16];
+                                tmem_load16(o_at + x, o);
+                                wait_loads16(o);
+                                if (r < left)
+                                    for (int k = 0; k < 16; ++k) o[k] += weight * static_cast<float>(v[x + k]);
+                                __syncwarp();
+                                tmem_store16(o_at + x, o);
+                                wait_stores();
+                            }
+                        }
+                }
+                if (j == first && lane == 0) ctl.keep[t] = keep;
+                fence_before();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(&ctl.p_full[t]);
             }
-            fence_before();
-            __syncwarp();
-            if (lane == 0) barrier_arrive(&ctl.p_full[t]);
-        }
-        if (mine > 0) {
-            wait(&ctl.o_full[t], 0);
-            fence_after();
-        }
-        const bool ok = real && !*gave_up;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const uint64_t at = (static_cast<uint64_t>(q0) + token) * d.q_heads + kv_head * a.group + row % a.group;
-        T* out = static_cast<T*>(d.out) + at * d.dim;
-        for (int x = 0; x < d.dim; x += 16) {
-            float o[16];
-            if (mine > 0) {
-                tmem_load16(o_at + x, o);
-                wait_loads16(o);
+            loads += 2 * (max(item.end[0], item.end[1]) - first);
+            const bool any = end > first;
+            if (any) {
+                wait(&ctl.o_full[t], o_used++ & 1);
+                fence_after();
             }
-            uint32_t u[8];
+            const bool ok = real && !*gave_up;
+            const uint64_t at = (static_cast<uint64_t>(item.q0) + item.token0 + row_token) * d.q_heads + item.kv_head * a.group + row % a.group;
+            if (a.chunks > 1) {
+                // a piece of the keys: unnormalised, to be joined
+                const uint64_t slot = item.chunk * (static_cast<uint64_t>(d.total_q) * d.q_heads) + at;
+                float* const out = ok ? a.part_o + slot * d.dim : nullptr;
+                for (int x = 0; any && x < d.dim; x += 32) {
+                    float o[32];
+                    tmem_load32(o_at + x, o);
+                    wait_loads32(o);
+                    uint32_t u[32];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] = mine > 0 && sum != 0.f ? Type16<T>::pack(o[2 * i] * inv, o[2 * i + 1] * inv) : 0;
-            if (ok) {
-                reinterpret_cast<uint4*>(out + x)[0] = make_uint4(u[0], u[1], u[2], u[3]);
-                reinterpret_cast<uint4*>(out + x)[1] = make_uint4(u[4], u[5], u[6], u[7]);
+                    for (int k = 0; k < 32; ++k) u[k] = __float_as_uint(o[k]);
+                    store_rows(u, staging + warp * 4096, out, x * 4, d.dim * 4);
+                }
+                if (ok) a.part_ml[slot] = make_float2(top * scale, sum);
+            } else {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                T* const out = ok ? static_cast<T*>(d.out) + at * d.dim : nullptr;
+                for (int x = 0; x < d.dim; x += 64) {
+                    uint32_t u[32];
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        float o[32];
+                        tmem_load32(o_at + x + 32 * half, o);
+                        wait_loads32(o);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            u[16 * half + k] = any && sum != 0.f ? Type16<T>::pack(o[2 * k] * inv, o[2 * k + 1] * inv) : 0;
+                    }
+                    store_rows(u, staging + warp * 4096, out, x * 2, d.dim * 2);
+                }
+                if (ok && d.lse) d.lse[at] = sum == 0.f ? -INFINITY : top * d.scale + logf(sum);
             }
+            item_read(i);
+            // the next item's first value product overwrites the outputs: it
+            // waits for weights that this warp makes after these loads
+            fence_before();
         }
-        if (ok && d.lse) d.lse[at] = sum == 0.f ? -INFINITY : top * d.scale + logf(sum);
     }
     fence_before();
     __syncthreads();
     if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+}
+
+// One warp per row: joins the pieces of its keys.
+__global__ void __launch_bounds__(128) k_prompt_join(const __grid_constant__ PromptArgs a) {
+    const bs_prompt_attention_desc& d = a.d;
+    const uint64_t rows = static_cast<uint64_t>(d.total_q) * d.q_heads, row = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    const uint32_t lane = threadIdx.x & 31;
+    cudaGridDependencySynchronize();       // in every block: what follows this kernel may count on both being done
+    if (row >= rows) return;
+    float2 ml[kMostChunks];
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (uint32_t c = 0; c < kMostChunks; ++c) {
+        ml[c] = c < a.chunks ? a.part_ml[c * rows + row] : make_float2(-INFINITY, 0.f);
+        m = fmaxf(m, ml[c].x);
+    }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 o[kMostChunks];
+    const bool mine = lane * 4 < static_cast<uint32_t>(d.dim);
+#pragma unroll
+    for (uint32_t c = 0; c < kMostChunks; ++c)          // (a piece that saw nothing was not written)
+        if (ml[c].y != 0.f && mine) o[c] = *reinterpret_cast<const float4*>(a.part_o + (c * rows + row) * d.dim + lane * 4);
+#pragma unroll
+    for (uint32_t c = 0; c < kMostChunks; ++c) {
+        if (ml[c].y == 0.f || !mine) continue;
+        const float w = exp2_fast(ml[c].x - m);
+        acc.x += o[c].x * w, acc.y += o[c].y * w, acc.z += o[c].z * w, acc.w += o[c].w * w;
+    }
+#pragma unroll
+    for (uint32_t c = 0; c < kMostChunks; ++c)
+        if (ml[c].y != 0.f) l += ml[c].y * exp2_fast(ml[c].x - m);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (lane == 0 && d.lse) d.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    if (!mine) return;
+    uint2 u;
+    if (d.dtype == BS_F16) u = make_uint2(Type16<__half>::pack(acc.x * inv, acc.y * inv), Type16<__half>::pack(acc.z * inv, acc.w * inv));
+    else u = make_uint2(Type16<__nv_bfloat16>::pack(acc.x * inv, acc.y * inv), Type16<__nv_bfloat16>::pack(acc.z * inv, acc.w * inv));
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(d.out) + row * d.dim + lane * 4) = u;
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -663,24 +893,51 @@ cudaError_t tensor_map(CUtensorMap* map, const void* p, int32_t dtype, int32_t d
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+uint32_t tile_tokens(const bs_prompt_attention_desc& d) { return kRows / static_cast<uint32_t>(d.q_heads / d.kv_heads); }
+
+// Pairs of tiles times key heads, at most.
+uint64_t most_items(const bs_prompt_attention_desc& d) {
+    return (d.total_q / (2 * tile_tokens(d)) + static_cast<uint64_t>(d.num_seqs)) * d.kv_heads;
+}
+
+// Pieces that the keys are cut into: where the pairs of tiles leave most of
+// the GPU idle and the keys are many tiles, enough for two blocks an SM.
+uint32_t chunks_of(const bs_prompt_attention_desc& d, const MemoryDevice& dev) {
+    const uint64_t items = most_items(d), tiles = d.total_k / kRows / (d.num_seqs ? d.num_seqs : 1);
+    uint64_t n = 1;
+    while (n < kMostChunks && items * n * 2 <= 2 * static_cast<uint64_t>(dev.num_sms) && tiles >= 8 * n) n *= 2;
+    return static_cast<uint32_t>(n);
+}
+
 template <typename T, int BOXES>
 cudaError_t launch(const PromptArgs& a, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(k_prompt<T, BOXES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<BOXES>);
     if (e != cudaSuccess) return e;
-    const uint64_t blocks = (a.d.total_q / (2 * a.tile_tokens) + static_cast<uint64_t>(a.d.num_seqs)) * a.d.kv_heads;
+    const uint64_t blocks = most_items(a.d) * a.chunks;
     if (blocks > 0x7fffffffu) return cudaErrorInvalidConfiguration;
     k_prompt<T, BOXES><<<static_cast<unsigned>(blocks), kThreads, kSmem<BOXES>, stream>>>(a);
-    return cudaGetLastError();
+    e = cudaGetLastError();
+    if (e != cudaSuccess || a.chunks == 1) return e;
+    const uint64_t rows = static_cast<uint64_t>(a.d.total_q) * a.d.q_heads;
+    return launch_after(k_prompt_join, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, stream, a);
 }
 
 }  // namespace
+
+size_t prompt_attention_scratch(const bs_prompt_attention_desc& d, const MemoryDevice& dev) {
+    const uint32_t chunks = chunks_of(d, dev);
+    return chunks == 1 ? 0 : static_cast<size_t>(chunks) * d.total_q * d.q_heads * (d.dim * 4 + 8);
+}
 
 cudaError_t launch_prompt_attention(const bs_prompt_attention_desc& d, const MemoryDevice& dev, cudaStream_t stream) {
     PromptArgs a{};
     a.d = d;
     a.errors = dev.errors;
     a.group = d.q_heads / d.kv_heads;
-    a.tile_tokens = kRows / a.group;
+    a.tile_tokens = tile_tokens(d);
+    a.chunks = chunks_of(d, dev);
+    a.part_o = static_cast<float*>(d.workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(a.chunks) * d.total_q * d.q_heads * d.dim);
     cudaError_t e = tensor_map(&a.q, d.q, d.dtype, d.dim, d.q_heads, d.total_q, d.q_stride, a.group, a.tile_tokens);
     // (no keys: nothing is read through the maps)
     if (e == cudaSuccess && d.total_k) e = tensor_map(&a.k, d.k, d.dtype, d.dim, d.kv_heads, d.total_k, d.k_stride, 1, kRows);

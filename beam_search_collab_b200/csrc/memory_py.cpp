@@ -121,8 +121,13 @@ py::tuple prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, co
     d.dtype = type_of(q);
     d.causal = causal;
     d.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(q.size(2), 1))));
+    size_t bytes = 0;
+    check(bs_prompt_attention_workspace(&d, &bytes));
+    const Tensor work = scratch(bytes, q.device());
+    d.workspace = bytes ? work.data_ptr() : nullptr;
+    d.workspace_bytes = bytes;
     check(bs_prompt_attention(&d, to.stream));
-    to.used({&out, &lse});
+    to.used({&out, &lse, &work});
     return py::make_tuple(out, maybe(lse));
 }
 

@@ -302,6 +302,8 @@ typedef struct bs_prompt_attention_desc {
     int64_t v_stride[2];
     const int32_t* cu_q;      /* [num_seqs + 1]                               */
     const int32_t* cu_k;
+    void* workspace;
+    size_t workspace_bytes;
     uint32_t total_q, total_k, num_seqs;
     int32_t q_heads, kv_heads, dim;
     int32_t dtype;            /* BS_F16 or BS_BF16                            */
@@ -310,6 +312,7 @@ typedef struct bs_prompt_attention_desc {
 } bs_prompt_attention_desc;
 
 BS_API bs_status bs_prompt_attention(const bs_prompt_attention_desc* desc, void* stream);
+BS_API bs_status bs_prompt_attention_workspace(const bs_prompt_attention_desc* desc, size_t* bytes);
 
 /* Appends tokens: rows cu[b] .. cu[b+1] of k and v become positions start[b],
  * start[b] + 1, ... of sequence b, whose position p lies in block

@@ -14,7 +14,8 @@ class _Cache(ctypes.Structure):
 
 class _Prompt(ctypes.Structure):
     _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("lse", _vp), ("q_stride", _i64 * 2),
-                ("k_stride", _i64 * 2), ("v_stride", _i64 * 2), ("cu_q", _vp), ("cu_k", _vp), ("total_q", _u32),
+                ("k_stride", _i64 * 2), ("v_stride", _i64 * 2), ("cu_q", _vp), ("cu_k", _vp),
+                ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t), ("total_q", _u32),
                 ("total_k", _u32), ("num_seqs", _u32), ("q_heads", _i32), ("kv_heads", _i32), ("dim", _i32),
                 ("dtype", _i32), ("causal", _i32), ("scale", ctypes.c_float)]
 
@@ -54,6 +55,7 @@ def _lib():
         L = lib()
         P = ctypes.POINTER
         for name, args in (("bs_prompt_attention", [P(_Prompt), _vp]),
+                           ("bs_prompt_attention_workspace", [P(_Prompt), P(ctypes.c_size_t)]),
                            ("bs_cache_write", [P(_Cache), P(_Write), _vp]),
                            ("bs_cache_read", [P(_Cache), P(_Read), _vp]),
                            ("bs_cache_attention", [P(_Cache), P(_Attention), _vp]),

@@ -41,7 +41,8 @@ def test_null_descriptors():
     ("out", None, 1, "NULL"), ("k", 72, 1, "16-byte aligned"), ("q_stride", (4, 64), 1, "multiples of 8"),
     ("v_stride", (-8, 64), 1, "non-negative")])
 def test_prompt_checks(field, value, code, text):
-    d = A._Prompt(64, 64, 64, 64, 64, (128, 64), (128, 64), (128, 64), 64, 64, 10, 10, 1, 2, 2, 64, 1, 1, 0.1)
+    d = A._Prompt(64, 64, 64, 64, 64, (128, 64), (128, 64), (128, 64), 64, 64, None, 0, 10, 10, 1, 2, 2, 64, 1, 1,
+                  0.1)
     setattr(d, field, (ctypes.c_int64 * 2)(*value) if isinstance(value, tuple) else value)
     rc, why = status("bs_prompt_attention", d, None)
     assert rc == code and text in why, (rc, why)
@@ -77,7 +78,7 @@ def test_evict_checks(field, value, code, text):
 
 
 def test_nothing_to_do_is_done_without_a_gpu():
-    d = A._Prompt(None, None, None, None, None, (0, 0), (0, 0), (0, 0), None, None, 0, 0, 0, 2, 2, 64, 1, 1, 0.1)
+    d = A._Prompt(None, None, None, None, None, (0, 0), (0, 0), (0, 0), None, None, None, 0, 0, 0, 0, 2, 2, 64, 1, 1, 0.1)
     assert status("bs_prompt_attention", d, None)[0] == 0
     assert status("bs_cache_write", cache(), A._Write(dtype=1), None)[0] == 0
     assert status("bs_cache_read", cache(), A._Read(dtype=1), None)[0] == 0
