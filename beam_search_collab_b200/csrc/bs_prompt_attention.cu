@@ -19,9 +19,10 @@
 //             in the order S0 S1 | P0V S0' P1V S1' | ...: while one tile's
 //             softmax runs, the tensor pipe has the other tile's work
 //   softmax   S_t to registers, P_t = 2^(scale' S_t - m) back to TMEM in the
-//             inputs' 16-bit type.  m is moved only when a row's maximum has
-//             grown by more than 2^8 (then O_t, in TMEM, is rescaled), so most
-//             tiles touch O_t not at all; sums are 32-bit of the unrounded P.
+//             inputs' 16-bit type.  m is moved only when a weight would be
+//             over 2^8 (then O_t, in TMEM, is rescaled), so most tiles touch
+//             O_t not at all and no maximum is taken before the exponentials;
+//             sums are 32-bit of the unrounded P.
 // TMEM (512 columns): S0 S1 O0 O1, 128 columns each.
 //
 // Keys of other sequences or of the future that a tile also covers are set to
@@ -44,10 +45,7 @@ using namespace dev;
 namespace {
 
 constexpr int kRows = 128;             // query rows of a tile, keys of a tile
-constexpr int kThreads = 384;          // three warpgroups; the last one's warps 10 and 11 have nothing to do
-// Registers: launched with 168 for each of 384 threads (64,512); the softmax
-// warpgroups take 200, the other gives up 64: 2 * 200 + 104 = 504 = 3 * 168.
-constexpr int kSoftmaxRegisters = 200, kOtherRegisters = 104;
+constexpr int kThreads = 320;
 constexpr int kBoxBytes = kRows * 128; // 128 rows of 64 elements
 constexpr unsigned kPolls = 1u << 22;
 constexpr uint32_t kMostChunks = 8;
@@ -134,11 +132,11 @@ __device__ __forceinline__ void wait_loads32(float* r) {
                  :
                  : "memory");
 }
-__device__ __forceinline__ void wait_loads16(float* r) {
+__device__ __forceinline__ void wait_loads16(uint32_t* r) {
     asm volatile("tcgen05.wait::ld.sync.aligned;\n"
-                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]),
-                   "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]),
-                   "+f"(r[14]), "+f"(r[15])
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                   "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+                   "+r"(r[14]), "+r"(r[15])
                  :
                  : "memory");
 }
@@ -156,28 +154,19 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, float* r) {
         : "r"(at)
         : "memory");
 }
-__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* u) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};\n" ::"r"(u[0]),
-        "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]),
-        "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]), "r"(u[21]),
-        "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(at)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_load16(uint32_t at, float* r) {
+__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t* r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
-        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]),
-          "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(at)
         : "memory");
 }
-__device__ __forceinline__ void tmem_store16(uint32_t at, const float* r) {
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* r) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};\n" ::"f"(r[0]),
-        "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]), "f"(r[10]), "f"(r[11]),
-        "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15]), "r"(at)
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};\n" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(at)
         : "memory");
 }
 __device__ __forceinline__ uint32_t tmem_load1(uint32_t at) {
@@ -241,58 +230,126 @@ template <int BOXES>
 constexpr int kStagesOf = BOXES == 2 ? 4 : 8;
 constexpr int kStagingBytes = 8 * 4096;
 
-// The row's largest score among the `left` first of a tile.
-__device__ __forceinline__ float largest(uint32_t s_at, int32_t left, int chunks) {
-    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+// 32 scores of a row: weights 2^(scale * s + base), packed in p; adds to two
+// pairs of sums and of largest weights.
+template <typename T>
+__device__ __forceinline__ void weights32(const float* s, float2 scale, float2 base, uint32_t* p, float2 (&add)[2], uint32_t (&high)[2]) {
 #pragma unroll
-    for (int c = 0; c < kRows / 32; ++c) {
-        if (c >= chunks) break;
-        float s[32];
-        tmem_load32(s_at + 32 * c, s);
-        wait_loads32(s);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) m[i & 3] = fmaxf(m[i & 3], 32 * c + i < left ? s[i] : -INFINITY);
+    for (int i = 0; i < 16; ++i) {
+        float2 x = fma2(make_float2(s[2 * i], s[2 * i + 1]), scale, base);
+        x.x = exp2_fast(x.x);
+        x.y = exp2_fast(x.y);
+        add[i & 1] = add2(add[i & 1], x);
+        p[i] = Type16<T>::pack(x.x, x.y);
+        high[i & 1] = Type16<T>::larger(high[i & 1], p[i]);
     }
-    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
-// One row of a tile, the first `chunks` times 32 keys: weights
-// 2^(scale * s + base), packed in p, their sum in `part`; returns the largest
-// weight.  Scores come from TMEM 32 at a time, the next 32 on their way
-// meanwhile.
-template <typename T, bool HIDES>
-__device__ __forceinline__ float weights(uint32_t s_at, int32_t left, float scale, float base, int chunks, uint32_t (&p)[kRows / 2],
-                                         float& part) {
+// 64 scores of a row that sees them all, 32 at a time; s[0] is on its way, the
+// next 32 follow (`more`: those after these too).  Returns the largest
+// weight, their sum in `part`.  (Unrolled: in a loop of 32 the
+// special-function pipe runs dry at each turn, 2,650 clocks a tile against
+// 1,650.)
+template <typename T>
+__device__ __forceinline__ float weights64(uint32_t s_at, bool more, float (&s)[2][32], float scale, float base, uint32_t (&p)[kRows / 4],
+                                           float& part) {
     const float2 scale2 = make_float2(scale, scale), base2 = make_float2(base, base);
     float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     uint32_t high[2] = {0, 0};
-    float s[2][32];
-    tmem_load32(s_at, s[0]);
 #pragma unroll
-    for (int c = 0; c < kRows / 32; ++c) {
-        if (HIDES && c >= chunks) break;
-        float* now = s[c & 1];
-        wait_loads32(now);
-        if (c + 1 < kRows / 32 && (!HIDES || c + 1 < chunks)) tmem_load32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float2 x = make_float2(now[2 * i], now[2 * i + 1]);
-            if (HIDES) {
-                x.x = 32 * c + 2 * i < left ? x.x : -INFINITY;
-                x.y = 32 * c + 2 * i + 1 < left ? x.y : -INFINITY;
-            }
-            x = fma2(x, scale2, base2);
-            x.x = exp2_fast(x.x);
-            x.y = exp2_fast(x.y);
-            add[i & 1] = add2(add[i & 1], x);
-            p[16 * c + i] = Type16<T>::pack(x.x, x.y);
-            high[i & 1] = Type16<T>::larger(high[i & 1], p[16 * c + i]);
-        }
+    for (int c = 0; c < 2; ++c) {
+        wait_loads32(s[c]);
+        if (c == 0 || more) tmem_load32(s_at + 32 * (c + 1), s[c ^ 1]);
+        weights32<T>(s[c], scale2, base2, p + 16 * c, add, high);
     }
     add[0] = add2(add[0], add[1]);
     part = add[0].x + add[0].y;
     const float2 h = Type16<T>::unpack(Type16<T>::larger(high[0], high[1]));
     return fmaxf(h.x, h.y);
+}
+
+// The same for 32 scores in registers.
+template <typename T>
+__device__ __forceinline__ float weights(const float (&s)[32], float scale, float base, uint32_t (&p)[16], float& part) {
+    float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    uint32_t high[2] = {0, 0};
+    weights32<T>(s, make_float2(scale, scale), make_float2(base, base), p, add, high);
+    add[0] = add2(add[0], add[1]);
+    part = add[0].x + add[0].y;
+    const float2 h = Type16<T>::unpack(Type16<T>::larger(high[0], high[1]));
+    return fmaxf(h.x, h.y);
+}
+
+// The warp's rows times `shrink`: the quarters from .. to of their weights of a
+// tile and `dim` columns of outputs.
+template <typename T>
+__device__ __forceinline__ void rescale(uint32_t p_at, uint32_t o_at, int from, int to, int dim, float shrink) {
+    wait_stores();
+#pragma unroll 1
+    for (int c = from; c < to; ++c) {
+        uint32_t p[16];
+        tmem_load16(p_at + 16 * c, p);
+        wait_loads16(p);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const float2 f = Type16<T>::unpack(p[k]);
+            p[k] = Type16<T>::pack(f.x * shrink, f.y * shrink);
+        }
+        tmem_store16(p_at + 16 * c, p);
+    }
+#pragma unroll 1
+    for (int x = 0; x < dim; x += 16) {
+        uint32_t o[16];
+        tmem_load16(o_at + x, o);
+        wait_loads16(o);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
+        tmem_store16(o_at + x, o);
+    }
+    wait_stores();
+}
+
+// The first tile, tiles with hidden keys, and where the maximum moves: 32
+// scores at a time, so that the weights can go to columns whose scores have
+// been read.  From the quarter `from` on (0, or 2 where the first half has been
+// multiplied already and only the outputs are left to rescale).  `state` is
+// the row's maximum and sum, returned as they become.
+template <typename T>
+__device__ __noinline__ float2 weights_with_care(uint32_t s_at, uint32_t o_at, int from, int chunks, int32_t left, bool real, float scale,
+                                                 int dim, float2 state) {
+    float top = state.x, sum = state.y;
+    float s[2][32];
+    tmem_load32(s_at + 32 * from, s[0]);
+#pragma unroll 1
+    for (int c = from; c < chunks; c += 2) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int at = c + x;
+            if (at >= chunks) break;
+            wait_loads32(s[x]);
+            if (at + 1 < chunks) tmem_load32(s_at + 32 * (at + 1), s[x ^ 1]);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) s[x][k] = 32 * at + k < left ? s[x][k] : -INFINITY;
+            uint32_t p[16];
+            float part;
+            const float high = weights<T>(s[x], scale, top == -INFINITY ? 0.f : -top * scale, p, part);
+            if (__any_sync(kFull, real && (high > kMost || top == -INFINITY))) {
+                // the maximum moves, what was summed is rescaled
+                float next = top;
+#pragma unroll
+                for (int k = 0; k < 32; ++k) next = fmaxf(next, s[x][k]);
+                const float shrink = next == -INFINITY ? 1.f : exp2_fast((top - next) * scale);
+                top = next;
+                sum *= shrink;
+                if (at + 1 < chunks) wait_loads32(s[x ^ 1]);
+                rescale<T>(s_at, o_at, 0, at, dim, shrink);
+                weights<T>(s[x], scale, top == -INFINITY ? 0.f : -top * scale, p, part);
+            }
+            sum += part;
+            tmem_store16(s_at + 16 * at, p);
+        }
+    }
+    return make_float2(top, sum);
 }
 
 // A warp's 32 rows, 128 bytes of each (a lane has its own row's), to memory: by
@@ -434,8 +491,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
     // columns of key tile j that a row seeing `most` keys sees, to a multiple of 16
     auto columns = [&](int32_t most, int32_t j) { return min(kRows, (most - j * kRows + 15) & ~15); };
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegisters));
     if (warp == 9) {
         // ------------------------------------------------------------ copies
         // Which sequence, tokens and key head a block of the grid stands for:
@@ -538,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                                 const int32_t r = 32 * i + lane;
                                 uint32_t carry = 0;          // an exponent of all ones plus one carries over
                                 if (32 * i + 31 >= hidden && 32 * i < past) {
-#pragma unroll
+#pragma unroll 1
                                     for (int x = 0; x < BOXES; ++x)
 #pragma unroll
                                         for (int u = 0; u < 8; ++u) {
@@ -551,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                                 const uint32_t rows = __ballot_sync(kFull, odd);
                                 if (lane == 0) ctl.not_finite[stage][i] = rows;
                                 if (odd || r >= past) {
-#pragma unroll
+#pragma unroll 1
                                     for (int x = 0; x < BOXES; ++x)
 #pragma unroll
                                         for (int u = 0; u < 8; ++u)
@@ -603,33 +658,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
         const uint64_t q_base = operand(smem_addr(smem), 16, 1024), k_base = operand(smem_addr(ring), 16, 1024);
         const uint64_t v_base = operand(smem_addr(ring), kBoxBytes, 1024);
         constexpr uint32_t kTileUnits = kTileBytes / 16, kBoxUnits = kBoxBytes / 16;
+        // (by the elected lane)
         auto scores = [&](int t, uint32_t stage, int32_t cols) {
             const uint64_t q = q_base + t * kTileUnits, k = k_base + stage * kTileUnits;
             const uint32_t what_s = kCommon | static_cast<uint32_t>(cols >> 3) << 17;
-            if (elected()) {
 #pragma unroll
-                for (int i = 0; i < 4 * BOXES; ++i) {
-                    const uint32_t off = (i >> 2) * kBoxUnits + (i & 3) * 2;
-                    if (i < steps) mma_shared(tmem + t * 128, q + off, k + off, what_s, i > 0);
-                }
-                mma_commit(&ctl.s_full[t]);
+            for (int i = 0; i < 4 * BOXES; ++i) {
+                const uint32_t off = (i >> 2) * kBoxUnits + (i & 3) * 2;
+                if (i < steps) mma_shared(tmem + t * 128, q + off, k + off, what_s, i > 0);
             }
-            __syncwarp();
+            mma_commit(&ctl.s_full[t]);
         };
         auto values = [&](int t, uint32_t stage, bool add, int32_t cols) {
             const uint64_t v = v_base + stage * kTileUnits;
-            if (elected()) {
 #pragma unroll
-                for (int i = 0; i < kRows / 16; ++i) {
-                    if (16 * i >= cols) break;
-                    mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + i * 8, v + i * 128, what_o, add || i > 0);
-                }
+            for (int i = 0; i < kRows / 16; ++i) {
+                if (16 * i >= cols) break;
+                mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + i * 8, v + i * 128, what_o, add || i > 0);
             }
-            __syncwarp();
-        };
-        auto commit = [&](uint64_t* bar) {
-            if (elected()) mma_commit(bar);
-            __syncwarp();
         };
         auto full = [&](uint32_t i) { wait(&ctl.full[i % kStages], (i / kStages) & 1); };
         uint32_t loads = 0, q_used[2] = {0, 0}, p_used[2] = {0, 0};
@@ -647,43 +693,57 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                 if (m.end[t] == m.first) continue;
                 wait(&ctl.q_full[t], q_used[t]++ & 1);
                 fence_after();
-                scores(t, loads % kStages, columns(m.most_see[t], m.first));
-                if (m.end[t] == m.first + 1) commit(&ctl.q_empty[t]);
+                const int32_t cols = columns(m.most_see[t], m.first);
+                if (elected()) {
+                    scores(t, loads % kStages, cols);
+                    if (m.end[t] == m.first + 1) mma_commit(&ctl.q_empty[t]);
+                }
+                __syncwarp();
             }
-            commit(&ctl.empty[loads % kStages]);
+            if (elected()) mma_commit(&ctl.empty[loads % kStages]);
+            __syncwarp();
             for (int32_t j = m.first; j < end; ++j) {
                 if (__any_sync(kFull, *gave_up != 0)) break;
                 const uint32_t v_load = loads + 1, k_load = loads + 2;
+                const uint32_t v_stage = v_load % kStages, k_stage = k_load % kStages;
                 loads += 2;
                 full(v_load);
                 if (j + 1 < end) full(k_load);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     if (j >= m.end[t]) continue;
+                    const int32_t cols = columns(m.most_see[t], j), next_cols = columns(m.most_see[t], j + 1);
+                    const bool last = j + 1 == m.end[t];
                     wait(&ctl.p_full[t], p_used[t]++ & 1);
                     fence_after();
-                    values(t, v_load % kStages, j > m.first || ctl.keep[t], columns(m.most_see[t], j));
-                    if (j + 1 == m.end[t]) {
-                        commit(&ctl.o_full[t]);
-                    } else {
-                        scores(t, k_load % kStages, columns(m.most_see[t], j + 1));
-                        if (j + 2 == m.end[t]) commit(&ctl.q_empty[t]);
+                    const bool add = j > m.first || ctl.keep[t];
+                    if (elected()) {
+                        values(t, v_stage, add, cols);
+                        if (last) {
+                            mma_commit(&ctl.o_full[t]);
+                        } else {
+                            scores(t, k_stage, next_cols);
+                            if (j + 2 == m.end[t]) mma_commit(&ctl.q_empty[t]);
+                        }
                     }
+                    __syncwarp();
                 }
-                commit(&ctl.empty[v_load % kStages]);
-                if (j + 1 < end) commit(&ctl.empty[k_load % kStages]);
+                if (elected()) {
+                    mma_commit(&ctl.empty[v_stage]);
+                    if (j + 1 < end) mma_commit(&ctl.empty[k_stage]);
+                }
+                __syncwarp();
             }
         }
         // TMEM and the stages are in use until this
         if (issued) {
-            commit(&ctl.done);
+            if (elected()) mma_commit(&ctl.done);
+            __syncwarp();
             drain(&ctl.done, 0);
         }
         __syncwarp();
-    }
     } else {
         // ----------------------------------------------------------- softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegisters));
         const uint32_t t = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (warp & 3) * 32 << 16;                  // this warp's TMEM lanes
         const uint32_t s_at = tmem + t * 128 + lanes, o_at = tmem + 256 + t * 128 + lanes;
@@ -699,38 +759,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
             const int32_t first = item.first, end = item.end[t], all_see = item.all_see;
             const bool real = in_tile && item.token0 + row_token < item.lq;
             const int32_t limit = real ? seen(item.lq, item.lk, item.token0 + row_token) : 0;
-            float top = -INFINITY, sum = 0.f;       // top: of the unscaled scores
+            float top = -INFINITY, sum = 0.f;       // top: of the unscaled scores, moved when a weight is past 2^8
             for (int32_t j = first; j < end && !*gave_up; ++j) {
                 wait(&ctl.s_full[t], s_used++ & 1);        // and the value product before it is done
                 fence_after();
                 const bool hides = (j + 1) * kRows > all_see;
                 const int32_t left = limit - j * kRows;         // keys of this tile that the row sees
                 const int chunks = hides ? (columns(item.most_see[t], j) + 31) / 32 : kRows / 32;
-                if (j == first) top = largest(s_at, left, chunks);
-                uint32_t p[kRows / 2];
-                float part;
-                for (bool again = false;; again = true) {
-                    const float base = top == -INFINITY ? 0.f : -top * scale;
-                    const float high = hides ? weights<T, true>(s_at, left, scale, base, chunks, p, part)
-                                             : weights<T, false>(s_at, left, scale, base, chunks, p, part);
-                    if (again || !__any_sync(kFull, real && high > kMost)) break;     // (other rows hold anything)
-                    // rare: the maximum moves, what was summed is rescaled
-                    const float next = fmaxf(top, largest(s_at, left, chunks));
-                    const float shrink = next == -INFINITY ? 1.f : exp2_fast((top - next) * scale);
-                    sum *= shrink;
-                    for (int x = 0; x < d.dim; x += 16) {
-                        float o[16];
-                        tmem_load16(o_at + x, o);
-                        wait_loads16(o);
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) o[k] *= shrink;
-                        tmem_store16(o_at + x, o);
+                int done = 0;           // quarters of the tile whose weights are made
+                if (!hides && j > first) {
+                    float s[2][32];
+                    tmem_load32(s_at, s[0]);
+#pragma unroll 1
+                    for (; done < 4; done += 2) {
+                        uint32_t p[kRows / 4];
+                        float part;
+                        const float high = weights64<T>(s_at + 32 * done, done == 0, s, scale, -top * scale, p, part);
+                        if (__any_sync(kFull, real && high > kMost)) break;       // (rows that are none of the tile's hold anything)
+                        sum += part;
+                        tmem_store16(s_at + 16 * done, p);
+                        tmem_store16(s_at + 16 * done + 16, p + 16);
                     }
-                    top = next;
+                    if (done == 0) wait_loads32(s[0]);
                 }
-                sum += part;
-                tmem_store32(s_at, p);
-                if (chunks > 2) tmem_store32(s_at + 32, p + 32);
+                if (done < 4) {
+                    const float2 r = weights_with_care<T>(s_at, o_at, done, chunks, hides ? left : kRows, real, scale, j > first ? d.dim : 0,
+                                                          make_float2(top, sum));
+                    top = r.x;
+                    sum = r.y;
+                }
                 wait_stores();
                 bool keep = false;
                 if (hides) {
@@ -741,7 +798,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                     const uint32_t* odd = ctl.not_finite[stage];
                     keep = j == first && (odd[0] | odd[1] | odd[2] | odd[3]);
                     if (keep) {
-                        const float zeros[16] = {};
+                        const uint32_t zeros[16] = {};
                         for (int x = 0; x < d.dim; x += 16) tmem_store16(o_at + x, zeros);
                         wait_stores();
                     }
@@ -753,11 +810,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                             const float weight = r & 1 ? f.y : f.x;
                             const T* v = static_cast<const T*>(d.v) + (item.k0 + j * kRows + r) * d.v_stride[0] + item.kv_head * d.v_stride[1];
                             for (int x = 0; x < d.dim; x += 16) {
-                                float o[16];
+                                uint32_t o[16];
                                 tmem_load16(o_at + x, o);
                                 wait_loads16(o);
                                 if (r < left)
-                                    for (int k = 0; k < 16; ++k) o[k] += weight * static_cast<float>(v[x + k]);
+#pragma unroll
+                                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) + weight * static_cast<float>(v[x + k]));
                                 __syncwarp();
                                 tmem_store16(o_at + x, o);
                                 wait_stores();
