@@ -35,6 +35,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cstdlib>
+
 #include "bs_device.cuh"
 #include "bs_memory.h"
 
@@ -56,6 +58,7 @@ struct PromptArgs {
     unsigned int* errors;
     uint32_t group;            // query heads per key head
     uint32_t tile_tokens;      // tokens of a tile: group * tile_tokens <= 128 rows
+    uint32_t polls;            // of a wait before it gives up (BSEARCH_WAIT_POLLS: a test sets 0)
     uint32_t chunks;           // pieces that the keys are cut into
     float* part_o;             // [chunks][rows][dim], where there are several
     float2* part_ml;           // [chunks][rows]: maximum (log2), sum
@@ -280,13 +283,13 @@ __device__ __forceinline__ float weights(const float (&s)[32], float scale, floa
     return fmaxf(h.x, h.y);
 }
 
-// The warp's rows times `shrink`: the quarters from .. to of their weights of a
-// tile and `dim` columns of outputs.
+// The warp's rows times `shrink`: the first `quarters` of their weights of a tile
+// and `dim` columns of outputs.
 template <typename T>
-__device__ __forceinline__ void rescale(uint32_t p_at, uint32_t o_at, int from, int to, int dim, float shrink) {
+__device__ __forceinline__ void rescale(uint32_t p_at, uint32_t o_at, int quarters, int dim, float shrink) {
     wait_stores();
 #pragma unroll 1
-    for (int c = from; c < to; ++c) {
+    for (int c = 0; c < quarters; ++c) {
         uint32_t p[16];
         tmem_load16(p_at + 16 * c, p);
         wait_loads16(p);
@@ -311,9 +314,8 @@ __device__ __forceinline__ void rescale(uint32_t p_at, uint32_t o_at, int from, 
 
 // The first tile, tiles with hidden keys, and where the maximum moves: 32
 // scores at a time, so that the weights can go to columns whose scores have
-// been read.  From the quarter `from` on (0, or 2 where the first half has been
-// multiplied already and only the outputs are left to rescale).  `state` is
-// the row's maximum and sum, returned as they become.
+// been read.  From the quarter `from` on (0, or 2 where the first half's weights
+// are made).  `state` is the row's maximum and sum, returned as they become.
 template <typename T>
 __device__ __noinline__ float2 weights_with_care(uint32_t s_at, uint32_t o_at, int from, int chunks, int32_t left, bool real, float scale,
                                                  int dim, float2 state) {
@@ -342,7 +344,7 @@ __device__ __noinline__ float2 weights_with_care(uint32_t s_at, uint32_t o_at, i
                 top = next;
                 sum *= shrink;
                 if (at + 1 < chunks) wait_loads32(s[x ^ 1]);
-                rescale<T>(s_at, o_at, 0, at, dim, shrink);
+                rescale<T>(s_at, o_at, at, dim, shrink);
                 weights<T>(s[x], scale, top == -INFINITY ? 0.f : -top * scale, p, part);
             }
             sum += part;
@@ -462,11 +464,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
     const uint32_t tmem = ctl.tmem;
 
     // A bounded wait.  Once one has given up none waits any more: the warps
-    // leave their loops, what is in flight is waited for (bounded too), and
-    // nothing is stored.
+    // leave their loops together, what is in flight is waited for (`drain`,
+    // bounded too), and nothing is stored.
     volatile uint32_t* const gave_up = &ctl.gave_up;
     auto wait = [&](uint64_t* bar, unsigned phase) {
-        for (unsigned i = 0; i < kPolls && !*gave_up; ++i)
+        for (unsigned i = 0; i < a.polls && !*gave_up; ++i)
             if (barrier_test(bar, phase)) return;
         if (!*gave_up) {
             *gave_up = 1;
@@ -760,8 +762,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
             const bool real = in_tile && item.token0 + row_token < item.lq;
             const int32_t limit = real ? seen(item.lq, item.lk, item.token0 + row_token) : 0;
             float top = -INFINITY, sum = 0.f;       // top: of the unscaled scores, moved when a weight is past 2^8
-            for (int32_t j = first; j < end && !*gave_up; ++j) {
+            for (int32_t j = first; j < end; ++j) {
                 wait(&ctl.s_full[t], s_used++ & 1);        // and the value product before it is done
+                if (__any_sync(kFull, *gave_up != 0)) break;
                 fence_after();
                 const bool hides = (j + 1) * kRows > all_see;
                 const int32_t left = limit - j * kRows;         // keys of this tile that the row sees
@@ -795,6 +798,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                     // for the query rows that see them
                     const uint32_t load = loads + 2 * (j - first) + 1, stage = load % kStages;
                     wait(&ctl.full[stage], (load / kStages) & 1);
+                    if (__any_sync(kFull, *gave_up != 0)) break;
                     const uint32_t* odd = ctl.not_finite[stage];
                     keep = j == first && (odd[0] | odd[1] | odd[2] | odd[3]);
                     if (keep) {
@@ -833,7 +837,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                 wait(&ctl.o_full[t], o_used++ & 1);
                 fence_after();
             }
-            const bool ok = real && !*gave_up;
+            const bool ok = !__any_sync(kFull, *gave_up != 0) && real;
             const uint64_t at = (static_cast<uint64_t>(item.q0) + item.token0 + row_token) * d.q_heads + item.kv_head * a.group + row % a.group;
             if (a.chunks > 1) {
                 // a piece of the keys: unnormalised, to be joined
@@ -991,6 +995,8 @@ cudaError_t launch_prompt_attention(const bs_prompt_attention_desc& d, const Mem
     PromptArgs a{};
     a.d = d;
     a.errors = dev.errors;
+    const char* polls = std::getenv("BSEARCH_WAIT_POLLS");
+    a.polls = polls ? static_cast<uint32_t>(std::strtoul(polls, nullptr, 10)) : kPolls;
     a.group = d.q_heads / d.kv_heads;
     a.tile_tokens = tile_tokens(d);
     a.chunks = chunks_of(d, dev);

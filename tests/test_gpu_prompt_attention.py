@@ -169,6 +169,43 @@ def test_bad_lengths_set_an_error_bit_and_touch_nothing_else():
     assert M.take_errors() == 0 and torch.equal(good, again)
 
 
+@pytest.mark.parametrize("d,lens", [(64, [300]), (128, [2000, 5]), (128, [1])])
+def test_a_wait_that_gives_up_is_reported_and_the_gpu_stays_usable(d, lens, monkeypatch):
+    # BSEARCH_WAIT_POLLS=0: the first wait of every block gives up at once
+    q, k, v = inputs(16, sum(lens), sum(lens), 4, 2, d, BF16)
+    good, _ = M.prompt_attention(q, k, v, R.cu(lens))
+    assert M.take_errors() == 0
+    monkeypatch.setenv("BSEARCH_WAIT_POLLS", "0")
+    M.prompt_attention(q, k, v, R.cu(lens))
+    assert M.take_errors() == 1 and M.take_errors() == 0
+    monkeypatch.delenv("BSEARCH_WAIT_POLLS")
+    again, _ = M.prompt_attention(q, k, v, R.cu(lens))
+    assert M.take_errors() == 0 and torch.equal(good, again)
+
+
+def test_few_queries_over_many_keys():
+    # few tiles of queries: the keys are cut into chunks that a second kernel joins
+    for lens_q, lens_k in (([1], [9000]), ([40, 3], [6000, 17]), ([128], [5000])):
+        q, k, v = inputs(17, sum(lens_q), sum(lens_k), 4, 2, 96, F16)
+        check(q, k, v, lens_q, lens_k)
+        check(q, k, v, lens_q, lens_k, causal=False)
+
+
+def test_values_that_are_not_finite_reach_those_who_see_them():
+    q, k, v = inputs(18, 400, 400, 2, 1, 128, BF16)
+    v[150, 0, 3], v[390, 0, 5] = math.inf, math.nan
+    out, _ = M.prompt_attention(q, k, v, R.cu([400]))
+    out = out.float()
+    assert torch.isfinite(out[:150]).all()
+    assert (out[150:, :, 3] == math.inf).all()
+    assert torch.isnan(out[390:, :, 5]).all() and torch.isfinite(out[:390, :, 5]).all()
+    rest = [i for i in range(128) if i not in (3, 5)]
+    assert torch.isfinite(out[:, :, rest]).all()
+    ref, _, weighted, _ = R.prompt(q, k, torch.nan_to_num(v, 0.0, 0.0, 0.0), [400], [400], True, 128 ** -0.5)
+    off = (out.double() - ref)[:, :, rest].abs() - R.out_bound(ref, weighted, BF16, R.UNIT[BF16])[:, :, rest]
+    assert off.max() <= 0
+
+
 def test_refusals():
     q, k, v = inputs(15, 10, 10, 4, 2, 64, F16)
     at = R.cu([10])
