@@ -434,6 +434,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
     const bs_prompt_attention_desc& d = a.d;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    if (warp == 9 && lane < 3) {
+        const CUtensorMap* map = lane == 0 ? &a.q : lane == 1 ? &a.k : &a.v;
+        if (lane == 0 || d.total_k) asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
+    }
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_addr(&ctl.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
