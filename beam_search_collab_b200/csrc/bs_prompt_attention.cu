@@ -38,6 +38,7 @@
 #include <cstdlib>
 
 #include "bs_device.cuh"
+#include "bs_f32x2.cuh"
 #include "bs_memory.h"
 
 namespace bsb {
@@ -183,21 +184,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("{\n .reg .b64 a, b, c, r;\n mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7}; fma.rn.f32x2 r, a, b, c; mov.b64 {%0, %1}, r;\n}\n"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("{\n .reg .b64 a, b, r;\n mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; add.rn.f32x2 r, a, b; mov.b64 {%0, %1}, r;\n}\n"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-
 template <typename T>
 struct Type16;
 template <>

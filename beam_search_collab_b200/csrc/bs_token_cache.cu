@@ -10,6 +10,7 @@
 #include <cuda_fp16.h>
 
 #include "bs_device.cuh"
+#include "bs_f32x2.cuh"
 #include "bs_memory.h"
 
 namespace bsb {
@@ -18,45 +19,60 @@ using namespace dev;
 
 namespace {
 
+// Two 16-bit values of a word: as floats, and the larger magnitudes of two
+// words' (exact in 16 bits).
 template <typename T>
 __device__ __forceinline__ float2 pair_to_float(uint32_t u);
+template <typename T>
+__device__ __forceinline__ uint32_t larger_magnitudes(uint32_t top, uint32_t u);
 template <>
 __device__ __forceinline__ float2 pair_to_float<__half>(uint32_t u) {
     return __half22float2(*reinterpret_cast<__half2*>(&u));
 }
 template <>
+__device__ __forceinline__ uint32_t larger_magnitudes<__half>(uint32_t top, uint32_t u) {
+    const __half2 h = __hmax2(*reinterpret_cast<__half2*>(&top), __habs2(*reinterpret_cast<__half2*>(&u)));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
 __device__ __forceinline__ float2 pair_to_float<__nv_bfloat16>(uint32_t u) {
     return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&u));
+}
+template <>
+__device__ __forceinline__ uint32_t larger_magnitudes<__nv_bfloat16>(uint32_t top, uint32_t u) {
+    const __nv_bfloat162 h = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&top), __habs2(*reinterpret_cast<__nv_bfloat162*>(&u)));
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 __device__ __forceinline__ uint4 ldg_stream(const void* p) { return __ldcs(static_cast<const uint4*>(p)); }
 
+struct Four {
+    float2 lo, hi;
+};
+
 // Four codes of a word as floats: 0x4b000000 | u is 2^23 + u.
-__device__ __forceinline__ float4 codes_to_floats(uint32_t w) {
+__device__ __forceinline__ Four codes_to_floats(uint32_t w) {
     const uint32_t u = w ^ 0x80808080u;
-    constexpr float kBias = 8388608.f + 128.f;
-    return make_float4(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540)) - kBias,
-                       __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7541)) - kBias,
-                       __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7542)) - kBias,
-                       __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7543)) - kBias);
+    const float2 bias = make_float2(-(8388608.f + 128.f), -(8388608.f + 128.f));
+    return {add2(make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7541))), bias),
+            add2(make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7542)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7543))), bias)};
 }
 
-// rint of four values below 2^22 in magnitude, their low bytes as a word:
-// x + 1.5 * 2^23 rounds to the nearest integer, ties to even.
-__device__ __forceinline__ uint32_t floats_to_codes(float4 x) {
-    constexpr float kMagic = 12582912.f;
-    const uint32_t lo = __byte_perm(__float_as_uint(x.x + kMagic), __float_as_uint(x.y + kMagic), 0x0040);
-    const uint32_t hi = __byte_perm(__float_as_uint(x.z + kMagic), __float_as_uint(x.w + kMagic), 0x0040);
+// Four values times `by` (rounded to 32 bits), rint, their low bytes as a word:
+// a sum with 1.5 * 2^23 rounds to the nearest integer, ties to even.  The
+// products are below 2^22 in magnitude.  (One at a time: a packed product and
+// sum were contracted to one rounding.)
+__device__ __forceinline__ uint32_t floats_to_codes(Four x, float by) {
+    const float2 magic = make_float2(12582912.f, 12582912.f);
+    const float2 a = add2(make_float2(__fmul_rn(x.lo.x, by), __fmul_rn(x.lo.y, by)), magic);
+    const float2 b = add2(make_float2(__fmul_rn(x.hi.x, by), __fmul_rn(x.hi.y, by)), magic);
+    const uint32_t lo = __byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
     return __byte_perm(lo, hi, 0x5410);
 }
 
-// Codes times a ratio of at most 1, rounded (the product first, to 32 bits).
-__device__ __forceinline__ uint32_t rescaled(uint32_t w, float ratio) {
-    const float4 f = codes_to_floats(w);
-    return floats_to_codes(make_float4(__fmul_rn(f.x, ratio), __fmul_rn(f.y, ratio), __fmul_rn(f.z, ratio), __fmul_rn(f.w, ratio)));
-}
-
-__device__ __forceinline__ float clamp127(float x) { return fmaxf(-127.f, fminf(127.f, x)); }
+// Codes times a ratio of at most 1, rounded.
+__device__ __forceinline__ uint32_t rescaled(uint32_t w, float ratio) { return floats_to_codes(codes_to_floats(w), ratio); }
 
 // ------------------------------------------------------------------- write
 
@@ -75,7 +91,7 @@ constexpr int kWriteThreads = 256;
 // its index.  Bound by the chain of loads before the values (lengths, table,
 // values) rather than by bytes, so both tensors' values are requested at once.
 template <typename T, int CHUNKS>
-__global__ void __launch_bounds__(kWriteThreads, 4) k_cache_write(const __grid_constant__ WriteArgs a) {
+__global__ void __launch_bounds__(kWriteThreads, CHUNKS <= 2 ? 4 : CHUNKS == 4 ? 3 : 2) k_cache_write(const __grid_constant__ WriteArgs a) {
     __shared__ float warp_max[2][kWriteThreads / 32];
     __shared__ int32_t found[3];               // cu[b], cu[b + 1], start[b]
     const bs_cache_write_desc& d = a.d;
@@ -140,15 +156,14 @@ __global__ void __launch_bounds__(kWriteThreads, 4) k_cache_write(const __grid_c
     }
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
+        uint32_t most = 0;
 #pragma unroll
         for (int i = 0; i < CHUNKS; ++i) {
-            const uint32_t w[4] = {x[kv][i].x, x[kv][i].y, x[kv][i].z, x[kv][i].w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 f = pair_to_float<T>(w[j]);
-                top[kv] = fmaxf(top[kv], fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
+            most = larger_magnitudes<T>(larger_magnitudes<T>(most, x[kv][i].x), x[kv][i].y);
+            most = larger_magnitudes<T>(larger_magnitudes<T>(most, x[kv][i].z), x[kv][i].w);
         }
+        const float2 two = pair_to_float<T>(most);
+        top[kv] = fmaxf(two.x, two.y);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top[kv] = fmaxf(top[kv], __shfl_xor_sync(kFull, top[kv], o));
         if ((threadIdx.x & 31) == 0) warp_max[kv][threadIdx.x >> 5] = top[kv];
@@ -176,14 +191,10 @@ __global__ void __launch_bounds__(kWriteThreads, 4) k_cache_write(const __grid_c
             const uint32_t chunk = held * per_row + i * kWriteThreads + threadIdx.x;
             if (chunk >= stop * per_row) continue;
             const uint32_t w[4] = {x[kv][i].x, x[kv][i].y, x[kv][i].z, x[kv][i].w};
-            uint32_t code[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const float2 f = pair_to_float<T>(w[2 * j]), g = pair_to_float<T>(w[2 * j + 1]);
-                code[j] = floats_to_codes(make_float4(clamp127(__fmul_rn(f.x, inv)), clamp127(__fmul_rn(f.y, inv)),
-                                                      clamp127(__fmul_rn(g.x, inv)), clamp127(__fmul_rn(g.y, inv))));
-            }
-            reinterpret_cast<uint2*>(codes)[chunk] = make_uint2(code[0], code[1]);
+            // (|x| * inv is at most 127 and a rounding: no clamp)
+            const uint32_t lo = floats_to_codes({pair_to_float<T>(w[0]), pair_to_float<T>(w[1])}, inv);
+            const uint32_t hi = floats_to_codes({pair_to_float<T>(w[2]), pair_to_float<T>(w[3])}, inv);
+            reinterpret_cast<uint2*>(codes)[chunk] = make_uint2(lo, hi);
         }
         if (threadIdx.x == 0) (kv ? a.c.v_scale : a.c.k_scale)[slab] = scale;
     }
@@ -231,11 +242,12 @@ __device__ __forceinline__ void store_values(void* out, uint64_t at, uint4 codes
     __align__(16) T v[16];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float4 f = codes_to_floats(w[j]);
-        v[4 * j] = rounded<T>(f.x * scale);
-        v[4 * j + 1] = rounded<T>(f.y * scale);
-        v[4 * j + 2] = rounded<T>(f.z * scale);
-        v[4 * j + 3] = rounded<T>(f.w * scale);
+        const Four f = codes_to_floats(w[j]);
+        const float2 lo = mul2(f.lo, make_float2(scale, scale)), hi = mul2(f.hi, make_float2(scale, scale));
+        v[4 * j] = rounded<T>(lo.x);
+        v[4 * j + 1] = rounded<T>(lo.y);
+        v[4 * j + 2] = rounded<T>(hi.x);
+        v[4 * j + 3] = rounded<T>(hi.y);
     }
     uint4* p = reinterpret_cast<uint4*>(static_cast<T*>(out) + at);
 #pragma unroll

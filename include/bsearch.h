@@ -319,8 +319,8 @@ BS_API bs_status bs_prompt_attention_workspace(const bs_prompt_attention_desc* d
  * table[b][p / block].  A block's scale is max|x| * (1 / 127) over its new tokens
  * (0 when that maximum is below 1e-30), and where it holds earlier tokens
  * (positions below start[b]) at least the scale it has; those tokens' codes
- * are rounded anew when the scale grows.  code = rint(x * (1 / scale)),
- * clamped to +-127.  Values must be finite.  A block is written by one
+ * are rounded anew when the scale grows.  code = rint(x * (1 / scale))
+ * (+-127 at most).  Values must be finite.  A block is written by one
  * sequence of a call only. */
 typedef struct bs_cache_write_desc {
     const void* k;            /* [total][kv_heads][dim]                       */
