@@ -74,6 +74,10 @@ __device__ __forceinline__ uint32_t floats_to_codes(Four x, float by) {
 // Codes times a ratio of at most 1, rounded.
 __device__ __forceinline__ uint32_t rescaled(uint32_t w, float ratio) { return floats_to_codes(codes_to_floats(w), ratio); }
 
+// x / d for x < 2048 and d <= 16, from reciprocal(d): off by less than x / 2^16.
+__device__ __forceinline__ uint32_t reciprocal(uint32_t d) { return 65536u / d + 1; }
+__device__ __forceinline__ uint32_t divided(uint32_t x, uint32_t by) { return (x * by) >> 16; }
+
 // ------------------------------------------------------------------- write
 
 struct WriteArgs {
@@ -141,6 +145,7 @@ __global__ void __launch_bounds__(kWriteThreads, CHUNKS <= 2 ? 4 : CHUNKS == 4 ?
 
     uint4 x[2][CHUNKS];
     float top[2] = {0.f, 0.f}, old[2];
+    const uint32_t by_row = reciprocal(per_row);
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
         const int64_t* stride = kv ? d.v_stride : d.k_stride;
@@ -151,7 +156,8 @@ __global__ void __launch_bounds__(kWriteThreads, CHUNKS <= 2 ? 4 : CHUNKS == 4 ?
         for (int i = 0; i < CHUNKS; ++i) {
             const uint32_t chunk = held * per_row + i * kWriteThreads + threadIdx.x;
             x[kv][i] = make_uint4(0, 0, 0, 0);
-            if (chunk < stop * per_row) x[kv][i] = ldg_stream(src + (chunk / per_row) * stride[0] + (chunk % per_row) * 8);
+            const uint32_t r = divided(chunk, by_row);
+            if (chunk < stop * per_row) x[kv][i] = ldg_stream(src + r * stride[0] + (chunk - r * per_row) * 8);
         }
     }
 #pragma unroll
@@ -256,13 +262,14 @@ __device__ __forceinline__ void store_values(void* out, uint64_t at, uint4 codes
 
 // One thread: 16 codes of one position's key and value.  (Two or four
 // positions a thread were slower: 62 and 66 us against 56 where 267 MB move.)
+constexpr int kReadThreads = 256;
 template <typename T>
-__global__ void __launch_bounds__(256) k_cache_read(const __grid_constant__ ReadArgs a) {
+__global__ void __launch_bounds__(kReadThreads) k_cache_read(const __grid_constant__ ReadArgs a) {
     const bs_cache_read_desc& d = a.d;
     const uint32_t per_row = a.c.dim / 16, h = blockIdx.y, b = blockIdx.z;
-    const uint64_t unit = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (unit >= static_cast<uint64_t>(d.count) * per_row) return;
-    const uint32_t i = static_cast<uint32_t>(unit / per_row), chunk = static_cast<uint32_t>(unit % per_row);
+    const uint32_t rows = kReadThreads / per_row, r = divided(threadIdx.x, reciprocal(per_row)), chunk = threadIdx.x - r * per_row;
+    const uint32_t i = blockIdx.x * rows + r;
+    if (r >= rows || i >= d.count) return;
     const int32_t pos = d.positions[b * d.position_seq_stride + h * d.position_head_stride + i];
     uint4 kc = make_uint4(0, 0, 0, 0), vc = kc;
     float ks = 0.f, vs = 0.f;
@@ -514,7 +521,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_evict_select(const 
 constexpr int kMoveThreads = 128;      // (256: 53 us for the 268 MB that four long contexts move, 128: 48)
 
 // One CTA: one new block of one head, keys and values.
-__global__ void __launch_bounds__(kMoveThreads) k_evict_move(const EvictArgs a) {
+__global__ void __launch_bounds__(kMoveThreads) k_evict_move(const __grid_constant__ EvictArgs a) {
     __shared__ int64_t from[128];          // row of each token in the codes, -1: none
     __shared__ float scale[2][128];
     __shared__ float top[2];
@@ -522,6 +529,7 @@ __global__ void __launch_bounds__(kMoveThreads) k_evict_move(const EvictArgs a) 
     const uint32_t col = blockIdx.x, h = blockIdx.y, b = blockIdx.z, t = threadIdx.x, block = a.c.block;
     const uint64_t row = static_cast<uint64_t>(b) * a.c.kv_heads + h;
     const uint32_t i0 = col * block;
+    cudaGridDependencySynchronize();       // launched while the selection still runs; in every block
     const uint32_t most = min(d.new_lens[b], d.budget);
     if (i0 >= most) return;
     const uint32_t id = d.new_table[static_cast<uint64_t>(b) * d.new_table_width + col];
@@ -561,25 +569,39 @@ __global__ void __launch_bounds__(kMoveThreads) k_evict_move(const EvictArgs a) 
         }
     }
     __syncthreads();
-    const uint32_t per_row = a.c.dim / 16, units = 2 * block * per_row;
+    for (uint32_t i = t; i < 2 * block; i += kMoveThreads) {       // scales become the ratios of the codes
+        const uint32_t kv = i >= block, x = i - kv * block;
+        scale[kv][x] = top[kv] > 0.f ? __fdiv_rn(scale[kv][x], top[kv]) : 0.f;
+    }
+    __syncthreads();
+    const uint32_t per_row = a.c.dim / 16, units = block * per_row, by_row = reciprocal(per_row);
     constexpr int kBatch = 4;              // loads of a thread in flight
-    for (uint32_t u0 = t; u0 < units; u0 += kBatch * kMoveThreads) {
-        uint4 codes[kBatch];
 #pragma unroll
-        for (int x = 0; x < kBatch; ++x) {
-            const uint32_t u = u0 + x * kMoveThreads, kv = u >= block * per_row, w = u - kv * block * per_row, i = w / per_row;
-            codes[x] = make_uint4(0, 0, 0, 0);
-            if (u < units && from[i] >= 0) codes[x] = ldg_stream((kv ? a.c.v : a.c.k) + from[i] * a.c.dim + w % per_row * 16);
-        }
+    for (uint32_t kv = 0; kv < 2; ++kv) {
+        int8_t* const base = kv ? a.c.v : a.c.k;
+        int8_t* const to = base + slab * block * a.c.dim;
+        for (uint32_t u0 = t; u0 < units; u0 += kBatch * kMoveThreads) {
+            uint4 codes[kBatch];
+            float ratio[kBatch];
 #pragma unroll
-        for (int x = 0; x < kBatch; ++x) {
-            const uint32_t u = u0 + x * kMoveThreads, kv = u >= block * per_row, w = u - kv * block * per_row, i = w / per_row;
-            if (u >= units) break;
-            const float ratio = top[kv] > 0.f ? __fdiv_rn(scale[kv][i], top[kv]) : 0.f;
-            if (ratio != 1.f)
-                codes[x] = make_uint4(rescaled(codes[x].x, ratio), rescaled(codes[x].y, ratio), rescaled(codes[x].z, ratio),
-                                      rescaled(codes[x].w, ratio));
-            *reinterpret_cast<uint4*>((kv ? a.c.v : a.c.k) + slab * block * a.c.dim + w * 16) = codes[x];
+            for (int x = 0; x < kBatch; ++x) {
+                const uint32_t u = u0 + x * kMoveThreads, i = divided(u, by_row);
+                codes[x] = make_uint4(0, 0, 0, 0);
+                ratio[x] = 1.f;
+                if (u < units && from[i] >= 0) {
+                    codes[x] = ldg_stream(base + from[i] * a.c.dim + (u - i * per_row) * 16);
+                    ratio[x] = scale[kv][i];
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < kBatch; ++x) {
+                const uint32_t u = u0 + x * kMoveThreads;
+                if (u >= units) break;
+                if (ratio[x] != 1.f)
+                    codes[x] = make_uint4(rescaled(codes[x].x, ratio[x]), rescaled(codes[x].y, ratio[x]), rescaled(codes[x].z, ratio[x]),
+                                          rescaled(codes[x].w, ratio[x]));
+                *reinterpret_cast<uint4*>(to + u * 16) = codes[x];
+            }
         }
     }
 }
@@ -614,11 +636,11 @@ cudaError_t launch_cache_write(const bs_token_cache& c, const bs_cache_write_des
 cudaError_t launch_cache_read(const bs_token_cache& c, const bs_cache_read_desc& d, const MemoryDevice& dev,
                               cudaStream_t stream) {
     const ReadArgs a{c, d, dev.errors};
-    const uint64_t units = static_cast<uint64_t>(d.count) * (c.dim / 16);
-    const dim3 grid(static_cast<unsigned>((units + 255) / 256), c.kv_heads, d.num_seqs);
-    if (d.dtype == BS_F32) k_cache_read<float><<<grid, 256, 0, stream>>>(a);
-    else if (d.dtype == BS_F16) k_cache_read<__half><<<grid, 256, 0, stream>>>(a);
-    else k_cache_read<__nv_bfloat16><<<grid, 256, 0, stream>>>(a);
+    const uint32_t rows = kReadThreads / (c.dim / 16);       // of a block
+    const dim3 grid((d.count + rows - 1) / rows, c.kv_heads, d.num_seqs);
+    if (d.dtype == BS_F32) k_cache_read<float><<<grid, kReadThreads, 0, stream>>>(a);
+    else if (d.dtype == BS_F16) k_cache_read<__half><<<grid, kReadThreads, 0, stream>>>(a);
+    else k_cache_read<__nv_bfloat16><<<grid, kReadThreads, 0, stream>>>(a);
     return cudaGetLastError();
 }
 
@@ -637,8 +659,7 @@ cudaError_t launch_cache_evict(const bs_token_cache& c, const bs_cache_evict_des
     if (e != cudaSuccess) return e;
     const uint32_t cols = (d.budget + c.block - 1) / c.block;
     const uint32_t used = cols < d.new_table_width ? cols : d.new_table_width;
-    if (used) k_evict_move<<<dim3(used, c.kv_heads, d.num_seqs), kMoveThreads, 0, stream>>>(a);
-    return cudaGetLastError();
+    return used ? launch_after(k_evict_move, dim3(used, c.kv_heads, d.num_seqs), kMoveThreads, stream, a) : cudaSuccess;
 }
 
 }  // namespace bsb
