@@ -39,7 +39,7 @@ namespace {
 constexpr int kWarps = 4;              // per block; they take a segment's tiles in turn
 constexpr int kThreads = kWarps * 32;
 // Tiles a warp has in flight or in use, and resident blocks: 8 query rows fit
-// three blocks with two stages each (35 us for a batch of 76 k tokens and 8
+// three blocks with two stages each (35 us for a batch of 74 k tokens and 8
 // key heads, 37 with two blocks of three stages), 16 rows only two (at three
 // they spill: 56 us against 41).
 template <int NT>
@@ -251,6 +251,12 @@ template <int NW, int NT>
 constexpr size_t kSplitSmem = kWarps * kStagesOf<NT> * kStageBytes<NW> + kJoinBytes<NW, NT> + kWarps * (8 * NT * 2 + 4) * 4 + 128;
 
 // One share of the tiles for one row tile of 8 * NT query rows.
+// Measured (without | with the weights' scores): 16 x 65,536 tokens, 8 key
+// heads of 128, 2.15 GB: 365 | 400 us (copies alone: 344); 32 sequences of 74 k
+// tokens in all 35 us with them; 4 of 54 k in all, 4 drafted tokens each, 41 us
+// without.  Long caches are
+// bound by DRAM (5.4 to 5.9 TB/s); the others by the first and last tiles of
+// the shares and, with 16 query rows, by the instructions of 8 warps an SM.
 // Registers: outputs NW * NT * 4, queries NW * NT * 2, and about 60.
 template <int NW, int NT>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(const __grid_constant__ CacheArgs a) {
@@ -651,6 +657,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(con
 // shares, writes zeros for an empty one.  A lane has four dimensions, the
 // warps take the pieces in turn.  Always the same order of additions.
 // Launched while the first kernel still runs; waits for it before it reads.
+// 5.7 us, most of it a launch and the chain of dependent loads.  Joining inside
+// k_cache_mass instead was not faster: 14.3 us against 5.5 + 8.3 for 32
+// sequences of 74 k tokens, 62 against 51 + 5 for 16 x 65,536.
 constexpr int kJoinThreads = 128;
 __global__ void __launch_bounds__(kJoinThreads) k_cache_join(const __grid_constant__ CacheArgs a, uint32_t tile_rows, uint32_t used_rows) {
     constexpr uint32_t kJoinWarps = kJoinThreads / 32;
@@ -727,7 +736,9 @@ __global__ void __launch_bounds__(kJoinThreads) k_cache_join(const __grid_consta
 }
 
 // One thread per four tokens of a key head: their weights over all query
-// rows, from the scores that the first kernel left and the rows' lse.
+// rows, from the scores that the first kernel left and the rows' lse.  Bound
+// by reading the scores: 45 us for 16 x 65,536 tokens of 32 heads (134 MB of
+// scores, 67 of sums: 4.5 TB/s), 8 us for 74 k tokens.
 constexpr int kMassThreads = 128;
 __global__ void __launch_bounds__(kMassThreads) k_cache_mass(const __grid_constant__ CacheArgs a) {
     const uint32_t j = (blockIdx.x * kMassThreads + threadIdx.x) * 4, h = blockIdx.y, b = blockIdx.z;
