@@ -49,7 +49,7 @@ using namespace dev;
 namespace {
 
 constexpr int kRows = 128;             // query rows of a tile, keys of a tile
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;
 constexpr int kBoxBytes = kRows * 128; // 128 rows of 64 elements
 constexpr unsigned kPolls = 1u << 22;
 constexpr uint32_t kMostChunks = 8;
@@ -374,9 +374,9 @@ struct Item {
 };
 
 struct Control {
-    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], done, raw;
+    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], done;
     uint64_t item_full[2], item_empty[2], next_full;
-    uint64_t full[8], empty[8];
+    uint64_t full[8], empty[8], raw[8];      // raw: values that warp 10 looks at before they are full
     __align__(16) uint32_t next[4]; // the launch control's answer
     Item item[2];
     uint32_t not_finite[8][4];      // by stage: value rows cleared because they are not finite
@@ -448,14 +448,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
             barrier_init(&ctl.p_full[t], 4);
             barrier_init(&ctl.o_full[t], 1);
             barrier_init(&ctl.item_full[t], 1);
-            barrier_init(&ctl.item_empty[t], 9);
+            barrier_init(&ctl.item_empty[t], 11);
         }
         barrier_init(&ctl.done, 1);
-        barrier_init(&ctl.raw, 1);
         barrier_init(&ctl.next_full, 1);
         for (int s = 0; s < kStages; ++s) {
             barrier_init(&ctl.full[s], 1);
             barrier_init(&ctl.empty[s], 1);
+            barrier_init(&ctl.raw[s], 1);
         }
         ctl.keep[0] = ctl.keep[1] = ctl.gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -495,46 +495,65 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
     // columns of key tile j that a row seeing `most` keys sees, to a multiple of 16
     auto columns = [&](int32_t most, int32_t j) { return min(kRows, (most - j * kRows + 15) & ~15); };
 
-    if (warp == 9) {
-        // ------------------------------------------------------------ copies
+    // value rows that a tile of keys has in sight of not all rows of an item
+    auto look = [&](const Item& m, int32_t j) { return m.all_see - j * kRows < kRows; };
+
+    if (warp == 11) {
+        // ------------------------------------------------------------- items
         // Which sequence, tokens and key head a block of the grid stands for:
         // sequence b has the places base(b) .. base(b + 1), base(b) =
         // cu_q[b] / pair + b, enough for its ceil(len / pair) pairs of tiles;
         // the last pair, with the most keys, first.  A place is all key heads,
         // each all chunks.
         const uint32_t pair = 2 * a.tile_tokens;
-        uint32_t stage = 0, phase = 0, raw_phase = 0, next_phase = 0, items = 0, q_used[2] = {0, 0}, loads = 0;
-        uint32_t block = blockIdx.x;
-        bool stop = false;
-        while (!stop) {
-            // (only this block's own place and those not yet started are asked for)
-            if (lane == 0) ask_next(ctl.next, &ctl.next_full);
+        uint32_t block = blockIdx.x, next_phase = 0;
+        bool more = true;
+        for (uint32_t items = 0; more; ++items) {
+            // (one item ahead of the softmax and no more: others may take it)
+            const uint32_t slot = items & 1;
+            if (lane == 0) wait(&ctl.item_empty[slot], ((items >> 1) & 1) ^ 1);
+            __syncwarp();
             Item m;
-            m.valid = 1;
-            m.chunk = block % a.chunks;
-            m.kv_head = block / a.chunks % d.kv_heads;
-            const uint32_t place = block / a.chunks / d.kv_heads;
-            uint32_t lo = 0, hi = d.num_seqs;              // base(lo) <= place, the answer is in [lo, hi)
-            while (hi - lo > 1) {                          // 32 probes at a time
-                const uint32_t step = (hi - lo + 31) / 32, at = lo + lane * step;
-                const bool below = at < hi && (at == 0 || static_cast<uint32_t>(d.cu_q[at]) / pair + at <= place);
-                const int last = 31 - __clz(__ballot_sync(kFull, below) | 1u);
-                hi = min(hi, lo + (last + 1) * step);
-                lo = lo + last * step;
-            }
-            const int32_t q1 = d.cu_q[lo + 1], k1 = d.cu_k[lo + 1];
-            m.q0 = d.cu_q[lo];
-            m.k0 = d.cu_k[lo];
-            m.lq = q1 - m.q0;
-            m.lk = k1 - m.k0;
-            bool work = true;
-            if (m.q0 < 0 || m.lq < 0 || static_cast<uint32_t>(q1) > d.total_q || m.k0 < 0 || m.lk < 0 || static_cast<uint32_t>(k1) > d.total_k) {
-                if (lane == 0) atomicOr(a.errors, kMemErrLength);
-                work = false;
-            }
-            const uint32_t pairs = work ? (m.lq + pair - 1) / pair : 0, local = place - (static_cast<uint32_t>(m.q0) / pair + lo);
-            work = local < pairs;
-            if (work) {
+            m.valid = 0;
+            for (bool own = items == 0; more && !m.valid; own = false) {
+                if (__any_sync(kFull, *gave_up != 0)) more = false;
+                if (more && !own) {
+                    // (only this block's own place and those not yet started are asked for)
+                    if (lane == 0) {
+                        ask_next(ctl.next, &ctl.next_full);
+                        drain(&ctl.next_full, next_phase);
+                    }
+                    __syncwarp();
+                    next_phase ^= 1;
+                    more = read_next(ctl.next, block);
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    __syncwarp();
+                }
+                if (!more) break;
+                m.chunk = block % a.chunks;
+                m.kv_head = block / a.chunks % d.kv_heads;
+                const uint32_t place = block / a.chunks / d.kv_heads;
+                uint32_t lo = 0, hi = d.num_seqs;              // base(lo) <= place, the answer is in [lo, hi)
+                while (hi - lo > 1) {                          // 32 probes at a time
+                    const uint32_t step = (hi - lo + 31) / 32, at = lo + lane * step;
+                    const bool below = at < hi && (at == 0 || static_cast<uint32_t>(d.cu_q[at]) / pair + at <= place);
+                    const int last = 31 - __clz(__ballot_sync(kFull, below) | 1u);
+                    hi = min(hi, lo + (last + 1) * step);
+                    lo = lo + last * step;
+                }
+                const int32_t q1 = d.cu_q[lo + 1], k1 = d.cu_k[lo + 1];
+                m.q0 = d.cu_q[lo];
+                m.k0 = d.cu_k[lo];
+                m.lq = q1 - m.q0;
+                m.lk = k1 - m.k0;
+                bool work = true;
+                if (m.q0 < 0 || m.lq < 0 || static_cast<uint32_t>(q1) > d.total_q || m.k0 < 0 || m.lk < 0 || static_cast<uint32_t>(k1) > d.total_k) {
+                    if (lane == 0) atomicOr(a.errors, kMemErrLength);
+                    work = false;
+                }
+                const uint32_t pairs = work ? (m.lq + pair - 1) / pair : 0, local = place - (static_cast<uint32_t>(m.q0) / pair + lo);
+                if (local >= pairs) continue;
+                m.valid = 1;
                 m.token0 = (pairs - 1 - local) * pair;
                 m.all_see = seen(m.lq, m.lk, m.token0);
                 int32_t tiles[2];
@@ -550,16 +569,92 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                 const int32_t end = static_cast<int32_t>(static_cast<int64_t>(n) * (m.chunk + 1) / chunks);
                 m.end[0] = max(m.first, min(end, tiles[0]));
                 m.end[1] = max(m.first, min(end, tiles[1]));
-                const uint32_t slot = items & 1;
-                if (lane == 0) {
-                    wait(&ctl.item_empty[slot], ((items >> 1) & 1) ^ 1);
-                    if (!*gave_up) {
-                        ctl.item[slot] = m;
-                        barrier_arrive(&ctl.item_full[slot]);
+            }
+            if (lane == 0 && !*gave_up) {
+                ctl.item[slot] = m;
+                barrier_arrive(&ctl.item_full[slot]);
+            }
+            __syncwarp();
+        }
+    } else if (warp == 10) {
+        // ----------------------------------------- value rows that are hidden
+        uint32_t loads = 0, raw_phases = 0;
+        for (uint32_t i = 0;; ++i) {
+            const Item m = next_item(i);
+            if (__any_sync(kFull, *gave_up != 0) || !m.valid) break;
+            item_read(i);
+            const int32_t end = max(m.end[0], m.end[1]);
+#pragma unroll 1
+            for (int32_t j = max(m.first, m.all_see / kRows); j < end; ++j) {
+                // value rows of this tile that not all rows see, and rows past the sequence
+                const int32_t hidden = max(0, m.all_see - j * kRows), past = m.lk - j * kRows;
+                const uint32_t stage = (loads + 2 * (j - m.first) + 1) % kStages;
+                unsigned char* const dst = ring + stage * kTileBytes;
+                wait(&ctl.raw[stage], (raw_phases >> stage) & 1);
+                if (__any_sync(kFull, *gave_up != 0)) break;
+                raw_phases ^= 1u << stage;
+#pragma unroll 1
+                for (int x = 0; x < kRows / 32; ++x) {
+                    const int32_t r = 32 * x + lane;
+                    uint32_t carry = 0;          // an exponent of all ones plus one carries over
+                    if (32 * x + 31 >= hidden && 32 * x < past) {
+#pragma unroll 1
+                        for (int box = 0; box < BOXES; ++box)
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) {
+                                const uint4 w = *reinterpret_cast<const uint4*>(dst + box * kBoxBytes + r * 128 + ((u + lane) & 7) * 16);
+                                constexpr uint32_t e = Type16<T>::kExponent, one = Type16<T>::kExponentOne;
+                                carry |= ((w.x & e) + one) | ((w.y & e) + one) | ((w.z & e) + one) | ((w.w & e) + one);
+                            }
+                    }
+                    const bool odd = (carry & 0x80008000u) && r >= hidden && r < past;
+                    const uint32_t rows = __ballot_sync(kFull, odd);
+                    if (lane == 0) ctl.not_finite[stage][x] = rows;
+                    if (odd || r >= past) {
+#pragma unroll 1
+                        for (int box = 0; box < BOXES; ++box)
+#pragma unroll
+                            for (int u = 0; u < 8; ++u)
+                                *reinterpret_cast<uint4*>(dst + box * kBoxBytes + r * 128 + ((u + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                 }
-                ++items;
-                if (lane == 0) {
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                __syncwarp();
+                if (lane == 0) barrier_arrive(&ctl.full[stage]);
+            }
+            loads += 2 * (end - m.first);
+        }
+    } else if (warp == 9) {
+        // ------------------------------------------------------------ copies
+        // (by lane 0)
+        uint32_t stage = 0, phase = 0, loads = 0, q_used[2] = {0, 0};
+        uint32_t raw = 0, raw_phases = 0;      // a bit a stage: its last load is warp 10's, of which phase
+        for (uint32_t i = 0;; ++i) {
+            const Item m = next_item(i);
+            if (__any_sync(kFull, *gave_up != 0) || !m.valid) break;
+            item_read(i);
+            const int32_t end = max(m.end[0], m.end[1]);
+            if (lane == 0) {
+                for (int32_t u = 0; u < 2 * (end - m.first); ++u) {          // keys, values of a tile
+                    const int32_t j = m.first + (u >> 1);
+                    wait(&ctl.empty[stage], phase ^ 1);
+                    if (*gave_up) break;
+                    uint64_t* bar = &ctl.full[stage];
+                    raw &= ~(1u << stage);
+                    if ((u & 1) && look(m, j)) {
+                        bar = &ctl.raw[stage];
+                        raw |= 1u << stage;
+                        raw_phases ^= 1u << stage;
+                    }
+                    ++loads;
+                    barrier_expect(bar, kTileBytes);
+                    unsigned char* const dst = ring + stage * kTileBytes;
+                    for (int x = 0; x < BOXES; ++x) load_box(dst + x * kBoxBytes, u & 1 ? &a.v : &a.k, 64 * x, m.kv_head, m.k0 + j * kRows, bar);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                    if (u) continue;
                     for (int t = 0; t < 2; ++t) {
                         if (m.end[t] == m.first) continue;
                         wait(&ctl.q_empty[t], (q_used[t] & 1) ^ 1);
@@ -571,84 +666,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                                      m.q0 + m.token0 + t * static_cast<int32_t>(a.tile_tokens), &ctl.q_full[t]);
                     }
                 }
-                for (int32_t j = m.first; j < max(m.end[0], m.end[1]) && !stop; ++j) {
-#pragma unroll
-                    for (int kv = 0; kv < 2; ++kv) {
-                        unsigned char* const dst = ring + stage * kTileBytes;
-                        // value rows of this tile that not all rows see, and rows past the sequence
-                        const int32_t hidden = max(0, m.all_see - j * kRows), past = m.lk - j * kRows;
-                        const bool look = kv == 1 && hidden < kRows;
-                        if (lane == 0) wait(&ctl.empty[stage], phase ^ 1);
-                        stop = __shfl_sync(kFull, *gave_up, 0) != 0;
-                        if (stop) break;
-                        ++loads;
-                        if (lane == 0) {
-                            uint64_t* const bar = look ? &ctl.raw : &ctl.full[stage];
-                            barrier_expect(bar, kTileBytes);
-                            for (int x = 0; x < BOXES; ++x)
-                                load_box(dst + x * kBoxBytes, kv ? &a.v : &a.k, 64 * x, m.kv_head, m.k0 + j * kRows, bar);
-                            if (look) drain(&ctl.raw, raw_phase);
-                        }
-                        __syncwarp();
-                        if (look) {
-                            raw_phase ^= 1;
-#pragma unroll 1
-                            for (int i = 0; i < kRows / 32; ++i) {
-                                const int32_t r = 32 * i + lane;
-                                uint32_t carry = 0;          // an exponent of all ones plus one carries over
-                                if (32 * i + 31 >= hidden && 32 * i < past) {
-#pragma unroll 1
-                                    for (int x = 0; x < BOXES; ++x)
-#pragma unroll
-                                        for (int u = 0; u < 8; ++u) {
-                                            const uint4 w = *reinterpret_cast<const uint4*>(dst + x * kBoxBytes + r * 128 + ((u + lane) & 7) * 16);
-                                            constexpr uint32_t e = Type16<T>::kExponent, one = Type16<T>::kExponentOne;
-                                            carry |= ((w.x & e) + one) | ((w.y & e) + one) | ((w.z & e) + one) | ((w.w & e) + one);
-                                        }
-                                }
-                                const bool odd = (carry & 0x80008000u) && r >= hidden && r < past;
-                                const uint32_t rows = __ballot_sync(kFull, odd);
-                                if (lane == 0) ctl.not_finite[stage][i] = rows;
-                                if (odd || r >= past) {
-#pragma unroll 1
-                                    for (int x = 0; x < BOXES; ++x)
-#pragma unroll
-                                        for (int u = 0; u < 8; ++u)
-                                            *reinterpret_cast<uint4*>(dst + x * kBoxBytes + r * 128 + ((u + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
-                                }
-                            }
-                            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                            __syncwarp();
-                            if (lane == 0) barrier_arrive(&ctl.full[stage]);
-                        }
-                        if (++stage == kStages) {
-                            stage = 0;
-                            phase ^= 1;
-                        }
-                    }
-                }
             }
-            // (whatever happened: an answer on its way is waited for)
-            if (lane == 0) drain(&ctl.next_full, next_phase);
             __syncwarp();
-            next_phase ^= 1;
-            const bool more = read_next(ctl.next, block);
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            __syncwarp();
-            stop = __shfl_sync(kFull, stop || *gave_up != 0, 0);
-            if (!more) break;
         }
         if (lane == 0) {
-            const uint32_t slot = items & 1;
-            wait(&ctl.item_empty[slot], ((items >> 1) & 1) ^ 1);
-            if (!*gave_up) {
-                ctl.item[slot].valid = 0;
-                barrier_arrive(&ctl.item_full[slot]);
-            }
             // no copy may be in flight when the block ends
             for (int t = 0; t < 2; ++t)
                 if (q_used[t]) drain(&ctl.q_full[t], (q_used[t] - 1) & 1);
-            for (uint32_t i = loads > kStages ? loads - kStages : 0; i < loads; ++i) drain(&ctl.full[i % kStages], (i / kStages) & 1);
+            for (uint32_t i = loads > kStages ? loads - kStages : 0; i < loads; ++i) {
+                const uint32_t s = i % kStages;
+                if ((raw >> s) & 1) drain(&ctl.raw[s], ((raw_phases >> s) & 1) ^ 1);
+                else drain(&ctl.full[s], (i / kStages) & 1);
+            }
         }
         __syncwarp();
     } else if (warp == 8) {
