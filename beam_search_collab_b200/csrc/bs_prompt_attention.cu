@@ -374,7 +374,7 @@ struct Item {
 };
 
 struct Control {
-    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], done;
+    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], done, asked;
     uint64_t item_full[2], item_empty[2], next_full;
     uint64_t full[8], empty[8], raw[8];      // raw: values that warp 10 looks at before they are full
     __align__(16) uint32_t next[4]; // the launch control's answer
@@ -452,6 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
         }
         barrier_init(&ctl.done, 1);
         barrier_init(&ctl.next_full, 1);
+        barrier_init(&ctl.asked, 1);
         for (int s = 0; s < kStages; ++s) {
             barrier_init(&ctl.full[s], 1);
             barrier_init(&ctl.empty[s], 1);
@@ -509,9 +510,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
         uint32_t block = blockIdx.x, next_phase = 0;
         bool more = true;
         for (uint32_t items = 0; more; ++items) {
-            // (one item ahead of the softmax and no more: others may take it)
+            // The next block of the grid is asked for when all of this one's
+            // copies are, not before: others may have nothing left to do.
             const uint32_t slot = items & 1;
-            if (lane == 0) wait(&ctl.item_empty[slot], ((items >> 1) & 1) ^ 1);
+            if (lane == 0) {
+                wait(&ctl.item_empty[slot], ((items >> 1) & 1) ^ 1);
+                if (items) wait(&ctl.asked, (items - 1) & 1);
+            }
             __syncwarp();
             Item m;
             m.valid = 0;
@@ -666,6 +671,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                                      m.q0 + m.token0 + t * static_cast<int32_t>(a.tile_tokens), &ctl.q_full[t]);
                     }
                 }
+                barrier_arrive(&ctl.asked);
             }
             __syncwarp();
         }
