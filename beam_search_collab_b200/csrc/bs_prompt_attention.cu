@@ -11,7 +11,8 @@
 // are cut into chunks and a second kernel joins them.
 //
 // Warps 0-3 and 4-7 are the softmax of tile 0 and 1 (a thread has one row),
-// warp 8 issues the matrix instructions, warp 9 the copies:
+// warp 8 issues the matrix instructions, warp 9 the copies, warp 10 looks at
+// hidden values, warp 11 finds the next item:
 //   copies    query tiles, then keys and values through one ring of stages
 //             (tiled TMA, 128-byte swizzle, 64 columns of a row at a time)
 //   matrix    S_t = Q_t K^T    (both K-major in shared memory, S_t in TMEM)
@@ -27,7 +28,7 @@
 //
 // Keys of other sequences or of the future that a tile also covers are set to
 // -infinity in S.  A zero weight would still pass an infinity or NaN of a
-// hidden VALUE on, so in tiles with hidden keys the copying warp clears value
+// hidden VALUE on, so in tiles with hidden keys warp 10 clears value
 // rows past the sequence, and rows that are not finite and not seen by all;
 // the softmax adds the latter for the rows that see them (never taken with
 // finite inputs).
@@ -413,14 +414,18 @@ __device__ __forceinline__ bool read_next(const void* answer, uint32_t& block) {
 // Work: 4 * dim operations per query head and visible pair.  Measured: one
 // prompt of 16,384 tokens, 16/4 heads of 128, 0.90 ms (1.22 PFLOP/s; a large
 // matrix product reaches 1.65 here); 13 prompts of 7,196 tokens in all, 32/8
-// heads, 116 us (0.58); 24 tokens 7 us.  On long prompts the tensor pipe is
+// heads, 110 us (0.61); 24 tokens 7 us.  On long prompts the tensor pipe is
 // busy 53% of the cycles and the exponentials' pipe 53%: what bounds it is the
 // chain S -> weights -> P V of each tile, which only the other tile hides (a
 // pair of tiles of keys takes 3,450 clocks, its products 2,048).  On short
-// ones it is each item's first and last tile and epilogue (about 4,000
-// clocks).  Not kept, at 16,384 tokens and the 13 prompts: two blocks of one
-// tile an SM 1.12 ms and 130 us; weights handed over in halves 1.03 ms; part
-// of the exponentials as a polynomial, slower at every share.
+// ones it is also each item's last tile, with hidden keys (3,800 clocks), and
+// its outputs (3,700).  Not kept, at 16,384 tokens and the 13 prompts: two
+// blocks of one tile an SM 1.12 ms and 130 us; weights handed over in halves
+// 1.03 ms; scores in halves too, the next ones made meanwhile, 1.16 ms and 120
+// us; part of the exponentials as a polynomial, slower at every share; outputs
+// by tensor copies 115 us.  With the copying warp also finding items and
+// looking at hidden values, and items taken one ahead, the 13 prompts took 117
+// us and 11 of 3,888 tokens 39 (now 29).
 template <typename T, int BOXES>
 __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ PromptArgs a) {
     extern __shared__ unsigned char raw_smem[];
@@ -1005,9 +1010,10 @@ uint64_t most_items(const bs_prompt_attention_desc& d) {
 // traffic (4 TB/s); the time is that of the longest item, or of all of them
 // over the SMs.  Lengths are not known here: the longest sequence is taken to
 // have twice the average's keys, a query half of its own piece of prompt.
-// Measured, in 1, 2, 4, 8 pieces: 3 of 12/4 heads, 8,000 keys 77, 58, 55, 56 us
-// (4 taken); 8 of one key head, 5,800 keys 72, 46, 32, 30 (4); 16 short ones over
-// 6,500 keys 39, 27, 21, 23 (4); 1,109 tokens of 18/3 heads 28, 36, 37, 44 (1).
+// Measured, in 1, 2, 4, 8 pieces (when items were still taken one ahead): 3
+// sequences of 12/4 heads, 8,000 keys 77, 58, 55, 56 us (4 taken); 8 of one key
+// head, 5,800 keys 72, 46, 32, 30 (4); 16 short ones over 6,500 keys 39, 27, 21,
+// 23 (4); 1,109 tokens of 18/3 heads 28, 36, 37, 44 (1).
 uint32_t chunks_of(const bs_prompt_attention_desc& d, const MemoryDevice& dev) {
     const double items = static_cast<double>(most_items(d)), seqs = d.num_seqs ? d.num_seqs : 1;
     const double total = d.total_k / static_cast<double>(kRows), most = std::min(total, 2 * total / seqs) + 1;
