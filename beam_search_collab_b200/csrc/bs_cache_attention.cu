@@ -268,6 +268,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(con
     float* join_ml = join_o + 2 * kRows * kDim;                 // [warps][kRows][2]
     uint64_t* sums = reinterpret_cast<uint64_t*>(smem);         // before the ring is used
 
+    cudaGridDependencySynchronize();       // in every block, before anything of the caller's
     // this block's share, and the piece it begins with
     const uint32_t hkv = a.c.kv_heads, row0 = blockIdx.y * kRows;
     Piece at;
@@ -823,8 +824,7 @@ template <int NW, int NT>
 cudaError_t launch_split(const CacheArgs& a, uint32_t row_tiles, cudaStream_t stream) {
     const cudaError_t e = cudaFuncSetAttribute(k_cache_split<NW, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitSmem<NW, NT>);
     if (e != cudaSuccess) return e;
-    k_cache_split<NW, NT><<<dim3(a.shares, row_tiles), kThreads, kSplitSmem<NW, NT>, stream>>>(a);
-    return cudaGetLastError();
+    return launch_after(k_cache_split<NW, NT>, dim3(a.shares, row_tiles), kThreads, kSplitSmem<NW, NT>, stream, a);
 }
 
 template <int NT>
@@ -866,10 +866,10 @@ cudaError_t launch_cache_attention(const bs_token_cache& c, const bs_cache_atten
     if (l.shares) e = l.nt == 1 ? launch_split<1>(a, l.row_tiles, stream) : launch_split<2>(a, l.row_tiles, stream);
     if (e != cudaSuccess) return e;
     const uint32_t tile_rows = 8 * l.nt, used_rows = a.rows < tile_rows ? a.rows : tile_rows;
-    if (!l.direct) e = launch_after(k_cache_join, dim3(c.kv_heads * used_rows, l.row_tiles, d.num_seqs), kJoinThreads, stream, a, tile_rows, used_rows);
+    if (!l.direct) e = launch_after(k_cache_join, dim3(c.kv_heads * used_rows, l.row_tiles, d.num_seqs), kJoinThreads, 0, stream, a, tile_rows, used_rows);
     if (e == cudaSuccess && d.out_mass)
         e = launch_after(k_cache_mass, dim3((d.mass_width + 4 * kMassThreads - 1) / (4 * kMassThreads), c.kv_heads, d.num_seqs),
-                         kMassThreads, stream, a);
+                         kMassThreads, 0, stream, a);
     return e;
 }
 

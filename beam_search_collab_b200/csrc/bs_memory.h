@@ -44,16 +44,18 @@ cudaError_t launch_cache_evict(const bs_token_cache& c, const bs_cache_evict_des
                                cudaStream_t stream);
 
 #ifdef __CUDACC__
-// A kernel that may start while the one before it on the stream still runs
-// (and waits for it by itself, in every block).
+// A kernel that may start while the one before it on the stream still runs,
+// whosever that is, and waits for it by itself, in every block, before it reads
+// or writes anything.
 template <typename... Params, typename... Given>
-cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, Given... given) {
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, int threads, size_t shared, cudaStream_t stream, Given... given) {
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
     config.gridDim = grid;
     config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared;
     config.stream = stream;
     config.attrs = &attr;
     config.numAttrs = 1;

@@ -470,6 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
     __syncthreads();
     fence_after();
     const uint32_t tmem = ctl.tmem;
+    cudaGridDependencySynchronize();       // nothing before this reads or writes a caller's memory
 
     // A bounded wait.  Once one has given up none waits any more: the warps
     // leave their loops together, what is in flight is waited for (`drain`,
@@ -1037,11 +1038,10 @@ cudaError_t launch(const PromptArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     const uint64_t blocks = most_items(a.d) * a.chunks;
     if (blocks > 0x7fffffffu) return cudaErrorInvalidConfiguration;
-    k_prompt<T, BOXES><<<static_cast<unsigned>(blocks), kThreads, kSmem<BOXES>, stream>>>(a);
-    e = cudaGetLastError();
+    e = launch_after(k_prompt<T, BOXES>, dim3(static_cast<unsigned>(blocks)), kThreads, kSmem<BOXES>, stream, a);
     if (e != cudaSuccess || a.chunks == 1) return e;
     const uint64_t rows = static_cast<uint64_t>(a.d.total_q) * a.d.q_heads;
-    return launch_after(k_prompt_join, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, stream, a);
+    return launch_after(k_prompt_join, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream, a);
 }
 
 }  // namespace

@@ -105,6 +105,7 @@ __global__ void __launch_bounds__(kWriteThreads, CHUNKS <= 2 ? 4 : CHUNKS == 4 ?
     // heads side by side: their rows are side by side in k and v
     const uint32_t h = blockIdx.x % a.c.kv_heads, place = blockIdx.x / a.c.kv_heads;
 
+    cudaGridDependencySynchronize();       // in every block, before anything of the caller's
     uint32_t at_or_below = 0;
     for (uint32_t b0 = 0; b0 < d.num_seqs; b0 += kWriteThreads) {
         const uint32_t i = b0 + threadIdx.x;
@@ -214,11 +215,10 @@ cudaError_t write_typed(const WriteArgs& a, cudaStream_t stream) {
     const uint64_t blocks = (a.d.total / a.c.block + 2ull * a.d.num_seqs + 1) * a.c.kv_heads;
     if (blocks > 0x7fffffffu) return cudaErrorInvalidConfiguration;
     const unsigned grid = static_cast<unsigned>(blocks);
-    if (chunks <= kWriteThreads) k_cache_write<T, 1><<<grid, kWriteThreads, 0, stream>>>(a);
-    else if (chunks <= 2 * kWriteThreads) k_cache_write<T, 2><<<grid, kWriteThreads, 0, stream>>>(a);
-    else if (chunks <= 4 * kWriteThreads) k_cache_write<T, 4><<<grid, kWriteThreads, 0, stream>>>(a);
-    else k_cache_write<T, 8><<<grid, kWriteThreads, 0, stream>>>(a);
-    return cudaGetLastError();
+    if (chunks <= kWriteThreads) return launch_after(k_cache_write<T, 1>, dim3(grid), kWriteThreads, 0, stream, a);
+    if (chunks <= 2 * kWriteThreads) return launch_after(k_cache_write<T, 2>, dim3(grid), kWriteThreads, 0, stream, a);
+    if (chunks <= 4 * kWriteThreads) return launch_after(k_cache_write<T, 4>, dim3(grid), kWriteThreads, 0, stream, a);
+    return launch_after(k_cache_write<T, 8>, dim3(grid), kWriteThreads, 0, stream, a);
 }
 
 // -------------------------------------------------------------------- read
@@ -272,6 +272,7 @@ __global__ void __launch_bounds__(kReadThreads) k_cache_read(const __grid_consta
     const uint32_t per_row = a.c.dim / 16, h = blockIdx.y, b = blockIdx.z;
     const uint32_t rows = kReadThreads / per_row, r = divided(threadIdx.x, reciprocal(per_row)), chunk = threadIdx.x - r * per_row;
     const uint32_t i = blockIdx.x * rows + r;
+    cudaGridDependencySynchronize();       // in every block, before anything of the caller's
     if (r >= rows || i >= d.count) return;
     const int32_t pos = d.positions[b * d.position_seq_stride + h * d.position_head_stride + i];
     uint4 kc = make_uint4(0, 0, 0, 0), vc = kc;
@@ -356,6 +357,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_evict_select(const 
     __shared__ uint32_t warp_sums[32];
     __shared__ uint32_t slice_counts[2];           // tokens that stay for certain, tokens equal to the threshold
     __shared__ uint32_t chosen[2];
+    cudaGridDependencySynchronize();       // in every block, before anything of the caller's
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = cluster.block_rank(), blocks = cluster.num_blocks();
     const bs_cache_evict_desc& d = a.d;
@@ -617,17 +619,19 @@ cudaError_t launch_select(const EvictArgs& a, uint32_t cluster, cudaStream_t str
     const uint32_t slice = ((a.d.mass_width + cluster - 1) / cluster + 3) & ~3u, cached = slice < kMostCached ? slice : kMostCached;
     cudaError_t e = cudaFuncSetAttribute(k_evict_select<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostCached * 4);
     if (e != cudaSuccess) return e;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(a.c.kv_heads * cluster, a.d.num_seqs);
     config.blockDim = dim3(THREADS);
     config.dynamicSmemBytes = cached * 4;
     config.stream = stream;
-    config.attrs = &attr;
-    config.numAttrs = 1;
+    config.attrs = attr;
+    config.numAttrs = 2;
     return cudaLaunchKernelEx(&config, k_evict_select<THREADS>, a, cached);
 }
 
@@ -644,10 +648,9 @@ cudaError_t launch_cache_read(const bs_token_cache& c, const bs_cache_read_desc&
     const ReadArgs a{c, d, dev.errors};
     const uint32_t rows = kReadThreads / (c.dim / 16);       // of a block
     const dim3 grid((d.count + rows - 1) / rows, c.kv_heads, d.num_seqs);
-    if (d.dtype == BS_F32) k_cache_read<float><<<grid, kReadThreads, 0, stream>>>(a);
-    else if (d.dtype == BS_F16) k_cache_read<__half><<<grid, kReadThreads, 0, stream>>>(a);
-    else k_cache_read<__nv_bfloat16><<<grid, kReadThreads, 0, stream>>>(a);
-    return cudaGetLastError();
+    if (d.dtype == BS_F32) return launch_after(k_cache_read<float>, grid, kReadThreads, 0, stream, a);
+    if (d.dtype == BS_F16) return launch_after(k_cache_read<__half>, grid, kReadThreads, 0, stream, a);
+    return launch_after(k_cache_read<__nv_bfloat16>, grid, kReadThreads, 0, stream, a);
 }
 
 size_t cache_evict_scratch(const bs_token_cache&, const bs_cache_evict_desc&, const MemoryDevice&) { return 0; }
@@ -665,7 +668,7 @@ cudaError_t launch_cache_evict(const bs_token_cache& c, const bs_cache_evict_des
     if (e != cudaSuccess) return e;
     const uint32_t cols = (d.budget + c.block - 1) / c.block;
     const uint32_t used = cols < d.new_table_width ? cols : d.new_table_width;
-    return used ? launch_after(k_evict_move, dim3(used, c.kv_heads, d.num_seqs), kMoveThreads, stream, a) : cudaSuccess;
+    return used ? launch_after(k_evict_move, dim3(used, c.kv_heads, d.num_seqs), kMoveThreads, 0, stream, a) : cudaSuccess;
 }
 
 }  // namespace bsb
