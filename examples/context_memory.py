@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import os
 import sys
+from dataclasses import dataclass
 
 import numpy as np
 import torch
@@ -33,10 +34,20 @@ def rows_for_search(keys: np.ndarray) -> np.ndarray:
     return np.concatenate((keys, np.sqrt(squares.max() - squares)[:, None]), 1).astype(np.float32)
 
 
+@dataclass
+class Archive:
+    """What one eviction gave up: an index a head over its keys, whose row i is
+    position gone[head, i] of the `lens` tokens that `table`'s blocks held."""
+    indexes: list[B.Index]
+    gone: torch.Tensor
+    table: torch.Tensor
+    lens: torch.Tensor
+
+
 class ContextMemory:
-    """The tokens of one sequence: `table` and `lens` say which of `cache`'s
-    blocks hold the recent ones and those that got much attention, `archive`
-    which held everything before the eviction."""
+    """The tokens of one sequence: `table` and `tokens` say which of `cache`'s
+    blocks hold the recent ones and those that got much attention, `archives`
+    (one an eviction) where the others are."""
 
     def __init__(self, room: int):
         self.cache = memory.TokenCache.empty(-(-room // BLOCK), HEADS, DIM, BLOCK)
@@ -44,7 +55,7 @@ class ContextMemory:
         self.table = torch.empty((1, 0), dtype=torch.int32, device="cuda")
         self.tokens = 0
         self.mass = None
-        self.indexes: list[B.Index] = []
+        self.archives: list[Archive] = []
 
     def blocks(self, tokens: int) -> torch.Tensor:
         n = -(-tokens // BLOCK)
@@ -72,44 +83,51 @@ class ContextMemory:
         return out[0, 0], lse[0, 0]
 
     def evict(self, budget: int, recent: int) -> None:
-        """Down to `budget` tokens a head; the others become rows of an index."""
+        """Down to `budget` tokens a head; the others become rows of an index of
+        this eviction's own."""
         lens = torch.tensor([self.tokens], dtype=torch.int32, device="cuda")
         new_table = self.blocks(budget)
         kept, new_lens, new_mass = self.cache.evict(self.mass, self.table, lens, new_table, budget, sinks=4, recent=recent)
         gone = torch.ones((HEADS, self.tokens), dtype=torch.bool, device="cuda").scatter_(1, kept[0].long(), False)
-        self.gone = torch.stack([g.nonzero()[:, 0] for g in gone]).to(torch.int32)
-        self.archive, self.archived = self.table, lens
-        keys, _ = self.cache.read(self.archive, lens, self.gone[None], values=False)
-        for h in range(HEADS):
-            self.indexes.append(B.Index.from_vectors(rows_for_search(keys[0, h].cpu().numpy()), degree=32))
-            self.indexes[-1].build_graph(beam_width=64)
+        gone = torch.stack([g.nonzero()[:, 0] for g in gone]).to(torch.int32)
+        keys, _ = self.cache.read(self.table, lens, gone[None], values=False)
+        indexes = [B.Index.from_vectors(rows_for_search(keys[0, h].cpu().numpy()), degree=32) for h in range(HEADS)]
+        for ix in indexes:
+            ix.build_graph(beam_width=64)
+        self.archives.append(Archive(indexes, gone, self.table, lens))
         self.table, self.mass, self.tokens = new_table, new_mass, budget
 
     def recall(self, q, k: int):
-        """Attention of q over the `k` evicted tokens of each query head's
-        nearest keys (every query head of a key head sees them all)."""
+        """Attention of q over the evicted tokens: of each eviction the `k`
+        nearest keys of each query head (every query head of a key head sees
+        them all)."""
         queries = torch.nn.functional.pad(q.float().view(HEADS, GROUP, DIM), (0, 1))
         torch.cuda.current_stream().synchronize()      # the search runs on the default stream
-        places = []
-        for h in range(HEADS):
-            ids, _, _ = self.indexes[h].search(queries[h].contiguous(), mode="warp4", K=k, topk_size=max(64, 2 * k))
-            found = torch.unique(ids[ids >= 0].long())
-            places.append(self.gone[h][found])
-        n = [len(p) for p in places]
-        table = torch.full((HEADS, max(n)), -1, dtype=torch.int32, device="cuda")
-        for h in range(HEADS):
-            table[h, :n[h]] = places[h]
-        keys, values = self.cache.read(self.archive, self.archived, table[None], dtype=q.dtype)
-        pick = lambda x: torch.cat([x[0, h, :n[h]] for h in range(HEADS)])[:, None]  # noqa: E731
+        found = [([], []) for _ in range(HEADS)]       # of each head: keys, values
+        for a in self.archives:
+            places = []
+            for h in range(HEADS):
+                ids, _, _ = a.indexes[h].search(queries[h].contiguous(), mode="warp4", K=k, topk_size=max(64, 2 * k))
+                places.append(a.gone[h][torch.unique(ids[ids >= 0].long())])
+            n = [len(p) for p in places]
+            table = torch.full((HEADS, max(n)), -1, dtype=torch.int32, device="cuda")
+            for h in range(HEADS):
+                table[h, :n[h]] = places[h]
+            for x, into in zip(self.cache.read(a.table, a.lens, table[None], dtype=q.dtype), (0, 1)):
+                for h in range(HEADS):
+                    found[h][into].append(x[0, h, :n[h]])
         # one sequence for each key head: its query heads over what they found
+        keys, values = (torch.cat([x for h in range(HEADS) for x in found[h][i]])[:, None] for i in (0, 1))
+        n = [sum(map(len, found[h][0])) for h in range(HEADS)]
         at = lambda x: torch.tensor(np.cumsum([0] + x), dtype=torch.int32, device="cuda")  # noqa: E731
-        out, lse = memory.prompt_attention(q.view(HEADS, GROUP, DIM), pick(keys), pick(values), at([1] * HEADS), at(n),
-                                           causal=False, with_lse=True)
+        out, lse = memory.prompt_attention(q.view(HEADS, GROUP, DIM), keys, values, at([1] * HEADS), at(n), causal=False,
+                                           with_lse=True)
         return out.reshape(HEADS * GROUP, DIM), lse.reshape(-1)
 
     def close(self) -> None:
-        for ix in self.indexes:
-            ix.close()
+        for a in self.archives:
+            for ix in a.indexes:
+                ix.close()
 
 
 def run(tokens: int = 6000, steps: int = 24, budget: int = 512, found: int = 32, seed: int = 0) -> dict:
@@ -153,7 +171,7 @@ def run(tokens: int = 6000, steps: int = 24, budget: int = 512, found: int = 32,
             errors[name] += float((got.float() - want).norm() / want.norm()) / steps
     flags = memory.take_errors()
     m.close()
-    return {"prompt": prompt_out, "errors": errors, "evicted": int(m.gone.shape[1]), "flags": flags}
+    return {"prompt": prompt_out, "errors": errors, "evicted": sum(int(a.gone.shape[1]) for a in m.archives), "flags": flags}
 
 
 if __name__ == "__main__":
