@@ -84,7 +84,9 @@ class ContextMemory:
 
     def evict(self, budget: int, recent: int) -> None:
         """Down to `budget` tokens a head; the others become rows of an index of
-        this eviction's own."""
+        this eviction's own.  Nothing to do where there are no more tokens."""
+        if self.tokens <= budget:
+            return
         lens = torch.tensor([self.tokens], dtype=torch.int32, device="cuda")
         new_table = self.blocks(budget)
         kept, new_lens, new_mass = self.cache.evict(self.mass, self.table, lens, new_table, budget, sinks=4, recent=recent)
@@ -100,7 +102,9 @@ class ContextMemory:
     def recall(self, q, k: int):
         """Attention of q over the evicted tokens: of each eviction the `k`
         nearest keys of each query head (every query head of a key head sees
-        them all)."""
+        them all).  Nothing evicted: zeros, whose log-sum is -infinity."""
+        if not self.archives:
+            return torch.zeros_like(q), torch.full((HEADS * GROUP,), -torch.inf, device="cuda")
         queries = torch.nn.functional.pad(q.float().view(HEADS, GROUP, DIM), (0, 1))
         torch.cuda.current_stream().synchronize()      # the search runs on the default stream
         found = [([], []) for _ in range(HEADS)]       # of each head: keys, values

@@ -5,6 +5,8 @@ import sys
 import pytest
 import torch
 
+from beam_search_collab_b200 import memory
+
 pytestmark = pytest.mark.gpu
 
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
@@ -36,4 +38,21 @@ def test_tokens_of_every_eviction_are_recalled():
         out, _ = m.recall(q, 16)
         want = v[at].float().repeat_interleave(C.GROUP, 0)
         assert (out.float() - want).abs().max() < 0.1, at       # (steps of the 8-bit codes are 0.03)
+    m.close()
+
+
+@pytest.mark.parametrize("tokens", [40, 64])
+def test_a_cache_within_its_budget_is_left_alone(tokens):
+    import context_memory as C
+    g = torch.Generator("cuda").manual_seed(48)
+    m = C.ContextMemory(400)
+    k, v = (torch.randn((tokens, C.HEADS, C.DIM), generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    m.append(k, v)
+    before = m.attend(k[0].repeat_interleave(C.GROUP, 0))
+    m.evict(64, recent=8)
+    assert m.tokens == tokens and not m.archives
+    q = k[0].repeat_interleave(C.GROUP, 0)
+    assert all(torch.equal(a, b) for a, b in zip(before, m.attend(q)))
+    out, lse = memory.merge(*zip(before, m.recall(q, 16)))
+    assert torch.equal(out, before[0]) and torch.allclose(lse, before[1])
     m.close()
