@@ -64,21 +64,31 @@ void strides(const Tensor& t, int64_t (&out)[N]) {
     for (size_t i = 0; i < N; ++i) out[i] = t.size(i) > 1 ? t.stride(i) : 0;
 }
 
-// The stream a call goes to.  Memory that PyTorch gave out for its current
-// stream is marked as used on another one.
+// The stream a call goes to, made PyTorch's current one for as long as the
+// call lasts: memory that it asks for is then free on that stream, where its
+// kernels run.  Where the caller's current stream is another, PyTorch is told
+// who else uses what.
 struct Target {
-    c10::cuda::CUDAGuard guard;
-    c10::cuda::CUDAStream current;
+    c10::cuda::CUDAGuard device;
+    c10::cuda::CUDAStream callers;
     cudaStream_t stream;
-    Target(at::Device device, std::optional<uint64_t> handle)
-        : guard(device), current(c10::cuda::getCurrentCUDAStream(device.index())), stream(current.stream()) {
-        if (handle) stream = reinterpret_cast<cudaStream_t>(*handle);
+    c10::cuda::OptionalCUDAStreamGuard guard;
+    Target(at::Device on, std::optional<uint64_t> handle)
+        : device(on), callers(c10::cuda::getCurrentCUDAStream(on.index())), stream(callers.stream()) {
+        if (!handle || reinterpret_cast<cudaStream_t>(*handle) == stream) return;
+        stream = reinterpret_cast<cudaStream_t>(*handle);
+        guard.reset_stream(stream ? c10::cuda::getStreamFromExternal(stream, on.index()) : c10::cuda::getDefaultCUDAStream(on.index()));
     }
-    void used(std::initializer_list<const Tensor*> made) const {
-        if (stream == current.stream()) return;
-        const c10::cuda::CUDAStream other = stream ? c10::cuda::getStreamFromExternal(stream, current.device_index())
-                                                   : c10::cuda::getDefaultCUDAStream(current.device_index());
-        for (const Tensor* t : made)
+    // Tensors of the caller that the kernels use: freed, they are not given
+    // out again before the kernels are done.
+    void uses(std::initializer_list<const Tensor*> given) const { record(given, c10::cuda::getCurrentCUDAStream(callers.device_index())); }
+    // Tensors made here that the caller's stream will use.
+    void gives(std::initializer_list<const Tensor*> made) const { record(made, callers); }
+
+private:
+    void record(std::initializer_list<const Tensor*> tensors, c10::cuda::CUDAStream other) const {
+        if (stream == callers.stream()) return;
+        for (const Tensor* t : tensors)
             if (t->defined()) t->record_stream(other);
     }
 };
@@ -127,7 +137,8 @@ py::tuple prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, co
     d.workspace = bytes ? work.data_ptr() : nullptr;
     d.workspace_bytes = bytes;
     check(bs_prompt_attention(&d, to.stream));
-    to.used({&out, &lse, &work});
+    to.uses({&q, &k, &v, &cu_q, &cu_k});
+    to.gives({&out, &lse});
     return py::make_tuple(out, maybe(lse));
 }
 
@@ -175,6 +186,7 @@ struct Cache {
         d.table_width = table.size(1);
         d.dtype = type_of(x);
         check(bs_cache_write(&c, &d, to.stream));
+        to.uses({&k, &v, &k_scale, &v_scale, &x, &y, &cu, &table, &start});
     }
 
     py::tuple read(const Tensor& table, const Tensor& lens, const Tensor& positions, at::ScalarType dtype, bool keys, bool values,
@@ -203,7 +215,8 @@ struct Cache {
         d.count = positions.size(-1);
         d.dtype = dtype == at::kFloat ? BS_F32 : dtype == at::kHalf ? BS_F16 : BS_BF16;
         check(bs_cache_read(&c, &d, to.stream));
-        to.used({&a, &b});
+        to.uses({&k, &v, &k_scale, &v_scale, &table, &lens, &positions});
+        to.gives({&a, &b});
         return py::make_tuple(maybe(a), maybe(b));
     }
 
@@ -248,7 +261,11 @@ struct Cache {
         d.workspace = bytes ? work.data_ptr() : nullptr;
         d.workspace_bytes = bytes;
         check(bs_cache_attention(&c, &d, to.stream));
-        to.used({&out, &lse, &sum, &work});
+        to.uses({&k, &v, &k_scale, &v_scale, &q, &table, &lens});
+        if (mass) to.uses({&*mass});
+        if (given_out) to.uses({&sum});
+        else to.gives({&sum});
+        to.gives({&out, &lse});
         return py::make_tuple(out, maybe(lse), maybe(sum));
     }
 
@@ -286,7 +303,8 @@ struct Cache {
         d.workspace = bytes ? work.data_ptr() : nullptr;
         d.workspace_bytes = bytes;
         check(bs_cache_evict(&c, &d, to.stream));
-        to.used({&kept, &new_lens, &new_mass, &work});
+        to.uses({&k, &v, &k_scale, &v_scale, &mass, &table, &lens, &new_table});
+        to.gives({&kept, &new_lens, &new_mass});
         return py::make_tuple(kept, new_lens, new_mass);
     }
 };

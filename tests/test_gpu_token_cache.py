@@ -456,3 +456,61 @@ def test_merge_joins_disjoint_sets():
     c = cache.attention(q, table, R.i32([0]), with_lse=True)
     out, joined = M.merge([a[0], b[0], c[0]], [a[1], b[1], c[1]])
     assert (out - whole).abs().max() <= 4 * R.UNIT[F16] * whole.abs().max() and (joined - lse).abs().max() <= 1e-5
+
+
+# ---- streams ----------------------------------------------------------------
+
+def side_calls():
+    """Calls by name: what to do on a stream, the cache's buffers it changes."""
+    g = gen(60)
+    pool, table, q = attention_case(60, [300, 90], 8, 2, 64, 64, 1, F16)
+    cache, lens, new_table = M.TokenCache(*pool), R.i32([300, 90]), R.i32([[7, 8], [9, 10]])
+    wide = M.TokenCache(*R.random_pool(g, 11, 2, 64, 64))
+    x = torch.randn((711, 8, 64), generator=g, device="cuda").to(F16)
+    cu, places, mass = R.cu([300, 411]), torch.arange(300, dtype=torch.int32, device="cuda").repeat(2, 1), torch.rand((2, 2, 300), device="cuda")
+    cut_q, cut_k = R.cu([20]), R.cu([711])                   # several pieces of keys: a workspace
+    torch.cuda.synchronize()
+    return {"prompt": lambda s: M.prompt_attention(x, x[:, :2], x[:, 2:4], cu, with_lse=True, stream=s),
+            "pieces": lambda s: M.prompt_attention(x[:20, :1], x[:, :1], x[:, 1:2], cut_q, cut_k, with_lse=True, stream=s),
+            "read": lambda s: cache.read(table, lens, places, stream=s),
+            "attention": lambda s: cache.attention(q, table, lens, with_lse=True, mass=mass, stream=s),
+            "evict": lambda s: wide.evict(mass, table, lens, new_table, 100, stream=s)}
+
+
+@pytest.mark.parametrize("name", ["prompt", "pieces", "read", "attention", "evict"])
+def test_memory_of_a_call_on_a_side_stream_is_not_in_use_elsewhere(name):
+    call = side_calls()[name]
+    side = torch.cuda.Stream()
+    want = call(side.cuda_stream)
+    side.synchronize()
+    want = [t.clone() for t in want]
+    torch.cuda.synchronize()
+    # freed on the current stream, which still has to write to it
+    torch.cuda._sleep(100_000_000)
+    freed = [torch.empty_like(t) for t in want] + [torch.empty(2 ** 21 * i, dtype=torch.uint8, device="cuda") for i in (1, 2, 4)]
+    for t in freed:
+        t.fill_(7)
+    del t, freed
+    got = call(side.cuda_stream)
+    assert not torch.cuda.current_stream().query()       # the writes are still to come
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_inputs_of_a_call_on_a_side_stream_may_be_dropped_at_once():
+    g = gen(61)
+    side = torch.cuda.Stream()
+    q, k, v = (torch.randn((500, 4, 64), generator=g, device="cuda").to(F16) for _ in range(3))
+    want, _ = M.prompt_attention(q, k, v, R.cu([200, 300]))
+    mine, at = [t.clone() for t in (q, k, v)], R.cu([200, 300])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+    got, _ = M.prompt_attention(*mine, at, stream=side.cuda_stream)
+    del mine, at
+    again = [torch.full_like(q, 3.0) for _ in range(6)] + [torch.full((3,), 99, dtype=torch.int32, device="cuda") for _ in range(6)]
+    torch.cuda.current_stream().synchronize()
+    assert not side.query()                              # what was dropped is still to be read
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and M.take_errors() == 0
+    del again
