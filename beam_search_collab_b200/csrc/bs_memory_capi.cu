@@ -10,8 +10,10 @@
 #include "bs_memory.h"
 
 // One word per GPU that holds the library; the kernels OR their error bits
-// into it, bs_memory_take_errors copies and clears it.
+// into it, bs_memory_take_errors reads it and clears the bits it has read.
 static __device__ unsigned int g_memory_errors;
+
+static __global__ void k_clear_errors(unsigned int bits) { atomicAnd(&g_memory_errors, ~bits); }
 
 namespace bsb {
 
@@ -316,8 +318,12 @@ BS_API bs_status bs_memory_take_errors(void* stream_, uint32_t* flags) {
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     uint32_t h = 0;
     cudaError_t e = cudaMemcpyAsync(&h, dev.errors, 4, cudaMemcpyDeviceToHost, stream);
-    if (e == cudaSuccess) e = cudaMemsetAsync(dev.errors, 0, 4, stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    if (e == cudaSuccess && h) {       // bits set meanwhile by another stream's kernels stay for the next call
+        k_clear_errors<<<1, 1, 0, stream>>>(h);
+        e = cudaGetLastError();
+        if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    }
     if (e != cudaSuccess) return cuda_error(e, "error word");
     *flags = h;
     return BS_OK;

@@ -408,9 +408,12 @@ BS_API bs_status bs_cache_evict(const bs_token_cache* cache, const bs_cache_evic
 BS_API bs_status bs_cache_evict_workspace(const bs_token_cache* cache, const bs_cache_evict_desc* desc, size_t* bytes);
 
 /* Error bits that token-memory kernels have set on the current device since
- * the last call, ordered after the work queued on `stream`, then cleared;
- * synchronises `stream`.  Bits: 1 a wait inside a kernel gave up, 2 a block id
- * outside the cache, 4 lengths outside their buffers. */
+ * the last call, ordered after the work queued on `stream`; synchronises
+ * `stream`.  The bits returned are cleared, others that kernels on other
+ * streams set meanwhile stay for the next call.  The bits are the device's,
+ * not a stream's or a caller's: who takes them takes everyone's, and of two
+ * calls at once both may return the same bit.  Bits: 1 a wait inside a kernel
+ * gave up, 2 a block id outside the cache, 4 lengths outside their buffers. */
 BS_API bs_status bs_memory_take_errors(void* stream, uint32_t* flags);
 
 /* Device buffers on the index's device (for callers that stage queries once

@@ -514,3 +514,20 @@ def test_inputs_of_a_call_on_a_side_stream_may_be_dropped_at_once():
     torch.cuda.synchronize()
     assert torch.equal(got, want) and M.take_errors() == 0
     del again
+
+
+def test_error_bits_of_another_stream_are_not_lost():
+    # a kernel on a side stream sets a bit while the errors are taken: by this call or the next
+    pool, table, q = attention_case(62, [40], 4, 2, 32, 64, 1, F16)
+    cache, bad, lens, places = M.TokenCache(*pool), R.i32([[pool[0].shape[0], 0]]), R.i32([40]), R.i32([[3]])
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(600):
+        M.prompt_attention(q[0], q[0, :, :2], q[0, :, :2], R.cu([1]), R.i32([0, 2]))      # another bit: there is something to clear
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(1000 + 50 * i)             # the bit is set 1 to 16 us after the call, or a little later
+        cache.read(bad, lens, places, stream=side.cuda_stream)
+        first = M.take_errors()
+        side.synchronize()
+        assert first & 4 and first | M.take_errors() == 6, i
