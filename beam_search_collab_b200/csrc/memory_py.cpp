@@ -312,7 +312,12 @@ struct Cache {
 uint32_t take_errors(int64_t device, std::optional<uint64_t> stream) {
     Target to(at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device)), stream);
     uint32_t flags = 0;
-    check(bs_memory_take_errors(to.stream, &flags));
+    bs_status s;
+    {
+        py::gil_scoped_release others;       // it waits for the stream
+        s = bs_memory_take_errors(to.stream, &flags);
+    }
+    check(s);
     return flags;
 }
 

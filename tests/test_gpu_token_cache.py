@@ -1,6 +1,8 @@
 """GPU: the 8-bit token cache (writing, reading, attention, eviction) against
 the operators' definitions."""
 import math
+import threading
+import time
 
 import pytest
 import torch
@@ -486,8 +488,9 @@ def test_memory_of_a_call_on_a_side_stream_is_not_in_use_elsewhere(name):
     want = [t.clone() for t in want]
     torch.cuda.synchronize()
     # freed on the current stream, which still has to write to it
-    torch.cuda._sleep(100_000_000)
-    freed = [torch.empty_like(t) for t in want] + [torch.empty(2 ** 21 * i, dtype=torch.uint8, device="cuda") for i in (1, 2, 4)]
+    freed = [torch.empty_like(t).fill_(0) for t in want] + [torch.zeros(2 ** 21 * i, dtype=torch.uint8, device="cuda") for i in (1, 2, 4)]
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)
     for t in freed:
         t.fill_(7)
     del t, freed
@@ -503,12 +506,16 @@ def test_inputs_of_a_call_on_a_side_stream_may_be_dropped_at_once():
     q, k, v = (torch.randn((500, 4, 64), generator=g, device="cuda").to(F16) for _ in range(3))
     want, _ = M.prompt_attention(q, k, v, R.cu([200, 300]))
     mine, at = [t.clone() for t in (q, k, v)], R.cu([200, 300])
+    fill = lambda n: [torch.full_like(q, 3.0) for _ in range(n)] + [torch.full_like(at, 99) for _ in range(n)]  # noqa: E731
+    keep = fill(12)                                      # (what loads kernels or asks the driver for memory waits for the GPU)
+    del keep
     torch.cuda.synchronize()
     with torch.cuda.stream(side):
-        torch.cuda._sleep(100_000_000)
+        torch.cuda._sleep(200_000_000)
     got, _ = M.prompt_attention(*mine, at, stream=side.cuda_stream)
-    del mine, at
-    again = [torch.full_like(q, 3.0) for _ in range(6)] + [torch.full((3,), 99, dtype=torch.int32, device="cuda") for _ in range(6)]
+    at = at.new_empty(3)                                 # (the first one is dropped)
+    del mine
+    again = fill(6)
     torch.cuda.current_stream().synchronize()
     assert not side.query()                              # what was dropped is still to be read
     torch.cuda.synchronize()
@@ -531,3 +538,21 @@ def test_error_bits_of_another_stream_are_not_lost():
         first = M.take_errors()
         side.synchronize()
         assert first & 4 and first | M.take_errors() == 6, i
+
+
+def test_other_threads_run_while_errors_are_waited_for():
+    M.take_errors()
+    at, done = [], threading.Event()
+
+    def tick():
+        while not done.wait(0.001):
+            at.append(time.monotonic())
+    thread = threading.Thread(target=tick)
+    thread.start()
+    torch.cuda._sleep(600_000_000)                       # 0.3 s
+    began = time.monotonic()
+    M.take_errors()
+    ended = time.monotonic()
+    done.set()
+    thread.join()
+    assert ended - began > 0.1 and sum(began < x < ended for x in at) >= 10
