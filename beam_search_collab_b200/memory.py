@@ -109,7 +109,8 @@ def take_errors(device=None, stream=None) -> int:
     waits for `stream`.  0: none; 1 a wait gave up, 2 a block id outside the
     cache, 4 lengths outside their buffers."""
     if not isinstance(device, int):
-        device = torch.cuda.current_device() if device is None else torch.device(device).index
+        device = None if device is None else torch.device(device).index
+        device = torch.cuda.current_device() if device is None else device
     return _memory.take_errors(device, stream)
 
 

@@ -124,3 +124,10 @@ def test_prompt_definition(causal):
                 assert torch.allclose(lse[a + i, h], torch.logsumexp(s, 0)) if n else lse[a + i, h] == -math.inf
         a, b = a + nq, b + nk
     assert (weighted >= out.abs() - 1e-12).all()
+
+
+@pytest.mark.parametrize("device,index", [(None, 3), ("cuda", 3), (torch.device("cuda"), 3), ("cuda:1", 1), (2, 2), (torch.device("cuda", 0), 0)])
+def test_take_errors_finds_its_device(device, index, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    monkeypatch.setattr(M._memory, "take_errors", lambda device, stream: (device, stream))
+    assert M.take_errors(device, 7) == (index, 7)
