@@ -159,7 +159,9 @@ BS_API bs_status bs_prompt_attention_workspace(const bs_prompt_attention_desc* d
 
 BS_API bs_status bs_prompt_attention(const bs_prompt_attention_desc* d, void* stream) {
     if (bs_status s = check_prompt(d)) return s;
-    if (d->total_q == 0 || d->num_seqs == 0) return BS_OK;
+    if (d->total_q == 0) return BS_OK;
+    if (d->num_seqs == 0)
+        return report_error(BS_ERR_INVALID_ARGUMENT, "num_seqs is 0, but q has %u rows", static_cast<unsigned>(d->total_q));
     if (any_null({d->q, d->out, d->cu_q, d->cu_k}) || (d->total_k && any_null({d->k, d->v})))
         return report_error(BS_ERR_INVALID_ARGUMENT, "a buffer is NULL");
     if (!aligned16({d->q, d->k, d->v, d->out, d->workspace}) || !strides_ok(d->q_stride, 2) || !strides_ok(d->k_stride, 2) ||

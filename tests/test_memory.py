@@ -131,3 +131,12 @@ def test_take_errors_finds_its_device(device, index, monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
     monkeypatch.setattr(M._memory, "take_errors", lambda device, stream: (device, stream))
     assert M.take_errors(device, 7) == (index, 7)
+
+
+def test_rows_of_no_sequence_are_refused():
+    # they would be left as the buffers were
+    d = A._Prompt(64, 64, 64, 64, 64, (128, 64), (128, 64), (128, 64), 64, 64, None, 0, 10, 10, 0, 2, 2, 64, 1, 1, 0.1)
+    rc, why = status("bs_prompt_attention", d, None)
+    assert rc == 1 and "num_seqs is 0" in why
+    d.total_q = 0
+    assert status("bs_prompt_attention", d, None)[0] == 0
