@@ -635,6 +635,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
             }
             loads += 2 * (end - m.first);
         }
+        // and, under the last item's epilogue, the ends of the lists (in every
+        // block that runs; at its start this held up pieces of prompts by 1 us)
+        if (lane < 4) {
+            const int32_t end = (lane & 1 ? d.cu_k : d.cu_q)[lane < 2 ? 0 : d.num_seqs];
+            if (static_cast<uint32_t>(end) != (lane < 2 ? 0 : lane & 1 ? d.total_k : d.total_q)) atomicOr(a.errors, kMemErrLength);
+        }
+        __syncwarp();
     } else if (warp == 9) {
         // ------------------------------------------------------------ copies
         // (by lane 0)

@@ -286,7 +286,9 @@ typedef struct bs_token_cache {
 
 /* Attention of packed prompts.  Sequence b's queries are rows cu_q[b] ..
  * cu_q[b+1] of q and its keys rows cu_k[b] .. cu_k[b+1] of k and v; both lists
- * start at 0, ascend and end at total_q and total_k.  With `causal`, query i
+ * start at 0, ascend and end at total_q and total_k (else error bit 4 is set,
+ * and the rows of out and lse that no sequence has, or one whose lists are
+ * wrong, hold anything).  With `causal`, query i
  * of Lq sees the keys j <= i + Lk - Lq (the last query sees all), else all.
  * Query head h goes with key head h / (q_heads / kv_heads).
  *   s_j = scale * <q, k_j>,  lse = log sum_j exp(s_j),  out = sum_j exp(s_j - lse) v_j

@@ -235,3 +235,21 @@ def test_refusals():
     with pytest.raises(BSearchError, match="NaN"):
         M.prompt_attention(q, k, v, at, scale=math.nan)
     assert M.take_errors() == 0
+
+
+@pytest.mark.parametrize("heads,keys", [(4, 60), (1, 6000)])            # (6,000 keys of one head: several pieces)
+def test_lists_that_begin_late_or_end_early_set_an_error_bit(heads, keys):
+    q, k, v = inputs(43, 40, keys, heads, heads, 64, F16)
+    whole_q, whole_k = R.cu([32, 8]), R.cu([keys - 10, 10])
+    M.prompt_attention(q, k, v, whole_q, whole_k)
+    assert M.take_errors() == 0
+    for cu_q, cu_k in ((R.i32([10, 22, 40]), whole_k), (R.i32([0, 22, 30]), whole_k), (whole_q, R.i32([3, 5, keys])),
+                       (whole_q, R.i32([0, 5, keys - 1]))):
+        M.prompt_attention(q, k, v, cu_q, cu_k)
+        assert M.take_errors() == 4
+    # the rows that the lists do cover are right all the same
+    out, lse = M.prompt_attention(q, k, v, R.i32([10, 22, 30]), R.i32([3, keys - 17, keys - 7]), with_lse=True)
+    assert M.take_errors() == 4
+    ref, ref_lse, weighted, big = R.prompt(q[10:30], k[3:-7], v[3:-7], [12, 8], [keys - 20, 10], True, 0.125)
+    assert ((out[10:30].double() - ref).abs() <= R.out_bound(ref, weighted, F16, R.UNIT[F16])).all()
+    assert ((lse[10:30].double() - ref_lse).abs() <= R.lse_bound(big)).all()
