@@ -746,6 +746,7 @@ __global__ void __launch_bounds__(kMassThreads) k_cache_mass(const __grid_consta
     const uint32_t width = a.d.mass_width;
     const uint32_t len = held_tokens(a, b);
     cudaGridDependencySynchronize();       // in every block, as above
+    if (j == 0 && len > width) atomicOr(a.errors, kMemErrLength);      // tokens whose weights have no place
     if (j >= width) return;
     const uint64_t seg = static_cast<uint64_t>(b) * a.c.kv_heads + h, at = seg * width + j;
     const uint32_t n = j < len ? min(len - j, 4u) : 0;

@@ -361,7 +361,9 @@ BS_API bs_status bs_cache_read(const bs_token_cache* cache, const bs_cache_read_
  * bs_prompt_attention.  With out_mass, the weight that each cached token got,
  *   out_mass[b][h][j] = mass[b][h][j] + sum over the queries and the heads of
  *                       key head h of exp(s_j - lse)        (j < lens[b])
- * and 0 for lens[b] <= j < mass_width; mass may be NULL (zeros) or out_mass. */
+ * and 0 for lens[b] <= j < mass_width; mass may be NULL (zeros) or out_mass.
+ * Weights of tokens at and past mass_width have no place: they are left out,
+ * and error bit 4 is set. */
 typedef struct bs_cache_attention_desc {
     const void* q;            /* [num_seqs][queries][q_heads][dim]            */
     int64_t q_stride[3];      /* elements from sequence to sequence, token to token, head to head */

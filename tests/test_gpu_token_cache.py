@@ -556,3 +556,15 @@ def test_other_threads_run_while_errors_are_waited_for():
     done.set()
     thread.join()
     assert ended - began > 0.1 and sum(began < x < ended for x in at) >= 10
+
+
+def test_weights_without_a_place_set_an_error_bit():
+    lens = [100, 33]
+    pool, table, q = attention_case(42, lens, 4, 2, 32, 64, 1, BF16)
+    cache = M.TokenCache(*pool)
+    mass = torch.rand((2, 2, 128), device="cuda")
+    _, _, whole = cache.attention(q, table, R.i32(lens), mass=mass)
+    assert M.take_errors() == 0
+    for width, flags in ((100, 0), (99, 4), (64, 4)):
+        _, _, got = cache.attention(q, table, R.i32(lens), mass=mass[:, :, :width].contiguous())
+        assert M.take_errors() == flags and torch.equal(got, whole[:, :, :width])
