@@ -668,10 +668,10 @@ __global__ void __launch_bounds__(kJoinThreads) k_cache_join(const __grid_consta
     __shared__ float4 parts[kJoinWarps][32];
     const uint32_t h = blockIdx.x / used_rows, r = blockIdx.x % used_rows, rt = blockIdx.y, b = blockIdx.z;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hkv = a.c.kv_heads, dim = a.c.dim, col = rt * tile_rows + r;
+    cudaGridDependencySynchronize();       // in every block, before anything of the caller's
     uint64_t before, all;
     count_cost(a, b, before, all, sums);
     const uint32_t tiles = tiles_of(held_tokens(a, b));
-    cudaGridDependencySynchronize();       // in every block: what follows this kernel may count on both being done
     if (col >= a.rows) return;
     const uint64_t w_all = all * hkv, s0 = before * hkv + static_cast<uint64_t>(h) * (tiles + kStart);
     uint32_t i0 = 0, pieces = 0, slot0 = 0;
@@ -744,8 +744,8 @@ constexpr int kMassThreads = 128;
 __global__ void __launch_bounds__(kMassThreads) k_cache_mass(const __grid_constant__ CacheArgs a) {
     const uint32_t j = (blockIdx.x * kMassThreads + threadIdx.x) * 4, h = blockIdx.y, b = blockIdx.z;
     const uint32_t width = a.d.mass_width;
+    cudaGridDependencySynchronize();       // in every block, before anything of the caller's
     const uint32_t len = held_tokens(a, b);
-    cudaGridDependencySynchronize();       // in every block, as above
     if (j == 0 && len > width) atomicOr(a.errors, kMemErrLength);      // tokens whose weights have no place
     if (j >= width) return;
     const uint64_t seg = static_cast<uint64_t>(b) * a.c.kv_heads + h, at = seg * width + j;

@@ -140,3 +140,21 @@ def test_rows_of_no_sequence_are_refused():
     assert rc == 1 and "num_seqs is 0" in why
     d.total_q = 0
     assert status("bs_prompt_attention", d, None)[0] == 0
+
+
+def test_kernels_wait_for_the_one_before_them_first():
+    # launched under the end of the kernel before: its results, lengths among them, are not read and no
+    # error bit is set before the wait
+    import os
+    import re
+    kernels = 0
+    for name in ("bs_prompt_attention.cu", "bs_cache_attention.cu", "bs_token_cache.cu"):
+        with open(os.path.join(B.PKG, "csrc", name)) as f:
+            text = f.read()
+        for m in re.finditer(r"__global__ void[^;{]*?(k_\w+)\(", text):
+            body = text[m.end():text.index("\n}\n", m.end())]
+            before, wait, _ = body.partition("cudaGridDependencySynchronize();")
+            assert wait, m[1]
+            assert not re.search(r"held_tokens\(|count_cost\(|atomicOr\(|\bd\.\w+\[|mass\[|kept\[", before), m[1]
+            kernels += 1
+    assert kernels == 9
