@@ -567,3 +567,26 @@ def test_weights_without_a_place_set_an_error_bit():
     for width, flags in ((100, 0), (99, 4), (64, 4)):
         _, _, got = cache.attention(q, table, R.i32(lens), mass=mass[:, :, :width].contiguous())
         assert M.take_errors() == flags and torch.equal(got, whole[:, :, :width])
+
+
+# ---- small weights ----------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("nats", [8, 11, 14, 17])
+def test_attention_small_weights_beside_a_large_one_and_a_large_scale(nats, dtype):
+    # one token without values has most of the weight, all others e^-nats of its; one block has 50 times the others' value scale
+    g = gen(40)
+    pool = R.random_pool(g, 16, 2, 64, 64)
+    table, _ = R.random_table(g, [16])
+    at = table[0].long()
+    pool[0].zero_(), pool[1].clamp_(min=0), pool[2].fill_(0.01), pool[3].fill_(0.01)
+    pool[0][at[0], :, 0], pool[1][at[0], :, 0] = 100, 0
+    pool[1][at[2]], pool[3][at[2]] = 0, 0.5
+    q, scale = torch.ones((1, 1, 8, 64), dtype=dtype, device="cuda"), nats / 64.0
+    out, _, _ = M.TokenCache(*pool).attention(q, table, R.i32([1024]), scale=scale)
+    ref, _, _, weighted, _ = R.cache(pool, q, table, [1024], scale)
+    # the result's rounding, a weight's and its score's, and half a step of f16's smallest numbers at 2^5 for the largest
+    codes = pool[1][at].double().abs().sum((0, 2)).repeat_interleave(4, 0)
+    bound = R.UNIT[dtype] * ref.abs() + (R.UNIT[F16] + 2.0 ** -12) * (1 + 2.0 ** -7) * weighted + 2.0 ** -30 * 0.5 * codes
+    assert ((out.double() - ref).abs() <= bound).all()
+
