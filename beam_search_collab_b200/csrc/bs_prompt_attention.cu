@@ -55,6 +55,17 @@ constexpr int kBoxBytes = kRows * 128; // 128 rows of 64 elements
 constexpr unsigned kPolls = 1u << 22;
 constexpr uint32_t kMostChunks = 8;
 constexpr float kMost = 256.f;         // weights may grow to this before the maximum is moved
+// Weights count in 2^-kLift: in f16 the room that kMost leaves above is room
+// for small ones (2^-21 of the largest with all bits; without it 2^-14, and
+// keys e^-15 of the first one's weight were 3% off).  bf16 has exponents enough.
+template <typename T>
+constexpr float kLift = 0.f;
+template <>
+constexpr float kLift<__half> = 7.f;
+template <typename T>
+constexpr float kLifted = 1.f;
+template <>
+constexpr float kLifted<__half> = 128.f;     // 2^kLift
 
 struct PromptArgs {
     bs_prompt_attention_desc d;
@@ -322,8 +333,8 @@ __device__ __noinline__ float2 weights_with_care(uint32_t s_at, uint32_t o_at, i
             for (int k = 0; k < 32; ++k) s[x][k] = 32 * at + k < left ? s[x][k] : -INFINITY;
             uint32_t p[16];
             float part;
-            const float high = weights<T>(s[x], scale, top == -INFINITY ? 0.f : -top * scale, p, part);
-            if (__any_sync(kFull, real && (high > kMost || top == -INFINITY))) {
+            const float high = weights<T>(s[x], scale, top == -INFINITY ? 0.f : kLift<T> - top * scale, p, part);
+            if (__any_sync(kFull, real && (high > kMost * kLifted<T> || top == -INFINITY))) {
                 // the maximum moves, what was summed is rescaled
                 float next = top;
 #pragma unroll
@@ -333,7 +344,7 @@ __device__ __noinline__ float2 weights_with_care(uint32_t s_at, uint32_t o_at, i
                 sum *= shrink;
                 if (at + 1 < chunks) wait_loads32(s[x ^ 1]);
                 rescale<T>(s_at, o_at, at, dim, shrink);
-                weights<T>(s[x], scale, top == -INFINITY ? 0.f : -top * scale, p, part);
+                weights<T>(s[x], scale, top == -INFINITY ? 0.f : kLift<T> - top * scale, p, part);
             }
             sum += part;
             tmem_store16(s_at + 16 * at, p);
@@ -827,8 +838,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                     for (; done < 4; done += 2) {
                         uint32_t p[kRows / 4];
                         float part;
-                        const float high = weights64<T>(s_at + 32 * done, done == 0, s, scale, -top * scale, p, part);
-                        if (__any_sync(kFull, real && high > kMost)) break;       // (rows that are none of the tile's hold anything)
+                        const float high = weights64<T>(s_at + 32 * done, done == 0, s, scale, kLift<T> - top * scale, p, part);
+                        if (__any_sync(kFull, real && high > kMost * kLifted<T>)) break;       // (rows that are none of the tile's hold anything)
                         sum += part;
                         tmem_store16(s_at + 16 * done, p);
                         tmem_store16(s_at + 16 * done + 16, p + 16);
@@ -902,7 +913,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                     for (int k = 0; k < 32; ++k) u[k] = __float_as_uint(o[k]);
                     store_rows(u, staging + warp * 4096, out, x * 4, d.dim * 4);
                 }
-                if (ok) a.part_ml[slot] = make_float2(top * scale, sum);
+                if (ok) a.part_ml[slot] = make_float2(top * scale - kLift<T>, sum);
             } else {
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
                 T* const out = ok ? static_cast<T*>(d.out) + at * d.dim : nullptr;
@@ -919,7 +930,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ 
                     }
                     store_rows(u, staging + warp * 4096, out, x * 2, d.dim * 2);
                 }
-                if (ok && d.lse) d.lse[at] = sum == 0.f ? -INFINITY : top * d.scale + logf(sum);
+                if (ok && d.lse) d.lse[at] = sum == 0.f ? -INFINITY : top * d.scale + logf(sum * (1.f / kLifted<T>));
             }
             item_read(i);
             // the next item's first value product overwrites the outputs: it

@@ -253,3 +253,28 @@ def test_lists_that_begin_late_or_end_early_set_an_error_bit(heads, keys):
     ref, ref_lse, weighted, big = R.prompt(q[10:30], k[3:-7], v[3:-7], [12, 8], [keys - 20, 10], True, 0.125)
     assert ((out[10:30].double() - ref).abs() <= R.out_bound(ref, weighted, F16, R.UNIT[F16])).all()
     assert ((lse[10:30].double() - ref_lse).abs() <= R.lse_bound(big)).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("nats", [8, 13, 14, 15])
+def test_small_weights_beside_a_large_one(nats, dtype):
+    # the first key has no value and most of the weight, all others e^-nats of its: what 16 bits lose of one they lose of all
+    n, heads, d = 1024, 160, 64                    # (so many heads that the keys stay in one piece)
+    q, k, v = inputs(41, 1, n, heads, heads, d, dtype)
+    q, v = torch.ones_like(q), v.abs()
+    k.zero_()
+    k[0], v[0] = nats / 8, 0
+    out, lse = M.prompt_attention(q, k, v, R.cu([1]), R.cu([n]), with_lse=True)
+    ref, ref_lse, weighted, big = R.prompt(q, k, v, [1], [n], True, 0.125)
+    # the result's rounding, a weight's and its score's, and (f16) half a step of the smallest numbers at 2^7 for the largest
+    bound = R.UNIT[dtype] * ref.abs() + (R.UNIT[dtype] + 2.0 ** -12) * (1 + 2.0 ** -7) * weighted + 2.0 ** -32 * v.double().sum(0)
+    assert ((out.double() - ref).abs() <= bound).all()
+    assert ((lse.double() - ref_lse).abs() <= R.lse_bound(big)).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_rows_whose_scores_are_far_below_zero_and_far_above(dtype):
+    lens = [300, 70]
+    q, k, v = inputs(42, 370, 370, 4, 2, 64, dtype)
+    k[:, :, 0], q[:, :, 0] = 20.0, torch.linspace(-60, 60, 370, device="cuda")[:, None].to(dtype)
+    check(q, k, v, lens, lens)
