@@ -55,6 +55,13 @@ bool aligned16(std::initializer_list<const void*> ptrs) {
     return true;
 }
 
+// Lists, lengths, scales and masses: read and written 4 bytes at a time.
+bool aligned4(std::initializer_list<const void*> ptrs) {
+    for (const void* p : ptrs)
+        if (reinterpret_cast<uintptr_t>(p) & 3) return false;
+    return true;
+}
+
 // Strides of 16-bit elements: non-negative multiples of 16 bytes, small
 // enough that no address arithmetic of the kernels can overflow.
 bool strides_ok(const int64_t* s, int n) {
@@ -64,6 +71,7 @@ bool strides_ok(const int64_t* s, int n) {
 }
 
 const char* const kWhere = "pointers must be memory of the current device";
+const char* const kAlign4 = "32-bit buffers must be 4-byte aligned";
 const char* const kAlign = "q, k, v and outputs must be 16-byte aligned, their strides non-negative multiples of 8 elements";
 
 bs_status check_dim(int32_t dim) {
@@ -95,6 +103,7 @@ bs_status check_cache(const bs_token_cache* c, int device, bool pointers) {
     if (!pointers) return BS_OK;
     if (any_null({c->k, c->v, c->k_scale, c->v_scale})) return report_error(BS_ERR_INVALID_ARGUMENT, "a cache buffer is NULL");
     if (!aligned16({c->k, c->v})) return report_error(BS_ERR_INVALID_ARGUMENT, "the cache's codes must be 16-byte aligned");
+    if (!aligned4({c->k_scale, c->v_scale})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign4);
     if (!on_device(device, {c->k, c->v, c->k_scale, c->v_scale}))
         return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kWhere);
     return BS_OK;
@@ -167,6 +176,7 @@ BS_API bs_status bs_prompt_attention(const bs_prompt_attention_desc* d, void* st
     if (!aligned16({d->q, d->k, d->v, d->out, d->workspace}) || !strides_ok(d->q_stride, 2) || !strides_ok(d->k_stride, 2) ||
         !strides_ok(d->v_stride, 2))
         return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign);
+    if (!aligned4({d->lse, d->cu_q, d->cu_k})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign4);
     // one head or token for many (a stride of 0) has no tensor map
     if ((d->total_q > 1 && d->q_stride[0] == 0) || (d->q_heads > 1 && d->q_stride[1] == 0) ||
         (d->total_k > 1 && (d->k_stride[0] == 0 || d->v_stride[0] == 0)) || (d->kv_heads > 1 && (d->k_stride[1] == 0 || d->v_stride[1] == 0)))
@@ -194,6 +204,7 @@ BS_API bs_status bs_cache_write(const bs_token_cache* c, const bs_cache_write_de
     if (any_null({d->k, d->v, d->cu, d->table, d->start})) return report_error(BS_ERR_INVALID_ARGUMENT, "a buffer is NULL");
     if (!aligned16({d->k, d->v}) || !strides_ok(d->k_stride, 2) || !strides_ok(d->v_stride, 2))
         return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign);
+    if (!aligned4({d->cu, d->table, d->start})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign4);
     if (bs_status s = memory_device(dev)) return s;
     if (bs_status s = check_cache(c, dev.device, true)) return s;
     if (!on_device(dev.device, {d->k, d->v, d->cu, d->table, d->start})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kWhere);
@@ -215,6 +226,7 @@ BS_API bs_status bs_cache_read(const bs_token_cache* c, const bs_cache_read_desc
     if (any_null({d->lens, d->positions}) || (d->table_width && !d->table))
         return report_error(BS_ERR_INVALID_ARGUMENT, "a buffer is NULL");
     if (!aligned16({d->k, d->v})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign);
+    if (!aligned4({d->table, d->lens, d->positions})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign4);
     if (bs_status s = memory_device(dev)) return s;
     if (bs_status s = check_cache(c, dev.device, true)) return s;
     if (!on_device(dev.device, {d->table, d->lens, d->positions, d->k, d->v}))
@@ -254,6 +266,7 @@ BS_API bs_status bs_cache_attention(const bs_token_cache* c, const bs_cache_atte
     if (d->out_mass && d->mass_width == 0) return report_error(BS_ERR_INVALID_ARGUMENT, "mass_width is 0");
     if (!aligned16({d->q, d->out, d->workspace}) || !strides_ok(d->q_stride, 3))
         return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign);
+    if (!aligned4({d->table, d->lens, d->lse, d->mass, d->out_mass})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign4);
     MemoryDevice dev;
     if (bs_status s = memory_device(dev)) return s;
     if (bs_status s = check_cache(c, dev.device, true)) return s;
@@ -300,6 +313,7 @@ BS_API bs_status bs_cache_evict(const bs_token_cache* c, const bs_cache_evict_de
         (d->new_table_width && !d->new_table) || (d->mass_width && !d->mass))
         return report_error(BS_ERR_INVALID_ARGUMENT, "a buffer is NULL");
     if (!aligned16({d->workspace})) return report_error(BS_ERR_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
+    if (!aligned4({d->mass, d->table, d->lens, d->new_table, d->kept, d->new_lens, d->new_mass})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign4);
     MemoryDevice dev;
     if (bs_status s = memory_device(dev)) return s;
     if (bs_status s = check_cache(c, dev.device, true)) return s;

@@ -267,7 +267,8 @@ BS_API bs_status bs_merge_shards(const float* dists, const uint32_t* ids, uint32
  *
  * dim is a multiple of 16 up to 128.  q, k and v have strides in elements
  * between tokens and between heads; they and the base address are multiples
- * of 16 bytes, the last dimension is contiguous.  Outputs are contiguous.
+ * of 16 bytes, the last dimension is contiguous.  Outputs are contiguous, of
+ * 16-bit types 16-byte aligned; 32-bit buffers are 4-byte aligned.
  * scale is positive and finite. */
 typedef enum bs_dtype { BS_F32 = 0, BS_F16 = 1, BS_BF16 = 2 } bs_dtype;
 

@@ -158,3 +158,28 @@ def test_kernels_wait_for_the_one_before_them_first():
             assert not re.search(r"held_tokens\(|count_cost\(|atomicOr\(|\bd\.\w+\[|mass\[|kept\[", before), m[1]
             kernels += 1
     assert kernels == 9
+
+
+def calls():
+    """A call of each entry that only lacks memory of a GPU."""
+    return {"bs_prompt_attention": A._Prompt(64, 64, 64, 64, 64, (128, 64), (128, 64), (128, 64), 64, 64, None, 0, 10, 10, 1, 2, 2, 64, 1, 1, 0.1),
+            "bs_cache_write": A._Write(64, 64, (128, 64), (128, 64), 64, 64, 64, 10, 1, 1, 1),
+            "bs_cache_read": A._Read(64, 64, 64, 0, 0, 64, 64, 1, 1, 1, 0),
+            "bs_cache_attention": A._Attention(64, (256, 256, 64), 64, 64, 64, 64, 64, 64, None, 0, 1, 2, 64, 1, 4, 1, 0.1),
+            "bs_cache_evict": A._Evict(64, 64, 64, 64, 64, 64, 64, None, 0, 1, 4, 1, 128, 32, 4, 8)}
+
+
+def call(name, d, **kw):
+    return status(name, d, None) if name == "bs_prompt_attention" else status(name, cache(**kw), d, None)
+
+
+@pytest.mark.parametrize("name,fields", [("bs_prompt_attention", "lse cu_q cu_k"), ("bs_cache_write", "cu table start"),
+                                         ("bs_cache_read", "table lens positions"),
+                                         ("bs_cache_attention", "table lens lse mass out_mass"),
+                                         ("bs_cache_evict", "mass table lens new_table kept new_lens new_mass")])
+def test_misaligned_32_bit_buffers_are_refused(name, fields):
+    for field in fields.split():
+        d = calls()[name]
+        setattr(d, field, 66)
+        rc, why = call(name, d)
+        assert rc == 1 and "4-byte aligned" in why, (field, rc, why)
