@@ -62,17 +62,30 @@ bool aligned4(std::initializer_list<const void*> ptrs) {
     return true;
 }
 
-// Strides of 16-bit elements: non-negative multiples of 16 bytes, small
-// enough that no address arithmetic of the kernels can overflow.
-bool strides_ok(const int64_t* s, int n) {
-    for (int i = 0; i < n; ++i)
-        if (s[i] < 0 || (s[i] & 7) || s[i] >= (int64_t{1} << 37)) return false;
+// Strides between `extents` places: not negative, and no place so far away
+// that address arithmetic could overflow.
+bool within_reach(const int64_t* s, std::initializer_list<uint32_t> extents) {
+    int64_t left = int64_t{1} << 59;
+    int i = 0;
+    for (uint32_t extent : extents) {
+        const int64_t steps = extent > 1 ? extent - 1 : 1;
+        if (s[i] < 0 || s[i] > left / steps) return false;
+        left -= s[i++] * steps;
+    }
     return true;
+}
+
+// Of 16-bit elements: multiples of 16 bytes too, below the 2^40 bytes of a
+// tensor map.
+bool strides_ok(const int64_t* s, std::initializer_list<uint32_t> extents) {
+    for (size_t i = 0; i < extents.size(); ++i)
+        if ((s[i] & 7) || s[i] >= (int64_t{1} << 37)) return false;
+    return within_reach(s, extents);
 }
 
 const char* const kWhere = "pointers must be memory of the current device";
 const char* const kAlign4 = "32-bit buffers must be 4-byte aligned";
-const char* const kAlign = "q, k, v and outputs must be 16-byte aligned, their strides non-negative multiples of 8 elements";
+const char* const kAlign = "q, k, v and outputs must be 16-byte aligned, their strides non-negative multiples of 8 elements within a buffer's reach";
 
 bs_status check_dim(int32_t dim) {
     if (dim <= 0) return report_error(BS_ERR_INVALID_ARGUMENT, "dim must be positive");
@@ -171,10 +184,11 @@ BS_API bs_status bs_prompt_attention(const bs_prompt_attention_desc* d, void* st
     if (d->total_q == 0) return BS_OK;
     if (d->num_seqs == 0)
         return report_error(BS_ERR_INVALID_ARGUMENT, "num_seqs is 0, but q has %u rows", static_cast<unsigned>(d->total_q));
+    const uint32_t q_heads = d->q_heads, kv_heads = d->kv_heads;
     if (any_null({d->q, d->out, d->cu_q, d->cu_k}) || (d->total_k && any_null({d->k, d->v})))
         return report_error(BS_ERR_INVALID_ARGUMENT, "a buffer is NULL");
-    if (!aligned16({d->q, d->k, d->v, d->out, d->workspace}) || !strides_ok(d->q_stride, 2) || !strides_ok(d->k_stride, 2) ||
-        !strides_ok(d->v_stride, 2))
+    if (!aligned16({d->q, d->k, d->v, d->out, d->workspace}) || !strides_ok(d->q_stride, {d->total_q, q_heads}) ||
+        !strides_ok(d->k_stride, {d->total_k, kv_heads}) || !strides_ok(d->v_stride, {d->total_k, kv_heads}))
         return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign);
     if (!aligned4({d->lse, d->cu_q, d->cu_k})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign4);
     // one head or token for many (a stride of 0) has no tensor map
@@ -202,7 +216,8 @@ BS_API bs_status bs_cache_write(const bs_token_cache* c, const bs_cache_write_de
     if (d->total >= (1u << 30)) return report_error(BS_ERR_UNSUPPORTED, "at most 2^30 tokens a call are supported");
     if (d->total == 0 || d->num_seqs == 0) return BS_OK;
     if (any_null({d->k, d->v, d->cu, d->table, d->start})) return report_error(BS_ERR_INVALID_ARGUMENT, "a buffer is NULL");
-    if (!aligned16({d->k, d->v}) || !strides_ok(d->k_stride, 2) || !strides_ok(d->v_stride, 2))
+    const uint32_t heads = c->kv_heads;
+    if (!aligned16({d->k, d->v}) || !strides_ok(d->k_stride, {d->total, heads}) || !strides_ok(d->v_stride, {d->total, heads}))
         return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign);
     if (!aligned4({d->cu, d->table, d->start})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign4);
     if (bs_status s = memory_device(dev)) return s;
@@ -220,8 +235,9 @@ BS_API bs_status bs_cache_read(const bs_token_cache* c, const bs_cache_read_desc
         return report_error(BS_ERR_INVALID_ARGUMENT, "dtype must be BS_F32, BS_F16 or BS_BF16");
     if (bs_status s = check_table(c, d->num_seqs, d->table_width)) return s;
     if (d->count >= (1u << 30)) return report_error(BS_ERR_UNSUPPORTED, "at most 2^30 positions are supported");
-    if (d->position_seq_stride < 0 || d->position_head_stride < 0)
-        return report_error(BS_ERR_INVALID_ARGUMENT, "strides of positions must not be negative");
+    const int64_t steps[2] = {d->position_seq_stride, d->position_head_stride};
+    if (!within_reach(steps, {d->num_seqs, static_cast<uint32_t>(c->kv_heads)}))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "strides of positions must not be negative or out of any buffer's reach");
     if (d->count == 0 || d->num_seqs == 0 || (!d->k && !d->v)) return BS_OK;
     if (any_null({d->lens, d->positions}) || (d->table_width && !d->table))
         return report_error(BS_ERR_INVALID_ARGUMENT, "a buffer is NULL");
@@ -264,7 +280,7 @@ BS_API bs_status bs_cache_attention(const bs_token_cache* c, const bs_cache_atte
         return report_error(BS_ERR_INVALID_ARGUMENT, "a buffer is NULL");
     if (d->mass && !d->out_mass) return report_error(BS_ERR_INVALID_ARGUMENT, "mass without out_mass");
     if (d->out_mass && d->mass_width == 0) return report_error(BS_ERR_INVALID_ARGUMENT, "mass_width is 0");
-    if (!aligned16({d->q, d->out, d->workspace}) || !strides_ok(d->q_stride, 3))
+    if (!aligned16({d->q, d->out, d->workspace}) || !strides_ok(d->q_stride, {d->num_seqs, static_cast<uint32_t>(d->queries), static_cast<uint32_t>(d->q_heads)}))
         return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign);
     if (!aligned4({d->table, d->lens, d->lse, d->mass, d->out_mass})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign4);
     MemoryDevice dev;

@@ -183,3 +183,19 @@ def test_misaligned_32_bit_buffers_are_refused(name, fields):
         setattr(d, field, 66)
         rc, why = call(name, d)
         assert rc == 1 and "4-byte aligned" in why, (field, rc, why)
+
+
+@pytest.mark.parametrize("name,field,value", [
+    ("bs_prompt_attention", "q_stride", (1 << 36, 64)), ("bs_prompt_attention", "k_stride", (1 << 36, 64)),
+    ("bs_prompt_attention", "v_stride", (1 << 36, 64)), ("bs_cache_write", "k_stride", (1 << 36, 64)),
+    ("bs_cache_write", "v_stride", (1 << 36, 64)), ("bs_cache_read", "position_seq_stride", 1 << 58),
+    ("bs_cache_read", "position_head_stride", 1 << 62)])
+def test_strides_beyond_64_bit_addresses_are_refused(name, field, value):
+    # legal by itself, but the last of 2^29 rows (or of 60,000 sequences) would be out of any address's reach
+    d = calls()[name]
+    for count, n in (("total_q", 1 << 29), ("total_k", 1 << 29), ("total", 1 << 29), ("num_seqs", 60000)):
+        if hasattr(d, count):
+            setattr(d, count, n)
+    setattr(d, field, (ctypes.c_int64 * len(value))(*value) if isinstance(value, tuple) else value)
+    rc, why = call(name, d)
+    assert rc == 1 and "reach" in why, (rc, why)
