@@ -32,6 +32,13 @@ void check(bs_status s) {
     throw py::error_already_set();
 }
 
+// A dimension as the C entries take it: one that 32 bits do not hold must not
+// become another.
+int32_t count(int64_t n) {
+    need(n < (int64_t{1} << 31), "a dimension of 2^31 or more is not supported");
+    return static_cast<int32_t>(n);
+}
+
 int type_of(const Tensor& t) {
     switch (t.scalar_type()) {
         case at::kFloat: return BS_F32;
@@ -122,12 +129,12 @@ py::tuple prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, co
     strides(q, d.q_stride);
     strides(k, d.k_stride);
     strides(v, d.v_stride);
-    d.total_q = q.size(0);
-    d.total_k = k.size(0);
-    d.num_seqs = cu_q.size(0) - 1;
-    d.q_heads = q.size(1);
-    d.kv_heads = k.size(1);
-    d.dim = q.size(2);
+    d.total_q = count(q.size(0));
+    d.total_k = count(k.size(0));
+    d.num_seqs = count(cu_q.size(0) - 1);
+    d.q_heads = count(q.size(1));
+    d.kv_heads = count(k.size(1));
+    d.dim = count(q.size(2));
     d.dtype = type_of(q);
     d.causal = causal;
     d.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(q.size(2), 1))));
@@ -158,10 +165,10 @@ struct Cache {
         c.v = static_cast<int8_t*>(v.data_ptr());
         c.k_scale = k_scale.data_ptr<float>();
         c.v_scale = v_scale.data_ptr<float>();
-        c.num_blocks = k.size(0);
-        c.kv_heads = k.size(1);
-        c.block = k.size(2);
-        c.dim = k.size(3);
+        c.num_blocks = count(k.size(0));
+        c.kv_heads = count(k.size(1));
+        c.block = count(k.size(2));
+        c.dim = count(k.size(3));
     }
 
     void write(const Tensor& x, const Tensor& y, const Tensor& cu, const Tensor& table, const Tensor& start,
@@ -181,9 +188,9 @@ struct Cache {
         d.v = y.const_data_ptr();
         strides(x, d.k_stride);
         strides(y, d.v_stride);
-        d.total = x.size(0);
-        d.num_seqs = n;
-        d.table_width = table.size(1);
+        d.total = count(x.size(0));
+        d.num_seqs = count(n);
+        d.table_width = count(table.size(1));
         d.dtype = type_of(x);
         check(bs_cache_write(&c, &d, to.stream));
         to.uses({&k, &v, &k_scale, &v_scale, &x, &y, &cu, &table, &start});
@@ -210,9 +217,9 @@ struct Cache {
         const Tensor b = values ? at::empty({n, heads, positions.size(-1), k.size(3)}, options) : Tensor();
         d.k = keys ? a.data_ptr() : nullptr;
         d.v = values ? b.data_ptr() : nullptr;
-        d.num_seqs = n;
-        d.table_width = table.size(1);
-        d.count = positions.size(-1);
+        d.num_seqs = count(n);
+        d.table_width = count(table.size(1));
+        d.count = count(positions.size(-1));
         d.dtype = dtype == at::kFloat ? BS_F32 : dtype == at::kHalf ? BS_F16 : BS_BF16;
         check(bs_cache_read(&c, &d, to.stream));
         to.uses({&k, &v, &k_scale, &v_scale, &table, &lens, &positions});
@@ -243,16 +250,16 @@ struct Cache {
                      "mass must be contiguous float32 [sequences, kv_heads, width]");
             d.mass = mass ? mass->const_data_ptr<float>() : nullptr;
             d.out_mass = sum.data_ptr<float>();
-            d.mass_width = sum.size(2);
+            d.mass_width = count(sum.size(2));
         }
         d.q = q.const_data_ptr();
         strides(q, d.q_stride);
         d.out = out.data_ptr();
         d.lse = with_lse ? lse.data_ptr<float>() : nullptr;
-        d.num_seqs = n;
-        d.table_width = table.size(1);
-        d.queries = q.size(1);
-        d.q_heads = q.size(2);
+        d.num_seqs = count(n);
+        d.table_width = count(table.size(1));
+        d.queries = count(q.size(1));
+        d.q_heads = count(q.size(2));
         d.dtype = type_of(q);
         d.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(q.size(3), 1))));
         size_t bytes = 0;
@@ -290,10 +297,10 @@ struct Cache {
         d.kept = kept.data_ptr<int32_t>();
         d.new_lens = new_lens.data_ptr<int32_t>();
         d.new_mass = new_mass.data_ptr<float>();
-        d.num_seqs = n;
-        d.table_width = table.size(1);
-        d.new_table_width = new_table.size(1);
-        d.mass_width = mass.size(2);
+        d.num_seqs = count(n);
+        d.table_width = count(table.size(1));
+        d.new_table_width = count(new_table.size(1));
+        d.mass_width = count(mass.size(2));
         d.budget = budget;
         d.sinks = sinks;
         d.recent = recent;

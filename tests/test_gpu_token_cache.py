@@ -590,3 +590,18 @@ def test_attention_small_weights_beside_a_large_one_and_a_large_scale(nats, dtyp
     bound = R.UNIT[dtype] * ref.abs() + (R.UNIT[F16] + 2.0 ** -12) * (1 + 2.0 ** -7) * weighted + 2.0 ** -30 * 0.5 * codes
     assert ((out.double() - ref).abs() <= bound).all()
 
+
+
+def test_dimensions_past_32_bits_are_refused():
+    cache, at = M.TokenCache.empty(2, 1, 16, block=16), R.i32([0])
+    x = torch.zeros((1, 1, 16), dtype=F16, device="cuda").expand(2 ** 32 + 1, 1, 16)          # 1 row in 32 bits
+    with pytest.raises(ValueError, match="2\\^31"):
+        cache.write(x, x, R.cu([1]), R.i32([[0]]), at)
+    with pytest.raises(ValueError, match="2\\^31"):
+        M.prompt_attention(x[:1], x, x, R.cu([1]), R.cu([1]))
+    many = torch.zeros((1, 2 ** 32 + 1), dtype=torch.int32, device="cuda")                    # (17 GB)
+    with pytest.raises(ValueError, match="2\\^31"):
+        cache.read(R.i32([[0]]), R.i32([1]), many, keys=False, values=False)
+    with pytest.raises(ValueError, match="2\\^31"):
+        cache.attention(x[:1, None], many, R.i32([1]))
+    del many
