@@ -104,6 +104,24 @@ Tensor scratch(size_t bytes, at::Device device) {
     return bytes ? at::empty({static_cast<int64_t>(bytes)}, at::TensorOptions().dtype(at::kByte).device(device)) : Tensor();
 }
 
+// These operators have no gradients.  An output made from something that needs
+// one says so when a backward pass reaches it, where it would be left out of
+// the pass without a word.
+struct NoGradient : torch::autograd::Function<NoGradient> {
+    static Tensor forward(torch::autograd::AutogradContext*, const Tensor& made, const Tensor&) { return made; }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+        TORCH_CHECK(false, "the token-memory operators have no gradient: use them under torch.no_grad() or on detached tensors");
+        return {};
+    }
+};
+
+Tensor from(const Tensor& made, std::initializer_list<const Tensor*> inputs) {
+    if (made.defined() && at::GradMode::is_enabled())
+        for (const Tensor* t : inputs)
+            if (t->requires_grad()) return NoGradient::apply(made, *t);
+    return made;
+}
+
 py::object maybe(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
 
 py::tuple prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const MaybeTensor& given_cu_k,
@@ -146,7 +164,7 @@ py::tuple prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, co
     check(bs_prompt_attention(&d, to.stream));
     to.uses({&q, &k, &v, &cu_q, &cu_k});
     to.gives({&out, &lse});
-    return py::make_tuple(out, maybe(lse));
+    return py::make_tuple(from(out, {&q, &k, &v}), maybe(from(lse, {&q, &k})));
 }
 
 struct Cache {
@@ -273,7 +291,8 @@ struct Cache {
         if (given_out) to.uses({&sum});
         else to.gives({&sum});
         to.gives({&out, &lse});
-        return py::make_tuple(out, maybe(lse), maybe(sum));
+        if (!given_out) sum = mass ? from(sum, {&q, &*mass}) : from(sum, {&q});
+        return py::make_tuple(from(out, {&q}), maybe(from(lse, {&q})), maybe(sum));
     }
 
     py::tuple evict(const Tensor& mass, const Tensor& table, const Tensor& lens, const Tensor& new_table, int64_t budget, int64_t sinks,
@@ -312,7 +331,7 @@ struct Cache {
         check(bs_cache_evict(&c, &d, to.stream));
         to.uses({&k, &v, &k_scale, &v_scale, &mass, &table, &lens, &new_table});
         to.gives({&kept, &new_lens, &new_mass});
-        return py::make_tuple(kept, new_lens, new_mass);
+        return py::make_tuple(kept, new_lens, from(new_mass, {&mass}));
     }
 };
 

@@ -15,7 +15,9 @@ gives up are rows for an :class:`Index`, found again by its search.
 Everything is a CUDA tensor; calls are asynchronous on `stream` (default: the
 current stream of the tensors' device) and never wait for the lengths, tables
 and positions, which stay on the device.  What only the device can see to be
-wrong is skipped and sets a bit that :func:`take_errors` returns.  C entries:
+wrong is skipped and sets a bit that :func:`take_errors` returns.  There are no
+gradients: a backward pass that reaches an output raises, and what is written
+to a cache is cut off from the pass that made it.  C entries:
 bs_prompt_attention, bs_cache_* of include/bsearch.h.
 """
 from __future__ import annotations

@@ -605,3 +605,24 @@ def test_dimensions_past_32_bits_are_refused():
     with pytest.raises(ValueError, match="2\\^31"):
         cache.attention(x[:1, None], many, R.i32([1]))
     del many
+
+
+def test_backward_through_an_output_raises():
+    pool, table, q = attention_case(63, [50], 4, 2, 32, 64, 1, F16)
+    cache, at, mass = M.TokenCache(*pool), R.i32([50]), torch.rand((1, 2, 64), device="cuda")
+    k = torch.randn((5, 2, 64), device="cuda").to(F16)
+    plain = [*M.prompt_attention(q[0], k, k, R.cu([1]), R.cu([5]), with_lse=True), *cache.attention(q, table, at, with_lse=True, mass=mass)]
+    assert not any(t.requires_grad for t in plain)
+    k.requires_grad_(), mass.requires_grad_()
+    some = [*M.prompt_attention(q[0], k, k, R.cu([1]), R.cu([5]), with_lse=True), cache.attention(q, table, at, mass=mass)[2]]
+    spare = ({0, 1, 2} - set(table[0].tolist())).pop()
+    some.append(cache.evict(mass, table, at, R.i32([[spare]]), 32)[2])
+    q.requires_grad_()
+    some += cache.attention(q, table, at, with_lse=True, with_mass=True)
+    for t in some:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            (t.float().sum() + q.float().sum()).backward()
+    same = [*M.prompt_attention(q[0], k, k, R.cu([1]), R.cu([5]), with_lse=True), *cache.attention(q, table, at, with_lse=True, mass=mass)]
+    assert all(torch.equal(a, b) for a, b in zip(plain, same))
+    with torch.no_grad():
+        assert not any(t.requires_grad for t in cache.attention(q, table, at, with_lse=True, mass=mass))
