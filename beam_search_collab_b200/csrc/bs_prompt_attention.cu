@@ -1017,6 +1017,16 @@ cudaError_t tensor_map(CUtensorMap* map, const void* p, int32_t dtype, int32_t d
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// Polls of a wait before it gives up: BSEARCH_WAIT_POLLS where that is a number
+// and nothing else.
+uint32_t wait_polls() {
+    const char* s = std::getenv("BSEARCH_WAIT_POLLS");
+    if (!s || *s < '0' || *s > '9') return kPolls;
+    char* end = nullptr;
+    const unsigned long n = std::strtoul(s, &end, 10);
+    return *end || n > 0xffffffffu ? kPolls : static_cast<uint32_t>(n);
+}
+
 uint32_t tile_tokens(const bs_prompt_attention_desc& d) { return kRows / static_cast<uint32_t>(d.q_heads / d.kv_heads); }
 
 // Pairs of tiles times key heads, at most.
@@ -1073,8 +1083,7 @@ cudaError_t launch_prompt_attention(const bs_prompt_attention_desc& d, const Mem
     PromptArgs a{};
     a.d = d;
     a.errors = dev.errors;
-    const char* polls = std::getenv("BSEARCH_WAIT_POLLS");
-    a.polls = polls ? static_cast<uint32_t>(std::strtoul(polls, nullptr, 10)) : kPolls;
+    a.polls = wait_polls();
     a.group = d.q_heads / d.kv_heads;
     a.tile_tokens = tile_tokens(d);
     a.chunks = chunks_of(d, dev);

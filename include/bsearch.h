@@ -293,7 +293,11 @@ typedef struct bs_token_cache {
  * of Lq sees the keys j <= i + Lk - Lq (the last query sees all), else all.
  * Query head h goes with key head h / (q_heads / kv_heads).
  *   s_j = scale * <q, k_j>,  lse = log sum_j exp(s_j),  out = sum_j exp(s_j - lse) v_j
- * A query that sees no key gives out = 0, lse = -infinity. */
+ * A query that sees no key gives out = 0, lse = -infinity.
+ * Every wait inside the kernel is bounded; one that gives up stores nothing and
+ * sets error bit 1.  The environment variable BSEARCH_WAIT_POLLS, read at each
+ * call, is the bound as a number of polls (default 4194304; 0, for tests of
+ * this path: the first wait gives up; what is not a number is ignored). */
 typedef struct bs_prompt_attention_desc {
     const void* q;            /* [total_q][q_heads][dim]                      */
     const void* k;            /* [total_k][kv_heads][dim]                     */

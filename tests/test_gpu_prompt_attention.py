@@ -278,3 +278,12 @@ def test_rows_whose_scores_are_far_below_zero_and_far_above(dtype):
     q, k, v = inputs(42, 370, 370, 4, 2, 64, dtype)
     k[:, :, 0], q[:, :, 0] = 20.0, torch.linspace(-60, 60, 370, device="cuda")[:, None].to(dtype)
     check(q, k, v, lens, lens)
+
+
+@pytest.mark.parametrize("value", ["", "many", "-1", "0x", "1e3", "0 ", "99999999999999999999999"])
+def test_what_is_not_a_number_of_polls_is_ignored(value, monkeypatch):
+    q, k, v = inputs(46, 40, 40, 4, 4, 64, F16)
+    good, _ = M.prompt_attention(q, k, v, R.cu([40]))
+    monkeypatch.setenv("BSEARCH_WAIT_POLLS", value)
+    got, _ = M.prompt_attention(q, k, v, R.cu([40]))
+    assert M.take_errors() == 0 and torch.equal(got, good)
