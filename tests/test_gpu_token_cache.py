@@ -1,5 +1,6 @@
 """GPU: the 8-bit token cache (writing, reading, attention, eviction) against
 the operators' definitions."""
+import ctypes
 import math
 import threading
 import time
@@ -7,6 +8,7 @@ import time
 import pytest
 import torch
 
+import memory_abi as A
 import memory_ref as R
 from beam_search_collab_b200 import BSearchError
 from beam_search_collab_b200 import memory as M
@@ -626,3 +628,20 @@ def test_backward_through_an_output_raises():
     assert all(torch.equal(a, b) for a, b in zip(plain, same))
     with torch.no_grad():
         assert not any(t.requires_grad for t in cache.attention(q, table, at, with_lse=True, mass=mass))
+
+
+# ---- workspaces -------------------------------------------------------------
+
+def test_many_query_rows_need_little_workspace():
+    c = A._Cache(None, None, None, None, 1000, 1, 64, 128)
+    for queries, q_heads in ((1024, 128), (1024, 1), (16, 128), (3, 128)):
+        d, n = A._Attention(queries=queries, q_heads=q_heads, num_seqs=4, table_width=2048, dtype=1, scale=1.0), ctypes.c_size_t()
+        assert A._lib().bs_cache_attention_workspace(c, d, n) == 0
+        assert n.value < 160e6, (queries, q_heads, n.value)
+
+
+@pytest.mark.parametrize("queries,hq", [(64, 128), (300, 128), (1000, 3)])
+def test_attention_many_query_rows(queries, hq):
+    lens = [1100, 2000, 30]
+    pool, table, q = attention_case(64, lens, hq, 1, 64, 64, queries, BF16)
+    check_attention(pool, table, q, lens)
