@@ -368,7 +368,10 @@ BS_API bs_status bs_cache_read(const bs_token_cache* cache, const bs_cache_read_
  *                       key head h of exp(s_j - lse)        (j < lens[b])
  * and 0 for lens[b] <= j < mass_width; mass may be NULL (zeros) or out_mass.
  * Weights of tokens at and past mass_width have no place: they are left out,
- * and error bit 4 is set. */
+ * and error bit 4 is set.  With out_mass the workspace holds a score of every
+ * query row and place of the tables, in use or not: 4 * num_seqs * queries *
+ * q_heads * table_width * block bytes (32 sequences of 32 heads over tables of
+ * 131,072 tokens: 0.54 GB). */
 typedef struct bs_cache_attention_desc {
     const void* q;            /* [num_seqs][queries][q_heads][dim]            */
     int64_t q_stride[3];      /* elements from sequence to sequence, token to token, head to head */
