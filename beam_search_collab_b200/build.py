@@ -112,15 +112,22 @@ def build(force: bool = False, verbose: bool = False) -> str:
               "-L", LIB_DIR, "-lbsearch_b200", "-Wl,-rpath,$ORIGIN/../lib"])
     mem_src = os.path.join(CSRC, "memory_py.cpp")
     if force or _stale(MEMORY_PY, [mem_src, LIB, os.path.join(INCLUDE, "bsearch.h")]):
-        _run(_memory_py_command(mem_src))
+        cmd = _memory_py_command(mem_src)
+        if cmd:
+            _run(cmd)
+        else:
+            print(f"PyTorch is not installed: {MEMORY_PY} (beam_search_collab_b200.memory) is not built", file=sys.stderr)
     return LIB
 
 
-def _memory_py_command(src: str) -> list[str]:
-    """The token-memory operators' binding for PyTorch tensors (beam_search_collab_b200/_memory.so)."""
+def _memory_py_command(src: str) -> list[str] | None:
+    """The token-memory operators' binding for PyTorch tensors (beam_search_collab_b200/_memory.so); None without PyTorch,
+    which nothing else that is built here needs."""
     import sysconfig
-
-    import torch
+    try:
+        import torch
+    except ImportError:
+        return None
     from torch.utils import cpp_extension as ext
     cmd = [_cxx(), "-std=c++17", "-O2", "-shared", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_memory",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE,

@@ -199,3 +199,15 @@ def test_strides_beyond_64_bit_addresses_are_refused(name, field, value):
     setattr(d, field, (ctypes.c_int64 * len(value))(*value) if isinstance(value, tuple) else value)
     rc, why = call(name, d)
     assert rc == 1 and "reach" in why, (rc, why)
+
+
+def test_the_build_needs_no_pytorch(monkeypatch, capfd):
+    import sys
+
+    from beam_search_collab_b200 import build
+    ran = []
+    monkeypatch.setitem(sys.modules, "torch", None)              # import torch: ImportError
+    monkeypatch.setattr(build, "_run", ran.append)
+    monkeypatch.setattr(build, "_stale", lambda target, sources: target == build.MEMORY_PY)
+    assert build.build() == build.LIB and not ran
+    assert "memory" in capfd.readouterr().err
