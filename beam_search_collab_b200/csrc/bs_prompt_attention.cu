@@ -37,6 +37,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdlib>
 
 #include "bs_device.cuh"
@@ -987,14 +988,15 @@ using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, voi
                               CUtensorMapFloatOOBfill);
 
 cudaError_t encoder(EncodeFn& out) {
-    static EncodeFn fn = nullptr;
+    static std::atomic<EncodeFn> known{nullptr};       // (threads may look it up at once)
+    EncodeFn fn = known.load();
     if (!fn) {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult r;
         const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r);
         if (e != cudaSuccess) return e;
         if (r != cudaDriverEntryPointSuccess || !p) return cudaErrorNotSupported;
-        fn = reinterpret_cast<EncodeFn>(p);
+        known.store(fn = reinterpret_cast<EncodeFn>(p));
     }
     out = fn;
     return cudaSuccess;
