@@ -287,3 +287,31 @@ def test_what_is_not_a_number_of_polls_is_ignored(value, monkeypatch):
     monkeypatch.setenv("BSEARCH_WAIT_POLLS", value)
     got, _ = M.prompt_attention(q, k, v, R.cu([40]))
     assert M.take_errors() == 0 and torch.equal(got, good)
+
+
+def test_keys_and_values_with_heads_outermost():
+    lens = [200, 57]
+    q, k, v = inputs(51, 257, 257, 6, 2, 80, F16)
+    one, lse = check(q, k, v, lens, lens)
+    k, v = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in (k, v))
+    two, lse2 = M.prompt_attention(q, k, v, R.cu(lens), with_lse=True)
+    assert torch.equal(one, two) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lens_q,lens_k,at", [([100], [100], 20), ([300, 40], [300, 40], 20),          # in an item's first tile of keys
+                                              ([64], [6000], 5950), ([64], [6000], 20)])               # keys in several pieces
+def test_values_that_are_not_finite_in_first_tiles_and_pieces(dtype, lens_q, lens_k, at):
+    q, k, v = inputs(52, sum(lens_q), sum(lens_k), 2, 1, 64, dtype)
+    v[at, 0, 3], v[at + 5, 0, 7] = math.inf, math.nan
+    out, _ = M.prompt_attention(q, k, v, R.cu(lens_q), R.cu(lens_k))
+    assert M.take_errors() == 0
+    first = out[:lens_q[0]].float()
+    sees = torch.arange(lens_q[0], device="cuda") + lens_k[0] - lens_q[0]
+    a, b = sees >= at, sees >= at + 5
+    assert (first[a][:, :, 3] == math.inf).all() and torch.isfinite(first[~a]).all()
+    assert torch.isnan(first[b][:, :, 7]).all() and torch.isfinite(first[~b][:, :, 7]).all()
+    ref, _, weighted, _ = R.prompt(q, k, torch.nan_to_num(v, 0.0, 0.0, 0.0), lens_q, lens_k, True, 0.125)
+    rest = [i for i in range(64) if i not in (3, 7)]
+    off = (out.double() - ref)[:, :, rest].abs() - R.out_bound(ref, weighted, dtype, R.UNIT[dtype])[:, :, rest]
+    assert off.max() <= 0

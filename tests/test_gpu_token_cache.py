@@ -645,3 +645,44 @@ def test_attention_many_query_rows(queries, hq):
     lens = [1100, 2000, 30]
     pool, table, q = attention_case(64, lens, hq, 1, 64, 64, queries, BF16)
     check_attention(pool, table, q, lens)
+
+
+# ---- branches that other sizes do not reach ---------------------------------
+
+@pytest.mark.parametrize("block,dim", [(16, 64), (64, 128), (128, 96)])
+def test_write_of_strided_rows(block, dim):
+    # slices of a fused projection, heads outermost, one row or head for all
+    g = gen(50)
+    lens, start, heads = [100, 0, 7, 129], [60, 30, 127, 1], 3
+    counts = [-(-(n + s) // block) for n, s in zip(lens, start)]
+    table, _ = R.random_table(g, counts, 2)
+    pool = R.random_pool(g, sum(counts) + 2, heads, block, dim)
+    x = torch.randn((236, 12, dim), generator=g, device="cuda").to(BF16)
+    fused = x[:, 6:9], x[:, 9:]
+    outermost = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in fused]
+    same = x[:, 6:7].expand(-1, 3, -1), x[:1, 9:].expand(236, -1, -1)
+    for k, v in (fused, outermost, same):
+        one, two = [p.clone() for p in pool], [p.clone() for p in pool]
+        M.TokenCache(*one).write(k, v, R.cu(lens), table, R.i32(start))
+        M.TokenCache(*two).write(k.contiguous(), v.contiguous(), R.cu(lens), table, R.i32(start))
+        assert M.take_errors() == 0 and all(torch.equal(a, b) for a, b in zip(one, two))
+
+
+@pytest.mark.parametrize("n_seqs,heads,n", [(1, 1, 400000), (20, 8, 50001)])
+def test_evict_rows_that_shared_memory_does_not_hold(n_seqs, heads, n):
+    # more than 47,104 keys for a block: one row over a cluster of 8, and so many rows that each has one block
+    g = gen(53)
+    budget, sinks, recent, block, dim = 777, 4, 100, 128, 16
+    mass = torch.rand((n_seqs, heads, n), generator=g, device="cuda")
+    mass[:, 0] = torch.round(mass[:, 0] * 1000)              # equal ones at the threshold
+    lens = [n - 13 * i for i in range(n_seqs)]
+    table = torch.randint(0, 50, (n_seqs, -(-n // block)), generator=g, device="cuda").to(torch.int32)
+    new_table = (50 + torch.arange(n_seqs * 7, device="cuda")).view(n_seqs, 7).to(torch.int32)
+    cache = M.TokenCache(*R.random_pool(g, 50 + n_seqs * 7, heads, block, dim))
+    kept, new_lens, new_mass = cache.evict(mass, table, R.i32(lens), new_table, budget, sinks=sinks, recent=recent)
+    assert M.take_errors() == 0 and (new_lens == budget).all()
+    for b, m in enumerate(lens):
+        best = torch.sort(mass[b, :, sinks:m - recent], dim=1, descending=True, stable=True).indices
+        ends = torch.cat((torch.arange(sinks, device="cuda"), torch.arange(m - recent, m, device="cuda"))).repeat(heads, 1)
+        want = torch.cat((best[:, :budget - sinks - recent] + sinks, ends), 1).sort(1).values
+        assert torch.equal(kept[b].long(), want) and torch.equal(new_mass[b], mass[b].gather(1, want))
