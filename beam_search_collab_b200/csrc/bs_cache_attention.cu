@@ -19,9 +19,9 @@
 // share of a fragment is what lies side by side in memory.
 //
 // Codes become f16 exactly (|code| <= 128); bf16 queries become f16 exactly
-// too, each row scaled by a power of two (elements 2^-31 below the row's
-// largest and less lose bits, far under a 32-bit sum's rounding).  Scores,
-// weights' sums and outputs are 32-bit.  Where a weight meets the values, its
+// too, each row scaled by a power of two (elements below 2^-29 of the row's
+// largest lose bits, far under a 32-bit sum's rounding).  Scores, weights' sums
+// and outputs are 32-bit.  Where a weight meets the values, its
 // product with their scale is rounded to f16: by 2^-11 of itself, as much as
 // an f16 output's own rounding, or, where that is more (f16 has no exponents
 // below), by 2^-30 of the largest weight times the largest value scale (at

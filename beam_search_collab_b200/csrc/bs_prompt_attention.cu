@@ -21,9 +21,10 @@
 //             softmax runs, the tensor pipe has the other tile's work
 //   softmax   S_t to registers, P_t = 2^(scale' S_t - m) back to TMEM in the
 //             inputs' 16-bit type.  m is moved only when a weight would be
-//             over 2^8 (then O_t, in TMEM, is rescaled), so most tiles touch
-//             O_t not at all and no maximum is taken before the exponentials;
-//             sums are 32-bit of the unrounded P.
+//             over 2^8 (then O_t, in TMEM, is rescaled, and so are the tile's
+//             weights that are there already, rounded a second time), so most
+//             tiles touch O_t not at all and no maximum is taken before the
+//             exponentials; sums are 32-bit of the unrounded P.
 // TMEM (512 columns): S0 S1 O0 O1, 128 columns each.
 //
 // Keys of other sequences or of the future that a tile also covers are set to
@@ -424,20 +425,22 @@ __device__ __forceinline__ bool read_next(const void* answer, uint32_t& block) {
 
 // BOXES: 64-column boxes of a row (1: dim <= 64, 2: dim <= 128).
 // Work: 4 * dim operations per query head and visible pair.  Measured: one
-// prompt of 16,384 tokens, 16/4 heads of 128, 0.90 ms (1.22 PFLOP/s; a large
-// matrix product reaches 1.65 here); 13 prompts of 7,196 tokens in all, 32/8
-// heads, 110 us (0.61); 24 tokens 7 us.  On long prompts the tensor pipe is
-// busy 53% of the cycles and the exponentials' pipe 53%: what bounds it is the
-// chain S -> weights -> P V of each tile, which only the other tile hides (a
-// pair of tiles of keys takes 3,450 clocks, its products 2,048).  On short
-// ones it is also each item's last tile, with hidden keys (3,800 clocks), and
-// its outputs (3,700).  Not kept, at 16,384 tokens and the 13 prompts: two
-// blocks of one tile an SM 1.12 ms and 130 us; weights handed over in halves
-// 1.03 ms; scores in halves too, the next ones made meanwhile, 1.16 ms and 120
-// us; part of the exponentials as a polynomial, slower at every share; outputs
-// by tensor copies 115 us.  With the copying warp also finding items and
-// looking at hidden values, and items taken one ahead, the 13 prompts took 117
-// us and 11 of 3,888 tokens 39 (now 29).
+// prompt of 16,384 tokens, 16/4 heads of 128, 1.02 to 1.05 ms run after run
+// under the power cap (1.05 to 1.08 PFLOP/s; a large matrix product reaches 1.38
+// there), 0.89 ms in a burst (1.24 of 1.65); 13 prompts of 7,196 tokens in all,
+// 32/8 heads, 109 us (0.62); 24 tokens 7 us.  On long prompts the tensor pipe is
+// busy 53% of the cycles and the exponentials' pipe 53%: at 8,192 tokens a pair
+// of tiles takes 3,820 clocks with all that goes with it, its products 2,048
+// and its exponentials, 32,768 at 16 a clock, 2,048 as well.  What bounds it is
+// the chain S -> weights -> P V of each tile, which only the other tile hides.
+// On short ones it is also each item's last tile, with hidden keys (3,800
+// clocks), and its outputs (3,700).  Not kept, at 16,384 tokens (bursts) and
+// the 13 prompts: two blocks of one tile an SM 1.12 ms and 130 us; weights
+// handed over in halves 1.03 ms; scores in halves too, the next ones made
+// meanwhile, 1.16 ms and 120 us; part of the exponentials as a polynomial,
+// slower at every share; outputs by tensor copies 115 us.  With the copying
+// warp also finding items and looking at hidden values, and items taken one
+// ahead, the 13 prompts took 117 us and 11 of 3,888 tokens 39 (now 29).
 template <typename T, int BOXES>
 __global__ void __launch_bounds__(kThreads, 1) k_prompt(const __grid_constant__ PromptArgs a) {
     extern __shared__ unsigned char raw_smem[];

@@ -41,7 +41,8 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, with_
     """Attention of a packed batch of prompts (bs_prompt_attention).
 
     q [total_q, q_heads, dim], k and v [total_k, kv_heads, dim], float16 or
-    bfloat16, any token and head strides that are multiples of 8 elements.
+    bfloat16, any token and head strides that are positive multiples of 8
+    elements (no broadcast tensors).
     cu_q and cu_k (default: cu_q), int32 [sequences + 1]: where each sequence
     begins.  With `causal` a sequence's last query sees all its keys and each
     earlier query one fewer.  scale defaults to dim ** -0.5.  Returns (out,

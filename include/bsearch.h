@@ -267,9 +267,10 @@ BS_API bs_status bs_merge_shards(const float* dists, const uint32_t* ids, uint32
  *
  * dim is a multiple of 16 up to 128.  q, k and v have strides in elements
  * between tokens and between heads; they and the base address are multiples
- * of 16 bytes, the last dimension is contiguous.  Outputs are contiguous, of
- * 16-bit types 16-byte aligned; 32-bit buffers are 4-byte aligned.
- * scale is positive and finite. */
+ * of 16 bytes (0, a row or head for all, too, but not in bs_prompt_attention),
+ * the last dimension is contiguous.  Outputs are contiguous; out, the values
+ * that bs_cache_read writes and workspaces are 16-byte aligned, other 32-bit
+ * buffers 4-byte.  scale is positive and finite. */
 typedef enum bs_dtype { BS_F32 = 0, BS_F16 = 1, BS_BF16 = 2 } bs_dtype;
 
 /* The 8-bit cache: blocks of `block` tokens (16, 32, 64 or 128).  A value is
@@ -401,7 +402,8 @@ BS_API bs_status bs_cache_attention_workspace(const bs_token_cache* cache, const
  * which must not be blocks of any sequence of `table`.  kept[b][h][i] is the
  * old position of new position i (-1 past the end), new_mass its mass (0 past
  * the end), new_lens[b] = min(lens[b], budget).  A new block's scale is the
- * largest of its tokens' old scales; codes become rint(code * (old / new)). */
+ * largest of its tokens' old scales; codes become rint(code * (old / new)).
+ * The workspace is not used yet: bs_cache_evict_workspace gives 0. */
 typedef struct bs_cache_evict_desc {
     const float* mass;        /* [num_seqs][kv_heads][mass_width]             */
     const int32_t* table;     /* [num_seqs][table_width]                      */
