@@ -5,17 +5,18 @@
 // special-function pipe (16 int <-> float conversions a clock and SM: the
 // eviction's move took 60 us through it, as long as all its traffic), so
 // integers are made and read through a float's low bits.
-#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "bs_device.cuh"
 #include "bs_f32x2.cuh"
 #include "bs_memory.h"
+#include "bs_select.cuh"
 
 namespace bsb {
 
 using namespace dev;
+using namespace select;
 
 namespace {
 
@@ -308,60 +309,21 @@ struct EvictArgs {
     unsigned int* errors;
 };
 
-// Order of weights as integers: larger weight, larger key; NaN above all.
-__device__ __forceinline__ uint32_t mass_key(float f) { return isnan(f) ? 0xffffffffu : f2ord(f); }
-
-// Which tokens of one sequence stay for one head: a cluster of blocks holds
-// the row's keys in shared memory, a slice each (what does not fit is read
-// again from L2).  The m-th largest key among the free tokens is found by its
-// digits of 11, 11 and 10 bits, counted by every block and added up through
-// distributed shared memory; then each block numbers the tokens of its slice
-// that stay, in order, from what the blocks before it have.
+// Which tokens of one sequence stay for one head (bs_select.cuh): their weights
+// are read once, into shared memory; what does not fit is read again from L2.
 //   measured, 32 rows of 8,000 to 65,536 tokens: 26 us (one block a row, 8-bit
 //   digits from L2: 219).  4.7 MB come from DRAM; bound by counting in shared
 //   memory and the barriers between the digits.  16 rows of 18,000 and 868,000
 //   tokens, where most keys are read again from L2, take 168 us.
-constexpr uint32_t kBins = 2048;
-constexpr uint32_t kMostCached = 46 * 1024;       // keys of a slice in shared memory
-constexpr uint32_t kMostCluster = 8;
-
-// Exclusive prefix over the block of one number per thread, and the total.
-template <int THREADS>
-__device__ __forceinline__ uint32_t block_prefix(uint32_t x, uint32_t* warp_sums, uint32_t& total) {
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint32_t sum = x;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(kFull, sum, o);
-        if (lane >= static_cast<uint32_t>(o)) sum += up;
-    }
-    __syncthreads();                 // the last use of warp_sums is over
-    if (lane == 31) warp_sums[warp] = sum;
-    __syncthreads();
-    const uint32_t mine = lane < THREADS / 32 ? warp_sums[lane] : 0;
-    uint32_t before = lane < warp ? mine : 0, all = mine;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        before += __shfl_xor_sync(kFull, before, o);
-        all += __shfl_xor_sync(kFull, all, o);
-    }
-    total = all;
-    return before + sum - x;
-}
-
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_evict_select(const __grid_constant__ EvictArgs a, uint32_t cached) {
-    namespace cg = cooperative_groups;
     extern __shared__ uint32_t keys[];             // [cached]
-    __shared__ __align__(16) uint32_t count[3][kBins];
-    __shared__ uint32_t warp_sums[32];
-    __shared__ uint32_t slice_counts[2];           // tokens that stay for certain, tokens equal to the threshold
-    __shared__ uint32_t chosen[2];
+    __shared__ __align__(16) SelectShared shared;
     cudaGridDependencySynchronize();       // in every block, before anything of the caller's
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = cluster.block_rank(), blocks = cluster.num_blocks();
     const bs_cache_evict_desc& d = a.d;
-    const uint32_t h = blockIdx.x / blocks, b = blockIdx.y, t = threadIdx.x, lane = t & 31;
+    const uint32_t h = blockIdx.x / blocks, b = blockIdx.y, t = threadIdx.x;
     const uint64_t row = static_cast<uint64_t>(b) * a.c.kv_heads + h;
     const float* mass = d.mass + row * d.mass_width;
     int32_t* kept = d.kept + row * d.budget;
@@ -386,143 +348,25 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_evict_select(const 
         return;
     }
     // this block's slice of the row
-    const uint32_t width = ((n + blocks - 1) / blocks + 3) & ~3u;
-    const uint32_t first = min(rank * width, n), size = min(width, n - first);
-    const uint32_t lo = d.sinks, hi = n - d.recent;              // free tokens
-    auto key_of = [&](uint32_t i) { return i < cached ? keys[i] : mass_key(mass[first + i]); };
-    auto sync = [&]() {
-        if (blocks > 1) cluster.sync();
-        else __syncthreads();
-    };
-#pragma unroll
-    for (uint32_t i = t; i < 3 * kBins / 4; i += THREADS) reinterpret_cast<uint4*>(&count[0][0])[i] = make_uint4(0, 0, 0, 0);
+    uint32_t first, size;
+    select_slice(n, blocks, rank, first, size);
+    clear_counts<THREADS>(shared);
     for (uint32_t i0 = t; i0 < min(size, cached); i0 += 8 * THREADS) {
         float x[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) x[u] = i0 + u * THREADS < size ? mass[first + i0 + u * THREADS] : 0.f;
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            if (i0 + u * THREADS < min(size, cached)) keys[i0 + u * THREADS] = mass_key(x[u]);
+            if (i0 + u * THREADS < min(size, cached)) keys[i0 + u * THREADS] = select_key(x[u]);
     }
     __syncthreads();
-
-    uint32_t need = budget - d.sinks - d.recent;   // of the free tokens; fewer than there are
-    const bool any = need > 0;
-    uint32_t prefix = 0;
-    const uint32_t free0 = max(lo, first) - first, free1 = max(min(hi, first + size), first + free0) - first;   // of the slice
-    uint32_t above = 0;                            // free tokens of the slice above the threshold
-    if (any) {
-#pragma unroll 1
-        for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, known = pass == 1 ? 21 : 10;
-            const uint32_t mask = pass == 2 ? 1023 : 2047;
-            for (uint32_t i0 = free0; i0 < free1; i0 += 4 * THREADS) {    // (all lanes together)
-                uint32_t key[4];
-                bool in[4];
-#pragma unroll
-                for (uint32_t u = 0; u < 4; ++u) {
-                    const uint32_t i = i0 + u * THREADS + t;
-                    in[u] = i < free1;
-                    key[u] = in[u] ? key_of(i) : 0;
-                    if (pass) in[u] = in[u] && (key[u] ^ prefix) >> known == 0;
-                }
-#pragma unroll
-                for (uint32_t u = 0; u < 4; ++u) {
-                    const uint32_t digit = (key[u] >> shift) & mask;
-                    // a warp whose tokens all agree counts once: rows of equal weights do not queue up
-                    const uint32_t lead = __shfl_sync(kFull, digit, 0);
-                    if (__all_sync(kFull, in[u] && digit == lead)) {
-                        if (lane == 0) atomicAdd(&count[pass][digit], 32u);
-                    } else if (in[u]) {
-                        atomicAdd(&count[pass][digit], 1u);
-                    }
-                }
-            }
-            __syncwarp();
-            sync();
-            // bins from the largest digit down, kBins / THREADS to a thread
-            constexpr int kEach = kBins / THREADS;
-            uint32_t mine[kEach] = {}, sum = 0;
-            const uint32_t top_bin = kBins - (t + 1) * kEach;
-#pragma unroll
-            for (uint32_t x = 0; x < kMostCluster; ++x) {
-                if (x >= blocks) break;
-                const uint2* from = reinterpret_cast<const uint2*>(cluster.map_shared_rank(&count[pass][0], x) + top_bin);
-#pragma unroll
-                for (int u = 0; u < kEach / 2; ++u) {
-                    const uint2 c = from[u];
-                    mine[kEach - 1 - 2 * u] += c.x;
-                    mine[kEach - 2 - 2 * u] += c.y;
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < kEach; ++u) sum += mine[u];
-            uint32_t total;
-            uint32_t before = block_prefix<THREADS>(sum, warp_sums, total);
-#pragma unroll
-            for (int u = 0; u < kEach; ++u) {
-                if (before < need && need <= before + mine[u]) {
-                    chosen[0] = prefix | (kBins - 1 - (t * kEach + u)) << shift;
-                    chosen[1] = need - before;
-                }
-                before += mine[u];
-            }
-            __syncthreads();
-            prefix = chosen[0];
-            need = chosen[1];
-            const uint32_t digit = (prefix >> shift) & mask;
-#pragma unroll
-            for (int u = 0; u < kEach; ++u)
-                if (top_bin + u > digit) above += count[pass][top_bin + u];
-        }
-    }
-    // a token stays if it is not free, above the threshold, or one of the
-    // first `need` equal to it; both kinds are counted in one number
-    auto kind = [&](uint32_t i) -> uint32_t {      // 1: stays for certain, 65536: equal
-        const uint32_t at = first + i;
-        if (i >= size) return 0;
-        if (at < lo || at >= hi) return 1;
-        if (!any) return 0;
-        const uint32_t key = key_of(i);
-        return key > prefix ? 1 : key == prefix ? 65536u : 0;
-    };
-    uint32_t total_above;
-    block_prefix<THREADS>(above, warp_sums, total_above);
-    const uint32_t total_sure = total_above + size - (free1 - free0), total_equal = any ? count[2][prefix & 1023] : 0;
-    if (t == 0) {
-        slice_counts[0] = total_sure;
-        slice_counts[1] = total_equal;
-    }
-    sync();
-    uint32_t base = 0, base_equal = 0;
-    for (uint32_t x = 0; x < rank; ++x) {
-        base += cluster.map_shared_rank(&slice_counts[0], x)[0];
-        base_equal += cluster.map_shared_rank(&slice_counts[0], x)[1];
-    }
-    if (blocks > 1) cluster.sync();                // no block ends while another reads it
-    constexpr uint32_t kRun = 4;                   // tokens of a thread, side by side
-    for (uint32_t i0 = 0; i0 < size; i0 += kRun * THREADS) {
-        uint32_t k[kRun], sum = 0, total;
-#pragma unroll
-        for (uint32_t u = 0; u < kRun; ++u) {
-            k[u] = kind(i0 + t * kRun + u);
-            sum += k[u];                           // (at most 4096 of each kind in the block)
-        }
-        const uint32_t before = block_prefix<THREADS>(sum, warp_sums, total);
-        uint32_t to = base + (before & 0xffffu), eq = base_equal + (before >> 16);
-#pragma unroll
-        for (uint32_t u = 0; u < kRun; ++u) {
-            const uint32_t i = first + i0 + t * kRun + u;
-            if (k[u] == 1 || (k[u] && eq < need)) {
-                kept[to + min(eq, need)] = i;
-                new_mass[to + min(eq, need)] = mass[i];
-            }
-            to += k[u] & 1;
-            eq += k[u] >> 16;
-        }
-        base += total & 0xffffu;
-        base_equal += total >> 16;
-    }
+    select_row<THREADS>(
+        cluster, shared, n, first, size, d.sinks, d.recent, budget,
+        [&](uint32_t i) { return i < cached ? keys[i] : select_key(mass[first + i]); },
+        [&](uint32_t slot, uint32_t i) {
+            kept[slot] = i;
+            new_mass[slot] = mass[i];
+        });
 }
 
 constexpr int kMoveThreads = 128;      // (256: 53 us for the 234 MB that four long contexts move, 128: 48, now 45)
