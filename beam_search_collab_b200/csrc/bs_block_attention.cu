@@ -1,0 +1,401 @@
+// bs_block_attention.cu -- attention over chosen blocks of the 8-bit token
+// cache, and the joint attention over shared and own tokens
+// (include/bsearch.h, bs_block_attention, bs_shared_attention).
+//
+// The products, their layout and their roundings are those of
+// bs_cache_attention.cu (bs_cache_tile.cuh).  What differs is where a tile's
+// tokens come from: a list of table columns for each query and key head.  A
+// cluster of blocks takes a segment (a query and a key head), a part of its
+// list each; the list's entries are looked up in the table once, into shared
+// memory, those without a visible token left out, so that the copies of tiles
+// wait for no chain of loads.  The blocks of a cluster join their outputs
+// through distributed shared memory: no second kernel, no workspace.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "bs_cache_tile.cuh"
+#include "bs_device.cuh"
+#include "bs_memory.h"
+
+namespace bsb {
+
+using namespace dev;
+using namespace tile;
+namespace cg = cooperative_groups;
+
+namespace {
+
+constexpr uint32_t kMostIds = 256;     // entries looked up at a time
+constexpr uint32_t kMostCluster = 8;
+template <int NT>
+constexpr int kStagesOf = NT == 1 ? 2 : 3;
+constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+
+struct RowsArgs {
+    bs_token_cache c;
+    bs_shared_attention_desc d;        // of a list of blocks: what both have
+    const int32_t* blocks;             // [num_seqs][queries][kv_heads][count]
+    unsigned int* errors;
+    uint32_t count;
+    uint32_t group;                    // query heads per key head
+    uint32_t rows;                     // of a segment
+    uint32_t block_log2;
+};
+
+template <int NW>
+constexpr int kListStage = kStageBytes<NW> + 16;               // and the halves' first positions
+constexpr int kIdBytes = kMostIds * 8 + kWarps * 4;
+// (the entries lie where the outputs are joined later: with 16 query rows two blocks just fit an SM)
+template <int NW, int NT>
+constexpr int kJoinOrIds = kJoinBytes<NW, NT> > kIdBytes ? kJoinBytes<NW, NT> : kIdBytes;
+template <int NW, int NT>
+constexpr size_t kRowsSmem = kWarps * kStagesOf<NT> * kListStage<NW> + (kWarps + 1) * 8 * NT * 2 * 4 + kJoinOrIds<NW, NT>;
+
+__device__ __forceinline__ uint32_t tokens_of(const RowsArgs& a, const int32_t* lens, uint32_t i, uint32_t width) {
+    const int32_t len = lens[i];
+    const int64_t most = static_cast<int64_t>(width) * a.c.block;
+    if (len >= 0 && len <= most) return len;
+    atomicOr(a.errors, kMemErrLength);
+    return len < 0 ? 0 : static_cast<uint32_t>(most);
+}
+
+template <int NW, int NT, bool LIST>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __grid_constant__ RowsArgs a) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    constexpr int kDim = NW * 16, kRows = 8 * NT, kStages = kStagesOf<NT>;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    unsigned char* const ring = smem + warp * kStages * kListStage<NW>;
+    float* const join_ml = reinterpret_cast<float*>(smem + kWarps * kStages * kListStage<NW>);     // [warps + 1][kRows][2]
+    float* const join_o = join_ml + (kWarps + 1) * kRows * 2;
+    int2* const ids = reinterpret_cast<int2*>(join_o);          // block, first position; till the outputs are joined
+    uint32_t* const found = reinterpret_cast<uint32_t*>(ids + kMostIds);      // [warps]
+
+    cudaGridDependencySynchronize();       // in every block, before anything of the caller's
+    const cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t rank = cluster.block_rank(), parts = cluster.num_blocks();
+    const bs_shared_attention_desc& d = a.d;
+    const uint32_t hkv = a.c.kv_heads, b = blockIdx.z, segment = blockIdx.x / parts, row0 = blockIdx.y * kRows;
+    const uint32_t h = LIST ? segment % hkv : segment, query = LIST ? segment / hkv : 0, block = a.c.block;
+    const uint32_t len = tokens_of(a, d.lens, b, d.table_width);
+
+    // this segment's query rows as the columns of K Q^T: column j is row row0 + j
+    uint32_t q[NT][NW][2];
+    float row_scale[NT][2];          // of columns 2c and 2c + 1
+    int32_t own_limit[NT][2];        // tokens of its own that row sees
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const uint32_t r = row0 + 8 * nt + g, col = row0 + 8 * nt + 2 * c;
+        const uint16_t* row = static_cast<const uint16_t*>(d.q) + b * d.q_stride[0] + static_cast<int64_t>(LIST ? query : r / a.group) * d.q_stride[1] +
+                              (static_cast<int64_t>(h) * a.group + r % a.group) * d.q_stride[2] + c * (NW * 4);
+        load_query_row<NW>(q[nt], row_scale[nt], row, r < a.rows, d.dtype != BS_F16, d.scale * 1.4426950408889634f, c);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            own_limit[nt][i] = static_cast<int32_t>(len) - d.queries + 1 + static_cast<int32_t>(LIST ? query : (col + i) / a.group);
+    }
+    float o[NT][NW][4];
+    float top[NT][2], sum[NT][2], unit = kFold / -kNoScore, inv_unit = -kNoScore;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        top[nt][0] = top[nt][1] = kNoScore;
+        sum[nt][0] = sum[nt][1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NW; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+    }
+
+    for (int source = LIST ? 1 : 0; source < 2; ++source) {
+        const int32_t* table;
+        const int32_t* list = nullptr;
+        uint32_t entries, width, tokens;           // tokens: some row sees those below
+        int32_t limit[NT][2];
+        if (source == 0) {                         // what the group shares
+            uint32_t m = 0;
+            while (m + 1 < d.num_groups && static_cast<uint32_t>(d.cu[m + 1]) <= b) ++m;
+            const int32_t first = d.cu[m], past = d.cu[m + 1];
+            const bool ok = first >= 0 && static_cast<uint32_t>(first) <= b && past > static_cast<int32_t>(b) && static_cast<uint32_t>(past) <= d.num_seqs;
+            if (!ok || d.cu[0] != 0 || static_cast<uint32_t>(d.cu[d.num_groups]) != d.num_seqs) atomicOr(a.errors, kMemErrLength);
+            width = d.shared_width;
+            table = d.shared_table + static_cast<uint64_t>(m) * width;
+            tokens = ok ? tokens_of(a, d.shared_lens, m, width) : 0;
+            entries = (tokens + block - 1) / block;
+        } else {
+            width = d.table_width;
+            table = d.table + static_cast<uint64_t>(b) * width;
+            const int32_t most = static_cast<int32_t>(len) - (LIST ? d.queries - 1 - static_cast<int32_t>(query) : 0);
+            tokens = most > 0 ? most : 0;
+            entries = LIST ? a.count : (tokens + block - 1) / block;
+            if (LIST) list = a.blocks + ((static_cast<uint64_t>(b) * d.queries + query) * hkv + h) * a.count;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) limit[nt][i] = source == 0 ? static_cast<int32_t>(tokens) : own_limit[nt][i];
+        // this block's part of the entries
+        const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(entries) * (rank + 1) / parts);
+        for (uint32_t from = static_cast<uint32_t>(static_cast<uint64_t>(entries) * rank / parts); from < end; from += kMostIds) {
+            // look them up; those without a token that is seen are left out
+            uint32_t held = 0;
+#pragma unroll
+            for (uint32_t e0 = 0; e0 < kMostIds; e0 += kThreads) {
+                const uint32_t e = from + e0 + threadIdx.x;
+                int64_t col = -1;
+                if (e < end) col = LIST ? list[e] : static_cast<int64_t>(e);
+                uint32_t id = kNoNode;
+                if (col >= 0 && col < width && col * block < tokens) {
+                    id = table[col];
+                    if (id >= a.c.num_blocks) {
+                        atomicOr(a.errors, kMemErrBlock);
+                        id = kNoNode;
+                    }
+                } else if (LIST && col >= width) {
+                    atomicOr(a.errors, kMemErrLength);
+                }
+                const unsigned in = __ballot_sync(kFull, id != kNoNode);
+                if (lane == 0) found[warp] = __popc(in);
+                __syncthreads();
+                uint32_t at = held + __popc(in & ((1u << lane) - 1));
+#pragma unroll
+                for (uint32_t x = 0; x < kWarps; ++x) {
+                    const uint32_t n = found[x];
+                    if (x < warp) at += n;
+                    held += n;
+                }
+                if (id != kNoNode) ids[at] = make_int2(id, static_cast<int32_t>(col * block));
+                __syncthreads();
+            }
+            const uint32_t tiles = ((held << a.block_log2) + kTile - 1) / kTile;
+            auto request = [&](uint32_t t, uint32_t stage) {
+                if (t < tiles) {
+                    unsigned char* s = ring + stage * kListStage<NW>;
+                    float* scales = reinterpret_cast<float*>(s + 2 * kTile * kPitch<NW>);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t at = t * kTile + 16 * half, e = at >> a.block_log2, in = at & (block - 1);
+                        const int2 entry = e < held ? ids[e] : make_int2(0, 0x40000000);
+                        const int32_t pos = entry.y + static_cast<int32_t>(in);
+                        if (pos < static_cast<int32_t>(tokens)) {
+                            const uint64_t slab = static_cast<uint64_t>(static_cast<uint32_t>(entry.x)) * hkv + h;
+                            const uint64_t row = ((slab << a.block_log2) + in) * kDim + lane * 16;
+                            const int8_t* k = a.c.k + row;
+                            const int8_t* v = a.c.v + row;
+#pragma unroll
+                            for (int j = 0; j < (NW + 1) / 2; ++j) {
+                                const uint32_t i = lane + 32 * j, r = i / NW + 16 * half, x = i % NW;
+                                if (NW % 2 && i >= 16 * NW) break;
+                                copy16(s + r * kPitch<NW> + unit_at<NW>(x, r), k + j * 512);
+                                copy16(s + (kTile + r) * kPitch<NW> + unit_at<NW>(x, r), v + j * 512);
+                            }
+                            if (lane < 2) copy4(scales + 2 * half + lane, (lane ? a.c.v_scale : a.c.k_scale) + slab);
+                        } else if (lane == 0) {       // no tokens to see: a value scale below zero says so
+                            scales[2 * half] = 0.f;
+                            scales[2 * half + 1] = -1.f;
+                        }
+                        if (lane == 2) reinterpret_cast<int32_t*>(scales)[4 + half] = pos;
+                    }
+                }
+                asm volatile("cp.async.commit_group;\n" ::: "memory");
+            };
+#pragma unroll
+            for (int i = 0; i < kStages - 1; ++i) request(warp + i * kWarps, i);
+            uint32_t stage = 0, fill = kStages - 1;
+            for (uint32_t t = warp; t < tiles; t += kWarps) {
+                asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
+                __syncwarp();
+                request(t + (kStages - 1) * kWarps, fill);       // the stage that the last tile used
+                fill = fill + 1 == kStages ? 0 : fill + 1;
+                const unsigned char* s = ring + stage * kListStage<NW>;
+                stage = stage + 1 == kStages ? 0 : stage + 1;
+                const float4 sc = *reinterpret_cast<const float4*>(s + 2 * kTile * kPitch<NW>);
+                const int2 first = *reinterpret_cast<const int2*>(s + 2 * kTile * kPitch<NW> + 16);
+                const float k_scale[2] = {sc.x, sc.z}, v_scale[2] = {sc.y, sc.w};
+                const int32_t pos[2] = {first.x, first.y};
+                float z[2][NT][4];           // [half]: tokens g and g + 8 (+ 16 half), columns 2c and 2c + 1
+                tile_scores<NW, NT>(z, s, q, g, c);
+                const bool edge = max(pos[0], pos[1]) + 16 > static_cast<int32_t>(tokens) - (LIST ? 0 : d.queries - 1);
+                bool move = fmaxf(v_scale[0], v_scale[1]) > 4.f * unit;
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            z[half][nt][i] *= row_scale[nt][i & 1] * k_scale[half];
+                            if (edge && pos[half] + static_cast<int32_t>(g) + (i & 2) * 4 >= limit[nt][i & 1]) z[half][nt][i] = -INFINITY;
+                            move |= z[half][nt][i] > top[nt][i & 1] + kSlack;
+                        }
+                if (__any_sync(kFull, move)) move_maxima<NW, NT>(z, v_scale, top, sum, o, unit, inv_unit);
+                tile_values<NW, NT>(z, s, v_scale, inv_unit, top, sum, o, g, c);
+                __syncwarp();
+            }
+            __syncthreads();               // `ids` is done with
+        }
+    }
+
+    float all_top[NT][2], all_sum[NT][2];
+    join_warps<NW, NT>(o, top, sum, unit, all_top, all_sum, join_o, join_ml, warp, lane);
+    auto row_at = [&](uint32_t r) {        // row of the outputs
+        const uint32_t i = LIST ? query : r / a.group;
+        return (static_cast<uint64_t>(b) * d.queries + i) * d.q_heads + h * a.group + (LIST ? r : r - i * a.group);
+    };
+    if (parts == 1) {
+        if (warp != 0) return;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t r = row0 + 8 * nt + 2 * c + i;
+                if (r >= a.rows) continue;
+                const float l = all_sum[nt][i], inv = l == 0.f ? 0.f : 1.f / l;
+                const uint64_t row = row_at(r);
+                if (g == 0 && d.lse) d.lse[row] = l == 0.f ? -INFINITY : (all_top[nt][i] + log2f(l)) * 0.6931471805599453f;
+#pragma unroll
+                for (int j = 0; j < NW; ++j) {
+                    const float x = o[nt][j][i] * inv, y = o[nt][j][2 + i] * inv;
+                    const uint64_t e = row * kDim + value_dim<NW>(j, g);
+                    if (d.dtype == BS_F16) *reinterpret_cast<__half2*>(static_cast<__half*>(d.out) + e) = __floats2half2_rn(x, y);
+                    else *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(d.out) + e) = __floats2bfloat162_rn(x, y);
+                }
+            }
+        return;
+    }
+    // the cluster's outputs as one: a thread has four dimensions of a row
+    float* const part_o = join_o + kRows * kDim;               // (read by warp 1 alone, a barrier ago)
+    float* const part_ml = join_ml + kWarps * kRows * 2;
+    if (warp == 0)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t r = 8 * nt + 2 * c + i;
+                if (g == 0) *reinterpret_cast<float2*>(part_ml + r * 2) = make_float2(all_top[nt][i], all_sum[nt][i]);
+#pragma unroll
+                for (int j = 0; j < NW; ++j)
+                    *reinterpret_cast<float2*>(part_o + r * kDim + value_dim<NW>(j, g)) = make_float2(o[nt][j][i], o[nt][j][2 + i]);
+            }
+    cluster.sync();
+    for (uint32_t x = rank * kThreads + threadIdx.x; x < kRows * kDim / 4; x += parts * kThreads) {
+        const uint32_t r = x / (kDim / 4), at = x % (kDim / 4) * 4;
+        if (row0 + r >= a.rows) break;
+        float2 ml[kMostCluster];
+        float m = kNoScore, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (uint32_t p = 0; p < kMostCluster; ++p) {
+            ml[p] = p < parts ? *reinterpret_cast<const float2*>(cluster.map_shared_rank(part_ml, p) + r * 2) : make_float2(kNoScore, 0.f);
+            m = fmaxf(m, ml[p].x);
+        }
+#pragma unroll
+        for (uint32_t p = 0; p < kMostCluster; ++p) {
+            if (p >= parts) break;
+            const float4 y = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part_o, p) + r * kDim + at);
+            const float w = exp2_fast(ml[p].x - m);
+            l += ml[p].y * w;
+            acc.x += y.x * w, acc.y += y.y * w, acc.z += y.z * w, acc.w += y.w * w;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const uint64_t row = row_at(row0 + r);
+        if (at == 0 && d.lse) d.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        uint2 u;
+        if (d.dtype == BS_F16) {
+            const __half2 lo = __floats2half2_rn(acc.x * inv, acc.y * inv), hi = __floats2half2_rn(acc.z * inv, acc.w * inv);
+            u = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        } else {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+            u = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        }
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(d.out) + row * kDim + at) = u;
+    }
+    cluster.sync();                        // no block ends while another reads it
+}
+
+// Blocks of a segment, by the time of its longest part and of all of them: a
+// block takes as long as kStart tiles to begin and end, and the join of a
+// cluster some more.
+uint32_t parts_of(uint64_t segments, uint64_t tokens, uint64_t resident) {
+    constexpr double kStart = 6, kJoin = 2;
+    uint32_t best = 1;
+    double least = 0;
+    for (uint32_t n = 1; n <= kMostCluster; n *= 2) {
+        const double waves = static_cast<double>((segments * n + resident - 1) / resident);
+        const double time = waves * (kStart + static_cast<double>(tokens) / kTile / n) + (n > 1 ? kJoin : 0);
+        if (n == 1 || time < least) {
+            least = time;
+            best = n;
+        }
+    }
+    return best;
+}
+
+template <int NW, int NT, bool LIST>
+cudaError_t launch_rows(const RowsArgs& a, const MemoryDevice& dev, cudaStream_t stream) {
+    const cudaError_t e = cudaFuncSetAttribute(k_rows<NW, NT, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem<NW, NT>);
+    if (e != cudaSuccess) return e;
+    const uint32_t row_tiles = (a.rows + 8 * NT - 1) / (8 * NT);
+    const uint64_t segments = static_cast<uint64_t>(a.c.kv_heads) * (LIST ? a.d.queries : 1);
+    const uint64_t width = LIST ? a.count : static_cast<uint64_t>(a.d.table_width) + a.d.shared_width;
+    const uint32_t parts = parts_of(segments * row_tiles * a.d.num_seqs, width * a.c.block, static_cast<uint64_t>(dev.num_sms) * blocks_per_sm(NT));
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(segments * parts), row_tiles, a.d.num_seqs);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = kRowsSmem<NW, NT>;
+    config.stream = stream;
+    config.attrs = attr;
+    config.numAttrs = 2;
+    return cudaLaunchKernelEx(&config, k_rows<NW, NT, LIST>, a);
+}
+
+template <int NT, bool LIST>
+cudaError_t launch_rows(const RowsArgs& a, const MemoryDevice& dev, cudaStream_t stream) {
+    switch (a.c.dim / 16) {
+        case 1: return launch_rows<1, NT, LIST>(a, dev, stream);
+        case 2: return launch_rows<2, NT, LIST>(a, dev, stream);
+        case 3: return launch_rows<3, NT, LIST>(a, dev, stream);
+        case 4: return launch_rows<4, NT, LIST>(a, dev, stream);
+        case 5: return launch_rows<5, NT, LIST>(a, dev, stream);
+        case 6: return launch_rows<6, NT, LIST>(a, dev, stream);
+        case 7: return launch_rows<7, NT, LIST>(a, dev, stream);
+        default: return launch_rows<8, NT, LIST>(a, dev, stream);
+    }
+}
+
+uint32_t log2_of(int32_t block) { return block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7; }
+
+}  // namespace
+
+cudaError_t launch_block_attention(const bs_token_cache& c, const bs_block_attention_desc& d, const MemoryDevice& dev, cudaStream_t stream) {
+    RowsArgs a{c, {}, d.blocks, dev.errors};
+    a.d.q = d.q;
+    for (int i = 0; i < 3; ++i) a.d.q_stride[i] = d.q_stride[i];
+    a.d.table = d.table;
+    a.d.lens = d.lens;
+    a.d.out = d.out;
+    a.d.lse = d.lse;
+    a.d.num_seqs = d.num_seqs;
+    a.d.table_width = d.table_width;
+    a.d.queries = d.queries;
+    a.d.q_heads = d.q_heads;
+    a.d.dtype = d.dtype;
+    a.d.scale = d.scale;
+    a.count = d.count;
+    a.group = a.rows = d.q_heads / c.kv_heads;
+    a.block_log2 = log2_of(c.block);
+    return a.rows <= 8 ? launch_rows<1, true>(a, dev, stream) : launch_rows<2, true>(a, dev, stream);
+}
+
+size_t shared_attention_scratch(const bs_token_cache&, const bs_shared_attention_desc&, const MemoryDevice&) { return 0; }
+
+cudaError_t launch_shared_attention(const bs_token_cache& c, const bs_shared_attention_desc& d, const MemoryDevice& dev, cudaStream_t stream) {
+    RowsArgs a{c, d, nullptr, dev.errors};
+    a.group = d.q_heads / c.kv_heads;
+    a.rows = a.group * d.queries;
+    a.block_log2 = log2_of(c.block);
+    return a.rows <= 8 ? launch_rows<1, false>(a, dev, stream) : launch_rows<2, false>(a, dev, stream);
+}
+
+}  // namespace bsb

@@ -1,0 +1,296 @@
+// bs_block_choice.cu -- bounds of the token cache's key blocks, and which
+// blocks a query attends to by them (include/bsearch.h, bs_block_bounds,
+// bs_block_choice).
+//
+// For any key k of a block, of codes between `lower` and `upper` in every
+// dimension, <q, k> <= k_scale * sum over d of max(q_d * upper_d, q_d * lower_d),
+// which splits q into its positive and negative part: the sum is the product
+// of (q+, q-) with (upper, lower).  So the query heads of a key head choose
+// together at the cost of one: their parts add up before the product.  q counts
+// in 127ths of its largest element, which makes every score an exact integer
+// times the block's scale, the same in any order of summation.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "bs_device.cuh"
+#include "bs_memory.h"
+#include "bs_select.cuh"
+
+namespace bsb {
+
+using namespace dev;
+using namespace select;
+
+namespace {
+
+// ------------------------------------------------------------------ bounds
+
+struct BoundsArgs {
+    bs_token_cache c;
+    bs_block_bounds_desc d;
+    unsigned int* errors;
+    uint32_t cols;        // blocks of a sequence that may have changed, at most
+};
+
+constexpr int kBoundsWarps = 4;
+
+// Larger and smaller of signed 16-bit halves whose upper bytes count; the
+// lower bytes only decide between equal ones.
+__device__ __forceinline__ void widen(uint32_t (&hi)[8], uint32_t (&lo)[8], uint4 x) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t even = w[i] << 8;             // bytes 0 and 2 into the upper places
+        hi[2 * i] = __vmaxs2(hi[2 * i], even);
+        lo[2 * i] = __vmins2(lo[2 * i], even);
+        hi[2 * i + 1] = __vmaxs2(hi[2 * i + 1], w[i]);
+        lo[2 * i + 1] = __vmins2(lo[2 * i + 1], w[i]);
+    }
+}
+
+// A warp: one block's keys of one head.  A lane has 16 dimensions of every
+// (32 / per_row)-th token.
+__global__ void __launch_bounds__(32 * kBoundsWarps) k_block_bounds(const __grid_constant__ BoundsArgs a) {
+    const bs_block_bounds_desc& d = a.d;
+    const uint32_t hkv = a.c.kv_heads, block = a.c.block, per_row = a.c.dim / 16, lane = threadIdx.x & 31, b = blockIdx.y;
+    const uint32_t unit = blockIdx.x * kBoundsWarps + (threadIdx.x >> 5), h = unit % hkv;
+    cudaGridDependencySynchronize();       // in every block, before anything of the caller's
+    int64_t len = d.lens[b];
+    const int64_t most = static_cast<int64_t>(d.table_width) * block;
+    if (len < 0 || len > most) {
+        if (unit == 0 && lane == 0) atomicOr(a.errors, kMemErrLength);
+        len = len < 0 ? 0 : most;
+    }
+    const int64_t from = d.last < 0 || d.last >= len ? 0 : (len - d.last) / block;
+    const int64_t col = from + unit / hkv, left = len - col * block;      // tokens from the block's first on
+    if (unit / hkv >= a.cols || left <= 0) return;
+    const uint32_t id = d.table[static_cast<uint64_t>(b) * d.table_width + col];
+    if (id >= a.c.num_blocks) {
+        if (lane == 0) atomicOr(a.errors, kMemErrBlock);
+        return;
+    }
+    const uint64_t slab = static_cast<uint64_t>(id) * hkv + h;
+    const uint32_t rows = 32 / per_row, row = lane / per_row, tokens = left < block ? static_cast<uint32_t>(left) : block;
+    uint32_t hi[8], lo[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        hi[i] = 0x80008000u;
+        lo[i] = 0x7fff7fffu;
+    }
+    if (row < rows) {
+        const uint4* codes = reinterpret_cast<const uint4*>(a.c.k + slab * block * a.c.dim) + lane;
+        constexpr uint32_t kBatch = 8;                 // loads on their way together
+        for (uint32_t r0 = row; r0 < tokens; r0 += kBatch * rows) {
+            uint4 x[kBatch];
+#pragma unroll
+            for (uint32_t u = 0; u < kBatch; ++u)      // (past the last token: this batch's first again)
+                x[u] = __ldcs(codes + (r0 - row + (r0 + u * rows < tokens ? u * rows : 0)) * per_row);
+#pragma unroll
+            for (uint32_t u = 0; u < kBatch; ++u) widen(hi, lo, x[u]);
+        }
+    }
+    for (uint32_t s = 16; s > 0; s >>= 1) {            // over the lanes of a chunk; rows of a lane past the others have none
+        if (s >= rows) continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t x = __shfl_down_sync(kFull, hi[i], s * per_row), y = __shfl_down_sync(kFull, lo[i], s * per_row);
+            if (row + s < rows) {
+                hi[i] = __vmaxs2(hi[i], x);
+                lo[i] = __vmins2(lo[i], y);
+            }
+        }
+    }
+    if (row != 0) return;
+    uint4 out[2];
+    uint32_t* const w = reinterpret_cast<uint32_t*>(out);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {                      // the upper bytes, in order
+        w[i] = __byte_perm(hi[2 * i], hi[2 * i + 1], 0x7351);
+        w[4 + i] = __byte_perm(lo[2 * i], lo[2 * i + 1], 0x7351);
+    }
+    uint4* const to = reinterpret_cast<uint4*>(d.bounds + slab * 2 * a.c.dim) + lane;
+    to[0] = out[0];
+    to[per_row] = out[1];
+}
+
+// ------------------------------------------------------------------ choice
+
+struct ChoiceArgs {
+    bs_token_cache c;
+    bs_block_choice_desc d;
+    unsigned int* errors;
+};
+
+constexpr int kChoiceThreads = 256;
+
+template <typename T>
+__device__ __forceinline__ float element(const void* p, int64_t i) {
+    return static_cast<float>(static_cast<const T*>(p)[i]);
+}
+
+// A cluster of blocks has one row: a query and a key head.  Each block scores
+// its slice of the table's columns, then the rows' largest are found among the
+// scores in shared memory (bs_select.cuh).
+template <typename T>
+__global__ void __launch_bounds__(kChoiceThreads) k_block_choice(const __grid_constant__ ChoiceArgs a, uint32_t cached) {
+    extern __shared__ uint32_t keys[];                     // [cached]
+    __shared__ __align__(16) SelectShared shared;
+    __shared__ __align__(16) int16_t parts[2][128];        // positive and negative part of the heads' codes
+    __shared__ float warp_max[kChoiceThreads / 32];
+    constexpr uint32_t kWarps = kChoiceThreads / 32;
+    cudaGridDependencySynchronize();       // in every block, before anything of the caller's
+    const cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t rank = cluster.block_rank(), blocks = cluster.num_blocks();
+    const bs_block_choice_desc& d = a.d;
+    const uint32_t hkv = a.c.kv_heads, group = d.q_heads / hkv, dim = a.c.dim, block = a.c.block;
+    const uint32_t h = blockIdx.x / blocks, i = blockIdx.y, b = blockIdx.z, t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    int64_t len = d.lens[b];
+    const int64_t most = static_cast<int64_t>(d.table_width) * block;
+    if (len < 0 || len > most) {
+        if (t == 0) atomicOr(a.errors, kMemErrLength);
+        len = len < 0 ? 0 : most;
+    }
+    const int64_t seen = len - d.queries + 1 + i;
+    const uint32_t n = seen > 0 ? static_cast<uint32_t>((seen + block - 1) / block) : 0, count = d.count;
+    int32_t* const out = d.blocks + ((static_cast<uint64_t>(b) * d.queries + i) * hkv + h) * count;
+    if (n <= count) {                                      // (the whole cluster)
+        for (uint32_t x = rank * kChoiceThreads + t; x < count; x += blocks * kChoiceThreads) out[x] = x < n ? static_cast<int32_t>(x) : -1;
+        return;
+    }
+    // the heads' elements as codes, added up by sign
+    const T* const q = static_cast<const T*>(d.q) + b * d.q_stride[0] + i * d.q_stride[1] + static_cast<int64_t>(h) * group * d.q_stride[2];
+    clear_counts<kChoiceThreads>(shared);
+    float top = 0.f;
+    if (t < dim)
+        for (uint32_t x = 0; x < group; ++x) top = fmaxf(top, fabsf(static_cast<float>(q[x * d.q_stride[2] + t])));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+    if (lane == 0) warp_max[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t x = 0; x < kWarps; ++x) top = fmaxf(top, warp_max[x]);
+    const float by = top < 1e-30f ? 0.f : __fdiv_rn(127.f, top);
+    if (t < dim) {
+        int32_t positive = 0, negative = 0;
+        for (uint32_t x = 0; x < group; ++x) {
+            const int32_t c = __float2int_rn(__fmul_rn(static_cast<float>(q[x * d.q_stride[2] + t]), by));
+            positive += max(c, 0);
+            negative += min(c, 0);
+        }
+        parts[0][t] = static_cast<int16_t>(positive);      // (at most 128 heads of 127)
+        parts[1][t] = static_cast<int16_t>(negative);
+    }
+    __syncthreads();
+
+    uint32_t first, size;
+    select_slice(n, blocks, rank, first, size);
+    const int32_t* const table = d.table + static_cast<uint64_t>(b) * d.table_width + first;
+    // a column's 2 * dim bounds lie side by side: 16 to a lane
+    const uint32_t per_col = dim / 8, cols = 32 / per_col, sub = lane / per_col, chunk = lane % per_col;
+    int32_t weights[8] = {};
+    if (sub < cols) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) weights[x] = reinterpret_cast<const int32_t*>(&parts[0][0] + (chunk * 16 < dim ? 0 : 128 - dim) + chunk * 16)[x];
+    }
+    auto product = [&](const uint4& x) {
+        const int32_t w[4] = {static_cast<int32_t>(x.x), static_cast<int32_t>(x.y), static_cast<int32_t>(x.z), static_cast<int32_t>(x.w)};
+        int32_t sum = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sum = __dp2a_hi(weights[2 * u + 1], w[u], __dp2a_lo(weights[2 * u], w[u], sum));
+        return sum;
+    };
+    auto key = [&](int32_t sum, float scale) { return select_key(__fmul_rn(__int2float_rn(sum), scale)); };
+    constexpr uint32_t kBatch = 4;
+    const uint32_t held = min(size, cached);
+    for (uint32_t x0 = warp * cols * kBatch; x0 < held; x0 += kWarps * cols * kBatch) {
+        uint4 x[kBatch];
+        uint64_t slab[kBatch];
+        float scale[kBatch];
+#pragma unroll
+        for (uint32_t u = 0; u < kBatch; ++u) {
+            const uint32_t col = x0 + u * cols + sub;
+            const uint32_t id = sub < cols && col < held ? static_cast<uint32_t>(table[col]) : 0u;
+            slab[u] = static_cast<uint64_t>(id) * hkv + h;
+            if (id >= a.c.num_blocks) slab[u] = ~0ull;
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kBatch; ++u) {
+            const bool ok = slab[u] != ~0ull && sub < cols && x0 + u * cols + sub < held;
+            x[u] = ok ? __ldg(reinterpret_cast<const uint4*>(d.bounds + slab[u] * 2 * dim) + chunk) : make_uint4(0, 0, 0, 0);
+            scale[u] = ok ? a.c.k_scale[slab[u]] : 0.f;
+            if (slab[u] == ~0ull && chunk == 0 && sub < cols) atomicOr(a.errors, kMemErrBlock);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kBatch; ++u) {
+            int32_t sum = product(x[u]);
+#pragma unroll
+            for (uint32_t s = 8; s > 0; s >>= 1) {
+                const int32_t y = __shfl_down_sync(kFull, sum, s);
+                if (chunk + s < per_col) sum += y;
+            }
+            const uint32_t col = x0 + u * cols + sub;
+            if (chunk == 0 && sub < cols && col < held) keys[col] = key(sum, scale[u]);
+        }
+    }
+    __syncthreads();
+    select_row<kChoiceThreads>(
+        cluster, shared, n, first, size, d.sinks, d.recent, count,
+        [&](uint32_t col) -> uint32_t {
+            if (col < cached) return keys[col];
+            // a row too long for shared memory: scored again, by one thread
+            const uint32_t id = table[col];
+            if (id >= a.c.num_blocks) return key(0, 0.f);
+            const uint64_t slab = static_cast<uint64_t>(id) * hkv + h;
+            int32_t sum = 0;
+            for (uint32_t x = 0; x < 2 * dim; ++x) sum += parts[x >= dim][x < dim ? x : x - dim] * d.bounds[slab * 2 * dim + x];
+            return key(sum, a.c.k_scale[slab]);
+        },
+        [&](uint32_t slot, uint32_t col) { out[slot] = col; });
+}
+
+template <typename T>
+cudaError_t launch_choice(const bs_token_cache& c, const bs_block_choice_desc& d, const MemoryDevice& dev, cudaStream_t stream) {
+    const ChoiceArgs a{c, d, dev.errors};
+    // a row goes to more blocks while they would have over 256 columns each and
+    // the rows alone do not fill the GPU
+    const uint64_t rows = static_cast<uint64_t>(c.kv_heads) * d.queries * d.num_seqs;
+    uint32_t cluster = 1;
+    while (cluster < kMostCluster && d.table_width / cluster > 256 && rows * cluster * 2 <= 2u * dev.num_sms) cluster *= 2;
+    const uint32_t slice = ((d.table_width + cluster - 1) / cluster + 3) & ~3u, cached = slice < kMostCached ? slice : kMostCached;
+    cudaError_t e = cudaFuncSetAttribute(k_block_choice<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostCached * 4);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(c.kv_heads * cluster, d.queries, d.num_seqs);
+    config.blockDim = dim3(kChoiceThreads);
+    config.dynamicSmemBytes = cached * 4;
+    config.stream = stream;
+    config.attrs = attr;
+    config.numAttrs = 2;
+    return cudaLaunchKernelEx(&config, k_block_choice<T>, a, cached);
+}
+
+}  // namespace
+
+cudaError_t launch_block_bounds(const bs_token_cache& c, const bs_block_bounds_desc& d, const MemoryDevice& dev, cudaStream_t stream) {
+    BoundsArgs a{c, d, dev.errors};
+    a.cols = d.table_width;
+    if (d.last >= 0) {          // the last tokens may begin and end inside a block
+        const uint64_t touched = (static_cast<uint64_t>(d.last) + c.block - 2) / c.block + 1;
+        if (touched < a.cols) a.cols = static_cast<uint32_t>(touched);
+    }
+    const uint64_t blocks = (static_cast<uint64_t>(a.cols) * c.kv_heads + kBoundsWarps - 1) / kBoundsWarps;
+    if (blocks > 0xffffffffu / kBoundsWarps / 2) return cudaErrorInvalidConfiguration;      // (units count in 32 bits)
+    return launch_after(k_block_bounds, dim3(static_cast<unsigned>(blocks), d.num_seqs), 32 * kBoundsWarps, 0, stream, a);
+}
+
+cudaError_t launch_block_choice(const bs_token_cache& c, const bs_block_choice_desc& d, const MemoryDevice& dev, cudaStream_t stream) {
+    return d.dtype == BS_F16 ? launch_choice<__half>(c, d, dev, stream) : launch_choice<__nv_bfloat16>(c, d, dev, stream);
+}
+
+}  // namespace bsb

@@ -43,6 +43,15 @@ size_t cache_evict_scratch(const bs_token_cache& c, const bs_cache_evict_desc& d
 cudaError_t launch_cache_evict(const bs_token_cache& c, const bs_cache_evict_desc& d, const MemoryDevice& dev,
                                cudaStream_t stream);
 
+cudaError_t launch_norm_rotate(const bs_norm_rotate_desc& d, const MemoryDevice& dev, cudaStream_t stream);
+cudaError_t launch_block_bounds(const bs_token_cache& c, const bs_block_bounds_desc& d, const MemoryDevice& dev, cudaStream_t stream);
+cudaError_t launch_block_choice(const bs_token_cache& c, const bs_block_choice_desc& d, const MemoryDevice& dev, cudaStream_t stream);
+cudaError_t launch_block_attention(const bs_token_cache& c, const bs_block_attention_desc& d, const MemoryDevice& dev,
+                                   cudaStream_t stream);
+size_t shared_attention_scratch(const bs_token_cache& c, const bs_shared_attention_desc& d, const MemoryDevice& dev);
+cudaError_t launch_shared_attention(const bs_token_cache& c, const bs_shared_attention_desc& d, const MemoryDevice& dev,
+                                    cudaStream_t stream);
+
 #ifdef __CUDACC__
 // A kernel that may start while the one before it on the stream still runs,
 // whosever that is, and waits for it by itself, in every block, before it reads

@@ -86,6 +86,7 @@ bool strides_ok(const int64_t* s, std::initializer_list<uint32_t> extents) {
 const char* const kWhere = "pointers must be memory of the current device";
 const char* const kAlign4 = "32-bit buffers must be 4-byte aligned";
 const char* const kAlign = "q, k, v and outputs must be 16-byte aligned, their strides non-negative multiples of 8 elements within a buffer's reach";
+const char* const kAlignBounds = "bounds must be 16-byte aligned";
 
 bs_status check_dim(int32_t dim) {
     if (dim <= 0) return report_error(BS_ERR_INVALID_ARGUMENT, "dim must be positive");
@@ -341,6 +342,153 @@ BS_API bs_status bs_cache_evict(const bs_token_cache* c, const bs_cache_evict_de
                             need);
     const cudaError_t e = launch_cache_evict(*c, *d, dev, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? BS_OK : cuda_error(e, "cache eviction launch");
+}
+
+BS_API bs_status bs_norm_rotate(const bs_norm_rotate_desc* d, void* stream) {
+    if (!d) return report_error(BS_ERR_INVALID_ARGUMENT, "desc is NULL");
+    if (bs_status s = check_dtype16(d->dtype)) return s;
+    if (bs_status s = check_dim(d->dim)) return s;
+    if (d->q_heads < 0 || d->kv_heads < 0 || d->q_heads + static_cast<int64_t>(d->kv_heads) <= 0)
+        return report_error(BS_ERR_INVALID_ARGUMENT, "q_heads and kv_heads must not be negative, nor both 0");
+    if (d->q_heads > 65535 || d->kv_heads > 65535 || d->total >= (1u << 30))
+        return report_error(BS_ERR_UNSUPPORTED, "at most 65535 heads and fewer than 2^30 tokens are supported");
+    if (d->rotary < 0 || d->rotary % 2 || d->rotary > d->dim)
+        return report_error(BS_ERR_INVALID_ARGUMENT, "rotary (%d) must be even and in 0 .. dim", d->rotary);
+    if ((d->q_weight || d->k_weight) && d->weight_dtype != BS_F32 && d->weight_dtype != BS_F16 && d->weight_dtype != BS_BF16)
+        return report_error(BS_ERR_INVALID_ARGUMENT, "weight_dtype must be BS_F32, BS_F16 or BS_BF16");
+    if (!(d->eps >= 0.f) || std::isinf(d->eps) || !std::isfinite(d->amplitude))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "eps must be finite and not negative, amplitude finite");
+    if (d->total == 0) return BS_OK;
+    if ((d->q_heads && any_null({d->q, d->out_q})) || (d->kv_heads && any_null({d->k, d->out_k})) ||
+        (d->rotary && any_null({d->positions, d->freqs})))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "a buffer is NULL");
+    const uint32_t q_heads = d->q_heads, kv_heads = d->kv_heads;
+    if (!aligned16({d->q, d->k, d->out_q, d->out_k}) || !strides_ok(d->q_stride, {d->total, q_heads}) ||
+        !strides_ok(d->k_stride, {d->total, kv_heads}))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign);
+    if (!aligned4({d->positions}) || (reinterpret_cast<uintptr_t>(d->freqs) & 7))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "positions must be 4-byte and freqs 8-byte aligned");
+    const uintptr_t size = d->weight_dtype == BS_F32 ? 4 : 2;
+    if (((reinterpret_cast<uintptr_t>(d->q_weight) | reinterpret_cast<uintptr_t>(d->k_weight)) & (size - 1)) != 0)
+        return report_error(BS_ERR_INVALID_ARGUMENT, "weights must be aligned to their type");
+    MemoryDevice dev;
+    if (bs_status s = memory_device(dev)) return s;
+    if (!on_device(dev.device, {d->q, d->k, d->out_q, d->out_k, d->q_weight, d->k_weight, d->positions, d->freqs}))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kWhere);
+    const cudaError_t e = launch_norm_rotate(*d, dev, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? BS_OK : cuda_error(e, "norm and rotary launch");
+}
+
+BS_API bs_status bs_block_bounds(const bs_token_cache* c, const bs_block_bounds_desc* d, void* stream) {
+    if (!d) return report_error(BS_ERR_INVALID_ARGUMENT, "desc is NULL");
+    if (bs_status s = check_cache(c, 0, false)) return s;
+    if (bs_status s = check_table(c, d->num_seqs, d->table_width)) return s;
+    if (d->num_seqs == 0 || d->table_width == 0 || d->last == 0) return BS_OK;
+    if (any_null({d->bounds, d->table, d->lens})) return report_error(BS_ERR_INVALID_ARGUMENT, "a buffer is NULL");
+    if (!aligned16({d->bounds})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlignBounds);
+    if (!aligned4({d->table, d->lens})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign4);
+    MemoryDevice dev;
+    if (bs_status s = memory_device(dev)) return s;
+    if (bs_status s = check_cache(c, dev.device, true)) return s;
+    if (!on_device(dev.device, {d->bounds, d->table, d->lens})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kWhere);
+    const cudaError_t e = launch_block_bounds(*c, *d, dev, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? BS_OK : cuda_error(e, "block bounds launch");
+}
+
+// What calls with a few query tokens of each sequence have in common.
+static bs_status check_queries(const bs_token_cache* c, int32_t dtype, int32_t q_heads, uint32_t num_seqs, uint32_t table_width, int32_t queries) {
+    if (bs_status s = check_cache(c, 0, false)) return s;
+    if (bs_status s = check_dtype16(dtype)) return s;
+    if (bs_status s = check_heads(q_heads, c->kv_heads)) return s;
+    if (bs_status s = check_table(c, num_seqs, table_width)) return s;
+    if (queries <= 0 || queries > 1024) return report_error(BS_ERR_INVALID_ARGUMENT, "queries must be in 1..1024");
+    return BS_OK;
+}
+
+static bs_status check_scale(float scale) {
+    if (!(scale > 0.f) || std::isinf(scale))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "scale must be positive and finite (not 0, negative, infinite or NaN)");
+    return BS_OK;
+}
+
+BS_API bs_status bs_block_choice(const bs_token_cache* c, const bs_block_choice_desc* d, void* stream) {
+    if (!d) return report_error(BS_ERR_INVALID_ARGUMENT, "desc is NULL");
+    if (bs_status s = check_queries(c, d->dtype, d->q_heads, d->num_seqs, d->table_width, d->queries)) return s;
+    if (d->count <= 0 || d->count >= (1 << 26) || d->sinks < 0 || d->recent < 0 ||
+        static_cast<int64_t>(d->sinks) + d->recent > d->count)
+        return report_error(BS_ERR_INVALID_ARGUMENT, "need 0 < count < 2^26 and sinks + recent <= count, none negative");
+    if (d->num_seqs == 0) return BS_OK;
+    if (any_null({d->q, d->bounds, d->lens, d->blocks}) || (d->table_width && !d->table))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "a buffer is NULL");
+    if (!aligned16({d->q}) || !strides_ok(d->q_stride, {d->num_seqs, static_cast<uint32_t>(d->queries), static_cast<uint32_t>(d->q_heads)}))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign);
+    if (!aligned16({d->bounds})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlignBounds);
+    if (!aligned4({d->table, d->lens, d->blocks})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign4);
+    MemoryDevice dev;
+    if (bs_status s = memory_device(dev)) return s;
+    if (bs_status s = check_cache(c, dev.device, true)) return s;
+    if (!on_device(dev.device, {d->q, d->bounds, d->table, d->lens, d->blocks})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kWhere);
+    const cudaError_t e = launch_block_choice(*c, *d, dev, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? BS_OK : cuda_error(e, "block choice launch");
+}
+
+BS_API bs_status bs_block_attention(const bs_token_cache* c, const bs_block_attention_desc* d, void* stream) {
+    if (!d) return report_error(BS_ERR_INVALID_ARGUMENT, "desc is NULL");
+    if (bs_status s = check_queries(c, d->dtype, d->q_heads, d->num_seqs, d->table_width, d->queries)) return s;
+    if (bs_status s = check_scale(d->scale)) return s;
+    if (d->count < 0 || static_cast<int64_t>(d->count) * c->block >= (1 << 30))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "count must not be negative, nor count * block reach 2^30");
+    if (d->num_seqs == 0) return BS_OK;
+    if (any_null({d->q, d->lens, d->out}) || (d->table_width && !d->table) || (d->count && !d->blocks))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "a buffer is NULL");
+    if (!aligned16({d->q, d->out}) || !strides_ok(d->q_stride, {d->num_seqs, static_cast<uint32_t>(d->queries), static_cast<uint32_t>(d->q_heads)}))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign);
+    if (!aligned4({d->table, d->lens, d->blocks, d->lse})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign4);
+    MemoryDevice dev;
+    if (bs_status s = memory_device(dev)) return s;
+    if (bs_status s = check_cache(c, dev.device, true)) return s;
+    if (!on_device(dev.device, {d->q, d->table, d->lens, d->blocks, d->out, d->lse})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kWhere);
+    const cudaError_t e = launch_block_attention(*c, *d, dev, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? BS_OK : cuda_error(e, "block attention launch");
+}
+
+static bs_status check_shared(const bs_token_cache* c, const bs_shared_attention_desc* d) {
+    if (!d) return report_error(BS_ERR_INVALID_ARGUMENT, "desc is NULL");
+    if (bs_status s = check_queries(c, d->dtype, d->q_heads, d->num_seqs, d->table_width, d->queries)) return s;
+    if (bs_status s = check_table(c, d->num_groups, d->shared_width)) return s;
+    return check_scale(d->scale);
+}
+
+BS_API bs_status bs_shared_attention_workspace(const bs_token_cache* c, const bs_shared_attention_desc* d, size_t* bytes) {
+    if (!bytes) return report_error(BS_ERR_INVALID_ARGUMENT, "bytes is NULL");
+    if (bs_status s = check_shared(c, d)) return s;
+    MemoryDevice dev;
+    if (bs_status s = memory_device(dev)) return s;
+    *bytes = shared_attention_scratch(*c, *d, dev);
+    return BS_OK;
+}
+
+BS_API bs_status bs_shared_attention(const bs_token_cache* c, const bs_shared_attention_desc* d, void* stream) {
+    if (bs_status s = check_shared(c, d)) return s;
+    if (d->num_seqs == 0) return BS_OK;
+    if (d->num_groups == 0)
+        return report_error(BS_ERR_INVALID_ARGUMENT, "num_groups is 0, but there are %u sequences", static_cast<unsigned>(d->num_seqs));
+    if (any_null({d->q, d->shared_lens, d->cu, d->lens, d->out}) || (d->table_width && !d->table) || (d->shared_width && !d->shared_table))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "a buffer is NULL");
+    if (!aligned16({d->q, d->out, d->workspace}) || !strides_ok(d->q_stride, {d->num_seqs, static_cast<uint32_t>(d->queries), static_cast<uint32_t>(d->q_heads)}))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign);
+    if (!aligned4({d->shared_table, d->shared_lens, d->cu, d->table, d->lens, d->lse})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlign4);
+    MemoryDevice dev;
+    if (bs_status s = memory_device(dev)) return s;
+    if (bs_status s = check_cache(c, dev.device, true)) return s;
+    if (!on_device(dev.device, {d->q, d->shared_table, d->shared_lens, d->cu, d->table, d->lens, d->out, d->lse, d->workspace}))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kWhere);
+    const size_t need = shared_attention_scratch(*c, *d, dev);
+    if (need > (d->workspace ? d->workspace_bytes : 0))
+        return report_error(BS_ERR_INVALID_ARGUMENT, "workspace of %zu bytes, %zu are needed", d->workspace ? d->workspace_bytes : 0,
+                            need);
+    const cudaError_t e = launch_shared_attention(*c, *d, dev, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? BS_OK : cuda_error(e, "shared attention launch");
 }
 
 BS_API bs_status bs_memory_take_errors(void* stream_, uint32_t* flags) {

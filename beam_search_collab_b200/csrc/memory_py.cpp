@@ -118,8 +118,12 @@ struct NoGradient : torch::autograd::Function<NoGradient> {
 Tensor from(const Tensor& made, std::initializer_list<const Tensor*> inputs) {
     if (made.defined() && at::GradMode::is_enabled())
         for (const Tensor* t : inputs)
-            if (t->requires_grad()) return NoGradient::apply(made, *t);
+            if (t->defined() && t->requires_grad()) return NoGradient::apply(made, *t);
     return made;
+}
+
+float scale_of(std::optional<double> scale, const Tensor& q) {
+    return static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(q.size(-1), 1))));
 }
 
 py::object maybe(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
@@ -165,6 +169,62 @@ py::tuple prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, co
     to.uses({&q, &k, &v, &cu_q, &cu_k});
     to.gives({&out, &lse});
     return py::make_tuple(from(out, {&q, &k, &v}), maybe(from(lse, {&q, &k})));
+}
+
+// [tokens, heads, dim] each; k may be None.
+py::tuple norm_rotate(const Tensor& q, const MaybeTensor& k, const Tensor& positions, const MaybeTensor& freqs, const MaybeTensor& q_weight,
+                      const MaybeTensor& k_weight, double eps, bool interleaved, double amplitude, std::optional<uint64_t> stream) {
+    check_rows(q, "q", nullptr);
+    if (k) {
+        check_rows(*k, "k", &q);
+        need(k->size(0) == q.size(0), "q and k must have as many rows");
+    }
+    need(k || !k_weight, "k_weight without k");
+    bs_norm_rotate_desc d{};
+    d.positions = indexes(positions, {q.size(0)}, "positions", q.device());
+    if (freqs) {
+        need(freqs->scalar_type() == at::kDouble && freqs->dim() == 1 && freqs->is_contiguous() && freqs->device() == q.device(),
+             "freqs must be a contiguous float64 tensor [rotary / 2] on q's device");
+        d.freqs = freqs->const_data_ptr<double>();
+        d.rotary = count(2 * freqs->size(0));
+    }
+    const Tensor* weight = nullptr;
+    for (const MaybeTensor* w : {&q_weight, &k_weight}) {
+        if (!*w) continue;
+        need((*w)->dim() == 1 && (*w)->size(0) == q.size(2) && (*w)->is_contiguous() && (*w)->device() == q.device() && type_of(**w) >= 0,
+             "weights must be contiguous float32, float16 or bfloat16 tensors [dim] on q's device");
+        need(!weight || weight->scalar_type() == (*w)->scalar_type(), "q_weight and k_weight must have the same type");
+        weight = &**w;
+    }
+    Target to(q.device(), stream);
+    const Tensor out_q = at::empty(q.sizes(), q.options()), out_k = k ? at::empty(k->sizes(), k->options()) : Tensor();
+    d.q = q.const_data_ptr();
+    d.out_q = out_q.data_ptr();
+    strides(q, d.q_stride);
+    d.q_heads = count(q.size(1));
+    if (k) {
+        d.k = k->const_data_ptr();
+        d.out_k = out_k.data_ptr();
+        strides(*k, d.k_stride);
+        d.kv_heads = count(k->size(1));
+    }
+    d.q_weight = q_weight ? q_weight->const_data_ptr() : nullptr;
+    d.k_weight = k_weight ? k_weight->const_data_ptr() : nullptr;
+    d.total = count(q.size(0));
+    d.dim = count(q.size(2));
+    d.interleaved = interleaved;
+    d.dtype = type_of(q);
+    d.weight_dtype = weight ? type_of(*weight) : BS_F32;
+    d.eps = static_cast<float>(eps);
+    d.amplitude = static_cast<float>(amplitude);
+    check(bs_norm_rotate(&d, to.stream));
+    to.uses({&q, &positions});
+    for (const MaybeTensor* t : {&k, &freqs, &q_weight, &k_weight})
+        if (*t) to.uses({&**t});
+    to.gives({&out_q, &out_k});
+    const Tensor none;
+    const Tensor &qw = q_weight ? *q_weight : none, &kw = k_weight ? *k_weight : none, &f = freqs ? *freqs : none;
+    return py::make_tuple(from(out_q, {&q, &qw, &f}), k ? py::cast(from(out_k, {&*k, &kw, &f})) : py::none());
 }
 
 struct Cache {
@@ -295,6 +355,129 @@ struct Cache {
         return py::make_tuple(from(out, {&q}), maybe(from(lse, {&q})), maybe(sum));
     }
 
+    // bounds int8 [blocks, kv_heads, 2, dim] of this cache
+    int8_t* check_bounds(const Tensor& t) const {
+        need(t.scalar_type() == at::kChar && t.device() == k.device() && t.is_contiguous() && t.dim() == 4 && t.size(0) == k.size(0) &&
+                 t.size(1) == k.size(1) && t.size(2) == 2 && t.size(3) == k.size(3),
+             "bounds must be a contiguous int8 tensor [blocks, kv_heads, 2, dim] on the cache's device");
+        return static_cast<int8_t*>(t.data_ptr());
+    }
+
+    void check_queries(const Tensor& q, const Tensor& table) const {
+        need(q.dim() == 4 && q.device() == k.device() && is_type16(q) && q.size(3) == k.size(3) && (q.size(3) <= 1 || q.stride(3) == 1),
+             "q must be float16 or bfloat16 [sequences, queries, q_heads, dim] on the cache's device, last dimension contiguous");
+        need(table.dim() == 2 && table.size(0) == q.size(0), "table must be [sequences, width], q have as many sequences");
+    }
+
+    void update_bounds(const Tensor& bounds, const Tensor& table, const Tensor& lens, std::optional<int64_t> last,
+                       std::optional<uint64_t> stream) const {
+        need(table.dim() == 2, "table must be [sequences, width]");
+        need(!last || *last >= 0, "last must not be negative");
+        bs_block_bounds_desc d{};
+        d.bounds = check_bounds(bounds);
+        d.table = indexes(table, table.sizes(), "table", k.device());
+        d.lens = indexes(lens, {table.size(0)}, "lens", k.device());
+        Target to(k.device(), stream);
+        d.num_seqs = count(table.size(0));
+        d.table_width = count(table.size(1));
+        d.last = last ? count(*last) : -1;
+        check(bs_block_bounds(&c, &d, to.stream));
+        to.uses({&k, &v, &k_scale, &v_scale, &bounds, &table, &lens});
+    }
+
+    Tensor choose_blocks(const Tensor& q, const Tensor& bounds, const Tensor& table, const Tensor& lens, int64_t most, int64_t sinks,
+                         int64_t recent, std::optional<uint64_t> stream) const {
+        check_queries(q, table);
+        need(most > 0 && most < (1 << 26), "count must be positive and below 2^26");
+        need(sinks >= 0 && recent >= 0 && sinks <= most && recent <= most, "sinks and recent must be in 0 .. count");
+        bs_block_choice_desc d{};
+        d.bounds = check_bounds(bounds);
+        d.table = indexes(table, table.sizes(), "table", k.device());
+        d.lens = indexes(lens, {table.size(0)}, "lens", k.device());
+        Target to(k.device(), stream);
+        const Tensor blocks = at::empty({q.size(0), q.size(1), k.size(1), most}, lens.options());
+        d.q = q.const_data_ptr();
+        strides(q, d.q_stride);
+        d.blocks = blocks.data_ptr<int32_t>();
+        d.num_seqs = count(q.size(0));
+        d.table_width = count(table.size(1));
+        d.queries = count(q.size(1));
+        d.q_heads = count(q.size(2));
+        d.count = most;
+        d.sinks = sinks;
+        d.recent = recent;
+        d.dtype = type_of(q);
+        check(bs_block_choice(&c, &d, to.stream));
+        to.uses({&k, &v, &k_scale, &v_scale, &q, &bounds, &table, &lens});
+        to.gives({&blocks});
+        return blocks;
+    }
+
+    py::tuple block_attention(const Tensor& q, const Tensor& table, const Tensor& lens, const Tensor& blocks, std::optional<double> scale,
+                              bool with_lse, std::optional<uint64_t> stream) const {
+        check_queries(q, table);
+        need(blocks.dim() == 4, "blocks must be [sequences, queries, kv_heads, count]");
+        bs_block_attention_desc d{};
+        d.table = indexes(table, table.sizes(), "table", k.device());
+        d.lens = indexes(lens, {table.size(0)}, "lens", k.device());
+        d.blocks = indexes(blocks, {q.size(0), q.size(1), k.size(1), blocks.size(3)}, "blocks", k.device());
+        Target to(k.device(), stream);
+        const Tensor out = at::empty(q.sizes(), q.options());
+        const Tensor lse = with_lse ? at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat)) : Tensor();
+        d.q = q.const_data_ptr();
+        strides(q, d.q_stride);
+        d.out = out.data_ptr();
+        d.lse = with_lse ? lse.data_ptr<float>() : nullptr;
+        d.num_seqs = count(q.size(0));
+        d.table_width = count(table.size(1));
+        d.queries = count(q.size(1));
+        d.q_heads = count(q.size(2));
+        d.count = count(blocks.size(3));
+        d.dtype = type_of(q);
+        d.scale = scale_of(scale, q);
+        check(bs_block_attention(&c, &d, to.stream));
+        to.uses({&k, &v, &k_scale, &v_scale, &q, &table, &lens, &blocks});
+        to.gives({&out, &lse});
+        return py::make_tuple(from(out, {&q}), maybe(from(lse, {&q})));
+    }
+
+    py::tuple shared_attention(const Tensor& q, const Tensor& shared_table, const Tensor& shared_lens, const Tensor& cu, const Tensor& table,
+                               const Tensor& lens, std::optional<double> scale, bool with_lse, std::optional<uint64_t> stream) const {
+        check_queries(q, table);
+        need(shared_table.dim() == 2, "shared_table must be [groups, width]");
+        const int64_t groups = shared_table.size(0);
+        bs_shared_attention_desc d{};
+        d.shared_table = indexes(shared_table, shared_table.sizes(), "shared_table", k.device());
+        d.shared_lens = indexes(shared_lens, {groups}, "shared_lens", k.device());
+        d.cu = indexes(cu, {groups + 1}, "cu", k.device());
+        d.table = indexes(table, table.sizes(), "table", k.device());
+        d.lens = indexes(lens, {table.size(0)}, "lens", k.device());
+        Target to(k.device(), stream);
+        const Tensor out = at::empty(q.sizes(), q.options());
+        const Tensor lse = with_lse ? at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat)) : Tensor();
+        d.q = q.const_data_ptr();
+        strides(q, d.q_stride);
+        d.out = out.data_ptr();
+        d.lse = with_lse ? lse.data_ptr<float>() : nullptr;
+        d.num_seqs = count(q.size(0));
+        d.num_groups = count(groups);
+        d.shared_width = count(shared_table.size(1));
+        d.table_width = count(table.size(1));
+        d.queries = count(q.size(1));
+        d.q_heads = count(q.size(2));
+        d.dtype = type_of(q);
+        d.scale = scale_of(scale, q);
+        size_t bytes = 0;
+        check(bs_shared_attention_workspace(&c, &d, &bytes));
+        const Tensor work = scratch(bytes, k.device());
+        d.workspace = bytes ? work.data_ptr() : nullptr;
+        d.workspace_bytes = bytes;
+        check(bs_shared_attention(&c, &d, to.stream));
+        to.uses({&k, &v, &k_scale, &v_scale, &q, &shared_table, &shared_lens, &cu, &table, &lens});
+        to.gives({&out, &lse});
+        return py::make_tuple(from(out, {&q}), maybe(from(lse, {&q})));
+    }
+
     py::tuple evict(const Tensor& mass, const Tensor& table, const Tensor& lens, const Tensor& new_table, int64_t budget, int64_t sinks,
                     int64_t recent, std::optional<uint64_t> stream) const {
         need(table.dim() == 2 && new_table.dim() == 2, "table and new_table must be [sequences, width]");
@@ -352,6 +535,7 @@ uint32_t take_errors(int64_t device, std::optional<uint64_t> stream) {
 PYBIND11_MODULE(_memory, m) {
     m.def("set_error", [](py::object e) { g_error = e.release().ptr(); });
     m.def("prompt_attention", &prompt_attention);
+    m.def("norm_rotate", &norm_rotate);
     m.def("take_errors", &take_errors);
     py::class_<Cache>(m, "Cache")
         .def(py::init<const Tensor&, const Tensor&, const Tensor&, const Tensor&>())
@@ -362,5 +546,9 @@ PYBIND11_MODULE(_memory, m) {
         .def("_write", &Cache::write)
         .def("_read", &Cache::read)
         .def("_attention", &Cache::attention)
+        .def("_update_bounds", &Cache::update_bounds)
+        .def("_choose_blocks", &Cache::choose_blocks)
+        .def("_block_attention", &Cache::block_attention)
+        .def("_shared_attention", &Cache::shared_attention)
         .def("_evict", &Cache::evict);
 }

@@ -8,7 +8,11 @@ gives up are rows for an :class:`Index`, found again by its search.
     out, _ = memory.prompt_attention(q, k, v, cu)             # a packed batch of prompts
     cache = memory.TokenCache.empty(num_blocks, kv_heads, dim, block=64)
     cache.write(k, v, cu, table, start)                       # its keys and values, quantised
-    out, lse, mass = cache.attention(q1, table, lens, mass=mass, with_mass=True)   # one new token each
+    q1, k1 = memory.norm_rotate(q1, k1, positions, freqs, q_weight=w, k_weight=w)  # of one new token each
+    out, lse, mass = cache.attention(q1, table, lens, mass=mass, with_mass=True)
+    blocks = cache.choose_blocks(q1, cache.update_bounds(bounds, table, lens), table, lens, count)
+    out, lse = cache.block_attention(q1, table, lens, blocks)                      # or over a part of its cache
+    out, lse = cache.shared_attention(q1, shared_table, shared_lens, cu, table, lens)   # or with a shared beginning
     kept, lens, mass = cache.evict(mass, table, lens, new_table, budget)
     keys, values = cache.read(old_table, old_lens, positions)  # float rows for Index.from_vectors
 
@@ -17,8 +21,8 @@ current stream of the tensors' device) and never wait for the lengths, tables
 and positions, which stay on the device.  What only the device can see to be
 wrong is skipped and sets a bit that :func:`take_errors` returns.  There are no
 gradients: a backward pass that reaches an output raises, and what is written
-to a cache is cut off from the pass that made it.  C entries:
-bs_prompt_attention, bs_cache_* of include/bsearch.h.
+to a cache is cut off from the pass that made it.  C entries: from bs_dtype
+on in include/bsearch.h.
 """
 from __future__ import annotations
 
@@ -48,6 +52,53 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, with_
     earlier query one fewer.  scale defaults to dim ** -0.5.  Returns (out,
     lse): out like q, contiguous; lse float32 [total_q, q_heads] or None."""
     return _memory.prompt_attention(q, k, v, cu_q, cu_k, causal, scale, with_lse, stream)
+
+
+def rotary_frequencies(rotary, base=10000.0, *, scaling=None, factor=1.0, trained=None, fast=32.0, slow=1.0, device=None):
+    """(freqs, amplitude) for :func:`norm_rotate`: freqs float64 [rotary / 2],
+    base ** (-2 j / rotary) radians a position, changed for contexts `factor`
+    times as long as those of training:
+
+    scaling None: not at all; "linear": positions count 1 / factor; "base":
+    the base grows so that the slowest pair turns 1 / factor as fast and the
+    fastest as before; "parts": pairs that turn more than `fast` times in
+    `trained` positions stay, those that turn less than `slow` times count
+    1 / factor, a linear mixture between, and the amplitude is 0.1 log(factor) + 1."""
+    if rotary < 0 or rotary % 2:
+        raise ValueError("rotary must be even and not negative")
+    if scaling not in (None, "linear", "base", "parts"):
+        raise ValueError('scaling must be None, "linear", "base" or "parts"')
+    if not factor >= 1 or not base > 1:
+        raise ValueError("factor must be at least 1, base above 1")
+    j = torch.arange(0, rotary, 2, dtype=torch.float64, device=device)
+    if scaling == "base" and rotary > 2:
+        base = base * factor ** (rotary / (rotary - 2))
+    freqs = base ** (-j / max(rotary, 1))
+    if scaling == "linear":
+        return freqs / factor, 1.0
+    if scaling != "parts":
+        return freqs, 1.0
+    if trained is None or not fast > slow:
+        raise ValueError('"parts" needs `trained`, the positions of training, and fast above slow')
+    stay = ((trained * freqs / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+    return freqs * (stay + (1 - stay) / factor), 0.1 * math.log(factor) + 1
+
+
+def norm_rotate(q, k, positions, freqs=None, *, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, amplitude=1.0, stream=None):
+    """Norm of queries and keys for each head, then their rotary position, in
+    one pass (bs_norm_rotate).
+
+    q [tokens, q_heads, dim] and k [tokens, kv_heads, dim] (or None), float16
+    or bfloat16, any token and head strides that are multiples of 8 elements
+    (slices of one projection's output, for instance).  A head is divided by
+    the root of its mean square and multiplied by q_weight or k_weight [dim]
+    where that is given.  Then its first 2 * len(freqs) dimensions are rotated
+    by positions (int32 [tokens], any sign) times freqs (float64, radians a
+    position; None: no rotation): pairs are the first and second half's j-th
+    dimensions, or with `interleaved` neighbours; `amplitude` multiplies sines
+    and cosines (:func:`rotary_frequencies` gives both).  Returns (q, k),
+    contiguous."""
+    return _memory.norm_rotate(q, k, positions, freqs, q_weight, k_weight, eps, interleaved, amplitude, stream)
 
 
 class TokenCache(_memory.Cache):
@@ -96,6 +147,44 @@ class TokenCache(_memory.Cache):
         is given (into `out_mass` where that is given, which may be `mass`),
         or None without with_mass, mass and out_mass."""
         return self._attention(q, table, lens, scale, with_lse, mass, with_mass, out_mass, stream)
+
+    def empty_bounds(self):
+        """Bounds of this cache's blocks, int8 [blocks, kv_heads, 2, dim], none known yet."""
+        blocks, heads, _, dim = self.k.shape
+        return torch.zeros((blocks, heads, 2, dim), dtype=torch.int8, device=self.k.device)
+
+    def update_bounds(self, bounds, table, lens, *, last=None, stream=None):
+        """Largest and smallest key code of each dimension (bs_block_bounds), into
+        `bounds`, for the blocks that hold any of the last `last` tokens of a
+        sequence (None: all its blocks); to be called when they have changed.
+        Returns bounds."""
+        self._update_bounds(bounds, table, lens, last, stream)
+        return bounds
+
+    def choose_blocks(self, q, bounds, table, lens, count, *, sinks=1, recent=1, stream=None):
+        """Which `count` blocks each query and key head attends to
+        (bs_block_choice: the first `sinks`, the last `recent`, and those that
+        may hold the largest scores by their bounds).  q [sequences, queries,
+        q_heads, dim] as in :meth:`attention`.  Returns int32 [sequences,
+        queries, kv_heads, count]: columns of the table, ascending, -1 past
+        the end."""
+        return self._choose_blocks(q, bounds, table, lens, count, sinks, recent, stream)
+
+    def block_attention(self, q, table, lens, blocks, *, scale=None, with_lse=False, stream=None):
+        """Attention of each sequence's last tokens over chosen blocks of its cache
+        (bs_block_attention): blocks int32 [sequences, queries, kv_heads,
+        count], columns of the table in any order, negative ones skipped.
+        Returns (out, lse) like :meth:`attention`."""
+        return self._block_attention(q, table, lens, blocks, scale, with_lse, stream)
+
+    def shared_attention(self, q, shared_table, shared_lens, cu, table, lens, *, scale=None, with_lse=False, stream=None):
+        """Attention of sequences that begin with the same tokens
+        (bs_shared_attention).  Sequences cu[m] .. cu[m + 1] (int32 [groups +
+        1]) begin with the shared_lens[m] tokens of shared_table[m] (int32
+        [groups, width]), which are read once for all of them; table and lens
+        are of what each has beyond those.  Returns (out, lse) like
+        :meth:`attention`, over both."""
+        return self._shared_attention(q, shared_table, shared_lens, cu, table, lens, scale, with_lse, stream)
 
     def evict(self, mass, table, lens, new_table, budget, *, sinks=4, recent=0, stream=None):
         """Cuts every sequence down to `budget` tokens for each head: the first

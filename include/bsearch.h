@@ -421,6 +421,131 @@ typedef struct bs_cache_evict_desc {
 BS_API bs_status bs_cache_evict(const bs_token_cache* cache, const bs_cache_evict_desc* desc, void* stream);
 BS_API bs_status bs_cache_evict_workspace(const bs_token_cache* cache, const bs_cache_evict_desc* desc, size_t* bytes);
 
+/* Norm and rotary position of queries and keys in one pass.  Each head's row x
+ * of q (and of k, with its own weight) becomes
+ *   y = x * w / sqrt(mean(x^2) + eps)        (no weight: y = x)
+ * and of its first `rotary` dimensions the pairs j < rotary / 2, (a, b) =
+ * (y[j], y[j + rotary / 2]) or, interleaved, (y[2 j], y[2 j + 1]), become
+ *   amplitude * (a cos t - b sin t, b cos t + a sin t),  t = position * freqs[j],
+ * rounded once, at the end.  An angle keeps its accuracy at any position: it is
+ * reduced to a part of a turn in integers, off by at most 2^-32 turns and 2^-52
+ * of itself.  freqs are finite, positions any.
+ * Outputs are contiguous; an output may be its own contiguous input. */
+typedef struct bs_norm_rotate_desc {
+    const void* q;            /* [total][q_heads][dim]                        */
+    const void* k;            /* [total][kv_heads][dim]; kv_heads 0: none     */
+    void* out_q;
+    void* out_k;
+    int64_t q_stride[2];      /* elements from token to token, head to head   */
+    int64_t k_stride[2];
+    const void* q_weight;     /* [dim], type weight_dtype, or NULL: no norm of q */
+    const void* k_weight;
+    const int32_t* positions; /* [total]; not read when rotary is 0           */
+    const double* freqs;      /* [rotary / 2], radians a position, 8-byte aligned */
+    uint32_t total;
+    int32_t q_heads, kv_heads, dim;
+    int32_t rotary;           /* even, at most dim; 0: norm alone             */
+    int32_t interleaved;
+    int32_t dtype;            /* BS_F16 or BS_BF16                            */
+    int32_t weight_dtype;     /* BS_F32, BS_F16 or BS_BF16                    */
+    float eps, amplitude;     /* eps finite and not negative, amplitude finite */
+} bs_norm_rotate_desc;
+
+BS_API bs_status bs_norm_rotate(const bs_norm_rotate_desc* desc, void* stream);
+
+/* Bounds of the key codes of a block: bounds[id][h][0][x] is the largest and
+ * [1][x] the smallest code of dimension x among the block's tokens at positions
+ * below lens[b].  Written are the blocks that hold any of the last `last` tokens
+ * of a sequence (last < 0: all its blocks), others stay as they are.  A block
+ * that is in the tables of several sequences gets the bounds of any of them.
+ * To be called when codes have changed: after bs_cache_write with the number of
+ * new tokens, after bs_cache_evict with last < 0 on the new tables. */
+typedef struct bs_block_bounds_desc {
+    int8_t* bounds;           /* [num_blocks][kv_heads][2][dim], 16-byte aligned */
+    const int32_t* table;     /* [num_seqs][table_width]                      */
+    const int32_t* lens;      /* [num_seqs], at most table_width * block      */
+    uint32_t num_seqs, table_width;
+    int32_t last;
+} bs_block_bounds_desc;
+
+BS_API bs_status bs_block_bounds(const bs_token_cache* cache, const bs_block_bounds_desc* desc, void* stream);
+
+/* Which blocks a query attends to, by what their bounds allow.  Query i of
+ * sequence b sees the positions below n = lens[b] - queries + 1 + i, so the
+ * first ceil(n / block) columns of its table.  If they are at most `count`, all
+ * are chosen; else the first `sinks`, the last `recent`, and of the others the
+ * count - sinks - recent of the largest score (ties: the lower column; NaN
+ * counts as largest).  A key head's query heads choose together:
+ *   m = max |q| over their elements,  c = rint(q * (127 / m))  (0 if m < 1e-30)
+ *   score = k_scale * sum over heads and dimensions of max(c * upper, c * lower),
+ * the sum exact in integers, then rounded to 32 bits, then the product: no sum
+ * of those heads' scores with a token of the block is larger, but for the
+ * rounding of q.  blocks[b][i][h]: columns in ascending order, -1 past the end. */
+typedef struct bs_block_choice_desc {
+    const void* q;            /* [num_seqs][queries][q_heads][dim]            */
+    int64_t q_stride[3];      /* elements from sequence to sequence, token to token, head to head */
+    const int8_t* bounds;     /* [num_blocks][kv_heads][2][dim], 16-byte aligned */
+    const int32_t* table;     /* [num_seqs][table_width]                      */
+    const int32_t* lens;      /* [num_seqs], at most table_width * block      */
+    int32_t* blocks;          /* [num_seqs][queries][kv_heads][count]         */
+    uint32_t num_seqs, table_width;
+    int32_t queries, q_heads, count, sinks, recent;
+    int32_t dtype;            /* BS_F16 or BS_BF16                            */
+} bs_block_choice_desc;
+
+BS_API bs_status bs_block_choice(const bs_token_cache* cache, const bs_block_choice_desc* desc, void* stream);
+
+/* Attention over chosen blocks: query i of sequence b and the heads of key head
+ * h see the tokens of the columns blocks[b][i][h][...] of the sequence's table
+ * at positions below lens[b] - queries + 1 + i.  Negative entries are skipped;
+ * a column twice in a list counts twice.  out, lse as in bs_prompt_attention. */
+typedef struct bs_block_attention_desc {
+    const void* q;            /* [num_seqs][queries][q_heads][dim]            */
+    int64_t q_stride[3];
+    const int32_t* table;     /* [num_seqs][table_width]                      */
+    const int32_t* lens;      /* [num_seqs], at most table_width * block      */
+    const int32_t* blocks;    /* [num_seqs][queries][kv_heads][count], in any order */
+    void* out;                /* [num_seqs][queries][q_heads][dim], type dtype */
+    float* lse;               /* [num_seqs][queries][q_heads], or NULL        */
+    uint32_t num_seqs, table_width;
+    int32_t queries, q_heads, count;
+    int32_t dtype;            /* BS_F16 or BS_BF16                            */
+    float scale;
+} bs_block_attention_desc;
+
+BS_API bs_status bs_block_attention(const bs_token_cache* cache, const bs_block_attention_desc* desc, void* stream);
+
+/* Attention of sequences that begin with the same tokens.  Sequences cu[m] ..
+ * cu[m+1] are group m, whose tokens' first shared_lens[m] are the positions of
+ * row m of shared_table; what a sequence has beyond them is in its own table,
+ * lens[b] tokens, the last `queries` of which are the query tokens: query i
+ * sees all shared tokens of its group and its own positions below
+ * lens[b] - queries + 1 + i.  cu starts at 0, ascends and ends at num_seqs
+ * (else error bit 4 is set and outputs may hold anything).  The shared keys and
+ * values are read once for all of a group's queries.  out, lse as in
+ * bs_prompt_attention, over both sets of tokens.  Waits inside are bounded as
+ * there. */
+typedef struct bs_shared_attention_desc {
+    const void* q;            /* [num_seqs][queries][q_heads][dim]            */
+    int64_t q_stride[3];
+    const int32_t* shared_table; /* [num_groups][shared_width]                */
+    const int32_t* shared_lens;  /* [num_groups], at most shared_width * block */
+    const int32_t* cu;        /* [num_groups + 1]                             */
+    const int32_t* table;     /* [num_seqs][table_width]                      */
+    const int32_t* lens;      /* [num_seqs], at most table_width * block      */
+    void* out;                /* [num_seqs][queries][q_heads][dim], type dtype */
+    float* lse;               /* [num_seqs][queries][q_heads], or NULL        */
+    void* workspace;
+    size_t workspace_bytes;
+    uint32_t num_seqs, num_groups, shared_width, table_width;
+    int32_t queries, q_heads;
+    int32_t dtype;            /* BS_F16 or BS_BF16                            */
+    float scale;
+} bs_shared_attention_desc;
+
+BS_API bs_status bs_shared_attention(const bs_token_cache* cache, const bs_shared_attention_desc* desc, void* stream);
+BS_API bs_status bs_shared_attention_workspace(const bs_token_cache* cache, const bs_shared_attention_desc* desc, size_t* bytes);
+
 /* Error bits that token-memory kernels have set on the current device since
  * the last call, ordered after the work queued on `stream`; synchronises
  * `stream`.  The bits returned are cleared, others that kernels on other

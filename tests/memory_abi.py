@@ -45,6 +45,36 @@ class _Evict(ctypes.Structure):
                 ("sinks", _i32), ("recent", _i32)]
 
 
+class _Rotate(ctypes.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("out_q", _vp), ("out_k", _vp), ("q_stride", _i64 * 2), ("k_stride", _i64 * 2),
+                ("q_weight", _vp), ("k_weight", _vp), ("positions", _vp), ("freqs", _vp), ("total", _u32), ("q_heads", _i32),
+                ("kv_heads", _i32), ("dim", _i32), ("rotary", _i32), ("interleaved", _i32), ("dtype", _i32),
+                ("weight_dtype", _i32), ("eps", ctypes.c_float), ("amplitude", ctypes.c_float)]
+
+
+class _Bounds(ctypes.Structure):
+    _fields_ = [("bounds", _vp), ("table", _vp), ("lens", _vp), ("num_seqs", _u32), ("table_width", _u32), ("last", _i32)]
+
+
+class _Choice(ctypes.Structure):
+    _fields_ = [("q", _vp), ("q_stride", _i64 * 3), ("bounds", _vp), ("table", _vp), ("lens", _vp), ("blocks", _vp),
+                ("num_seqs", _u32), ("table_width", _u32), ("queries", _i32), ("q_heads", _i32), ("count", _i32),
+                ("sinks", _i32), ("recent", _i32), ("dtype", _i32)]
+
+
+class _Blocks(ctypes.Structure):
+    _fields_ = [("q", _vp), ("q_stride", _i64 * 3), ("table", _vp), ("lens", _vp), ("blocks", _vp), ("out", _vp), ("lse", _vp),
+                ("num_seqs", _u32), ("table_width", _u32), ("queries", _i32), ("q_heads", _i32), ("count", _i32),
+                ("dtype", _i32), ("scale", ctypes.c_float)]
+
+
+class _Shared(ctypes.Structure):
+    _fields_ = [("q", _vp), ("q_stride", _i64 * 3), ("shared_table", _vp), ("shared_lens", _vp), ("cu", _vp), ("table", _vp),
+                ("lens", _vp), ("out", _vp), ("lse", _vp), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+                ("num_seqs", _u32), ("num_groups", _u32), ("shared_width", _u32), ("table_width", _u32), ("queries", _i32),
+                ("q_heads", _i32), ("dtype", _i32), ("scale", ctypes.c_float)]
+
+
 _ready = None
 
 
@@ -62,6 +92,12 @@ def _lib():
                            ("bs_cache_attention_workspace", [P(_Cache), P(_Attention), P(ctypes.c_size_t)]),
                            ("bs_cache_evict", [P(_Cache), P(_Evict), _vp]),
                            ("bs_cache_evict_workspace", [P(_Cache), P(_Evict), P(ctypes.c_size_t)]),
+                           ("bs_norm_rotate", [P(_Rotate), _vp]),
+                           ("bs_block_bounds", [P(_Cache), P(_Bounds), _vp]),
+                           ("bs_block_choice", [P(_Cache), P(_Choice), _vp]),
+                           ("bs_block_attention", [P(_Cache), P(_Blocks), _vp]),
+                           ("bs_shared_attention", [P(_Cache), P(_Shared), _vp]),
+                           ("bs_shared_attention_workspace", [P(_Cache), P(_Shared), P(ctypes.c_size_t)]),
                            ("bs_memory_take_errors", [_vp, P(_u32)])):
             f = getattr(L, name)
             f.argtypes, f.restype = args, ctypes.c_int
