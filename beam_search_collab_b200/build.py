@@ -33,7 +33,7 @@ MEMORY_PY = os.path.join(PKG, "_memory.so")
 
 CU_SOURCES = ["bs_search.cu", "bs_search_nb.cu", "bs_search_bq.cu", "bs_rabitq.cu", "bs_rabitq_nb.cu", "bs_graph_build.cu", "bs_ground_truth.cu", "bs_load.cu", "bs_entry.cu", "bs_merge.cu", "bs_codebook.cu",
               "bs_prompt_attention.cu", "bs_cache_attention.cu", "bs_token_cache.cu", "bs_norm_rotate.cu", "bs_block_choice.cu",
-              "bs_block_attention.cu", "bs_memory_capi.cu",
+              "bs_block_attention.cu", "bs_shared_attention.cu", "bs_memory_capi.cu",
               "bs_capi.cu"]
 NVCC_FLAGS = ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",

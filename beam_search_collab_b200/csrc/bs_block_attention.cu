@@ -14,33 +14,35 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "bs_cache_tile.cuh"
 #include "bs_device.cuh"
 #include "bs_memory.h"
+#include "bs_shared.cuh"
 
 namespace bsb {
 
 using namespace dev;
 using namespace tile;
+using shared::Group;
+using shared::SharedArgs;
 namespace cg = cooperative_groups;
 
 namespace {
 
 constexpr uint32_t kMostIds = 256;     // entries looked up at a time
 constexpr uint32_t kMostCluster = 8;
+constexpr uint32_t kBatch = 4;          // pieces of the shared tokens' outputs on their way together
 template <int NT>
 constexpr int kStagesOf = NT == 1 ? 2 : 3;
 constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 
 struct RowsArgs {
-    bs_token_cache c;
-    bs_shared_attention_desc d;        // of a list of blocks: what both have
+    SharedArgs s;                      // of a list of blocks: what both have
     const int32_t* blocks;             // [num_seqs][queries][kv_heads][count]
-    unsigned int* errors;
     uint32_t count;
-    uint32_t group;                    // query heads per key head
     uint32_t rows;                     // of a segment
-    uint32_t block_log2;
 };
 
 template <int NW>
@@ -52,7 +54,13 @@ constexpr int kJoinOrIds = kJoinBytes<NW, NT> > kIdBytes ? kJoinBytes<NW, NT> : 
 template <int NW, int NT>
 constexpr size_t kRowsSmem = kWarps * kStagesOf<NT> * kListStage<NW> + (kWarps + 1) * 8 * NT * 2 * 4 + kJoinOrIds<NW, NT>;
 
-__device__ __forceinline__ uint32_t tokens_of(const RowsArgs& a, const int32_t* lens, uint32_t i, uint32_t width) {
+// Where a row's outputs over the shared tokens are: `pieces` of them, by row of
+// the outputs if there is one, else from slot `first` of the share on.
+struct FarRow {
+    uint32_t pieces, share, slot, row;
+};
+
+__device__ __forceinline__ uint32_t tokens_of(const SharedArgs& a, const int32_t* lens, uint32_t i, uint32_t width) {
     const int32_t len = lens[i];
     const int64_t most = static_cast<int64_t>(width) * a.c.block;
     if (len >= 0 && len <= most) return len;
@@ -61,7 +69,7 @@ __device__ __forceinline__ uint32_t tokens_of(const RowsArgs& a, const int32_t* 
 }
 
 template <int NW, int NT, bool LIST>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __grid_constant__ RowsArgs a) {
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __grid_constant__ RowsArgs given) {
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr int kDim = NW * 16, kRows = 8 * NT, kStages = kStagesOf<NT>;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -74,24 +82,59 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
     cudaGridDependencySynchronize();       // in every block, before anything of the caller's
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = cluster.block_rank(), parts = cluster.num_blocks();
+    const SharedArgs& a = given.s;
     const bs_shared_attention_desc& d = a.d;
     const uint32_t hkv = a.c.kv_heads, b = blockIdx.z, segment = blockIdx.x / parts, row0 = blockIdx.y * kRows;
     const uint32_t h = LIST ? segment % hkv : segment, query = LIST ? segment / hkv : 0, block = a.c.block;
     const uint32_t len = tokens_of(a, d.lens, b, d.table_width);
 
+    // what the sequence shares: its group's place among the shares of that work
+    FarRow* const far_rows = reinterpret_cast<FarRow*>(smem);   // (over the ring, once that is done with)
+    Group shares_with{};
+    uint64_t units_before = 0, units = 0;
+    if (!LIST && a.shares) {
+        uint32_t m = 0;
+        for (uint32_t past = d.num_groups; past - m > 1;) {    // the last group that begins at b or before
+            const uint32_t mid = (m + past) / 2;
+            (d.cu[mid] <= static_cast<int32_t>(b) ? m : past) = mid;
+        }
+        shares_with = shared::group_of(a, m);
+        if (b < shares_with.first || static_cast<int32_t>(b) >= d.cu[m + 1]) shares_with.tiles = 0;
+        shared::count_cost(a, m, units_before, units, reinterpret_cast<uint64_t*>(smem));
+    }
+    if (!LIST && blockIdx.x == 0 && blockIdx.y == 0 && b == 0)
+        for (uint32_t i = threadIdx.x; i <= d.num_groups; i += kThreads) {
+            const int32_t x = d.cu[i];
+            if (i == 0 ? x != 0 : x < d.cu[i - 1] || (i == d.num_groups && static_cast<uint32_t>(x) != d.num_seqs))
+                atomicOr(a.errors, kMemErrLength);
+        }
+    auto far_of = [&](uint32_t r) {
+        FarRow far{};
+        if (shares_with.tiles == 0) return far;
+        const uint32_t in_group = (b - shares_with.first) * a.rows + r, pair = in_group / shared::kPairRows;
+        const uint64_t w = units * hkv;
+        const uint64_t s0 = units_before * hkv + (static_cast<uint64_t>(h) * shares_with.pairs + pair) * (shares_with.tiles + shared::kStart);
+        const uint32_t n = shared::used_shares(w, a.shares);
+        far.share = shared::share_of(w, n, s0 + shared::kStart);
+        far.pieces = shared::share_of(w, n, s0 + shared::kStart + shares_with.tiles - 1) - far.share + 1;
+        far.slot = shared::share_first(w, n, far.share) >= s0 ? 0 : 1;       // later shares begin inside the segment
+        far.row = in_group % shared::kPairRows;
+        return far;
+    };
+
     // this segment's query rows as the columns of K Q^T: column j is row row0 + j
     uint32_t q[NT][NW][2];
     float row_scale[NT][2];          // of columns 2c and 2c + 1
-    int32_t own_limit[NT][2];        // tokens of its own that row sees
+    int32_t limit[NT][2];        // tokens of its own that row sees
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const uint32_t r = row0 + 8 * nt + g, col = row0 + 8 * nt + 2 * c;
         const uint16_t* row = static_cast<const uint16_t*>(d.q) + b * d.q_stride[0] + static_cast<int64_t>(LIST ? query : r / a.group) * d.q_stride[1] +
                               (static_cast<int64_t>(h) * a.group + r % a.group) * d.q_stride[2] + c * (NW * 4);
-        load_query_row<NW>(q[nt], row_scale[nt], row, r < a.rows, d.dtype != BS_F16, d.scale * 1.4426950408889634f, c);
+        load_query_row<NW>(q[nt], row_scale[nt], row, r < given.rows, d.dtype != BS_F16, d.scale * 1.4426950408889634f, c);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            own_limit[nt][i] = static_cast<int32_t>(len) - d.queries + 1 + static_cast<int32_t>(LIST ? query : (col + i) / a.group);
+            limit[nt][i] = static_cast<int32_t>(len) - d.queries + 1 + static_cast<int32_t>(LIST ? query : (col + i) / a.group);
     }
     float o[NT][NW][4];
     float top[NT][2], sum[NT][2], unit = kFold / -kNoScore, inv_unit = -kNoScore;
@@ -103,132 +146,110 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
         for (int j = 0; j < NW; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
     }
 
-    for (int source = LIST ? 1 : 0; source < 2; ++source) {
-        const int32_t* table;
-        const int32_t* list = nullptr;
-        uint32_t entries, width, tokens;           // tokens: some row sees those below
-        int32_t limit[NT][2];
-        if (source == 0) {                         // what the group shares
-            uint32_t m = 0;
-            while (m + 1 < d.num_groups && static_cast<uint32_t>(d.cu[m + 1]) <= b) ++m;
-            const int32_t first = d.cu[m], past = d.cu[m + 1];
-            const bool ok = first >= 0 && static_cast<uint32_t>(first) <= b && past > static_cast<int32_t>(b) && static_cast<uint32_t>(past) <= d.num_seqs;
-            if (!ok || d.cu[0] != 0 || static_cast<uint32_t>(d.cu[d.num_groups]) != d.num_seqs) atomicOr(a.errors, kMemErrLength);
-            width = d.shared_width;
-            table = d.shared_table + static_cast<uint64_t>(m) * width;
-            tokens = ok ? tokens_of(a, d.shared_lens, m, width) : 0;
-            entries = (tokens + block - 1) / block;
-        } else {
-            width = d.table_width;
-            table = d.table + static_cast<uint64_t>(b) * width;
-            const int32_t most = static_cast<int32_t>(len) - (LIST ? d.queries - 1 - static_cast<int32_t>(query) : 0);
-            tokens = most > 0 ? most : 0;
-            entries = LIST ? a.count : (tokens + block - 1) / block;
-            if (LIST) list = a.blocks + ((static_cast<uint64_t>(b) * d.queries + query) * hkv + h) * a.count;
-        }
+    // the entries: the list's, or every block of its own
+    const int32_t* const table = d.table + static_cast<uint64_t>(b) * d.table_width;
+    const int32_t* const list = given.blocks + ((static_cast<uint64_t>(b) * d.queries + query) * hkv + h) * given.count;
+    const int32_t most = static_cast<int32_t>(len) - (LIST ? d.queries - 1 - static_cast<int32_t>(query) : 0);
+    const uint32_t width = d.table_width, tokens = most > 0 ? most : 0;           // some row sees the tokens below
+    const uint32_t entries = LIST ? given.count : (tokens + block - 1) / block;
+    // this block's part of the entries
+    const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(entries) * (rank + 1) / parts);
+    for (uint32_t from = static_cast<uint32_t>(static_cast<uint64_t>(entries) * rank / parts); from < end; from += kMostIds) {
+        // look them up; those without a token that is seen are left out
+        uint32_t held = 0;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) limit[nt][i] = source == 0 ? static_cast<int32_t>(tokens) : own_limit[nt][i];
-        // this block's part of the entries
-        const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(entries) * (rank + 1) / parts);
-        for (uint32_t from = static_cast<uint32_t>(static_cast<uint64_t>(entries) * rank / parts); from < end; from += kMostIds) {
-            // look them up; those without a token that is seen are left out
-            uint32_t held = 0;
-#pragma unroll
-            for (uint32_t e0 = 0; e0 < kMostIds; e0 += kThreads) {
-                const uint32_t e = from + e0 + threadIdx.x;
-                int64_t col = -1;
-                if (e < end) col = LIST ? list[e] : static_cast<int64_t>(e);
-                uint32_t id = kNoNode;
-                if (col >= 0 && col < width && col * block < tokens) {
-                    id = table[col];
-                    if (id >= a.c.num_blocks) {
-                        atomicOr(a.errors, kMemErrBlock);
-                        id = kNoNode;
-                    }
-                } else if (LIST && col >= width) {
-                    atomicOr(a.errors, kMemErrLength);
+        for (uint32_t e0 = 0; e0 < kMostIds; e0 += kThreads) {
+            const uint32_t e = from + e0 + threadIdx.x;
+            int64_t col = -1;
+            if (e < end) col = LIST ? list[e] : static_cast<int64_t>(e);
+            uint32_t id = kNoNode;
+            if (col >= 0 && col < width && col * block < tokens) {
+                id = table[col];
+                if (id >= a.c.num_blocks) {
+                    atomicOr(a.errors, kMemErrBlock);
+                    id = kNoNode;
                 }
-                const unsigned in = __ballot_sync(kFull, id != kNoNode);
-                if (lane == 0) found[warp] = __popc(in);
-                __syncthreads();
-                uint32_t at = held + __popc(in & ((1u << lane) - 1));
-#pragma unroll
-                for (uint32_t x = 0; x < kWarps; ++x) {
-                    const uint32_t n = found[x];
-                    if (x < warp) at += n;
-                    held += n;
-                }
-                if (id != kNoNode) ids[at] = make_int2(id, static_cast<int32_t>(col * block));
-                __syncthreads();
+            } else if (LIST && col >= width) {
+                atomicOr(a.errors, kMemErrLength);
             }
-            const uint32_t tiles = ((held << a.block_log2) + kTile - 1) / kTile;
-            auto request = [&](uint32_t t, uint32_t stage) {
-                if (t < tiles) {
-                    unsigned char* s = ring + stage * kListStage<NW>;
-                    float* scales = reinterpret_cast<float*>(s + 2 * kTile * kPitch<NW>);
+            const unsigned in = __ballot_sync(kFull, id != kNoNode);
+            if (lane == 0) found[warp] = __popc(in);
+            __syncthreads();
+            uint32_t at = held + __popc(in & ((1u << lane) - 1));
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const uint32_t at = t * kTile + 16 * half, e = at >> a.block_log2, in = at & (block - 1);
-                        const int2 entry = e < held ? ids[e] : make_int2(0, 0x40000000);
-                        const int32_t pos = entry.y + static_cast<int32_t>(in);
-                        if (pos < static_cast<int32_t>(tokens)) {
-                            const uint64_t slab = static_cast<uint64_t>(static_cast<uint32_t>(entry.x)) * hkv + h;
-                            const uint64_t row = ((slab << a.block_log2) + in) * kDim + lane * 16;
-                            const int8_t* k = a.c.k + row;
-                            const int8_t* v = a.c.v + row;
-#pragma unroll
-                            for (int j = 0; j < (NW + 1) / 2; ++j) {
-                                const uint32_t i = lane + 32 * j, r = i / NW + 16 * half, x = i % NW;
-                                if (NW % 2 && i >= 16 * NW) break;
-                                copy16(s + r * kPitch<NW> + unit_at<NW>(x, r), k + j * 512);
-                                copy16(s + (kTile + r) * kPitch<NW> + unit_at<NW>(x, r), v + j * 512);
-                            }
-                            if (lane < 2) copy4(scales + 2 * half + lane, (lane ? a.c.v_scale : a.c.k_scale) + slab);
-                        } else if (lane == 0) {       // no tokens to see: a value scale below zero says so
-                            scales[2 * half] = 0.f;
-                            scales[2 * half + 1] = -1.f;
-                        }
-                        if (lane == 2) reinterpret_cast<int32_t*>(scales)[4 + half] = pos;
-                    }
-                }
-                asm volatile("cp.async.commit_group;\n" ::: "memory");
-            };
-#pragma unroll
-            for (int i = 0; i < kStages - 1; ++i) request(warp + i * kWarps, i);
-            uint32_t stage = 0, fill = kStages - 1;
-            for (uint32_t t = warp; t < tiles; t += kWarps) {
-                asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
-                __syncwarp();
-                request(t + (kStages - 1) * kWarps, fill);       // the stage that the last tile used
-                fill = fill + 1 == kStages ? 0 : fill + 1;
-                const unsigned char* s = ring + stage * kListStage<NW>;
-                stage = stage + 1 == kStages ? 0 : stage + 1;
-                const float4 sc = *reinterpret_cast<const float4*>(s + 2 * kTile * kPitch<NW>);
-                const int2 first = *reinterpret_cast<const int2*>(s + 2 * kTile * kPitch<NW> + 16);
-                const float k_scale[2] = {sc.x, sc.z}, v_scale[2] = {sc.y, sc.w};
-                const int32_t pos[2] = {first.x, first.y};
-                float z[2][NT][4];           // [half]: tokens g and g + 8 (+ 16 half), columns 2c and 2c + 1
-                tile_scores<NW, NT>(z, s, q, g, c);
-                const bool edge = max(pos[0], pos[1]) + 16 > static_cast<int32_t>(tokens) - (LIST ? 0 : d.queries - 1);
-                bool move = fmaxf(v_scale[0], v_scale[1]) > 4.f * unit;
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            z[half][nt][i] *= row_scale[nt][i & 1] * k_scale[half];
-                            if (edge && pos[half] + static_cast<int32_t>(g) + (i & 2) * 4 >= limit[nt][i & 1]) z[half][nt][i] = -INFINITY;
-                            move |= z[half][nt][i] > top[nt][i & 1] + kSlack;
-                        }
-                if (__any_sync(kFull, move)) move_maxima<NW, NT>(z, v_scale, top, sum, o, unit, inv_unit);
-                tile_values<NW, NT>(z, s, v_scale, inv_unit, top, sum, o, g, c);
-                __syncwarp();
+            for (uint32_t x = 0; x < kWarps; ++x) {
+                const uint32_t n = found[x];
+                if (x < warp) at += n;
+                held += n;
             }
-            __syncthreads();               // `ids` is done with
+            if (id != kNoNode) ids[at] = make_int2(id, static_cast<int32_t>(col * block));
+            __syncthreads();
         }
+        const uint32_t tiles = ((held << a.block_log2) + kTile - 1) / kTile;
+        auto request = [&](uint32_t t, uint32_t stage) {
+            if (t < tiles) {
+                unsigned char* s = ring + stage * kListStage<NW>;
+                float* scales = reinterpret_cast<float*>(s + 2 * kTile * kPitch<NW>);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t at = t * kTile + 16 * half, e = at >> a.block_log2, in = at & (block - 1);
+                    const int2 entry = e < held ? ids[e] : make_int2(0, 0x40000000);
+                    const int32_t pos = entry.y + static_cast<int32_t>(in);
+                    if (pos < static_cast<int32_t>(tokens)) {
+                        const uint64_t slab = static_cast<uint64_t>(static_cast<uint32_t>(entry.x)) * hkv + h;
+                        const uint64_t row = ((slab << a.block_log2) + in) * kDim + lane * 16;
+                        const int8_t* k = a.c.k + row;
+                        const int8_t* v = a.c.v + row;
+#pragma unroll
+                        for (int j = 0; j < (NW + 1) / 2; ++j) {
+                            const uint32_t i = lane + 32 * j, r = i / NW + 16 * half, x = i % NW;
+                            if (NW % 2 && i >= 16 * NW) break;
+                            copy16(s + r * kPitch<NW> + unit_at<NW>(x, r), k + j * 512);
+                            copy16(s + (kTile + r) * kPitch<NW> + unit_at<NW>(x, r), v + j * 512);
+                        }
+                        if (lane < 2) copy4(scales + 2 * half + lane, (lane ? a.c.v_scale : a.c.k_scale) + slab);
+                    } else if (lane == 0) {       // no tokens to see: a value scale below zero says so
+                        scales[2 * half] = 0.f;
+                        scales[2 * half + 1] = -1.f;
+                    }
+                    if (lane == 2) reinterpret_cast<int32_t*>(scales)[4 + half] = pos;
+                }
+            }
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) request(warp + i * kWarps, i);
+        uint32_t stage = 0, fill = kStages - 1;
+        for (uint32_t t = warp; t < tiles; t += kWarps) {
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
+            __syncwarp();
+            request(t + (kStages - 1) * kWarps, fill);       // the stage that the last tile used
+            fill = fill + 1 == kStages ? 0 : fill + 1;
+            const unsigned char* s = ring + stage * kListStage<NW>;
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+            const float4 sc = *reinterpret_cast<const float4*>(s + 2 * kTile * kPitch<NW>);
+            const int2 first = *reinterpret_cast<const int2*>(s + 2 * kTile * kPitch<NW> + 16);
+            const float k_scale[2] = {sc.x, sc.z}, v_scale[2] = {sc.y, sc.w};
+            const int32_t pos[2] = {first.x, first.y};
+            float z[2][NT][4];           // [half]: tokens g and g + 8 (+ 16 half), columns 2c and 2c + 1
+            tile_scores<NW, NT>(z, s, q, g, c);
+            const bool edge = max(pos[0], pos[1]) + 16 > static_cast<int32_t>(tokens) - (LIST ? 0 : d.queries - 1);
+            bool move = fmaxf(v_scale[0], v_scale[1]) > 4.f * unit;
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        z[half][nt][i] *= row_scale[nt][i & 1] * k_scale[half];
+                        if (edge && pos[half] + static_cast<int32_t>(g) + (i & 2) * 4 >= limit[nt][i & 1]) z[half][nt][i] = -INFINITY;
+                        move |= z[half][nt][i] > top[nt][i & 1] + kSlack;
+                    }
+            if (__any_sync(kFull, move)) move_maxima<NW, NT>(z, v_scale, top, sum, o, unit, inv_unit);
+            tile_values<NW, NT>(z, s, v_scale, inv_unit, top, sum, o, g, c);
+            __syncwarp();
+        }
+        __syncthreads();               // `ids` is done with
     }
 
     float all_top[NT][2], all_sum[NT][2];
@@ -237,14 +258,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
         const uint32_t i = LIST ? query : r / a.group;
         return (static_cast<uint64_t>(b) * d.queries + i) * d.q_heads + h * a.group + (LIST ? r : r - i * a.group);
     };
-    if (parts == 1) {
+    if (LIST && parts == 1) {
         if (warp != 0) return;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint32_t r = row0 + 8 * nt + 2 * c + i;
-                if (r >= a.rows) continue;
+                if (r >= given.rows) continue;
                 const float l = all_sum[nt][i], inv = l == 0.f ? 0.f : 1.f / l;
                 const uint64_t row = row_at(r);
                 if (g == 0 && d.lse) d.lse[row] = l == 0.f ? -INFINITY : (all_top[nt][i] + log2f(l)) * 0.6931471805599453f;
@@ -258,7 +279,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
             }
         return;
     }
-    // the cluster's outputs as one: a thread has four dimensions of a row
+    // the cluster's outputs as one, and those over the shared tokens: a thread
+    // has four dimensions of a row
     float* const part_o = join_o + kRows * kDim;               // (read by warp 1 alone, a barrier ago)
     float* const part_ml = join_ml + kWarps * kRows * 2;
     if (warp == 0)
@@ -272,10 +294,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
                 for (int j = 0; j < NW; ++j)
                     *reinterpret_cast<float2*>(part_o + r * kDim + value_dim<NW>(j, g)) = make_float2(o[nt][j][i], o[nt][j][2 + i]);
             }
-    cluster.sync();
+    if (!LIST && threadIdx.x < kRows && row0 + threadIdx.x < given.rows) far_rows[threadIdx.x] = far_of(row0 + threadIdx.x);
+    if (parts > 1) cluster.sync();
+    else __syncthreads();
     for (uint32_t x = rank * kThreads + threadIdx.x; x < kRows * kDim / 4; x += parts * kThreads) {
         const uint32_t r = x / (kDim / 4), at = x % (kDim / 4) * 4;
-        if (row0 + r >= a.rows) break;
+        if (row0 + r >= given.rows) break;
         float2 ml[kMostCluster];
         float m = kNoScore, l = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -292,8 +316,34 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
             l += ml[p].y * w;
             acc.x += y.x * w, acc.y += y.y * w, acc.z += y.z * w, acc.w += y.w * w;
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
         const uint64_t row = row_at(row0 + r);
+        const FarRow far = LIST ? FarRow{} : far_rows[r];
+        for (uint32_t p0 = 0; p0 < far.pieces; p0 += kBatch) {
+            float2 far_ml[kBatch];
+            float4 y[kBatch];
+            float high = m;
+#pragma unroll
+            for (uint32_t u = 0; u < kBatch; ++u) {
+                const uint32_t p = min(p0 + u, far.pieces - 1);
+                const uint64_t slot = ((static_cast<uint64_t>(far.share) + p) * 2 + (p == 0 ? far.slot : 0)) * shared::kPairRows + far.row;
+                far_ml[u] = far.pieces == 1 ? a.whole_ml[row] : a.part_ml[slot];
+                y[u] = *reinterpret_cast<const float4*>(far.pieces == 1 ? a.whole_o + row * kDim + at : a.part_o + slot * kDim + at);
+                if (p0 + u >= far.pieces) far_ml[u] = make_float2(kNoScore, 0.f);
+                high = fmaxf(high, far_ml[u].x);
+            }
+            const float shrink = exp2_fast(m - high);
+            m = high;
+            l *= shrink;
+            acc.x *= shrink, acc.y *= shrink, acc.z *= shrink, acc.w *= shrink;
+#pragma unroll
+            for (uint32_t u = 0; u < kBatch; ++u) {
+                if (p0 + u >= far.pieces) break;
+                const float w = exp2_fast(far_ml[u].x - m);
+                l += far_ml[u].y * w;
+                acc.x += y[u].x * w, acc.y += y[u].y * w, acc.z += y[u].z * w, acc.w += y[u].w * w;
+            }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         if (at == 0 && d.lse) d.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
         uint2 u;
         if (d.dtype == BS_F16) {
@@ -305,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
         }
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(d.out) + row * kDim + at) = u;
     }
-    cluster.sync();                        // no block ends while another reads it
+    if (parts > 1) cluster.sync();         // no block ends while another reads it
 }
 
 // Blocks of a segment, by the time of its longest part and of all of them: a
@@ -331,9 +381,9 @@ cudaError_t launch_rows(const RowsArgs& a, const MemoryDevice& dev, cudaStream_t
     const cudaError_t e = cudaFuncSetAttribute(k_rows<NW, NT, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem<NW, NT>);
     if (e != cudaSuccess) return e;
     const uint32_t row_tiles = (a.rows + 8 * NT - 1) / (8 * NT);
-    const uint64_t segments = static_cast<uint64_t>(a.c.kv_heads) * (LIST ? a.d.queries : 1);
-    const uint64_t width = LIST ? a.count : static_cast<uint64_t>(a.d.table_width) + a.d.shared_width;
-    const uint32_t parts = parts_of(segments * row_tiles * a.d.num_seqs, width * a.c.block, static_cast<uint64_t>(dev.num_sms) * blocks_per_sm(NT));
+    const uint64_t segments = static_cast<uint64_t>(a.s.c.kv_heads) * (LIST ? a.s.d.queries : 1);
+    const uint64_t width = LIST ? a.count : a.s.d.table_width;
+    const uint32_t parts = parts_of(segments * row_tiles * a.s.d.num_seqs, width * a.s.c.block, static_cast<uint64_t>(dev.num_sms) * blocks_per_sm(NT));
     cudaLaunchAttribute attr[2] = {};
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = parts;
@@ -341,7 +391,7 @@ cudaError_t launch_rows(const RowsArgs& a, const MemoryDevice& dev, cudaStream_t
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(static_cast<unsigned>(segments * parts), row_tiles, a.d.num_seqs);
+    config.gridDim = dim3(static_cast<unsigned>(segments * parts), row_tiles, a.s.d.num_seqs);
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = kRowsSmem<NW, NT>;
     config.stream = stream;
@@ -352,7 +402,7 @@ cudaError_t launch_rows(const RowsArgs& a, const MemoryDevice& dev, cudaStream_t
 
 template <int NT, bool LIST>
 cudaError_t launch_rows(const RowsArgs& a, const MemoryDevice& dev, cudaStream_t stream) {
-    switch (a.c.dim / 16) {
+    switch (a.s.c.dim / 16) {
         case 1: return launch_rows<1, NT, LIST>(a, dev, stream);
         case 2: return launch_rows<2, NT, LIST>(a, dev, stream);
         case 3: return launch_rows<3, NT, LIST>(a, dev, stream);
@@ -366,35 +416,80 @@ cudaError_t launch_rows(const RowsArgs& a, const MemoryDevice& dev, cudaStream_t
 
 uint32_t log2_of(int32_t block) { return block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7; }
 
+struct Layout {
+    uint32_t shares;
+    size_t whole_ml, whole_o, part_ml, part_o, total;
+};
+
+Layout plan(const bs_token_cache& c, const bs_shared_attention_desc& d, const MemoryDevice& dev) {
+    Layout l{};
+    const uint64_t tiles = (static_cast<uint64_t>(d.shared_width) * c.block + shared::kTileTokens - 1) / shared::kTileTokens;
+    if (tiles == 0) return l;
+    const uint64_t rows = static_cast<uint64_t>(d.num_seqs) * d.queries * d.q_heads;
+    // pairs of row tiles: those that the rows fill, and one more for each group
+    const uint64_t pairs = rows / c.kv_heads / shared::kPairRows + std::min(d.num_groups, d.num_seqs);
+    const uint64_t units = pairs * c.kv_heads * (tiles + shared::kStart), most = (units + 2 * shared::kStart - 1) / (2 * shared::kStart);
+    l.shares = static_cast<uint32_t>(most < static_cast<uint64_t>(dev.num_sms) ? most : dev.num_sms);
+    auto take = [&l](size_t bytes) {
+        const size_t at = l.total;
+        l.total += (bytes + 255) & ~static_cast<size_t>(255);
+        return at;
+    };
+    const size_t slots = static_cast<size_t>(l.shares) * 2 * shared::kPairRows;
+    l.whole_ml = take(rows * 8);
+    l.whole_o = take(rows * c.dim * 4);
+    l.part_ml = take(slots * 8);
+    l.part_o = take(slots * c.dim * 4);
+    return l;
+}
+
 }  // namespace
 
 cudaError_t launch_block_attention(const bs_token_cache& c, const bs_block_attention_desc& d, const MemoryDevice& dev, cudaStream_t stream) {
-    RowsArgs a{c, {}, d.blocks, dev.errors};
-    a.d.q = d.q;
-    for (int i = 0; i < 3; ++i) a.d.q_stride[i] = d.q_stride[i];
-    a.d.table = d.table;
-    a.d.lens = d.lens;
-    a.d.out = d.out;
-    a.d.lse = d.lse;
-    a.d.num_seqs = d.num_seqs;
-    a.d.table_width = d.table_width;
-    a.d.queries = d.queries;
-    a.d.q_heads = d.q_heads;
-    a.d.dtype = d.dtype;
-    a.d.scale = d.scale;
+    RowsArgs a{};
+    a.s.c = c;
+    a.s.errors = dev.errors;
+    a.s.d.q = d.q;
+    for (int i = 0; i < 3; ++i) a.s.d.q_stride[i] = d.q_stride[i];
+    a.s.d.table = d.table;
+    a.s.d.lens = d.lens;
+    a.s.d.out = d.out;
+    a.s.d.lse = d.lse;
+    a.s.d.num_seqs = d.num_seqs;
+    a.s.d.table_width = d.table_width;
+    a.s.d.queries = d.queries;
+    a.s.d.q_heads = d.q_heads;
+    a.s.d.dtype = d.dtype;
+    a.s.d.scale = d.scale;
+    a.s.group = d.q_heads / c.kv_heads;
+    a.s.block_log2 = log2_of(c.block);
+    a.blocks = d.blocks;
     a.count = d.count;
-    a.group = a.rows = d.q_heads / c.kv_heads;
-    a.block_log2 = log2_of(c.block);
+    a.rows = a.s.group;
     return a.rows <= 8 ? launch_rows<1, true>(a, dev, stream) : launch_rows<2, true>(a, dev, stream);
 }
 
-size_t shared_attention_scratch(const bs_token_cache&, const bs_shared_attention_desc&, const MemoryDevice&) { return 0; }
+size_t shared_attention_scratch(const bs_token_cache& c, const bs_shared_attention_desc& d, const MemoryDevice& dev) {
+    return plan(c, d, dev).total;
+}
 
 cudaError_t launch_shared_attention(const bs_token_cache& c, const bs_shared_attention_desc& d, const MemoryDevice& dev, cudaStream_t stream) {
-    RowsArgs a{c, d, nullptr, dev.errors};
-    a.group = d.q_heads / c.kv_heads;
-    a.rows = a.group * d.queries;
-    a.block_log2 = log2_of(c.block);
+    const Layout l = plan(c, d, dev);
+    unsigned char* const work = static_cast<unsigned char*>(d.workspace);
+    RowsArgs a{};
+    a.s.c = c;
+    a.s.d = d;
+    a.s.errors = dev.errors;
+    a.s.whole_ml = reinterpret_cast<float2*>(work + l.whole_ml);
+    a.s.whole_o = reinterpret_cast<float*>(work + l.whole_o);
+    a.s.part_ml = reinterpret_cast<float2*>(work + l.part_ml);
+    a.s.part_o = reinterpret_cast<float*>(work + l.part_o);
+    a.s.group = d.q_heads / c.kv_heads;
+    a.s.rows = a.rows = a.s.group * d.queries;
+    a.s.shares = l.shares;
+    a.s.block_log2 = log2_of(c.block);
+    const cudaError_t e = l.shares ? launch_shared_part(a.s, stream) : cudaSuccess;
+    if (e != cudaSuccess) return e;
     return a.rows <= 8 ? launch_rows<1, false>(a, dev, stream) : launch_rows<2, false>(a, dev, stream);
 }
 

@@ -456,6 +456,8 @@ static bs_status check_shared(const bs_token_cache* c, const bs_shared_attention
     if (!d) return report_error(BS_ERR_INVALID_ARGUMENT, "desc is NULL");
     if (bs_status s = check_queries(c, d->dtype, d->q_heads, d->num_seqs, d->table_width, d->queries)) return s;
     if (bs_status s = check_table(c, d->num_groups, d->shared_width)) return s;
+    if (static_cast<uint64_t>(d->num_seqs) * d->queries * d->q_heads >= (1ull << 31))
+        return report_error(BS_ERR_UNSUPPORTED, "fewer than 2^31 query rows (sequences, queries and heads) are supported");
     return check_scale(d->scale);
 }
 

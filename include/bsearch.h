@@ -524,7 +524,7 @@ BS_API bs_status bs_block_attention(const bs_token_cache* cache, const bs_block_
  * (else error bit 4 is set and outputs may hold anything).  The shared keys and
  * values are read once for all of a group's queries.  out, lse as in
  * bs_prompt_attention, over both sets of tokens.  Waits inside are bounded as
- * there. */
+ * there; after one that gave up (error bit 1) outputs hold anything. */
 typedef struct bs_shared_attention_desc {
     const void* q;            /* [num_seqs][queries][q_heads][dim]            */
     int64_t q_stride[3];

@@ -258,6 +258,18 @@ def test_two_streams_at_once():
         assert all(torch.equal(x, want[i]) for x in got[i])
 
 
+def test_a_wait_that_gives_up_sets_a_bit(monkeypatch):
+    groups, shared, lens = [40], [3000], [3] * 40
+    pool, shared_table, table, q = case(18, groups, shared, lens, 8, 2, 32, 128, 1, BF16)
+    good = check(pool, shared_table, table, q, groups, shared, lens)
+    monkeypatch.setenv("BSEARCH_WAIT_POLLS", "0")
+    M.TokenCache(*pool).shared_attention(q, shared_table, R.i32(shared), R.cu(groups), table, R.i32(lens))
+    assert M.take_errors() & 1
+    monkeypatch.delenv("BSEARCH_WAIT_POLLS")
+    again = check(pool, shared_table, table, q, groups, shared, lens)
+    assert all(torch.equal(a, b) for a, b in zip(good, again))
+
+
 def test_refusals():
     groups, shared, lens = [3, 2], [300, 200], [40] * 5
     pool, shared_table, table, q = case(15, groups, shared, lens, 4, 2, 32, 64, 1, F16)

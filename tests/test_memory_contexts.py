@@ -137,16 +137,16 @@ def test_host_tensors_are_refused():
 def test_kernels_wait_for_the_one_before_them_first():
     # launched under the end of the kernel before: nothing of the caller's is read and no error bit set before the wait
     kernels = 0
-    for name in ("bs_norm_rotate.cu", "bs_block_choice.cu", "bs_block_attention.cu"):
+    for name in ("bs_norm_rotate.cu", "bs_block_choice.cu", "bs_block_attention.cu", "bs_shared_attention.cu"):
         with open(os.path.join(B.PKG, "csrc", name)) as f:
             text = f.read()
         for m in re.finditer(r"__global__ void[^;{]*?(k_\w+)\(", text):
             body = text[m.end():text.index("\n}\n", m.end())]
             before, wait, _ = body.partition("cudaGridDependencySynchronize();")
             assert wait, m[1]
-            assert not re.search(r"tokens_of\(|atomicOr\(|\bd\.\w+\[|table\[", before), m[1]
+            assert not re.search(r"tokens_of\(|group_of\(|count_cost\(|atomicOr\(|\bd\.\w+\[|table\[", before), m[1]
             kernels += 1
-    assert kernels >= 4
+    assert kernels >= 5
 
 
 def test_frequencies():
