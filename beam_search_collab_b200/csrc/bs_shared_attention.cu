@@ -12,14 +12,17 @@
 // Every row sees every token, but for the end of the last tile.
 //
 // Warps 0-3 and 4-7 are the softmax of tile 0 and 1 (a thread has one row),
-// 8-11 load and convert keys and values, 12 issues the matrix instructions:
-//   S_t = Q_t K^T     codes of K exact in the queries' 16-bit type
+// 8-13 convert keys and values, 14 issues the matrix instructions, 15 copies
+// codes (a bulk copy for each block) and scales to shared memory:
+//   S_t = Q_t K^T     codes of K exact in f16, as are bf16 queries times a power
+//                     of two of each row's own (elements below 2^-29 of the
+//                     row's largest lose bits)
 //   O_t += P_t V      codes of V exact in f16, P_t f16: a weight times its values'
 //                     scale, over the largest of the piece, rounded to 2^-11 of
-//                     itself or, where that is more, 2^-31 of a weight of 1 at
+//                     itself or, where that is more, 2^-29 of a weight of 1 at
 //                     the largest scale (weights count in 2^-kLift, the room
-//                     that a maximum moved at 2^8 leaves)
-// The maximum is moved only when a sum of 32 weights passes 2^8 (no maximum is
+//                     that a maximum moved at 2^10 leaves)
+// The maximum is moved only when a sum of 32 weights passes 2^10 (no maximum is
 // taken before the exponentials); sums are 32-bit, of the unrounded weights.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -38,51 +41,44 @@ using namespace tc;
 
 namespace {
 
-constexpr int kConverters = 4;         // warps
+constexpr int kConverters = 6;         // warps
 constexpr int kIssuer = 8 + kConverters;
-constexpr int kThreads = 32 * (kIssuer + 1);
-constexpr int kStages = 2;             // of keys, and of values
-constexpr float kLift = 7.f, kLifted = 128.f;
-constexpr float kMost = 256.f * kLifted;      // of a sum of 32 weights, and so of each: below f16's 65504
+constexpr int kCopier = kIssuer + 1;
+constexpr int kThreads = 32 * (kCopier + 1);
+constexpr int kStages = 2;             // of converted keys, and of values
+// Stages of codes: with rows of 128 dimensions one of each fits beside the others.
+template <int BOXES>
+constexpr int kRaw = BOXES == 2 ? 1 : 4;
+constexpr float kLift = 5.f;
+constexpr float kMost = 32768.f;       // of a sum of 32 lifted weights, and so of each: below f16's 65504
+// Tiles whose scales are in shared memory: the copies of a tile wait for the
+// conversion of the one kRaw before it, that for products with keys kStages
+// earlier, issued when the weights of the tile before are made: a tile's scales
+// are read no more when those of the one kRaw + kStages + 1 after it are written.
+constexpr int kScales = 8;
+static_assert(kRaw<1> + kStages + 1 <= kScales && kRaw<2> + kStages + 1 <= kScales, "scales are overwritten while they are read");
 
-template <typename T>
-__device__ __forceinline__ uint4 codes_to_16(uint32_t a, uint32_t b);
-// Four codes to a word: 0x6400 | u is 1024 + u in f16, minus 1152.
-template <>
-__device__ __forceinline__ uint4 codes_to_16<__half>(uint32_t a, uint32_t b) {
+// Eight codes in f16: 0x6400 | u is 1024 + u, minus 1152.
+__device__ __forceinline__ uint4 codes_to_halves(uint2 x) {
     uint4 r;
     uint32_t* const w = reinterpret_cast<uint32_t*>(&r);
-    a ^= 0x80808080u;
-    b ^= 0x80808080u;
+    x.x ^= 0x80808080u;
+    x.y ^= 0x80808080u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t u = __byte_perm(i < 2 ? a : b, 0x64646464u, i & 1 ? 0x4342 : 0x4140);
+        const uint32_t u = __byte_perm(i < 2 ? x.x : x.y, 0x64646464u, i & 1 ? 0x4342 : 0x4140);
         const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&u), __float2half2_rn(1152.f));
         w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     return r;
 }
-// In bf16 0x4300 | x is 128 + x for x < 128: the code's low seven bits, minus
-// 128, or 256 where its sign is set.
-template <>
-__device__ __forceinline__ uint4 codes_to_16<__nv_bfloat16>(uint32_t a, uint32_t b) {
-    uint4 r;
-    uint32_t* const w = reinterpret_cast<uint32_t*>(&r);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t u = __byte_perm(i < 2 ? a : b, 0x43434343u, i & 1 ? 0x4342 : 0x4140);
-        const uint32_t x = u & 0xff7fff7fu, y = u & 0xff80ff80u;
-        const __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return r;
-}
 
-// 16 codes of row r, two 16-byte units of it.
-template <typename T>
-__device__ __forceinline__ void put_codes(unsigned char* row, uint32_t unit, uint32_t r, const uint4& x) {
-    *reinterpret_cast<uint4*>(row + ((unit ^ r) * 16)) = codes_to_16<T>(x.x, x.y);
-    *reinterpret_cast<uint4*>(row + (((unit + 1) ^ r) * 16)) = codes_to_16<T>(x.z, x.w);
+// 16-byte aligned bytes of memory into shared memory.
+__device__ __forceinline__ void copy_bulk(void* dst, const void* src, unsigned bytes, uint64_t* bar) {
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");     // after what was read there before
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_addr(dst)), "l"(src),
+                 "r"(bytes), "r"(smem_addr(bar))
+                 : "memory");
 }
 
 // Where a block is in its share: tiles t .. end of a segment (group m, key
@@ -97,15 +93,18 @@ struct Piece {
 
 struct Control {
     uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
-    uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-    uint64_t sums[2 * (kIssuer + 1)];
+    uint64_t full[2][kStages], empty[2][kStages];        // [keys, values]
+    uint64_t raw_full[2][4], raw_empty[2][4];
+    uint64_t sums[2 * (kCopier + 1)];
+    uint32_t missing[kScales];          // by tile: bits of 16 tokens whose block is not there
+    __align__(16) float2 scales[kScales][8];      // by tile and 16 tokens: of keys, of values
     Piece start;
     uint32_t tmem;
     uint32_t gave_up;
 };
 
 template <int BOXES>
-constexpr size_t kSmem = 1024 + (2 + 2 * kStages) * BOXES * kBoxBytes + sizeof(Control);
+constexpr size_t kSmem = 1024 + (2 + 2 * kStages + kRaw<BOXES>) * BOXES * kBoxBytes + sizeof(Control);
 
 // The piece of a segment from its unit `from` on; its first kStart units
 // stand for no tiles.
@@ -195,15 +194,15 @@ __device__ __forceinline__ void rescale(uint32_t p_at, uint32_t o_at, int quarte
 }
 
 // 32 scores of a row: weights 2^(key scale * s + base) added to `part`, and
-// times their value scale packed in p.  `scales`: a lane below 8 has the tile's
-// block's key scale (log2 units), the next 8 lanes the value scales.
-__device__ __forceinline__ void weights32(const float* s, float scales, uint32_t col, uint32_t block_log2, float base, uint32_t* p, float& part) {
+// times their value scale packed in p.  scales: of 16 tokens each; k_by and v_by
+// belong to the row and to the piece.
+__device__ __forceinline__ void weights32(const float* s, const float2* scales, float k_by, float v_by, float base, uint32_t* p, float& part) {
     const float2 base2 = make_float2(base, base);
     float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-        const uint32_t e = (col + 16 * half) >> block_log2;
-        const float k = __shfl_sync(kFull, scales, e), v = __shfl_sync(kFull, scales, 8 + e);
+        const float2 scale = scales[half];
+        const float k = scale.x * k_by, v = scale.y * v_by;
 #pragma unroll
         for (int i = 8 * half; i < 8 * half + 8; ++i) {
             float2 x = fma2(make_float2(s[2 * i], s[2 * i + 1]), make_float2(k, k), base2);
@@ -219,68 +218,64 @@ __device__ __forceinline__ void weights32(const float* s, float scales, uint32_t
 }
 
 // The first tile, the last one where the tokens end inside it, tiles with
-// blocks that are not there, and where the maximum moves.  From the quarter
-// `from` on; `left` tokens of the tile are there, `bad` has a bit for each 16
-// that are not.  `state` is the row's maximum (log2) and sum, returned as they
-// become.
-__device__ __noinline__ float2 weights_with_care(uint32_t s_at, uint32_t o_at, int from, int quarters, int32_t left, uint32_t bad, bool real,
-                                                 float scales, uint32_t block_log2, int dim, float2 state) {
-    float top = state.x, sum = state.y;
-#pragma unroll 1
-    for (int c = from; c < quarters; ++c) {
-        float s[32];
-        tmem_load32(s_at + 32 * c, s);
-        wait_loads32(s);
-        float z[32];
+// blocks that are not there, and where the maximum moves: the largest score
+// first, then the weights.  From the quarter `from` on; `left` tokens of the
+// tile are there, `missing` has a bit for each 16 that are not.  `state` is the
+// row's maximum (log2) and sum, returned as they become.
+__device__ __noinline__ float2 weights_with_care(uint32_t s_at, uint32_t o_at, int from, int quarters, int32_t left, uint32_t missing,
+                                                 const float2* scales, float k_by, float v_by, int dim, float2 state) {
+    float next = state.x;
+    float z[32];
+    auto scores = [&](int c) {             // in log2 units, -infinity where there is no token
+        tmem_load32(s_at + 32 * c, z);
+        wait_loads32(z);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const float k = __shfl_sync(kFull, scales, (32 * c + 16 * half) >> block_log2);
-            const bool gone = bad >> (2 * c + half) & 1;
+            const float k = scales[2 * c + half].x * k_by;
+            const int32_t there = missing >> (2 * c + half) & 1 ? 0 : left - 32 * c;
 #pragma unroll
-            for (int i = 16 * half; i < 16 * half + 16; ++i) z[i] = gone || 32 * c + i >= left ? -INFINITY : s[i] * k;
+            for (int i = 16 * half; i < 16 * half + 16; ++i) z[i] = i < there ? z[i] * k : -INFINITY;
         }
-        auto make = [&](uint32_t (&p)[16], float& part) {
-            const float base = top == -INFINITY ? 0.f : kLift - top;
-            part = 0.f;
+    };
+#pragma unroll 1
+    for (int c = from; c < quarters; ++c) {
+        scores(c);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const float v = __shfl_sync(kFull, scales, 8 + ((32 * c + 16 * half) >> block_log2));
-#pragma unroll
-                for (int i = 8 * half; i < 8 * half + 8; ++i) {
-                    const float x = exp2_fast(z[2 * i] + base), y = exp2_fast(z[2 * i + 1] + base);
-                    part += x + y;
-                    p[i] = Type16<__half>::pack(x * v, y * v);
-                }
-            }
-        };
+        for (int i = 0; i < 32; i += 2) next = fmaxf(next, fmaxf(z[i], z[i + 1]));
+    }
+    if (__any_sync(kFull, next > state.x)) {
+        // the maximum moves, what was summed is rescaled
+        const float shrink = state.x == -INFINITY ? 0.f : exp2_fast(state.x - next);
+        state.y *= shrink;
+        if (from || dim) rescale(s_at, o_at, from, dim, next == -INFINITY ? 1.f : shrink);
+    }
+    const float base = next == -INFINITY ? 0.f : kLift - next;
+#pragma unroll 1
+    for (int c = from; c < quarters; ++c) {
+        scores(c);
         uint32_t p[16];
-        float part;
-        make(p, part);
-        if (__any_sync(kFull, real && (part > kMost || top == -INFINITY))) {
-            // the maximum moves, what was summed is rescaled
-            float next = top;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) next = fmaxf(next, z[i]);
-            const float shrink = next == -INFINITY || top == -INFINITY ? (next == top ? 1.f : 0.f) : exp2_fast(top - next);
-            top = next;
-            sum *= shrink;
-            rescale(s_at, o_at, c, dim, shrink);
-            make(p, part);
+        for (int i = 0; i < 16; ++i) {
+            const float v = scales[2 * c + i / 8].y * v_by;
+            const float x = exp2_fast(z[2 * i] + base), y = exp2_fast(z[2 * i + 1] + base);
+            state.y += x + y;
+            p[i] = Type16<__half>::pack(x * v, y * v);
         }
-        sum += part;
         tmem_store16(s_at + 16 * c, p);
     }
-    return make_float2(top, sum);
+    return make_float2(next, state.y);
 }
 
-template <typename T, int BOXES>
+template <int BOXES>
 __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ SharedArgs a) {
     extern __shared__ unsigned char raw_smem[];
     unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t{1023});
     constexpr int kTileBytes = BOXES * kBoxBytes;
     unsigned char* const keys = smem + 2 * kTileBytes;
     unsigned char* const values = keys + kStages * kTileBytes;
-    Control& ctl = *reinterpret_cast<Control*>(values + kStages * kTileBytes);
+    unsigned char* const raw = values + kStages * kTileBytes;         // codes of keys, then of values
+    constexpr int kRawBytes = kTileBytes / 2;
+    Control& ctl = *reinterpret_cast<Control*>(raw + 2 * kRaw<BOXES> * kRawBytes);
     const bs_shared_attention_desc& d = a.d;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hkv = a.c.kv_heads, dim = a.c.dim, block = a.c.block;
 
@@ -304,11 +299,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                 barrier_init(&ctl.o_full[t], 1);
             }
             barrier_init(&ctl.done, 1);
-            for (int s = 0; s < kStages; ++s) {
-                barrier_init(&ctl.k_full[s], kConverters);
-                barrier_init(&ctl.v_full[s], kConverters);
-                barrier_init(&ctl.k_empty[s], 1);
-                barrier_init(&ctl.v_empty[s], 1);
+            for (int kv = 0; kv < 2; ++kv) {
+                for (int s = 0; s < kStages; ++s) {
+                    barrier_init(&ctl.full[kv][s], kConverters);
+                    barrier_init(&ctl.empty[kv][s], 1);
+                }
+                for (int s = 0; s < kRaw<BOXES>; ++s) {
+                    barrier_init(&ctl.raw_full[kv][s], 1);
+                    barrier_init(&ctl.raw_empty[kv][s], kConverters);
+                }
             }
             ctl.gave_up = 0;
             asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -354,15 +353,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         // ---------------------------------------------------- matrix products
         // (the whole warp runs the loop, one elected lane issues)
         constexpr uint32_t kCommon = 1u << 4 | static_cast<uint32_t>(kRows >> 4) << 24;
-        constexpr uint32_t kScores = kCommon | Type16<T>::kFormat << 7 | Type16<T>::kFormat << 10;
-        const uint32_t what_o = kCommon | 1u << 16 | (dim >> 3) << 17;         // f16 by f16, values not along the contraction
+        const uint32_t what_o = kCommon | 1u << 16 | (dim >> 3) << 17;         // (values do not lie along the contraction)
         const int steps = dim / 16;
         const uint64_t q_base = operand(smem_addr(smem), 16, 1024), k_base = operand(smem_addr(keys), 16, 1024);
         const uint64_t v_base = operand(smem_addr(values), kBoxBytes, 1024);
         constexpr uint32_t kTileUnits = kTileBytes / 16, kBoxUnits = kBoxBytes / 16;
         auto scores = [&](int t, uint32_t stage, uint32_t cols) {
             const uint64_t q = q_base + t * kTileUnits, k = k_base + stage * kTileUnits;
-            const uint32_t what = kScores | (cols >> 3) << 17;
+            const uint32_t what = kCommon | (cols >> 3) << 17;
 #pragma unroll
             for (int i = 0; i < 4 * BOXES; ++i) {
                 const uint32_t off = (i >> 2) * kBoxUnits + (i & 3) * 2;
@@ -382,21 +380,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         bool issued = false;
         pieces([&](const Piece& p) {
             const bool both = rows_left(p) > kRows;
-            wait(&ctl.k_full[loads % kStages], loads / kStages & 1);
+            wait(&ctl.full[0][loads % kStages], loads / kStages & 1);
             for (int t = 0; t <= both; ++t) wait(&ctl.q_full[t], q_used[t]++ & 1);
             if (stopped()) return false;
             issued = true;
             fence_after();
             if (elected()) {
                 for (int t = 0; t <= both; ++t) scores(t, loads % kStages, columns(p, p.t));
-                mma_commit(&ctl.k_empty[loads % kStages]);
+                mma_commit(&ctl.empty[0][loads % kStages]);
             }
             __syncwarp();
             for (uint32_t j = p.t; j < p.end; ++j, ++loads) {
                 const uint32_t stage = loads % kStages, next = (loads + 1) % kStages;
                 const bool last = j + 1 == p.end;
-                wait(&ctl.v_full[stage], loads / kStages & 1);
-                if (!last) wait(&ctl.k_full[next], (loads + 1) / kStages & 1);
+                wait(&ctl.full[1][stage], loads / kStages & 1);
+                if (!last) wait(&ctl.full[0][next], (loads + 1) / kStages & 1);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     if (t && !both) break;
@@ -411,8 +409,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                     __syncwarp();
                 }
                 if (elected()) {
-                    mma_commit(&ctl.v_empty[stage]);
-                    if (!last) mma_commit(&ctl.k_empty[next]);
+                    mma_commit(&ctl.empty[1][stage]);
+                    if (!last) mma_commit(&ctl.empty[0][next]);
                 }
                 __syncwarp();
             }
@@ -425,92 +423,106 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
             for (unsigned i = 0; i < kPolls && !barrier_test(&ctl.done, 0); ++i) {}
         }
         __syncwarp();
-    } else if (warp >= 8) {
-        // --------------------------------------------------------- conversion
-        // (eight lanes: one 16-byte chunk of eight tokens side by side, so that
-        // the swizzled stores fall on all banks; four such for 64 bytes of a row)
-        const uint32_t who = threadIdx.x - 256, sub = who >> 3, nw = dim / 16;
-        constexpr int kEach = 4 * BOXES;                     // chunks of a thread, of keys and of values
-        uint32_t row_of[kEach], chunk_of[kEach];
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const uint32_t u = sub + 16 * i;                 // of 16 * nw
-            row_of[i] = u / nw * 8 + (who & 7);
-            chunk_of[i] = u % nw;
-        }
-        // chunk i's place in the codes, in 16 bytes; kNothing: there are none
-        constexpr uint64_t kNothing = ~0ull;
-        auto find = [&](const Piece& p, uint32_t j, uint64_t (&place)[kEach]) {
+    } else if (warp == kCopier) {
+        // ------------------------------------------------------------ copies
+        // (a lane for every 16 tokens of a tile, the first of each block copies it)
+        const uint32_t per_block = block >> 4, bytes = block * dim;
+        uint32_t loads = 0, issued[2] = {0, 0};
+        pieces([&](const Piece& p) {
             const int32_t* const table = d.shared_table + static_cast<uint64_t>(p.m) * d.shared_width;
-            const uint32_t first = j * kTileTokens, h = p.segment / p.g.pairs;
-            uint32_t id[kEach];
+            const uint32_t h = p.segment / p.g.pairs;
+            auto there = [&](uint32_t j) { return lane < 8 && j * kTileTokens + lane * 16 < p.g.tokens; };
+            auto id_at = [&](uint32_t j) { return there(j) ? static_cast<uint32_t>(table[(j * kTileTokens + lane * 16) >> a.block_log2]) : kNoNode; };
+            uint32_t next = id_at(p.t);
+            for (uint32_t j = p.t; j < p.end; ++j, ++loads) {
+                const uint32_t id = next, stage = loads % kRaw<BOXES>;
+                if (j + 1 < p.end) next = id_at(j + 1);
+                const bool ok = id < a.c.num_blocks;
+                const uint32_t copies = __ballot_sync(kFull, ok && lane % per_block == 0), missing = __ballot_sync(kFull, there(j) && !ok);
+                if (missing && lane == 0) atomicOr(a.errors, kMemErrBlock);
+                const uint64_t slab = static_cast<uint64_t>(id) * hkv + h;
+                const float2 scale = ok ? make_float2(a.c.k_scale[slab], a.c.v_scale[slab]) : make_float2(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const uint32_t pos = first + row_of[i];
-                id[i] = i < static_cast<int>(nw) && (pos & ~15u) < p.g.tokens ? static_cast<uint32_t>(table[pos >> a.block_log2]) : kNoNode;
-            }
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const uint32_t pos = first + row_of[i];
-                place[i] = (((static_cast<uint64_t>(id[i]) * hkv + h) << a.block_log2) + (pos & (block - 1))) * nw + chunk_of[i];
-                if (id[i] >= a.c.num_blocks) {
-                    if (i < static_cast<int>(nw) && (pos & ~15u) < p.g.tokens) atomicOr(a.errors, kMemErrBlock);
-                    place[i] = kNothing;
+                for (int kv = 0; kv < 2; ++kv) {
+                    wait(&ctl.raw_empty[kv][stage], (loads / kRaw<BOXES> & 1) ^ 1);
+                    if (stopped()) return false;
+                    if (kv == 0) {
+                        if (lane < 8) ctl.scales[loads % kScales][lane] = scale;
+                        if (lane == 0) ctl.missing[loads % kScales] = missing;
+                        __syncwarp();
+                    }
+                    if (lane == 0) barrier_expect(&ctl.raw_full[kv][stage], __popc(copies) * bytes);
+                    __syncwarp();
+                    if (ok && lane % per_block == 0)
+                        copy_bulk(raw + (kv * kRaw<BOXES> + stage) * kRawBytes + lane * 16 * dim, (kv ? a.c.v : a.c.k) + slab * bytes, bytes, &ctl.raw_full[kv][stage]);
+                    ++issued[kv];
                 }
             }
-        };
-        auto load = [&](const int8_t* codes, const uint64_t (&place)[kEach], uint4 (&x)[kEach]) {
+            return true;
+        });
+        // no copy may be in flight when the block ends
+        if (lane == 0)
+            for (int kv = 0; kv < 2; ++kv)
+                for (uint32_t i = issued[kv] > kRaw<BOXES> ? issued[kv] - kRaw<BOXES> : 0; i < issued[kv]; ++i)
+                    for (unsigned x = 0; x < kPolls && !barrier_test(&ctl.raw_full[kv][i % kRaw<BOXES>], i / kRaw<BOXES> & 1); ++x) {}
+        __syncwarp();
+    } else if (warp >= 8) {
+        // --------------------------------------------------------- conversion
+        // (16 codes side by side to a lane, the next 16 to the next; of a row of
+        // 128, lanes of the upper half take their second eight first, so that
+        // the units that eight lanes store fall on all banks)
+        const uint32_t who = threadIdx.x - 256, nw = dim / 16;
+        constexpr int kWorkers = 32 * kConverters;
+        constexpr int kEach = (kRows * 4 * BOXES + kWorkers - 1) / kWorkers;     // 16 codes of a thread, of keys and of values
+        uint32_t from[kEach], to[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const uint32_t u = who + kWorkers * i, r = u / nw, x = u % nw, later = x >> 2;      // of 128 * nw
+            from[i] = u * 16 + later * 8;
+            to[i] = later * kBoxBytes + r * 128 + (((2 * (x & 3)) ^ (r & 7)) ^ later) * 16;
+        }
+        const uint32_t mine = kRows * nw > who ? (kRows * nw - who + kWorkers - 1) / kWorkers : 0;
+        uint32_t loads = 0;
+        // the next tile's codes of keys (kv 0) or values (1)
+        auto convert = [&](int kv) {
+            const uint32_t at = loads % kRaw<BOXES>, stage = loads % kStages;
+            const unsigned char* const codes = raw + (kv * kRaw<BOXES> + at) * kRawBytes;
+            unsigned char* const tile = (kv ? values : keys) + stage * kTileBytes;
+            wait(&ctl.raw_full[kv][at], loads / kRaw<BOXES> & 1);
+            wait(&ctl.empty[kv][stage], (loads / kStages & 1) ^ 1);
+            if (stopped()) return false;
+            const uint32_t missing = ctl.missing[loads % kScales];
+            uint2 x[kEach][2];
 #pragma unroll
             for (int i = 0; i < kEach; ++i)
-                x[i] = place[i] != kNothing ? reinterpret_cast<const uint4*>(codes)[place[i]] : make_uint4(0, 0, 0, 0);
-        };
-        uint32_t loads = 0;
-        auto leave = [&](const uint4 (&x)[kEach], bool is_v) {
-            const uint32_t stage = loads % kStages;
-            wait(&(is_v ? ctl.v_empty : ctl.k_empty)[stage], (loads / kStages & 1) ^ 1);
-            if (stopped()) return false;
-            unsigned char* const to = (is_v ? values : keys) + stage * kTileBytes;
+                if (i < static_cast<int>(mine)) {
+                    x[i][0] = *reinterpret_cast<const uint2*>(codes + from[i]);
+                    x[i][1] = *reinterpret_cast<const uint2*>(codes + (from[i] ^ 8));
+                }
+            if (missing) {
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                if (i >= static_cast<int>(nw)) break;
-                unsigned char* const row = to + (chunk_of[i] >> 2) * kBoxBytes + row_of[i] * 128;
-                const uint32_t unit = (chunk_of[i] & 3) * 2, r = row_of[i] & 7;
-                if (is_v) put_codes<__half>(row, unit, r, x[i]);
-                else put_codes<T>(row, unit, r, x[i]);
+                for (int i = 0; i < kEach; ++i)
+                    if (missing >> ((who + kWorkers * i) / nw / 16) & 1) x[i][0] = x[i][1] = make_uint2(0, 0);
             }
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                if (i < static_cast<int>(mine)) {
+                    *reinterpret_cast<uint4*>(tile + to[i]) = codes_to_halves(x[i][0]);
+                    *reinterpret_cast<uint4*>(tile + (to[i] ^ 16)) = codes_to_halves(x[i][1]);
+                }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
-            if (lane == 0) barrier_arrive(&(is_v ? ctl.v_full : ctl.k_full)[stage]);
+            if (lane == 0) {
+                barrier_arrive(&ctl.raw_empty[kv][at]);
+                barrier_arrive(&ctl.full[kv][stage]);
+            }
             return true;
         };
-        // each tile's codes are on their way while the one before is converted
-        Piece p = ctl.start;
-        bool more = true;
-        auto skip = [&]() {
-            while (more && p.t == p.end) more = next_piece(a, p);
-        };
-        skip();
-        uint32_t j = p.t;
-        uint64_t place[kEach];
-        uint4 k[kEach], v[kEach];
-        if (more) {
-            find(p, j, place);
-            load(a.c.k, place, k);
-            load(a.c.v, place, v);
-        }
-        while (more) {
-            if (++j == p.end) {
-                more = next_piece(a, p);
-                skip();
-                j = p.t;
-            }
-            if (more) find(p, j, place);
-            if (!leave(k, false)) break;
-            if (more) load(a.c.k, place, k);
-            if (!leave(v, true)) break;
-            if (more) load(a.c.v, place, v);
-            ++loads;
-        }
+        pieces([&](const Piece& p) {
+            for (uint32_t j = p.t; j < p.end; ++j, ++loads)
+                if (!convert(0) || !convert(1)) return false;
+            return true;
+        });
     } else {
         // ----------------------------------------------------------- softmax
         const uint32_t t = warp >> 2, row = threadIdx.x & 127;
@@ -518,68 +530,82 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         const uint32_t s_at = tmem + t * 128 + lanes, o_at = tmem + 256 + t * 128 + lanes;
         unsigned char* const tile = smem + t * kTileBytes;
         unsigned char* const staging = tile + (warp & 3) * 4096;       // the queries' place, once they are done with
-        const float score_scale = d.scale * 1.4426950408889634f;
-        const uint32_t per_tile = kTileTokens >> a.block_log2, e = lane & 7;
-        const bool has_scale = lane < 16 && e < per_tile;
-        uint32_t s_used = 0, o_used = 0;
+        uint32_t s_used = 0, o_used = 0, tiles = 0;
         pieces([&](const Piece& p) {
-            if (rows_left(p) <= t * kRows) return true;
+            if (rows_left(p) <= t * kRows) {
+                tiles += p.end - p.t;
+                return true;
+            }
             const uint32_t h = p.segment / p.g.pairs, r = p.segment % p.g.pairs * kPairRows + t * kRows + row;
             const bool real = r < p.g.rows;
             const uint32_t b = p.g.first + r / a.rows, i = r % a.rows / a.group, head = h * a.group + r % a.rows % a.group;
-            // this row's query
+            // this row's query, and the power of two that it was divided by
+            float row_scale = 1.f;
             {
                 const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(d.q) + b * d.q_stride[0] + i * d.q_stride[1] +
                                                                 head * d.q_stride[2]);
-#pragma unroll
-                for (int c0 = 0; c0 < 8 * BOXES; c0 += 8) {
-                    uint4 x[8];
+                auto units = [&](int c0, uint4 (&x)[8]) {
 #pragma unroll
                     for (int c = 0; c < 8; ++c) x[c] = real && c0 + c < static_cast<int>(dim / 8) ? q[c0 + c] : make_uint4(0, 0, 0, 0);
+                };
+                float up = 1.f;
+                if (d.dtype != BS_F16) {
+                    // times 2^e with the row's largest in [2^12, 2^13); rows of zeros, infinities and NaN as they are
+                    uint32_t high = 0;       // magnitudes of bf16 order as integers
+#pragma unroll 1
+                    for (int c0 = 0; c0 < 8 * BOXES; c0 += 8) {
+                        uint4 x[8];
+                        units(c0, x);
 #pragma unroll
-                    for (int c = 0; c < 8; ++c)
+                        for (int c = 0; c < 8; ++c)
+                            high = __vmaxu2(high, __vmaxu2(__vmaxu2(x[c].x & 0x7fff7fffu, x[c].y & 0x7fff7fffu), __vmaxu2(x[c].z & 0x7fff7fffu, x[c].w & 0x7fff7fffu)));
+                    }
+                    high = max(high >> 16, high & 0xffffu);
+                    uint32_t e = high >> 7;  // biased exponent
+                    e = high == 0 || e == 255 ? 139 : e < 13 ? 13 : e;
+                    up = __uint_as_float((266 - e) << 23);
+                    row_scale = __uint_as_float((e - 12) << 23);
+                }
+#pragma unroll 1
+                for (int c0 = 0; c0 < 8 * BOXES; c0 += 8) {
+                    uint4 x[8];
+                    units(c0, x);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        if (d.dtype != BS_F16) {
+                            uint32_t* const w = reinterpret_cast<uint32_t*>(&x[c]);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) w[k] = Type16<__half>::pack(__uint_as_float(w[k] << 16) * up, __uint_as_float(w[k] & 0xffff0000u) * up);
+                        }
                         *reinterpret_cast<uint4*>(tile + (c0 >> 3) * kBoxBytes + row * 128 + ((c ^ row) & 7) * 16) = x[c];
+                    }
                 }
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 __syncwarp();
                 if (lane == 0) barrier_arrive(&ctl.q_full[t]);
             }
-            const int32_t* const table = d.shared_table + static_cast<uint64_t>(p.m) * d.shared_width;
-            const uint32_t blocks = (p.g.tokens + block - 1) >> a.block_log2;
-            auto id_at = [&](uint32_t col) { return col < blocks ? static_cast<uint32_t>(table[col]) : 0u; };
             // the largest value scale of the piece
+            const int32_t* const table = d.shared_table + static_cast<uint64_t>(p.m) * d.shared_width;
+            const uint32_t past = min(p.end * kTileTokens, p.g.tokens);
             float unit = 0.f;
-            for (uint32_t col = p.t * per_tile + lane; col < min(p.end * per_tile, blocks); col += 32) {
+            for (uint32_t col = (p.t * kTileTokens >> a.block_log2) + lane; col << a.block_log2 < past; col += 32) {
                 const uint32_t id = table[col];
                 if (id < a.c.num_blocks) unit = fmaxf(unit, a.c.v_scale[static_cast<uint64_t>(id) * hkv + h]);
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) unit = fmaxf(unit, __shfl_xor_sync(kFull, unit, o));
             if (!(unit > 0.f)) unit = 1.f;
-            const float factor = lane < 8 ? score_scale : 1.f / unit;
-            auto scale_of = [&](uint32_t id, bool& missing) {          // of block e of a tile: lanes below 8 keys', the next 8 values'
-                missing = has_scale && id >= a.c.num_blocks;
-                if (!has_scale || missing) return 0.f;
-                return (lane < 8 ? a.c.k_scale : a.c.v_scale)[static_cast<uint64_t>(id) * hkv + h] * factor;
-            };
-            bool missing;
-            float next_scales = scale_of(id_at(p.t * per_tile + e), missing);
-            uint32_t next_bad = __ballot_sync(kFull, missing), next_id = id_at((p.t + 1) * per_tile + e);
+            const float k_by = d.scale * 1.4426950408889634f * row_scale, v_by = 1.f / unit;
             float top = -INFINITY, sum = 0.f;       // top: in log2 units, moved when weights are past 2^8
-            for (uint32_t j = p.t; j < p.end; ++j) {
-                const float scales = next_scales;
-                const uint32_t bad_blocks = next_bad & 255u;
-                if (j + 1 < p.end) {
-                    next_scales = scale_of(next_id, missing);
-                    next_bad = __ballot_sync(kFull, missing);
-                    next_id = id_at((j + 2) * per_tile + e);
-                }
+            for (uint32_t j = p.t; j < p.end; ++j, ++tiles) {
                 wait(&ctl.s_full[t], s_used++ & 1);        // and the value product before it is done
                 if (stopped()) return false;
                 fence_after();
                 const uint32_t left = p.g.tokens - j * kTileTokens;
                 int done = 0;           // quarters of the tile whose weights are made
-                if (j > p.t && left >= kTileTokens && !bad_blocks) {
+                const float2* const scales = ctl.scales[tiles % kScales];
+                const uint32_t missing = ctl.missing[tiles % kScales];
+                if (j > p.t && left >= kTileTokens && !missing) {
                     float s[2][32];
                     tmem_load32(s_at, s[0]);
 #pragma unroll
@@ -588,8 +614,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                         if (c < 3) tmem_load32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
                         uint32_t w16[16];
                         float part;
-                        weights32(s[c & 1], scales, 32 * c, a.block_log2, kLift - top, w16, part);
-                        if (__any_sync(kFull, real && part > kMost)) break;       // (rows that are none hold zeros)
+                        weights32(s[c & 1], scales + 2 * c, k_by, v_by, kLift - top, w16, part);
+                        if (__any_sync(kFull, real && part > kMost)) break;       // (rows that are none hold anything)
                         sum += part;
                         tmem_store16(s_at + 16 * c, w16);
                         done = c + 1;
@@ -600,11 +626,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                     }
                 }
                 if (done < 4) {
-                    uint32_t bad = 0;       // by 16 columns
-                    for (uint32_t x = 0; bad_blocks && x < 8; ++x) bad |= (bad_blocks >> ((16 * x) >> a.block_log2) & 1) << x;
                     const int quarters = (static_cast<int>(columns(p, j)) + 31) / 32;
-                    const float2 state = weights_with_care(s_at, o_at, done, quarters, left < kTileTokens ? left : kTileTokens, bad, real, scales,
-                                                           a.block_log2, j > p.t ? dim : 0, make_float2(top, sum));
+                    const float2 state = weights_with_care(s_at, o_at, done, quarters, left < kTileTokens ? left : kTileTokens, missing, scales, k_by,
+                                                           v_by, j > p.t ? dim : 0, make_float2(top, sum));
                     top = state.x;
                     sum = state.y;
                 }
@@ -642,11 +666,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
     if (warp == kIssuer) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
 }
 
-template <typename T, int BOXES>
+template <int BOXES>
 cudaError_t launch(const SharedArgs& a, cudaStream_t stream) {
-    const cudaError_t e = cudaFuncSetAttribute(k_shared<T, BOXES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<BOXES>);
+    const cudaError_t e = cudaFuncSetAttribute(k_shared<BOXES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<BOXES>);
     if (e != cudaSuccess) return e;
-    return launch_after(k_shared<T, BOXES>, dim3(a.shares), kThreads, kSmem<BOXES>, stream, a);
+    return launch_after(k_shared<BOXES>, dim3(a.shares), kThreads, kSmem<BOXES>, stream, a);
 }
 
 }  // namespace
@@ -654,8 +678,7 @@ cudaError_t launch(const SharedArgs& a, cudaStream_t stream) {
 cudaError_t launch_shared_part(const SharedArgs& given, cudaStream_t stream) {
     SharedArgs a = given;
     a.polls = wait_polls();
-    if (a.d.dtype == BS_F16) return a.c.dim <= 64 ? launch<__half, 1>(a, stream) : launch<__half, 2>(a, stream);
-    return a.c.dim <= 64 ? launch<__nv_bfloat16, 1>(a, stream) : launch<__nv_bfloat16, 2>(a, stream);
+    return a.c.dim <= 64 ? launch<1>(a, stream) : launch<2>(a, stream);
 }
 
 }  // namespace bsb
