@@ -25,6 +25,7 @@ namespace bsb {
 
 using namespace dev;
 using namespace tile;
+using shared::FarRow;
 using shared::Group;
 using shared::SharedArgs;
 namespace cg = cooperative_groups;
@@ -54,12 +55,6 @@ constexpr int kJoinOrIds = kJoinBytes<NW, NT> > kIdBytes ? kJoinBytes<NW, NT> : 
 template <int NW, int NT>
 constexpr size_t kRowsSmem = kWarps * kStagesOf<NT> * kListStage<NW> + (kWarps + 1) * 8 * NT * 2 * 4 + kJoinOrIds<NW, NT>;
 
-// Where a row's outputs over the shared tokens are: `pieces` of them, by row of
-// the outputs if there is one, else from slot `first` of the share on.
-struct FarRow {
-    uint32_t pieces, share, slot, row;
-};
-
 __device__ __forceinline__ uint32_t tokens_of(const SharedArgs& a, const int32_t* lens, uint32_t i, uint32_t width) {
     const int32_t len = lens[i];
     const int64_t most = static_cast<int64_t>(width) * a.c.block;
@@ -79,63 +74,34 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
     int2* const ids = reinterpret_cast<int2*>(join_o);          // block, first position; till the outputs are joined
     uint32_t* const found = reinterpret_cast<uint32_t*>(ids + kMostIds);      // [warps]
 
-    cudaGridDependencySynchronize();       // in every block, before anything of the caller's
+    const SharedArgs& a = given.s;
+    // In every block, before anything of the caller's.  (After the shared tokens'
+    // kernel this one waits where it needs that one's outputs: that kernel has
+    // waited for what came before, in all its blocks, before this one starts.)
+    if (LIST || !a.shares) cudaGridDependencySynchronize();
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = cluster.block_rank(), parts = cluster.num_blocks();
-    const SharedArgs& a = given.s;
     const bs_shared_attention_desc& d = a.d;
     const uint32_t hkv = a.c.kv_heads, b = blockIdx.z, segment = blockIdx.x / parts, row0 = blockIdx.y * kRows;
     const uint32_t h = LIST ? segment % hkv : segment, query = LIST ? segment / hkv : 0, block = a.c.block;
     const uint32_t len = tokens_of(a, d.lens, b, d.table_width);
 
-    // what the sequence shares: its group's place among the shares of that work
-    FarRow* const far_rows = reinterpret_cast<FarRow*>(smem);   // (over the ring, once that is done with)
-    Group shares_with{};
-    uint64_t units_before = 0, units = 0;
-    if (!LIST && a.shares) {
-        uint32_t m = 0;
-        for (uint32_t past = d.num_groups; past - m > 1;) {    // the last group that begins at b or before
-            const uint32_t mid = (m + past) / 2;
-            (d.cu[mid] <= static_cast<int32_t>(b) ? m : past) = mid;
-        }
-        shares_with = shared::group_of(a, m);
-        if (b < shares_with.first || static_cast<int32_t>(b) >= d.cu[m + 1]) shares_with.tiles = 0;
-        shared::count_cost(a, m, units_before, units, reinterpret_cast<uint64_t*>(smem));
-    }
-    if (!LIST && blockIdx.x == 0 && blockIdx.y == 0 && b == 0)
-        for (uint32_t i = threadIdx.x; i <= d.num_groups; i += kThreads) {
-            const int32_t x = d.cu[i];
-            if (i == 0 ? x != 0 : x < d.cu[i - 1] || (i == d.num_groups && static_cast<uint32_t>(x) != d.num_seqs))
-                atomicOr(a.errors, kMemErrLength);
-        }
-    auto far_of = [&](uint32_t r) {
-        FarRow far{};
-        if (shares_with.tiles == 0) return far;
-        const uint32_t in_group = (b - shares_with.first) * a.rows + r, pair = in_group / shared::kPairRows;
-        const uint64_t w = units * hkv;
-        const uint64_t s0 = units_before * hkv + (static_cast<uint64_t>(h) * shares_with.pairs + pair) * (shares_with.tiles + shared::kStart);
-        const uint32_t n = shared::used_shares(w, a.shares);
-        far.share = shared::share_of(w, n, s0 + shared::kStart);
-        far.pieces = shared::share_of(w, n, s0 + shared::kStart + shares_with.tiles - 1) - far.share + 1;
-        far.slot = shared::share_first(w, n, far.share) >= s0 ? 0 : 1;       // later shares begin inside the segment
-        far.row = in_group % shared::kPairRows;
-        return far;
-    };
-
     // this segment's query rows as the columns of K Q^T: column j is row row0 + j
     uint32_t q[NT][NW][2];
     float row_scale[NT][2];          // of columns 2c and 2c + 1
-    int32_t limit[NT][2];        // tokens of its own that row sees
+    int32_t limit[NT][2];            // tokens of its own that row sees
+    auto load_queries = [&]() {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const uint32_t r = row0 + 8 * nt + g, col = row0 + 8 * nt + 2 * c;
-        const uint16_t* row = static_cast<const uint16_t*>(d.q) + b * d.q_stride[0] + static_cast<int64_t>(LIST ? query : r / a.group) * d.q_stride[1] +
-                              (static_cast<int64_t>(h) * a.group + r % a.group) * d.q_stride[2] + c * (NW * 4);
-        load_query_row<NW>(q[nt], row_scale[nt], row, r < given.rows, d.dtype != BS_F16, d.scale * 1.4426950408889634f, c);
+        for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t r = row0 + 8 * nt + g, col = row0 + 8 * nt + 2 * c;
+            const uint16_t* row = static_cast<const uint16_t*>(d.q) + b * d.q_stride[0] + static_cast<int64_t>(LIST ? query : r / a.group) * d.q_stride[1] +
+                                  (static_cast<int64_t>(h) * a.group + r % a.group) * d.q_stride[2] + c * (NW * 4);
+            load_query_row<NW>(q[nt], row_scale[nt], row, r < given.rows, d.dtype != BS_F16, d.scale * 1.4426950408889634f, c);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            limit[nt][i] = static_cast<int32_t>(len) - d.queries + 1 + static_cast<int32_t>(LIST ? query : (col + i) / a.group);
-    }
+            for (int i = 0; i < 2; ++i)
+                limit[nt][i] = static_cast<int32_t>(len) - d.queries + 1 + static_cast<int32_t>(LIST ? query : (col + i) / a.group);
+        }
+    };
     float o[NT][NW][4];
     float top[NT][2], sum[NT][2], unit = kFold / -kNoScore, inv_unit = -kNoScore;
 #pragma unroll
@@ -154,7 +120,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
     const uint32_t entries = LIST ? given.count : (tokens + block - 1) / block;
     // this block's part of the entries
     const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(entries) * (rank + 1) / parts);
-    for (uint32_t from = static_cast<uint32_t>(static_cast<uint64_t>(entries) * rank / parts); from < end; from += kMostIds) {
+    const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(entries) * rank / parts);
+    for (uint32_t from = begin; from < end; from += kMostIds) {
         // look them up; those without a token that is seen are left out
         uint32_t held = 0;
 #pragma unroll
@@ -219,6 +186,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
         };
 #pragma unroll
         for (int i = 0; i < kStages - 1; ++i) request(warp + i * kWarps, i);
+        if (from == begin) load_queries();             // (under the first copies)
         uint32_t stage = 0, fill = kStages - 1;
         for (uint32_t t = warp; t < tiles; t += kWarps) {
             asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
@@ -294,7 +262,26 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
                 for (int j = 0; j < NW; ++j)
                     *reinterpret_cast<float2*>(part_o + r * kDim + value_dim<NW>(j, g)) = make_float2(o[nt][j][i], o[nt][j][2 + i]);
             }
-    if (!LIST && threadIdx.x < kRows && row0 + threadIdx.x < given.rows) far_rows[threadIdx.x] = far_of(row0 + threadIdx.x);
+    // and those over the shared tokens: where the row's pair of tiles is (bs_shared.cuh)
+    FarRow* const far_rows = reinterpret_cast<FarRow*>(smem);  // (over the ring)
+    if (!LIST && a.shares) {
+        uint32_t m = 0;
+        for (uint32_t past = d.num_groups; past - m > 1;) {    // the last group that begins at b or before
+            const uint32_t mid = (m + past) / 2;
+            (d.cu[mid] <= static_cast<int32_t>(b) ? m : past) = mid;
+        }
+        const Group group = shared::group_of(a, m);
+        const bool shares = group.tiles && b >= group.first && static_cast<int32_t>(b) < d.cu[m + 1];
+        cudaGridDependencySynchronize();
+        if (threadIdx.x < kRows && row0 + threadIdx.x < given.rows)
+            far_rows[threadIdx.x] = shares ? shared::far_row(a, group, b, h, row0 + threadIdx.x) : FarRow{};
+    }
+    if (!LIST && blockIdx.x == 0 && blockIdx.y == 0 && b == 0)
+        for (uint32_t i = threadIdx.x; i <= d.num_groups; i += kThreads) {
+            const int32_t x = d.cu[i];
+            if (i == 0 ? x != 0 : x < d.cu[i - 1] || (i == d.num_groups && static_cast<uint32_t>(x) != d.num_seqs))
+                atomicOr(a.errors, kMemErrLength);
+        }
     if (parts > 1) cluster.sync();
     else __syncthreads();
     for (uint32_t x = rank * kThreads + threadIdx.x; x < kRows * kDim / 4; x += parts * kThreads) {
@@ -317,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
             acc.x += y.x * w, acc.y += y.y * w, acc.z += y.z * w, acc.w += y.w * w;
         }
         const uint64_t row = row_at(row0 + r);
-        const FarRow far = LIST ? FarRow{} : far_rows[r];
+        const FarRow far = LIST || !a.shares ? FarRow{} : far_rows[r];
         for (uint32_t p0 = 0; p0 < far.pieces; p0 += kBatch) {
             float2 far_ml[kBatch];
             float4 y[kBatch];
@@ -365,7 +352,7 @@ uint32_t parts_of(uint64_t segments, uint64_t tokens, uint64_t resident) {
     constexpr double kStart = 6, kJoin = 2;
     uint32_t best = 1;
     double least = 0;
-    for (uint32_t n = 1; n <= kMostCluster; n *= 2) {
+    for (uint32_t n = 1; n <= kMostCluster; ++n) {
         const double waves = static_cast<double>((segments * n + resident - 1) / resident);
         const double time = waves * (kStart + static_cast<double>(tokens) / kTile / n) + (n > 1 ? kJoin : 0);
         if (n == 1 || time < least) {
@@ -418,7 +405,7 @@ uint32_t log2_of(int32_t block) { return block == 16 ? 4 : block == 32 ? 5 : blo
 
 struct Layout {
     uint32_t shares;
-    size_t whole_ml, whole_o, part_ml, part_o, total;
+    size_t far, whole_ml, whole_o, part_ml, part_o, total;
 };
 
 Layout plan(const bs_token_cache& c, const bs_shared_attention_desc& d, const MemoryDevice& dev) {
@@ -436,6 +423,7 @@ Layout plan(const bs_token_cache& c, const bs_shared_attention_desc& d, const Me
         return at;
     };
     const size_t slots = static_cast<size_t>(l.shares) * 2 * shared::kPairRows;
+    l.far = take(rows * sizeof(FarRow));
     l.whole_ml = take(rows * 8);
     l.whole_o = take(rows * c.dim * 4);
     l.part_ml = take(slots * 8);
@@ -480,6 +468,7 @@ cudaError_t launch_shared_attention(const bs_token_cache& c, const bs_shared_att
     a.s.c = c;
     a.s.d = d;
     a.s.errors = dev.errors;
+    a.s.far = reinterpret_cast<FarRow*>(work + l.far);
     a.s.whole_ml = reinterpret_cast<float2*>(work + l.whole_ml);
     a.s.whole_o = reinterpret_cast<float*>(work + l.whole_o);
     a.s.part_ml = reinterpret_cast<float2*>(work + l.part_ml);

@@ -24,10 +24,17 @@ constexpr uint32_t kPairRows = 256;
 // products, its outputs.
 constexpr uint32_t kStart = 2;
 
+// Where the outputs of a segment's rows are: by row of the outputs if there is
+// one piece, else from slot `slot` of the share on (row `row` there).
+struct FarRow {
+    uint32_t pieces, share, slot, row;
+};
+
 struct SharedArgs {
     bs_token_cache c;
     bs_shared_attention_desc d;
     unsigned int* errors;
+    FarRow* far;           // [rows of the outputs]: at a segment's first row, what the segment's rows have in common
     float* whole_o;        // [rows of the outputs][dim]
     float2* whole_ml;      // [rows of the outputs]: maximum (log2), sum
     float* part_o;         // [shares][2][256][dim]
@@ -106,6 +113,22 @@ __device__ __forceinline__ void count_cost(const SharedArgs& a, uint32_t m, uint
         all += sums[warps + i];
     }
     __syncthreads();
+}
+
+// Row of the outputs of a group's row r (of key head h).
+__device__ __forceinline__ uint64_t output_row(const SharedArgs& a, const Group& g, uint32_t h, uint32_t r) {
+    const uint32_t b = g.first + r / a.rows, i = r % a.rows / a.group, head = h * a.group + r % a.rows % a.group;
+    return (static_cast<uint64_t>(b) * a.d.queries + i) * a.d.q_heads + head;
+}
+
+// Of sequence b's row r of key head h, b one of group g.
+__device__ __forceinline__ FarRow far_row(const SharedArgs& a, const Group& g, uint32_t b, uint32_t h, uint32_t r) {
+    const uint32_t in_group = (b - g.first) * a.rows + r;
+    FarRow f = a.far[output_row(a, g, h, in_group / kPairRows * kPairRows)];
+    f.row = in_group % kPairRows;
+    // (anything may be there after a wait that gave up)
+    if (f.share >= a.shares || f.pieces > a.shares - f.share || f.slot > 1) f.pieces = 0;
+    return f;
 }
 
 }  // namespace shared

@@ -45,18 +45,23 @@ constexpr int kConverters = 6;         // warps
 constexpr int kIssuer = 8 + kConverters;
 constexpr int kCopier = kIssuer + 1;
 constexpr int kThreads = 32 * (kCopier + 1);
-constexpr int kStages = 2;             // of converted keys, and of values
-// Stages of codes: with rows of 128 dimensions one of each fits beside the others.
+// Rings of converted tiles and of their codes, keys and values in turn: with
+// rows of 128 dimensions no more fit.  (Three converted ones do: a tile's values
+// and the next one's keys are in use together, meanwhile the next values are
+// converted.  With two of each converted and one of each of codes, a copy's 1.2 us
+// came after each conversion, 5,500 clocks a tile.)
 template <int BOXES>
-constexpr int kRaw = BOXES == 2 ? 1 : 4;
+constexpr int kStages = BOXES == 2 ? 3 : 4;
+template <int BOXES>
+constexpr int kRaw = BOXES == 2 ? 4 : 8;
 constexpr float kLift = 5.f;
 constexpr float kMost = 32768.f;       // of a sum of 32 lifted weights, and so of each: below f16's 65504
-// Tiles whose scales are in shared memory: the copies of a tile wait for the
-// conversion of the one kRaw before it, that for products with keys kStages
-// earlier, issued when the weights of the tile before are made: a tile's scales
-// are read no more when those of the one kRaw + kStages + 1 after it are written.
+// Tiles whose scales are in shared memory.  Those of tile n are written when the
+// codes of tile n - kRaw / 2 have been converted, into the place of something that
+// was multiplied kStages conversions before; the scores of the tile after that one
+// are issued when its weights are made, and its scales read no more.
 constexpr int kScales = 8;
-static_assert(kRaw<1> + kStages + 1 <= kScales && kRaw<2> + kStages + 1 <= kScales, "scales are overwritten while they are read");
+static_assert(kRaw<1> / 2 + kStages<1> / 2 + 1 <= kScales && kRaw<2> / 2 + kStages<2> / 2 + 1 <= kScales, "scales are overwritten while they are read");
 
 // Eight codes in f16: 0x6400 | u is 1024 + u, minus 1152.
 __device__ __forceinline__ uint4 codes_to_halves(uint2 x) {
@@ -87,14 +92,14 @@ struct Piece {
     uint32_t m, segment;       // segment: h * pairs + pair
     uint32_t t, end;
     uint64_t left;             // units of the share after this piece
+    uint64_t at, begin;        // units: of the piece's end, of the segment's begin
     Group g;
     uint32_t slot;             // 0: the share's first piece
 };
 
 struct Control {
     uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
-    uint64_t full[2][kStages], empty[2][kStages];        // [keys, values]
-    uint64_t raw_full[2][4], raw_empty[2][4];
+    uint64_t full[4], empty[4], raw_full[8], raw_empty[8];
     uint64_t sums[2 * (kCopier + 1)];
     uint32_t missing[kScales];          // by tile: bits of 16 tokens whose block is not there
     __align__(16) float2 scales[kScales][8];      // by tile and 16 tokens: of keys, of values
@@ -104,7 +109,7 @@ struct Control {
 };
 
 template <int BOXES>
-constexpr size_t kSmem = 1024 + (2 + 2 * kStages + kRaw<BOXES>) * BOXES * kBoxBytes + sizeof(Control);
+constexpr size_t kSmem = 1024 + (2 + kStages<BOXES>) * BOXES * kBoxBytes + kRaw<BOXES> * (BOXES * kBoxBytes / 2) + sizeof(Control);
 
 // The piece of a segment from its unit `from` on; its first kStart units
 // stand for no tiles.
@@ -113,6 +118,8 @@ __device__ __forceinline__ void cut_piece(Piece& p, uint32_t from) {
     p.t = from > kStart ? from - kStart : 0;
     p.end = from + take > kStart ? from + take - kStart : 0;
     p.left -= take;
+    p.begin = p.at - from;
+    p.at += take;
 }
 
 // To the next piece; false: there is none.
@@ -162,6 +169,7 @@ __device__ __forceinline__ void find_piece(const SharedArgs& a, Piece& p, uint64
     const uint32_t cost = p.g.tiles + kStart;
     p.segment = static_cast<uint32_t>((first - seen) / cost);
     p.slot = 0;
+    p.at = first;
     cut_piece(p, static_cast<uint32_t>((first - seen) % cost));
 }
 
@@ -270,16 +278,16 @@ template <int BOXES>
 __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ SharedArgs a) {
     extern __shared__ unsigned char raw_smem[];
     unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t{1023});
-    constexpr int kTileBytes = BOXES * kBoxBytes;
-    unsigned char* const keys = smem + 2 * kTileBytes;
-    unsigned char* const values = keys + kStages * kTileBytes;
-    unsigned char* const raw = values + kStages * kTileBytes;         // codes of keys, then of values
-    constexpr int kRawBytes = kTileBytes / 2;
-    Control& ctl = *reinterpret_cast<Control*>(raw + 2 * kRaw<BOXES> * kRawBytes);
+    constexpr int kTileBytes = BOXES * kBoxBytes, kRawBytes = kTileBytes / 2;
+    constexpr uint32_t kRing = kStages<BOXES>, kRawRing = kRaw<BOXES>;
+    unsigned char* const ring = smem + 2 * kTileBytes;
+    unsigned char* const raw = ring + kRing * kTileBytes;             // codes
+    Control& ctl = *reinterpret_cast<Control*>(raw + kRawRing * kRawBytes);
     const bs_shared_attention_desc& d = a.d;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hkv = a.c.kv_heads, dim = a.c.dim, block = a.c.block;
 
     cudaGridDependencySynchronize();       // in every block, before anything of the caller's
+    cudaTriggerProgrammaticLaunchCompletion();       // the kernel after this one begins with what does not need it
     uint64_t before, all;
     count_cost(a, 0, before, all, ctl.sums);
     const uint64_t w = all * hkv;
@@ -299,15 +307,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                 barrier_init(&ctl.o_full[t], 1);
             }
             barrier_init(&ctl.done, 1);
-            for (int kv = 0; kv < 2; ++kv) {
-                for (int s = 0; s < kStages; ++s) {
-                    barrier_init(&ctl.full[kv][s], kConverters);
-                    barrier_init(&ctl.empty[kv][s], 1);
-                }
-                for (int s = 0; s < kRaw<BOXES>; ++s) {
-                    barrier_init(&ctl.raw_full[kv][s], 1);
-                    barrier_init(&ctl.raw_empty[kv][s], kConverters);
-                }
+            for (uint32_t s = 0; s < kRing; ++s) {
+                barrier_init(&ctl.full[s], kConverters);
+                barrier_init(&ctl.empty[s], 1);
+            }
+            for (uint32_t s = 0; s < kRawRing; ++s) {
+                barrier_init(&ctl.raw_full[s], 1);
+                barrier_init(&ctl.raw_empty[s], kConverters);
             }
             ctl.gave_up = 0;
             asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -355,8 +361,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         constexpr uint32_t kCommon = 1u << 4 | static_cast<uint32_t>(kRows >> 4) << 24;
         const uint32_t what_o = kCommon | 1u << 16 | (dim >> 3) << 17;         // (values do not lie along the contraction)
         const int steps = dim / 16;
-        const uint64_t q_base = operand(smem_addr(smem), 16, 1024), k_base = operand(smem_addr(keys), 16, 1024);
-        const uint64_t v_base = operand(smem_addr(values), kBoxBytes, 1024);
+        const uint64_t q_base = operand(smem_addr(smem), 16, 1024), k_base = operand(smem_addr(ring), 16, 1024);
+        const uint64_t v_base = operand(smem_addr(ring), kBoxBytes, 1024);
         constexpr uint32_t kTileUnits = kTileBytes / 16, kBoxUnits = kBoxBytes / 16;
         auto scores = [&](int t, uint32_t stage, uint32_t cols) {
             const uint64_t q = q_base + t * kTileUnits, k = k_base + stage * kTileUnits;
@@ -376,25 +382,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                 mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + i * 8, v + i * 128, what_o, add || i > 0);
             }
         };
-        uint32_t loads = 0, q_used[2] = {0, 0}, p_used[2] = {0, 0};
+        uint32_t tiles = 0, q_used[2] = {0, 0}, p_used[2] = {0, 0};      // tile i's keys are the ring's 2 i, its values 2 i + 1
         bool issued = false;
+        auto full = [&](uint32_t i) { wait(&ctl.full[i % kRing], i / kRing & 1); };
         pieces([&](const Piece& p) {
             const bool both = rows_left(p) > kRows;
-            wait(&ctl.full[0][loads % kStages], loads / kStages & 1);
+            full(2 * tiles);
             for (int t = 0; t <= both; ++t) wait(&ctl.q_full[t], q_used[t]++ & 1);
             if (stopped()) return false;
             issued = true;
             fence_after();
             if (elected()) {
-                for (int t = 0; t <= both; ++t) scores(t, loads % kStages, columns(p, p.t));
-                mma_commit(&ctl.empty[0][loads % kStages]);
+                for (int t = 0; t <= both; ++t) scores(t, 2 * tiles % kRing, columns(p, p.t));
+                mma_commit(&ctl.empty[2 * tiles % kRing]);
             }
             __syncwarp();
-            for (uint32_t j = p.t; j < p.end; ++j, ++loads) {
-                const uint32_t stage = loads % kStages, next = (loads + 1) % kStages;
+            for (uint32_t j = p.t; j < p.end; ++j, ++tiles) {
+                const uint32_t stage = (2 * tiles + 1) % kRing, next = (2 * tiles + 2) % kRing;
                 const bool last = j + 1 == p.end;
-                wait(&ctl.full[1][stage], loads / kStages & 1);
-                if (!last) wait(&ctl.full[0][next], (loads + 1) / kStages & 1);
+                full(2 * tiles + 1);
+                if (!last) full(2 * tiles + 2);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     if (t && !both) break;
@@ -409,8 +416,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                     __syncwarp();
                 }
                 if (elected()) {
-                    mma_commit(&ctl.empty[1][stage]);
-                    if (!last) mma_commit(&ctl.empty[0][next]);
+                    mma_commit(&ctl.empty[stage]);
+                    if (!last) mma_commit(&ctl.empty[next]);
                 }
                 __syncwarp();
             }
@@ -427,15 +434,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         // ------------------------------------------------------------ copies
         // (a lane for every 16 tokens of a tile, the first of each block copies it)
         const uint32_t per_block = block >> 4, bytes = block * dim;
-        uint32_t loads = 0, issued[2] = {0, 0};
+        uint32_t tiles = 0, loads = 0;
         pieces([&](const Piece& p) {
             const int32_t* const table = d.shared_table + static_cast<uint64_t>(p.m) * d.shared_width;
             const uint32_t h = p.segment / p.g.pairs;
             auto there = [&](uint32_t j) { return lane < 8 && j * kTileTokens + lane * 16 < p.g.tokens; };
             auto id_at = [&](uint32_t j) { return there(j) ? static_cast<uint32_t>(table[(j * kTileTokens + lane * 16) >> a.block_log2]) : kNoNode; };
             uint32_t next = id_at(p.t);
-            for (uint32_t j = p.t; j < p.end; ++j, ++loads) {
-                const uint32_t id = next, stage = loads % kRaw<BOXES>;
+            for (uint32_t j = p.t; j < p.end; ++j, ++tiles) {
+                const uint32_t id = next;
                 if (j + 1 < p.end) next = id_at(j + 1);
                 const bool ok = id < a.c.num_blocks;
                 const uint32_t copies = __ballot_sync(kFull, ok && lane % per_block == 0), missing = __ballot_sync(kFull, there(j) && !ok);
@@ -444,27 +451,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                 const float2 scale = ok ? make_float2(a.c.k_scale[slab], a.c.v_scale[slab]) : make_float2(0.f, 0.f);
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv) {
-                    wait(&ctl.raw_empty[kv][stage], (loads / kRaw<BOXES> & 1) ^ 1);
+                    const uint32_t stage = loads % kRawRing;
+                    wait(&ctl.raw_empty[stage], (loads / kRawRing & 1) ^ 1);
                     if (stopped()) return false;
                     if (kv == 0) {
-                        if (lane < 8) ctl.scales[loads % kScales][lane] = scale;
-                        if (lane == 0) ctl.missing[loads % kScales] = missing;
+                        if (lane < 8) ctl.scales[tiles % kScales][lane] = scale;
+                        if (lane == 0) ctl.missing[tiles % kScales] = missing;
                         __syncwarp();
                     }
-                    if (lane == 0) barrier_expect(&ctl.raw_full[kv][stage], __popc(copies) * bytes);
+                    if (lane == 0) barrier_expect(&ctl.raw_full[stage], __popc(copies) * bytes);
                     __syncwarp();
                     if (ok && lane % per_block == 0)
-                        copy_bulk(raw + (kv * kRaw<BOXES> + stage) * kRawBytes + lane * 16 * dim, (kv ? a.c.v : a.c.k) + slab * bytes, bytes, &ctl.raw_full[kv][stage]);
-                    ++issued[kv];
+                        copy_bulk(raw + stage * kRawBytes + lane * 16 * dim, (kv ? a.c.v : a.c.k) + slab * bytes, bytes, &ctl.raw_full[stage]);
+                    ++loads;
                 }
             }
             return true;
         });
         // no copy may be in flight when the block ends
         if (lane == 0)
-            for (int kv = 0; kv < 2; ++kv)
-                for (uint32_t i = issued[kv] > kRaw<BOXES> ? issued[kv] - kRaw<BOXES> : 0; i < issued[kv]; ++i)
-                    for (unsigned x = 0; x < kPolls && !barrier_test(&ctl.raw_full[kv][i % kRaw<BOXES>], i / kRaw<BOXES> & 1); ++x) {}
+            for (uint32_t i = loads > kRawRing ? loads - kRawRing : 0; i < loads; ++i)
+                for (unsigned x = 0; x < kPolls && !barrier_test(&ctl.raw_full[i % kRawRing], i / kRawRing & 1); ++x) {}
         __syncwarp();
     } else if (warp >= 8) {
         // --------------------------------------------------------- conversion
@@ -482,16 +489,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
             to[i] = later * kBoxBytes + r * 128 + (((2 * (x & 3)) ^ (r & 7)) ^ later) * 16;
         }
         const uint32_t mine = kRows * nw > who ? (kRows * nw - who + kWorkers - 1) / kWorkers : 0;
-        uint32_t loads = 0;
+        uint32_t tiles = 0;
         // the next tile's codes of keys (kv 0) or values (1)
         auto convert = [&](int kv) {
-            const uint32_t at = loads % kRaw<BOXES>, stage = loads % kStages;
-            const unsigned char* const codes = raw + (kv * kRaw<BOXES> + at) * kRawBytes;
-            unsigned char* const tile = (kv ? values : keys) + stage * kTileBytes;
-            wait(&ctl.raw_full[kv][at], loads / kRaw<BOXES> & 1);
-            wait(&ctl.empty[kv][stage], (loads / kStages & 1) ^ 1);
+            const uint32_t load = 2 * tiles + kv, at = load % kRawRing, stage = load % kRing;
+            const unsigned char* const codes = raw + at * kRawBytes;
+            unsigned char* const tile = ring + stage * kTileBytes;
+            wait(&ctl.raw_full[at], load / kRawRing & 1);
+            wait(&ctl.empty[stage], (load / kRing & 1) ^ 1);
             if (stopped()) return false;
-            const uint32_t missing = ctl.missing[loads % kScales];
+            const uint32_t missing = ctl.missing[tiles % kScales];
             uint2 x[kEach][2];
 #pragma unroll
             for (int i = 0; i < kEach; ++i)
@@ -513,13 +520,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-                barrier_arrive(&ctl.raw_empty[kv][at]);
-                barrier_arrive(&ctl.full[kv][stage]);
+                barrier_arrive(&ctl.raw_empty[at]);
+                barrier_arrive(&ctl.full[stage]);
             }
             return true;
         };
         pieces([&](const Piece& p) {
-            for (uint32_t j = p.t; j < p.end; ++j, ++loads)
+            for (uint32_t j = p.t; j < p.end; ++j, ++tiles)
                 if (!convert(0) || !convert(1)) return false;
             return true;
         });
@@ -532,6 +539,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         unsigned char* const staging = tile + (warp & 3) * 4096;       // the queries' place, once they are done with
         uint32_t s_used = 0, o_used = 0, tiles = 0;
         pieces([&](const Piece& p) {
+            if (p.t == 0 && threadIdx.x == 0) {        // where the segment's pieces are
+                const uint32_t last = share_of(w, n, p.begin + kStart + p.g.tiles - 1);
+                a.far[output_row(a, p.g, p.segment / p.g.pairs, p.segment % p.g.pairs * kPairRows)] =
+                    FarRow{last - blockIdx.x + 1, blockIdx.x, p.slot, 0};
+            }
             if (rows_left(p) <= t * kRows) {
                 tiles += p.end - p.t;
                 return true;
