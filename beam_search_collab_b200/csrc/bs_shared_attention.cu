@@ -12,11 +12,10 @@
 // Every row sees every token, but for the end of the last tile.
 //
 // Warps 0-3 and 4-7 are the softmax of tile 0 and 1 (a thread has one row),
-// 8-13 convert keys and values, 14 issues the matrix instructions, 15 copies
-// codes (a bulk copy for each block) and scales to shared memory:
-//   S_t = Q_t K^T     codes of K exact in f16, as are bf16 queries times a power
-//                     of two of each row's own (elements below 2^-29 of the
-//                     row's largest lose bits)
+// 8-13 convert keys and values, 14 issues the matrix instructions, 15 finds the
+// pieces of the share and copies codes (a bulk copy for each block) and scales to
+// shared memory:
+//   S_t = Q_t K^T     codes of K exact in the queries' 16-bit type
 //   O_t += P_t V      codes of V exact in f16, P_t f16: a weight times its values'
 //                     scale, over the largest of the piece, rounded to 2^-11 of
 //                     itself or, where that is more, 2^-29 of a weight of 1 at
@@ -63,8 +62,12 @@ constexpr float kMost = 32768.f;       // of a sum of 32 lifted weights, and so 
 constexpr int kScales = 8;
 static_assert(kRaw<1> / 2 + kStages<1> / 2 + 1 <= kScales && kRaw<2> / 2 + kStages<2> / 2 + 1 <= kScales, "scales are overwritten while they are read");
 
-// Eight codes in f16: 0x6400 | u is 1024 + u, minus 1152.
-__device__ __forceinline__ uint4 codes_to_halves(uint2 x) {
+// Eight codes in 16 bits each.
+template <typename T>
+__device__ __forceinline__ uint4 codes_to_16(uint2 x);
+// 0x6400 | u is 1024 + u in f16, minus 1152.
+template <>
+__device__ __forceinline__ uint4 codes_to_16<__half>(uint2 x) {
     uint4 r;
     uint32_t* const w = reinterpret_cast<uint32_t*>(&r);
     x.x ^= 0x80808080u;
@@ -73,6 +76,21 @@ __device__ __forceinline__ uint4 codes_to_halves(uint2 x) {
     for (int i = 0; i < 4; ++i) {
         const uint32_t u = __byte_perm(i < 2 ? x.x : x.y, 0x64646464u, i & 1 ? 0x4342 : 0x4140);
         const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&u), __float2half2_rn(1152.f));
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return r;
+}
+// 0x4300 | x is 128 + x in bf16 for x < 128: the code's low seven bits, minus
+// 128, or 256 where its sign is set.
+template <>
+__device__ __forceinline__ uint4 codes_to_16<__nv_bfloat16>(uint2 x) {
+    uint4 r;
+    uint32_t* const w = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t u = __byte_perm(i < 2 ? x.x : x.y, 0x43434343u, i & 1 ? 0x4342 : 0x4140);
+        const uint32_t y = u & 0xff7fff7fu, z = u & 0xff80ff80u;
+        const __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&z));
         w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     return r;
@@ -97,13 +115,24 @@ struct Piece {
     uint32_t slot;             // 0: the share's first piece
 };
 
+// What the block works on: a piece, as the warp that finds them leaves it to
+// the others.
+struct Item {
+    uint32_t valid;                     // 0: there is no more
+    uint32_t m, h;                      // group, key head
+    uint32_t row0, rows, first;         // first row of the pair in the group, rows from there on; the group's first sequence
+    uint32_t tokens, t, end;
+    uint32_t slot, whole;
+};
+
 struct Control {
     uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
     uint64_t full[4], empty[4], raw_full[8], raw_empty[8];
+    uint64_t item_full[2], item_empty[2];
+    Item item[2];
     uint64_t sums[2 * (kCopier + 1)];
     uint32_t missing[kScales];          // by tile: bits of 16 tokens whose block is not there
     __align__(16) float2 scales[kScales][8];      // by tile and 16 tokens: of keys, of values
-    Piece start;
     uint32_t tmem;
     uint32_t gave_up;
 };
@@ -201,33 +230,59 @@ __device__ __forceinline__ void rescale(uint32_t p_at, uint32_t o_at, int quarte
     wait_stores();
 }
 
-// 32 scores of a row: weights 2^(key scale * s + base) added to `part`, and
-// times their value scale packed in p.  scales: of 16 tokens each; k_by and v_by
-// belong to the row and to the piece.
-__device__ __forceinline__ void weights32(const float* s, const float2* scales, float k_by, float v_by, float base, uint32_t* p, float& part) {
+// 64 scores of a row that are all seen, 32 at a time; s[0] is on its way, the
+// next 32 follow (`more`: those after these too): weights 2^(key scale * s +
+// base), their sum returned, times their value scale packed in p.  scales: of 16
+// tokens each; k_by and v_by are what they are multiplied by besides.  (Unrolled: at 32
+// a turn the special-function pipe runs dry at each, 2,400 clocks a tile.)
+__device__ __forceinline__ float weights64(uint32_t s_at, bool more, float (&s)[2][32], const float2* scales, float k_by, float v_by, float base,
+                                           uint32_t (&p)[32]) {
     const float2 base2 = make_float2(base, base);
     float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const float2 scale = scales[half];
-        const float k = scale.x * k_by, v = scale.y * v_by;
+    for (int c = 0; c < 2; ++c) {
+        wait_loads32(s[c]);
+        if (c == 0 || more) tmem_load32(s_at + 32 * (c + 1), s[c ^ 1]);
 #pragma unroll
-        for (int i = 8 * half; i < 8 * half + 8; ++i) {
-            float2 x = fma2(make_float2(s[2 * i], s[2 * i + 1]), make_float2(k, k), base2);
-            x.x = exp2_fast(x.x);
-            x.y = exp2_fast(x.y);
-            add[i & 1] = add2(add[i & 1], x);
-            x = mul2(x, make_float2(v, v));
-            p[i] = Type16<__half>::pack(x.x, x.y);
+        for (int half = 0; half < 2; ++half) {
+            const float2 scale = scales[2 * c + half];
+            const float2 k = make_float2(scale.x * k_by, scale.x * k_by), v = make_float2(scale.y * v_by, scale.y * v_by);
+#pragma unroll
+            for (int i = 8 * half; i < 8 * half + 8; ++i) {
+                float2 x = fma2(make_float2(s[c][2 * i], s[c][2 * i + 1]), k, base2);
+                x.x = exp2_fast(x.x);
+                x.y = exp2_fast(x.y);
+                add[i & 1] = add2(add[i & 1], x);
+                x = mul2(x, v);
+                p[16 * c + i] = Type16<__half>::pack(x.x, x.y);
+            }
         }
     }
     add[0] = add2(add[0], add[1]);
-    part = add[0].x + add[0].y;
+    return add[0].x + add[0].y;
 }
 
-// The first tile, the last one where the tokens end inside it, tiles with
-// blocks that are not there, and where the maximum moves: the largest score
-// first, then the weights.  From the quarter `from` on; `left` tokens of the
+// The largest of a row's 128 scores, in log2 units.
+__device__ __noinline__ float largest_score(uint32_t s_at, const float2* scales, float k_by) {
+    float most = -INFINITY;
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        float s[32];
+        tmem_load32(s_at + 32 * c, s);
+        wait_loads32(s);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            float high = s[16 * half];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) high = fmaxf(high, s[16 * half + i]);
+            most = fmaxf(most, high * (scales[2 * c + half].x * k_by));
+        }
+    }
+    return most;
+}
+
+// The last tile where the tokens end inside it, tiles with blocks that are not
+// there, and where the maximum moves: the largest score first, then the weights.  From the quarter `from` on; `left` tokens of the
 // tile are there, `missing` has a bit for each 16 that are not.  `state` is the
 // row's maximum (log2) and sum, returned as they become.
 __device__ __noinline__ float2 weights_with_care(uint32_t s_at, uint32_t o_at, int from, int quarters, int32_t left, uint32_t missing,
@@ -274,7 +329,7 @@ __device__ __noinline__ float2 weights_with_care(uint32_t s_at, uint32_t o_at, i
     return make_float2(next, state.y);
 }
 
-template <int BOXES>
+template <typename T, int BOXES>
 __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ SharedArgs a) {
     extern __shared__ unsigned char raw_smem[];
     unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t{1023});
@@ -293,32 +348,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
     const uint64_t w = all * hkv;
     const uint32_t n = used_shares(w, a.shares);
     if (blockIdx.x >= n) return;
-    if (warp == 0) {
-        const uint64_t first = share_first(w, n, blockIdx.x);
-        Piece p;
-        p.left = share_first(w, n, blockIdx.x + 1) - first;
-        find_piece(a, p, first);
-        if (lane == 0) {
-            ctl.start = p;
-            for (int t = 0; t < 2; ++t) {
-                barrier_init(&ctl.q_full[t], 4);
-                barrier_init(&ctl.s_full[t], 1);
-                barrier_init(&ctl.p_full[t], 4);
-                barrier_init(&ctl.o_full[t], 1);
-            }
-            barrier_init(&ctl.done, 1);
-            for (uint32_t s = 0; s < kRing; ++s) {
-                barrier_init(&ctl.full[s], kConverters);
-                barrier_init(&ctl.empty[s], 1);
-            }
-            for (uint32_t s = 0; s < kRawRing; ++s) {
-                barrier_init(&ctl.raw_full[s], 1);
-                barrier_init(&ctl.raw_empty[s], kConverters);
-            }
-            ctl.gave_up = 0;
-            asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    if (threadIdx.x == 0) {
+        for (int t = 0; t < 2; ++t) {
+            barrier_init(&ctl.q_full[t], 4);
+            barrier_init(&ctl.s_full[t], 1);
+            barrier_init(&ctl.p_full[t], 4);
+            barrier_init(&ctl.o_full[t], 1);
+            barrier_init(&ctl.item_full[t], 1);
+            barrier_init(&ctl.item_empty[t], kCopier);       // (all other warps)
         }
-        __syncwarp();
+        barrier_init(&ctl.done, 1);
+        for (uint32_t s = 0; s < kRing; ++s) {
+            barrier_init(&ctl.full[s], kConverters);
+            barrier_init(&ctl.empty[s], 1);
+        }
+        for (uint32_t s = 0; s < kRawRing; ++s) {
+            barrier_init(&ctl.raw_full[s], 1);
+            barrier_init(&ctl.raw_empty[s], kConverters);
+        }
+        ctl.gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == kIssuer) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_addr(&ctl.tmem)) : "memory");
@@ -341,17 +390,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         }
     };
     auto stopped = [&]() { return __any_sync(kFull, *gave_up != 0); };
-    auto rows_left = [&](const Piece& p) { return p.g.rows - p.segment % p.g.pairs * kPairRows; };     // of the segment, from its first on
-    auto pieces = [&](auto&& work) {           // every piece of the share, till `work` says no
-        Piece p = ctl.start;
-        do {
-            if (p.t == p.end) continue;        // (a share that ends before a segment's first tile)
-            if (!work(p)) return;
-        } while (next_piece(a, p));
+    // The next item for a warp that does not find them (not valid: the end), and
+    // that it has read it.  (What a loop does not need every time stays in shared
+    // memory: a register that is put aside costs more than its time, since what
+    // comes back from local memory waits behind the copies on their way.)
+    auto next_item = [&](uint32_t i) -> const Item& {
+        wait(&ctl.item_full[i & 1], i >> 1 & 1);
+        return ctl.item[i & 1];
+    };
+    auto item_read = [&](uint32_t i) {
+        __syncwarp();
+        if (lane == 0) barrier_arrive(&ctl.item_empty[i & 1]);
     };
     // columns of tile j that hold tokens, to a multiple of 16
-    auto columns = [&](const Piece& p, uint32_t j) {
-        const uint32_t left = p.g.tokens - j * kTileTokens;
+    auto columns = [&](uint32_t tokens, uint32_t j) {
+        const uint32_t left = tokens - j * kTileTokens;
         return left >= kTileTokens ? kTileTokens : (left + 15) & ~15u;
     };
 
@@ -359,14 +412,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         // ---------------------------------------------------- matrix products
         // (the whole warp runs the loop, one elected lane issues)
         constexpr uint32_t kCommon = 1u << 4 | static_cast<uint32_t>(kRows >> 4) << 24;
-        const uint32_t what_o = kCommon | 1u << 16 | (dim >> 3) << 17;         // (values do not lie along the contraction)
+        constexpr uint32_t kScores = kCommon | Type16<T>::kFormat << 7 | Type16<T>::kFormat << 10;
+        const uint32_t what_o = kCommon | 1u << 16 | (dim >> 3) << 17;         // f16 by f16, values not along the contraction
         const int steps = dim / 16;
         const uint64_t q_base = operand(smem_addr(smem), 16, 1024), k_base = operand(smem_addr(ring), 16, 1024);
         const uint64_t v_base = operand(smem_addr(ring), kBoxBytes, 1024);
         constexpr uint32_t kTileUnits = kTileBytes / 16, kBoxUnits = kBoxBytes / 16;
         auto scores = [&](int t, uint32_t stage, uint32_t cols) {
             const uint64_t q = q_base + t * kTileUnits, k = k_base + stage * kTileUnits;
-            const uint32_t what = kCommon | (cols >> 3) << 17;
+            const uint32_t what = kScores | (cols >> 3) << 17;
 #pragma unroll
             for (int i = 0; i < 4 * BOXES; ++i) {
                 const uint32_t off = (i >> 2) * kBoxUnits + (i & 3) * 2;
@@ -385,34 +439,43 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         uint32_t tiles = 0, q_used[2] = {0, 0}, p_used[2] = {0, 0};      // tile i's keys are the ring's 2 i, its values 2 i + 1
         bool issued = false;
         auto full = [&](uint32_t i) { wait(&ctl.full[i % kRing], i / kRing & 1); };
-        pieces([&](const Piece& p) {
-            const bool both = rows_left(p) > kRows;
+        for (uint32_t it = 0;; ++it) {
+            const Item& m = next_item(it);
+            if (stopped() || !m.valid) break;
+            const uint32_t first = m.t, end = m.end, tokens = m.tokens;
+            const bool both = m.rows > kRows;
+            item_read(it);
             full(2 * tiles);
             for (int t = 0; t <= both; ++t) wait(&ctl.q_full[t], q_used[t]++ & 1);
-            if (stopped()) return false;
+            if (stopped()) break;
             issued = true;
             fence_after();
             if (elected()) {
-                for (int t = 0; t <= both; ++t) scores(t, 2 * tiles % kRing, columns(p, p.t));
+                for (int t = 0; t <= both; ++t) scores(t, 2 * tiles % kRing, columns(tokens, first));
                 mma_commit(&ctl.empty[2 * tiles % kRing]);
             }
             __syncwarp();
-            for (uint32_t j = p.t; j < p.end; ++j, ++tiles) {
+            for (uint32_t j = first; j < end; ++j, ++tiles) {
                 const uint32_t stage = (2 * tiles + 1) % kRing, next = (2 * tiles + 2) % kRing;
-                const bool last = j + 1 == p.end;
+                const bool last = j + 1 == end;
                 full(2 * tiles + 1);
-                if (!last) full(2 * tiles + 2);
+                if (stopped()) break;
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     if (t && !both) break;
                     wait(&ctl.p_full[t], p_used[t]++ & 1);
-                    if (stopped()) return false;
                     fence_after();
                     if (elected()) {
-                        products(t, stage, j > p.t, columns(p, j));
+                        products(t, stage, j > first, columns(tokens, j));
                         if (last) mma_commit(&ctl.o_full[t]);
-                        else scores(t, next, columns(p, j + 1));
                     }
+                    __syncwarp();
+                    if (last) continue;
+                    if (t == 0) {
+                        full(2 * tiles + 2);
+                        fence_after();
+                    }
+                    if (elected()) scores(t, next, columns(tokens, j + 1));
                     __syncwarp();
                 }
                 if (elected()) {
@@ -421,8 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                 }
                 __syncwarp();
             }
-            return true;
-        });
+        }
         // TMEM and the stages are in use until this
         if (issued) {
             if (elected()) mma_commit(&ctl.done);
@@ -434,14 +496,28 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         // ------------------------------------------------------------ copies
         // (a lane for every 16 tokens of a tile, the first of each block copies it)
         const uint32_t per_block = block >> 4, bytes = block * dim;
-        uint32_t tiles = 0, loads = 0;
-        pieces([&](const Piece& p) {
+        uint32_t tiles = 0, loads = 0, items = 0;
+        Piece p;
+        p.left = share_first(w, n, blockIdx.x + 1) - share_first(w, n, blockIdx.x);
+        find_piece(a, p, share_first(w, n, blockIdx.x));
+        for (bool more = true; more && !stopped(); more = next_piece(a, p)) {
+            if (p.t == p.end) continue;            // (a share that ends before a segment's first tile)
+            const uint32_t h = p.segment / p.g.pairs, row0 = p.segment % p.g.pairs * kPairRows;
+            wait(&ctl.item_empty[items & 1], (items >> 1 & 1) ^ 1);
+            if (lane == 0) {
+                ctl.item[items & 1] = Item{1, p.m, h, row0, p.g.rows - row0, p.g.first, p.g.tokens, p.t, p.end, p.slot, p.t == 0 && p.end == p.g.tiles};
+                barrier_arrive(&ctl.item_full[items & 1]);
+                if (p.t == 0)                      // where the segment's pieces are
+                    a.far[output_row(a, p.g, h, row0)] =
+                        FarRow{share_of(w, n, p.begin + kStart + p.g.tiles - 1) - blockIdx.x + 1, blockIdx.x, p.slot, 0};
+            }
+            __syncwarp();
+            ++items;
             const int32_t* const table = d.shared_table + static_cast<uint64_t>(p.m) * d.shared_width;
-            const uint32_t h = p.segment / p.g.pairs;
             auto there = [&](uint32_t j) { return lane < 8 && j * kTileTokens + lane * 16 < p.g.tokens; };
             auto id_at = [&](uint32_t j) { return there(j) ? static_cast<uint32_t>(table[(j * kTileTokens + lane * 16) >> a.block_log2]) : kNoNode; };
             uint32_t next = id_at(p.t);
-            for (uint32_t j = p.t; j < p.end; ++j, ++tiles) {
+            for (uint32_t j = p.t; j < p.end && !stopped(); ++j, ++tiles) {
                 const uint32_t id = next;
                 if (j + 1 < p.end) next = id_at(j + 1);
                 const bool ok = id < a.c.num_blocks;
@@ -453,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                 for (int kv = 0; kv < 2; ++kv) {
                     const uint32_t stage = loads % kRawRing;
                     wait(&ctl.raw_empty[stage], (loads / kRawRing & 1) ^ 1);
-                    if (stopped()) return false;
+                    if (stopped()) break;
                     if (kv == 0) {
                         if (lane < 8) ctl.scales[tiles % kScales][lane] = scale;
                         if (lane == 0) ctl.missing[tiles % kScales] = missing;
@@ -466,8 +542,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                     ++loads;
                 }
             }
-            return true;
-        });
+        }
+        wait(&ctl.item_empty[items & 1], (items >> 1 & 1) ^ 1);
+        if (lane == 0) {
+            ctl.item[items & 1].valid = 0;
+            barrier_arrive(&ctl.item_full[items & 1]);
+        }
         // no copy may be in flight when the block ends
         if (lane == 0)
             for (uint32_t i = loads > kRawRing ? loads - kRawRing : 0; i < loads; ++i)
@@ -514,8 +594,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
 #pragma unroll
             for (int i = 0; i < kEach; ++i)
                 if (i < static_cast<int>(mine)) {
-                    *reinterpret_cast<uint4*>(tile + to[i]) = codes_to_halves(x[i][0]);
-                    *reinterpret_cast<uint4*>(tile + (to[i] ^ 16)) = codes_to_halves(x[i][1]);
+                    *reinterpret_cast<uint4*>(tile + to[i]) = kv ? codes_to_16<__half>(x[i][0]) : codes_to_16<T>(x[i][0]);
+                    *reinterpret_cast<uint4*>(tile + (to[i] ^ 16)) = kv ? codes_to_16<__half>(x[i][1]) : codes_to_16<T>(x[i][1]);
                 }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
@@ -525,11 +605,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
             }
             return true;
         };
-        pieces([&](const Piece& p) {
-            for (uint32_t j = p.t; j < p.end; ++j, ++tiles)
-                if (!convert(0) || !convert(1)) return false;
-            return true;
-        });
+        for (uint32_t it = 0;; ++it) {
+            const Item& m = next_item(it);
+            if (stopped() || !m.valid) break;
+            const uint32_t past = tiles + m.end - m.t;
+            item_read(it);
+            for (; tiles < past; ++tiles)
+                if (!convert(0) || !convert(1)) break;
+            if (tiles < past) break;
+        }
     } else {
         // ----------------------------------------------------------- softmax
         const uint32_t t = warp >> 2, row = threadIdx.x & 127;
@@ -538,109 +622,88 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         unsigned char* const tile = smem + t * kTileBytes;
         unsigned char* const staging = tile + (warp & 3) * 4096;       // the queries' place, once they are done with
         uint32_t s_used = 0, o_used = 0, tiles = 0;
-        pieces([&](const Piece& p) {
-            if (p.t == 0 && threadIdx.x == 0) {        // where the segment's pieces are
-                const uint32_t last = share_of(w, n, p.begin + kStart + p.g.tiles - 1);
-                a.far[output_row(a, p.g, p.segment / p.g.pairs, p.segment % p.g.pairs * kPairRows)] =
-                    FarRow{last - blockIdx.x + 1, blockIdx.x, p.slot, 0};
+        for (uint32_t it = 0;; ++it) {
+            const Item& m = next_item(it);
+            if (stopped() || !m.valid) break;
+            const uint32_t first = m.t, end = m.end;
+            if (m.rows <= t * kRows) {
+                tiles += end - first;
+                item_read(it);
+                continue;
             }
-            if (rows_left(p) <= t * kRows) {
-                tiles += p.end - p.t;
-                return true;
-            }
-            const uint32_t h = p.segment / p.g.pairs, r = p.segment % p.g.pairs * kPairRows + t * kRows + row;
-            const bool real = r < p.g.rows;
-            const uint32_t b = p.g.first + r / a.rows, i = r % a.rows / a.group, head = h * a.group + r % a.rows % a.group;
-            // this row's query, and the power of two that it was divided by
-            float row_scale = 1.f;
+            const bool real = t * kRows + row < m.rows;
+            // this row's place in the outputs and in the queries
+            auto place = [&](uint32_t& b, uint32_t& i, uint32_t& head) {
+                const uint32_t r = m.row0 + t * kRows + row, in = r % a.rows;
+                b = m.first + r / a.rows;
+                i = in / a.group;
+                head = m.h * a.group + in % a.group;
+            };
+            // The warp's queries, a row's units to lanes side by side.  (As little code
+            // as can be: what a warp executes for the first time takes 230 clocks for
+            // eight instructions.)
             {
-                const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(d.q) + b * d.q_stride[0] + i * d.q_stride[1] +
-                                                                head * d.q_stride[2]);
-                auto units = [&](int c0, uint4 (&x)[8]) {
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) x[c] = real && c0 + c < static_cast<int>(dim / 8) ? q[c0 + c] : make_uint4(0, 0, 0, 0);
-                };
-                float up = 1.f;
-                if (d.dtype != BS_F16) {
-                    // times 2^e with the row's largest in [2^12, 2^13); rows of zeros, infinities and NaN as they are
-                    uint32_t high = 0;       // magnitudes of bf16 order as integers
+                constexpr uint32_t kLanes = 8 * BOXES, kAtOnce = 32 / kLanes;
+                const uint32_t c = lane % kLanes;
+                uint32_t b, i, head;
+                place(b, i, head);
+                const uint16_t* const mine = static_cast<const uint16_t*>(d.q) + (real ? b * d.q_stride[0] + i * d.q_stride[1] + head * d.q_stride[2] : 0);
 #pragma unroll 1
-                    for (int c0 = 0; c0 < 8 * BOXES; c0 += 8) {
-                        uint4 x[8];
-                        units(c0, x);
-#pragma unroll
-                        for (int c = 0; c < 8; ++c)
-                            high = __vmaxu2(high, __vmaxu2(__vmaxu2(x[c].x & 0x7fff7fffu, x[c].y & 0x7fff7fffu), __vmaxu2(x[c].z & 0x7fff7fffu, x[c].w & 0x7fff7fffu)));
-                    }
-                    high = max(high >> 16, high & 0xffffu);
-                    uint32_t e = high >> 7;  // biased exponent
-                    e = high == 0 || e == 255 ? 139 : e < 13 ? 13 : e;
-                    up = __uint_as_float((266 - e) << 23);
-                    row_scale = __uint_as_float((e - 12) << 23);
+                for (uint32_t y = lane / kLanes; y < 32; y += kAtOnce) {
+                    const uint16_t* const q = reinterpret_cast<const uint16_t*>(__shfl_sync(kFull, reinterpret_cast<uintptr_t>(mine), y));
+                    const uint32_t there = __shfl_sync(kFull, real, y) && c < dim / 8 ? 16 : 0, to = (warp & 3) * 32 + y;      // (else zeros)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(
+                                     smem_addr(tile + (c >> 3) * kBoxBytes + to * 128 + ((c ^ to) & 7) * 16)),
+                                 "l"(there ? q + c * 8 : q), "r"(there)
+                                 : "memory");
                 }
-#pragma unroll 1
-                for (int c0 = 0; c0 < 8 * BOXES; c0 += 8) {
-                    uint4 x[8];
-                    units(c0, x);
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        if (d.dtype != BS_F16) {
-                            uint32_t* const w = reinterpret_cast<uint32_t*>(&x[c]);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) w[k] = Type16<__half>::pack(__uint_as_float(w[k] << 16) * up, __uint_as_float(w[k] & 0xffff0000u) * up);
-                        }
-                        *reinterpret_cast<uint4*>(tile + (c0 >> 3) * kBoxBytes + row * 128 + ((c ^ row) & 7) * 16) = x[c];
-                    }
-                }
+                asm volatile("cp.async.wait_all;\n" ::: "memory");
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 __syncwarp();
                 if (lane == 0) barrier_arrive(&ctl.q_full[t]);
             }
             // the largest value scale of the piece
-            const int32_t* const table = d.shared_table + static_cast<uint64_t>(p.m) * d.shared_width;
-            const uint32_t past = min(p.end * kTileTokens, p.g.tokens);
             float unit = 0.f;
-            for (uint32_t col = (p.t * kTileTokens >> a.block_log2) + lane; col << a.block_log2 < past; col += 32) {
-                const uint32_t id = table[col];
-                if (id < a.c.num_blocks) unit = fmaxf(unit, a.c.v_scale[static_cast<uint64_t>(id) * hkv + h]);
+            {
+                const int32_t* const table = d.shared_table + static_cast<uint64_t>(m.m) * d.shared_width;
+                const uint32_t past = min(end * kTileTokens, m.tokens);
+                for (uint32_t col = (first * kTileTokens >> a.block_log2) + lane; col << a.block_log2 < past; col += 32) {
+                    const uint32_t id = table[col];
+                    if (id < a.c.num_blocks) unit = fmaxf(unit, a.c.v_scale[static_cast<uint64_t>(id) * hkv + m.h]);
+                }
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) unit = fmaxf(unit, __shfl_xor_sync(kFull, unit, o));
             if (!(unit > 0.f)) unit = 1.f;
-            const float k_by = d.scale * 1.4426950408889634f * row_scale, v_by = 1.f / unit;
+            const float k_by = d.scale * 1.4426950408889634f, v_by = 1.f / unit;
             float top = -INFINITY, sum = 0.f;       // top: in log2 units, moved when weights are past 2^8
-            for (uint32_t j = p.t; j < p.end; ++j, ++tiles) {
+            for (uint32_t j = first; j < end; ++j, ++tiles) {
                 wait(&ctl.s_full[t], s_used++ & 1);        // and the value product before it is done
-                if (stopped()) return false;
+                if (stopped()) break;
                 fence_after();
-                const uint32_t left = p.g.tokens - j * kTileTokens;
+                const uint32_t left = m.tokens - j * kTileTokens;
                 int done = 0;           // quarters of the tile whose weights are made
                 const float2* const scales = ctl.scales[tiles % kScales];
                 const uint32_t missing = ctl.missing[tiles % kScales];
-                if (j > p.t && left >= kTileTokens && !missing) {
+                if (left >= kTileTokens && !missing) {
+                    if (j == first) top = largest_score(s_at, scales, k_by);
                     float s[2][32];
                     tmem_load32(s_at, s[0]);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        wait_loads32(s[c & 1]);
-                        if (c < 3) tmem_load32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
-                        uint32_t w16[16];
-                        float part;
-                        weights32(s[c & 1], scales + 2 * c, k_by, v_by, kLift - top, w16, part);
+#pragma unroll 1
+                    for (; done < 4; done += 2) {
+                        uint32_t w16[32];
+                        const float part = weights64(s_at + 32 * done, done == 0, s, scales + 2 * done, k_by, v_by, kLift - top, w16);
                         if (__any_sync(kFull, real && part > kMost)) break;       // (rows that are none hold anything)
                         sum += part;
-                        tmem_store16(s_at + 16 * c, w16);
-                        done = c + 1;
+                        tmem_store16(s_at + 16 * done, w16);
+                        tmem_store16(s_at + 16 * done + 16, w16 + 16);
                     }
-                    if (done < 4) {
-                        wait_loads32(s[0]);
-                        wait_loads32(s[1]);
-                    }
+                    if (done == 0) wait_loads32(s[0]);
                 }
                 if (done < 4) {
-                    const int quarters = (static_cast<int>(columns(p, j)) + 31) / 32;
+                    const int quarters = (static_cast<int>(columns(m.tokens, j)) + 31) / 32;
                     const float2 state = weights_with_care(s_at, o_at, done, quarters, left < kTileTokens ? left : kTileTokens, missing, scales, k_by,
-                                                           v_by, j > p.t ? dim : 0, make_float2(top, sum));
+                                                           v_by, j > first ? dim : 0, make_float2(top, sum));
                     top = state.x;
                     sum = state.y;
                 }
@@ -650,13 +713,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                 if (lane == 0) barrier_arrive(&ctl.p_full[t]);
             }
             wait(&ctl.o_full[t], o_used++ & 1);
-            if (stopped()) return false;
+            if (stopped()) break;
             fence_after();
             // unnormalised outputs, to be joined with those over the sequences' own tokens
-            const bool whole = p.t == 0 && p.end == p.g.tiles;
-            const uint64_t at = whole ? (static_cast<uint64_t>(b) * d.queries + i) * d.q_heads + head
-                                      : (static_cast<uint64_t>(blockIdx.x) * 2 + p.slot) * kPairRows + t * kRows + row;
-            float* const out = real ? (whole ? a.whole_o : a.part_o) + at * dim : nullptr;
+            uint32_t b, i, head;
+            place(b, i, head);
+            const uint64_t at = m.whole ? (static_cast<uint64_t>(b) * d.queries + i) * d.q_heads + head
+                                        : (static_cast<uint64_t>(blockIdx.x) * 2 + m.slot) * kPairRows + t * kRows + row;
+            float* const out = real ? (m.whole ? a.whole_o : a.part_o) + at * dim : nullptr;
+            if (real) (m.whole ? a.whole_ml : a.part_ml)[at] = make_float2(top - kLift, sum);
+#pragma unroll 1
             for (uint32_t x = 0; x < dim; x += 32) {
                 float o[32];
                 tmem_load32(o_at + x, o);
@@ -666,23 +732,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                 for (int k = 0; k < 32; ++k) u[k] = __float_as_uint(o[k] * unit);
                 store_rows(u, staging, out, x * 4, dim * 4);
             }
-            if (real) (whole ? a.whole_ml : a.part_ml)[at] = make_float2(top - kLift, sum);
-            // the next piece's first value product overwrites the outputs: it
+            item_read(it);
+            // the next item's first value product overwrites the outputs: it
             // waits for weights that this warp makes after these loads
             fence_before();
-            return true;
-        });
+        }
     }
     fence_before();
     __syncthreads();
     if (warp == kIssuer) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
 }
 
-template <int BOXES>
+template <typename T, int BOXES>
 cudaError_t launch(const SharedArgs& a, cudaStream_t stream) {
-    const cudaError_t e = cudaFuncSetAttribute(k_shared<BOXES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<BOXES>);
+    const cudaError_t e = cudaFuncSetAttribute(k_shared<T, BOXES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<BOXES>);
     if (e != cudaSuccess) return e;
-    return launch_after(k_shared<BOXES>, dim3(a.shares), kThreads, kSmem<BOXES>, stream, a);
+    return launch_after(k_shared<T, BOXES>, dim3(a.shares), kThreads, kSmem<BOXES>, stream, a);
 }
 
 }  // namespace
@@ -690,7 +755,8 @@ cudaError_t launch(const SharedArgs& a, cudaStream_t stream) {
 cudaError_t launch_shared_part(const SharedArgs& given, cudaStream_t stream) {
     SharedArgs a = given;
     a.polls = wait_polls();
-    return a.c.dim <= 64 ? launch<1>(a, stream) : launch<2>(a, stream);
+    if (a.d.dtype == BS_F16) return a.c.dim <= 64 ? launch<__half, 1>(a, stream) : launch<__half, 2>(a, stream);
+    return a.c.dim <= 64 ? launch<__nv_bfloat16, 1>(a, stream) : launch<__nv_bfloat16, 2>(a, stream);
 }
 
 }  // namespace bsb
