@@ -33,8 +33,10 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr uint32_t kMostIds = 256;     // entries looked up at a time
+constexpr int32_t kHidden = 0x40000000;     // a position past all that are seen
+constexpr int32_t kShared = -0x40000000;    // and where those of shared tokens begin
 constexpr uint32_t kMostCluster = 8;
-constexpr uint32_t kBatch = 4;          // pieces of the shared tokens' outputs on their way together
+constexpr uint32_t kBatch = 8;          // pieces of the shared tokens' outputs on their way together
 template <int NT>
 constexpr int kStagesOf = NT == 1 ? 2 : 3;
 constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
@@ -44,11 +46,12 @@ struct RowsArgs {
     const int32_t* blocks;             // [num_seqs][queries][kv_heads][count]
     uint32_t count;
     uint32_t rows;                     // of a segment
+    uint32_t direct;                   // 1: the shared tokens are this kernel's too
 };
 
 template <int NW>
 constexpr int kListStage = kStageBytes<NW> + 16;               // and the halves' first positions
-constexpr int kIdBytes = kMostIds * 8 + kWarps * 4;
+constexpr int kIdBytes = kMostIds * 8;
 // (the entries lie where the outputs are joined later: with 16 query rows two blocks just fit an SM)
 template <int NW, int NT>
 constexpr int kJoinOrIds = kJoinBytes<NW, NT> > kIdBytes ? kJoinBytes<NW, NT> : kIdBytes;
@@ -72,7 +75,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
     float* const join_ml = reinterpret_cast<float*>(smem + kWarps * kStages * kListStage<NW>);     // [warps + 1][kRows][2]
     float* const join_o = join_ml + (kWarps + 1) * kRows * 2;
     int2* const ids = reinterpret_cast<int2*>(join_o);          // block, first position; till the outputs are joined
-    uint32_t* const found = reinterpret_cast<uint32_t*>(ids + kMostIds);      // [warps]
 
     const SharedArgs& a = given.s;
     // In every block, before anything of the caller's.  (After the shared tokens'
@@ -102,6 +104,16 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
                 limit[nt][i] = static_cast<int32_t>(len) - d.queries + 1 + static_cast<int32_t>(LIST ? query : (col + i) / a.group);
         }
     };
+    Group group{};                   // what the sequence shares (none: no tokens)
+    uint32_t m = 0;
+    auto find_group = [&]() {
+        for (uint32_t past = d.num_groups; past - m > 1;) {    // the last group that begins at b or before
+            const uint32_t mid = (m + past) / 2;
+            (d.cu[mid] <= static_cast<int32_t>(b) ? m : past) = mid;
+        }
+        group = shared::group_of(a, m);
+        if (b < group.first || static_cast<int32_t>(b) >= d.cu[m + 1]) group = Group{};
+    };
     float o[NT][NW][4];
     float top[NT][2], sum[NT][2], unit = kFold / -kNoScore, inv_unit = -kNoScore;
 #pragma unroll
@@ -112,46 +124,41 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
         for (int j = 0; j < NW; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
     }
 
-    // the entries: the list's, or every block of its own
+    // the entries: the list's, or every block of what it shares, where that is done
+    // here, and of its own.  Positions of shared tokens count from kShared.
+    if (!LIST && given.direct) find_group();
+    const uint32_t shared_entries = !LIST && given.direct ? (group.tokens + block - 1) / block : 0;
     const int32_t* const table = d.table + static_cast<uint64_t>(b) * d.table_width;
     const int32_t* const list = given.blocks + ((static_cast<uint64_t>(b) * d.queries + query) * hkv + h) * given.count;
     const int32_t most = static_cast<int32_t>(len) - (LIST ? d.queries - 1 - static_cast<int32_t>(query) : 0);
     const uint32_t width = d.table_width, tokens = most > 0 ? most : 0;           // some row sees the tokens below
-    const uint32_t entries = LIST ? given.count : (tokens + block - 1) / block;
+    const uint32_t entries = LIST ? given.count : shared_entries + (tokens + block - 1) / block;
     // this block's part of the entries
     const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(entries) * (rank + 1) / parts);
     const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(entries) * rank / parts);
     for (uint32_t from = begin; from < end; from += kMostIds) {
-        // look them up; those without a token that is seen are left out
-        uint32_t held = 0;
-#pragma unroll
-        for (uint32_t e0 = 0; e0 < kMostIds; e0 += kThreads) {
-            const uint32_t e = from + e0 + threadIdx.x;
-            int64_t col = -1;
-            if (e < end) col = LIST ? list[e] : static_cast<int64_t>(e);
-            uint32_t id = kNoNode;
-            if (col >= 0 && col < width && col * block < tokens) {
-                id = table[col];
-                if (id >= a.c.num_blocks) {
-                    atomicOr(a.errors, kMemErrBlock);
-                    id = kNoNode;
-                }
-            } else if (LIST && col >= width) {
+        // look them up; one without a token that is seen begins past all of them
+        const uint32_t held = min(end - from, kMostIds);
+        for (uint32_t e = threadIdx.x; e < held; e += kThreads) {
+            int2 entry = make_int2(0, kHidden);
+            if (!LIST && from + e < shared_entries) {
+                const uint32_t id = d.shared_table[static_cast<uint64_t>(m) * d.shared_width + from + e];
+                if (id < a.c.num_blocks) entry = make_int2(id, kShared + static_cast<int32_t>((from + e) * block));
+                else atomicOr(a.errors, kMemErrBlock);
+                ids[e] = entry;
+                continue;
+            }
+            const int32_t col = LIST ? list[from + e] : static_cast<int32_t>(from + e - shared_entries);
+            if (col >= 0 && static_cast<uint32_t>(col) < width && static_cast<int64_t>(col) * block < tokens) {
+                const uint32_t id = table[col];
+                if (id < a.c.num_blocks) entry = make_int2(id, static_cast<int32_t>(col * block));
+                else atomicOr(a.errors, kMemErrBlock);
+            } else if (LIST && col >= 0 && static_cast<uint32_t>(col) >= width) {
                 atomicOr(a.errors, kMemErrLength);
             }
-            const unsigned in = __ballot_sync(kFull, id != kNoNode);
-            if (lane == 0) found[warp] = __popc(in);
-            __syncthreads();
-            uint32_t at = held + __popc(in & ((1u << lane) - 1));
-#pragma unroll
-            for (uint32_t x = 0; x < kWarps; ++x) {
-                const uint32_t n = found[x];
-                if (x < warp) at += n;
-                held += n;
-            }
-            if (id != kNoNode) ids[at] = make_int2(id, static_cast<int32_t>(col * block));
-            __syncthreads();
+            ids[e] = entry;
         }
+        __syncthreads();
         const uint32_t tiles = ((held << a.block_log2) + kTile - 1) / kTile;
         auto request = [&](uint32_t t, uint32_t stage) {
             if (t < tiles) {
@@ -160,9 +167,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const uint32_t at = t * kTile + 16 * half, e = at >> a.block_log2, in = at & (block - 1);
-                    const int2 entry = e < held ? ids[e] : make_int2(0, 0x40000000);
+                    const int2 entry = e < held ? ids[e] : make_int2(0, kHidden);
                     const int32_t pos = entry.y + static_cast<int32_t>(in);
-                    if (pos < static_cast<int32_t>(tokens)) {
+                    const int32_t left = (pos < 0 ? kShared + static_cast<int32_t>(group.tokens) : static_cast<int32_t>(tokens)) - pos;
+                    if (left > 0) {
                         const uint64_t slab = static_cast<uint64_t>(static_cast<uint32_t>(entry.x)) * hkv + h;
                         const uint64_t row = ((slab << a.block_log2) + in) * kDim + lane * 16;
                         const int8_t* k = a.c.k + row;
@@ -179,29 +187,35 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
                         scales[2 * half] = 0.f;
                         scales[2 * half + 1] = -1.f;
                     }
-                    if (lane == 2) reinterpret_cast<int32_t*>(scales)[4 + half] = pos;
+                    if (lane == 2) *reinterpret_cast<int2*>(scales + 4 + 2 * half) = make_int2(pos, left);
                 }
             }
             asm volatile("cp.async.commit_group;\n" ::: "memory");
         };
 #pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) request(warp + i * kWarps, i);
-        if (from == begin) load_queries();             // (under the first copies)
-        uint32_t stage = 0, fill = kStages - 1;
+        for (int i = 0; i < kStages; ++i) request(warp + i * kWarps, i);
+        if (from == begin) {                           // (under the first copies)
+            load_queries();
+            if (!LIST && a.shares) find_group();
+        }
+        uint32_t stage = 0;
         for (uint32_t t = warp; t < tiles; t += kWarps) {
-            asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 1) : "memory");
             __syncwarp();
-            request(t + (kStages - 1) * kWarps, fill);       // the stage that the last tile used
-            fill = fill + 1 == kStages ? 0 : fill + 1;
             const unsigned char* s = ring + stage * kListStage<NW>;
-            stage = stage + 1 == kStages ? 0 : stage + 1;
             const float4 sc = *reinterpret_cast<const float4*>(s + 2 * kTile * kPitch<NW>);
-            const int2 first = *reinterpret_cast<const int2*>(s + 2 * kTile * kPitch<NW> + 16);
+            const int4 first = *reinterpret_cast<const int4*>(s + 2 * kTile * kPitch<NW> + 16);
             const float k_scale[2] = {sc.x, sc.z}, v_scale[2] = {sc.y, sc.w};
-            const int32_t pos[2] = {first.x, first.y};
+            const int32_t pos[2] = {first.x, first.z}, left[2] = {first.y, first.w};
+            if (fmaxf(v_scale[0], v_scale[1]) < 0.f) {      // none to see
+                __syncwarp();
+                request(t + kStages * kWarps, stage);
+                stage = stage + 1 == kStages ? 0 : stage + 1;
+                continue;
+            }
             float z[2][NT][4];           // [half]: tokens g and g + 8 (+ 16 half), columns 2c and 2c + 1
             tile_scores<NW, NT>(z, s, q, g, c);
-            const bool edge = max(pos[0], pos[1]) + 16 > static_cast<int32_t>(tokens) - (LIST ? 0 : d.queries - 1);
+            const bool edge = min(left[0], left[1]) < 16 || (!LIST && max(pos[0], pos[1]) + 16 > static_cast<int32_t>(tokens) - d.queries + 1);
             bool move = fmaxf(v_scale[0], v_scale[1]) > 4.f * unit;
 #pragma unroll
             for (int half = 0; half < 2; ++half)
@@ -210,16 +224,25 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         z[half][nt][i] *= row_scale[nt][i & 1] * k_scale[half];
-                        if (edge && pos[half] + static_cast<int32_t>(g) + (i & 2) * 4 >= limit[nt][i & 1]) z[half][nt][i] = -INFINITY;
+                        const int32_t in = static_cast<int32_t>(g) + (i & 2) * 4;
+                        if (edge && (in >= left[half] || pos[half] + in >= limit[nt][i & 1])) z[half][nt][i] = -INFINITY;
                         move |= z[half][nt][i] > top[nt][i & 1] + kSlack;
                     }
             if (__any_sync(kFull, move)) move_maxima<NW, NT>(z, v_scale, top, sum, o, unit, inv_unit);
             tile_values<NW, NT>(z, s, v_scale, inv_unit, top, sum, o, g, c);
             __syncwarp();
+            request(t + kStages * kWarps, stage);          // where this tile was
+            stage = stage + 1 == kStages ? 0 : stage + 1;
         }
         __syncthreads();               // `ids` is done with
     }
 
+    if (!LIST && a.shares && begin == end) find_group();
+    FarRow far{};                    // a thread below kRows: where that row's outputs over the shared tokens are
+    if (!LIST && a.shares) {
+        cudaGridDependencySynchronize();
+        if (group.tiles && threadIdx.x < kRows && row0 + threadIdx.x < given.rows) far = shared::far_row(a, group, b, h, row0 + threadIdx.x);
+    }
     float all_top[NT][2], all_sum[NT][2];
     join_warps<NW, NT>(o, top, sum, unit, all_top, all_sum, join_o, join_ml, warp, lane);
     auto row_at = [&](uint32_t r) {        // row of the outputs
@@ -262,20 +285,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
                 for (int j = 0; j < NW; ++j)
                     *reinterpret_cast<float2*>(part_o + r * kDim + value_dim<NW>(j, g)) = make_float2(o[nt][j][i], o[nt][j][2 + i]);
             }
-    // and those over the shared tokens: where the row's pair of tiles is (bs_shared.cuh)
     FarRow* const far_rows = reinterpret_cast<FarRow*>(smem);  // (over the ring)
-    if (!LIST && a.shares) {
-        uint32_t m = 0;
-        for (uint32_t past = d.num_groups; past - m > 1;) {    // the last group that begins at b or before
-            const uint32_t mid = (m + past) / 2;
-            (d.cu[mid] <= static_cast<int32_t>(b) ? m : past) = mid;
-        }
-        const Group group = shared::group_of(a, m);
-        const bool shares = group.tiles && b >= group.first && static_cast<int32_t>(b) < d.cu[m + 1];
-        cudaGridDependencySynchronize();
-        if (threadIdx.x < kRows && row0 + threadIdx.x < given.rows)
-            far_rows[threadIdx.x] = shares ? shared::far_row(a, group, b, h, row0 + threadIdx.x) : FarRow{};
-    }
+    if (!LIST && threadIdx.x < kRows) far_rows[threadIdx.x] = far;
     if (!LIST && blockIdx.x == 0 && blockIdx.y == 0 && b == 0)
         for (uint32_t i = threadIdx.x; i <= d.num_groups; i += kThreads) {
             const int32_t x = d.cu[i];
@@ -304,18 +315,18 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
             acc.x += y.x * w, acc.y += y.y * w, acc.z += y.z * w, acc.w += y.w * w;
         }
         const uint64_t row = row_at(row0 + r);
-        const FarRow far = LIST || !a.shares ? FarRow{} : far_rows[r];
-        for (uint32_t p0 = 0; p0 < far.pieces; p0 += kBatch) {
+        const FarRow at_far = LIST ? FarRow{} : far_rows[r];
+        for (uint32_t p0 = 0; p0 < at_far.pieces; p0 += kBatch) {
             float2 far_ml[kBatch];
             float4 y[kBatch];
             float high = m;
 #pragma unroll
             for (uint32_t u = 0; u < kBatch; ++u) {
-                const uint32_t p = min(p0 + u, far.pieces - 1);
-                const uint64_t slot = ((static_cast<uint64_t>(far.share) + p) * 2 + (p == 0 ? far.slot : 0)) * shared::kPairRows + far.row;
-                far_ml[u] = far.pieces == 1 ? a.whole_ml[row] : a.part_ml[slot];
-                y[u] = *reinterpret_cast<const float4*>(far.pieces == 1 ? a.whole_o + row * kDim + at : a.part_o + slot * kDim + at);
-                if (p0 + u >= far.pieces) far_ml[u] = make_float2(kNoScore, 0.f);
+                const uint32_t p = min(p0 + u, at_far.pieces - 1);
+                const uint64_t slot = ((static_cast<uint64_t>(at_far.share) + p) * 2 + (p == 0 ? at_far.slot : 0)) * shared::kPairRows + at_far.row;
+                far_ml[u] = at_far.pieces == 1 ? a.whole_ml[row] : a.part_ml[slot];
+                y[u] = *reinterpret_cast<const float4*>(at_far.pieces == 1 ? a.whole_o + row * kDim + at : a.part_o + slot * kDim + at);
+                if (p0 + u >= at_far.pieces) far_ml[u] = make_float2(kNoScore, 0.f);
                 high = fmaxf(high, far_ml[u].x);
             }
             const float shrink = exp2_fast(m - high);
@@ -324,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
             acc.x *= shrink, acc.y *= shrink, acc.z *= shrink, acc.w *= shrink;
 #pragma unroll
             for (uint32_t u = 0; u < kBatch; ++u) {
-                if (p0 + u >= far.pieces) break;
+                if (p0 + u >= at_far.pieces) break;
                 const float w = exp2_fast(far_ml[u].x - m);
                 l += far_ml[u].y * w;
                 acc.x += y[u].x * w, acc.y += y[u].y * w, acc.z += y[u].z * w, acc.w += y[u].w * w;
@@ -345,22 +356,29 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
     if (parts > 1) cluster.sync();         // no block ends while another reads it
 }
 
-// Blocks of a segment, by the time of its longest part and of all of them: a
-// block takes as long as kStart tiles to begin and end, and the join of a
-// cluster some more.
-uint32_t parts_of(uint64_t segments, uint64_t tokens, uint64_t resident) {
+// Blocks of a segment, by the time of its longest part and of all of them, and
+// that time: a block takes as long as kStart tiles to begin and end, and the join
+// of a cluster some more; a tile takes a block 0.45 us.
+uint32_t parts_of(uint64_t segments, uint64_t tokens, uint64_t resident, double& time) {
     constexpr double kStart = 6, kJoin = 2;
     uint32_t best = 1;
-    double least = 0;
     for (uint32_t n = 1; n <= kMostCluster; ++n) {
         const double waves = static_cast<double>((segments * n + resident - 1) / resident);
-        const double time = waves * (kStart + static_cast<double>(tokens) / kTile / n) + (n > 1 ? kJoin : 0);
-        if (n == 1 || time < least) {
-            least = time;
+        const double t = waves * (kStart + static_cast<double>(tokens) / kTile / n) + (n > 1 ? kJoin : 0);
+        if (n == 1 || t < time) {
+            time = t;
             best = n;
         }
     }
     return best;
+}
+
+uint64_t resident_blocks(const MemoryDevice& dev, uint32_t rows) { return static_cast<uint64_t>(dev.num_sms) * blocks_per_sm(rows <= 8 ? 1 : 2); }
+
+// The segments of attention over own tokens, as many as row tiles of key heads.
+uint64_t own_segments(const bs_token_cache& c, const bs_shared_attention_desc& d, uint32_t rows) {
+    const uint32_t tile = rows <= 8 ? 8 : 16;
+    return static_cast<uint64_t>(c.kv_heads) * d.num_seqs * ((rows + tile - 1) / tile);
 }
 
 template <int NW, int NT, bool LIST>
@@ -369,8 +387,9 @@ cudaError_t launch_rows(const RowsArgs& a, const MemoryDevice& dev, cudaStream_t
     if (e != cudaSuccess) return e;
     const uint32_t row_tiles = (a.rows + 8 * NT - 1) / (8 * NT);
     const uint64_t segments = static_cast<uint64_t>(a.s.c.kv_heads) * (LIST ? a.s.d.queries : 1);
-    const uint64_t width = LIST ? a.count : a.s.d.table_width;
-    const uint32_t parts = parts_of(segments * row_tiles * a.s.d.num_seqs, width * a.s.c.block, static_cast<uint64_t>(dev.num_sms) * blocks_per_sm(NT));
+    const uint64_t width = LIST ? a.count : a.s.d.table_width + (a.direct ? a.s.d.shared_width : 0ull);
+    double time = 0;
+    const uint32_t parts = parts_of(segments * row_tiles * a.s.d.num_seqs, width * a.s.c.block, resident_blocks(dev, a.rows), time);
     cudaLaunchAttribute attr[2] = {};
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = parts;
@@ -410,6 +429,17 @@ struct Layout {
 
 Layout plan(const bs_token_cache& c, const bs_shared_attention_desc& d, const MemoryDevice& dev) {
     Layout l{};
+    // Few shared tokens or few sequences: each sequence reads them by itself, in
+    // the kernel for its own.  The times of both ways, in tiles of that kernel
+    // (0.45 us): the other one takes 14 us for its start, its end and the join, and
+    // 2.6 us for 256 rows over 128 tokens.  (4 sequences over 700 tokens: 8.9 us
+    // this way, 20 that way; 64 over 900 to 17,001: 256 and 101.)
+    const uint32_t in_sequence = static_cast<uint32_t>(d.q_heads / c.kv_heads) * d.queries;
+    const uint64_t segments = own_segments(c, d, in_sequence), resident = resident_blocks(dev, in_sequence);
+    const uint64_t own = static_cast<uint64_t>(d.table_width) * c.block;
+    double here = 0, there = 0;
+    parts_of(segments, own + static_cast<uint64_t>(d.shared_width) * c.block, resident, here);
+    parts_of(segments, own, resident, there);
     const uint64_t tiles = (static_cast<uint64_t>(d.shared_width) * c.block + shared::kTileTokens - 1) / shared::kTileTokens;
     if (tiles == 0) return l;
     const uint64_t rows = static_cast<uint64_t>(d.num_seqs) * d.queries * d.q_heads;
@@ -417,6 +447,11 @@ Layout plan(const bs_token_cache& c, const bs_shared_attention_desc& d, const Me
     const uint64_t pairs = rows / c.kv_heads / shared::kPairRows + std::min(d.num_groups, d.num_seqs);
     const uint64_t units = pairs * c.kv_heads * (tiles + shared::kStart), most = (units + 2 * shared::kStart - 1) / (2 * shared::kStart);
     l.shares = static_cast<uint32_t>(most < static_cast<uint64_t>(dev.num_sms) ? most : dev.num_sms);
+    there += (14 + 2.6 * static_cast<double>(units) / l.shares) / 0.45;
+    if (here <= there) {
+        l.shares = 0;
+        return l;
+    }
     auto take = [&l](size_t bytes) {
         const size_t at = l.total;
         l.total += (bytes + 255) & ~static_cast<size_t>(255);
@@ -476,6 +511,7 @@ cudaError_t launch_shared_attention(const bs_token_cache& c, const bs_shared_att
     a.s.group = d.q_heads / c.kv_heads;
     a.s.rows = a.rows = a.s.group * d.queries;
     a.s.shares = l.shares;
+    a.direct = l.shares == 0 && d.shared_width > 0;
     a.s.block_log2 = log2_of(c.block);
     const cudaError_t e = l.shares ? launch_shared_part(a.s, stream) : cudaSuccess;
     if (e != cudaSuccess) return e;

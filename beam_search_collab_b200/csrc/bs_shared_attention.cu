@@ -15,13 +15,16 @@
 // 8-13 convert keys and values, 14 issues the matrix instructions, 15 finds the
 // pieces of the share and copies codes (a bulk copy for each block) and scales to
 // shared memory:
-//   S_t = Q_t K^T     codes of K exact in the queries' 16-bit type
+//   S_t = Q_t K^T     codes of K exact in f16, as are bf16 queries times a power
+//                     of two of each row's own (elements below 2^-29 of the
+//                     row's largest lose bits); bf16 keys took twice the
+//                     instructions to convert
 //   O_t += P_t V      codes of V exact in f16, P_t f16: a weight times its values'
 //                     scale, over the largest of the piece, rounded to 2^-11 of
 //                     itself or, where that is more, 2^-29 of a weight of 1 at
 //                     the largest scale (weights count in 2^-kLift, the room
 //                     that a maximum moved at 2^10 leaves)
-// The maximum is moved only when a sum of 32 weights passes 2^10 (no maximum is
+// The maximum is moved only when a sum of 64 weights passes 2^10 (no maximum is
 // taken before the exponentials); sums are 32-bit, of the unrounded weights.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -44,30 +47,23 @@ constexpr int kConverters = 6;         // warps
 constexpr int kIssuer = 8 + kConverters;
 constexpr int kCopier = kIssuer + 1;
 constexpr int kThreads = 32 * (kCopier + 1);
-// Rings of converted tiles and of their codes, keys and values in turn: with
-// rows of 128 dimensions no more fit.  (Three converted ones do: a tile's values
-// and the next one's keys are in use together, meanwhile the next values are
-// converted.  With two of each converted and one of each of codes, a copy's 1.2 us
-// came after each conversion, 5,500 clocks a tile.)
+// Rings of converted tiles (keys and values in turn: a tile's values and the next
+// one's keys are in use together, meanwhile the next ones are converted) and of
+// halves of tiles of codes, of which four take the 1.2 us that a copy takes.
+constexpr uint32_t kRing = 4;
 template <int BOXES>
-constexpr int kStages = BOXES == 2 ? 3 : 4;
-template <int BOXES>
-constexpr int kRaw = BOXES == 2 ? 4 : 8;
+constexpr uint32_t kRawRing = BOXES == 2 ? 4 : 8;
 constexpr float kLift = 5.f;
-constexpr float kMost = 32768.f;       // of a sum of 32 lifted weights, and so of each: below f16's 65504
-// Tiles whose scales are in shared memory.  Those of tile n are written when the
-// codes of tile n - kRaw / 2 have been converted, into the place of something that
-// was multiplied kStages conversions before; the scores of the tile after that one
-// are issued when its weights are made, and its scales read no more.
+constexpr float kMost = 32768.f;       // of a sum of 64 lifted weights, and so of each: below f16's 65504
+// Tiles whose scales are in shared memory.  Those of tile n are written when
+// codes of tile n - kRawRing / 4 have been converted, into the place of keys that
+// were multiplied two tiles before; those products are issued when the weights of
+// the tile before that are made, and its scales read no more.
 constexpr int kScales = 8;
-static_assert(kRaw<1> / 2 + kStages<1> / 2 + 1 <= kScales && kRaw<2> / 2 + kStages<2> / 2 + 1 <= kScales, "scales are overwritten while they are read");
+static_assert(kRawRing<1> / 4 + 3 <= kScales && kRawRing<2> / 4 + 3 <= kScales, "scales are overwritten while they are read");
 
-// Eight codes in 16 bits each.
-template <typename T>
-__device__ __forceinline__ uint4 codes_to_16(uint2 x);
-// 0x6400 | u is 1024 + u in f16, minus 1152.
-template <>
-__device__ __forceinline__ uint4 codes_to_16<__half>(uint2 x) {
+// Eight codes in f16: 0x6400 | u is 1024 + u, minus 1152.
+__device__ __forceinline__ uint4 codes_to_halves(uint2 x) {
     uint4 r;
     uint32_t* const w = reinterpret_cast<uint32_t*>(&r);
     x.x ^= 0x80808080u;
@@ -76,21 +72,6 @@ __device__ __forceinline__ uint4 codes_to_16<__half>(uint2 x) {
     for (int i = 0; i < 4; ++i) {
         const uint32_t u = __byte_perm(i < 2 ? x.x : x.y, 0x64646464u, i & 1 ? 0x4342 : 0x4140);
         const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&u), __float2half2_rn(1152.f));
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return r;
-}
-// 0x4300 | x is 128 + x in bf16 for x < 128: the code's low seven bits, minus
-// 128, or 256 where its sign is set.
-template <>
-__device__ __forceinline__ uint4 codes_to_16<__nv_bfloat16>(uint2 x) {
-    uint4 r;
-    uint32_t* const w = reinterpret_cast<uint32_t*>(&r);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t u = __byte_perm(i < 2 ? x.x : x.y, 0x43434343u, i & 1 ? 0x4342 : 0x4140);
-        const uint32_t y = u & 0xff7fff7fu, z = u & 0xff80ff80u;
-        const __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&z));
         w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     return r;
@@ -138,7 +119,7 @@ struct Control {
 };
 
 template <int BOXES>
-constexpr size_t kSmem = 1024 + (2 + kStages<BOXES>) * BOXES * kBoxBytes + kRaw<BOXES> * (BOXES * kBoxBytes / 2) + sizeof(Control);
+constexpr size_t kSmem = 1024 + (2 + kRing) * BOXES * kBoxBytes + kRawRing<BOXES> * (BOXES * kBoxBytes / 4) + sizeof(Control);
 
 // The piece of a segment from its unit `from` on; its first kStart units
 // stand for no tiles.
@@ -329,15 +310,15 @@ __device__ __noinline__ float2 weights_with_care(uint32_t s_at, uint32_t o_at, i
     return make_float2(next, state.y);
 }
 
-template <typename T, int BOXES>
+template <int BOXES>
 __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ SharedArgs a) {
     extern __shared__ unsigned char raw_smem[];
     unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t{1023});
-    constexpr int kTileBytes = BOXES * kBoxBytes, kRawBytes = kTileBytes / 2;
-    constexpr uint32_t kRing = kStages<BOXES>, kRawRing = kRaw<BOXES>;
+    constexpr int kTileBytes = BOXES * kBoxBytes, kRawBytes = kTileBytes / 4;
+    constexpr uint32_t kRaw = kRawRing<BOXES>;
     unsigned char* const ring = smem + 2 * kTileBytes;
     unsigned char* const raw = ring + kRing * kTileBytes;             // codes
-    Control& ctl = *reinterpret_cast<Control*>(raw + kRawRing * kRawBytes);
+    Control& ctl = *reinterpret_cast<Control*>(raw + kRaw * kRawBytes);
     const bs_shared_attention_desc& d = a.d;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hkv = a.c.kv_heads, dim = a.c.dim, block = a.c.block;
 
@@ -359,10 +340,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         }
         barrier_init(&ctl.done, 1);
         for (uint32_t s = 0; s < kRing; ++s) {
-            barrier_init(&ctl.full[s], kConverters);
+            barrier_init(&ctl.full[s], 2 * kConverters);
             barrier_init(&ctl.empty[s], 1);
         }
-        for (uint32_t s = 0; s < kRawRing; ++s) {
+        for (uint32_t s = 0; s < kRaw; ++s) {
             barrier_init(&ctl.raw_full[s], 1);
             barrier_init(&ctl.raw_empty[s], kConverters);
         }
@@ -412,15 +393,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         // ---------------------------------------------------- matrix products
         // (the whole warp runs the loop, one elected lane issues)
         constexpr uint32_t kCommon = 1u << 4 | static_cast<uint32_t>(kRows >> 4) << 24;
-        constexpr uint32_t kScores = kCommon | Type16<T>::kFormat << 7 | Type16<T>::kFormat << 10;
-        const uint32_t what_o = kCommon | 1u << 16 | (dim >> 3) << 17;         // f16 by f16, values not along the contraction
+        const uint32_t what_o = kCommon | 1u << 16 | (dim >> 3) << 17;         // (values do not lie along the contraction)
         const int steps = dim / 16;
         const uint64_t q_base = operand(smem_addr(smem), 16, 1024), k_base = operand(smem_addr(ring), 16, 1024);
         const uint64_t v_base = operand(smem_addr(ring), kBoxBytes, 1024);
         constexpr uint32_t kTileUnits = kTileBytes / 16, kBoxUnits = kBoxBytes / 16;
         auto scores = [&](int t, uint32_t stage, uint32_t cols) {
             const uint64_t q = q_base + t * kTileUnits, k = k_base + stage * kTileUnits;
-            const uint32_t what = kScores | (cols >> 3) << 17;
+            const uint32_t what = kCommon | (cols >> 3) << 17;
 #pragma unroll
             for (int i = 0; i < 4 * BOXES; ++i) {
                 const uint32_t off = (i >> 2) * kBoxUnits + (i & 3) * 2;
@@ -458,8 +438,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
             for (uint32_t j = first; j < end; ++j, ++tiles) {
                 const uint32_t stage = (2 * tiles + 1) % kRing, next = (2 * tiles + 2) % kRing;
                 const bool last = j + 1 == end;
-                full(2 * tiles + 1);
                 if (stopped()) break;
+                full(2 * tiles + 1);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     if (t && !both) break;
@@ -494,8 +474,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         __syncwarp();
     } else if (warp == kCopier) {
         // ------------------------------------------------------------ copies
-        // (a lane for every 16 tokens of a tile, the first of each block copies it)
-        const uint32_t per_block = block >> 4, bytes = block * dim;
+        // (a lane for every 16 tokens of a tile, the first of each block or, of a
+        // block of 128, of its halves copies it)
+        const uint32_t run = block < 64 ? block : 64, bytes = run * dim;
         uint32_t tiles = 0, loads = 0, items = 0;
         Piece p;
         p.left = share_first(w, n, blockIdx.x + 1) - share_first(w, n, blockIdx.x);
@@ -516,29 +497,38 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
             const int32_t* const table = d.shared_table + static_cast<uint64_t>(p.m) * d.shared_width;
             auto there = [&](uint32_t j) { return lane < 8 && j * kTileTokens + lane * 16 < p.g.tokens; };
             auto id_at = [&](uint32_t j) { return there(j) ? static_cast<uint32_t>(table[(j * kTileTokens + lane * 16) >> a.block_log2]) : kNoNode; };
-            uint32_t next = id_at(p.t);
+            auto scale_of = [&](uint32_t id) {
+                const uint64_t slab = static_cast<uint64_t>(id) * hkv + h;
+                return id < a.c.num_blocks ? make_float2(a.c.k_scale[slab], a.c.v_scale[slab]) : make_float2(0.f, 0.f);
+            };
+            // (asked for ahead: ids two tiles, scales one)
+            uint32_t next = id_at(p.t), later = p.t + 1 < p.end ? id_at(p.t + 1) : kNoNode;
+            float2 next_scale = scale_of(next);
             for (uint32_t j = p.t; j < p.end && !stopped(); ++j, ++tiles) {
                 const uint32_t id = next;
-                if (j + 1 < p.end) next = id_at(j + 1);
+                const float2 scale = next_scale;
+                next = later;
+                next_scale = scale_of(next);
+                later = j + 2 < p.end ? id_at(j + 2) : kNoNode;
                 const bool ok = id < a.c.num_blocks;
-                const uint32_t copies = __ballot_sync(kFull, ok && lane % per_block == 0), missing = __ballot_sync(kFull, there(j) && !ok);
+                const bool copies = ok && (lane & ((run >> 4) - 1)) == 0;
+                const uint32_t copied = __ballot_sync(kFull, copies), missing = __ballot_sync(kFull, there(j) && !ok);
                 if (missing && lane == 0) atomicOr(a.errors, kMemErrBlock);
-                const uint64_t slab = static_cast<uint64_t>(id) * hkv + h;
-                const float2 scale = ok ? make_float2(a.c.k_scale[slab], a.c.v_scale[slab]) : make_float2(0.f, 0.f);
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    const uint32_t stage = loads % kRawRing;
-                    wait(&ctl.raw_empty[stage], (loads / kRawRing & 1) ^ 1);
+                const uint64_t from = ((static_cast<uint64_t>(id) * hkv + h) * block + (lane * 16 & (block - 1))) * dim;
+#pragma unroll 1
+                for (int u = 0; u < 4; ++u) {          // halves of keys, halves of values
+                    const uint32_t stage = loads % kRaw, half = u & 1;
+                    wait(&ctl.raw_empty[stage], (loads / kRaw & 1) ^ 1);
                     if (stopped()) break;
-                    if (kv == 0) {
+                    if (u == 0) {
                         if (lane < 8) ctl.scales[tiles % kScales][lane] = scale;
                         if (lane == 0) ctl.missing[tiles % kScales] = missing;
                         __syncwarp();
                     }
-                    if (lane == 0) barrier_expect(&ctl.raw_full[stage], __popc(copies) * bytes);
+                    if (lane == 0) barrier_expect(&ctl.raw_full[stage], __popc(copied >> 4 * half & 15) * bytes);
                     __syncwarp();
-                    if (ok && lane % per_block == 0)
-                        copy_bulk(raw + stage * kRawBytes + lane * 16 * dim, (kv ? a.c.v : a.c.k) + slab * bytes, bytes, &ctl.raw_full[stage]);
+                    if (copies && lane >> 2 == half)
+                        copy_bulk(raw + stage * kRawBytes + (lane & 3) * 16 * dim, (u < 2 ? a.c.k : a.c.v) + from, bytes, &ctl.raw_full[stage]);
                     ++loads;
                 }
             }
@@ -550,8 +540,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         }
         // no copy may be in flight when the block ends
         if (lane == 0)
-            for (uint32_t i = loads > kRawRing ? loads - kRawRing : 0; i < loads; ++i)
-                for (unsigned x = 0; x < kPolls && !barrier_test(&ctl.raw_full[i % kRawRing], i / kRawRing & 1); ++x) {}
+            for (uint32_t i = loads > kRaw ? loads - kRaw : 0; i < loads; ++i)
+                for (unsigned x = 0; x < kPolls && !barrier_test(&ctl.raw_full[i % kRaw], i / kRaw & 1); ++x) {}
         __syncwarp();
     } else if (warp >= 8) {
         // --------------------------------------------------------- conversion
@@ -560,25 +550,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         // the units that eight lanes store fall on all banks)
         const uint32_t who = threadIdx.x - 256, nw = dim / 16;
         constexpr int kWorkers = 32 * kConverters;
-        constexpr int kEach = (kRows * 4 * BOXES + kWorkers - 1) / kWorkers;     // 16 codes of a thread, of keys and of values
+        constexpr int kEach = (kRows / 2 * 4 * BOXES + kWorkers - 1) / kWorkers;       // 16 codes of a thread, of a half
         uint32_t from[kEach], to[kEach];
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const uint32_t u = who + kWorkers * i, r = u / nw, x = u % nw, later = x >> 2;      // of 128 * nw
+            const uint32_t u = who + kWorkers * i, r = u / nw, x = u % nw, later = x >> 2;      // of 64 * nw
             from[i] = u * 16 + later * 8;
             to[i] = later * kBoxBytes + r * 128 + (((2 * (x & 3)) ^ (r & 7)) ^ later) * 16;
         }
-        const uint32_t mine = kRows * nw > who ? (kRows * nw - who + kWorkers - 1) / kWorkers : 0;
+        const uint32_t mine = kRows / 2 * nw > who ? (kRows / 2 * nw - who + kWorkers - 1) / kWorkers : 0;
         uint32_t tiles = 0;
-        // the next tile's codes of keys (kv 0) or values (1)
-        auto convert = [&](int kv) {
-            const uint32_t load = 2 * tiles + kv, at = load % kRawRing, stage = load % kRing;
+        // the next tile's codes: halves of keys (0, 1) and of values
+        auto convert = [&](uint32_t u) {
+            const uint32_t load = 4 * tiles + u, at = load % kRaw, stage = load / 2 % kRing;
             const unsigned char* const codes = raw + at * kRawBytes;
-            unsigned char* const tile = ring + stage * kTileBytes;
-            wait(&ctl.raw_full[at], load / kRawRing & 1);
-            wait(&ctl.empty[stage], (load / kRing & 1) ^ 1);
+            unsigned char* const tile = ring + stage * kTileBytes + (u & 1) * (kRows / 2 * 128);
+            if (!(u & 1)) wait(&ctl.empty[stage], (load / 2 / kRing & 1) ^ 1);
+            wait(&ctl.raw_full[at], load / kRaw & 1);
             if (stopped()) return false;
-            const uint32_t missing = ctl.missing[tiles % kScales];
+            const uint32_t missing = ctl.missing[tiles % kScales] >> 4 * (u & 1) & 15;
             uint2 x[kEach][2];
 #pragma unroll
             for (int i = 0; i < kEach; ++i)
@@ -594,8 +584,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
 #pragma unroll
             for (int i = 0; i < kEach; ++i)
                 if (i < static_cast<int>(mine)) {
-                    *reinterpret_cast<uint4*>(tile + to[i]) = kv ? codes_to_16<__half>(x[i][0]) : codes_to_16<T>(x[i][0]);
-                    *reinterpret_cast<uint4*>(tile + (to[i] ^ 16)) = kv ? codes_to_16<__half>(x[i][1]) : codes_to_16<T>(x[i][1]);
+                    *reinterpret_cast<uint4*>(tile + to[i]) = codes_to_halves(x[i][0]);
+                    *reinterpret_cast<uint4*>(tile + (to[i] ^ 16)) = codes_to_halves(x[i][1]);
                 }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
@@ -610,8 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
             if (stopped() || !m.valid) break;
             const uint32_t past = tiles + m.end - m.t;
             item_read(it);
-            for (; tiles < past; ++tiles)
-                if (!convert(0) || !convert(1)) break;
+            for (uint32_t u = 0; tiles < past && convert(u); u = (u + 1) & 3) tiles += u == 3;
             if (tiles < past) break;
         }
     } else {
@@ -642,6 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
             // The warp's queries, a row's units to lanes side by side.  (As little code
             // as can be: what a warp executes for the first time takes 230 clocks for
             // eight instructions.)
+            float row_scale = 1.f;
             {
                 constexpr uint32_t kLanes = 8 * BOXES, kAtOnce = 32 / kLanes;
                 const uint32_t c = lane % kLanes;
@@ -658,6 +648,30 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                                  : "memory");
                 }
                 asm volatile("cp.async.wait_all;\n" ::: "memory");
+                __syncwarp();
+                if (d.dtype != BS_F16) {
+                    // a lane's own row times 2^e with its largest in [2^12, 2^13); rows of zeros, infinities and NaN as they are
+                    auto unit_at = [&](uint32_t x) { return reinterpret_cast<uint4*>(tile + (x >> 3) * kBoxBytes + row * 128 + ((x ^ row) & 7) * 16); };
+                    uint32_t high = 0;       // magnitudes of bf16 order as integers
+#pragma unroll 2
+                    for (uint32_t x = 0; x < dim / 8; ++x) {
+                        const uint4 w = *unit_at(x);
+                        high = __vmaxu2(high, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
+                    }
+                    high = max(high >> 16, high & 0xffffu);
+                    uint32_t e = high >> 7;  // biased exponent
+                    e = high == 0 || e == 255 ? 139 : e < 13 ? 13 : e;
+                    const float up = __uint_as_float((266 - e) << 23);
+                    row_scale = __uint_as_float((e - 12) << 23);
+#pragma unroll 2
+                    for (uint32_t x = 0; x < dim / 8; ++x) {
+                        uint4 u = *unit_at(x);
+                        uint32_t* const w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) w[k] = Type16<__half>::pack(__uint_as_float(w[k] << 16) * up, __uint_as_float(w[k] & 0xffff0000u) * up);
+                        *unit_at(x) = u;
+                    }
+                }
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 __syncwarp();
                 if (lane == 0) barrier_arrive(&ctl.q_full[t]);
@@ -675,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) unit = fmaxf(unit, __shfl_xor_sync(kFull, unit, o));
             if (!(unit > 0.f)) unit = 1.f;
-            const float k_by = d.scale * 1.4426950408889634f, v_by = 1.f / unit;
+            const float k_by = d.scale * 1.4426950408889634f * row_scale, v_by = 1.f / unit;
             float top = -INFINITY, sum = 0.f;       // top: in log2 units, moved when weights are past 2^8
             for (uint32_t j = first; j < end; ++j, ++tiles) {
                 wait(&ctl.s_full[t], s_used++ & 1);        // and the value product before it is done
@@ -743,11 +757,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
     if (warp == kIssuer) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
 }
 
-template <typename T, int BOXES>
+template <int BOXES>
 cudaError_t launch(const SharedArgs& a, cudaStream_t stream) {
-    const cudaError_t e = cudaFuncSetAttribute(k_shared<T, BOXES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<BOXES>);
+    const cudaError_t e = cudaFuncSetAttribute(k_shared<BOXES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<BOXES>);
     if (e != cudaSuccess) return e;
-    return launch_after(k_shared<T, BOXES>, dim3(a.shares), kThreads, kSmem<BOXES>, stream, a);
+    return launch_after(k_shared<BOXES>, dim3(a.shares), kThreads, kSmem<BOXES>, stream, a);
 }
 
 }  // namespace
@@ -755,8 +769,7 @@ cudaError_t launch(const SharedArgs& a, cudaStream_t stream) {
 cudaError_t launch_shared_part(const SharedArgs& given, cudaStream_t stream) {
     SharedArgs a = given;
     a.polls = wait_polls();
-    if (a.d.dtype == BS_F16) return a.c.dim <= 64 ? launch<__half, 1>(a, stream) : launch<__half, 2>(a, stream);
-    return a.c.dim <= 64 ? launch<__nv_bfloat16, 1>(a, stream) : launch<__nv_bfloat16, 2>(a, stream);
+    return a.c.dim <= 64 ? launch<1>(a, stream) : launch<2>(a, stream);
 }
 
 }  // namespace bsb

@@ -96,6 +96,106 @@ def test_rows(seqs, hq, hkv, queries):
     check(*case(3, [seqs], [901], lens, hq, hkv, 32, 128, queries, BF16), [seqs], [901], lens)
 
 
+# Many sequences: what they share is multiplied for all of them at once.
+
+@pytest.mark.parametrize("dim", [16, 32, 48, 64, 80, 96, 112, 128])
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_dimensions_of_many_sequences(dim, block, dtype):
+    groups, shared, lens = [250, 50], [700, 1329], [(7 * i) % 20 for i in range(300)]
+    check(*case(19, groups, shared, lens, 6, 3, block, dim, 1, dtype), groups, shared, lens)
+
+
+@pytest.mark.parametrize("groups,shared", [([300], [1]), ([300], [128]), ([300], [129]), ([300], [2049]), ([31, 33, 32, 200], [513, 2000, 640, 5000]),
+                                           ([1] * 10 + [290], [3000] * 10 + [777]), ([150, 0, 150], [999, 50, 0]), ([64, 65, 128, 129], [1500] * 4)])
+@pytest.mark.parametrize("dtype,hq,hkv,block,dim,queries", [(F16, 4, 2, 16, 64, 1), (BF16, 8, 2, 64, 128, 1), (BF16, 6, 2, 128, 96, 2)])
+def test_groups_of_many_sequences(groups, shared, dtype, hq, hkv, block, dim, queries):
+    lens = [(11 * i) % 30 for i in range(sum(groups))]
+    check(*case(20, groups, shared, lens, hq, hkv, block, dim, queries, dtype), groups, shared, lens)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_scales_and_maxima_of_many_sequences(dtype):
+    # flat and peaked scores, scales of 0 and of all sizes, scores that grow from tile to tile, blocks that are not there
+    groups, shared, lens = [200, 100], [2500, 3001], [(3 * i) % 10 for i in range(300)]
+    for spread in (0.0, 1.0, 6.0):
+        pool, shared_table, table, q = case(21, groups, shared, lens, 8, 2, 64, 128, 1, dtype, spread)
+        for col, factor in ((3, 0), (5, 1e4), (6, 1e-6)):
+            pool[3][shared_table[:, col].long()] *= factor
+        pool[2][shared_table[0, 4].long()] = 0
+        one = check(pool, shared_table, table, q, groups, shared, lens)
+        two = check(pool, shared_table, table, q, groups, shared, lens)
+        assert all(torch.equal(a, b) for a, b in zip(one, two))            # the same every time
+    pool, shared_table, table, q = case(22, groups, shared, lens, 4, 1, 16, 64, 1, dtype)
+    for col in range(shared_table.shape[1]):
+        at = shared_table[:, col]
+        pool[2][at[at >= 0].long()] = 1e-5 * 1.08 ** col
+    check(pool, shared_table, table, q, groups, shared, lens)
+    pool, shared_table, table, q = case(23, groups, shared, lens, 8, 2, 32, 64, 1, BF16)
+    check(pool, shared_table, table, (q.float() * 2.0 ** 40).to(BF16), groups, shared, lens, scale=2.0 ** -43)
+    check(pool, shared_table, table, (q.float() * 2.0 ** -60).to(BF16), groups, shared, lens, scale=2.0 ** 57)
+
+
+def test_blocks_that_are_not_there_of_many_sequences():
+    # as if their tokens were not there: the same as a table without them, where they are whole blocks
+    groups, shared, lens = [300], [1500], [5] * 300
+    pool, shared_table, table, q = case(24, groups, shared, lens, 8, 2, 16, 128, 1, BF16)
+    cache = M.TokenCache(*pool)
+    bad = shared_table.clone()
+    bad[0, [0, 1, 2, 3, 4, 5, 6, 7, 9, 40]] = R.i32([-1, 99999, -7, 2 ** 31 - 1, -1, -1, -1, -1, 12345, -2 ** 31])
+    keep = [i for i in range(94) if i not in (0, 1, 2, 3, 4, 5, 6, 7, 9, 40)]
+    out, lse = cache.shared_attention(q, bad, R.i32(shared), R.cu(groups), table, R.i32(lens), with_lse=True)
+    assert M.take_errors() == 2
+    less = shared_table[:, keep].contiguous()
+    ref, ref_lse, weighted, big = reference(pool, less, table, q, groups, [1500 - 160], lens, 128 ** -0.5)
+    assert ((out.double() - ref).abs() <= R.out_bound(ref, weighted, BF16, R.UNIT[F16])).all()
+    assert ((lse.double() - ref_lse).abs() <= R.lse_bound(big)).all()
+
+
+@pytest.mark.parametrize("cu", [[1, 200, 300], [0, 200, 299], [0, 200, 301], [0, 300, 200], [0, -1, 300], [0, 1 << 30, 300], [-5, 200, 300], [0, 0, 0]])
+def test_wrong_lists_of_many_sequences_set_a_bit(cu):
+    groups, shared, lens = [200, 100], [2500, 3001], [2] * 300
+    pool, shared_table, table, q = case(25, groups, shared, lens, 8, 2, 64, 64, 1, F16)
+    M.TokenCache(*pool).shared_attention(q, shared_table, R.i32(shared), R.i32(cu), table, R.i32(lens))
+    assert M.take_errors() & 4
+
+
+def test_lengths_and_groups_that_change_in_a_graph_of_many_sequences():
+    groups, shared, lens = [150, 150], [3000, 3000], [40] * 300
+    pool, shared_table, table, q = case(26, groups, shared, lens, 8, 2, 32, 64, 1, F16)
+    cache = M.TokenCache(*pool)
+    far, near, cu = R.i32(shared), R.i32(lens), R.cu(groups)
+    graph = torch.cuda.CUDAGraph()
+    cache.shared_attention(q, shared_table, far, cu, table, near)
+    with torch.cuda.graph(graph):
+        got = cache.shared_attention(q, shared_table, far, cu, table, near, with_lse=True)
+    for groups, shared in (([10, 290], [130, 2999]), ([300, 0], [2000, 17]), ([150, 150], [0, 0])):
+        lens = [(13 * i) % 41 for i in range(300)]
+        far.copy_(R.i32(shared)), near.copy_(R.i32(lens)), cu.copy_(R.cu(groups))
+        graph.replay()
+        want = check(pool, shared_table, table, q, groups, shared, lens)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_two_streams_of_many_sequences():
+    groups, shared, lens = [150, 150], [3000, 2000], [20] * 300
+    pool, shared_table, table, q = case(27, groups, shared, lens, 8, 2, 32, 128, 1, BF16)
+    cache = M.TokenCache(*pool)
+    args = (shared_table, R.i32(shared), R.cu(groups), table, R.i32(lens))
+    qs = [q, (q.float() * 0.5).to(BF16)]
+    want = [cache.shared_attention(x, *args)[0] for x in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            got[i].append(cache.shared_attention(qs[i], *args, stream=s.cuda_stream)[0])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
 def test_many_groups_and_long_beginnings():
     groups = [1] * 40 + [7, 30, 2]
     shared = [(37 * i) % 400 for i in range(40)] + [9000, 5001, 12800]
@@ -259,7 +359,7 @@ def test_two_streams_at_once():
 
 
 def test_a_wait_that_gives_up_sets_a_bit(monkeypatch):
-    groups, shared, lens = [40], [3000], [3] * 40
+    groups, shared, lens = [300], [3000], [3] * 300           # (few sequences have no wait in their kernel)
     pool, shared_table, table, q = case(18, groups, shared, lens, 8, 2, 32, 128, 1, BF16)
     good = check(pool, shared_table, table, q, groups, shared, lens)
     monkeypatch.setenv("BSEARCH_WAIT_POLLS", "0")
