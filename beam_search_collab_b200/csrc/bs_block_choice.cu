@@ -12,6 +12,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "bs_device.cuh"
 #include "bs_memory.h"
 #include "bs_select.cuh"
@@ -121,29 +123,108 @@ struct ChoiceArgs {
     unsigned int* errors;
 };
 
-constexpr int kChoiceThreads = 256;
+constexpr uint32_t kMostHeld = 8;      // scores of a thread where one block has a row
 
-template <typename T>
-__device__ __forceinline__ float element(const void* p, int64_t i) {
-    return static_cast<float>(static_cast<const T*>(p)[i]);
+// Which of a row's n > count scores stay, by one block with kMostHeld of them in
+// a thread's registers: the m-th largest of the free ones by its digits of 8 bits,
+// then their places by prefix sums.  A row of 1,024 takes 2 us; the cluster's way
+// (bs_select.cuh), with digits of 11 bits for longer rows, 6.
+template <int THREADS>
+struct SmallShared {
+    uint32_t count[4][256];
+    uint32_t chosen[2];
+};
+template <int THREADS, typename Keep>
+__device__ __forceinline__ void select_small(SmallShared<THREADS>& shared, uint32_t* warp_sums, const uint32_t* keys, uint32_t n, uint32_t sinks,
+                                             uint32_t recent, uint32_t budget, Keep keep) {
+    const uint32_t t = threadIdx.x, lane = t & 31, hi = n - recent;
+    // places side by side: t * each and on
+    const uint32_t each = (n + THREADS - 1) / THREADS;
+    uint32_t key[kMostHeld];
+#pragma unroll
+    for (uint32_t u = 0; u < kMostHeld; ++u) key[u] = u < each && t * each + u < n ? keys[t * each + u] : 0;
+    auto is_free = [&](uint32_t u) { return u < each && t * each + u >= sinks && t * each + u < hi; };
+    for (uint32_t i = t; i < 4 * 256; i += THREADS) (&shared.count[0][0])[i] = 0;
+    __syncthreads();
+    uint32_t need = budget - sinks - recent, prefix = 0;
+    const bool any = need > 0;
+#pragma unroll 1
+    for (int pass = 0; any && pass < 4; ++pass) {
+        const int shift = 24 - 8 * pass;
+#pragma unroll
+        for (uint32_t u = 0; u < kMostHeld; ++u)
+            if (is_free(u) && (pass == 0 || (key[u] ^ prefix) >> (shift + 8) == 0)) atomicAdd(&shared.count[pass][key[u] >> shift & 255], 1u);
+        __syncthreads();
+        if (t < 32) {                                  // eight bins to a lane, from the largest down
+            uint32_t c[8], sum = 0;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                c[u] = shared.count[pass][255 - (lane * 8 + u)];
+                sum += c[u];
+            }
+            uint32_t up_to = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t up = __shfl_up_sync(kFull, up_to, o);
+                if (lane >= static_cast<uint32_t>(o)) up_to += up;
+            }
+            uint32_t before = up_to - sum;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                if (before < need && need <= before + c[u]) {
+                    shared.chosen[0] = prefix | (255 - (lane * 8 + u)) << shift;
+                    shared.chosen[1] = need - before;
+                }
+                before += c[u];
+            }
+        }
+        __syncthreads();
+        prefix = shared.chosen[0];
+        need = shared.chosen[1];
+    }
+    // of those equal to the threshold the first `need`
+    uint32_t kind[kMostHeld], sum = 0, total;          // 1: stays for certain, 65536: equal
+#pragma unroll
+    for (uint32_t u = 0; u < kMostHeld; ++u) {
+        const uint32_t at = t * each + u;
+        kind[u] = u >= each || at >= n ? 0 : !is_free(u) ? 1 : !any ? 0 : key[u] > prefix ? 1 : key[u] == prefix ? 65536u : 0;
+        sum += kind[u];
+    }
+    const uint32_t before = block_prefix<THREADS>(sum, warp_sums, total);
+    uint32_t to = before & 0xffffu, equal = before >> 16;
+#pragma unroll
+    for (uint32_t u = 0; u < kMostHeld; ++u) {
+        if (kind[u] == 1 || (kind[u] && equal < need)) keep(to + min(equal, need), t * each + u);
+        to += kind[u] & 1;
+        equal += kind[u] >> 16;
+    }
 }
 
 // A cluster of blocks has one row: a query and a key head.  Each block scores
-// its slice of the table's columns, then the rows' largest are found among the
-// scores in shared memory (bs_select.cuh).
-template <typename T>
-__global__ void __launch_bounds__(kChoiceThreads) k_block_choice(const __grid_constant__ ChoiceArgs a, uint32_t cached) {
-    extern __shared__ uint32_t keys[];                     // [cached]
-    __shared__ __align__(16) SelectShared shared;
+// its slice of the table's columns, then the row's largest are found among the
+// scores in shared memory.  SMALL: one block, and at most kMostHeld columns a
+// thread.
+template <typename T, int THREADS, bool SMALL>
+__global__ void __launch_bounds__(THREADS) k_block_choice(const __grid_constant__ ChoiceArgs a, uint32_t cached) {
+    extern __shared__ uint32_t keys[];                     // [cached]: the columns' blocks, then their keys
+    using Shared = std::conditional_t<SMALL, SmallShared<THREADS>, SelectShared>;
+    __shared__ __align__(16) Shared shared;
     __shared__ __align__(16) int16_t parts[2][128];        // positive and negative part of the heads' codes
-    __shared__ float warp_max[kChoiceThreads / 32];
-    constexpr uint32_t kWarps = kChoiceThreads / 32;
+    __shared__ float warp_max[THREADS / 32];
+    __shared__ uint32_t warp_sums[32];
+    constexpr uint32_t kWarps = THREADS / 32;
     cudaGridDependencySynchronize();       // in every block, before anything of the caller's
     const cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t rank = cluster.block_rank(), blocks = cluster.num_blocks();
+    const uint32_t rank = SMALL ? 0 : cluster.block_rank(), blocks = SMALL ? 1 : cluster.num_blocks();
     const bs_block_choice_desc& d = a.d;
     const uint32_t hkv = a.c.kv_heads, group = d.q_heads / hkv, dim = a.c.dim, block = a.c.block;
     const uint32_t h = blockIdx.x / blocks, i = blockIdx.y, b = blockIdx.z, t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    // the heads' elements as codes, added up by sign (asked for with the length)
+    const T* const q = static_cast<const T*>(d.q) + b * d.q_stride[0] + i * d.q_stride[1] + static_cast<int64_t>(h) * group * d.q_stride[2];
+    constexpr uint32_t kHeads = 8;                         // of which a thread keeps the elements
+    float x[kHeads];
+#pragma unroll
+    for (uint32_t g = 0; g < kHeads; ++g) x[g] = t < dim && g < group ? static_cast<float>(q[g * d.q_stride[2] + t]) : 0.f;
     int64_t len = d.lens[b];
     const int64_t most = static_cast<int64_t>(d.table_width) * block;
     if (len < 0 || len > most) {
@@ -154,125 +235,140 @@ __global__ void __launch_bounds__(kChoiceThreads) k_block_choice(const __grid_co
     const uint32_t n = seen > 0 ? static_cast<uint32_t>((seen + block - 1) / block) : 0, count = d.count;
     int32_t* const out = d.blocks + ((static_cast<uint64_t>(b) * d.queries + i) * hkv + h) * count;
     if (n <= count) {                                      // (the whole cluster)
-        for (uint32_t x = rank * kChoiceThreads + t; x < count; x += blocks * kChoiceThreads) out[x] = x < n ? static_cast<int32_t>(x) : -1;
+        for (uint32_t y = rank * THREADS + t; y < count; y += blocks * THREADS) out[y] = y < n ? static_cast<int32_t>(y) : -1;
         return;
     }
-    // the heads' elements as codes, added up by sign
-    const T* const q = static_cast<const T*>(d.q) + b * d.q_stride[0] + i * d.q_stride[1] + static_cast<int64_t>(h) * group * d.q_stride[2];
-    clear_counts<kChoiceThreads>(shared);
+    uint32_t first, size;
+    select_slice(n, blocks, rank, first, size);
+    const int32_t* const table = d.table + static_cast<uint64_t>(b) * d.table_width + first;
+    const uint32_t held = min(size, cached);
+    for (uint32_t col = t; col < held; col += THREADS) {
+        const uint32_t id = table[col];
+        if (id >= a.c.num_blocks) atomicOr(a.errors, kMemErrBlock);
+        keys[col] = id < a.c.num_blocks ? id : kNoNode;
+    }
+    if constexpr (!SMALL) clear_counts<THREADS>(shared);
     float top = 0.f;
+#pragma unroll
+    for (uint32_t g = 0; g < kHeads; ++g) top = fmaxf(top, fabsf(x[g]));
     if (t < dim)
-        for (uint32_t x = 0; x < group; ++x) top = fmaxf(top, fabsf(static_cast<float>(q[x * d.q_stride[2] + t])));
+        for (uint32_t g = kHeads; g < group; ++g) top = fmaxf(top, fabsf(static_cast<float>(q[g * d.q_stride[2] + t])));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
     if (lane == 0) warp_max[warp] = top;
     __syncthreads();
 #pragma unroll
-    for (uint32_t x = 0; x < kWarps; ++x) top = fmaxf(top, warp_max[x]);
+    for (uint32_t w = 0; w < kWarps; ++w) top = fmaxf(top, warp_max[w]);
     const float by = top < 1e-30f ? 0.f : __fdiv_rn(127.f, top);
     if (t < dim) {
         int32_t positive = 0, negative = 0;
-        for (uint32_t x = 0; x < group; ++x) {
-            const int32_t c = __float2int_rn(__fmul_rn(static_cast<float>(q[x * d.q_stride[2] + t]), by));
+        auto add = [&](float y) {
+            const int32_t c = __float2int_rn(__fmul_rn(y, by));
             positive += max(c, 0);
             negative += min(c, 0);
-        }
+        };
+#pragma unroll
+        for (uint32_t g = 0; g < kHeads; ++g) add(x[g]);
+        for (uint32_t g = kHeads; g < group; ++g) add(static_cast<float>(q[g * d.q_stride[2] + t]));
         parts[0][t] = static_cast<int16_t>(positive);      // (at most 128 heads of 127)
         parts[1][t] = static_cast<int16_t>(negative);
     }
     __syncthreads();
 
-    uint32_t first, size;
-    select_slice(n, blocks, rank, first, size);
-    const int32_t* const table = d.table + static_cast<uint64_t>(b) * d.table_width + first;
     // a column's 2 * dim bounds lie side by side: 16 to a lane
     const uint32_t per_col = dim / 8, cols = 32 / per_col, sub = lane / per_col, chunk = lane % per_col;
     int32_t weights[8] = {};
     if (sub < cols) {
 #pragma unroll
-        for (int x = 0; x < 8; ++x) weights[x] = reinterpret_cast<const int32_t*>(&parts[0][0] + (chunk * 16 < dim ? 0 : 128 - dim) + chunk * 16)[x];
+        for (int y = 0; y < 8; ++y) weights[y] = reinterpret_cast<const int32_t*>(&parts[0][0] + (chunk * 16 < dim ? 0 : 128 - dim) + chunk * 16)[y];
     }
-    auto product = [&](const uint4& x) {
-        const int32_t w[4] = {static_cast<int32_t>(x.x), static_cast<int32_t>(x.y), static_cast<int32_t>(x.z), static_cast<int32_t>(x.w)};
+    auto product = [&](const uint4& y) {
+        const int32_t w[4] = {static_cast<int32_t>(y.x), static_cast<int32_t>(y.y), static_cast<int32_t>(y.z), static_cast<int32_t>(y.w)};
         int32_t sum = 0;
 #pragma unroll
         for (int u = 0; u < 4; ++u) sum = __dp2a_hi(weights[2 * u + 1], w[u], __dp2a_lo(weights[2 * u], w[u], sum));
         return sum;
     };
     auto key = [&](int32_t sum, float scale) { return select_key(__fmul_rn(__int2float_rn(sum), scale)); };
-    constexpr uint32_t kBatch = 4;
-    const uint32_t held = min(size, cached);
+    constexpr uint32_t kBatch = 8;                         // columns of a lane whose bounds are on their way together
     for (uint32_t x0 = warp * cols * kBatch; x0 < held; x0 += kWarps * cols * kBatch) {
-        uint4 x[kBatch];
-        uint64_t slab[kBatch];
+        uint4 y[kBatch];
         float scale[kBatch];
 #pragma unroll
         for (uint32_t u = 0; u < kBatch; ++u) {
-            const uint32_t col = x0 + u * cols + sub;
-            const uint32_t id = sub < cols && col < held ? static_cast<uint32_t>(table[col]) : 0u;
-            slab[u] = static_cast<uint64_t>(id) * hkv + h;
-            if (id >= a.c.num_blocks) slab[u] = ~0ull;
+            const uint32_t col = x0 + u * cols + sub, id = sub < cols && col < held ? keys[col] : kNoNode;
+            const uint64_t slab = static_cast<uint64_t>(id) * hkv + h;
+            y[u] = id != kNoNode ? __ldg(reinterpret_cast<const uint4*>(d.bounds + slab * 2 * dim) + chunk) : make_uint4(0, 0, 0, 0);
+            scale[u] = id != kNoNode && chunk == 0 ? a.c.k_scale[slab] : 0.f;
         }
+        __syncwarp();                                      // (the blocks are read: keys take their place)
 #pragma unroll
         for (uint32_t u = 0; u < kBatch; ++u) {
-            const bool ok = slab[u] != ~0ull && sub < cols && x0 + u * cols + sub < held;
-            x[u] = ok ? __ldg(reinterpret_cast<const uint4*>(d.bounds + slab[u] * 2 * dim) + chunk) : make_uint4(0, 0, 0, 0);
-            scale[u] = ok ? a.c.k_scale[slab[u]] : 0.f;
-            if (slab[u] == ~0ull && chunk == 0 && sub < cols) atomicOr(a.errors, kMemErrBlock);
-        }
-#pragma unroll
-        for (uint32_t u = 0; u < kBatch; ++u) {
-            int32_t sum = product(x[u]);
+            int32_t sum = product(y[u]);
 #pragma unroll
             for (uint32_t s = 8; s > 0; s >>= 1) {
-                const int32_t y = __shfl_down_sync(kFull, sum, s);
-                if (chunk + s < per_col) sum += y;
+                const int32_t z = __shfl_down_sync(kFull, sum, s);
+                if (chunk + s < per_col) sum += z;
             }
             const uint32_t col = x0 + u * cols + sub;
             if (chunk == 0 && sub < cols && col < held) keys[col] = key(sum, scale[u]);
         }
     }
     __syncthreads();
-    select_row<kChoiceThreads>(
-        cluster, shared, n, first, size, d.sinks, d.recent, count,
-        [&](uint32_t col) -> uint32_t {
-            if (col < cached) return keys[col];
-            // a row too long for shared memory: scored again, by one thread
-            const uint32_t id = table[col];
-            if (id >= a.c.num_blocks) return key(0, 0.f);
-            const uint64_t slab = static_cast<uint64_t>(id) * hkv + h;
-            int32_t sum = 0;
-            for (uint32_t x = 0; x < 2 * dim; ++x) sum += parts[x >= dim][x < dim ? x : x - dim] * d.bounds[slab * 2 * dim + x];
-            return key(sum, a.c.k_scale[slab]);
-        },
-        [&](uint32_t slot, uint32_t col) { out[slot] = col; });
+    auto keep = [&](uint32_t slot, uint32_t col) { out[slot] = col; };
+    if constexpr (SMALL) {
+        select_small<THREADS>(shared, warp_sums, keys, n, d.sinks, d.recent, count, keep);
+    } else {
+        select_row<THREADS>(
+            cluster, shared, n, first, size, d.sinks, d.recent, count,
+            [&](uint32_t col) -> uint32_t {
+                if (col < cached) return keys[col];
+                // a row too long for shared memory: scored again, by one thread
+                const uint32_t id = table[col];
+                if (id >= a.c.num_blocks) return key(0, 0.f);
+                const uint64_t slab = static_cast<uint64_t>(id) * hkv + h;
+                int32_t sum = 0;
+                for (uint32_t y = 0; y < 2 * dim; ++y) sum += parts[y >= dim][y < dim ? y : y - dim] * d.bounds[slab * 2 * dim + y];
+                return key(sum, a.c.k_scale[slab]);
+            },
+            keep);
+    }
+}
+
+template <typename T, int THREADS, bool SMALL>
+cudaError_t launch_choice(const ChoiceArgs& a, uint32_t cluster, cudaStream_t stream) {
+    const uint32_t slice = ((a.d.table_width + cluster - 1) / cluster + 3) & ~3u, cached = slice < kMostCached ? slice : kMostCached;
+    cudaError_t e = cudaFuncSetAttribute(k_block_choice<T, THREADS, SMALL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostCached * 4);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(a.c.kv_heads * cluster, a.d.queries, a.d.num_seqs);
+    config.blockDim = dim3(THREADS);
+    config.dynamicSmemBytes = cached * 4;
+    config.stream = stream;
+    config.attrs = attr;
+    config.numAttrs = SMALL ? 1 : 2;
+    return cudaLaunchKernelEx(&config, k_block_choice<T, THREADS, SMALL>, a, cached);
 }
 
 template <typename T>
 cudaError_t launch_choice(const bs_token_cache& c, const bs_block_choice_desc& d, const MemoryDevice& dev, cudaStream_t stream) {
     const ChoiceArgs a{c, d, dev.errors};
-    // a row goes to more blocks while they would have over 256 columns each and
-    // the rows alone do not fill the GPU
     const uint64_t rows = static_cast<uint64_t>(c.kv_heads) * d.queries * d.num_seqs;
+    // a block to a row while it holds the row's keys in registers and the rows fill
+    // a good part of the GPU
+    if (d.table_width <= 256) return launch_choice<T, 128, true>(a, 1, stream);
+    if (d.table_width <= 512 * kMostHeld && rows * 3 > static_cast<uint64_t>(dev.num_sms)) return launch_choice<T, 512, true>(a, 1, stream);
+    // else a row goes to more blocks while they would have over 256 columns each
+    // and the rows alone do not fill the GPU
     uint32_t cluster = 1;
     while (cluster < kMostCluster && d.table_width / cluster > 256 && rows * cluster * 2 <= 2u * dev.num_sms) cluster *= 2;
-    const uint32_t slice = ((d.table_width + cluster - 1) / cluster + 3) & ~3u, cached = slice < kMostCached ? slice : kMostCached;
-    cudaError_t e = cudaFuncSetAttribute(k_block_choice<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostCached * 4);
-    if (e != cudaSuccess) return e;
-    cudaLaunchAttribute attr[2] = {};
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(c.kv_heads * cluster, d.queries, d.num_seqs);
-    config.blockDim = dim3(kChoiceThreads);
-    config.dynamicSmemBytes = cached * 4;
-    config.stream = stream;
-    config.attrs = attr;
-    config.numAttrs = 2;
-    return cudaLaunchKernelEx(&config, k_block_choice<T>, a, cached);
+    return launch_choice<T, 256, false>(a, cluster, stream);
 }
 
 }  // namespace
