@@ -357,14 +357,18 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
 }
 
 // Blocks of a segment, by the time of its longest part and of all of them, and
-// that time: a block takes as long as kStart tiles to begin and end, and the join
-// of a cluster some more; a tile takes a block 0.45 us.
-uint32_t parts_of(uint64_t segments, uint64_t tokens, uint64_t resident, double& time) {
-    constexpr double kStart = 6, kJoin = 2;
+// that time, in tiles (0.34 us a block's): a block takes as long as kStart of them
+// to begin and end, and the join of a cluster some more.  Lists are as long as one
+// another, so the blocks go in waves; sequences are taken to have half the tokens
+// that their table has room for.
+uint32_t parts_of(uint64_t segments, uint64_t tokens, uint64_t resident, bool lists, double& time) {
+    constexpr double kStart = 16, kJoin = 2;
     uint32_t best = 1;
     for (uint32_t n = 1; n <= kMostCluster; ++n) {
-        const double waves = static_cast<double>((segments * n + resident - 1) / resident);
-        const double t = waves * (kStart + static_cast<double>(tokens) / kTile / n) + (n > 1 ? kJoin : 0);
+        const double part = static_cast<double>(tokens) / kTile / n, ends = kStart + (n > 1 ? kJoin : 0);
+        const uint64_t blocks = segments * n;
+        const double waves = lists ? static_cast<double>((blocks + resident - 1) / resident) : static_cast<double>(blocks) / resident;
+        const double all = waves * (ends + (lists ? part : part / 2)), t = all > ends + part ? all : ends + part;
         if (n == 1 || t < time) {
             time = t;
             best = n;
@@ -389,7 +393,7 @@ cudaError_t launch_rows(const RowsArgs& a, const MemoryDevice& dev, cudaStream_t
     const uint64_t segments = static_cast<uint64_t>(a.s.c.kv_heads) * (LIST ? a.s.d.queries : 1);
     const uint64_t width = LIST ? a.count : a.s.d.table_width + (a.direct ? a.s.d.shared_width : 0ull);
     double time = 0;
-    const uint32_t parts = parts_of(segments * row_tiles * a.s.d.num_seqs, width * a.s.c.block, resident_blocks(dev, a.rows), time);
+    const uint32_t parts = parts_of(segments * row_tiles * a.s.d.num_seqs, width * a.s.c.block, resident_blocks(dev, a.rows), LIST, time);
     cudaLaunchAttribute attr[2] = {};
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = parts;
@@ -431,15 +435,15 @@ Layout plan(const bs_token_cache& c, const bs_shared_attention_desc& d, const Me
     Layout l{};
     // Few shared tokens or few sequences: each sequence reads them by itself, in
     // the kernel for its own.  The times of both ways, in tiles of that kernel
-    // (0.45 us): the other one takes 14 us for its start, its end and the join, and
+    // (0.34 us): the other one takes 14 us for its start, its end and the join, and
     // 2.6 us for 256 rows over 128 tokens.  (4 sequences over 700 tokens: 8.9 us
     // this way, 20 that way; 64 over 900 to 17,001: 256 and 101.)
     const uint32_t in_sequence = static_cast<uint32_t>(d.q_heads / c.kv_heads) * d.queries;
     const uint64_t segments = own_segments(c, d, in_sequence), resident = resident_blocks(dev, in_sequence);
     const uint64_t own = static_cast<uint64_t>(d.table_width) * c.block;
     double here = 0, there = 0;
-    parts_of(segments, own + static_cast<uint64_t>(d.shared_width) * c.block, resident, here);
-    parts_of(segments, own, resident, there);
+    parts_of(segments, own + static_cast<uint64_t>(d.shared_width) * c.block, resident, false, here);
+    parts_of(segments, own, resident, false, there);
     const uint64_t tiles = (static_cast<uint64_t>(d.shared_width) * c.block + shared::kTileTokens - 1) / shared::kTileTokens;
     if (tiles == 0) return l;
     const uint64_t rows = static_cast<uint64_t>(d.num_seqs) * d.queries * d.q_heads;
@@ -447,7 +451,7 @@ Layout plan(const bs_token_cache& c, const bs_shared_attention_desc& d, const Me
     const uint64_t pairs = rows / c.kv_heads / shared::kPairRows + std::min(d.num_groups, d.num_seqs);
     const uint64_t units = pairs * c.kv_heads * (tiles + shared::kStart), most = (units + 2 * shared::kStart - 1) / (2 * shared::kStart);
     l.shares = static_cast<uint32_t>(most < static_cast<uint64_t>(dev.num_sms) ? most : dev.num_sms);
-    there += (14 + 2.6 * static_cast<double>(units) / l.shares) / 0.45;
+    there += (14 + 2.6 * static_cast<double>(units) / l.shares) / 0.34;
     if (here <= there) {
         l.shares = 0;
         return l;
