@@ -12,7 +12,7 @@
 // Every row sees every token, but for the end of the last tile.
 //
 // Warps 0-3 and 4-7 are the softmax of tile 0 and 1 (a thread has one row),
-// 8-13 convert keys and values, 14 issues the matrix instructions, 15 finds the
+// 8-11 convert keys and values, 12 issues the matrix instructions, 13 finds the
 // pieces of the share and copies codes (a bulk copy for each block) and scales to
 // shared memory:
 //   S_t = Q_t K^T     codes of K exact in f16, as are bf16 queries times a power
@@ -43,24 +43,29 @@ using namespace tc;
 
 namespace {
 
-constexpr int kConverters = 6;         // warps
+constexpr int kConverters = 4;         // warps
 constexpr int kIssuer = 8 + kConverters;
 constexpr int kCopier = kIssuer + 1;
 constexpr int kThreads = 32 * (kCopier + 1);
 // Rings of converted tiles (keys and values in turn: a tile's values and the next
 // one's keys are in use together, meanwhile the next ones are converted) and of
-// halves of tiles of codes, of which four take the 1.2 us that a copy takes.
+// quarters of tiles of codes.  A quarter is one warp's, the same of every tile (a
+// barrier's parity tells a phase from the one before it, not from the one before
+// that, so whoever waits for one has to wait for each): with all warps on each part
+// of a tile their barriers took a third of the time.
 constexpr uint32_t kRing = 4;
+constexpr uint32_t kQuarter = kRows / 4;
 template <int BOXES>
-constexpr uint32_t kRawRing = BOXES == 2 ? 4 : 8;
+constexpr uint32_t kRawRing = BOXES == 2 ? 8 : 16;
 constexpr float kLift = 5.f;
 constexpr float kMost = 32768.f;       // of a sum of 64 lifted weights, and so of each: below f16's 65504
 // Tiles whose scales are in shared memory.  Those of tile n are written when
-// codes of tile n - kRawRing / 4 have been converted, into the place of keys that
+// codes of tile n - kRawRing / 8 have been converted, into the place of keys that
 // were multiplied two tiles before; those products are issued when the weights of
 // the tile before that are made, and its scales read no more.
 constexpr int kScales = 8;
-static_assert(kRawRing<1> / 4 + 3 <= kScales && kRawRing<2> / 4 + 3 <= kScales, "scales are overwritten while they are read");
+static_assert(kConverters * kQuarter == kRows, "a quarter for each warp");
+static_assert(kRawRing<1> / 8 + 3 <= kScales && kRawRing<2> / 8 + 3 <= kScales, "scales are overwritten while they are read");
 
 // Eight codes in f16: 0x6400 | u is 1024 + u, minus 1152.
 __device__ __forceinline__ uint4 codes_to_halves(uint2 x) {
@@ -83,6 +88,16 @@ __device__ __forceinline__ void copy_bulk(void* dst, const void* src, unsigned b
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_addr(dst)), "l"(src),
                  "r"(bytes), "r"(smem_addr(bar))
                  : "memory");
+}
+
+// Whether a phase is over, without a wait (lanes may ask of barriers of their own).
+__device__ __forceinline__ bool barrier_done(uint64_t* b, unsigned phase) {
+    unsigned ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok)
+                 : "r"(smem_addr(b)), "r"(phase)
+                 : "memory");
+    return ok != 0;
 }
 
 // Where a block is in its share: tiles t .. end of a segment (group m, key
@@ -108,7 +123,7 @@ struct Item {
 
 struct Control {
     uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
-    uint64_t full[4], empty[4], raw_full[8], raw_empty[8];
+    uint64_t full[kRing], empty[kRing], raw_full[16], raw_empty[16];
     uint64_t item_full[2], item_empty[2];
     Item item[2];
     uint64_t sums[2 * (kCopier + 1)];
@@ -119,7 +134,7 @@ struct Control {
 };
 
 template <int BOXES>
-constexpr size_t kSmem = 1024 + (2 + kRing) * BOXES * kBoxBytes + kRawRing<BOXES> * (BOXES * kBoxBytes / 4) + sizeof(Control);
+constexpr size_t kSmem = 1024 + (2 + kRing) * BOXES * kBoxBytes + kRawRing<BOXES> * (BOXES * kBoxBytes / 8) + sizeof(Control);
 
 // The piece of a segment from its unit `from` on; its first kStart units
 // stand for no tiles.
@@ -314,7 +329,7 @@ template <int BOXES>
 __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ SharedArgs a) {
     extern __shared__ unsigned char raw_smem[];
     unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t{1023});
-    constexpr int kTileBytes = BOXES * kBoxBytes, kRawBytes = kTileBytes / 4;
+    constexpr int kTileBytes = BOXES * kBoxBytes, kRawBytes = kTileBytes / 8;
     constexpr uint32_t kRaw = kRawRing<BOXES>;
     unsigned char* const ring = smem + 2 * kTileBytes;
     unsigned char* const raw = ring + kRing * kTileBytes;             // codes
@@ -340,12 +355,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         }
         barrier_init(&ctl.done, 1);
         for (uint32_t s = 0; s < kRing; ++s) {
-            barrier_init(&ctl.full[s], 2 * kConverters);
+            barrier_init(&ctl.full[s], 4);
             barrier_init(&ctl.empty[s], 1);
         }
         for (uint32_t s = 0; s < kRaw; ++s) {
             barrier_init(&ctl.raw_full[s], 1);
-            barrier_init(&ctl.raw_empty[s], kConverters);
+            barrier_init(&ctl.raw_empty[s], 1);
         }
         ctl.gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -474,10 +489,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         __syncwarp();
     } else if (warp == kCopier) {
         // ------------------------------------------------------------ copies
-        // (a lane for every 16 tokens of a tile, the first of each block or, of a
-        // block of 128, of its halves copies it)
-        const uint32_t run = block < 64 ? block : 64, bytes = run * dim;
-        uint32_t tiles = 0, loads = 0, items = 0;
+        // (lanes 0-7 look up every 16 tokens of a tile, and copy its quarters of keys
+        // and of values, each when there is room for it: one after the other, with
+        // the whole warp, took 700 clocks each)
+        const uint32_t run = block < kQuarter ? block : kQuarter, bytes = run * dim, quarter = lane & 3;
+        uint32_t tiles = 0, items = 0, copied = 0;     // copied: quarters by this lane
         Piece p;
         p.left = share_first(w, n, blockIdx.x + 1) - share_first(w, n, blockIdx.x);
         find_piece(a, p, share_first(w, n, blockIdx.x));
@@ -511,25 +527,38 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                 next_scale = scale_of(next);
                 later = j + 2 < p.end ? id_at(j + 2) : kNoNode;
                 const bool ok = id < a.c.num_blocks;
-                const bool copies = ok && (lane & ((run >> 4) - 1)) == 0;
-                const uint32_t copied = __ballot_sync(kFull, copies), missing = __ballot_sync(kFull, there(j) && !ok);
+                const uint32_t missing = __ballot_sync(kFull, there(j) && !ok);
                 if (missing && lane == 0) atomicOr(a.errors, kMemErrBlock);
-                const uint64_t from = ((static_cast<uint64_t>(id) * hkv + h) * block + (lane * 16 & (block - 1))) * dim;
-#pragma unroll 1
-                for (int u = 0; u < 4; ++u) {          // halves of keys, halves of values
-                    const uint32_t stage = loads % kRaw, half = u & 1;
-                    wait(&ctl.raw_empty[stage], (loads / kRaw & 1) ^ 1);
-                    if (stopped()) break;
-                    if (u == 0) {
-                        if (lane < 8) ctl.scales[tiles % kScales][lane] = scale;
-                        if (lane == 0) ctl.missing[tiles % kScales] = missing;
-                        __syncwarp();
+                // this lane's quarter: a run of a block, or two blocks of 16
+                const uint32_t one = __shfl_sync(kFull, id, 2 * quarter), two = run < kQuarter ? __shfl_sync(kFull, id, 2 * quarter + 1) : kNoNode;
+                const uint32_t load = 8 * tiles + lane, stage = load % kRaw;
+                wait(&ctl.raw_empty[8 * tiles % kRaw], (8 * tiles / kRaw & 1) ^ 1);
+                if (stopped()) break;
+                if (lane < 8) ctl.scales[tiles % kScales][lane] = scale;
+                if (lane == 0) ctl.missing[tiles % kScales] = missing;
+                __syncwarp();
+                bool waits = lane < 8;
+                for (unsigned i = 0; i < a.polls && __any_sync(kFull, waits); ++i) {
+                    if (waits && barrier_done(&ctl.raw_empty[stage], (load / kRaw & 1) ^ 1)) {
+                        waits = false;
+                        const bool first = one < a.c.num_blocks, second = two < a.c.num_blocks;
+                        barrier_expect(&ctl.raw_full[stage], (first + second) * bytes);
+                        const int8_t* const codes = lane < 4 ? a.c.k : a.c.v;
+                        unsigned char* const to = raw + stage * kRawBytes;
+                        auto from = [&](uint32_t x) { return codes + ((static_cast<uint64_t>(x) * hkv + h) * block + (quarter * kQuarter & (block - 1))) * dim; };
+                        if (first) copy_bulk(to, from(one), bytes, &ctl.raw_full[stage]);
+                        if (second) copy_bulk(to + 16 * dim, codes + (static_cast<uint64_t>(two) * hkv + h) * bytes, bytes, &ctl.raw_full[stage]);
+                        copied += 1;
                     }
-                    if (lane == 0) barrier_expect(&ctl.raw_full[stage], __popc(copied >> 4 * half & 15) * bytes);
+                    if (i % 64 == 63 && stopped()) break;
+                }
+                if (__any_sync(kFull, waits)) {            // (the others' wait has given up, or this one does)
+                    if (lane == 0 && !*gave_up) {
+                        *gave_up = 1;
+                        atomicOr(a.errors, kMemErrWait);
+                    }
                     __syncwarp();
-                    if (copies && lane >> 2 == half)
-                        copy_bulk(raw + stage * kRawBytes + (lane & 3) * 16 * dim, (u < 2 ? a.c.k : a.c.v) + from, bytes, &ctl.raw_full[stage]);
-                    ++loads;
+                    break;
                 }
             }
         }
@@ -538,52 +567,51 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
             ctl.item[items & 1].valid = 0;
             barrier_arrive(&ctl.item_full[items & 1]);
         }
-        // no copy may be in flight when the block ends
-        if (lane == 0)
-            for (uint32_t i = loads > kRaw ? loads - kRaw : 0; i < loads; ++i)
-                for (unsigned x = 0; x < kPolls && !barrier_test(&ctl.raw_full[i % kRaw], i / kRaw & 1); ++x) {}
+        // no copy may be in flight when the block ends: this lane's last ones
+        for (uint32_t i = copied > kRaw / 8 ? copied - kRaw / 8 : 0; i < copied; ++i) {
+            const uint32_t load = 8 * i + lane;
+            for (unsigned x = 0; x < kPolls && !barrier_test(&ctl.raw_full[load % kRaw], load / kRaw & 1); ++x) {}
+        }
         __syncwarp();
     } else if (warp >= 8) {
         // --------------------------------------------------------- conversion
-        // (16 codes side by side to a lane, the next 16 to the next; of a row of
-        // 128, lanes of the upper half take their second eight first, so that
-        // the units that eight lanes store fall on all banks)
-        const uint32_t who = threadIdx.x - 256, nw = dim / 16;
-        constexpr int kWorkers = 32 * kConverters;
-        constexpr int kEach = (kRows / 2 * 4 * BOXES + kWorkers - 1) / kWorkers;       // 16 codes of a thread, of a half
+        // (a warp has a quarter; 16 codes side by side to a lane, the next
+        // 16 to the next; of a row of 128, lanes of the upper half take their second
+        // eight first, so that the units that eight lanes store fall on all banks)
+        const uint32_t nw = dim / 16;
+        constexpr int kEach = 4 * BOXES;                     // 16 codes of a lane, of a quarter
         uint32_t from[kEach], to[kEach];
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const uint32_t u = who + kWorkers * i, r = u / nw, x = u % nw, later = x >> 2;      // of 64 * nw
+            const uint32_t u = lane + 32 * i, r = u / nw, x = u % nw, later = x >> 2;      // of 32 * nw
             from[i] = u * 16 + later * 8;
             to[i] = later * kBoxBytes + r * 128 + (((2 * (x & 3)) ^ (r & 7)) ^ later) * 16;
         }
-        const uint32_t mine = kRows / 2 * nw > who ? (kRows / 2 * nw - who + kWorkers - 1) / kWorkers : 0;
-        uint32_t tiles = 0;
-        // the next tile's codes: halves of keys (0, 1) and of values
-        auto convert = [&](uint32_t u) {
-            const uint32_t load = 4 * tiles + u, at = load % kRaw, stage = load / 2 % kRing;
+        // load 8 i + u: tile i's quarters of keys (u < 4) and of values
+        const uint32_t quarter = warp - 8;
+        auto convert = [&](uint32_t load) {
+            const uint32_t at = load % kRaw, stage = load / 4 % kRing;
             const unsigned char* const codes = raw + at * kRawBytes;
-            unsigned char* const tile = ring + stage * kTileBytes + (u & 1) * (kRows / 2 * 128);
-            if (!(u & 1)) wait(&ctl.empty[stage], (load / 2 / kRing & 1) ^ 1);
+            unsigned char* const tile = ring + stage * kTileBytes + quarter * (kQuarter * 128);
+            wait(&ctl.empty[stage], (load / 4 / kRing & 1) ^ 1);
             wait(&ctl.raw_full[at], load / kRaw & 1);
             if (stopped()) return false;
-            const uint32_t missing = ctl.missing[tiles % kScales] >> 4 * (u & 1) & 15;
+            const uint32_t missing = ctl.missing[load / 8 % kScales] >> 2 * quarter & 3;
             uint2 x[kEach][2];
 #pragma unroll
             for (int i = 0; i < kEach; ++i)
-                if (i < static_cast<int>(mine)) {
+                if (i < static_cast<int>(nw)) {
                     x[i][0] = *reinterpret_cast<const uint2*>(codes + from[i]);
                     x[i][1] = *reinterpret_cast<const uint2*>(codes + (from[i] ^ 8));
                 }
             if (missing) {
 #pragma unroll
                 for (int i = 0; i < kEach; ++i)
-                    if (missing >> ((who + kWorkers * i) / nw / 16) & 1) x[i][0] = x[i][1] = make_uint2(0, 0);
+                    if (missing >> ((lane + 32 * i) / nw / 16) & 1) x[i][0] = x[i][1] = make_uint2(0, 0);
             }
 #pragma unroll
             for (int i = 0; i < kEach; ++i)
-                if (i < static_cast<int>(mine)) {
+                if (i < static_cast<int>(nw)) {
                     *reinterpret_cast<uint4*>(tile + to[i]) = codes_to_halves(x[i][0]);
                     *reinterpret_cast<uint4*>(tile + (to[i] ^ 16)) = codes_to_halves(x[i][1]);
                 }
@@ -595,13 +623,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
             }
             return true;
         };
+        uint32_t load = quarter, past = 0;
         for (uint32_t it = 0;; ++it) {
             const Item& m = next_item(it);
             if (stopped() || !m.valid) break;
-            const uint32_t past = tiles + m.end - m.t;
+            past += 8 * (m.end - m.t);
             item_read(it);
-            for (uint32_t u = 0; tiles < past && convert(u); u = (u + 1) & 3) tiles += u == 3;
-            if (tiles < past) break;
+            while (load < past && convert(load)) load += 4;
+            if (load < past) break;
         }
     } else {
         // ----------------------------------------------------------- softmax
