@@ -86,22 +86,33 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
     const bs_shared_attention_desc& d = a.d;
     const uint32_t hkv = a.c.kv_heads, b = blockIdx.z, segment = blockIdx.x / parts, row0 = blockIdx.y * kRows;
     const uint32_t h = LIST ? segment % hkv : segment, query = LIST ? segment / hkv : 0, block = a.c.block;
-    const uint32_t len = tokens_of(a, d.lens, b, d.table_width);
-
-    // this segment's query rows as the columns of K Q^T: column j is row row0 + j
+    // what is known from the start is asked for at once: the queries, as columns of
+    // K Q^T (column j is row row0 + j), the list's first entries, the length
     uint32_t q[NT][NW][2];
     float row_scale[NT][2];          // of columns 2c and 2c + 1
     int32_t limit[NT][2];            // tokens of its own that row sees
-    auto load_queries = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const uint32_t r = row0 + 8 * nt + g;
+        const uint16_t* row = static_cast<const uint16_t*>(d.q) + b * d.q_stride[0] + static_cast<int64_t>(LIST ? query : r / a.group) * d.q_stride[1] +
+                              (static_cast<int64_t>(h) * a.group + r % a.group) * d.q_stride[2] + c * (NW * 4);
+        fetch_query_row<NW>(q[nt], row, r < given.rows);
+    }
+    const int32_t* const list = given.blocks + ((static_cast<uint64_t>(b) * d.queries + query) * hkv + h) * given.count;
+    int32_t ahead[kMostIds / kThreads];
+    if (LIST) {
+        const uint32_t from = static_cast<uint32_t>(static_cast<uint64_t>(given.count) * rank / parts) + threadIdx.x;
+#pragma unroll
+        for (uint32_t i = 0; i < kMostIds / kThreads; ++i) ahead[i] = from + i * kThreads < given.count ? list[from + i * kThreads] : -1;
+    }
+    const uint32_t len = tokens_of(a, d.lens, b, d.table_width);
+    auto scale_queries = [&]() {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const uint32_t r = row0 + 8 * nt + g, col = row0 + 8 * nt + 2 * c;
-            const uint16_t* row = static_cast<const uint16_t*>(d.q) + b * d.q_stride[0] + static_cast<int64_t>(LIST ? query : r / a.group) * d.q_stride[1] +
-                                  (static_cast<int64_t>(h) * a.group + r % a.group) * d.q_stride[2] + c * (NW * 4);
-            load_query_row<NW>(q[nt], row_scale[nt], row, r < given.rows, d.dtype != BS_F16, d.scale * 1.4426950408889634f, c);
+            scale_query_row<NW>(q[nt], row_scale[nt], d.dtype != BS_F16, d.scale * 1.4426950408889634f, c);
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                limit[nt][i] = static_cast<int32_t>(len) - d.queries + 1 + static_cast<int32_t>(LIST ? query : (col + i) / a.group);
+                limit[nt][i] = static_cast<int32_t>(len) - d.queries + 1 + static_cast<int32_t>(LIST ? query : (row0 + 8 * nt + 2 * c + i) / a.group);
         }
     };
     Group group{};                   // what the sequence shares (none: no tokens)
@@ -129,7 +140,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
     if (!LIST && given.direct) find_group();
     const uint32_t shared_entries = !LIST && given.direct ? (group.tokens + block - 1) / block : 0;
     const int32_t* const table = d.table + static_cast<uint64_t>(b) * d.table_width;
-    const int32_t* const list = given.blocks + ((static_cast<uint64_t>(b) * d.queries + query) * hkv + h) * given.count;
     const int32_t most = static_cast<int32_t>(len) - (LIST ? d.queries - 1 - static_cast<int32_t>(query) : 0);
     const uint32_t width = d.table_width, tokens = most > 0 ? most : 0;           // some row sees the tokens below
     const uint32_t entries = LIST ? given.count : shared_entries + (tokens + block - 1) / block;
@@ -139,7 +149,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
     for (uint32_t from = begin; from < end; from += kMostIds) {
         // look them up; one without a token that is seen begins past all of them
         const uint32_t held = min(end - from, kMostIds);
-        for (uint32_t e = threadIdx.x; e < held; e += kThreads) {
+#pragma unroll
+        for (uint32_t i = 0; i < kMostIds / kThreads; ++i) {
+            const uint32_t e = threadIdx.x + i * kThreads;
+            if (e >= held) break;
             int2 entry = make_int2(0, kHidden);
             if (!LIST && from + e < shared_entries) {
                 const uint32_t id = d.shared_table[static_cast<uint64_t>(m) * d.shared_width + from + e];
@@ -148,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
                 ids[e] = entry;
                 continue;
             }
-            const int32_t col = LIST ? list[from + e] : static_cast<int32_t>(from + e - shared_entries);
+            const int32_t col = !LIST ? static_cast<int32_t>(from + e - shared_entries) : from == begin ? ahead[i] : list[from + e];
             if (col >= 0 && static_cast<uint32_t>(col) < width && static_cast<int64_t>(col) * block < tokens) {
                 const uint32_t id = table[col];
                 if (id < a.c.num_blocks) entry = make_int2(id, static_cast<int32_t>(col * block));
@@ -195,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
 #pragma unroll
         for (int i = 0; i < kStages; ++i) request(warp + i * kWarps, i);
         if (from == begin) {                           // (under the first copies)
-            load_queries();
+            scale_queries();
             if (!LIST && a.shares) find_group();
         }
         uint32_t stage = 0;

@@ -114,14 +114,16 @@ __device__ __forceinline__ constexpr uint32_t value_dim(int t, uint32_t g) {
 // One query row as column g of the products; `scale` times what its scaling
 // by a power of two took off is returned for columns 2c and 2c + 1.
 template <int NW>
-__device__ __forceinline__ void load_query_row(uint32_t (&q)[NW][2], float (&row_scale)[2], const uint16_t* row, bool real, bool bf16,
-                                               float scale, uint32_t c) {
+__device__ __forceinline__ void fetch_query_row(uint32_t (&q)[NW][2], const uint16_t* row, bool real) {
 #pragma unroll
     for (int j = 0; j < NW; ++j) {
         const uint2 u = real ? *reinterpret_cast<const uint2*>(row + 4 * j) : make_uint2(0, 0);
         q[j][0] = u.x;
         q[j][1] = u.y;
     }
+}
+template <int NW>
+__device__ __forceinline__ void scale_query_row(uint32_t (&q)[NW][2], float (&row_scale)[2], bool bf16, float scale, uint32_t c) {
     if (bf16) {
         // times 2^e with the row's largest in [2^12, 2^13); rows of zeros, infinities and NaN as they are
         uint32_t top = 0;        // magnitudes of bf16 order as integers
@@ -144,6 +146,12 @@ __device__ __forceinline__ void load_query_row(uint32_t (&q)[NW][2], float (&row
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) row_scale[i] = __shfl_sync(kFull, scale, (2 * c + i) * 4);
+}
+template <int NW>
+__device__ __forceinline__ void load_query_row(uint32_t (&q)[NW][2], float (&row_scale)[2], const uint16_t* row, bool real, bool bf16,
+                                               float scale, uint32_t c) {
+    fetch_query_row<NW>(q, row, real);
+    scale_query_row<NW>(q, row_scale, bf16, scale, c);
 }
 
 // Products of the tile's key codes with the queries: z[half] has tokens g and
