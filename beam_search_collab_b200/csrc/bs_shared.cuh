@@ -87,32 +87,19 @@ __device__ __forceinline__ uint32_t share_of(uint64_t w, uint32_t n, uint64_t x)
     return static_cast<uint32_t>(x < wide ? x / (q + 1) : r + (x - wide) / q);
 }
 
-// Cost of a key head's segments before group m, and of all groups; every
-// thread of the block (a multiple of 32 threads) gets both.  sums: [2 * warps].
-__device__ __forceinline__ void count_cost(const SharedArgs& a, uint32_t m, uint64_t& before, uint64_t& all, uint64_t* sums) {
-    uint64_t mine = 0, total = 0;
-    for (uint32_t i = threadIdx.x; i < a.d.num_groups; i += blockDim.x) {
-        const uint64_t t = cost_of(group_of(a, i));
-        total += t;
-        mine += i < m ? t : 0;
-    }
+// Cost of a key head's segments of all groups, for every thread of the block (a
+// multiple of 32 threads).  sums: [warps].
+__device__ __forceinline__ uint64_t count_cost(const SharedArgs& a, uint64_t* sums) {
+    uint64_t total = 0;
+    for (uint32_t i = threadIdx.x; i < a.d.num_groups; i += blockDim.x) total += cost_of(group_of(a, i));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        mine += __shfl_xor_sync(kFull, mine, o);
-        total += __shfl_xor_sync(kFull, total, o);
-    }
-    const uint32_t warps = blockDim.x / 32, warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) {
-        sums[warp] = mine;
-        sums[warps + warp] = total;
-    }
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kFull, total, o);
+    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = total;
     __syncthreads();
-    before = all = 0;
-    for (uint32_t i = 0; i < warps; ++i) {
-        before += sums[i];
-        all += sums[warps + i];
-    }
+    total = 0;
+    for (uint32_t i = 0; i < blockDim.x / 32; ++i) total += sums[i];
     __syncthreads();
+    return total;
 }
 
 // Row of the outputs of a group's row r (of key head h).

@@ -57,6 +57,9 @@ constexpr uint32_t kRing = 4;
 constexpr uint32_t kQuarter = kRows / 4;
 template <int BOXES>
 constexpr uint32_t kRawRing = BOXES == 2 ? 8 : 16;
+// Up to so many groups the warp that finds the pieces counts their cost too, a group
+// to a lane, meanwhile the other warps get ready; more are counted by all warps first.
+constexpr uint32_t kFewGroups = 32;
 constexpr float kLift = 5.f;
 constexpr float kMost = 32768.f;       // of a sum of 64 lifted weights, and so of each: below f16's 65504
 // Tiles whose scales are in shared memory.  Those of tile n are written when
@@ -126,7 +129,7 @@ struct Control {
     uint64_t full[kRing], empty[kRing], raw_full[16], raw_empty[16];
     uint64_t item_full[2], item_empty[2];
     Item item[2];
-    uint64_t sums[2 * (kCopier + 1)];
+    uint64_t sums[kCopier + 1];
     uint32_t missing[kScales];          // by tile: bits of 16 tokens whose block is not there
     __align__(16) float2 scales[kScales][8];      // by tile and 16 tokens: of keys, of values
     uint32_t tmem;
@@ -162,14 +165,18 @@ __device__ __forceinline__ bool next_piece(const SharedArgs& a, Piece& p) {
     return true;
 }
 
-// The first piece of the share that begins at unit `first` (by one warp).
-__device__ __forceinline__ void find_piece(const SharedArgs& a, Piece& p, uint64_t first) {
-    const uint32_t lane = threadIdx.x & 31;
-    uint64_t seen = 0;
-    p.m = a.d.num_groups - 1;
-    for (uint32_t m0 = 0; m0 < a.d.num_groups; m0 += 32) {       // 32 at a time
+// The first piece of the block's share (by one warp); none: p.left and its tiles
+// are 0.  w, n: cost of all pieces and shares in use, found here too if the groups
+// are few.
+__device__ __forceinline__ void find_piece(const SharedArgs& a, Piece& p, uint64_t& w, uint32_t& n) {
+    const uint32_t lane = threadIdx.x & 31, groups = a.d.num_groups;
+    uint64_t seen = 0, first = 0;
+    p.left = p.t = p.end = p.segment = p.slot = 0;
+    p.m = groups - 1;
+    p.g = Group{};
+    for (uint32_t m0 = 0; m0 < groups; m0 += 32) {       // 32 at a time
         Group g{};
-        if (m0 + lane < a.d.num_groups) g = group_of(a, m0 + lane);
+        if (m0 + lane < groups) g = group_of(a, m0 + lane);
         const uint64_t mine = cost_of(g) * a.c.kv_heads;
         uint64_t sum = mine;
 #pragma unroll
@@ -177,23 +184,36 @@ __device__ __forceinline__ void find_piece(const SharedArgs& a, Piece& p, uint64
             const uint64_t up = __shfl_up_sync(kFull, sum, o);
             if (lane >= static_cast<uint32_t>(o)) sum += up;
         }
+        const uint64_t together = __shfl_sync(kFull, sum, 31);
+        if (m0 == 0) {
+            if (groups <= kFewGroups) {
+                w = together;
+                n = used_shares(w, a.shares);
+            }
+            if (blockIdx.x >= n) return;
+            first = share_first(w, n, blockIdx.x);
+            p.left = share_first(w, n, blockIdx.x + 1) - first;
+        }
         const unsigned past = __ballot_sync(kFull, seen + sum > first);
         if (past) {
             const int l = __ffs(past) - 1;
             seen += __shfl_sync(kFull, sum - mine, l);
             p.m = m0 + l;
+            p.g.first = __shfl_sync(kFull, g.first, l);
+            p.g.rows = __shfl_sync(kFull, g.rows, l);
+            p.g.pairs = __shfl_sync(kFull, g.pairs, l);
+            p.g.tokens = __shfl_sync(kFull, g.tokens, l);
+            p.g.tiles = __shfl_sync(kFull, g.tiles, l);
             break;
         }
-        seen += __shfl_sync(kFull, sum, 31);
+        seen += together;
     }
-    p.g = group_of(a, p.m);
-    if (p.g.tiles == 0) {                                        // (not with lists that stay as they are)
-        p.left = p.t = p.end = p.segment = p.slot = 0;
+    if (p.g.tiles == 0) {                                // (not with lists that stay as they are)
+        p.left = 0;
         return;
     }
     const uint32_t cost = p.g.tiles + kStart;
     p.segment = static_cast<uint32_t>((first - seen) / cost);
-    p.slot = 0;
     p.at = first;
     cut_piece(p, static_cast<uint32_t>((first - seen) % cost));
 }
@@ -339,11 +359,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
 
     cudaGridDependencySynchronize();       // in every block, before anything of the caller's
     cudaTriggerProgrammaticLaunchCompletion();       // the kernel after this one begins with what does not need it
-    uint64_t before, all;
-    count_cost(a, 0, before, all, ctl.sums);
-    const uint64_t w = all * hkv;
-    const uint32_t n = used_shares(w, a.shares);
-    if (blockIdx.x >= n) return;
+    uint64_t w = 0;                        // cost of all pieces
+    uint32_t n = 0;                        // shares in use
+    if (d.num_groups > kFewGroups) {
+        w = count_cost(a, ctl.sums) * hkv;
+        n = used_shares(w, a.shares);
+        if (blockIdx.x >= n) return;
+    }
     if (threadIdx.x == 0) {
         for (int t = 0; t < 2; ++t) {
             barrier_init(&ctl.q_full[t], 4);
@@ -495,8 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
         const uint32_t run = block < kQuarter ? block : kQuarter, bytes = run * dim, quarter = lane & 3;
         uint32_t tiles = 0, items = 0, copied = 0;     // copied: quarters by this lane
         Piece p;
-        p.left = share_first(w, n, blockIdx.x + 1) - share_first(w, n, blockIdx.x);
-        find_piece(a, p, share_first(w, n, blockIdx.x));
+        find_piece(a, p, w, n);
         for (bool more = true; more && !stopped(); more = next_piece(a, p)) {
             if (p.t == p.end) continue;            // (a share that ends before a segment's first tile)
             const uint32_t h = p.segment / p.g.pairs, row0 = p.segment % p.g.pairs * kPairRows;
