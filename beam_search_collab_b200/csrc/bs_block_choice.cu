@@ -128,7 +128,8 @@ constexpr uint32_t kMostHeld = 8;      // scores of a thread where one block has
 // Which of a row's n > count scores stay, by one block with kMostHeld of them in
 // a thread's registers: the m-th largest of the free ones by its digits of 8 bits,
 // then their places by prefix sums.  A row of 1,024 takes 2 us; the cluster's way
-// (bs_select.cuh), with digits of 11 bits for longer rows, 6.
+// (bs_select.cuh), with digits of 11 bits for longer rows, 6 and more (8 rows of
+// 1,024 columns 24.6 us in all, against 8.8).
 template <int THREADS>
 struct SmallShared {
     uint32_t count[4][256];
@@ -202,8 +203,8 @@ __device__ __forceinline__ void select_small(SmallShared<THREADS>& shared, uint3
 
 // A cluster of blocks has one row: a query and a key head.  Each block scores
 // its slice of the table's columns, then the row's largest are found among the
-// scores in shared memory.  SMALL: one block, and at most kMostHeld columns a
-// thread.
+// scores in shared memory.  SMALL: by the first block alone, for rows of at most
+// kMostHeld columns a thread; the others leave their scores with it.
 template <typename T, int THREADS, bool SMALL>
 __global__ void __launch_bounds__(THREADS) k_block_choice(const __grid_constant__ ChoiceArgs a, uint32_t cached) {
     extern __shared__ uint32_t keys[];                     // [cached]: the columns' blocks, then their keys
@@ -215,7 +216,8 @@ __global__ void __launch_bounds__(THREADS) k_block_choice(const __grid_constant_
     constexpr uint32_t kWarps = THREADS / 32;
     cudaGridDependencySynchronize();       // in every block, before anything of the caller's
     const cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t rank = SMALL ? 0 : cluster.block_rank(), blocks = SMALL ? 1 : cluster.num_blocks();
+    constexpr bool kAlone = SMALL && THREADS == 128;       // no cluster
+    const uint32_t rank = kAlone ? 0 : cluster.block_rank(), blocks = kAlone ? 1 : cluster.num_blocks();
     const bs_block_choice_desc& d = a.d;
     const uint32_t hkv = a.c.kv_heads, group = d.q_heads / hkv, dim = a.c.dim, block = a.c.block;
     const uint32_t h = blockIdx.x / blocks, i = blockIdx.y, b = blockIdx.z, t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -238,6 +240,7 @@ __global__ void __launch_bounds__(THREADS) k_block_choice(const __grid_constant_
         for (uint32_t y = rank * THREADS + t; y < count; y += blocks * THREADS) out[y] = y < n ? static_cast<int32_t>(y) : -1;
         return;
     }
+    if (SMALL && !kAlone && blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");     // this block has begun
     uint32_t first, size;
     select_slice(n, blocks, rank, first, size);
     const int32_t* const table = d.table + static_cast<uint64_t>(b) * d.table_width + first;
@@ -290,6 +293,11 @@ __global__ void __launch_bounds__(THREADS) k_block_choice(const __grid_constant_
         return sum;
     };
     auto key = [&](int32_t sum, float scale) { return select_key(__fmul_rn(__int2float_rn(sum), scale)); };
+    uint32_t* scores = keys;                               // of this block's columns
+    if (SMALL && !kAlone && blocks > 1) {
+        asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
+        scores = cluster.map_shared_rank(keys, 0) + first;
+    }
     constexpr uint32_t kBatch = 8;                         // columns of a lane whose bounds are on their way together
     for (uint32_t x0 = warp * cols * kBatch; x0 < held; x0 += kWarps * cols * kBatch) {
         uint4 y[kBatch];
@@ -311,10 +319,15 @@ __global__ void __launch_bounds__(THREADS) k_block_choice(const __grid_constant_
                 if (chunk + s < per_col) sum += z;
             }
             const uint32_t col = x0 + u * cols + sub;
-            if (chunk == 0 && sub < cols && col < held) keys[col] = key(sum, scale[u]);
+            if (chunk == 0 && sub < cols && col < held) scores[col] = key(sum, scale[u]);
         }
     }
-    __syncthreads();
+    if (SMALL && !kAlone && blocks > 1) {
+        cluster.sync();
+        if (rank != 0) return;
+    } else {
+        __syncthreads();
+    }
     auto keep = [&](uint32_t slot, uint32_t col) { out[slot] = col; };
     if constexpr (SMALL) {
         select_small<THREADS>(shared, warp_sums, keys, n, d.sinks, d.recent, count, keep);
@@ -337,7 +350,7 @@ __global__ void __launch_bounds__(THREADS) k_block_choice(const __grid_constant_
 
 template <typename T, int THREADS, bool SMALL>
 cudaError_t launch_choice(const ChoiceArgs& a, uint32_t cluster, cudaStream_t stream) {
-    const uint32_t slice = ((a.d.table_width + cluster - 1) / cluster + 3) & ~3u, cached = slice < kMostCached ? slice : kMostCached;
+    const uint32_t slice = ((a.d.table_width + (SMALL ? 0 : cluster - 1)) / (SMALL ? 1 : cluster) + 3) & ~3u, cached = slice < kMostCached ? slice : kMostCached;
     cudaError_t e = cudaFuncSetAttribute(k_block_choice<T, THREADS, SMALL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostCached * 4);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr[2] = {};
@@ -352,7 +365,7 @@ cudaError_t launch_choice(const ChoiceArgs& a, uint32_t cluster, cudaStream_t st
     config.dynamicSmemBytes = cached * 4;
     config.stream = stream;
     config.attrs = attr;
-    config.numAttrs = SMALL ? 1 : 2;
+    config.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&config, k_block_choice<T, THREADS, SMALL>, a, cached);
 }
 
@@ -360,13 +373,22 @@ template <typename T>
 cudaError_t launch_choice(const bs_token_cache& c, const bs_block_choice_desc& d, const MemoryDevice& dev, cudaStream_t stream) {
     const ChoiceArgs a{c, d, dev.errors};
     const uint64_t rows = static_cast<uint64_t>(c.kv_heads) * d.queries * d.num_seqs;
-    // a block to a row while it holds the row's keys in registers and the rows fill
-    // a good part of the GPU
-    if (d.table_width <= 256) return launch_choice<T, 128, true>(a, 1, stream);
-    if (d.table_width <= 512 * kMostHeld && rows * 3 > static_cast<uint64_t>(dev.num_sms)) return launch_choice<T, 512, true>(a, 1, stream);
-    // else a row goes to more blocks while they would have over 256 columns each
-    // and the rows alone do not fill the GPU
+    // Rows that one block's registers hold: more blocks score them while they would have
+    // over 256 columns each and all are resident at once, one to an SM (clusters of 8
+    // fit only half of the SMs, as they must not cross a group of SMs).  8 rows of
+    // 1,024 columns take 8.8 us by 4 blocks and 14.2 by one; 16 rows 9.2 by 4, 13.6 by
+    // 8; 64 rows 11.2 by 2, 14.4 by one and 17.7 by 4; 128 rows 14.6 by one, 21.6 by 2.
+    // Small blocks are for many short rows (256 rows of 200 columns 11.2 against
+    // 15.6 us, 96 rows 10.6 against 8.5) and for rows that they read at once (8 rows
+    // of 40 columns 6.1 against 7.9).
+    const uint64_t sms = dev.num_sms;
+    if (d.table_width <= 64 || (d.table_width <= 256 && rows > sms)) return launch_choice<T, 128, true>(a, 1, stream);
     uint32_t cluster = 1;
+    if (d.table_width <= 512 * kMostHeld) {
+        while (cluster < kMostCluster && d.table_width / cluster > 256 && rows * cluster * (cluster < 4 ? 2 : 4) <= sms) cluster *= 2;
+        return launch_choice<T, 512, true>(a, cluster, stream);
+    }
+    // longer rows: counted by all blocks of a cluster
     while (cluster < kMostCluster && d.table_width / cluster > 256 && rows * cluster * 2 <= 2u * dev.num_sms) cluster *= 2;
     return launch_choice<T, 256, false>(a, cluster, stream);
 }
