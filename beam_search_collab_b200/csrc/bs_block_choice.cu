@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(THREADS) k_block_choice(const __grid_constant_
     __syncthreads();
 #pragma unroll
     for (uint32_t w = 0; w < kWarps; ++w) top = fmaxf(top, warp_max[w]);
-    const float by = top < 1e-30f ? 0.f : __fdiv_rn(127.f, top);
+    const float by = top < 1e-30f ? 0.f : __fmul_rn(__frcp_rn(top), 127.f);
     if (t < dim) {
         int32_t positive = 0, negative = 0;
         auto add = [&](float y) {

@@ -476,7 +476,8 @@ BS_API bs_status bs_block_bounds(const bs_token_cache* cache, const bs_block_bou
  * are chosen; else the first `sinks`, the last `recent`, and of the others the
  * count - sinks - recent of the largest score (ties: the lower column; NaN
  * counts as largest).  A key head's query heads choose together:
- *   m = max |q| over their elements,  c = rint(q * (127 / m))  (0 if m < 1e-30)
+ *   m = max |q| over their elements,  c = rint(q * (127 * (1 / m)))  (0 if
+ *   m < 1e-30; each step rounded to 32 bits)
  *   score = k_scale * sum over heads and dimensions of max(c * upper, c * lower),
  * the sum exact in integers, then rounded to 32 bits, then the product: no sum
  * of those heads' scores with a token of the block is larger, but for the
