@@ -7,9 +7,13 @@
 // tokens come from: a list of table columns for each query and key head.  A
 // cluster of blocks takes a segment (a query and a key head), a part of its
 // list each; the list's entries are looked up in the table once, into shared
-// memory, those without a visible token left out, so that the copies of tiles
-// wait for no chain of loads.  The blocks of a cluster join their outputs
-// through distributed shared memory: no second kernel, no workspace.
+// memory (one without a visible token gets a position past all of them), so that
+// the copies of tiles wait for no chain of loads.  The blocks of a cluster join
+// their outputs through distributed shared memory: no second kernel, no workspace.
+// 128 segments of 4,096 tokens (134 MB of codes) take 31 us, 4.3 TB/s, where the
+// bytes alone are 20: three blocks to an SM, each with two tiles a warp on their way,
+// and their ends; 128 of 2,048 whose tokens four have in common 17.5 us, most of
+// it the 67 MB that they copy from the second-level cache.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -369,19 +373,24 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
     if (parts > 1) cluster.sync();         // no block ends while another reads it
 }
 
-// Blocks of a segment, by the time of its longest part and of all of them, and
-// that time, in tiles (0.34 us a block's): a block takes as long as kStart of them
-// to begin and end, and the join of a cluster some more.  Lists are as long as one
-// another, so the blocks go in waves; sequences are taken to have half the tokens
-// that their table has room for.
-uint32_t parts_of(uint64_t segments, uint64_t tokens, uint64_t resident, bool lists, double& time) {
-    constexpr double kStart = 16, kJoin = 2;
+// Blocks of a segment, by the time that they were measured to take, in us: a block
+// with one, two or three to an SM 3.7, 4.9 or 6.0 to begin and end and 0.29, 0.38 or
+// 0.47 for a tile of 32 tokens, a cluster of n 0.8 + n / 10 more.  Lists are as long
+// as one another, so the blocks go in waves.  Sequences are taken to have half the
+// tokens that their table has room for, those with all of them in the last wave.
+// (64 segments of 4 blocks of 64 tokens: 6.3 us by 2, 14.0 by 8; 8 segments of 64:
+// 39.9 by 1, 10.3 by 8; 128 of 2,000 own tokens: 23.7 by 1, 19.1 by 2, 24.2 by 4.)
+// `shared` and `own`: tiles of a segment.
+uint32_t parts_of(uint64_t segments, double shared, double own, uint32_t num_sms, uint32_t per_sm, bool lists, double& time) {
     uint32_t best = 1;
     for (uint32_t n = 1; n <= kMostCluster; ++n) {
-        const double part = static_cast<double>(tokens) / kTile / n, ends = kStart + (n > 1 ? kJoin : 0);
-        const uint64_t blocks = segments * n;
-        const double waves = lists ? static_cast<double>((blocks + resident - 1) / resident) : static_cast<double>(blocks) / resident;
-        const double all = waves * (ends + (lists ? part : part / 2)), t = all > ends + part ? all : ends + part;
+        const uint64_t blocks = segments * n, resident = static_cast<uint64_t>(num_sms) * per_sm;
+        auto wave = [&](uint64_t on_sm, double tiles) {
+            return 3.7 + 1.15 * (on_sm - 1) + (n > 1 ? 0.8 + 0.1 * n : 0.) + (0.285 + 0.09 * (on_sm - 1)) * tiles / n;
+        };
+        const uint64_t rest = blocks % resident;
+        const double t = blocks / resident * wave(per_sm, shared + (lists ? own : own / 2)) +
+                         (rest ? wave((rest + num_sms - 1) / num_sms, shared + own) : 0.);
         if (n == 1 || t < time) {
             time = t;
             best = n;
@@ -390,7 +399,7 @@ uint32_t parts_of(uint64_t segments, uint64_t tokens, uint64_t resident, bool li
     return best;
 }
 
-uint64_t resident_blocks(const MemoryDevice& dev, uint32_t rows) { return static_cast<uint64_t>(dev.num_sms) * blocks_per_sm(rows <= 8 ? 1 : 2); }
+double tiles_of(const bs_token_cache& c, uint64_t blocks) { return static_cast<double>(blocks * c.block) / kTile; }
 
 // The segments of attention over own tokens, as many as row tiles of key heads.
 uint64_t own_segments(const bs_token_cache& c, const bs_shared_attention_desc& d, uint32_t rows) {
@@ -404,9 +413,9 @@ cudaError_t launch_rows(const RowsArgs& a, const MemoryDevice& dev, cudaStream_t
     if (e != cudaSuccess) return e;
     const uint32_t row_tiles = (a.rows + 8 * NT - 1) / (8 * NT);
     const uint64_t segments = static_cast<uint64_t>(a.s.c.kv_heads) * (LIST ? a.s.d.queries : 1);
-    const uint64_t width = LIST ? a.count : a.s.d.table_width + (a.direct ? a.s.d.shared_width : 0ull);
     double time = 0;
-    const uint32_t parts = parts_of(segments * row_tiles * a.s.d.num_seqs, width * a.s.c.block, resident_blocks(dev, a.rows), LIST, time);
+    const uint32_t parts = parts_of(segments * row_tiles * a.s.d.num_seqs, a.direct ? tiles_of(a.s.c, a.s.d.shared_width) : 0.,
+                                    tiles_of(a.s.c, LIST ? a.count : a.s.d.table_width), dev.num_sms, blocks_per_sm(NT), LIST, time);
     cudaLaunchAttribute attr[2] = {};
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = parts;
@@ -447,16 +456,18 @@ struct Layout {
 Layout plan(const bs_token_cache& c, const bs_shared_attention_desc& d, const MemoryDevice& dev) {
     Layout l{};
     // Few shared tokens or few sequences: each sequence reads them by itself, in
-    // the kernel for its own.  The times of both ways, in tiles of that kernel
-    // (0.34 us): the other one takes 14 us for its start, its end and the join, and
-    // 2.6 us for 256 rows over 128 tokens.  (4 sequences over 700 tokens: 8.9 us
-    // this way, 20 that way; 64 over 900 to 17,001: 256 and 101.)
+    // the kernel for its own.  The times of both ways, in us: the other one takes
+    // 14 for its start, its end and the join, and 2.6 for 256 rows over 128 tokens.
+    // (Of 32 query and 8 key heads of 128: 8 sequences over 1,000 tokens 11 us this
+    // way and 25 that way; 64 over 1,000 39 and 38; 128 over 3,500 155 and 51; each
+    // with 200 tokens of its own.)
     const uint32_t in_sequence = static_cast<uint32_t>(d.q_heads / c.kv_heads) * d.queries;
-    const uint64_t segments = own_segments(c, d, in_sequence), resident = resident_blocks(dev, in_sequence);
-    const uint64_t own = static_cast<uint64_t>(d.table_width) * c.block;
+    const uint64_t segments = own_segments(c, d, in_sequence);
+    const uint32_t per_sm = blocks_per_sm(in_sequence <= 8 ? 1 : 2);
+    const double own = tiles_of(c, d.table_width);
     double here = 0, there = 0;
-    parts_of(segments, own + static_cast<uint64_t>(d.shared_width) * c.block, resident, false, here);
-    parts_of(segments, own, resident, false, there);
+    parts_of(segments, tiles_of(c, d.shared_width), own, dev.num_sms, per_sm, false, here);
+    parts_of(segments, 0., own, dev.num_sms, per_sm, false, there);
     const uint64_t tiles = (static_cast<uint64_t>(d.shared_width) * c.block + shared::kTileTokens - 1) / shared::kTileTokens;
     if (tiles == 0) return l;
     const uint64_t rows = static_cast<uint64_t>(d.num_seqs) * d.queries * d.q_heads;
@@ -464,7 +475,7 @@ Layout plan(const bs_token_cache& c, const bs_shared_attention_desc& d, const Me
     const uint64_t pairs = rows / c.kv_heads / shared::kPairRows + std::min(d.num_groups, d.num_seqs);
     const uint64_t units = pairs * c.kv_heads * (tiles + shared::kStart), most = (units + 2 * shared::kStart - 1) / (2 * shared::kStart);
     l.shares = static_cast<uint32_t>(most < static_cast<uint64_t>(dev.num_sms) ? most : dev.num_sms);
-    there += (14 + 2.6 * static_cast<double>(units) / l.shares) / 0.34;
+    there += 14 + 2.6 * static_cast<double>(units) / l.shares;
     if (here <= there) {
         l.shares = 0;
         return l;
