@@ -75,7 +75,8 @@ EXPORTS = ("bs_search_params_default", "bs_index_create", "bs_index_load", "bs_i
            "bs_index_load_codebook", "bs_index_build_codebook", "bs_index_info", "bs_index_entry_point", "bs_index_rabitq_entry",
            "bs_index_build_graph", "bs_ground_truth", "bs_index_prepare", "bs_index_take_errors", "bs_index_destroy", "bs_search", "bs_search_no_alloc", "bs_merge_shards",
            "bs_prompt_attention", "bs_prompt_attention_workspace", "bs_cache_write", "bs_cache_read", "bs_cache_attention",
-           "bs_cache_attention_workspace", "bs_cache_evict", "bs_cache_evict_workspace", "bs_memory_take_errors",
+           "bs_cache_attention_workspace", "bs_cache_evict", "bs_cache_evict_workspace", "bs_norm_rotate", "bs_block_bounds",
+           "bs_block_choice", "bs_block_attention", "bs_shared_attention", "bs_shared_attention_workspace", "bs_memory_take_errors",
            "bs_device_alloc",
            "bs_device_free",
            "bs_copy_to_device",
