@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(THREADS) k_block_choice(const __grid_constant_
         for (uint32_t y = rank * THREADS + t; y < count; y += blocks * THREADS) out[y] = y < n ? static_cast<int32_t>(y) : -1;
         return;
     }
-    if (SMALL && !kAlone && blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");     // this block has begun
+    if (SMALL && !kAlone && blocks > 1) asm volatile("barrier.cluster.arrive.relaxed;\n" ::: "memory");     // this block has begun
     uint32_t first, size;
     select_slice(n, blocks, rank, first, size);
     const int32_t* const table = d.table + static_cast<uint64_t>(b) * d.table_width + first;
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(THREADS) k_block_choice(const __grid_constant_
     auto key = [&](int32_t sum, float scale) { return select_key(__fmul_rn(__int2float_rn(sum), scale)); };
     uint32_t* scores = keys;                               // of this block's columns
     if (SMALL && !kAlone && blocks > 1) {
-        asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
+        asm volatile("barrier.cluster.wait;\n" ::: "memory");
         scores = cluster.map_shared_rank(keys, 0) + first;
     }
     constexpr uint32_t kBatch = 8;                         // columns of a lane whose bounds are on their way together

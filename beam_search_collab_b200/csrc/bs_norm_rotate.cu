@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) k_norm_rotate(const __grid_
     __syncthreads();
     float cosine[kEach][kPairs], sine[kEach][kPairs];
     uint64_t known = ~0ull;                // item whose angles those are
+    const float one_of_dim = 1.f / dim;
     while (b.item < items) {
         Word now[kBatch][kEach][2];
 #pragma unroll
@@ -257,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) k_norm_rotate(const __grid_
                 }
             if (norm) {                                             // (all lanes)
                 for (uint32_t o = a.lanes / 2; o > 0; o >>= 1) squares += __shfl_xor_sync(kFull, squares, o);
-                const float by = rsqrtf(squares / dim + d.eps);
+                const float by = rsqrtf(fmaf(squares, one_of_dim, d.eps));
 #pragma unroll
                 for (int e = 0; e < kEach; ++e)
 #pragma unroll
