@@ -480,8 +480,8 @@ BS_API bs_status bs_block_bounds(const bs_token_cache* cache, const bs_block_bou
  *   m < 1e-30; each step rounded to 32 bits)
  *   score = k_scale * sum over heads and dimensions of max(c * upper, c * lower),
  * the sum exact in integers, then rounded to 32 bits, then the product: no sum
- * of those heads' scores with a token of the block is larger, but for the
- * rounding of q.  blocks[b][i][h]: columns in ascending order, -1 past the end. */
+ * of those heads' scores with a token of the block, in units of m / 127, is
+ * larger, but for the rounding of q.  blocks[b][i][h]: columns in ascending order, -1 past the end. */
 typedef struct bs_block_choice_desc {
     const void* q;            /* [num_seqs][queries][q_heads][dim]            */
     int64_t q_stride[3];      /* elements from sequence to sequence, token to token, head to head */
