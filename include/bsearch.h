@@ -457,7 +457,8 @@ BS_API bs_status bs_norm_rotate(const bs_norm_rotate_desc* desc, void* stream);
  * [1][x] the smallest code of dimension x among the block's tokens at positions
  * below lens[b].  Written are the blocks that hold any of the last `last` tokens
  * of a sequence (last < 0: all its blocks), others stay as they are.  A block
- * that is in the tables of several sequences gets the bounds of any of them.
+ * that is in the tables of several sequences gets, value by value, the bounds of
+ * any of them (so all should have the same of its tokens).
  * To be called when codes have changed: after bs_cache_write with the number of
  * new tokens, after bs_cache_evict with last < 0 on the new tables. */
 typedef struct bs_block_bounds_desc {
