@@ -131,10 +131,12 @@ __global__ void __launch_bounds__(kThreads, kBlocks) k_norm_rotate(const __grid_
     // where the lane's chunks lie in a row
     uint32_t lo[kEach], hi[kEach];
     bool mine[kEach];
+    int turned[kEach];                                 // pairs that are rotated, the first ones
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
         const uint32_t u = at + e * a.lanes;
         mine[e] = u < slots;
+        turned[e] = V * u < half ? static_cast<int>(min(half - V * u, static_cast<uint32_t>(kPairs))) : 0;
         if (INTERLEAVED || u >= half / V) {
             lo[e] = INTERLEAVED ? 2 * V * u : 2 * half + 2 * V * (u - half / V);
             hi[e] = lo[e] + V;
@@ -268,15 +270,23 @@ __global__ void __launch_bounds__(kThreads, kBlocks) k_norm_rotate(const __grid_
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
                 if (!mine[e]) continue;
+                // past the rotated part values pass as they are (by a cosine of 1 and a sine of
+                // 0 an infinity would make its partner NaN): `only` says of some pairs which
                 float z[2][V];
+                auto rotate = [&](auto only) {
 #pragma unroll
-                for (int j = 0; j < kPairs; ++j) {
-                    const int s = INTERLEAVED ? j / (V / 2) : 0, i = INTERLEAVED ? 2 * (j % (V / 2)) : j;
-                    const int s2 = INTERLEAVED ? s : 1, i2 = INTERLEAVED ? i + 1 : i;
-                    const float p = y[e][s][i], q = y[e][s2][i2];
-                    z[s][i] = fmaf(cosine[e][j], p, -sine[e][j] * q);
-                    z[s2][i2] = fmaf(cosine[e][j], q, sine[e][j] * p);
-                }
+                    for (int j = 0; j < kPairs; ++j) {
+                        const int s = INTERLEAVED ? j / (V / 2) : 0, i = INTERLEAVED ? 2 * (j % (V / 2)) : j;
+                        const int s2 = INTERLEAVED ? s : 1, i2 = INTERLEAVED ? i + 1 : i;
+                        const float p = y[e][s][i], q = y[e][s2][i2];
+                        const bool turn = only(j);
+                        z[s][i] = turn ? fmaf(cosine[e][j], p, -sine[e][j] * q) : p;
+                        z[s2][i2] = turn ? fmaf(cosine[e][j], q, sine[e][j] * p) : q;
+                    }
+                };
+                if (turned[e] == kPairs) rotate([](int) { return true; });
+                else if (INTERLEAVED) rotate([&](int j) { return j < turned[e]; });
+                else rotate([](int) { return false; });             // (half is a multiple of V: a chunk is in or out)
                 Word w[2];
                 rounded<T, V>(w[0], z[0]);
                 rounded<T, V>(w[1], z[1]);

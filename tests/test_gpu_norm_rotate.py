@@ -1,4 +1,6 @@
 """GPU: norm and rotary position of queries and keys (bs_norm_rotate) against the definition in 64 bits."""
+import math
+
 import pytest
 import torch
 
@@ -192,3 +194,29 @@ def test_gradients_are_refused():
         assert out.requires_grad and not out_k.requires_grad
         with pytest.raises(RuntimeError, match="no gradient"):
             out.float().sum().backward()
+
+
+def same(a, b):
+    return torch.allclose(a, b, rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,rotary", [(128, 0), (16, 0), (128, 64), (96, 40), (80, 12), (48, 6), (128, 100), (64, 62)])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_a_value_that_is_not_finite_stays_in_its_place(dim, rotary, value, interleaved):
+    # token i has it in dimension i: past the rotated part it passes, in it the other of its pair alone is not finite either
+    g = gen(14)
+    x = torch.randn((dim, 3, dim), generator=g, device="cuda").to(F16 if rotary % 8 else BF16)
+    positions = torch.randint(-9999, 9999, (dim,), generator=g, device="cuda", dtype=torch.int32)
+    freqs = M.rotary_frequencies(rotary, device="cuda")[0] if rotary else None
+    weight = torch.rand(dim, generator=g, device="cuda") + 0.5
+    kw = dict(interleaved=interleaved, k_weight=weight)
+    want, clean_k = M.norm_rotate(x, x[:, :1], positions, freqs, **kw)
+    y, at = x.clone(), torch.arange(dim, device="cuda")
+    y[at, 1, at] = value
+    got, got_k = M.norm_rotate(y, x[:, :1], positions, freqs, **kw)
+    want[at, 1, at] = value
+    for d in range(rotary):
+        for out in (want, got):
+            out[d, 1, d] = out[d, 1, d ^ 1 if interleaved else (d + rotary // 2) % rotary] = 0
+    assert same(got, want) and torch.equal(got_k, clean_k)
