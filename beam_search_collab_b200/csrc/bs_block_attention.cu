@@ -81,10 +81,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
     int2* const ids = reinterpret_cast<int2*>(join_o);          // block, first position; till the outputs are joined
 
     const SharedArgs& a = given.s;
-    // In every block, before anything of the caller's.  (After the shared tokens'
-    // kernel this one waits where it needs that one's outputs: that kernel has
-    // waited for what came before, in all its blocks, before this one starts.)
-    if (LIST || !a.shares) cudaGridDependencySynchronize();
+    // In every block, before anything of the caller's.  (After the shared tokens' kernel
+    // too: what the kernels before that one wrote is promised to this one by its own wait
+    // alone.  Begun before it, its own tokens hid under that kernel's end.)
+    cudaGridDependencySynchronize();
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = cluster.block_rank(), parts = cluster.num_blocks();
     const bs_shared_attention_desc& d = a.d;
@@ -256,10 +256,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
 
     if (!LIST && a.shares && begin == end) find_group();
     FarRow far{};                    // a thread below kRows: where that row's outputs over the shared tokens are
-    if (!LIST && a.shares) {
-        cudaGridDependencySynchronize();
-        if (group.tiles && threadIdx.x < kRows && row0 + threadIdx.x < given.rows) far = shared::far_row(a, group, b, h, row0 + threadIdx.x);
-    }
+    if (!LIST && a.shares && group.tiles && threadIdx.x < kRows && row0 + threadIdx.x < given.rows)
+        far = shared::far_row(a, group, b, h, row0 + threadIdx.x);
     float all_top[NT][2], all_sum[NT][2];
     join_warps<NW, NT>(o, top, sum, unit, all_top, all_sum, join_o, join_ml, warp, lane);
     auto row_at = [&](uint32_t r) {        // row of the outputs

@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hkv = a.c.kv_heads, dim = a.c.dim, block = a.c.block;
 
     cudaGridDependencySynchronize();       // in every block, before anything of the caller's
-    cudaTriggerProgrammaticLaunchCompletion();       // the kernel after this one begins with what does not need it
+    cudaTriggerProgrammaticLaunchCompletion();       // the kernel after this one is launched meanwhile, and waits
     uint64_t w = 0;                        // cost of all pieces
     uint32_t n = 0;                        // shares in use
     if (d.num_groups > kFewGroups) {

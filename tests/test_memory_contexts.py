@@ -186,3 +186,19 @@ def test_angles_reduced_in_integers_are_right():
             off = abs(got - want)
             off = float(min(off, 1 - off))
             assert off <= 2.0 ** -32 + abs(position) * (2.0 ** -64 + 2.0 ** -52 * abs(turn)), (freq, position, off)
+
+
+@pytest.mark.parametrize("name", ["bs_prompt_attention.cu", "bs_cache_attention.cu", "bs_token_cache.cu", "bs_norm_rotate.cu", "bs_block_choice.cu",
+                                  "bs_block_attention.cu", "bs_shared_attention.cu"])
+def test_every_block_waits_whatever_the_call_is(name):
+    # the wait is a statement of its own, under no condition, and alone: a kernel that begins without it would count on what a
+    # kernel two before it wrote, which is promised to those alone that wait themselves
+    with open(os.path.join(B.PKG, "csrc", name)) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    kernels = [(m[1], text[m.end():text.index("\n}\n", m.end())]) for m in re.finditer(r"__global__ void[^;{]*?(k_\w+)\(", text)]
+    assert kernels
+    for kernel, body in kernels:
+        assert body.count("cudaGridDependencySynchronize()") == 1, kernel
+        before, wait, _ = body.partition("\n    cudaGridDependencySynchronize();")        # (four spaces: the kernel's own block)
+        assert wait and re.search(r"[;{}]\s*\Z", before), kernel
+        assert not re.search(r"\breturn\b|atomicOr\(|\blens\b|\bd\.\w+\[", before.partition("{")[2]), kernel
