@@ -234,6 +234,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
             tile_scores<NW, NT>(z, s, q, g, c);
             const bool edge = min(left[0], left[1]) < 16 || (!LIST && max(pos[0], pos[1]) + 16 > static_cast<int32_t>(tokens) - d.queries + 1);
             bool move = fmaxf(v_scale[0], v_scale[1]) > 4.f * unit;
+            const float room[2] = {kSlack - scale_log2(v_scale[0], inv_unit), kSlack - scale_log2(v_scale[1], inv_unit)};
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
                         z[half][nt][i] *= row_scale[nt][i & 1] * k_scale[half];
                         const int32_t in = static_cast<int32_t>(g) + (i & 2) * 4;
                         if (edge && (in >= left[half] || pos[half] + in >= limit[nt][i & 1])) z[half][nt][i] = -INFINITY;
-                        move |= z[half][nt][i] > top[nt][i & 1] + kSlack;
+                        move |= z[half][nt][i] > top[nt][i & 1] + room[half];
                     }
             if (__any_sync(kFull, move)) move_maxima<NW, NT>(z, v_scale, top, sum, o, unit, inv_unit);
             tile_values<NW, NT>(z, s, v_scale, inv_unit, top, sum, o, g, c);

@@ -24,11 +24,11 @@
 // and outputs are 32-bit.  Where a weight meets the values, its
 // product with their scale is rounded to f16: by 2^-11 of itself, as much as
 // an f16 output's own rounding, or, where that is more (f16 has no exponents
-// below), by 2^-30 of the largest weight times the largest value scale (at
-// least 3e-29) that the warp has met.  A fold of 2^5 (kFold) in those units
-// uses the exponents that f16 has above 2^kSlack; without it the second figure
-// is 2^-25, and weights e^-14 of the largest beside a scale 50 times theirs
-// vanished.  The sum of weights takes them unrounded.
+// below), by 2^-30 of the largest such product that the warp has met (value
+// scales count down to 2^-60 of the largest).  A fold of 2^5 (kFold) in those
+// units uses the exponents that f16 has above 2^kSlack; without it the second
+// figure is 2^-25, and weights e^-14 of the largest beside a scale 50 times
+// theirs vanished.  The sum of weights takes them unrounded.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -332,6 +332,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(con
             const bool edge = static_cast<int32_t>((t + 1) * kTile) > static_cast<int32_t>(at.len) - a.d.queries + 1 ||
                               fminf(v_scale[0], v_scale[1]) < 0.f;
             bool move = fmaxf(v_scale[0], v_scale[1]) > 4.f * unit;
+            const float room[2] = {kSlack - scale_log2(v_scale[0], inv_unit), kSlack - scale_log2(v_scale[1], inv_unit)};
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_cache_split(con
                             const int32_t pos = static_cast<int32_t>(t * kTile + 16 * half + g) + (i & 2) * 4;
                             if (pos >= limit[nt][i & 1] || v_scale[half] < 0.f) z[half][nt][i] = -INFINITY;
                         }
-                        move |= z[half][nt][i] > top[nt][i & 1] + kSlack;
+                        move |= z[half][nt][i] > top[nt][i & 1] + room[half];
                     }
             if (score_at) {
 #pragma unroll

@@ -19,7 +19,9 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;              // tokens: two halves of 16, independent chains of instructions
 constexpr float kNoScore = -1e30f;     // running maximum before the first score
 constexpr float kSlack = 8.f;          // weights may grow to 2^kSlack before the maximum is moved
-constexpr float kFold = 32.f;          // a weight of 1 at the largest value scale in f16; 2^kSlack * 4 * kFold is below 65504
+constexpr float kFold = 32.f;          // a weight of 2^top at the largest value scale in f16; 2^kSlack * 4 * kFold is below 65504
+constexpr float kDeep = 60.f;          // value scales count down to 2^-kDeep of the largest
+constexpr float kMostSum = 80.f;       // the maximum is moved down only as far as sums stay below 2^kMostSum
 
 __device__ __forceinline__ unsigned smem_addr(const void* p) { return static_cast<unsigned>(__cvta_generic_to_shared(p)); }
 
@@ -48,6 +50,21 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
+
+__device__ __forceinline__ float log2_fast(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The maximum that weights count from is that of a score and this: log2 of its
+// value scale in units of the warp's largest (a scale below zero, of tokens that
+// are not seen, is NaN there and counts as the least).  What is rounded to f16 is a
+// weight times its value scale: counted from the largest score alone, weights of
+// 1 at a value scale 10^-7 of another's had two bits left, whatever weight that
+// other one got.
+__device__ __forceinline__ float scale_log2(float v_scale, float inv_unit) { return fmaxf(log2_fast(v_scale * inv_unit) - 5.f, -kDeep); }
+static_assert(kFold == 32.f, "log2 of it is above");
 
 // Bytes [x, y] (in bits 0-7 and 8-15, or 16-23 and 24-31) biased by 128 ->
 // two f16 of the codes: 0x6400 | u is 1024 + u, minus 1152.
@@ -180,22 +197,26 @@ __device__ __forceinline__ void tile_scores(float (&z)[2][NT][4], const unsigned
         }
 }
 
-// Rare: the maxima move, what was summed is rescaled.
+// Rare: the maxima move, what was summed is rescaled.  Where a larger value scale
+// than before becomes the unit, they move down by as much, so that weights at the
+// old scales keep their bits.
 template <int NW, int NT>
 __device__ __forceinline__ void move_maxima(const float (&z)[2][NT][4], const float (&v_scale)[2], float (&top)[NT][2], float (&sum)[NT][2],
                                             float (&o)[NT][NW][4], float& unit, float& inv_unit) {
     const float new_unit = fmaxf(unit, fmaxf(v_scale[0], v_scale[1]));
-    const float by_unit = unit / new_unit;
+    const float by_unit = unit / new_unit, less = log2_fast(by_unit);
     unit = new_unit;
     inv_unit = kFold / unit;
+    const float deep[2] = {scale_log2(v_scale[0], inv_unit), scale_log2(v_scale[1], inv_unit)};
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            float m = fmaxf(fmaxf(z[0][nt][i], z[0][nt][2 + i]), fmaxf(z[1][nt][i], z[1][nt][2 + i]));
+            float m = fmaxf(fmaxf(z[0][nt][i], z[0][nt][2 + i]) + deep[0], fmaxf(z[1][nt][i], z[1][nt][2 + i]) + deep[1]);
+            m = fmaxf(m, top[nt][i] + fmaxf(less, log2_fast(sum[nt][i]) - kMostSum));
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, x));
-            m = fmaxf(m, top[nt][i]);
+            m = fmaxf(m, kNoScore);
             const float shrink = exp2_fast(top[nt][i] - m);
             top[nt][i] = m;
             sum[nt][i] *= shrink;

@@ -21,11 +21,15 @@
 //                     instructions to convert
 //   O_t += P_t V      codes of V exact in f16, P_t f16: a weight times its values'
 //                     scale, over the largest of the piece, rounded to 2^-11 of
-//                     itself or, where that is more, 2^-29 of a weight of 1 at
-//                     the largest scale (weights count in 2^-kLift, the room
-//                     that a maximum moved at 2^10 leaves)
-// The maximum is moved only when a sum of 64 weights passes 2^10 (no maximum is
-// taken before the exponentials); sums are 32-bit, of the unrounded weights.
+//                     itself or, where that is more, 2^-29 of the row's largest
+//                     such product (they count in 2^-kLift, the room that a
+//                     maximum moved at 2^10 leaves)
+// So the maximum that weights count from is that of a score plus log2 of its value
+// scale over the piece's largest (at least -kDeep): counted from the largest score
+// alone, weights of 1 at a scale 10^-7 of another's had few bits left, whatever weight
+// that other one got.  It is moved only when 16 weights times their scale pass 2^10
+// together (no maximum is taken before the exponentials); sums are 32-bit, of the
+// unrounded weights.
 //
 // 512 rows of each of 8 key heads over 32,768 tokens take 104 us here: 28 times 128 tokens
 // a block, 4,100 to 4,600 clocks each, and 12,000 to the first scores and 5,500 for the
@@ -71,7 +75,9 @@ constexpr uint32_t kRawRing = BOXES == 2 ? 8 : 16;
 // to a lane, meanwhile the other warps get ready; more are counted by all warps first.
 constexpr uint32_t kFewGroups = 32;
 constexpr float kLift = 5.f;
-constexpr float kMost = 32768.f;       // of a sum of 64 lifted weights, and so of each: below f16's 65504
+constexpr float kMost = 32768.f;       // of 16 lifted weights times their scale together, and so of each: below f16's 65504
+constexpr float kDeep = 60.f;          // value scales count down to 2^-kDeep of the piece's largest
+constexpr float kDeepest = 0x1p-60f;
 // Tiles whose scales are in shared memory.  Those of tile n are written when
 // codes of tile n - kRawRing / 8 have been converted, into the place of keys that
 // were multiplied two tiles before; those products are issued when the weights of
@@ -256,15 +262,20 @@ __device__ __forceinline__ void rescale(uint32_t p_at, uint32_t o_at, int quarte
     wait_stores();
 }
 
+// log2 of a value scale (v_by: 1 over the piece's largest), what a score counts for besides its weight.
+__device__ __forceinline__ float scale_log2(float v_scale, float v_by) { return __log2f(fmaxf(v_scale * v_by, kDeepest)); }
+
 // 64 scores of a row that are all seen, 32 at a time; s[0] is on its way, the
 // next 32 follow (`more`: those after these too): weights 2^(key scale * s +
 // base), their sum returned, times their value scale packed in p.  scales: of 16
-// tokens each; k_by and v_by are what they are multiplied by besides.  (Unrolled: at 32
-// a turn the special-function pipe runs dry at each, 2,400 clocks a tile.)
+// tokens each; k_by and v_by are what they are multiplied by besides.  `most`: the
+// largest of 16 weights together times their scale.  (Unrolled: at 32 a turn the
+// special-function pipe runs dry at each, 2,400 clocks a tile.)
 __device__ __forceinline__ float weights64(uint32_t s_at, bool more, float (&s)[2][32], const float2* scales, float k_by, float v_by, float base,
-                                           uint32_t (&p)[32]) {
+                                           uint32_t (&p)[32], float& most) {
     const float2 base2 = make_float2(base, base);
-    float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    float sum = 0.f;
+    most = 0.f;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
         wait_loads32(s[c]);
@@ -273,6 +284,7 @@ __device__ __forceinline__ float weights64(uint32_t s_at, bool more, float (&s)[
         for (int half = 0; half < 2; ++half) {
             const float2 scale = scales[2 * c + half];
             const float2 k = make_float2(scale.x * k_by, scale.x * k_by), v = make_float2(scale.y * v_by, scale.y * v_by);
+            float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
             for (int i = 8 * half; i < 8 * half + 8; ++i) {
                 float2 x = fma2(make_float2(s[c][2 * i], s[c][2 * i + 1]), k, base2);
@@ -282,14 +294,17 @@ __device__ __forceinline__ float weights64(uint32_t s_at, bool more, float (&s)[
                 x = mul2(x, v);
                 p[16 * c + i] = Type16<__half>::pack(x.x, x.y);
             }
+            add[0] = add2(add[0], add[1]);
+            const float together = add[0].x + add[0].y;
+            sum += together;
+            most = fmaxf(most, together * fmaxf(v.x, kDeepest));
         }
     }
-    add[0] = add2(add[0], add[1]);
-    return add[0].x + add[0].y;
+    return sum;
 }
 
-// The largest of a row's 128 scores, in log2 units.
-__device__ __noinline__ float largest_score(uint32_t s_at, const float2* scales, float k_by) {
+// The largest of a row's 128 scores, in log2 units, each plus its value scale's.
+__device__ __noinline__ float largest_score(uint32_t s_at, const float2* scales, float k_by, float v_by) {
     float most = -INFINITY;
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
@@ -301,16 +316,17 @@ __device__ __noinline__ float largest_score(uint32_t s_at, const float2* scales,
             float high = s[16 * half];
 #pragma unroll
             for (int i = 1; i < 16; ++i) high = fmaxf(high, s[16 * half + i]);
-            most = fmaxf(most, high * (scales[2 * c + half].x * k_by));
+            most = fmaxf(most, fmaf(high, scales[2 * c + half].x * k_by, scale_log2(scales[2 * c + half].y, v_by)));
         }
     }
     return most;
 }
 
 // The last tile where the tokens end inside it, tiles with blocks that are not
-// there, and where the maximum moves: the largest score first, then the weights.  From the quarter `from` on; `left` tokens of the
-// tile are there, `missing` has a bit for each 16 that are not.  `state` is the
-// row's maximum (log2) and sum, returned as they become.
+// there, and where the maximum moves: the largest first, then the weights.  From
+// the quarter `from` on; `left` tokens of the tile are there, `missing` has a bit
+// for each 16 that are not.  `state` is the row's maximum (log2, of scores and value
+// scales) and sum, returned as they become.
 __device__ __noinline__ float2 weights_with_care(uint32_t s_at, uint32_t o_at, int from, int quarters, int32_t left, uint32_t missing,
                                                  const float2* scales, float k_by, float v_by, int dim, float2 state) {
     float next = state.x;
@@ -330,7 +346,12 @@ __device__ __noinline__ float2 weights_with_care(uint32_t s_at, uint32_t o_at, i
     for (int c = from; c < quarters; ++c) {
         scores(c);
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) next = fmaxf(next, fmaxf(z[i], z[i + 1]));
+        for (int half = 0; half < 2; ++half) {
+            float high = z[16 * half];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) high = fmaxf(high, z[16 * half + i]);
+            next = fmaxf(next, high + scale_log2(scales[2 * c + half].y, v_by));
+        }
     }
     if (__any_sync(kFull, next > state.x)) {
         // the maximum moves, what was summed is rescaled
@@ -750,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
             for (int o = 16; o > 0; o >>= 1) unit = fmaxf(unit, __shfl_xor_sync(kFull, unit, o));
             if (!(unit > 0.f)) unit = 1.f;
             const float k_by = d.scale * 1.4426950408889634f * row_scale, v_by = 1.f / unit;
-            float top = -INFINITY, sum = 0.f;       // top: in log2 units, moved when weights are past 2^8
+            float top = -INFINITY, sum = 0.f;       // top: in log2 units
             for (uint32_t j = first; j < end; ++j, ++tiles) {
                 wait(&ctl.s_full[t], s_used++ & 1);        // and the value product before it is done
                 if (stopped()) break;
@@ -760,14 +781,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_shared(const __grid_constant__ 
                 const float2* const scales = ctl.scales[tiles % kScales];
                 const uint32_t missing = ctl.missing[tiles % kScales];
                 if (left >= kTileTokens && !missing) {
-                    if (j == first) top = largest_score(s_at, scales, k_by);
+                    if (j == first) top = largest_score(s_at, scales, k_by, v_by);
                     float s[2][32];
                     tmem_load32(s_at, s[0]);
 #pragma unroll 1
                     for (; done < 4; done += 2) {
                         uint32_t w16[32];
-                        const float part = weights64(s_at + 32 * done, done == 0, s, scales + 2 * done, k_by, v_by, kLift - top, w16);
-                        if (__any_sync(kFull, real && part > kMost)) break;       // (rows that are none hold anything)
+                        float most;
+                        const float part = weights64(s_at + 32 * done, done == 0, s, scales + 2 * done, k_by, v_by, kLift - top, w16, most);
+                        if (__any_sync(kFull, real && most > kMost)) break;       // (rows that are none hold anything)
                         sum += part;
                         tmem_store16(s_at + 16 * done, w16);
                         tmem_store16(s_at + 16 * done + 16, w16 + 16);
