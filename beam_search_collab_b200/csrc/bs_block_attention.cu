@@ -308,6 +308,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
             const int32_t x = d.cu[i];
             if (i == 0 ? x != 0 : x < d.cu[i - 1] || (i == d.num_groups && static_cast<uint32_t>(x) != d.num_seqs))
                 atomicOr(a.errors, kMemErrLength);
+            // (groups without sequences and tables without columns are looked up nowhere else)
+            if (i < d.num_groups) tokens_of(a, d.shared_lens, i, d.shared_width);
         }
     if (parts > 1) cluster.sync();
     else __syncthreads();

@@ -450,3 +450,27 @@ def test_a_decoding_step_of_conversations_about_one_document():
                 assert off.max() <= 0
                 assert ((lse[b, 0, h * 4:h * 4 + 4].double() - ref[1]).abs() <= R.lse_bound(ref[4])).all()
     assert M.take_errors() == 0
+
+
+@pytest.mark.parametrize("seqs", [6, 300])
+def test_lengths_of_shared_tokens_outside_their_table_set_a_bit(seqs):
+    # a table without columns, and groups without sequences, have lengths too
+    groups, shared, lens = [seqs - 1, 0, 1], [2000, 50, 300], [(7 * i) % 40 for i in range(seqs)]
+    pool, shared_table, table, q = case(28, groups, shared, lens, 8, 2, 32, 64, 1, BF16)
+    cache = M.TokenCache(*pool)
+
+    def run(t, n):
+        out, _ = cache.shared_attention(q, t, R.i32(n), R.cu(groups), table, R.i32(lens))
+        return out, M.take_errors()
+
+    good, flags = run(shared_table, shared)
+    assert flags == 0
+    for n in (1 << 20, -1):
+        out, flags = run(shared_table, [2000, n, 300])
+        assert flags == 4 and torch.equal(out, good)
+    none = shared_table[:, :0].contiguous()
+    own, flags = run(none, [0, 0, 0])
+    assert flags == 0
+    for n in ([5, 0, 0], [0, 0, -1], [0, 1, 0]):
+        out, flags = run(none, n)
+        assert flags == 4 and torch.equal(out, own)
