@@ -341,7 +341,10 @@ __global__ void __launch_bounds__(THREADS) k_block_choice(const __grid_constant_
                 if (col < cached) return keys[col];
                 // a row too long for shared memory: scored again, by one thread
                 const uint32_t id = table[col];
-                if (id >= a.c.num_blocks) return key(0, 0.f);
+                if (id >= a.c.num_blocks) {
+                    atomicOr(a.errors, kMemErrBlock);
+                    return key(0, 0.f);
+                }
                 const uint64_t slab = static_cast<uint64_t>(id) * hkv + h;
                 int32_t sum = 0;
                 for (uint32_t y = 0; y < 2 * dim; ++y) sum += parts[y >= dim][y < dim ? y : y - dim] * d.bounds[slab * 2 * dim + y];

@@ -439,3 +439,24 @@ def test_gradients_are_refused():
     for x in cache.block_attention(q, table, at, blocks, with_lse=True):
         with pytest.raises(RuntimeError, match="no gradient"):
             x.float().sum().backward()
+
+
+def test_blocks_that_are_not_there_far_on_in_a_long_row_set_a_bit():
+    # a row of which a thread block has more columns than it keeps: they count as score 0 there too
+    g = torch.Generator("cuda").manual_seed(31)
+    width, block, dim = 400000, 16, 16
+    pool = R.random_pool(g, 9, 1, block, dim)
+    pool[2][8] = 0
+    table = torch.randint(0, 8, (1, width), generator=g, device="cuda", dtype=torch.int32)
+    q = torch.randn((1, 1, 2, dim), generator=g, device="cuda").to(F16)
+    cache = M.TokenCache(*pool)
+    all_blocks = torch.arange(9, device="cuda", dtype=torch.int32)[None]
+    bounds = cache.update_bounds(cache.empty_bounds(), all_blocks, R.i32([9 * block]))
+    lens, far = R.i32([width * block]), 49000
+    table[0, far] = 8
+    want = cache.choose_blocks(q, bounds, table, lens, 1000)
+    assert M.take_errors() == 0
+    for bad in (9, -1, 2 ** 31 - 1):
+        table[0, far] = bad
+        got = cache.choose_blocks(q, bounds, table, lens, 1000)
+        assert M.take_errors() == 2 and torch.equal(got, want)
