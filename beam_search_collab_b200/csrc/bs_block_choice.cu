@@ -405,13 +405,8 @@ cudaError_t launch_choice(const bs_token_cache& c, const bs_block_choice_desc& d
 
 cudaError_t launch_block_bounds(const bs_token_cache& c, const bs_block_bounds_desc& d, const MemoryDevice& dev, cudaStream_t stream) {
     BoundsArgs a{c, d, dev.errors};
-    a.cols = d.table_width;
-    if (d.last >= 0) {          // the last tokens may begin and end inside a block
-        const uint64_t touched = (static_cast<uint64_t>(d.last) + c.block - 2) / c.block + 1;
-        if (touched < a.cols) a.cols = static_cast<uint32_t>(touched);
-    }
+    a.cols = bounds_columns(c, d);
     const uint64_t blocks = (static_cast<uint64_t>(a.cols) * c.kv_heads + kBoundsWarps - 1) / kBoundsWarps;
-    if (blocks > 0xffffffffu / kBoundsWarps / 2) return cudaErrorInvalidConfiguration;      // (units count in 32 bits)
     return launch_after(k_block_bounds, dim3(static_cast<unsigned>(blocks), d.num_seqs), 32 * kBoundsWarps, 0, stream, a);
 }
 

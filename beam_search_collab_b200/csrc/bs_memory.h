@@ -44,6 +44,12 @@ cudaError_t launch_cache_evict(const bs_token_cache& c, const bs_cache_evict_des
                                cudaStream_t stream);
 
 cudaError_t launch_norm_rotate(const bs_norm_rotate_desc& d, const MemoryDevice& dev, cudaStream_t stream);
+// Blocks of a sequence that hold any of its last tokens, at most (these may begin
+// and end inside a block).
+inline uint32_t bounds_columns(const bs_token_cache& c, const bs_block_bounds_desc& d) {
+    const uint64_t touched = d.last < 0 ? d.table_width : d.last == 0 ? 0 : (static_cast<uint64_t>(d.last) + c.block - 2) / c.block + 1;
+    return touched < d.table_width ? static_cast<uint32_t>(touched) : d.table_width;
+}
 cudaError_t launch_block_bounds(const bs_token_cache& c, const bs_block_bounds_desc& d, const MemoryDevice& dev, cudaStream_t stream);
 cudaError_t launch_block_choice(const bs_token_cache& c, const bs_block_choice_desc& d, const MemoryDevice& dev, cudaStream_t stream);
 cudaError_t launch_block_attention(const bs_token_cache& c, const bs_block_attention_desc& d, const MemoryDevice& dev,

@@ -383,6 +383,8 @@ BS_API bs_status bs_block_bounds(const bs_token_cache* c, const bs_block_bounds_
     if (!d) return report_error(BS_ERR_INVALID_ARGUMENT, "desc is NULL");
     if (bs_status s = check_cache(c, 0, false)) return s;
     if (bs_status s = check_table(c, d->num_seqs, d->table_width)) return s;
+    if (static_cast<uint64_t>(bounds_columns(*c, *d)) * c->kv_heads >= (1ull << 31))       // (counted in 32 bits)
+        return report_error(BS_ERR_UNSUPPORTED, "fewer than 2^31 blocks of a sequence, times key heads, are supported");
     if (d->num_seqs == 0 || d->table_width == 0 || d->last == 0) return BS_OK;
     if (any_null({d->bounds, d->table, d->lens})) return report_error(BS_ERR_INVALID_ARGUMENT, "a buffer is NULL");
     if (!aligned16({d->bounds})) return report_error(BS_ERR_INVALID_ARGUMENT, "%s", kAlignBounds);

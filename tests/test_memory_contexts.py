@@ -202,3 +202,15 @@ def test_every_block_waits_whatever_the_call_is(name):
         before, wait, _ = body.partition("\n    cudaGridDependencySynchronize();")        # (four spaces: the kernel's own block)
         assert wait and re.search(r"[;{}]\s*\Z", before), kernel
         assert not re.search(r"\breturn\b|atomicOr\(|\blens\b|\bd\.\w+\[", before.partition("{")[2]), kernel
+
+
+def test_bounds_of_more_blocks_than_32_bits_count():
+    # (the widest table of blocks of 16, and key heads: its product with them reaches 2^31)
+    d = calls()["bs_block_bounds"]
+    d.table_width = (1 << 26) - 1
+    rc, why = call("bs_block_bounds", d, block=16, kv_heads=33)
+    assert rc == 2 and "2^31" in why, (rc, why)
+    for heads, last in ((32, -1), (65535, 1)):
+        d.last = last
+        rc, why = call("bs_block_bounds", d, block=16, kv_heads=heads)
+        assert rc != 2 and ("current device" in why or "device query" in why), (rc, why)
