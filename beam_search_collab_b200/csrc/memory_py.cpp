@@ -172,7 +172,7 @@ py::tuple prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, co
 }
 
 // [tokens, heads, dim] each; k may be None.
-py::tuple norm_rotate(const Tensor& q, const MaybeTensor& k, const Tensor& positions, const MaybeTensor& freqs, const MaybeTensor& q_weight,
+py::tuple norm_rotate(const Tensor& q, const MaybeTensor& k, const MaybeTensor& positions, const MaybeTensor& freqs, const MaybeTensor& q_weight,
                       const MaybeTensor& k_weight, double eps, bool interleaved, double amplitude, std::optional<uint64_t> stream) {
     check_rows(q, "q", nullptr);
     if (k) {
@@ -181,7 +181,8 @@ py::tuple norm_rotate(const Tensor& q, const MaybeTensor& k, const Tensor& posit
     }
     need(k || !k_weight, "k_weight without k");
     bs_norm_rotate_desc d{};
-    d.positions = indexes(positions, {q.size(0)}, "positions", q.device());
+    need(positions || !freqs || freqs->numel() == 0, "positions are needed for a rotation");
+    if (positions) d.positions = indexes(*positions, {q.size(0)}, "positions", q.device());
     if (freqs) {
         need(freqs->scalar_type() == at::kDouble && freqs->dim() == 1 && freqs->is_contiguous() && freqs->device() == q.device(),
              "freqs must be a contiguous float64 tensor [rotary / 2] on q's device");
@@ -218,8 +219,8 @@ py::tuple norm_rotate(const Tensor& q, const MaybeTensor& k, const Tensor& posit
     d.eps = static_cast<float>(eps);
     d.amplitude = static_cast<float>(amplitude);
     check(bs_norm_rotate(&d, to.stream));
-    to.uses({&q, &positions});
-    for (const MaybeTensor* t : {&k, &freqs, &q_weight, &k_weight})
+    to.uses({&q});
+    for (const MaybeTensor* t : {&k, &positions, &freqs, &q_weight, &k_weight})
         if (*t) to.uses({&**t});
     to.gives({&out_q, &out_k});
     const Tensor none;

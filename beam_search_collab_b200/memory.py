@@ -84,7 +84,7 @@ def rotary_frequencies(rotary, base=10000.0, *, scaling=None, factor=1.0, traine
     return freqs * (stay + (1 - stay) / factor), 0.1 * math.log(factor) + 1
 
 
-def norm_rotate(q, k, positions, freqs=None, *, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, amplitude=1.0, stream=None):
+def norm_rotate(q, k, positions=None, freqs=None, *, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, amplitude=1.0, stream=None):
     """Norm of queries and keys for each head, then their rotary position, in
     one pass (bs_norm_rotate).
 
@@ -94,7 +94,7 @@ def norm_rotate(q, k, positions, freqs=None, *, q_weight=None, k_weight=None, ep
     the root of its mean square and multiplied by q_weight or k_weight [dim]
     where that is given.  Then its first 2 * len(freqs) dimensions are rotated
     by positions (int32 [tokens], any sign) times freqs (float64, radians a
-    position; None: no rotation): pairs are the first and second half's j-th
+    position; None: no rotation, and positions may be None): pairs are the first and second half's j-th
     dimensions, or with `interleaved` neighbours; `amplitude` multiplies sines
     and cosines (:func:`rotary_frequencies` gives both).  Returns (q, k),
     contiguous."""

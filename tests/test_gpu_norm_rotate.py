@@ -220,3 +220,19 @@ def test_a_value_that_is_not_finite_stays_in_its_place(dim, rotary, value, inter
         for out in (want, got):
             out[d, 1, d] = out[d, 1, d ^ 1 if interleaved else (d + rotary // 2) % rotary] = 0
     assert same(got, want) and torch.equal(got_k, clean_k)
+
+
+def test_positions_are_needed_for_a_rotation_alone():
+    g = torch.Generator("cuda").manual_seed(15)
+    q, k = (torch.randn((7, h, 64), generator=g, device="cuda").to(F16) for h in (4, 2))
+    w = torch.rand(64, generator=g, device="cuda") + 0.5
+    positions = torch.arange(7, dtype=torch.int32, device="cuda")
+    want = M.norm_rotate(q, k, positions, q_weight=w)
+    for got in (M.norm_rotate(q, k, q_weight=w), M.norm_rotate(q, k, None, None, q_weight=w)):
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    none = M.rotary_frequencies(0, device="cuda")[0]
+    assert torch.equal(M.norm_rotate(q, k, None, none, q_weight=w)[0], want[0])
+    with pytest.raises(ValueError, match="positions"):
+        M.norm_rotate(q, k, freqs=M.rotary_frequencies(32, device="cuda")[0])
+    with pytest.raises(ValueError, match="positions"):
+        M.norm_rotate(q, k, positions[:3])
