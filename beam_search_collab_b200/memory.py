@@ -9,12 +9,13 @@ gives up are rows for an :class:`Index`, found again by its search.
     cache = memory.TokenCache.empty(num_blocks, kv_heads, dim, block=64)
     cache.write(k, v, cu, table, start)                       # its keys and values, quantised
     q1, k1 = memory.norm_rotate(q1, k1, positions, freqs, q_weight=w, k_weight=w)  # of one new token each
+    q1 = q1[:, None]                                           # [sequences, queries, heads, dim]
     out, lse, mass = cache.attention(q1, table, lens, mass=mass, with_mass=True)
     blocks = cache.choose_blocks(q1, cache.update_bounds(bounds, table, lens), table, lens, count)
     out, lse = cache.block_attention(q1, table, lens, blocks)                      # or over a part of its cache
-    out, lse = cache.shared_attention(q1, shared_table, shared_lens, cu, table, lens)   # or with a shared beginning
+    out, lse = cache.shared_attention(q1, shared_table, shared_lens, groups, table, lens)   # or with a shared beginning
     kept, lens, mass = cache.evict(mass, table, lens, new_table, budget)
-    keys, values = cache.read(old_table, old_lens, positions)  # float rows for Index.from_vectors
+    keys, values = cache.read(old_table, old_lens, found)      # float rows for Index.from_vectors
 
 Everything is a CUDA tensor; calls are asynchronous on `stream` (default: the
 current stream of the tensors' device) and never wait for the lengths, tables

@@ -1,6 +1,7 @@
 """GPU: the operators for long and shared contexts at their far ends: caches and rows past 32-bit offsets, empty tables,
 the most queries, many groups, outputs over their inputs, graphs that run at once."""
 import ctypes
+import re
 
 import pytest
 import torch
@@ -196,3 +197,28 @@ def test_graphs_that_run_at_once():
     for a, b in zip(got, want):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
     assert M.take_errors() == 0
+
+
+def test_the_modules_example_runs():
+    # (its lines from the documentation, two conversations of an instruction and a few tokens each)
+    g = torch.Generator("cuda").manual_seed(18)
+    hq, kv_heads, dim, block, count, budget = 8, 2, 64, 64, 2, 100
+    code = re.search(r"\n\n((?:    .*\n)+)", M.__doc__)[1]
+    lines = [x[4:] for x in code.splitlines() if "import" not in x]
+    lengths, num_blocks = [300, 150], 40
+
+    def rows(n, heads):
+        return torch.randn((n, heads, dim), generator=g, device="cuda").to(BF16)
+
+    ids = torch.randperm(num_blocks, generator=g, device="cuda").to(torch.int32)
+    w = torch.ones(dim, device="cuda")
+    names = dict(memory=M, q=rows(450, hq), k=rows(450, kv_heads), v=rows(450, kv_heads), cu=R.cu(lengths), num_blocks=num_blocks,
+                 kv_heads=kv_heads, dim=dim, table=ids[:16].view(2, 8), start=R.i32([0, 0]), lens=R.i32(lengths), w=w, count=count, budget=budget,
+                 q1=rows(2, hq), k1=rows(2, kv_heads), positions=R.i32(lengths), freqs=M.rotary_frequencies(dim, device="cuda")[0],
+                 mass=torch.zeros((2, kv_heads, 512), device="cuda"), bounds=torch.zeros((num_blocks, kv_heads, 2, dim), dtype=torch.int8, device="cuda"),
+                 shared_table=ids[16:18][None].contiguous(), shared_lens=R.i32([128]), groups=R.cu([2]), new_table=ids[20:24].view(2, 2).contiguous(),
+                 old_table=ids[:16].view(2, 8), old_lens=R.i32(lengths))
+    names["found"] = R.i32([[3, 7], [1, 149]])
+    exec("\n".join(lines), names)
+    assert M.take_errors() == 0
+    assert names["blocks"].shape == (2, 1, kv_heads, count) and names["keys"].shape[:2] == (2, kv_heads)
