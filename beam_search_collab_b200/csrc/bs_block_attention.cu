@@ -115,8 +115,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NT)) k_rows(const __gr
         for (int nt = 0; nt < NT; ++nt) {
             scale_query_row<NW>(q[nt], row_scale[nt], d.dtype != BS_F16, d.scale * 1.4426950408889634f, c);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 2; ++i) {
                 limit[nt][i] = static_cast<int32_t>(len) - d.queries + 1 + static_cast<int32_t>(LIST ? query : (row0 + 8 * nt + 2 * c + i) / a.group);
+                if (!LIST) limit[nt][i] = max(limit[nt][i], 0);       // (below 0 are the shared tokens, which it sees)
+            }
         }
     };
     Group group{};                   // what the sequence shares (none: no tokens)

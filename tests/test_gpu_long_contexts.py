@@ -1,6 +1,7 @@
 """GPU: the operators for long and shared contexts at their far ends: caches and rows past 32-bit offsets, empty tables,
 the most queries, many groups, outputs over their inputs, graphs that run at once."""
 import ctypes
+import math
 import re
 
 import pytest
@@ -222,3 +223,21 @@ def test_the_modules_example_runs():
     exec("\n".join(lines), names)
     assert M.take_errors() == 0
     assert names["blocks"].shape == (2, 1, kv_heads, count) and names["keys"].shape[:2] == (2, kv_heads)
+
+
+def test_as_many_shared_tokens_as_there_can_be():
+    # 2^30 - 16 tokens that each sequence reads by itself, and no own ones: the queries see the last shared tokens too
+    heads, queries, block, dim, width = 9, 32, 16, 16, (1 << 26) - 1
+    pool = [torch.zeros((2, heads, block, dim), dtype=torch.int8, device="cuda") for _ in range(2)] + [torch.zeros((2, heads), device="cuda") for _ in range(2)]
+    pool[0][1], pool[1][1], pool[2][1], pool[3][1] = 100, 50, 0.03, 0.02        # scores of 100 * 0.03 * 16 = 48 against 0
+    shared_table = torch.zeros((1, width), dtype=torch.int32, device="cuda")
+    shared_table[0, -1] = 1
+    q = torch.ones((1, queries, heads, dim), dtype=F16, device="cuda")
+    table = torch.zeros((1, 0), dtype=torch.int32, device="cuda")
+    out, lse = M.TokenCache(*pool).shared_attention(q, shared_table, R.i32([width * block]), R.cu([1]), table, R.i32([0]), scale=1.0, with_lse=True)
+    assert M.take_errors() == 0
+    n, top = (width - 1) * block, torch.tensor(0.03).item() * 1600
+    far = math.log(n * math.exp(-top) + 16)
+    # (16 of e^48 against 2^30 of 1: sums of 2^30 ones in 32 bits may lose all of them, e^-48 * 2^30 / 16 = 1e-13 of the whole)
+    assert (lse.double() - (top + far)).abs().max() <= 2.0 ** -17 * top + 2.0 ** -17
+    assert (out.double() - 1.0).abs().max() <= 2.0 ** -10
