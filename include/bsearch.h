@@ -427,9 +427,11 @@ BS_API bs_status bs_cache_evict_workspace(const bs_token_cache* cache, const bs_
  * and of its first `rotary` dimensions the pairs j < rotary / 2, (a, b) =
  * (y[j], y[j + rotary / 2]) or, interleaved, (y[2 j], y[2 j + 1]), become
  *   amplitude * (a cos t - b sin t, b cos t + a sin t),  t = position * freqs[j],
- * rounded once, at the end.  An angle keeps its accuracy at any position: it is
- * reduced to a part of a turn in integers, off by at most 2^-32 turns and 2^-52
- * of itself.  freqs are finite, positions any.
+ * rounded once, at the end, from 32-bit floats.  An angle keeps its accuracy at
+ * any position: it is reduced to a part of a turn in integers, off by at most
+ * 2^-32 turns and 2^-52 of itself; its sine and cosine, from a 32-bit float, are
+ * off by at most 2^-19 (not of themselves).  The sum of squares is finite for
+ * |x| below 2^60.  freqs are finite, positions any.
  * Outputs are contiguous; an output may be its own contiguous input. */
 typedef struct bs_norm_rotate_desc {
     const void* q;            /* [total][q_heads][dim]                        */

@@ -236,3 +236,22 @@ def test_positions_are_needed_for_a_rotation_alone():
         M.norm_rotate(q, k, freqs=M.rotary_frequencies(32, device="cuda")[0])
     with pytest.raises(ValueError, match="positions"):
         M.norm_rotate(q, k, positions[:3])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_sines_and_cosines_of_far_positions(interleaved):
+    # one dimension of a pair is 1: the pair becomes the cosine and the sine.  Off by one rounding (f16's below 2^-14: half of
+    # 2^-24) and by 2^-19: the angle, a part of a turn, is reduced to 2^-32 turns (2^-29 radians), and in 32 bits rounded
+    # three times, up to pi * 3 * 2^-24 = 2^-20.8; sine and cosine are off by 2^-21.2; in all 2^-19.9.  The angle itself
+    # keeps 2^-52 of it, 2^-21 radians at 2^31, so the frequencies here are such that 2^53 holds the products exactly.
+    g = torch.Generator("cuda").manual_seed(16)
+    freqs = torch.tensor([1.0, 0.5, 3 * 2.0 ** -12, 2.0 ** -20, 5 * 2.0 ** -7, 1.5, 2.0 ** -16, 2.0 ** -9], dtype=torch.float64, device="cuda")
+    positions = torch.randint(-(1 << 24), 1 << 24, (5000,), generator=g, device="cuda", dtype=torch.int32)
+    x = torch.zeros((5000, 2, 16), dtype=F16, device="cuda")
+    one, two = (slice(0, 16, 2), slice(1, 16, 2)) if interleaved else (slice(0, 8), slice(8, 16))
+    x[:, 0, one] = x[:, 1, two] = 1
+    out = M.norm_rotate(x, None, positions, freqs, interleaved=interleaved)[0].double()
+    t = positions.double()[:, None] * freqs
+    off = 2.0 ** -19 + 2.0 ** -25 + t.abs() * 2.0 ** -51
+    for got, want in ((out[:, 0, one], t.cos()), (out[:, 0, two], t.sin()), (out[:, 1, two], t.cos()), (out[:, 1, one], -t.sin())):
+        assert ((got - want).abs() <= 2.0 ** -11 * want.abs() + off).all()
