@@ -35,6 +35,7 @@ def reference(pool, q, rows):
         for h in range(hkv):
             k, v = ((pool[i][ids, h].double() * pool[2 + i][ids, h].double()[:, None, None])[held] for i in (0, 1))
             s = pool[3][ids, h].double()[:, None].expand(held.shape)[held]
+            s = s.clamp(min=2.0 ** -60 * s.max())                # (as far down as scales count; of 0 too)
             at = (b, 0, slice(h * g, h * g + g))
             out[at], _, w, weighted[at], _ = R.attend(q[at].double(), k, v, 1.0, torch.full((g,), len(k), device="cuda"))
             lost[at] = torch.minimum(w, 2.0 ** -29 * (w * s).amax(1, keepdim=True) / s) @ v.abs()
@@ -49,8 +50,11 @@ def tokens(table, n, block):
 def check(out, ref, weighted, lost):
     # no more than each element's own: the output's rounding, the weights' to f16 and 2^-12 for exponentials and scores, of what the
     # element is a sum of, and what f16 loses of it (no part of the others' size, but half of f16's smallest step)
-    off = (out.double() - ref).abs() - (R.UNIT[out.dtype] * ref.abs() + (R.UNIT[F16] + 2.0 ** -12) * weighted * (1 + 2.0 ** -7) + lost +
-                                        (2.0 ** -25 if out.dtype == F16 else 0))
+    size = (R.UNIT[out.dtype] * ref.abs() + (R.UNIT[F16] + 2.0 ** -12) * weighted * (1 + 2.0 ** -7) + lost +
+            (2.0 ** -25 if out.dtype == F16 else 0))
+    # (f16 rounds to infinity from 65520 on: one is right where the element is as large within its bound)
+    right = torch.isinf(out) & (ref.sign() == out.sign()) & (ref.abs() + size >= 65520) & (out.dtype == F16)
+    off = torch.where(right, -size, (out.double() - ref).abs() - size)
     assert off.max() <= 0, off.max()
 
 
@@ -94,4 +98,32 @@ def test_shared_tokens(seqs, place, ratio, spread, dtype, size):
         far, near = tokens(shared_table[b // (seqs - 1)], shared[b // (seqs - 1)], block), tokens(table[b], n, block)
         rows.append([torch.cat(x) for x in zip(far, near)])
     check(out, *reference(pool, q, rows))
+    assert M.take_errors() == 0
+
+
+@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("seqs", [2, 300])
+@pytest.mark.parametrize("dtype,size", [(BF16, 0), (F16, 1), (BF16, 3)])
+def test_every_block_at_a_scale_of_its_own(seed, seqs, dtype, size):
+    # 10^-8 to 10^8 (10^-4 to 10^3 for f16 outputs), and 0; scores that favour one or the other block
+    dim, block, hq, hkv = SIZES[size]
+    groups, shared, lens = [seqs], [1700], [(37 * i + 11) % 150 for i in range(seqs)]
+    pool, shared_table, table, q = S.case(50 + seed, groups, shared, lens, hq, hkv, block, dim, 1, dtype, 1 + seed)
+    g = torch.Generator("cuda").manual_seed(60 + seed)
+    low, high = (-4, 3) if dtype == F16 else (-8, 8)
+    pool[3][:] = 10.0 ** (low + (high - low) * torch.rand(pool[3].shape, generator=g, device="cuda"))
+    pool[3][torch.rand(pool[3].shape, generator=g, device="cuda") < 0.05] = 0
+    pool[2] *= dim ** -0.5
+    cache = M.TokenCache(*pool)
+    rows = []
+    for b, n in enumerate(lens):
+        rows.append([torch.cat(x) for x in zip(tokens(shared_table[0], shared[0], block), tokens(table[b], n, block))])
+    out, _ = cache.shared_attention(q, shared_table, R.i32(shared), R.cu(groups), table, R.i32(lens), scale=1.0)
+    check(out, *reference(pool, q, rows))
+    own = [tokens(shared_table[0], 1700 - 13 * b, block) for b in range(2)]
+    both, length = shared_table.expand(2, -1).contiguous(), R.i32([1700, 1687])
+    want = reference(pool, q[:2], own)
+    check(cache.attention(q[:2], both, length, scale=1.0)[0], *want)
+    order = torch.randperm(both.shape[1], generator=g, device="cuda").to(torch.int32).expand(2, 1, hkv, -1).contiguous()
+    check(cache.block_attention(q[:2], both, length, order, scale=1.0)[0], *want)
     assert M.take_errors() == 0
