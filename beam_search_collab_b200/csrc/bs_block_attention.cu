@@ -462,8 +462,12 @@ Layout plan(const bs_token_cache& c, const bs_shared_attention_desc& d, const Me
     // the kernel for its own.  The times of both ways, in us: the other one takes
     // 14 for its start, its end and the join, and 2.6 for 256 rows over 128 tokens.
     // (Of 32 query and 8 key heads of 128: 8 sequences over 1,000 tokens 11 us this
-    // way and 25 that way; 64 over 1,000 39 and 38; 128 over 3,500 155 and 51; each
-    // with 200 tokens of its own.)
+    // way and 27 that way; 64 over 1,000 38 and 39; 128 over 4,000 173 and 52.  Of 64
+    // dimensions 9 and 23, 31 and 33, 132 and 43.  Each with 200 tokens of its own.
+    // The constants are those of 128 dimensions, and the table's width stands for
+    // the tokens; over 175 combinations of 32, 64 and 128 dimensions, 2 and 8 key heads,
+    // 4 to 256 sequences and 256 to 16,000 tokens in tables of their width the way
+    // taken was the slower one by more than 10% in three, 14% at most.)
     const uint32_t in_sequence = static_cast<uint32_t>(d.q_heads / c.kv_heads) * d.queries;
     const uint64_t segments = own_segments(c, d, in_sequence);
     const uint32_t per_sm = blocks_per_sm(in_sequence <= 8 ? 1 : 2);

@@ -131,13 +131,12 @@ constexpr uint32_t kMostHeld = 8;      // scores of a thread where one block has
 // then their places by prefix sums.  A row of 1,024 takes 2 us; the cluster's way
 // (bs_select.cuh), with digits of 11 bits for longer rows, 6 and more (8 rows of
 // 1,024 columns 24.6 us in all, against 8.8).
-template <int THREADS>
 struct SmallShared {
     uint32_t count[4][256];
     uint32_t chosen[2];
 };
 template <int THREADS, typename Keep>
-__device__ __forceinline__ void select_small(SmallShared<THREADS>& shared, uint32_t* warp_sums, const uint32_t* keys, uint32_t n, uint32_t sinks,
+__device__ __forceinline__ void select_small(SmallShared& shared, uint32_t* warp_sums, const uint32_t* keys, uint32_t n, uint32_t sinks,
                                              uint32_t recent, uint32_t budget, Keep keep) {
     const uint32_t t = threadIdx.x, lane = t & 31, hi = n - recent;
     // places side by side: t * each and on
@@ -209,7 +208,7 @@ __device__ __forceinline__ void select_small(SmallShared<THREADS>& shared, uint3
 template <typename T, int THREADS, bool SMALL>
 __global__ void __launch_bounds__(THREADS) k_block_choice(const __grid_constant__ ChoiceArgs a, uint32_t cached) {
     extern __shared__ uint32_t keys[];                     // [cached]: the columns' blocks, then their keys
-    using Shared = std::conditional_t<SMALL, SmallShared<THREADS>, SelectShared>;
+    using Shared = std::conditional_t<SMALL, SmallShared, SelectShared>;
     __shared__ __align__(16) Shared shared;
     __shared__ __align__(16) int16_t parts[2][128];        // positive and negative part of the heads' codes
     __shared__ float warp_max[THREADS / 32];

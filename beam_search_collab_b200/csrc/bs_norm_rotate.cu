@@ -116,7 +116,8 @@ __device__ __forceinline__ float weight_at(const void* w, int32_t dtype, uint32_
 // Every block takes tokens (or parts of them) in turn, and a warp asks for its
 // next rows before it works on the last ones: with a block for each four tokens the
 // loads stood still while angles were computed (50 us against 30 for 7,196 tokens of
-// 40 heads of 128: 147 MB, 4.8 TB/s, where the copies alone are 22.5 us).
+// 40 heads of 128: 147 MB, 4.8 TB/s, where the copies alone are 22.5 us).  What is left
+// is instructions, 2.6 of 4 a cycle; DRAM is at a third of its rate.
 template <typename T, int V, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads, kBlocks) k_norm_rotate(const __grid_constant__ RotateArgs a) {
     constexpr int kEach = V == 1 ? 2 : 1;              // pairs of chunks of a lane: 128 dimensions are 64 of them

@@ -31,8 +31,8 @@
 // together (no maximum is taken before the exponentials); sums are 32-bit, of the
 // unrounded weights.
 //
-// 512 rows of each of 8 key heads over 32,768 tokens take 104 us here: 28 times 128 tokens
-// a block, 4,100 to 4,600 clocks each, and 12,000 to the first scores and 5,500 for the
+// 512 rows of each of 8 key heads over 32,768 tokens take 106 us here: 28 times 128 tokens
+// a block, 4,100 to 4,700 clocks each, and 12,000 to the first scores and 5,500 for the
 // outputs.  128 tokens need 2,048 clocks of the tensor cores and 2,560 of shared memory
 // (operands 192 KB, codes in and out 64, converted 64, at 128 bytes a clock); the rest
 // is each tile's chain of scores, weights and products, which the other tile alone

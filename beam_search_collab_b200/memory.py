@@ -64,7 +64,8 @@ def rotary_frequencies(rotary, base=10000.0, *, scaling=None, factor=1.0, traine
     the base grows so that the slowest pair turns 1 / factor as fast and the
     fastest as before; "parts": pairs that turn more than `fast` times in
     `trained` positions stay, those that turn less than `slow` times count
-    1 / factor, a linear mixture between, and the amplitude is 0.1 log(factor) + 1."""
+    1 / factor, those between a mixture that is linear in their turns (a program
+    that mixes linearly in the index j gets others there), and the amplitude is 0.1 log(factor) + 1."""
     if rotary < 0 or rotary % 2:
         raise ValueError("rotary must be even and not negative")
     if scaling not in (None, "linear", "base", "parts"):
@@ -182,8 +183,9 @@ class TokenCache(_memory.Cache):
         """Attention of sequences that begin with the same tokens
         (bs_shared_attention).  Sequences cu[m] .. cu[m + 1] (int32 [groups +
         1]) begin with the shared_lens[m] tokens of shared_table[m] (int32
-        [groups, width]), which are read once for all of them; table and lens
-        are of what each has beyond those.  Returns (out, lse) like
+        [groups, width]), which are read once for many query rows where sequences
+        and shared tokens are many, by each sequence where they are few; table
+        and lens are of what each has beyond those.  Returns (out, lse) like
         :meth:`attention`, over both."""
         return self._shared_attention(q, shared_table, shared_lens, cu, table, lens, scale, with_lse, stream)
 

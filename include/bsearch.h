@@ -361,6 +361,14 @@ typedef struct bs_cache_read_desc {
 
 BS_API bs_status bs_cache_read(const bs_token_cache* cache, const bs_cache_read_desc* desc, void* stream);
 
+/* Attention over the cache, over chosen blocks of it and over shared tokens
+ * (bs_cache_attention, bs_block_attention, bs_shared_attention) rounds twice
+ * before its output: elements of a bf16 query below 2^-29 of its row's largest
+ * lose bits (f16 queries are exact), and a weight times its value scale meets the
+ * codes as f16, off by 2^-11 of itself or, where that is more, by 2^-29 of the
+ * row's largest such product (value scales count down to 2^-60 of the largest).
+ * Scores, sums of weights, lse and mass are 32-bit, of weights not rounded. */
+
 /* Attention over the cache.  Sequence b holds lens[b] tokens, the last
  * `queries` of which are the query tokens: query i sees the positions below
  * lens[b] - queries + 1 + i (one query: all).  out, lse as in
@@ -525,8 +533,11 @@ BS_API bs_status bs_block_attention(const bs_token_cache* cache, const bs_block_
  * lens[b] tokens, the last `queries` of which are the query tokens: query i
  * sees all shared tokens of its group and its own positions below
  * lens[b] - queries + 1 + i.  cu starts at 0, ascends and ends at num_seqs
- * (else error bit 4 is set and outputs may hold anything).  The shared keys and
- * values are read once for all of a group's queries.  out, lse as in
+ * (else error bit 4 is set and outputs may hold anything).  Where sequences and
+ * shared tokens are many, the shared keys and values are read once for up to 256
+ * query rows of a group (sequences x queries x heads of a key head); where they
+ * are few, by each sequence.  Which way is taken goes by the numbers of
+ * sequences, heads and columns of the tables.  out, lse as in
  * bs_prompt_attention, over both sets of tokens.  Waits inside are bounded as
  * there; after one that gave up (error bit 1) outputs hold anything. */
 typedef struct bs_shared_attention_desc {
